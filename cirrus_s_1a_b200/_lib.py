@@ -27,6 +27,10 @@ STATUS = {0: "ok", 1: "invalid argument", 2: "shape not supported", 3: "CUDA lau
           8: "a bounded wait in the persistent kernel timed out"}
 CB_PATH_AUTO, CB_PATH_MULTI_KERNEL = 0, 1
 CB_NOALLOC_MAX_SCORES = 1 << 20
+CB_KV8_BLOCK = 64
+CB_KV8_E4M3, CB_KV8_INT8 = 0, 1
+CB_F32, CB_BF16, CB_F16 = 0, 1, 2
+CB_LOGPROB_MAX_TOP, CB_LOGPROB_MAX_VOCAB = 32, 1 << 20
 CB_GEMM_PRE_NONE, CB_GEMM_PRE_RMSNORM = 0, 1
 CB_GEMM_EPI_STORE, CB_GEMM_EPI_ADD, CB_GEMM_EPI_SWIGLU = 0, 1, 2
 
@@ -36,7 +40,8 @@ EXPORTS = ("cb_abi_version", "cb_status_string", "cb_nvfp4_quantize", "cb_nvfp4_
            "cb_gdn_chunk_prefill", "cb_set_wait_limit",
            "cb_workspace_layout", "cb_nvfp4_slice_bytes", "cb_nvfp4_pack_slices", "cb_prompt_lookup_draft",
            "cb_spec_accept", "cb_mtp_workspace_bytes", "cb_mtp_draft", "cb_gemm_nvfp4", "cb_gemm_scratch_bytes",
-           "cb_stream_plan_bytes", "cb_stream_plan", "cb_weight_stream_nvfp4")
+           "cb_stream_plan_bytes", "cb_stream_plan", "cb_weight_stream_nvfp4", "cb_kv8_append",
+           "cb_kv8_attend_scratch_bytes", "cb_kv8_attend", "cb_kv8_evict", "cb_token_logprobs")
 
 P = C.c_void_p
 I32 = C.c_int32
@@ -94,6 +99,11 @@ class CbCache(C.Structure):
                 ("kv_v", P), ("kv_ik", P), ("snap_state", P), ("snap_conv", P)]
 
 
+class CbKv8(C.Structure):
+    _fields_ = [("batch", I32), ("n_kv_heads", I32), ("head_dim", I32), ("max_len", I32), ("format", I32),
+                ("k", P), ("v", P), ("k_scale", P), ("v_scale", P), ("mass", P)]
+
+
 class CbWorkspaceLayout(C.Structure):
     _fields_ = [("bytes", C.c_uint64), ("proj", C.c_uint64), ("sel_idx", C.c_uint64), ("sel_cnt", C.c_uint64),
                 ("ld_proj", I32), ("sel_ld", I32), ("rows", I32)]
@@ -149,12 +159,19 @@ def lib() -> C.CDLL:
         L.cb_clear_status.argtypes = [P, P]
         L.cb_set_wait_limit.argtypes = [P, C.c_uint64, I32, P]
         L.cb_workspace_layout.argtypes = [C.POINTER(CbModel), I32, I32, I32, C.POINTER(CbWorkspaceLayout)]
+        L.cb_kv8_append.argtypes = [P, P, P, I32, P, P, I32, P, P, P, P]
+        L.cb_kv8_attend_scratch_bytes.restype = C.c_size_t
+        L.cb_kv8_attend_scratch_bytes.argtypes = [P, I32, I32, I32]
+        L.cb_kv8_attend.argtypes = [P, P, I32, P, I32, I32, P, P, I32, C.c_float, I32, P, P, P, C.c_size_t, P]
+        L.cb_kv8_evict.argtypes = [P, P, I32, I32, P, P, P]
+        L.cb_token_logprobs.argtypes = [P, I32, C.c_int64, I32, I32, P, I32, P, P, P, P, P, P, P]
         L.cb_read_trace.argtypes = [C.POINTER(CbModel), I32, I32, I32, P, P, I32, P]
         L.cb_launch_count.restype = C.c_int64
         L.cb_launch_count.argtypes = []
         for name in EXPORTS:
             if name not in ("cb_status_string", "cb_workspace_bytes", "cb_launch_count", "cb_nvfp4_slice_bytes",
-                            "cb_mtp_workspace_bytes", "cb_gemm_scratch_bytes", "cb_stream_plan_bytes"):
+                            "cb_mtp_workspace_bytes", "cb_gemm_scratch_bytes", "cb_stream_plan_bytes",
+                            "cb_kv8_attend_scratch_bytes"):
                 getattr(L, name).restype = C.c_int
         if L.cb_abi_version() != 3:
             raise CbError("libcirrus_b200.so ABI version mismatch")

@@ -1,0 +1,63 @@
+// Device helpers of the 8-bit K/V cache (kv8_cache.cu, kv8_attend.cu, kv8_evict.cu).
+//
+// The cache holds codes in 8 bits, [batch][kv head][slot][dim], and one scale
+// for each block of kKv8Block slots and head.  A scale is a power of two, the
+// smallest 2^e with absmax <= qmax * 2^e, so multiplying and dividing by it is
+// exact in float32 and a code moved onto a larger scale is rounded once on a
+// grid that contains the new one.  Every code (|int8| <= 127, every finite
+// E4M3 value) is exact in f16, so a product with an f16 operand is exact too.
+#pragma once
+
+#include "common.cuh"
+
+namespace cb {
+
+constexpr int kKv8Block = CB_KV8_BLOCK;
+constexpr int kKv8EMin = -100, kKv8EMax = 120;
+
+// 2^e for -126 <= e <= 127.
+__host__ __device__ __forceinline__ float kv8_pow2(int e) {
+#ifdef __CUDA_ARCH__
+  return __int_as_float((e + 127) << 23);
+#else
+  union { int i; float f; } u;
+  u.i = (e + 127) << 23;
+  return u.f;
+#endif
+}
+
+// Exponent of a power of two in the normal range.
+__device__ __forceinline__ int kv8_exponent(float s) { return (__float_as_int(s) >> 23) - 127; }
+
+// The smallest e with absmax <= qmax * 2^e (qmax 448 = 1.75 * 2^8 for E4M3,
+// 127 = 1.984375 * 2^6 for int8), within [kKv8EMin, kKv8EMax]; absmax finite, >= 0.
+template <int FMT>
+__device__ __forceinline__ int kv8_need(float absmax) {
+  const int bits = __float_as_int(absmax);
+  const int ex = (bits >> 23) - 127, mant = bits & 0x7fffff;
+  const int e = FMT == CB_KV8_E4M3 ? ex - 8 + (mant > 0x600000) : ex - 6 + (mant > 0x7e0000);
+  return min(max(e, kKv8EMin), kKv8EMax);
+}
+
+// y = x / scale -> code: nearest, ties to even.  Infinities saturate; a NaN is
+// kept by E4M3 and becomes 0 in int8, which has none.
+template <int FMT>
+__device__ __forceinline__ uint32_t kv8_encode(float y) {
+  if (FMT == CB_KV8_E4M3) return f32_to_e4m3(y);
+  return (uint32_t)(min(max(__float2int_rn(y), -127), 127) & 0xFF);
+}
+
+template <int FMT>
+__device__ __forceinline__ float kv8_decode(uint32_t b) {
+  if (FMT == CB_KV8_E4M3) return e4m3_to_f32(b & 0xFF);
+  return (float)(int8_t)(b & 0xFF);
+}
+
+// Element i of an array of one of the three input types.
+__device__ __forceinline__ float kv8_load(const void* p, int64_t i, int dtype) {
+  if (dtype == CB_F32) return static_cast<const float*>(p)[i];
+  const uint32_t u = static_cast<const uint16_t*>(p)[i];
+  return dtype == CB_BF16 ? bf16_to_f32(u) : __half2float(__ushort_as_half((unsigned short)u));
+}
+
+}  // namespace cb

@@ -1,0 +1,31 @@
+// Internal interface of the attention over the 8-bit K/V cache.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "cirrus_b200.h"
+
+namespace cb {
+
+struct AttendParams {
+  CbKv8 c;
+  const void* q;
+  int dtype;
+  int64_t qs[3];        // element strides between sequences, tokens, heads
+  int G, T, rows;       // query heads per KV head; rows = T * G of a KV head
+  const int32_t* pos;
+  const int32_t* counts;
+  float scale;
+  bool add_mass;
+  void* out;            // [batch][T][heads][dim], the queries' type
+  float* lse;           // [batch][T][heads]
+  int splits;
+  float* part_ml;       // [batch * kv heads][rows][splits][2] running maximum (log2 units) and sum
+  float* part_o;        // [batch * kv heads][rows][splits][dim]
+};
+
+int kv8_check(const CbKv8* c);
+bool kv8_dtype_ok(int dtype);
+
+}  // namespace cb

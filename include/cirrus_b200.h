@@ -391,6 +391,89 @@ int cb_spec_accept(const CbModel* m, const CbCache* c, const int32_t* argmax, co
                    const int32_t* draft_len, int32_t T, int32_t* tokens, int32_t ld, int32_t* lens,
                    int32_t* budget, int64_t* emitted, void* stream);
 
+/* --------------------------------------------- K/V cache in 8 bits */
+/* A K/V cache of `batch` sequences whose keys and values are held in 8 bits with
+ * one float32 scale for each block of CB_KV8_BLOCK slots and KV head.  A scale is
+ * a power of two, the smallest 2^e (-100 <= e <= 120) with absmax <= qmax * 2^e
+ * (qmax 448 for E4M3, 127 for int8); a value is code * scale.  How many slots of
+ * sequence b are in use is the caller's pos[b] (device int32), passed to every
+ * call; slots from pos[b] on may hold anything.  mass[b][h][j] adds up the
+ * attention weight that slot j has received (null: not kept).
+ * head_dim 16, 32, 64 or 128; max_len a multiple of CB_KV8_BLOCK; k and v
+ * 16-byte aligned.  The reference keeps the shared K/V in the model's type
+ * (cirrus/model/model.py:41-51) and has no 8-bit cache. */
+#define CB_KV8_BLOCK 64
+enum { CB_KV8_E4M3 = 0, CB_KV8_INT8 = 1 };
+enum { CB_F32 = 0, CB_BF16 = 1, CB_F16 = 2 };
+typedef struct CbKv8 {
+  int32_t batch, n_kv_heads, head_dim, max_len, format;
+  uint8_t* k;      /* [batch][n_kv_heads][max_len][head_dim] codes */
+  uint8_t* v;
+  float* k_scale;  /* [batch][n_kv_heads][max_len / CB_KV8_BLOCK] */
+  float* v_scale;
+  float* mass;     /* [batch][n_kv_heads][max_len] or null */
+} CbKv8;
+
+/* Writes T tokens per sequence (counts[b] of them where counts is given) to slots
+ * pos[b] .. of every KV head, and zeroes their mass.  k, v: CB_F32 / CB_BF16 /
+ * CB_F16, element (b, t, h, d) at b * strides[0] + t * strides[1] + h * strides[2]
+ * + d.  The scale of a block that holds tokens already becomes the larger of its
+ * own and the one the new tokens need, and its codes are rounded onto it (nearest,
+ * ties to even); a block that starts empty takes the scale its tokens need.
+ * Infinities saturate and do not raise the scale; a NaN stays one in E4M3 and
+ * becomes 0 in int8.  pos is not advanced.  Tokens that would pass max_len are
+ * dropped and *status (device int32, may be null) receives CB_ERR_CTX_FULL;
+ * a negative pos[b] leaves sequence b alone. */
+int cb_kv8_append(const CbKv8* c, const void* k, const void* v, int32_t dtype, const int64_t* k_strides,
+                  const int64_t* v_strides, int32_t T, const int32_t* pos, const int32_t* counts, int32_t* status,
+                  void* stream);
+
+/* Causal attention of T query tokens per sequence over the cache, after their keys
+ * have been appended with the same pos: row t of sequence b sees slots
+ * j <= pos[b] + t.  q (its type and strides as k above) holds n_q_heads heads, a
+ * multiple of n_kv_heads; query head i reads KV head i / (n_q_heads / n_kv_heads).
+ *   out [batch][T][n_q_heads][head_dim], q's type: softmax(scale * q . k) v
+ *   lse [batch][T][n_q_heads] float32: log of the softmax's sum (natural log)
+ *   add_mass: mass[b][h][j] += the probabilities of slot j over the head's rows
+ * Rows that see nothing (t >= counts[b], pos[b] + t < 0) give 0 and -infinity.
+ * Sums are float32; 16-bit queries meet the codes exactly and the probabilities
+ * are rounded to f16 for the product with v; float32 queries and probabilities
+ * are carried in about 22 bits.  longest: a bound on pos[b] + T that sizes the
+ * launch.  scratch: cb_kv8_attend_scratch_bytes(c, n_q_heads, T, longest) bytes,
+ * 16-byte aligned, not shared by calls that overlap.
+ * Replaces the dense attention of CrossAttention.forward over the shared K/V
+ * (cirrus/model/layers.py:183-192, 325-339). */
+size_t cb_kv8_attend_scratch_bytes(const CbKv8* c, int32_t n_q_heads, int32_t T, int32_t longest);
+int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const int64_t* q_strides, int32_t n_q_heads,
+                  int32_t T, const int32_t* pos, const int32_t* counts, int32_t longest, float scale,
+                  int32_t add_mass, void* out, float* lse, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Brings every sequence with pos[b] > keep down to keep tokens, for each KV head
+ * on its own: the `recent` last slots stay, and of the older ones the
+ * keep - recent of largest mass (ties to the lowest slot; NaN counts as the
+ * smallest).  The kept tokens move to slots 0 .. keep - 1 in order, with their
+ * mass; each block takes the scale its tokens need.  kept [batch][n_kv_heads][keep]
+ * (device int32) receives the slots they came from, -1 past the end of shorter
+ * sequences, which stay as they are; new_pos[b] = min(pos[b], keep) (not pos itself). */
+int cb_kv8_evict(const CbKv8* c, const int32_t* pos, int32_t keep, int32_t recent, int32_t* kept, int32_t* new_pos,
+                 void* stream);
+
+/* ------------------------------------------------- log probabilities */
+/* For each of `rows` rows of logits [rows][ld] (CB_F32 / CB_BF16 / CB_F16, V of
+ * them): logprob = log softmax(x)[tokens[r]], entropy = -sum p log p (natural
+ * log), rank = how many logits are larger than the token's, and the `top` largest
+ * in order (ties to the lowest token) as top_logprob / top_token [rows][top].
+ * tokens[r] < 0: no token (logprob 0, rank -1); tokens[r] >= V: the same, and
+ * *status (device int32, may be null) receives CB_ERR_TOKEN.  -infinity marks a
+ * token that cannot occur.  Sums are float32.  top <= CB_LOGPROB_MAX_TOP and <= V,
+ * V <= CB_LOGPROB_MAX_VOCAB.
+ * Replaces log_softmax + gather of the reference's loss (cirrus/model/model.py:176-228). */
+#define CB_LOGPROB_MAX_TOP 32
+#define CB_LOGPROB_MAX_VOCAB (1 << 20)
+int cb_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t V, const int32_t* tokens,
+                      int32_t top, float* logprob, float* entropy, int32_t* rank, float* top_logprob,
+                      int32_t* top_token, int32_t* status, void* stream);
+
 /* Copy the workspace's device status word into *status (synchronises on the stream). */
 int cb_read_status(const void* workspace, int32_t* status, void* stream);
 /* Clear the status word (stream-ordered). */
