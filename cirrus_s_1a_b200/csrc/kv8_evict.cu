@@ -3,19 +3,38 @@
 // keep - recent with the largest accumulated attention weight (ties to the
 // lowest slot).  The kept tokens move to slots 0 .. keep - 1 in order, in place.
 //
-// One CTA per (sequence, KV head): a radix select over the weights' order keys
-// (8 bits a pass), an ordered scan that writes the kept slots, then the blocks
-// of 64 kept tokens one after another.  In place is safe in that order: the
-// token for slot j comes from a slot >= j, so what block i overwrites (slots
-// below 64 (i + 1)) is read by no later block.  A new block's scale is the one
-// its values need; a code is rounded again only where its scale grows.
+// One cluster of CTAs per (sequence, KV head).
+//   1. The smallest weight that stays: a radix select over the weights' order
+//      keys in three passes of 11, 11 and 10 bits.  Each CTA counts a stretch of
+//      the slots; each adds up its share of the bins over all histograms through
+//      distributed shared memory, and all read the sums and find the same digit.
+//      (Every CTA reading all histograms took 24 us a pass in a cluster of 16.)
+//   2. The kept slots in order: each warp counts its stretch, the counts are
+//      shared, and a second walk writes the slot numbers.
+//   3. The move, in rounds of 32 KB of codes per CTA.  The token for slot j comes
+//      from a slot >= j, so what a round writes is read by no later round, and
+//      copies run two rounds ahead (cp.async into a ring of three stages); within
+//      a round every CTA has read before any writes, which takes one cluster
+//      barrier, arrived at when the round's copies have landed.
+// A new block takes the scale its values need; a code is rounded again only
+// where its scale grows, and copied as it is where the scale stays.
+#include <cooperative_groups.h>
+
 #include "kv8.cuh"
 #include "kv8_attend.cuh"
 
 namespace cb {
 namespace {
 
-constexpr int kET = 1024;
+namespace cg = cooperative_groups;
+
+constexpr int kET = 512;
+constexpr int kEWarps = kET / 32;
+constexpr int kBins = 2048;
+constexpr int kPieces = 4;  // 16-byte pieces of one thread in a round
+constexpr int kMaxCluster = 16;
+constexpr int kStages = 3;
+constexpr int kSrcRing = 4;
 
 struct EvictParams {
   CbKv8 c;
@@ -28,151 +47,313 @@ struct EvictParams {
 // Order key of a weight: larger weight, larger key; NaN below everything.
 __device__ __forceinline__ uint32_t weight_key(float w) { return w != w ? 0u : score_key(w); }
 
-// Exclusive prefix sum over the CTA of one int per thread; total to *all.
-__device__ __forceinline__ int block_scan(int v, int* red, int* all) {
+// Sum over the threads after this one (higher tid) of v; needs 32 ints of scratch.
+__device__ __forceinline__ int sum_after(int v, int* red) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   int x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+    const int y = __shfl_down_sync(0xffffffffu, x, o);
+    if (lane + o < 32) x += y;
   }
   __syncthreads();
-  if (lane == 31) red[w] = x;
+  if (lane == 0) red[w] = x;
   __syncthreads();
-  if (w == 0) {
-    int y = red[lane];
+  int after = x - v;
+  for (int i = w + 1; i < kEWarps; ++i) after += red[i];
+  return after;
+}
+
+// Largest |code| of 16 bytes as the float it stands for (a NaN does not count).
+template <int FMT>
+__device__ __forceinline__ float piece_max(uint4 c) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  if (FMT == CB_KV8_INT8) {
+    const uint32_t a = __vmaxu4(__vmaxu4(__vabs4(w[0]), __vabs4(w[1])), __vmaxu4(__vabs4(w[2]), __vabs4(w[3])));
+    return (float)max(max(a & 0xFF, (a >> 8) & 0xFF), max((a >> 16) & 0xFF, a >> 24));
+  }
+  uint32_t a = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int z = __shfl_up_sync(0xffffffffu, y, o);
-      if (lane >= o) y += z;
-    }
-    red[lane] = y;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t m = w[i] & 0x7F7F7F7Fu;
+    a = __vmaxu4(a, m & ~__vcmpeq4(m, 0x7F7F7F7Fu));
   }
-  __syncthreads();
-  *all = red[31];
-  return x - v + (w ? red[w - 1] : 0);
+  return e4m3_to_f32(max(max(a & 0xFF, (a >> 8) & 0xFF), max((a >> 16) & 0xFF, a >> 24)));
+}
+
+// 16 codes times a power of two, as codes.
+template <int FMT>
+__device__ __forceinline__ uint4 rescale(uint4 c, float f) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t o[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    o[i / 4] |= kv8_encode<FMT>(kv8_decode<FMT>(w[i / 4] >> (8 * (i & 3))) * f) << (8 * (i & 3));
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Shared memory of the move: the ring of codes, then of each token's two scales
+// and mass, then of source slots.  The selection's histograms lie under it.
+template <int D>
+struct Move {
+  static constexpr int kRow = D / 16;                        // 16-byte pieces of a token
+  static constexpr int kUnit = kKv8Block * kRow;             // of a block of K or V
+  static constexpr int kUnits = kPieces * kET / kUnit;       // per round, K and V of a block in turn
+  static constexpr int kBlocks = kUnits / 2;
+  static constexpr int kTokens = kBlocks * kKv8Block;
+  static constexpr int kCodes = kPieces * kET * 16;          // bytes of a stage
+  static constexpr int kBytes = kStages * (kCodes + 3 * kTokens * 4) + kSrcRing * kTokens * 4;
+  static_assert(kBytes >= 4 * kBins * 4, "the histograms lie under the ring");
+};
+
+__device__ __forceinline__ void cp16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void cp4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
 }
 
 template <int D, int FMT>
-__global__ void __launch_bounds__(kET) kv8_evict_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ int hist[256];
-  __shared__ int red[32];
-  __shared__ float fred[33];
-  __shared__ uint32_t s_prefix;
+__global__ void __launch_bounds__(kET, 2) kv8_evict_kernel(const __grid_constant__ EvictParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  int(*hist)[kBins] = reinterpret_cast<int(*)[kBins]>(smem);  // [3]
+  int* total = reinterpret_cast<int*>(smem) + 3 * kBins;      // this CTA's share of the bins, all CTAs
+  __shared__ int red[kEWarps];
+  __shared__ uint32_t s_digit;
   __shared__ int s_rest;
-  const int h = blockIdx.x % p.c.n_kv_heads, b = blockIdx.x / p.c.n_kv_heads, tid = threadIdx.x;
+  __shared__ int s_stay[kEWarps], s_tie[kEWarps];
+  __shared__ int s_count[2];
+  cg::cluster_group cl = cg::this_cluster();
+  const int nc = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t head = blockIdx.x / nc;
+  const int b = (int)(head / p.c.n_kv_heads);
   const int n = min(max(p.pos[b], 0), p.c.max_len), keep = p.keep;
-  const int64_t head = blockIdx.x;
   int32_t* kept = p.kept + head * keep;
-  if (h == 0 && tid == 0) p.new_pos[b] = min(n, keep);
-  if (n <= keep) {
-    for (int j = tid; j < keep; j += kET) kept[j] = j < n ? j : -1;
+  if (head % p.c.n_kv_heads == 0 && rank == 0 && tid == 0) p.new_pos[b] = min(n, keep);
+  if (n <= keep) {  // the whole cluster takes this way
+    for (int j = rank * kET + tid; j < keep; j += nc * kET) kept[j] = j < n ? j : -1;
     return;
   }
   float* mass = p.c.mass + head * p.c.max_len;
-  const int old = n - p.recent;       // candidates: slots below this
-  const int want = keep - p.recent;   // how many of them stay, < old
+  const int old = n - p.recent;      // candidates: slots below this
+  const int want = keep - p.recent;  // how many of them stay, < old
+  // this CTA's stretch of the slots, whole warps' worth of 32 each
+  const int seg = ceil_div(ceil_div(n, nc), kET) * 32, chunk = seg * kEWarps;
+  const int beg = min(n, rank * chunk), end = min(n, beg + chunk);
 
-  // the want-th largest key: `prefix`, and how many of its ties stay
-  uint32_t prefix = 0, mask = 0;
+  // 1. the want-th largest key, and how many of its equals stay
+  for (int i = tid; i < 3 * kBins; i += kET) (&hist[0][0])[i] = 0;
+  uint32_t key = 0, mask = 0;
   int rest = want;
-  if (want > 0)
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kET) hist[i] = 0;
-      __syncthreads();
-      for (int j = tid; j < old; j += kET) {
+  __syncthreads();
+  if (want > 0) {
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      int* h = hist[pass];
+      for (int j = beg + tid; j < min(end, old); j += kET) {
         const uint32_t u = weight_key(mass[j]);
-        if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255], 1);
+        if ((u & mask) == key) atomicAdd(&h[(u >> shift) & ((1 << bits) - 1)], 1);
+      }
+      cl.sync();  // the histograms are complete, and the last pass's totals read
+      const int share = kBins / nc;
+      for (int i = tid; i < share; i += kET) total[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = tid; i < kBins; i += kET)
+        atomicAdd(&total[i % share], cl.map_shared_rank(h, i / share)[rank * share + i % share]);
+      cl.sync();
+      // bins 4 tid .. + 3
+      const int4 c4 = *reinterpret_cast<const int4*>(cl.map_shared_rank(total, 4 * tid / share) + 4 * tid % share);
+      const int c[kBins / kET] = {c4.x, c4.y, c4.z, c4.w};
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < kBins / kET; ++i) mine += c[i];
+      int after = sum_after(mine, red);
+      if (after < rest && after + mine >= rest) {
+        int i = kBins / kET - 1;
+        while (after + c[i] < rest) after += c[i--];
+        s_digit = (uint32_t)(tid * (kBins / kET) + i);
+        s_rest = rest - after;
       }
       __syncthreads();
-      if (tid == 0) {
-        int d = 255, left = rest;
-        while (hist[d] < left) left -= hist[d--];
-        s_prefix = prefix | ((uint32_t)d << shift);
-        s_rest = left;
-      }
-      __syncthreads();
-      prefix = s_prefix;
+      key |= s_digit << shift;
+      mask |= ((1u << bits) - 1u) << shift;
       rest = s_rest;
-      mask |= 255u << shift;
       __syncthreads();
     }
+  }
 
-  // kept slots in order
-  int base = 0, ties = 0;
-  for (int j0 = 0; j0 < n; j0 += kET) {
-    const int j = j0 + tid;
-    bool above = false, tie = false;
-    if (j < old && want > 0) {
-      const uint32_t u = weight_key(mass[j]);
-      above = u > prefix;
-      tie = u == prefix;
-    }
-    int nt;
-    const int tb = ties + block_scan(tie, red, &nt);
-    const bool stay = j < n && (j >= old || above || (tie && tb < rest));
-    ties += nt;
-    int ns;
-    const int at = base + block_scan(stay, red, &ns);
-    if (stay) kept[at] = j;
-    base += ns;
+  // 2. the kept slots in order
+  const int w0 = beg + warp * seg, w1 = min(end, w0 + seg);
+  int stay = 0, tie = 0;
+  for (int j0 = w0; j0 < w1; j0 += 32) {
+    const int j = j0 + lane;
+    const uint32_t u = j < w1 && j < old ? weight_key(mass[j]) : 0u;
+    stay += __popc(__ballot_sync(0xffffffffu, j < w1 && (j >= old || (want > 0 && u > key))));
+    tie += __popc(__ballot_sync(0xffffffffu, j < w1 && j < old && want > 0 && u == key));
+  }
+  if (lane == 0) {
+    s_stay[warp] = stay;
+    s_tie[warp] = tie;
   }
   __syncthreads();
-
-  // blocks of 64 kept tokens
-  constexpr int kPer = D / 8, kPieces = kKv8Block * kPer;
-  constexpr int kMine = (kPieces + kET - 1) / kET;
-  const int64_t nb = p.c.max_len / kKv8Block;
-  for (int first = 0; first < keep; first += kKv8Block) {
-    const int cnt = min(kKv8Block, keep - first);
-#pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      uint8_t* codes = (kv ? p.c.v : p.c.k) + head * p.c.max_len * D;
-      float* scale = (kv ? p.c.v_scale : p.c.k_scale) + head * nb;
-      float x[kMine][8];
-      float top = 0.0f;
-#pragma unroll
-      for (int m = 0; m < kMine; ++m) {
-        const int piece = tid + m * kET, tok = piece / kPer;
-        if (tok >= cnt) continue;
-        const int src = kept[first + tok];
-        const uint2 c = *reinterpret_cast<const uint2*>(codes + (int64_t)src * D + (piece % kPer) * 8);
-        const float s = scale[src / kKv8Block];
-        const uint32_t w[2] = {c.x, c.y};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[m][i] = kv8_decode<FMT>(w[i / 4] >> (8 * (i & 3))) * s;
-          if (fabsf(x[m][i]) < INFINITY) top = fmaxf(top, fabsf(x[m][i]));
-        }
-      }
-      top = block_max(top, fred);  // its barriers end the reads of this block
-      const int e = kv8_need<FMT>(top);
-      const float inv = kv8_pow2(-e);
-#pragma unroll
-      for (int m = 0; m < kMine; ++m) {
-        const int piece = tid + m * kET, tok = piece / kPer;
-        if (tok >= cnt) continue;
-        uint32_t w[2] = {0u, 0u};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i / 4] |= kv8_encode<FMT>(x[m][i] * inv) << (8 * (i & 3));
-        *reinterpret_cast<uint2*>(codes + (int64_t)first * D + piece * 8) = make_uint2(w[0], w[1]);
-      }
-      if (tid == 0) scale[first / kKv8Block] = kv8_pow2(e);
+  int base = 0, ties = 0;  // of the warps before this one
+  for (int w = 0; w < kEWarps; ++w) {
+    if (tid == 0) {
+      if (w == 0) s_count[0] = s_count[1] = 0;
+      s_count[0] += s_stay[w];
+      s_count[1] += s_tie[w];
     }
-    float w = 0.0f;
-    if (tid < cnt) w = mass[kept[first + tid]];
-    __syncthreads();
-    if (tid < cnt) mass[first + tid] = w;
-    __syncthreads();
+    base += w < warp ? s_stay[w] : 0;
+    ties += w < warp ? s_tie[w] : 0;
   }
+  cl.sync();
+  for (int r = 0; r < rank; ++r) {
+    const int* o = cl.map_shared_rank(s_count, r);
+    base += o[0];
+    ties += o[1];
+  }
+  for (int j0 = w0; j0 < w1; j0 += 32) {
+    const int j = j0 + lane;
+    const uint32_t u = j < w1 && j < old ? weight_key(mass[j]) : 0u;
+    const bool st = j < w1 && (j >= old || (want > 0 && u > key));
+    const bool ti = j < w1 && j < old && want > 0 && u == key;
+    const unsigned sb = __ballot_sync(0xffffffffu, st), tb = __ballot_sync(0xffffffffu, ti);
+    const unsigned before = (1u << lane) - 1u;
+    const int t = ties + __popc(tb & before);
+    if (st || (ti && t < rest)) kept[base + __popc(sb & before) + min(rest, t)] = j;
+    base += __popc(sb);
+    ties += __popc(tb);
+  }
+  cl.sync();  // every CTA's slot numbers are visible to the cluster
+
+  // 3. the move.  Piece i of a round: 16 bytes of one token, in unit i / kUnit.
+  using M = Move<D>;
+  __shared__ unsigned s_max[2][M::kUnits];
+  float* s_float = reinterpret_cast<float*>(smem + kStages * M::kCodes);                  // [stage][3][tokens]
+  int* s_src = reinterpret_cast<int*>(s_float + kStages * 3 * M::kTokens);                // [ring][tokens]
+  const int64_t nb = p.c.max_len / kKv8Block;
+  auto codes = [&](int kv) { return (kv ? p.c.v : p.c.k) + head * p.c.max_len * D; };
+  auto scales = [&](int kv) { return (kv ? p.c.v_scale : p.c.k_scale) + head * nb; };
+  const int rounds = ceil_div(ceil_div(keep, kKv8Block), M::kBlocks * nc);
+  if (tid < 2 * M::kUnits) (&s_max[0][0])[tid] = 0u;
+  // destination slot of token t of this CTA in a round, -1: none
+  auto dest = [&](int round, int t) {
+    const int j = (round * nc + rank) * M::kTokens + t;
+    return round < rounds && j < keep ? j : -1;
+  };
+  auto copy_src = [&](int round) {
+    for (int t = tid; t < M::kTokens; t += kET)
+      if (const int j = dest(round, t); j >= 0) cp4(s_src + round % kSrcRing * M::kTokens + t, kept + j);
+  };
+  auto copy_codes = [&](int round) {
+    const int* src = s_src + round % kSrcRing * M::kTokens;
+    float* f = s_float + round % kStages * 3 * M::kTokens;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int piece = tid + i * kET, unit = piece / M::kUnit, in = piece % M::kUnit;
+      const int t = unit / 2 * kKv8Block + in / M::kRow;
+      if (dest(round, t) >= 0)
+        cp16(smem + round % kStages * M::kCodes + piece * 16,
+             codes(unit & 1) + (int64_t)src[t] * D + in % M::kRow * 16);
+    }
+    for (int t = tid; t < M::kTokens; t += kET)
+      if (dest(round, t) >= 0) {
+        cp4(f + t, scales(0) + src[t] / kKv8Block);
+        cp4(f + M::kTokens + t, scales(1) + src[t] / kKv8Block);
+        cp4(f + 2 * M::kTokens + t, mass + src[t]);
+      }
+  };
+  auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  for (int r = 0; r < kSrcRing; ++r) copy_src(r);
+  commit();
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  copy_codes(0);
+  commit();
+  copy_codes(1);
+  commit();
+  for (int round = 0; round < rounds; ++round) {
+    // all but the newest group: this round's codes, and the sources of round + 2
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncthreads();
+    cl.barrier_arrive();  // this CTA has read what this round's writes may lie over
+    copy_codes(round + 2);
+    copy_src(round + kSrcRing);
+    commit();
+    unsigned* top = s_max[round & 1];
+    const uint8_t* stage = smem + round % kStages * M::kCodes;
+    const float* f = s_float + round % kStages * 3 * M::kTokens;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int piece = tid + i * kET, unit = piece / M::kUnit, t = unit / 2 * kKv8Block + piece % M::kUnit / M::kRow;
+      float a = 0.0f;
+      if (dest(round, t) >= 0)
+        a = piece_max<FMT>(*reinterpret_cast<const uint4*>(stage + piece * 16)) * f[(unit & 1) * M::kTokens + t];
+      const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(a));
+      if (lane == 0) atomicMax(&top[unit], m);
+    }
+    __syncthreads();
+    if (tid < M::kUnits) s_max[(round + 1) & 1][tid] = 0u;  // read last before this round's first barrier
+    cl.barrier_wait();
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int piece = tid + i * kET, unit = piece / M::kUnit, in = piece % M::kUnit;
+      const int t = unit / 2 * kKv8Block + in / M::kRow, j = dest(round, t);
+      if (j < 0) continue;
+      const uint4 c = *reinterpret_cast<const uint4*>(stage + piece * 16);
+      const float was = f[(unit & 1) * M::kTokens + t];
+      const int e = kv8_need<FMT>(__uint_as_float(top[unit]));
+      const float now = kv8_pow2(e);
+      // no code but 0 stays within its format under a factor above 2^20
+      const uint4 o = was == now ? c : rescale<FMT>(c, fminf(was * kv8_pow2(-e), 1048576.0f));
+      *reinterpret_cast<uint4*>(codes(unit & 1) + (int64_t)j * D + in % M::kRow * 16) = o;
+      if (in == 0) scales(unit & 1)[j / kKv8Block] = now;
+    }
+    for (int t = tid; t < M::kTokens; t += kET)
+      if (const int j = dest(round, t); j >= 0) mass[j] = f[2 * M::kTokens + t];
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+template <int D, int FMT>
+int launch_df(const EvictParams& p, cudaStream_t st) {
+  // the largest cluster that leaves all of them resident at two CTAs per SM:
+  // few heads get many CTAs each, many heads get few
+  const int heads = p.c.batch * p.c.n_kv_heads;
+  auto fn = kv8_evict_kernel<D, FMT>;
+  if (const int rc = ensure_smem_attr((const void*)fn, Move<D>::kBytes)) return rc;
+  int nc = kMaxCluster;
+  while (nc > 1 && heads * nc > 2 * num_sms()) nc >>= 1;
+  if (nc == kMaxCluster &&
+      cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    (void)cudaGetLastError();
+    nc = 8;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(heads * nc);
+  cfg.blockDim = dim3(kET);
+  cfg.dynamicSmemBytes = Move<D>::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = nc;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, fn, p);
+  count_launch();
+  return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
 }
 
 template <int D>
-void launch(const EvictParams& p, cudaStream_t st) {
-  const int grid = p.c.batch * p.c.n_kv_heads;
-  if (p.c.format == CB_KV8_E4M3) kv8_evict_kernel<D, CB_KV8_E4M3><<<grid, kET, 0, st>>>(p);
-  else kv8_evict_kernel<D, CB_KV8_INT8><<<grid, kET, 0, st>>>(p);
+int launch(const EvictParams& p, cudaStream_t st) {
+  return p.c.format == CB_KV8_E4M3 ? launch_df<D, CB_KV8_E4M3>(p, st) : launch_df<D, CB_KV8_INT8>(p, st);
 }
 
 }  // namespace
@@ -189,11 +370,9 @@ extern "C" int cb_kv8_evict(const CbKv8* c, const int32_t* pos, int32_t keep, in
   const EvictParams p{*c, pos, keep, recent, kept, new_pos};
   cudaStream_t st = (cudaStream_t)stream;
   switch (c->head_dim) {
-    case 16: launch<16>(p, st); break;
-    case 32: launch<32>(p, st); break;
-    case 64: launch<64>(p, st); break;
-    default: launch<128>(p, st); break;
+    case 16: return launch<16>(p, st);
+    case 32: return launch<32>(p, st);
+    case 64: return launch<64>(p, st);
+    default: return launch<128>(p, st);
   }
-  count_launch();
-  return cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
 }

@@ -132,7 +132,8 @@ def evict(c: dict, fmt: str, pos: list, keep: int, recent: int) -> tuple:
 
 def token_logprobs(x: torch.Tensor, tokens: list, top: int) -> tuple:
     """x float64 [R, V] -> (logprob, entropy, rank, top_logprob, top_token)."""
-    logp = x - torch.logsumexp(x, -1, keepdim=True)
+    d = x - x.amax(-1, keepdim=True)  # first: the sum's logarithm would be lost next to a logit of 1e38
+    logp = d - d.exp().sum(-1, keepdim=True).log()
     entropy = torch.special.entr(logp.exp()).sum(-1)
     logprob = torch.tensor([0.0 if t < 0 else float(logp[r, t]) for r, t in enumerate(tokens)], dtype=torch.float64)
     rank = torch.tensor([-1 if t < 0 else int((x[r] > x[r, t]).sum()) for r, t in enumerate(tokens)])
