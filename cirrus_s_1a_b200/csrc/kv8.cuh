@@ -53,6 +53,42 @@ __device__ __forceinline__ float kv8_decode(uint32_t b) {
   return (float)(int8_t)(b & 0xFF);
 }
 
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// Four codes of one word -> exact f16x2 of bytes (0, 1) and (2, 3).
+template <int FMT>
+__device__ __forceinline__ void codes_to_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (FMT == CB_KV8_E4M3) {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFF), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    lo = (uint32_t)a.x | ((uint32_t)a.y << 16);
+    hi = (uint32_t)b.x | ((uint32_t)b.y << 16);
+  } else {
+    // byte u = code + 128 under the exponent of 1024: the half 1024 + u, less 1152
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+    lo = h2_bits(__hsub2(bits_h2(__byte_perm(u, 0x64646464u, 0x4140)), off));
+    hi = h2_bits(__hsub2(bits_h2(__byte_perm(u, 0x64646464u, 0x4342)), off));
+  }
+}
+
+// Two pairs of exact code values times a power of two f <= 2^15, rounded to four
+// codes.  E4M3: the f16 product is exact down to 2^-24, far below half the
+// smallest code.  int8: v * f + 1536 rounds to an integer (ties to even), whose
+// low byte is the code.
+template <int FMT>
+__device__ __forceinline__ uint32_t h2_to_codes(uint32_t lo, uint32_t hi, __half2 f) {
+  if (FMT == CB_KV8_E4M3) {
+    const __half2 a = __hmul2(bits_h2(lo), f), b = __hmul2(bits_h2(hi), f);
+    const uint32_t x = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(a), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t y = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(b), __NV_SATFINITE, __NV_E4M3);
+    return x | (y << 16);
+  }
+  const __half2 magic = __floats2half2_rn(1536.0f, 1536.0f);
+  return __byte_perm(h2_bits(__hfma2(bits_h2(lo), f, magic)), h2_bits(__hfma2(bits_h2(hi), f, magic)), 0x6420);
+}
+
 // Element i of an array of one of the three input types.
 __device__ __forceinline__ float kv8_load(const void* p, int64_t i, int dtype) {
   if (dtype == CB_F32) return static_cast<const float*>(p)[i];

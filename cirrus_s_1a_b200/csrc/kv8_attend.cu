@@ -42,26 +42,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-
-// Four codes of one word -> f16x2 of bytes (0, 1) and (2, 3).
-template <int FMT>
-__device__ __forceinline__ void codes_to_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if (FMT == CB_KV8_E4M3) {
-    __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFF), __NV_E4M3);
-    __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
-    lo = (uint32_t)a.x | ((uint32_t)a.y << 16);
-    hi = (uint32_t)b.x | ((uint32_t)b.y << 16);
-  } else {
-    // byte u = code + 128 under the exponent of 1024: the half 1024 + u, less 1152
-    const uint32_t u = w ^ 0x80808080u;
-    const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
-    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    lo = h2_bits(__hsub2(*reinterpret_cast<__half2*>(&a), off));
-    hi = h2_bits(__hsub2(*reinterpret_cast<__half2*>(&b), off));
-  }
-}
-
 __device__ __forceinline__ float exp2a(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

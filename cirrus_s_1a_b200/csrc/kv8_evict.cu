@@ -64,32 +64,13 @@ __device__ __forceinline__ int sum_after(int v, int* red) {
   return after;
 }
 
-// Largest |code| of 16 bytes as the float it stands for (a NaN does not count).
-template <int FMT>
-__device__ __forceinline__ float piece_max(uint4 c) {
-  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-  if (FMT == CB_KV8_INT8) {
-    const uint32_t a = __vmaxu4(__vmaxu4(__vabs4(w[0]), __vabs4(w[1])), __vmaxu4(__vabs4(w[2]), __vabs4(w[3])));
-    return (float)max(max(a & 0xFF, (a >> 8) & 0xFF), max((a >> 16) & 0xFF, a >> 24));
-  }
-  uint32_t a = 0;
+// Largest magnitude of 16 codes (as f16 pairs); a NaN does not count.
+__device__ __forceinline__ float piece_max(const uint32_t (&h)[8]) {
+  __half2 a = __habs2(bits_h2(h[0]));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t m = w[i] & 0x7F7F7F7Fu;
-    a = __vmaxu4(a, m & ~__vcmpeq4(m, 0x7F7F7F7Fu));
-  }
-  return e4m3_to_f32(max(max(a & 0xFF, (a >> 8) & 0xFF), max((a >> 16) & 0xFF, a >> 24)));
-}
-
-// 16 codes times a power of two, as codes.
-template <int FMT>
-__device__ __forceinline__ uint4 rescale(uint4 c, float f) {
-  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-  uint32_t o[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    o[i / 4] |= kv8_encode<FMT>(kv8_decode<FMT>(w[i / 4] >> (8 * (i & 3))) * f) << (8 * (i & 3));
-  return make_uint4(o[0], o[1], o[2], o[3]);
+  for (int i = 1; i < 8; ++i) a = __hmax2(a, __habs2(bits_h2(h[i])));
+  const float m = __half2float(__hmax(__low2half(a), __high2half(a)));
+  return m == m ? m : 0.0f;
 }
 
 // Shared memory of the move: the ring of codes, then of each token's two scales
@@ -189,12 +170,26 @@ __global__ void __launch_bounds__(kET, 2) kv8_evict_kernel(const __grid_constant
 
   // 2. the kept slots in order
   const int w0 = beg + warp * seg, w1 = min(end, w0 + seg);
+  constexpr int kAhead = 8;  // loads of a warp in flight
+  auto weights = [&](int j0, uint32_t (&u)[kAhead]) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = j0 + 32 * i + lane;
+      u[i] = j < min(w1, old) ? weight_key(mass[j]) : 0u;
+    }
+  };
+  auto stays = [&](int j, uint32_t u) { return j < w1 && (j >= old || (want > 0 && u > key)); };
+  auto ties_in = [&](int j, uint32_t u) { return j < min(w1, old) && want > 0 && u == key; };
   int stay = 0, tie = 0;
-  for (int j0 = w0; j0 < w1; j0 += 32) {
-    const int j = j0 + lane;
-    const uint32_t u = j < w1 && j < old ? weight_key(mass[j]) : 0u;
-    stay += __popc(__ballot_sync(0xffffffffu, j < w1 && (j >= old || (want > 0 && u > key))));
-    tie += __popc(__ballot_sync(0xffffffffu, j < w1 && j < old && want > 0 && u == key));
+  for (int j0 = w0; j0 < w1; j0 += 32 * kAhead) {
+    uint32_t u[kAhead];
+    weights(j0, u);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = j0 + 32 * i + lane;
+      stay += __popc(__ballot_sync(0xffffffffu, stays(j, u[i])));
+      tie += __popc(__ballot_sync(0xffffffffu, ties_in(j, u[i])));
+    }
   }
   if (lane == 0) {
     s_stay[warp] = stay;
@@ -217,17 +212,20 @@ __global__ void __launch_bounds__(kET, 2) kv8_evict_kernel(const __grid_constant
     base += o[0];
     ties += o[1];
   }
-  for (int j0 = w0; j0 < w1; j0 += 32) {
-    const int j = j0 + lane;
-    const uint32_t u = j < w1 && j < old ? weight_key(mass[j]) : 0u;
-    const bool st = j < w1 && (j >= old || (want > 0 && u > key));
-    const bool ti = j < w1 && j < old && want > 0 && u == key;
-    const unsigned sb = __ballot_sync(0xffffffffu, st), tb = __ballot_sync(0xffffffffu, ti);
-    const unsigned before = (1u << lane) - 1u;
-    const int t = ties + __popc(tb & before);
-    if (st || (ti && t < rest)) kept[base + __popc(sb & before) + min(rest, t)] = j;
-    base += __popc(sb);
-    ties += __popc(tb);
+  for (int j0 = w0; j0 < w1; j0 += 32 * kAhead) {
+    uint32_t u[kAhead];
+    weights(j0, u);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = j0 + 32 * i + lane;
+      const bool st = stays(j, u[i]), ti = ties_in(j, u[i]);
+      const unsigned sb = __ballot_sync(0xffffffffu, st), tb = __ballot_sync(0xffffffffu, ti);
+      const unsigned before = (1u << lane) - 1u;
+      const int t = ties + __popc(tb & before);
+      if (st || (ti && t < rest)) kept[base + __popc(sb & before) + min(rest, t)] = j;
+      base += __popc(sb);
+      ties += __popc(tb);
+    }
   }
   cl.sync();  // every CTA's slot numbers are visible to the cluster
 
@@ -288,12 +286,16 @@ __global__ void __launch_bounds__(kET, 2) kv8_evict_kernel(const __grid_constant
     unsigned* top = s_max[round & 1];
     const uint8_t* stage = smem + round % kStages * M::kCodes;
     const float* f = s_float + round % kStages * 3 * M::kTokens;
+    uint32_t h[kPieces][8];  // the codes' values, exact in f16
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int piece = tid + i * kET, unit = piece / M::kUnit, t = unit / 2 * kKv8Block + piece % M::kUnit / M::kRow;
-      float a = 0.0f;
-      if (dest(round, t) >= 0)
-        a = piece_max<FMT>(*reinterpret_cast<const uint4*>(stage + piece * 16)) * f[(unit & 1) * M::kTokens + t];
+      const uint4 c = *reinterpret_cast<const uint4*>(stage + piece * 16);
+      codes_to_h2<FMT>(c.x, h[i][0], h[i][1]);
+      codes_to_h2<FMT>(c.y, h[i][2], h[i][3]);
+      codes_to_h2<FMT>(c.z, h[i][4], h[i][5]);
+      codes_to_h2<FMT>(c.w, h[i][6], h[i][7]);
+      const float a = dest(round, t) >= 0 ? piece_max(h[i]) * f[(unit & 1) * M::kTokens + t] : 0.0f;
       const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(a));
       if (lane == 0) atomicMax(&top[unit], m);
     }
@@ -305,12 +307,25 @@ __global__ void __launch_bounds__(kET, 2) kv8_evict_kernel(const __grid_constant
       const int piece = tid + i * kET, unit = piece / M::kUnit, in = piece % M::kUnit;
       const int t = unit / 2 * kKv8Block + in / M::kRow, j = dest(round, t);
       if (j < 0) continue;
-      const uint4 c = *reinterpret_cast<const uint4*>(stage + piece * 16);
       const float was = f[(unit & 1) * M::kTokens + t];
       const int e = kv8_need<FMT>(__uint_as_float(top[unit]));
       const float now = kv8_pow2(e);
-      // no code but 0 stays within its format under a factor above 2^20
-      const uint4 o = was == now ? c : rescale<FMT>(c, fminf(was * kv8_pow2(-e), 1048576.0f));
+      uint4 o;
+      if (was == now) {
+        o = *reinterpret_cast<const uint4*>(stage + piece * 16);
+      } else {
+        // E4M3 codes may grow by up to 2^17: two factors of at most 2^15.  Only
+        // codes of 0 see a larger one cut off.
+        const float by = was * kv8_pow2(-e), by1 = fminf(by, 32768.0f);
+        const __half2 f1 = __float2half2_rn(by1);
+        if (FMT == CB_KV8_E4M3 && by > by1) {
+          const __half2 f2 = __float2half2_rn(fminf(by * (1.0f / 32768.0f), 32768.0f));
+#pragma unroll
+          for (int k = 0; k < 8; ++k) h[i][k] = h2_bits(__hmul2(bits_h2(h[i][k]), f2));
+        }
+        o = make_uint4(h2_to_codes<FMT>(h[i][0], h[i][1], f1), h2_to_codes<FMT>(h[i][2], h[i][3], f1),
+                       h2_to_codes<FMT>(h[i][4], h[i][5], f1), h2_to_codes<FMT>(h[i][6], h[i][7], f1));
+      }
       *reinterpret_cast<uint4*>(codes(unit & 1) + (int64_t)j * D + in % M::kRow * 16) = o;
       if (in == 0) scales(unit & 1)[j / kKv8Block] = now;
     }

@@ -32,6 +32,10 @@ HEAD_DIMS = (16, 32, 64, 128)
 _Strides = C.c_int64 * 3
 
 
+#: device index -> the current stream's pointer (what ``torch.cuda.current_stream`` wraps, without the object)
+raw_stream = torch._C._cuda_getCurrentRawStream if torch.cuda.is_available() else None
+
+
 def _dtype(t: torch.Tensor, name: str) -> int:
     code = DTYPES.get(t.dtype)
     if code is None:
@@ -134,7 +138,7 @@ class Kv8Cache:
         return t.shape[1], t.shape[2], _Strides(sb, st, sh)
 
     def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return raw_stream(self.device.index)
 
     def _call(self, fn, what: str, *args) -> None:
         if torch.cuda.current_device() == self.device.index:

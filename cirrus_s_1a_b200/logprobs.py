@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from cirrus_s_1a_b200 import _lib
-from cirrus_s_1a_b200.kv8 import _dtype
+from cirrus_s_1a_b200.kv8 import _dtype, raw_stream
 
 
 class TokenLogprobs(NamedTuple):
@@ -43,15 +43,16 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
         raise ValueError(f"top must be between 0 and {min(_lib.CB_LOGPROB_MAX_TOP, V)}")
     dtype = _dtype(logits, "logits")
     dev = logits.device
-    f = torch.empty(R * (2 + top), dtype=torch.float32, device=dev)
-    i = torch.empty(R * (1 + top), dtype=torch.int32, device=dev)
-    r = TokenLogprobs(f[:R], f[R:2 * R], i[:R], f[2 * R:].view(R, top), i[R:].view(R, top))
+    r = TokenLogprobs(torch.empty(R, dtype=torch.float32, device=dev), torch.empty(R, dtype=torch.float32, device=dev),
+                      torch.empty(R, dtype=torch.int32, device=dev),
+                      torch.empty(R, top, dtype=torch.float32, device=dev),
+                      torch.empty(R, top, dtype=torch.int32, device=dev))
     if R:
         L = _lib.lib()
-        fp, ip = f.data_ptr(), i.data_ptr()
         ld = logits.stride(0) if R > 1 else V
-        args = (logits.data_ptr(), dtype, ld, R, V, tokens.data_ptr(), top, fp, fp + 4 * R, ip, fp + 8 * R, ip + 4 * R,
-                _lib.ptr(status), torch.cuda.current_stream(dev).cuda_stream)
+        args = (logits.data_ptr(), dtype, ld, R, V, tokens.data_ptr(), top, r.logprob.data_ptr(), r.entropy.data_ptr(),
+                r.rank.data_ptr(), r.top_logprob.data_ptr(), r.top_token.data_ptr(), _lib.ptr(status),
+                raw_stream(dev.index))
         if torch.cuda.current_device() == dev.index:
             rc = L.cb_token_logprobs(*args)
         else:
