@@ -25,6 +25,8 @@
 // as a head and a tail (about 22 bits), two products each.  f16 P (11 bits) for
 // 16-bit outputs adds less than the output's own rounding.
 // Softmax statistics, the sums over V and the joins of parts are float32.
+#include <algorithm>
+
 #include "kv8.cuh"
 #include "kv8_attend.cuh"
 
@@ -365,13 +367,19 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mass_kernel(const __grid_cons
 
 template <int D, int FMT, bool HL>
 int launch_dfh(const AttendParams& p, int bh, int longest, cudaStream_t st) {
-  const int smem = kWarps * 16 * D * (int)sizeof(float);
-  auto fn = kv8_attend_kernel<D, FMT, HL>;
-  if (const int rc = ensure_smem_attr((const void*)fn, smem)) return rc;
-  fn<<<dim3(p.splits, ceil_div(p.rows, 16), bh), kWarps * 32, smem, st>>>(p);
-  count_launch();
-  kv8_join_kernel<<<dim3(p.rows, bh), D, 0, st>>>(p);
-  count_launch();
+  if (p.row_tiles > 0) {
+    if (const int rc = kv8_prompt_launch(p, bh, st)) return rc;
+  } else {
+    const int smem = kWarps * 16 * D * (int)sizeof(float);
+    auto fn = kv8_attend_kernel<D, FMT, HL>;
+    if (const int rc = ensure_smem_attr((const void*)fn, smem)) return rc;
+    fn<<<dim3(p.splits, ceil_div(p.rows, 16), bh), kWarps * 32, smem, st>>>(p);
+    count_launch();
+  }
+  if (p.row_tiles == 0 || p.splits > 1) {
+    kv8_join_kernel<<<dim3(p.rows, bh), D, 0, st>>>(p);
+    count_launch();
+  }
   if (p.add_mass) {
     kv8_mass_kernel<D, FMT, HL><<<dim3(ceil_div(longest, kWarps * kKv8Block), bh), kWarps * 32, 0, st>>>(p);
     count_launch();
@@ -388,12 +396,52 @@ int launch_d(const AttendParams& p, int bh, int longest, cudaStream_t st) {
   return launch_dfh<D, CB_KV8_INT8, false>(p, bh, longest, st);
 }
 
-// Splits of the key axis: enough CTAs for about four on every SM, each with at
-// least one block of 64 keys for each of its warps.
-int attend_splits(int bh, int rows, int longest) {
-  const int tiles = bh * ceil_div(rows, 16);
-  const int want = ceil_div(148 * 4, tiles), most = ceil_div(longest, kWarps * kKv8Block);
-  return want < most ? want : most;
+// How a call is cut up, and where its parts lie in the scratch.
+struct Plan {
+  int rows = 0, row_tiles = 0, splits = 0;
+  size_t o = 0, q16 = 0, back = 0, bytes = 0;  // part_ml at 0
+};
+
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+Plan plan_of(const CbKv8& c, int dtype, int n_q_heads, int T, int longest) {
+  Plan pl;
+  const int bh = c.batch * c.n_kv_heads;
+  pl.rows = T * (n_q_heads / c.n_kv_heads);
+  // From 33 rows on the tensor cores' 128-row tiles pay for the rows they leave empty.
+  if (pl.rows > 32 && c.head_dim >= 64 && dtype != CB_F32) {
+    pl.row_tiles = ceil_div(pl.rows, 128);
+    // runs of key tiles that leave the fewest tile times (and three more a CTA to
+    // start and end) on the busiest SM
+    const int items = bh * ceil_div(pl.row_tiles, 2), tiles = ceil_div(longest, 128);
+    long best = 0;
+    for (int s = 1; s <= 32 && s <= ceil_div(tiles, 2); ++s) {
+      const long cost = (long)ceil_div(items * s, 148) * (ceil_div(tiles, s) + 3);
+      if (pl.splits == 0 || cost < best) {
+        pl.splits = s;
+        best = cost;
+      }
+    }
+  } else {
+    // enough CTAs for about four on every SM, each with at least one block of 64
+    // keys for each of its warps
+    const int items = bh * ceil_div(pl.rows, 16);
+    pl.splits = std::max(1, std::min(ceil_div(148 * 4, items), ceil_div(longest, kWarps * kKv8Block)));
+  }
+  const int64_t parts = (int64_t)bh * pl.rows * pl.splits;
+  pl.o = align256((size_t)parts * 2 * sizeof(float));
+  pl.q16 = pl.o + align256((size_t)parts * c.head_dim * sizeof(float));
+  pl.back = pl.q16 + (size_t)bh * pl.row_tiles * 128 * c.head_dim * 2;
+  pl.bytes = pl.back + (size_t)bh * pl.row_tiles * 128 * sizeof(float);
+  return pl;
+}
+
+int check_call(const CbKv8* c, int dtype, int n_q_heads, int T, int longest) {
+  if (const int rc = kv8_check(c)) return rc;
+  if (T <= 0 || longest <= 0 || !kv8_dtype_ok(dtype)) return CB_ERR_ARG;
+  if (n_q_heads <= 0 || n_q_heads % c->n_kv_heads) return CB_ERR_SHAPE;
+  if ((int64_t)T * (n_q_heads / c->n_kv_heads) > 65535 * 16) return CB_ERR_SHAPE;
+  return CB_OK;
 }
 
 }  // namespace
@@ -401,29 +449,23 @@ int attend_splits(int bh, int rows, int longest) {
 
 using namespace cb;
 
-extern "C" size_t cb_kv8_attend_scratch_bytes(const CbKv8* c, int32_t n_q_heads, int32_t T, int32_t longest) {
-  if (kv8_check(c) != CB_OK || T <= 0 || n_q_heads <= 0 || n_q_heads % c->n_kv_heads || longest <= 0) return 0;
-  if (longest > c->max_len) longest = c->max_len;
-  const int64_t rows = (int64_t)T * (n_q_heads / c->n_kv_heads), bh = (int64_t)c->batch * c->n_kv_heads;
-  if (rows > 65535 * 16) return 0;
-  const int64_t parts = bh * rows * attend_splits((int)bh, (int)rows, longest);
-  return (size_t)parts * (c->head_dim + 2) * sizeof(float);
+extern "C" size_t cb_kv8_attend_scratch_bytes(const CbKv8* c, int32_t dtype, int32_t n_q_heads, int32_t T,
+                                              int32_t longest) {
+  if (check_call(c, dtype, n_q_heads, T, longest) != CB_OK) return 0;
+  return plan_of(*c, dtype, n_q_heads, T, std::min(longest, c->max_len)).bytes;
 }
 
 extern "C" int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const int64_t* q_strides, int32_t n_q_heads,
                              int32_t T, const int32_t* pos, const int32_t* counts, int32_t longest, float scale,
                              int32_t add_mass, void* out, float* lse, void* scratch, size_t scratch_bytes,
-                             void* stream) {
-  const int rc = kv8_check(c);
-  if (rc != CB_OK) return rc;
-  if (!q || !q_strides || !pos || !out || !lse || !scratch || T <= 0 || longest <= 0 || !kv8_dtype_ok(dtype))
+                             int32_t* status, void* stream) {
+  if (const int rc = check_call(c, dtype, n_q_heads, T, longest)) return rc;
+  if (!q || !q_strides || !pos || !out || !lse || !scratch || ((uintptr_t)scratch & 15) || ((uintptr_t)out & 15))
     return CB_ERR_ARG;
-  if (n_q_heads <= 0 || n_q_heads % c->n_kv_heads) return CB_ERR_SHAPE;
   if (add_mass && !c->mass) return CB_ERR_ARG;
-  if (longest > c->max_len) longest = c->max_len;
-  const size_t need = cb_kv8_attend_scratch_bytes(c, n_q_heads, T, longest);
-  if (need == 0) return CB_ERR_SHAPE;
-  if (scratch_bytes < need) return CB_ERR_WORKSPACE;
+  longest = std::min(longest, c->max_len);
+  const Plan pl = plan_of(*c, dtype, n_q_heads, T, longest);
+  if (scratch_bytes < pl.bytes) return CB_ERR_WORKSPACE;
   AttendParams p{};
   p.c = *c;
   p.q = q;
@@ -431,17 +473,22 @@ extern "C" int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const
   for (int i = 0; i < 3; ++i) p.qs[i] = q_strides[i];
   p.G = n_q_heads / c->n_kv_heads;
   p.T = T;
-  p.rows = T * p.G;
+  p.rows = pl.rows;
   p.pos = pos;
   p.counts = counts;
   p.scale = scale;
   p.add_mass = add_mass != 0;
   p.out = out;
   p.lse = lse;
+  p.splits = pl.splits;
+  uint8_t* base = static_cast<uint8_t*>(scratch);
+  p.part_ml = reinterpret_cast<float*>(base);
+  p.part_o = reinterpret_cast<float*>(base + pl.o);
+  p.row_tiles = pl.row_tiles;
+  p.q16 = base + pl.q16;
+  p.q_back = reinterpret_cast<float*>(base + pl.back);
+  p.status = status;
   const int bh = c->batch * c->n_kv_heads;
-  p.splits = attend_splits(bh, p.rows, longest);
-  p.part_ml = static_cast<float*>(scratch);
-  p.part_o = p.part_ml + (int64_t)2 * bh * p.rows * p.splits;
   cudaStream_t st = (cudaStream_t)stream;
   switch (c->head_dim) {
     case 16: return launch_d<16>(p, bh, longest, st);

@@ -23,7 +23,16 @@ struct AttendParams {
   int splits;
   float* part_ml;       // [batch * kv heads][rows][splits][2] running maximum (log2 units) and sum
   float* part_o;        // [batch * kv heads][rows][splits][dim]
+  // the prompt form: query rows prepared in 128-row operand tiles, and the factors that undo their scaling
+  int row_tiles;
+  uint8_t* q16;         // [batch * kv heads][row_tiles][128 * dim * 2 bytes]
+  float* q_back;        // [batch * kv heads][row_tiles * 128]
+  int32_t* status;
 };
+
+// Many query rows, head_dim 64 or 128, 16-bit queries (kv8_prompt.cu).  Writes out
+// and lse where splits is 1, parts otherwise.
+int kv8_prompt_launch(const AttendParams& p, int bh, cudaStream_t st);
 
 int kv8_check(const CbKv8* c);
 bool kv8_dtype_ok(int dtype);

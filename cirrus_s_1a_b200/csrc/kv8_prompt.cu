@@ -1,0 +1,543 @@
+// Attention of many query rows over the 8-bit K/V cache on the 5th-generation
+// tensor cores: the prompt form of cb_kv8_attend for head_dim 64 and 128 and
+// 16-bit queries.
+//
+// kv8_query_kernel prepares the query rows once: each scaled by a power of two
+// (largest element in [256, 512)), rounded to f16 and written as 128-row operand
+// tiles (8-row x 16-byte core matrices), with the factor that undoes the scaling.
+//
+// kv8_prompt_kernel: a CTA owns 256 query rows of one KV head (two tiles of 128)
+// and a run of 128-key tiles.
+//   * 4 warps turn codes into f16 operands in shared memory (two stages each of K
+//     and V): plain conversions, exact; no scale is applied there.
+//   * one thread issues tcgen05.mma kind::f16: S = Q K^T into tensor memory, and
+//     O += P V with P read from tensor memory (V's dims are its contiguous
+//     direction, an MN-major operand).
+//   * two warpgroups, a thread per row, do the softmax.  With x = S * a_b
+//     (a_b = row factor * block b's key scale, in log2 units) and e_b the exponent
+//     of its value scale, a thread keeps m' = max (x + e_b) and writes
+//       P = exp2(x + e_b - m')
+//     so that P times the bare codes is the sum over values, and neither a block
+//     of tiny values nor one of huge ones costs the others precision: P's f16
+//     rounding is relative to what the row adds up.  The row's sum is
+//     l = sum_b 2^-e_b sum P (before P is rounded), the same in float32.
+//   * O is rescaled in tensor memory only when m' has grown by more than 2^8
+//     (P stays below 2^8, the result is exact either way).
+// While one tile is in its softmax the tensor cores work for the other.  The two
+// tiles' exponentials bound it for head_dim 64: 128 x 128 per tile at 16 a clock
+// take 1024 clocks, its products 512.
+// With several runs per row tile, kv8_join_kernel joins them (kv8_attend.cu).
+// Every wait is bounded (%globaltimer); a wait that gives up sets CB_ERR_TIMEOUT
+// in the status word, and the CTA ends without writing results.
+#include "kv8.cuh"
+#include "kv8_attend.cuh"
+
+namespace cb {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kRows = 128;                 // of a tile (MMA M)
+constexpr int kKeys = 128;                 // of a key tile
+constexpr int kTiles = 2;                  // row tiles of a CTA
+constexpr int kStages = 2;
+constexpr int kSoftWarps = 4 * kTiles;
+constexpr int kConvThreads = 128;
+constexpr int kThreads = kSoftWarps * 32 + kConvThreads + 32;
+constexpr float kLazy = 8.0f;              // growth of the maximum, in powers of two, that O follows
+constexpr unsigned long long kTimeoutNs = 200ull * 1000 * 1000;
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ unsigned long long timer_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+  if (mbar_try(bar, parity)) return true;
+  const unsigned long long t0 = timer_ns();
+  while (!mbar_try(bar, parity))
+    if (timer_ns() - t0 > kTimeoutNs) return false;
+  return true;
+}
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Shared-memory matrix descriptor without swizzle, version 1 (bits 46-47).
+// K-major: lbo between K-adjacent core matrices, sbo between 8-row groups.
+// MN-major: lbo between 8-row groups of K, sbo between 16-byte pieces of MN.
+__device__ __forceinline__ uint64_t mat_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 |
+         (uint64_t)((sbo >> 4) & 0x3FFF) << 32 | (uint64_t)1 << 46;
+}
+
+// Instruction descriptor, kind::f16: D f32, A and B f16; bit 16: B is MN-major.
+__host__ __device__ constexpr uint32_t idesc(int m, int n, bool b_mn) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"((uint32_t)add)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"((uint32_t)add)
+      : "memory");
+}
+
+// 32 columns of the warp's 32 lanes of tensor memory, and back.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
+  const uint32_t* u = reinterpret_cast<const uint32_t*>(v);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31,%32};" ::"r"(addr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]),
+      "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]),
+      "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&u)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2a(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Offset of (row, 8-element piece kb) in a K-major operand tile of D dims.
+template <int D>
+__device__ __forceinline__ uint32_t kmajor(int row, int kb) {
+  return (uint32_t)((row >> 3) * (D / 8) * 128 + kb * 128 + (row & 7) * 16);
+}
+
+// The last slot row r of a KV head sees (rows of padding tokens: -1).
+__device__ __forceinline__ int row_limit(const AttendParams& p, int r, int pos, int cnt) {
+  const int t = r / p.G;
+  if (r >= p.rows || t >= cnt) return -1;
+  return min(pos + t, p.c.max_len - 1);
+}
+
+// ------------------------------------------------------------------ queries
+// D/8 lanes per row, 8 elements each.
+template <int D>
+__global__ void __launch_bounds__(256) kv8_query_kernel(const __grid_constant__ AttendParams p) {
+  constexpr int kLanes = D / 8;
+  const int64_t head = blockIdx.y;
+  const int hk = (int)(head % p.c.n_kv_heads), b = (int)(head / p.c.n_kv_heads);
+  const int r = (int)(blockIdx.x * 256 + threadIdx.x) / kLanes, kb = threadIdx.x % kLanes;
+  if (r >= p.row_tiles * kRows) return;  // whole rows leave together
+  float x[8];
+  float top = 0.0f;
+  const bool live = r < p.rows;
+  const int64_t base =
+      (int64_t)b * p.qs[0] + (int64_t)(r / p.G) * p.qs[1] + (hk * p.G + r % p.G) * p.qs[2] + kb * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = live ? kv8_load(p.q, base + i, p.dtype) : 0.0f;
+    top = fmaxf(top, fabsf(x[i]));
+  }
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  int e = 0;
+  if (top > 0.0f && top < INFINITY) e = min(max((__float_as_int(top) >> 23) - 127, -100), 100);
+  const float f = copysignf(kv8_pow2(8 - e), p.scale);
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = h2_bits(__floats2half2_rn(x[2 * i] * f, x[2 * i + 1] * f));
+  uint8_t* tile = p.q16 + (head * p.row_tiles + r / kRows) * (int64_t)(kRows * D * 2);
+  *reinterpret_cast<uint4*>(tile + kmajor<D>(r % kRows, kb)) = make_uint4(h[0], h[1], h[2], h[3]);
+  if (kb == 0) p.q_back[head * p.row_tiles * kRows + r] = live ? kv8_pow2(e - 8) * fabsf(p.scale) * kLog2e : 0.0f;
+}
+
+// --------------------------------------------------------------- attention
+template <int D>
+struct Prompt {
+  static constexpr int kQ = kRows * D * 2;      // bytes of a query tile
+  static constexpr int kKV = kKeys * D * 2;     // of a K or V tile
+  static constexpr int kSmem = kTiles * kQ + 2 * kStages * kKV;
+  // tensor memory: S of both tiles, then P where there is room (else over S), then O
+  static constexpr bool kOver = D == 128;
+  static constexpr int kP = kOver ? 0 : 256, kPStep = kOver ? 128 : 64;
+  static constexpr int kO = kOver ? 256 : 384;
+  static constexpr int kPieces = D / 16;        // 16-byte pieces of a K or V tile per converting thread
+};
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_constant__ AttendParams p) {
+  using C = Prompt<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(8) unsigned long long bars[16];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  uint8_t* sq = smem;
+  uint8_t* sk = smem + kTiles * C::kQ;
+  uint8_t* sv = sk + kStages * C::kKV;
+  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t q_full = bar0, k_full = bar0 + 8, k_free = bar0 + 24, v_full = bar0 + 40, v_free = bar0 + 56,
+                 s_full = bar0 + 72, p_full = bar0 + 88, o_full = bar0 + 104, end = bar0 + 120;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t head = blockIdx.y;
+  const int b = (int)(head / p.c.n_kv_heads);
+  const int pair = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
+  const int row0 = pair * kTiles * kRows;
+  const int tiles = min(kTiles, p.row_tiles - pair * kTiles);
+  const int pos = p.pos[b], cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
+  // the last slot any of the CTA's rows sees, and this run of key tiles
+  int last = -1;
+  {
+    const int rl = min(min(row0 + tiles * kRows, p.rows), cnt * p.G) - 1;
+    if (rl >= row0) last = max(last, row_limit(p, rl, pos, cnt));
+  }
+  const int all = (last + kKeys) / kKeys, per = (all + p.splits - 1) / p.splits;
+  const int beg = min(all, split * per), n = min(all, beg + per) - beg;
+
+  if (tid == 0) {
+    const uint32_t one[] = {q_full, k_free, k_free + 8, v_free, v_free + 8, s_full, s_full + 8, o_full, o_full + 8, end};
+    for (uint32_t bar : one) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar));
+    for (int i = 0; i < 2; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(k_full + 8 * i), "n"(kConvThreads));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(v_full + 8 * i), "n"(kConvThreads));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(p_full + 8 * i), "n"(kRows));
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_abort = 0;
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = s_tmem;
+  bool ok = true;
+  auto wait = [&](uint32_t bar, int phase) {
+    if (ok && !mbar_wait(bar, phase & 1)) {
+      ok = false;
+      s_abort = 1;
+    }
+    return ok;
+  };
+
+  if (warp < kSoftWarps) {
+    // ---------------------------------------------------------- softmax
+    const int tile = warp / 4, r = row0 + tile * kRows + (warp % 4) * 32 + lane;
+    if (tile < tiles) {
+      const uint32_t lanes = (uint32_t)(warp % 4) << 21;  // this warp's lanes of tensor memory (bits 16-31)
+      const uint32_t ts = tmem + lanes + tile * 128, tp = tmem + lanes + C::kP + tile * C::kPStep,
+                     to = tmem + lanes + C::kO + tile * D;
+      const int lim = row_limit(p, r, pos, cnt);
+      const float back = p.q_back[head * p.row_tiles * kRows + r];
+      const float* ksc = p.c.k_scale + head * (p.c.max_len / kKv8Block);
+      const float* vsc = p.c.v_scale + head * (p.c.max_len / kKv8Block);
+      const int vis = last / kKv8Block;  // the last block any row sees
+      float m = -INFINITY, l = 0.0f;
+      const int e_ref = n > 0 ? kv8_exponent(vsc[2 * beg]) : 0;
+      float ks[2], vs[2];
+      auto scales = [&](int j) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int blk = min(2 * (beg + j) + h, vis);
+          ks[h] = __ldg(ksc + blk);
+          vs[h] = __ldg(vsc + blk);
+        }
+      };
+      if (n > 0) scales(0);
+      for (int j = 0; j < n; ++j) {
+        const int key0 = (beg + j) * kKeys;
+        const float a[2] = {back * ks[0], back * ks[1]};
+        const int ev[2] = {kv8_exponent(vs[0]), kv8_exponent(vs[1])};
+        if (j + 1 < n) scales(j + 1);
+        if (!wait(s_full + 8 * tile, j)) break;
+        fence_after();
+        const bool whole = __all_sync(0xffffffffu, lim >= key0 + kKeys - 1);
+        float top[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float t = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float s[32];
+            tmem_ld32(ts + h * 64 + q * 32, s);
+            tmem_ld_wait();
+            if (whole) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) t = fmaxf(t, s[i]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (key0 + h * 64 + q * 32 + i <= lim) t = fmaxf(t, s[i]);
+            }
+          }
+          top[h] = t > -INFINITY ? fmaf(t, a[h], (float)ev[h]) : -INFINITY;
+        }
+        const float now = fmaxf(fmaxf(m, top[0]), top[1]);
+        const bool grow = now > m + kLazy || (m == -INFINITY && now > m);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = !grow ? 1.0f : m == -INFINITY ? 0.0f : exp2a(m - now);
+          if (grow) m = now;
+          l *= alpha;
+          if (j > 0) {
+            // s_full(j) was committed after the product with tile j - 1's P: O is at rest
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              float o[32];
+              tmem_ld32(to + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] *= alpha;
+              tmem_st32(to + c, o);
+            }
+          }
+        }
+        const float sub = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float add = (float)ev[h] - sub;
+          float sum = 0.0f;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float s[32];
+            tmem_ld32(ts + h * 64 + q * 32, s);
+            tmem_ld_wait();
+            if (whole) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[i] = exp2a(fmaf(s[i], a[h], add));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                s[i] = key0 + h * 64 + q * 32 + i <= lim ? exp2a(fmaf(s[i], a[h], add)) : 0.0f;
+            }
+            uint32_t ph[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              sum += s[2 * i] + s[2 * i + 1];
+              ph[i] = h2_bits(__floats2half2_rn(s[2 * i], s[2 * i + 1]));
+            }
+            tmem_st16(tp + (h * 2 + q) * 16, ph);
+          }
+          l = fmaf(sum, kv8_pow2(min(max(e_ref - ev[h], -100), 100)), l);
+        }
+        tmem_st_wait();
+        fence_before();
+        mbar_arrive(p_full + 8 * tile);
+      }
+      // results: O, m' and l (against e_ref)
+      // (over S it is committed for every key tile; all but the last are known done)
+      if (n > 0) wait(o_full + 8 * tile, C::kOver ? n - 1 : 0);
+      fence_after();
+      const float lsum = l * kv8_pow2(-e_ref);
+      const int t = r / p.G, hq = (int)(head % p.c.n_kv_heads) * p.G + r % p.G;
+      const int64_t orow = ((int64_t)b * p.T + t) * (p.G * p.c.n_kv_heads) + hq;
+      const int64_t at = (head * p.rows + r) * p.splits + split;
+      const float inv = m > -INFINITY ? 1.0f / lsum : 0.0f;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        if (n > 0) {
+          tmem_ld32(to + c, o);
+          tmem_ld_wait();
+        }
+        if (r >= p.rows || !ok) continue;
+        if (m == -INFINITY)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+        if (p.splits > 1) {
+          float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + orow * D + c);
+          uint32_t u[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float y0 = o[2 * i] * inv, y1 = o[2 * i + 1] * inv;
+            u[i] = p.dtype == CB_BF16 ? (uint32_t)f32_to_bf16(y0) | (uint32_t)f32_to_bf16(y1) << 16
+                                      : h2_bits(__floats2half2_rn(y0, y1));
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dst[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+        }
+      }
+      if (r < p.rows && ok) {
+        if (p.splits > 1) {
+          p.part_ml[2 * at] = m;
+          p.part_ml[2 * at + 1] = lsum;
+        } else {
+          p.lse[orow] = m > -INFINITY ? (m + log2f(lsum)) * kLn2 : -INFINITY;
+        }
+      }
+    }
+  } else if (warp < kSoftWarps + kConvThreads / 32) {
+    // ------------------------------------------------- codes to operands
+    const int d = tid - kSoftWarps * 32;
+    const uint8_t* src[2] = {p.c.k + head * p.c.max_len * D, p.c.v + head * p.c.max_len * D};
+    uint4 raw[2][C::kPieces];
+    // piece i: 16 bytes of one key, 8 consecutive keys to 8 consecutive threads
+    auto key_of = [&](int i) { return (d & 7) + 8 * ((i * kConvThreads + d) / (8 * C::kPieces)); };
+    auto chunk_of = [&](int i) { return (i * kConvThreads + d) / 8 % C::kPieces; };
+    auto load = [&](int kv, int j) {
+#pragma unroll
+      for (int i = 0; i < C::kPieces; ++i) {
+        const int key = (beg + j) * kKeys + key_of(i);
+        // slots no row sees may hold anything, an E4M3 NaN too: they read as 0
+        raw[kv][i] = j < n && key <= last
+                         ? __ldg(reinterpret_cast<const uint4*>(src[kv] + (int64_t)key * D) + chunk_of(i))
+                         : make_uint4(0u, 0u, 0u, 0u);
+      }
+    };
+    load(0, 0);
+    load(1, 0);
+    for (int j = 0; j < n; ++j) {
+      const int st = j & 1;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        if (j >= kStages && !wait((kv ? v_free : k_free) + 8 * st, (j - kStages) / kStages)) break;
+        uint8_t* dst = (kv ? sv : sk) + st * C::kKV;
+#pragma unroll
+        for (int i = 0; i < C::kPieces; ++i) {
+          const int key = key_of(i), c = chunk_of(i);
+          uint4 lo, hi;
+          codes_to_h2<FMT>(raw[kv][i].x, lo.x, lo.y);
+          codes_to_h2<FMT>(raw[kv][i].y, lo.z, lo.w);
+          codes_to_h2<FMT>(raw[kv][i].z, hi.x, hi.y);
+          codes_to_h2<FMT>(raw[kv][i].w, hi.z, hi.w);
+          if (kv == 0) {
+            *reinterpret_cast<uint4*>(dst + kmajor<D>(key, 2 * c)) = lo;
+            *reinterpret_cast<uint4*>(dst + kmajor<D>(key, 2 * c + 1)) = hi;
+          } else {  // MN-major: 16-byte pieces of 8 dims, one after another over the keys
+            *reinterpret_cast<uint4*>(dst + (2 * c) * (kKeys * 16) + key * 16) = lo;
+            *reinterpret_cast<uint4*>(dst + (2 * c + 1) * (kKeys * 16) + key * 16) = hi;
+          }
+        }
+        load(kv, j + 1);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive((kv ? v_full : k_full) + 8 * st);
+      }
+      if (!ok) break;
+    }
+  } else if (lane == 0 && n > 0) {
+    // ---------------------------------------------------------- products
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(q_full), "r"(tiles * C::kQ) : "memory");
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(sq)),
+        "l"(p.q16 + (head * p.row_tiles + pair * kTiles) * (int64_t)C::kQ), "r"(tiles * C::kQ), "r"(q_full)
+        : "memory");
+    constexpr uint32_t kIdS = idesc(kRows, kKeys, false), kIdO = idesc(kRows, D, true);
+    auto qk = [&](int t, int st) {
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+        mma_ss(tmem + t * 128, mat_desc(smem_u32(sq) + t * C::kQ + s * 256, 128, D / 8 * 128),
+               mat_desc(smem_u32(sk) + st * C::kKV + s * 256, 128, D / 8 * 128), kIdS, s > 0);
+      commit(s_full + 8 * t);
+    };
+    wait(q_full, 0);
+    wait(k_full, 0);
+    if (ok) {
+      for (int t = 0; t < tiles; ++t) qk(t, 0);
+      commit(k_free);
+    }
+    for (int j = 0; j < n && ok; ++j) {
+      const int st = j & 1, next = (j + 1) & 1;
+      for (int t = 0; t < tiles; ++t) {
+        if (!wait(p_full + 8 * t, j) || (t == 0 && !wait(v_full + 8 * st, j / 2))) break;
+        fence_after();
+#pragma unroll
+        for (int s = 0; s < kKeys / 16; ++s)
+          mma_ts(tmem + C::kO + t * D, tmem + C::kP + t * C::kPStep + s * 8,
+                 mat_desc(smem_u32(sv) + st * C::kKV + s * 256, 128, kKeys * 16), kIdO, j > 0 || s > 0);
+        if (C::kOver || j + 1 == n) commit(o_full + 8 * t);
+        if (t + 1 == tiles) commit(v_free + 8 * st);
+        if (j + 1 < n) {
+          if (t == 0 && !wait(k_full + 8 * next, (j + 1) / 2)) break;
+          // P lies over S: the product that reads it ends before S is written again
+          if (C::kOver && !wait(o_full + 8 * t, j)) break;
+          qk(t, next);
+          if (t + 1 == tiles) commit(k_free + 8 * next);
+        }
+      }
+    }
+    if (!ok) {  // let the copy and the products in flight end before their memory goes
+      mbar_wait(q_full, 0);
+      commit(end);
+      mbar_wait(end, 0);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (tid == 0 && s_abort) set_status(p.status, CB_ERR_TIMEOUT);
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+template <int D>
+int launch_prompt(const AttendParams& p, int bh, cudaStream_t st) {
+  kv8_query_kernel<D><<<dim3(ceil_div(p.row_tiles * kRows * (D / 8), 256), bh), 256, 0, st>>>(p);
+  count_launch();
+  const dim3 grid(ceil_div(p.row_tiles, kTiles) * p.splits, bh);
+  auto fn = p.c.format == CB_KV8_E4M3 ? kv8_prompt_kernel<D, CB_KV8_E4M3> : kv8_prompt_kernel<D, CB_KV8_INT8>;
+  if (const int rc = ensure_smem_attr((const void*)fn, Prompt<D>::kSmem)) return rc;
+  fn<<<grid, kThreads, Prompt<D>::kSmem, st>>>(p);
+  count_launch();
+  return cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
+}
+
+}  // namespace
+
+int kv8_prompt_launch(const AttendParams& p, int bh, cudaStream_t st) {
+  return p.c.head_dim == 64 ? launch_prompt<64>(p, bh, st) : launch_prompt<128>(p, bh, st);
+}
+
+}  // namespace cb

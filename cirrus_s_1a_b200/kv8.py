@@ -111,7 +111,7 @@ class Kv8Cache:
         return of(self.k, self.k_scale), of(self.v, self.v_scale)
 
     def read_status(self) -> int:
-        """The device status (0, or 5 when an append passed ``max_len``); synchronises."""
+        """The device status (0; 5 when an append passed ``max_len``; 8 when a wait gave up); synchronises."""
         return int(self.status.item())
 
     def clear_status(self) -> None:
@@ -187,10 +187,10 @@ class Kv8Cache:
             raise ValueError("out must be contiguous, of q's shape, type and device")
         lse = torch.empty(self.batch, T, heads, dtype=torch.float32, device=self.device)
         st = self._stream()
-        key = (st, heads, T, longest)
+        key = (st, dtype, heads, T, longest)
         scratch = self._scratch.get(key)
         if scratch is None:
-            nbytes = self._lib.cb_kv8_attend_scratch_bytes(self._ref, heads, T, longest)
+            nbytes = self._lib.cb_kv8_attend_scratch_bytes(self._ref, dtype, heads, T, longest)
             if nbytes == 0:
                 raise _lib.CbError("cb_kv8_attend_scratch_bytes: shape not supported")
             scratch = self._grow(st, nbytes)
@@ -198,7 +198,7 @@ class Kv8Cache:
         self._call(self._lib.cb_kv8_attend, "cb_kv8_attend", self._ref, q.data_ptr(), dtype, qs, heads, T,
                    self._ints(pos, "pos"), self._ints(counts, "counts"), longest,
                    self.head_dim ** -0.5 if scale is None else float(scale), int(add_mass), out.data_ptr(),
-                   lse.data_ptr(), scratch.data_ptr(), scratch.numel(), st)
+                   lse.data_ptr(), scratch.data_ptr(), scratch.numel(), self.status.data_ptr(), st)
         return out, lse
 
     def _grow(self, stream: int, nbytes: int) -> torch.Tensor:

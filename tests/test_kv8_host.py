@@ -36,12 +36,14 @@ def test_entry_points_refuse_bad_arguments_without_launching(built_lib):  # noqa
     assert app(desc(), T=129) == 1  # more tokens than slots
     big = 1 << 40
     att = lambda c, hq=2, T=1, longest=128, mass=0, scratch=256, n=big, dtype=1: L.cb_kv8_attend(  # noqa: E731
-        c, 256, dtype, s3, hq, T, 256, None, longest, 1.0, mass, 256, 256, scratch, n, None)
+        c, 256, dtype, s3, hq, T, 256, None, longest, 1.0, mass, 256, 256, scratch, n, None, None)
     assert att(None) == 1 and att(desc(), hq=3) == 2 and att(desc(), T=0) == 1 and att(desc(), longest=0) == 1
     assert att(desc(), scratch=None) == 1 and att(desc(), n=0) == 4 and att(desc(mass=None), mass=1) == 1
     assert att(desc(), dtype=7) == 1 and att(desc(head_dim=100)) == 2
-    assert L.cb_kv8_attend_scratch_bytes(desc(), 2, 1, 128) > 0
-    assert L.cb_kv8_attend_scratch_bytes(desc(), 3, 1, 128) == 0 and L.cb_kv8_attend_scratch_bytes(None, 2, 1, 1) == 0
+    assert att(desc(), scratch=264) == 1
+    need = L.cb_kv8_attend_scratch_bytes
+    assert need(desc(), 1, 2, 1, 128) > 0 and need(desc(), 1, 2, 100, 128) > need(desc(), 0, 2, 1, 128)
+    assert need(desc(), 1, 3, 1, 128) == 0 and need(None, 1, 2, 1, 1) == 0 and need(desc(), 5, 2, 1, 1) == 0
     ev = lambda c, keep=4, recent=2, pos=256, new=512: L.cb_kv8_evict(c, pos, keep, recent, 256, new, None)  # noqa: E731
     assert ev(None) == 1 and ev(desc(mass=None)) == 1 and ev(desc(), keep=0) == 1 and ev(desc(), recent=5) == 1
     assert ev(desc(), keep=129, recent=0) == 1 and ev(desc(), new=256) == 1 and ev(desc(), recent=-1) == 1
