@@ -1,4 +1,4 @@
-// Device helpers of the 8-bit K/V cache (kv8_cache.cu, kv8_attend.cu, kv8_evict.cu).
+// Device helpers of the 8-bit K/V cache (kv8_*.cu) and of the log probabilities.
 //
 // The cache holds codes in 8 bits, [batch][kv head][slot][dim], and one scale
 // for each block of kKv8Block slots and head.  A scale is a power of two, the
@@ -51,6 +51,41 @@ template <int FMT>
 __device__ __forceinline__ float kv8_decode(uint32_t b) {
   if (FMT == CB_KV8_E4M3) return e4m3_to_f32(b & 0xFF);
   return (float)(int8_t)(b & 0xFF);
+}
+
+// 2^x to about 2^-22; 0 below 2^-126.
+__device__ __forceinline__ float exp2a(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Pairs of floats on the packed float32 units.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }

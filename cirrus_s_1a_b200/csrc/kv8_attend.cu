@@ -44,12 +44,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ float exp2a(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // N bytes (2, 4, 8, 16 or 32, aligned to min(N, 16)) as words.
 template <int N>
 __device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t (&w)[(N + 3) / 4]) {
@@ -413,7 +407,7 @@ Plan plan_of(const CbKv8& c, int dtype, int n_q_heads, int T, int longest) {
     pl.row_tiles = ceil_div(pl.rows, 128);
     // runs of key tiles that leave the fewest tile times (and three more a CTA to
     // start and end) on the busiest SM
-    const int items = bh * ceil_div(pl.row_tiles, 2), tiles = ceil_div(longest, 128);
+    const int items = bh * ceil_div(pl.row_tiles, 2), tiles = ceil_div(longest, 8192 / c.head_dim);
     long best = 0;
     for (int s = 1; s <= 32 && s <= ceil_div(tiles, 2); ++s) {
       const long cost = (long)ceil_div(items * s, 148) * (ceil_div(tiles, s) + 3);

@@ -3,11 +3,11 @@
 // 16-bit queries.
 //
 // kv8_query_kernel prepares the query rows once: each scaled by a power of two
-// (largest element in [256, 512)), rounded to f16 and written as 128-row operand
-// tiles (8-row x 16-byte core matrices), with the factor that undoes the scaling.
+// (largest element in [256, 512)), rounded to f16 and written as swizzled 128-row
+// operand tiles, with the factor that undoes the scaling.
 //
 // kv8_prompt_kernel: a CTA owns 256 query rows of one KV head (two tiles of 128)
-// and a run of 128-key tiles.
+// and a run of key tiles (128 keys for 64 dims, 64 for 128).
 //   * 4 warps turn codes into f16 operands in shared memory (two stages each of K
 //     and V): plain conversions, exact; no scale is applied there.
 //   * one thread issues tcgen05.mma kind::f16: S = Q K^T into tensor memory, and
@@ -21,8 +21,10 @@
 //     of tiny values nor one of huge ones costs the others precision: P's f16
 //     rounding is relative to what the row adds up.  The row's sum is
 //     l = sum_b 2^-e_b sum P (before P is rounded), the same in float32.
-//   * O is rescaled in tensor memory only when m' has grown by more than 2^8
-//     (P stays below 2^8, the result is exact either way).
+//   * P is taken against the maximum so far, in the same pass over S that finds the
+//     tile's own.  Only where a row's has grown by more than 2^15 is the tile's P
+//     taken again, and O rescaled in tensor memory (f16 P stays below 2^15; the result
+//     is the same either way).
 // While one tile is in its softmax the tensor cores work for the other.  The two
 // tiles' exponentials bound it for head_dim 64: 128 x 128 per tile at 16 a clock
 // take 1024 clocks, its products 512.
@@ -38,13 +40,12 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kRows = 128;                 // of a tile (MMA M)
-constexpr int kKeys = 128;                 // of a key tile
 constexpr int kTiles = 2;                  // row tiles of a CTA
 constexpr int kStages = 2;
 constexpr int kSoftWarps = 4 * kTiles;
 constexpr int kConvThreads = 128;
 constexpr int kThreads = kSoftWarps * 32 + kConvThreads + 32;
-constexpr float kLazy = 8.0f;              // growth of the maximum, in powers of two, that O follows
+constexpr float kLazy = 15.0f;             // growth of the maximum, in powers of two, that O follows: f16 P ends at 2^16
 constexpr unsigned long long kTimeoutNs = 200ull * 1000 * 1000;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -84,12 +85,27 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Shared-memory matrix descriptor without swizzle, version 1 (bits 46-47).
-// K-major: lbo between K-adjacent core matrices, sbo between 8-row groups.
-// MN-major: lbo between 8-row groups of K, sbo between 16-byte pieces of MN.
-__device__ __forceinline__ uint64_t mat_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 |
-         (uint64_t)((sbo >> 4) & 0x3FFF) << 32 | (uint64_t)1 << 46;
+// Operand tiles lie in rows of 128 bytes (64 elements), 16-byte piece c of row r at
+// piece c ^ (r % 8), the 128-byte swizzle; elements 64 on start a second block of rows.
+// Offset of 8-element piece kb of a row, in a tile of ROWS rows.
+template <int ROWS>
+__device__ __forceinline__ uint32_t swizzled(int row, int kb) {
+  return (uint32_t)((kb >> 3) * ROWS * 128 + row * 128 + (((kb & 7) ^ (row & 7)) << 4));
+}
+
+// One thread of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle (2 at bits 61-63), version 1
+// (bits 46-47), 8-row groups 1024 bytes apart.  lbo, for an operand whose rows run
+// along K (MN-major): between its blocks of 64 elements.
+__device__ __forceinline__ uint64_t mat_desc(uint32_t saddr, uint32_t lbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
 // Instruction descriptor, kind::f16: D f32, A and B f16; bit 16: B is MN-major.
@@ -114,7 +130,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 }
 
 // 32 columns of the warp's 32 lanes of tensor memory, and back.
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
   uint32_t* u = reinterpret_cast<uint32_t*>(v);
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -128,7 +144,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const float* v) {
   const uint32_t* u = reinterpret_cast<const uint32_t*>(v);
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -149,18 +165,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&u)[16]
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ float exp2a(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Offset of (row, 8-element piece kb) in a K-major operand tile of D dims.
-template <int D>
-__device__ __forceinline__ uint32_t kmajor(int row, int kb) {
-  return (uint32_t)((row >> 3) * (D / 8) * 128 + kb * 128 + (row & 7) * 16);
-}
 
 // The last slot row r of a KV head sees (rows of padding tokens: -1).
 __device__ __forceinline__ int row_limit(const AttendParams& p, int r, int pos, int cnt) {
@@ -197,27 +201,31 @@ __global__ void __launch_bounds__(256) kv8_query_kernel(const __grid_constant__ 
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = h2_bits(__floats2half2_rn(x[2 * i] * f, x[2 * i + 1] * f));
   uint8_t* tile = p.q16 + (head * p.row_tiles + r / kRows) * (int64_t)(kRows * D * 2);
-  *reinterpret_cast<uint4*>(tile + kmajor<D>(r % kRows, kb)) = make_uint4(h[0], h[1], h[2], h[3]);
+  *reinterpret_cast<uint4*>(tile + swizzled<kRows>(r % kRows, kb)) = make_uint4(h[0], h[1], h[2], h[3]);
   if (kb == 0) p.q_back[head * p.row_tiles * kRows + r] = live ? kv8_pow2(e - 8) * fabsf(p.scale) * kLog2e : 0.0f;
 }
 
 // --------------------------------------------------------------- attention
 template <int D>
 struct Prompt {
+  static constexpr int kKeys = 8192 / D;        // of a key tile: S, P and O of two tiles fill tensor memory
+  static constexpr int kHalves = kKeys / kKv8Block;
   static constexpr int kQ = kRows * D * 2;      // bytes of a query tile
   static constexpr int kKV = kKeys * D * 2;     // of a K or V tile
-  static constexpr int kSmem = kTiles * kQ + 2 * kStages * kKV;
-  // tensor memory: S of both tiles, then P where there is room (else over S), then O
-  static constexpr bool kOver = D == 128;
-  static constexpr int kP = kOver ? 0 : 256, kPStep = kOver ? 128 : 64;
-  static constexpr int kO = kOver ? 256 : 384;
-  static constexpr int kPieces = D / 16;        // 16-byte pieces of a K or V tile per converting thread
+  static constexpr int kSmem = kTiles * kQ + 2 * kStages * kKV + 1024;
+  // tensor memory: S, P (f16, half as many columns) and O of both tiles
+  static constexpr int kP = kTiles * kKeys, kO = 512 - kTiles * D;
+  static_assert(kP + kTiles * kKeys / 2 <= kO, "S, P and O fit 512 columns");
+  static constexpr int kPieces = kKeys * D / 16 / kConvThreads;  // 16-byte pieces of a tile per converting thread
+  static constexpr int kRow = D / 16;                            // of a key
 };
 
 template <int D, int FMT>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_constant__ AttendParams p) {
   using C = Prompt<D>;
-  extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr int kKeys = C::kKeys, kHalves = C::kHalves;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);  // the swizzle counts from 1024-byte boundaries
   __shared__ __align__(8) unsigned long long bars[16];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
@@ -261,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = 0;  // all 512 columns are this CTA's: they start at 0
   bool ok = true;
   auto wait = [&](uint32_t bar, int phase) {
     if (ok && !mbar_wait(bar, phase & 1)) {
@@ -276,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     const int tile = warp / 4, r = row0 + tile * kRows + (warp % 4) * 32 + lane;
     if (tile < tiles) {
       const uint32_t lanes = (uint32_t)(warp % 4) << 21;  // this warp's lanes of tensor memory (bits 16-31)
-      const uint32_t ts = tmem + lanes + tile * 128, tp = tmem + lanes + C::kP + tile * C::kPStep,
+      const uint32_t ts = tmem + lanes + tile * kKeys, tp = tmem + lanes + C::kP + tile * (kKeys / 2),
                      to = tmem + lanes + C::kO + tile * D;
       const int lim = row_limit(p, r, pos, cnt);
       const float back = p.q_back[head * p.row_tiles * kRows + r];
@@ -284,12 +292,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       const float* vsc = p.c.v_scale + head * (p.c.max_len / kKv8Block);
       const int vis = last / kKv8Block;  // the last block any row sees
       float m = -INFINITY, l = 0.0f;
-      const int e_ref = n > 0 ? kv8_exponent(vsc[2 * beg]) : 0;
-      float ks[2], vs[2];
+      const int e_ref = n > 0 ? kv8_exponent(vsc[kHalves * beg]) : 0;
+      float ks[kHalves], vs[kHalves];
       auto scales = [&](int j) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int blk = min(2 * (beg + j) + h, vis);
+        for (int h = 0; h < kHalves; ++h) {
+          const int blk = min(kHalves * (beg + j) + h, vis);
           ks[h] = __ldg(ksc + blk);
           vs[h] = __ldg(vsc + blk);
         }
@@ -297,86 +305,117 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       if (n > 0) scales(0);
       for (int j = 0; j < n; ++j) {
         const int key0 = (beg + j) * kKeys;
-        const float a[2] = {back * ks[0], back * ks[1]};
-        const int ev[2] = {kv8_exponent(vs[0]), kv8_exponent(vs[1])};
+        float a[kHalves];
+        int ev[kHalves];
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          a[h] = fmaxf(back * ks[h], 1.2e-38f);  // above 0: a masked score times it stays -infinity
+          ev[h] = kv8_exponent(vs[h]);
+        }
         if (j + 1 < n) scales(j + 1);
         if (!wait(s_full + 8 * tile, j)) break;
         fence_after();
         const bool whole = __all_sync(0xffffffffu, lim >= key0 + kKeys - 1);
-        float top[2];
+        // 32 scores at a time, the next ones on their way
+        float s[2][32];
+        auto fetch = [&](int q) { tmem_ld32(ts + q * 32, s[q & 1]); };
+        auto mask = [&](int q) {
+          if (whole) return;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float t = -INFINITY;
+          for (int i = 0; i < 32; ++i)
+            if (key0 + q * 32 + i > lim) s[q & 1][i] = -INFINITY;
+        };
+        auto max_of = [&](int q) {
+          const float* v = s[q & 1];
+          float t[4];
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            float s[32];
-            tmem_ld32(ts + h * 64 + q * 32, s);
+          for (int k = 0; k < 4; ++k) t[k] = v[k];
+#pragma unroll
+          for (int i = 4; i < 28; i += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], v[i + k]), v[i + 4 + k]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], v[28 + k]);
+          return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        };
+        // the largest x + e of the tile
+        auto top_of = [&](const float (&t)[kHalves]) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h)
+            if (t[h] > -INFINITY) top = fmaxf(top, fmaf(t[h], a[h], (float)ev[h]));
+          return top;
+        };
+        if (__any_sync(0xffffffffu, m == -INFINITY)) {  // rows without a maximum yet: take the tile's
+          float t[kHalves];
+          fetch(0);
+#pragma unroll
+          for (int q = 0; q < kKeys / 32; ++q) {
             tmem_ld_wait();
-            if (whole) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) t = fmaxf(t, s[i]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (key0 + h * 64 + q * 32 + i <= lim) t = fmaxf(t, s[i]);
-            }
+            if (q + 1 < kKeys / 32) fetch(q + 1);
+            mask(q);
+            const float x = max_of(q);
+            t[q / 2] = q & 1 ? fmaxf(t[q / 2], x) : x;
           }
-          top[h] = t > -INFINITY ? fmaf(t, a[h], (float)ev[h]) : -INFINITY;
+          if (m == -INFINITY) m = top_of(t);
         }
-        const float now = fmaxf(fmaxf(m, top[0]), top[1]);
-        const bool grow = now > m + kLazy || (m == -INFINITY && now > m);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float alpha = !grow ? 1.0f : m == -INFINITY ? 0.0f : exp2a(m - now);
+        // P against the maximum so far; again where the tile raised it too far
+        float sum_l = 0.0f;
+        for (int turn = 0;; ++turn) {
+          const float sub = m == -INFINITY ? 0.0f : m;
+          float t[kHalves];
+          sum_l = 0.0f;
+          fetch(0);
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h) {
+            const f32x2 a2 = pack2(a[h], a[h]), c2 = pack2((float)ev[h] - sub, (float)ev[h] - sub);
+            f32x2 sum[2] = {0, 0};  // pairs of zeros
+#pragma unroll
+            for (int q = 2 * h; q < 2 * h + 2; ++q) {
+              tmem_ld_wait();
+              if (q + 1 < kKeys / 32) fetch(q + 1);
+              mask(q);
+              const float x = max_of(q);
+              t[h] = q & 1 ? fmaxf(t[h], x) : x;
+              uint32_t ph[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 d = unpack2(fma2(pack2(s[q & 1][2 * i], s[q & 1][2 * i + 1]), a2, c2));
+                const float y0 = exp2a(d.x), y1 = exp2a(d.y);
+                sum[i & 1] = add2(sum[i & 1], pack2(y0, y1));
+                ph[i] = h2_bits(__floats2half2_rn(y0, y1));
+              }
+              tmem_st16(tp + q * 16, ph);
+            }
+            const float2 both = unpack2(add2(sum[0], sum[1]));
+            sum_l = fmaf(both.x + both.y, kv8_pow2(min(max(e_ref - ev[h], -100), 100)), sum_l);
+          }
+          const float now = top_of(t);
+          const bool grow = now > m + kLazy;
+          if (turn > 0 || !__any_sync(0xffffffffu, grow)) break;
+          const float alpha = grow ? exp2a(m - now) : 1.0f;
           if (grow) m = now;
           l *= alpha;
           if (j > 0) {
             // s_full(j) was committed after the product with tile j - 1's P: O is at rest
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
-              float o[32];
-              tmem_ld32(to + c, o);
+              tmem_ld32(to + c, s[0]);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] *= alpha;
-              tmem_st32(to + c, o);
+              for (int i = 0; i < 32; ++i) s[0][i] *= alpha;
+              tmem_st32(to + c, s[0]);
             }
           }
+          tmem_st_wait();  // P is written once more
         }
-        const float sub = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float add = (float)ev[h] - sub;
-          float sum = 0.0f;
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            float s[32];
-            tmem_ld32(ts + h * 64 + q * 32, s);
-            tmem_ld_wait();
-            if (whole) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) s[i] = exp2a(fmaf(s[i], a[h], add));
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                s[i] = key0 + h * 64 + q * 32 + i <= lim ? exp2a(fmaf(s[i], a[h], add)) : 0.0f;
-            }
-            uint32_t ph[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              sum += s[2 * i] + s[2 * i + 1];
-              ph[i] = h2_bits(__floats2half2_rn(s[2 * i], s[2 * i + 1]));
-            }
-            tmem_st16(tp + (h * 2 + q) * 16, ph);
-          }
-          l = fmaf(sum, kv8_pow2(min(max(e_ref - ev[h], -100), 100)), l);
-        }
+        l += sum_l;
         tmem_st_wait();
         fence_before();
         mbar_arrive(p_full + 8 * tile);
       }
       // results: O, m' and l (against e_ref)
-      // (over S it is committed for every key tile; all but the last are known done)
-      if (n > 0) wait(o_full + 8 * tile, C::kOver ? n - 1 : 0);
+      if (n > 0) wait(o_full + 8 * tile, 0);
       fence_after();
       const float lsum = l * kv8_pow2(-e_ref);
       const int t = r / p.G, hq = (int)(head % p.c.n_kv_heads) * p.G + r % p.G;
@@ -426,8 +465,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     const uint8_t* src[2] = {p.c.k + head * p.c.max_len * D, p.c.v + head * p.c.max_len * D};
     uint4 raw[2][C::kPieces];
     // piece i: 16 bytes of one key, 8 consecutive keys to 8 consecutive threads
-    auto key_of = [&](int i) { return (d & 7) + 8 * ((i * kConvThreads + d) / (8 * C::kPieces)); };
-    auto chunk_of = [&](int i) { return (i * kConvThreads + d) / 8 % C::kPieces; };
+    auto key_of = [&](int i) { return (d & 7) + 8 * ((i * kConvThreads + d) / (8 * C::kRow)); };
+    auto chunk_of = [&](int i) { return (i * kConvThreads + d) / 8 % C::kRow; };
     auto load = [&](int kv, int j) {
 #pragma unroll
       for (int i = 0; i < C::kPieces; ++i) {
@@ -454,13 +493,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           codes_to_h2<FMT>(raw[kv][i].y, lo.z, lo.w);
           codes_to_h2<FMT>(raw[kv][i].z, hi.x, hi.y);
           codes_to_h2<FMT>(raw[kv][i].w, hi.z, hi.w);
-          if (kv == 0) {
-            *reinterpret_cast<uint4*>(dst + kmajor<D>(key, 2 * c)) = lo;
-            *reinterpret_cast<uint4*>(dst + kmajor<D>(key, 2 * c + 1)) = hi;
-          } else {  // MN-major: 16-byte pieces of 8 dims, one after another over the keys
-            *reinterpret_cast<uint4*>(dst + (2 * c) * (kKeys * 16) + key * 16) = lo;
-            *reinterpret_cast<uint4*>(dst + (2 * c + 1) * (kKeys * 16) + key * 16) = hi;
-          }
+          *reinterpret_cast<uint4*>(dst + swizzled<kKeys>(key, 2 * c)) = lo;
+          *reinterpret_cast<uint4*>(dst + swizzled<kKeys>(key, 2 * c + 1)) = hi;
         }
         load(kv, j + 1);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -468,50 +502,62 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       }
       if (!ok) break;
     }
-  } else if (lane == 0 && n > 0) {
+  } else if (n > 0) {
     // ---------------------------------------------------------- products
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(q_full), "r"(tiles * C::kQ) : "memory");
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(sq)),
-        "l"(p.q16 + (head * p.row_tiles + pair * kTiles) * (int64_t)C::kQ), "r"(tiles * C::kQ), "r"(q_full)
-        : "memory");
-    constexpr uint32_t kIdS = idesc(kRows, kKeys, false), kIdO = idesc(kRows, D, true);
-    auto qk = [&](int t, int st) {
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s)
-        mma_ss(tmem + t * 128, mat_desc(smem_u32(sq) + t * C::kQ + s * 256, 128, D / 8 * 128),
-               mat_desc(smem_u32(sk) + st * C::kKV + s * 256, 128, D / 8 * 128), kIdS, s > 0);
-      commit(s_full + 8 * t);
-    };
-    wait(q_full, 0);
-    wait(k_full, 0);
-    if (ok) {
-      for (int t = 0; t < tiles; ++t) qk(t, 0);
-      commit(k_free);
+    // The whole warp walks the loop, so that addresses and descriptors stay in
+    // uniform registers; one elected thread issues.  (A branch of one thread moved
+    // them there for every instruction: 90 to 140 clocks each instead of 32 or 64.)
+    const bool lead = elect_one();
+    const uint32_t q_at = smem_u32(sq), k_at = smem_u32(sk), v_at = smem_u32(sv);
+    if (lead) {
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(q_full), "r"(tiles * C::kQ) : "memory");
+      asm volatile(
+          "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(q_at),
+          "l"(p.q16 + (head * p.row_tiles + pair * kTiles) * (int64_t)C::kQ), "r"(tiles * C::kQ), "r"(q_full)
+          : "memory");
     }
-    for (int j = 0; j < n && ok; ++j) {
-      const int st = j & 1, next = (j + 1) & 1;
-      for (int t = 0; t < tiles; ++t) {
-        if (!wait(p_full + 8 * t, j) || (t == 0 && !wait(v_full + 8 * st, j / 2))) break;
-        fence_after();
+    constexpr uint32_t kIdS = idesc(kRows, kKeys, false), kIdO = idesc(kRows, D, true);
+    auto all_wait = [&](uint32_t bar, int phase) { return __all_sync(0xffffffffu, wait(bar, phase)); };
+    auto qk = [&](int t, int st) {
+      const uint64_t qd = mat_desc(q_at + t * C::kQ, 16), kd = mat_desc(k_at + st * C::kKV, 16);
+      if (lead) {
 #pragma unroll
-        for (int s = 0; s < kKeys / 16; ++s)
-          mma_ts(tmem + C::kO + t * D, tmem + C::kP + t * C::kPStep + s * 8,
-                 mat_desc(smem_u32(sv) + st * C::kKV + s * 256, 128, kKeys * 16), kIdO, j > 0 || s > 0);
-        if (C::kOver || j + 1 == n) commit(o_full + 8 * t);
-        if (t + 1 == tiles) commit(v_free + 8 * st);
+        for (int s = 0; s < D / 16; ++s)
+          mma_ss(t * kKeys, qd + (s / 4 * (kRows * 128) + s % 4 * 32) / 16, kd + (s / 4 * (kKeys * 128) + s % 4 * 32) / 16,
+                 kIdS, s > 0);
+        commit(s_full + 8 * t);
+      }
+    };
+    bool go = all_wait(q_full, 0) && all_wait(k_full, 0);
+    if (go) {
+      for (int t = 0; t < tiles; ++t) qk(t, 0);
+      if (lead) commit(k_free);
+    }
+    for (int j = 0; j < n && go; ++j) {
+      const int st = j & 1, next = (j + 1) & 1;
+      for (int t = 0; t < tiles && go; ++t) {
+        go = all_wait(p_full + 8 * t, j) && (t > 0 || all_wait(v_full + 8 * st, j / 2));
+        if (!go) break;
+        fence_after();
+        const uint64_t vd = mat_desc(v_at + st * C::kKV, kKeys * 128);
+        if (lead) {
+#pragma unroll
+          for (int s = 0; s < kKeys / 16; ++s)
+            mma_ts(C::kO + t * D, C::kP + t * (kKeys / 2) + s * 8, vd + s * 2048 / 16, kIdO, j > 0 || s > 0);
+          if (j + 1 == n) commit(o_full + 8 * t);
+          if (t + 1 == tiles) commit(v_free + 8 * st);
+        }
         if (j + 1 < n) {
-          if (t == 0 && !wait(k_full + 8 * next, (j + 1) / 2)) break;
-          // P lies over S: the product that reads it ends before S is written again
-          if (C::kOver && !wait(o_full + 8 * t, j)) break;
+          if (t == 0) go = all_wait(k_full + 8 * next, (j + 1) / 2);
+          if (!go) break;
           qk(t, next);
-          if (t + 1 == tiles) commit(k_free + 8 * next);
+          if (lead && t + 1 == tiles) commit(k_free + 8 * next);
         }
       }
     }
-    if (!ok) {  // let the copy and the products in flight end before their memory goes
+    if (!go) {  // let the copy and the products in flight end before their memory goes
       mbar_wait(q_full, 0);
-      commit(end);
+      if (lead) commit(end);
       mbar_wait(end, 0);
     }
   }
@@ -519,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   __syncthreads();
   fence_after();
   if (tid == 0 && s_abort) set_status(p.status, CB_ERR_TIMEOUT);
-  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(s_tmem));
 }
 
 template <int D>
