@@ -9,7 +9,7 @@
 // kv8_prompt_kernel: a CTA owns 256 query rows of one KV head (two tiles of 128)
 // and a run of key tiles (128 keys for 64 dims, 64 for 128).
 //   * 4 warps turn codes into f16 operands in shared memory (two stages each of K
-//     and V): plain conversions, exact; no scale is applied there.
+//     and V), exact; no scale is applied there.
 //   * one thread issues tcgen05.mma kind::f16: S = Q K^T into tensor memory, and
 //     O += P V with P read from tensor memory (V's dims are its contiguous
 //     direction, an MN-major operand).
@@ -22,12 +22,13 @@
 //     rounding is relative to what the row adds up.  The row's sum is
 //     l = sum_b 2^-e_b sum P (before P is rounded), the same in float32.
 //   * P is taken against the maximum so far, in the same pass over S that finds the
-//     tile's own.  Only where a row's has grown by more than 2^15 is the tile's P
-//     taken again, and O rescaled in tensor memory (f16 P stays below 2^15; the result
-//     is the same either way).
-// While one tile is in its softmax the tensor cores work for the other.  The two
-// tiles' exponentials bound it for head_dim 64: 128 x 128 per tile at 16 a clock
-// take 1024 clocks, its products 512.
+//     tile's own, 32 scores at a time.  Only where they pass it by more than 2^15
+//     (f16 P ends at 2^16) is it raised, by a power of two, and what was written
+//     against it rescaled in tensor memory.
+// The next tile's scores are taken while the last exponentials of this one run,
+// and its products with V while the next exponentials do, so a warpgroup hardly
+// waits.  The exponentials bound it for head_dim 64: 128 x 128 per tile at 16 a
+// clock take 1024 clocks, its products 512.
 // With several runs per row tile, kv8_join_kernel joins them (kv8_attend.cu).
 // Every wait is bounded (%globaltimer); a wait that gives up sets CB_ERR_TIMEOUT
 // in the status word, and the CTA ends without writing results.
@@ -44,7 +45,11 @@ constexpr int kTiles = 2;                  // row tiles of a CTA
 constexpr int kStages = 2;
 constexpr int kSoftWarps = 4 * kTiles;
 constexpr int kConvThreads = 128;
-constexpr int kThreads = kSoftWarps * 32 + kConvThreads + 32;
+constexpr int kThreads = kSoftWarps * 32 + kConvThreads + 128;
+// Registers a thread of the four warpgroups, out of the 128 at launch: two of
+// softmax, one that converts, one whose first warp issues the products.
+constexpr int kSoftRegs = 184, kConvRegs = 88, kMmaRegs = 56;
+static_assert(2 * kSoftRegs + kConvRegs + kMmaRegs <= 4 * 128, "the shares fit what the block was launched with");
 constexpr float kLazy = 15.0f;             // growth of the maximum, in powers of two, that O follows: f16 P ends at 2^16
 constexpr unsigned long long kTimeoutNs = 200ull * 1000 * 1000;
 
@@ -142,20 +147,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
         "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&u)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(addr));
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const float* v) {
-  const uint32_t* u = reinterpret_cast<const uint32_t*>(v);
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-      "%30,%31,%32};" ::"r"(addr),
-      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
-      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]),
-      "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]),
-      "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&u)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -165,6 +165,40 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&u)[16]
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 16 codes as f16 operand values: int8 as they are, E4M3 divided by 256, which
+// moves its bits without arithmetic (the hardware converter shares its unit with
+// the exponentials).  Pieces that hold a NaN go through the converter.
+template <int FMT>
+__device__ __forceinline__ void to_operand(uint4 c, uint4& lo, uint4& hi) {
+  if (FMT == CB_KV8_INT8) {
+    codes_to_h2<FMT>(c.x, lo.x, lo.y);
+    codes_to_h2<FMT>(c.y, lo.z, lo.w);
+    codes_to_h2<FMT>(c.z, hi.x, hi.y);
+    codes_to_h2<FMT>(c.w, hi.z, hi.w);
+    return;
+  }
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t u[8], nan = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    nan |= (w[i] & 0x7F7F7F7Fu) + 0x01010101u;
+    const uint32_t x = __byte_perm(w[i], 0u, 0x1404), y = __byte_perm(w[i], 0u, 0x3424);
+    u[2 * i] = (x >> 1 & 0x3F803F80u) | (x & 0x80008000u);
+    u[2 * i + 1] = (y >> 1 & 0x3F803F80u) | (y & 0x80008000u);
+  }
+  if (nan & 0x80808080u) {
+    const __half2 f = __float2half2_rn(1.0f / 256.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      codes_to_h2<FMT>(w[i], u[2 * i], u[2 * i + 1]);
+      u[2 * i] = h2_bits(__hmul2(bits_h2(u[2 * i]), f));
+      u[2 * i + 1] = h2_bits(__hmul2(bits_h2(u[2 * i + 1]), f));
+    }
+  }
+  lo = make_uint4(u[0], u[1], u[2], u[3]);
+  hi = make_uint4(u[4], u[5], u[6], u[7]);
+}
 
 // The last slot row r of a KV head sees (rows of padding tokens: -1).
 __device__ __forceinline__ int row_limit(const AttendParams& p, int r, int pos, int cnt) {
@@ -226,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   constexpr int kKeys = C::kKeys, kHalves = C::kHalves;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);  // the swizzle counts from 1024-byte boundaries
-  __shared__ __align__(8) unsigned long long bars[16];
+  __shared__ __align__(8) unsigned long long bars[20];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   uint8_t* sq = smem;
@@ -234,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   uint8_t* sv = sk + kStages * C::kKV;
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t q_full = bar0, k_full = bar0 + 8, k_free = bar0 + 24, v_full = bar0 + 40, v_free = bar0 + 56,
-                 s_full = bar0 + 72, p_full = bar0 + 88, o_full = bar0 + 104, end = bar0 + 120;
+                 s_full = bar0 + 72, s_free = bar0 + 88, p_full = bar0 + 104, o_full = bar0 + 120, end = bar0 + 136;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t head = blockIdx.y;
   const int b = (int)(head / p.c.n_kv_heads);
@@ -257,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     for (int i = 0; i < 2; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(k_full + 8 * i), "n"(kConvThreads));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(v_full + 8 * i), "n"(kConvThreads));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s_free + 8 * i), "n"(kRows));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(p_full + 8 * i), "n"(kRows));
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -281,6 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 
   if (warp < kSoftWarps) {
     // ---------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     const int tile = warp / 4, r = row0 + tile * kRows + (warp % 4) * 32 + lane;
     if (tile < tiles) {
       const uint32_t lanes = (uint32_t)(warp % 4) << 21;  // this warp's lanes of tensor memory (bits 16-31)
@@ -292,7 +328,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       const float* vsc = p.c.v_scale + head * (p.c.max_len / kKv8Block);
       const int vis = last / kKv8Block;  // the last block any row sees
       float m = -INFINITY, l = 0.0f;
-      const int e_ref = n > 0 ? kv8_exponent(vsc[kHalves * beg]) : 0;
+      constexpr float kCode = FMT == CB_KV8_E4M3 ? 256.0f : 1.0f;  // the operands hold codes / kCode
+      const int e_ref = n > 0 ? kv8_exponent(vsc[kHalves * beg] * kCode) : 0;
       float ks[kHalves], vs[kHalves];
       auto scales = [&](int j) {
 #pragma unroll
@@ -309,8 +346,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         int ev[kHalves];
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
-          a[h] = fmaxf(back * ks[h], 1.2e-38f);  // above 0: a masked score times it stays -infinity
-          ev[h] = kv8_exponent(vs[h]);
+          a[h] = fmaxf(back * (ks[h] * kCode), 1.2e-38f);  // above 0: a masked score times it stays -infinity
+          ev[h] = kv8_exponent(vs[h] * kCode);
         }
         if (j + 1 < n) scales(j + 1);
         if (!wait(s_full + 8 * tile, j)) break;
@@ -338,84 +375,89 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], v[28 + k]);
           return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
         };
-        // the largest x + e of the tile
-        auto top_of = [&](const float (&t)[kHalves]) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int h = 0; h < kHalves; ++h)
-            if (t[h] > -INFINITY) top = fmaxf(top, fmaf(t[h], a[h], (float)ev[h]));
-          return top;
-        };
-        if (__any_sync(0xffffffffu, m == -INFINITY)) {  // rows without a maximum yet: take the tile's
-          float t[kHalves];
-          fetch(0);
-#pragma unroll
-          for (int q = 0; q < kKeys / 32; ++q) {
-            tmem_ld_wait();
-            if (q + 1 < kKeys / 32) fetch(q + 1);
-            mask(q);
-            const float x = max_of(q);
-            t[q / 2] = q & 1 ? fmaxf(t[q / 2], x) : x;
-          }
-          if (m == -INFINITY) m = top_of(t);
-        }
-        // P against the maximum so far; again where the tile raised it too far
+        // P against the maximum so far, raised where 32 scores pass it by 2^kLazy.
+        // All scores are read before the last 32 are exponentiated: from there on
+        // the next tile's may replace them.
         float sum_l = 0.0f;
-        for (int turn = 0;; ++turn) {
-          const float sub = m == -INFINITY ? 0.0f : m;
-          float t[kHalves];
-          sum_l = 0.0f;
-          fetch(0);
+        fetch(0);
 #pragma unroll
-          for (int h = 0; h < kHalves; ++h) {
-            const f32x2 a2 = pack2(a[h], a[h]), c2 = pack2((float)ev[h] - sub, (float)ev[h] - sub);
-            f32x2 sum[2] = {0, 0};  // pairs of zeros
+        for (int h = 0; h < kHalves; ++h) {
+          const f32x2 a2 = pack2(a[h], a[h]);
+          const float back_l = kv8_pow2(min(max(e_ref - ev[h], -100), 100));
+          f32x2 sum[2] = {0, 0};  // pairs of zeros
 #pragma unroll
-            for (int q = 2 * h; q < 2 * h + 2; ++q) {
-              tmem_ld_wait();
-              if (q + 1 < kKeys / 32) fetch(q + 1);
-              mask(q);
-              const float x = max_of(q);
-              t[h] = q & 1 ? fmaxf(t[h], x) : x;
-              uint32_t ph[16];
+          for (int q = 2 * h; q < 2 * h + 2; ++q) {
+            tmem_ld_wait();
+            if (q + 1 < kKeys / 32) {
+              fetch(q + 1);
+            } else {
+              fence_before();
+              mbar_arrive(s_free + 8 * tile);
+            }
+            mask(q);
+            const float top = max_of(q), now = top > -INFINITY ? fmaf(top, a[h], (float)ev[h]) : -INFINITY;
+            const bool grow = now > m + kLazy || (m == -INFINITY && now > m);
+            if (__any_sync(0xffffffffu, grow)) {
+              // by a power of two: what is written already is scaled without rounding
+              const float by = grow && m > -INFINITY ? ceilf(now - m) : 0.0f, alpha = exp2a(-by);
+              if (grow) m = m > -INFINITY ? m + by : now;
+              l *= alpha;
+              sum_l *= alpha;
+              sum[0] = mul2(sum[0], pack2(alpha, alpha));
+              sum[1] = mul2(sum[1], pack2(alpha, alpha));
+              const __half2 ah = __float2half2_rn(alpha);
+              if (q > 0) {  // P of this tile
+                tmem_st_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 d = unpack2(fma2(pack2(s[q & 1][2 * i], s[q & 1][2 * i + 1]), a2, c2));
-                const float y0 = exp2a(d.x), y1 = exp2a(d.y);
-                sum[i & 1] = add2(sum[i & 1], pack2(y0, y1));
-                ph[i] = h2_bits(__floats2half2_rn(y0, y1));
+                for (int c = 0; c < 16 * q; c += 16) {
+                  uint32_t u[16];
+                  tmem_ld16(tp + c, u);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) u[i] = h2_bits(__hmul2(bits_h2(u[i]), ah));
+                  tmem_st16(tp + c, u);
+                }
               }
-              tmem_st16(tp + q * 16, ph);
-            }
-            const float2 both = unpack2(add2(sum[0], sum[1]));
-            sum_l = fmaf(both.x + both.y, kv8_pow2(min(max(e_ref - ev[h], -100), 100)), sum_l);
-          }
-          const float now = top_of(t);
-          const bool grow = now > m + kLazy;
-          if (turn > 0 || !__any_sync(0xffffffffu, grow)) break;
-          const float alpha = grow ? exp2a(m - now) : 1.0f;
-          if (grow) m = now;
-          l *= alpha;
-          if (j > 0) {
-            // s_full(j) was committed after the product with tile j - 1's P: O is at rest
+              if (j > 0) {
+                wait(o_full + 8 * tile, j - 1);
+                fence_after();
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              tmem_ld32(to + c, s[0]);
-              tmem_ld_wait();
+                for (int c = 0; c < D; c += 16) {
+                  uint32_t u[16];
+                  tmem_ld16(to + c, u);
+                  tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) s[0][i] *= alpha;
-              tmem_st32(to + c, s[0]);
+                  for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * alpha);
+                  tmem_st16(to + c, u);
+                }
+              }
             }
+            const float add = (float)ev[h] - (m == -INFINITY ? 0.0f : m);
+            const f32x2 c2 = pack2(add, add);
+            uint32_t ph[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 d = unpack2(fma2(pack2(s[q & 1][2 * i], s[q & 1][2 * i + 1]), a2, c2));
+              const float y0 = exp2a(d.x), y1 = exp2a(d.y);
+              sum[i & 1] = add2(sum[i & 1], pack2(y0, y1));
+              ph[i] = h2_bits(__floats2half2_rn(y0, y1));
+            }
+            if (q == 0 && j > 0) {  // the product with the last tile's P has read it
+              wait(o_full + 8 * tile, j - 1);
+              fence_after();
+            }
+            tmem_st16(tp + q * 16, ph);
           }
-          tmem_st_wait();  // P is written once more
+          const float2 both = unpack2(add2(sum[0], sum[1]));
+          sum_l = fmaf(both.x + both.y, back_l, sum_l);
         }
         l += sum_l;
         tmem_st_wait();
         fence_before();
         mbar_arrive(p_full + 8 * tile);
       }
-      // results: O, m' and l (against e_ref)
-      if (n > 0) wait(o_full + 8 * tile, 0);
+      // results: O, m' and l (against e_ref).  (Products n - 2 and before are known done.)
+      if (n > 0) wait(o_full + 8 * tile, n - 1);
       fence_after();
       const float lsum = l * kv8_pow2(-e_ref);
       const int t = r / p.G, hq = (int)(head % p.c.n_kv_heads) * p.G + r % p.G;
@@ -461,6 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     }
   } else if (warp < kSoftWarps + kConvThreads / 32) {
     // ------------------------------------------------- codes to operands
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
     const int d = tid - kSoftWarps * 32;
     const uint8_t* src[2] = {p.c.k + head * p.c.max_len * D, p.c.v + head * p.c.max_len * D};
     uint4 raw[2][C::kPieces];
@@ -489,10 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         for (int i = 0; i < C::kPieces; ++i) {
           const int key = key_of(i), c = chunk_of(i);
           uint4 lo, hi;
-          codes_to_h2<FMT>(raw[kv][i].x, lo.x, lo.y);
-          codes_to_h2<FMT>(raw[kv][i].y, lo.z, lo.w);
-          codes_to_h2<FMT>(raw[kv][i].z, hi.x, hi.y);
-          codes_to_h2<FMT>(raw[kv][i].w, hi.z, hi.w);
+          to_operand<FMT>(raw[kv][i], lo, hi);
           *reinterpret_cast<uint4*>(dst + swizzled<kKeys>(key, 2 * c)) = lo;
           *reinterpret_cast<uint4*>(dst + swizzled<kKeys>(key, 2 * c + 1)) = hi;
         }
@@ -502,63 +542,67 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       }
       if (!ok) break;
     }
-  } else if (n > 0) {
+  } else {
     // ---------------------------------------------------------- products
-    // The whole warp walks the loop, so that addresses and descriptors stay in
-    // uniform registers; one elected thread issues.  (A branch of one thread moved
-    // them there for every instruction: 90 to 140 clocks each instead of 32 or 64.)
-    const bool lead = elect_one();
-    const uint32_t q_at = smem_u32(sq), k_at = smem_u32(sk), v_at = smem_u32(sv);
-    if (lead) {
-      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(q_full), "r"(tiles * C::kQ) : "memory");
-      asm volatile(
-          "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(q_at),
-          "l"(p.q16 + (head * p.row_tiles + pair * kTiles) * (int64_t)C::kQ), "r"(tiles * C::kQ), "r"(q_full)
-          : "memory");
-    }
-    constexpr uint32_t kIdS = idesc(kRows, kKeys, false), kIdO = idesc(kRows, D, true);
-    auto all_wait = [&](uint32_t bar, int phase) { return __all_sync(0xffffffffu, wait(bar, phase)); };
-    auto qk = [&](int t, int st) {
-      const uint64_t qd = mat_desc(q_at + t * C::kQ, 16), kd = mat_desc(k_at + st * C::kKV, 16);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+    if (warp == kSoftWarps + kConvThreads / 32 && n > 0) {
+      // The whole warp walks the loop, so that addresses and descriptors stay in
+      // uniform registers; one elected thread issues.  (A branch of one thread moved
+      // them there for every instruction: 90 to 140 clocks each instead of 32 or 64.)
+      const bool lead = elect_one();
+      const uint32_t q_at = smem_u32(sq), k_at = smem_u32(sk), v_at = smem_u32(sv);
       if (lead) {
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-          mma_ss(t * kKeys, qd + (s / 4 * (kRows * 128) + s % 4 * 32) / 16, kd + (s / 4 * (kKeys * 128) + s % 4 * 32) / 16,
-                 kIdS, s > 0);
-        commit(s_full + 8 * t);
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(q_full), "r"(tiles * C::kQ) : "memory");
+        asm volatile(
+            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(q_at),
+            "l"(p.q16 + (head * p.row_tiles + pair * kTiles) * (int64_t)C::kQ), "r"(tiles * C::kQ), "r"(q_full)
+            : "memory");
       }
-    };
-    bool go = all_wait(q_full, 0) && all_wait(k_full, 0);
-    if (go) {
-      for (int t = 0; t < tiles; ++t) qk(t, 0);
-      if (lead) commit(k_free);
-    }
-    for (int j = 0; j < n && go; ++j) {
-      const int st = j & 1, next = (j + 1) & 1;
-      for (int t = 0; t < tiles && go; ++t) {
-        go = all_wait(p_full + 8 * t, j) && (t > 0 || all_wait(v_full + 8 * st, j / 2));
-        if (!go) break;
-        fence_after();
-        const uint64_t vd = mat_desc(v_at + st * C::kKV, kKeys * 128);
+      constexpr uint32_t kIdS = idesc(kRows, kKeys, false), kIdO = idesc(kRows, D, true);
+      auto all_wait = [&](uint32_t bar, int phase) { return __all_sync(0xffffffffu, wait(bar, phase)); };
+      auto qk = [&](int t, int st) {
+        const uint64_t qd = mat_desc(q_at + t * C::kQ, 16), kd = mat_desc(k_at + st * C::kKV, 16);
         if (lead) {
 #pragma unroll
-          for (int s = 0; s < kKeys / 16; ++s)
-            mma_ts(C::kO + t * D, C::kP + t * (kKeys / 2) + s * 8, vd + s * 2048 / 16, kIdO, j > 0 || s > 0);
-          if (j + 1 == n) commit(o_full + 8 * t);
-          if (t + 1 == tiles) commit(v_free + 8 * st);
+          for (int s = 0; s < D / 16; ++s)
+            mma_ss(t * kKeys, qd + (s / 4 * (kRows * 128) + s % 4 * 32) / 16, kd + (s / 4 * (kKeys * 128) + s % 4 * 32) / 16,
+                   kIdS, s > 0);
+          commit(s_full + 8 * t);
         }
-        if (j + 1 < n) {
-          if (t == 0) go = all_wait(k_full + 8 * next, (j + 1) / 2);
+      };
+      bool go = all_wait(q_full, 0) && all_wait(k_full, 0);
+      if (go) {
+        for (int t = 0; t < tiles; ++t) qk(t, 0);
+        if (lead) commit(k_free);
+      }
+      for (int j = 0; j < n && go; ++j) {
+        const int st = j & 1, next = (j + 1) & 1;
+        for (int t = 0; t < tiles && go; ++t) {
+          if (j + 1 < n) {
+            go = (t > 0 || all_wait(k_full + 8 * next, (j + 1) / 2)) && all_wait(s_free + 8 * t, j);
+            if (!go) break;
+            fence_after();
+            qk(t, next);
+            if (lead && t + 1 == tiles) commit(k_free + 8 * next);
+          }
+          go = all_wait(p_full + 8 * t, j) && (t > 0 || all_wait(v_full + 8 * st, j / 2));
           if (!go) break;
-          qk(t, next);
-          if (lead && t + 1 == tiles) commit(k_free + 8 * next);
+          fence_after();
+          const uint64_t vd = mat_desc(v_at + st * C::kKV, kKeys * 128);
+          if (lead) {
+#pragma unroll
+            for (int s = 0; s < kKeys / 16; ++s)
+              mma_ts(C::kO + t * D, C::kP + t * (kKeys / 2) + s * 8, vd + s * 2048 / 16, kIdO, j > 0 || s > 0);
+            commit(o_full + 8 * t);
+            if (t + 1 == tiles) commit(v_free + 8 * st);
+          }
         }
       }
-    }
-    if (!go) {  // let the copy and the products in flight end before their memory goes
-      mbar_wait(q_full, 0);
-      if (lead) commit(end);
-      mbar_wait(end, 0);
+      if (!go) {  // let the copy and the products in flight end before their memory goes
+        mbar_wait(q_full, 0);
+        if (lead) commit(end);
+        mbar_wait(end, 0);
+      }
     }
   }
   fence_before();
