@@ -21,13 +21,13 @@
 //     of tiny values nor one of huge ones costs the others precision: P's f16
 //     rounding is relative to what the row adds up.  The row's sum is
 //     l = sum_b 2^-e_b sum P (before P is rounded), the same in float32.
-//   * P is taken against the maximum so far, in the same pass over S that finds the
-//     tile's own, 32 scores at a time.  Only where they pass it by more than 2^15
-//     (f16 P ends at 2^16) is it raised, by a power of two, and what was written
-//     against it rescaled in tensor memory.
-// The next tile's scores are taken while the last exponentials of this one run,
-// and its products with V while the next exponentials do, so a warpgroup hardly
-// waits.  The exponentials bound it for head_dim 64: 128 x 128 per tile at 16 a
+//   * a thread reads its row of S into registers at once, so that the next tile's
+//     scores can follow, and takes P against the maximum so far.  Only where the
+//     tile's passes it by more than 2^15 (f16 P ends at 2^16) is it raised, and O
+//     rescaled in tensor memory.
+// The next tile's scores are taken while the exponentials of this one run, and its
+// product with V while the next ones do; the two warpgroups take turns at the
+// exponentials and at what lies between them.  The exponentials bound it for head_dim 64: 128 x 128 per tile at 16 a
 // clock take 1024 clocks, its products 512.
 // With several runs per row tile, kv8_join_kernel joins them (kv8_attend.cu).
 // Every wait is bounded (%globaltimer); a wait that gives up sets CB_ERR_TIMEOUT
@@ -48,7 +48,7 @@ constexpr int kConvThreads = 128;
 constexpr int kThreads = kSoftWarps * 32 + kConvThreads + 128;
 // Registers a thread of the four warpgroups, out of the 128 at launch: two of
 // softmax, one that converts, one whose first warp issues the products.
-constexpr int kSoftRegs = 184, kConvRegs = 88, kMmaRegs = 56;
+constexpr int kSoftRegs = 192, kConvRegs = 88, kMmaRegs = 40;
 static_assert(2 * kSoftRegs + kConvRegs + kMmaRegs <= 4 * 128, "the shares fit what the block was launched with");
 constexpr float kLazy = 15.0f;             // growth of the maximum, in powers of two, that O follows: f16 P ends at 2^16
 constexpr unsigned long long kTimeoutNs = 200ull * 1000 * 1000;
@@ -353,103 +353,74 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         if (!wait(s_full + 8 * tile, j)) break;
         fence_after();
         const bool whole = __all_sync(0xffffffffu, lim >= key0 + kKeys - 1);
-        // 32 scores at a time, the next ones on their way
-        float s[2][32];
-        auto fetch = [&](int q) { tmem_ld32(ts + q * 32, s[q & 1]); };
-        auto mask = [&](int q) {
-          if (whole) return;
+        float s[kKeys];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (key0 + q * 32 + i > lim) s[q & 1][i] = -INFINITY;
-        };
-        auto max_of = [&](int q) {
-          const float* v = s[q & 1];
+        for (int q = 0; q < kKeys / 32; ++q) tmem_ld32(ts + q * 32, s + q * 32);
+        tmem_ld_wait();
+        fence_before();
+        mbar_arrive(s_free + 8 * tile);  // the next tile's scores may replace them
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i)
+            if (key0 + i > lim) s[i] = -INFINITY;
+        }
+        float now = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          const float* v = s + h * 64;
           float t[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) t[k] = v[k];
 #pragma unroll
-          for (int i = 4; i < 28; i += 8)
+          for (int i = 4; i < 60; i += 8)
 #pragma unroll
             for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], v[i + k]), v[i + 4 + k]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], v[28 + k]);
-          return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-        };
-        // P against the maximum so far, raised where 32 scores pass it by 2^kLazy.
-        // All scores are read before the last 32 are exponentiated: from there on
-        // the next tile's may replace them.
+          for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], v[60 + k]);
+          const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+          if (top > -INFINITY) now = fmaxf(now, fmaf(top, a[h], (float)ev[h]));
+        }
+        const bool grow = now > m + kLazy || (m == -INFINITY && now > m);
+        if (j > 0) {  // the product with the last tile's P has read it, and O is at rest
+          wait(o_full + 8 * tile, j - 1);
+          fence_after();
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = !grow ? 1.0f : m > -INFINITY ? exp2a(m - now) : 0.0f;
+          if (grow) m = now;
+          l *= alpha;
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < D; c += 16) {
+              uint32_t u[16];
+              tmem_ld16(to + c, u);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * alpha);
+              tmem_st16(to + c, u);
+            }
+          }
+        }
         float sum_l = 0.0f;
-        fetch(0);
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
-          const f32x2 a2 = pack2(a[h], a[h]);
-          const float back_l = kv8_pow2(min(max(e_ref - ev[h], -100), 100));
+          const float add = (float)ev[h] - (m == -INFINITY ? 0.0f : m);
+          const f32x2 a2 = pack2(a[h], a[h]), c2 = pack2(add, add);
           f32x2 sum[2] = {0, 0};  // pairs of zeros
 #pragma unroll
           for (int q = 2 * h; q < 2 * h + 2; ++q) {
-            tmem_ld_wait();
-            if (q + 1 < kKeys / 32) {
-              fetch(q + 1);
-            } else {
-              fence_before();
-              mbar_arrive(s_free + 8 * tile);
-            }
-            mask(q);
-            const float top = max_of(q), now = top > -INFINITY ? fmaf(top, a[h], (float)ev[h]) : -INFINITY;
-            const bool grow = now > m + kLazy || (m == -INFINITY && now > m);
-            if (__any_sync(0xffffffffu, grow)) {
-              // by a power of two: what is written already is scaled without rounding
-              const float by = grow && m > -INFINITY ? ceilf(now - m) : 0.0f, alpha = exp2a(-by);
-              if (grow) m = m > -INFINITY ? m + by : now;
-              l *= alpha;
-              sum_l *= alpha;
-              sum[0] = mul2(sum[0], pack2(alpha, alpha));
-              sum[1] = mul2(sum[1], pack2(alpha, alpha));
-              const __half2 ah = __float2half2_rn(alpha);
-              if (q > 0) {  // P of this tile
-                tmem_st_wait();
-#pragma unroll
-                for (int c = 0; c < 16 * q; c += 16) {
-                  uint32_t u[16];
-                  tmem_ld16(tp + c, u);
-                  tmem_ld_wait();
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) u[i] = h2_bits(__hmul2(bits_h2(u[i]), ah));
-                  tmem_st16(tp + c, u);
-                }
-              }
-              if (j > 0) {
-                wait(o_full + 8 * tile, j - 1);
-                fence_after();
-#pragma unroll
-                for (int c = 0; c < D; c += 16) {
-                  uint32_t u[16];
-                  tmem_ld16(to + c, u);
-                  tmem_ld_wait();
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * alpha);
-                  tmem_st16(to + c, u);
-                }
-              }
-            }
-            const float add = (float)ev[h] - (m == -INFINITY ? 0.0f : m);
-            const f32x2 c2 = pack2(add, add);
             uint32_t ph[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float2 d = unpack2(fma2(pack2(s[q & 1][2 * i], s[q & 1][2 * i + 1]), a2, c2));
+              const float2 d = unpack2(fma2(pack2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), a2, c2));
               const float y0 = exp2a(d.x), y1 = exp2a(d.y);
               sum[i & 1] = add2(sum[i & 1], pack2(y0, y1));
               ph[i] = h2_bits(__floats2half2_rn(y0, y1));
             }
-            if (q == 0 && j > 0) {  // the product with the last tile's P has read it
-              wait(o_full + 8 * tile, j - 1);
-              fence_after();
-            }
             tmem_st16(tp + q * 16, ph);
           }
           const float2 both = unpack2(add2(sum[0], sum[1]));
-          sum_l = fmaf(both.x + both.y, back_l, sum_l);
+          sum_l = fmaf(both.x + both.y, kv8_pow2(min(max(e_ref - ev[h], -100), 100)), sum_l);
         }
         l += sum_l;
         tmem_st_wait();
