@@ -60,6 +60,13 @@ __device__ __forceinline__ float exp2a(float x) {
   return y;
 }
 
+// The larger of two; NaN if either is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 // Pairs of floats on the packed float32 units.
 using f32x2 = unsigned long long;
 __device__ __forceinline__ f32x2 pack2(float a, float b) {

@@ -374,7 +374,9 @@ int launch_dfh(const AttendParams& p, int bh, int longest, cudaStream_t st) {
     kv8_join_kernel<<<dim3(p.rows, bh), D, 0, st>>>(p);
     count_launch();
   }
-  if (p.add_mass) {
+  if (p.add_mass && p.row_tiles > 0) {
+    if (const int rc = kv8_prompt_mass_launch(p, bh, longest, st)) return rc;
+  } else if (p.add_mass) {
     kv8_mass_kernel<D, FMT, HL><<<dim3(ceil_div(longest, kWarps * kKv8Block), bh), kWarps * 32, 0, st>>>(p);
     count_launch();
   }

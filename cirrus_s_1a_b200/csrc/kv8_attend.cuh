@@ -33,6 +33,8 @@ struct AttendParams {
 // Many query rows, head_dim 64 or 128, 16-bit queries (kv8_prompt.cu).  Writes out
 // and lse where splits is 1, parts otherwise.
 int kv8_prompt_launch(const AttendParams& p, int bh, cudaStream_t st);
+// The rows' attention weights into mass, after lse is complete.
+int kv8_prompt_mass_launch(const AttendParams& p, int bh, int longest, cudaStream_t st);
 
 int kv8_check(const CbKv8* c);
 bool kv8_dtype_ok(int dtype);

@@ -583,6 +583,179 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(s_tmem));
 }
 
+// ----------------------------------------------------------------- weights
+// mass_j += sum_r exp(x[r][j] - lse_r) for the query rows of a KV head: the scores
+// are taken again, transposed (keys in the 128 lanes, 128 query rows in the
+// columns), so that a thread owns a key and adds its probabilities up in one fixed
+// order, without atomics.  A CTA owns 128 keys, turned into an operand once; query
+// tiles and their rows' factors stream through four stages, the scores through four
+// buffers of tensor memory, two warpgroups take them in turn.
+constexpr int kMassStages = 4;
+template <int D>
+struct Mass {
+  static constexpr int kQ = kRows * D * 2;
+  static constexpr int kInfo = kRows * 8;  // of each row: the factor of its scores, and -lse (log2 units)
+  static constexpr int kSmem = kQ + kMassStages * (kQ + kInfo) + 1024;
+};
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __grid_constant__ AttendParams p) {
+  using C = Mass<D>;
+  constexpr float kCode = FMT == CB_KV8_E4M3 ? 256.0f : 1.0f;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sk = smem_raw + (-smem_u32(smem_raw) & 1023);
+  uint8_t* sq = sk + C::kQ;
+  float* s_info = reinterpret_cast<float*>(sq + kMassStages * C::kQ);  // [stage][2][128]
+  __shared__ __align__(8) unsigned long long bars[3 * kMassStages + 1];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  __shared__ float s_sum[kRows];
+  const uint32_t q_full = smem_u32(bars), q_free = q_full + 8 * kMassStages, s_full = q_free + 8 * kMassStages,
+                 end = s_full + 8 * kMassStages;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t head = blockIdx.y;
+  const int b = (int)(head / p.c.n_kv_heads), hk = (int)(head % p.c.n_kv_heads);
+  const int key0 = blockIdx.x * kRows;
+  const int pos = p.pos[b], cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
+  const int last = cnt > 0 ? min(pos + cnt, p.c.max_len) - 1 : -1;
+  if (key0 > last) return;
+  // row tiles from the first row that sees key0
+  const int first = max(0, key0 - pos) * p.G / kRows, n = ceil_div(cnt * p.G, kRows) - first;
+
+  if (tid == 0) {
+    for (int i = 0; i < kMassStages; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(q_full + 8 * i), "n"(kConvThreads + 1));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(q_free + 8 * i), "n"(kRows + 1));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(s_full + 8 * i));
+    }
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(end));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_abort = 0;
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // the keys, slots no row sees as 0
+  const uint8_t* src = p.c.k + head * p.c.max_len * D;
+  for (int i = tid; i < kRows * (D / 16); i += kThreads) {
+    const int key = (i & 7) + 8 * (i / (8 * (D / 16))), c = i / 8 % (D / 16);
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u), lo, hi;
+    if (key0 + key <= last) raw = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)(key0 + key) * D) + c);
+    to_operand<FMT>(raw, lo, hi);
+    *reinterpret_cast<uint4*>(sk + swizzled<kRows>(key, 2 * c)) = lo;
+    *reinterpret_cast<uint4*>(sk + swizzled<kRows>(key, 2 * c + 1)) = hi;
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  fence_before();
+  __syncthreads();
+  fence_after();
+  bool ok = true;
+  auto wait = [&](uint32_t bar, int phase) {
+    if (ok && !mbar_wait(bar, phase & 1)) {
+      ok = false;
+      s_abort = 1;
+    }
+    return ok;
+  };
+  float mine = 0.0f;
+  if (warp < kSoftWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    const int group = warp / 4, key = key0 + (warp % 4) * 32 + lane;
+    const float ks = p.c.k_scale[head * (p.c.max_len / kKv8Block) + min(key, last) / kKv8Block] * kCode;
+    const f32x2 ks2 = pack2(ks, ks);
+    f32x2 sum[2] = {0, 0};
+    for (int k = group; k < n; k += 2) {
+      const int st = k % kMassStages;
+      if (!wait(s_full + 8 * st, k / kMassStages)) break;
+      fence_after();
+      float s[kRows];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) tmem_ld32(((uint32_t)(warp % 4) << 21) + st * kRows + q * 32, s + q * 32);
+      tmem_ld_wait();
+      fence_before();
+      const int row0 = (first + k) * kRows;
+      // the tile's first row sees the least: a key past it is not seen by all of them
+      if (!__all_sync(0xffffffffu, key <= pos + row0 / p.G)) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+          if (key > pos + (row0 + i) / p.G) s[i] = -INFINITY;
+      }
+      const float* f = s_info + st * 2 * kRows;
+#pragma unroll
+      for (int i = 0; i < kRows; i += 4) {
+        const float4 by = *reinterpret_cast<const float4*>(f + i), sub = *reinterpret_cast<const float4*>(f + kRows + i);
+        const float2 x = unpack2(fma2(mul2(pack2(s[i], s[i + 1]), ks2), pack2(by.x, by.y), pack2(sub.x, sub.y)));
+        const float2 y = unpack2(fma2(mul2(pack2(s[i + 2], s[i + 3]), ks2), pack2(by.z, by.w), pack2(sub.z, sub.w)));
+        sum[0] = add2(sum[0], pack2(exp2a(x.x), exp2a(x.y)));
+        sum[1] = add2(sum[1], pack2(exp2a(y.x), exp2a(y.y)));
+      }
+      mbar_arrive(q_free + 8 * st);
+    }
+    const float2 both = unpack2(add2(sum[0], sum[1]));
+    mine = both.x + both.y;
+    if (group == 1) s_sum[(warp % 4) * 32 + lane] = mine;
+  } else if (warp < kSoftWarps + kConvThreads / 32) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
+    const int d = tid - kSoftWarps * 32;
+    for (int k = 0; k < n; ++k) {
+      const int st = k % kMassStages, tile = first + k, r = tile * kRows + d, t = r / p.G;
+      if (k >= kMassStages && !wait(q_free + 8 * st, k / kMassStages - 1)) break;
+      if (d == 0) {
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(q_full + 8 * st), "r"(C::kQ) : "memory");
+        asm volatile(
+            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                smem_u32(sq) + st * C::kQ),
+            "l"(p.q16 + (head * p.row_tiles + tile) * (int64_t)C::kQ), "r"(C::kQ), "r"(q_full + 8 * st)
+            : "memory");
+      }
+      // rows that see nothing: a factor that leaves any score finite, and -infinity
+      float by = 1.2e-38f, sub = -INFINITY;
+      if (t < cnt && pos + t >= 0) {
+        by = fmaxf(p.q_back[head * p.row_tiles * kRows + r], 1.2e-38f);
+        sub = -p.lse[((int64_t)b * p.T + t) * (p.G * p.c.n_kv_heads) + hk * p.G + r % p.G] * kLog2e;
+      }
+      s_info[st * 2 * kRows + d] = by;
+      s_info[st * 2 * kRows + kRows + d] = sub;
+      mbar_arrive(q_full + 8 * st);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+    if (warp == kSoftWarps + kConvThreads / 32) {
+      const bool lead = elect_one();
+      const uint32_t k_at = smem_u32(sk), q_at = smem_u32(sq);
+      bool go = true;
+      for (int k = 0; k < n && go; ++k) {
+        const int st = k % kMassStages;
+        // the stage's query tile is new, so its scores' buffer has been read
+        go = __all_sync(0xffffffffu, wait(q_full + 8 * st, k / kMassStages));
+        if (!go) break;
+        fence_after();
+        const uint64_t kd = mat_desc(k_at, 16), qd = mat_desc(q_at + st * C::kQ, 16);
+        if (lead) {
+#pragma unroll
+          for (int s = 0; s < D / 16; ++s)
+            mma_ss(st * kRows, kd + (s / 4 * (kRows * 128) + s % 4 * 32) / 16,
+                   qd + (s / 4 * (kRows * 128) + s % 4 * 32) / 16, idesc(kRows, kRows, false), s > 0);
+          commit(s_full + 8 * st);
+          commit(q_free + 8 * st);
+        }
+      }
+      if (!go) {
+        if (lead) commit(end);
+        mbar_wait(end, 0);
+        for (int k = max(0, n - kMassStages); k < n; ++k) mbar_wait(q_full + 8 * (k % kMassStages), k / kMassStages & 1);
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (tid < kRows && key0 + tid <= last && !s_abort) p.c.mass[head * p.c.max_len + key0 + tid] += mine + s_sum[tid];
+  if (tid == 0 && s_abort) set_status(p.status, CB_ERR_TIMEOUT);
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(s_tmem));
+}
+
 template <int D>
 int launch_prompt(const AttendParams& p, int bh, cudaStream_t st) {
   kv8_query_kernel<D><<<dim3(ceil_div(p.row_tiles * kRows * (D / 8), 256), bh), 256, 0, st>>>(p);
@@ -596,6 +769,17 @@ int launch_prompt(const AttendParams& p, int bh, cudaStream_t st) {
 }
 
 }  // namespace
+
+int kv8_prompt_mass_launch(const AttendParams& p, int bh, int longest, cudaStream_t st) {
+  const bool e = p.c.format == CB_KV8_E4M3, narrow = p.c.head_dim == 64;
+  auto fn = narrow ? (e ? kv8_prompt_mass_kernel<64, CB_KV8_E4M3> : kv8_prompt_mass_kernel<64, CB_KV8_INT8>)
+                   : (e ? kv8_prompt_mass_kernel<128, CB_KV8_E4M3> : kv8_prompt_mass_kernel<128, CB_KV8_INT8>);
+  const int smem = narrow ? Mass<64>::kSmem : Mass<128>::kSmem;
+  if (const int rc = ensure_smem_attr((const void*)fn, smem)) return rc;
+  fn<<<dim3(ceil_div(longest, kRows), bh), kThreads, smem, st>>>(p);
+  count_launch();
+  return cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
+}
 
 int kv8_prompt_launch(const AttendParams& p, int bh, cudaStream_t st) {
   return p.c.head_dim == 64 ? launch_prompt<64>(p, bh, st) : launch_prompt<128>(p, bh, st);

@@ -56,13 +56,6 @@ __device__ __forceinline__ unsigned long long top_key(float v, int i) {
   return ((unsigned long long)score_key(v) << 32) | (uint32_t)~i;
 }
 
-// The larger of two; NaN if either is one.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
 // Running maximum m of one thread, and relative to c = m * log2(e) (rounded: every
 // term is taken against the rounded c, so its rounding cancels) the sums
 // l = sum 2^(x log2(e) - c) and t = sum of exponent * 2^exponent, each in two
