@@ -161,7 +161,7 @@ def lib() -> C.CDLL:
         L.cb_workspace_layout.argtypes = [C.POINTER(CbModel), I32, I32, I32, C.POINTER(CbWorkspaceLayout)]
         L.cb_kv8_append.argtypes = [P, P, P, I32, P, P, I32, P, P, P, P]
         L.cb_kv8_attend_scratch_bytes.restype = C.c_size_t
-        L.cb_kv8_attend_scratch_bytes.argtypes = [P, I32, I32, I32, I32]
+        L.cb_kv8_attend_scratch_bytes.argtypes = [P, I32, I32, I32, I32, I32]
         L.cb_kv8_attend.argtypes = [P, P, I32, P, I32, I32, P, P, I32, C.c_float, I32, P, P, P, C.c_size_t, P, P]
         L.cb_kv8_evict.argtypes = [P, P, I32, I32, P, P, P]
         L.cb_token_logprobs.argtypes = [P, I32, C.c_int64, I32, I32, P, I32, P, P, P, P, P, P, P]

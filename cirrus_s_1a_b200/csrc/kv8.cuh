@@ -53,6 +53,34 @@ __device__ __forceinline__ float kv8_decode(uint32_t b) {
   return (float)(int8_t)(b & 0xFF);
 }
 
+// Waits on an mbarrier phase, at most kTimeoutNs.
+constexpr unsigned long long kTimeoutNs = 200ull * 1000 * 1000;
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ unsigned long long timer_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+  if (mbar_try(bar, parity)) return true;
+  const unsigned long long t0 = timer_ns();
+  while (!mbar_try(bar, parity))
+    if (timer_ns() - t0 > kTimeoutNs) return false;
+  return true;
+}
+
 // 2^x to about 2^-22; 0 below 2^-126.
 __device__ __forceinline__ float exp2a(float x) {
   float y;

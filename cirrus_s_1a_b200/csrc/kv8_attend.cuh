@@ -16,13 +16,20 @@ struct AttendParams {
   int G, T, rows;       // query heads per KV head; rows = T * G of a KV head
   const int32_t* pos;
   const int32_t* counts;
+  int limit;            // slots from here on are not seen
   float scale;
   bool add_mass;
   void* out;            // [batch][T][heads][dim], the queries' type
   float* lse;           // [batch][T][heads]
-  int splits;
-  float* part_ml;       // [batch * kv heads][rows][splits][2] running maximum (log2 units) and sum
-  float* part_o;        // [batch * kv heads][rows][splits][dim]
+  int splits;           // runs: of all heads' blocks (decode form), of each row tile's keys (prompt form)
+  // parts: maximum (log2 units) and sum, and values.  Decode form: [16 rows][run + head][16]
+  // rows, part_rows of them for each 16 query rows; prompt form: [head][rows][splits].
+  int64_t part_rows;
+  float* part_ml;       // [part][2]
+  float* part_o;        // [part][dim]
+  int* arrived;         // [16 rows][head]: parts finished; zero between calls
+  float* scores;        // [head][rows][ld_scores] in log2 units, or null
+  int64_t ld_scores;
   // the prompt form: query rows prepared in 128-row operand tiles, and the factors that undo their scaling
   int row_tiles;
   uint8_t* q16;         // [batch * kv heads][row_tiles][128 * dim * 2 bytes]

@@ -51,33 +51,6 @@ constexpr int kThreads = kSoftWarps * 32 + kConvThreads + 128;
 constexpr int kSoftRegs = 192, kConvRegs = 88, kMmaRegs = 40;
 static_assert(2 * kSoftRegs + kConvRegs + kMmaRegs <= 4 * 128, "the shares fit what the block was launched with");
 constexpr float kLazy = 15.0f;             // growth of the maximum, in powers of two, that O follows: f16 P ends at 2^16
-constexpr unsigned long long kTimeoutNs = 200ull * 1000 * 1000;
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ unsigned long long timer_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  if (mbar_try(bar, parity)) return true;
-  const unsigned long long t0 = timer_ns();
-  while (!mbar_try(bar, parity))
-    if (timer_ns() - t0 > kTimeoutNs) return false;
-  return true;
-}
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -204,7 +177,7 @@ __device__ __forceinline__ void to_operand(uint4 c, uint4& lo, uint4& hi) {
 __device__ __forceinline__ int row_limit(const AttendParams& p, int r, int pos, int cnt) {
   const int t = r / p.G;
   if (r >= p.rows || t >= cnt) return -1;
-  return min(pos + t, p.c.max_len - 1);
+  return min(pos + t, p.limit - 1);
 }
 
 // ------------------------------------------------------------------ queries
@@ -617,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
   const int b = (int)(head / p.c.n_kv_heads), hk = (int)(head % p.c.n_kv_heads);
   const int key0 = blockIdx.x * kRows;
   const int pos = p.pos[b], cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
-  const int last = cnt > 0 ? min(pos + cnt, p.c.max_len) - 1 : -1;
+  const int last = cnt > 0 ? min(pos + cnt, p.limit) - 1 : -1;
   if (key0 > last) return;
   // row tiles from the first row that sees key0
   const int first = max(0, key0 - pos) * p.G / kRows, n = ceil_div(cnt * p.G, kRows) - first;

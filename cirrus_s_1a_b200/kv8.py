@@ -187,10 +187,10 @@ class Kv8Cache:
             raise ValueError("out must be contiguous, of q's shape, type and device")
         lse = torch.empty(self.batch, T, heads, dtype=torch.float32, device=self.device)
         st = self._stream()
-        key = (st, dtype, heads, T, longest)
+        key = (st, dtype, heads, T, longest, add_mass)
         scratch = self._scratch.get(key)
         if scratch is None:
-            nbytes = self._lib.cb_kv8_attend_scratch_bytes(self._ref, dtype, heads, T, longest)
+            nbytes = self._lib.cb_kv8_attend_scratch_bytes(self._ref, dtype, heads, T, longest, int(add_mass))
             if nbytes == 0:
                 raise _lib.CbError("cb_kv8_attend_scratch_bytes: shape not supported")
             scratch = self._grow(st, nbytes)

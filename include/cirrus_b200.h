@@ -439,13 +439,15 @@ int cb_kv8_append(const CbKv8* c, const void* k, const void* v, int32_t dtype, c
  * Sums are float32; 16-bit queries meet the codes exactly and the probabilities
  * are rounded to f16 for the product with v; float32 queries and probabilities
  * are carried in about 22 bits.  longest: a bound on pos[b] + T that sizes the
- * launch.  scratch: cb_kv8_attend_scratch_bytes(c, dtype, n_q_heads, T, longest)
- * bytes, 16-byte aligned (as is out), not shared by calls that overlap.  status
+ * launch; slots from it on are not seen.  scratch: cb_kv8_attend_scratch_bytes(c, dtype, n_q_heads, T, longest,
+ * add_mass) bytes, 16-byte aligned (as is out), zeroed once before its first use
+ * (calls of any sizes may follow), not shared by calls that overlap.  status
  * (device int32, may be null) receives CB_ERR_TIMEOUT if a bounded wait on the
  * tensor-core pipeline gives up.
  * Replaces the dense attention of CrossAttention.forward over the shared K/V
  * (cirrus/model/layers.py:183-192, 325-339). */
-size_t cb_kv8_attend_scratch_bytes(const CbKv8* c, int32_t dtype, int32_t n_q_heads, int32_t T, int32_t longest);
+size_t cb_kv8_attend_scratch_bytes(const CbKv8* c, int32_t dtype, int32_t n_q_heads, int32_t T, int32_t longest,
+                                   int32_t add_mass);
 int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const int64_t* q_strides, int32_t n_q_heads,
                   int32_t T, const int32_t* pos, const int32_t* counts, int32_t longest, float scale,
                   int32_t add_mass, void* out, float* lse, void* scratch, size_t scratch_bytes, int32_t* status,

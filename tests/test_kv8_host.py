@@ -41,8 +41,8 @@ def test_entry_points_refuse_bad_arguments_without_launching(built_lib):  # noqa
     assert att(desc(), scratch=None) == 1 and att(desc(), n=0) == 4 and att(desc(mass=None), mass=1) == 1
     assert att(desc(), dtype=7) == 1 and att(desc(head_dim=100)) == 2
     assert att(desc(), scratch=264) == 1
-    need = L.cb_kv8_attend_scratch_bytes
-    assert need(desc(), 1, 2, 1, 128) > 0 and need(desc(), 1, 2, 100, 128) > need(desc(), 0, 2, 1, 128)
+    need = lambda c, dtype, hq, T, n: L.cb_kv8_attend_scratch_bytes(c, dtype, hq, T, n, 0)  # noqa: E731
+    assert need(desc(), 1, 2, 1, 128) > 0 and L.cb_kv8_attend_scratch_bytes(desc(), 1, 2, 1, 128, 1) > need(desc(), 1, 2, 1, 128)
     assert need(desc(), 1, 3, 1, 128) == 0 and need(None, 1, 2, 1, 1) == 0 and need(desc(), 5, 2, 1, 1) == 0
     ev = lambda c, keep=4, recent=2, pos=256, new=512: L.cb_kv8_evict(c, pos, keep, recent, 256, new, None)  # noqa: E731
     assert ev(None) == 1 and ev(desc(mass=None)) == 1 and ev(desc(), keep=0) == 1 and ev(desc(), recent=5) == 1
