@@ -7,24 +7,32 @@
 //
 // The rows of a KV head are its G query heads of the T tokens, r = t * G + g, so
 // the codes are read once for all of them.  kv8_attend_kernel runs on warp-level
-// matrix products (m16n8k16, f16 operands, f32 sums).  Codes are exact in f16;
-// the products' free index order is used so that no operand needs a transpose
+// matrix products (m16n8k16, f16 operands, f32 sums) with the codes as their left
+// operand: 16 keys, or 16 dims, by 8 NT query rows, so that a decode step's few rows
+// leave half of an 8-row operand empty, not of a 16-row one.  Codes are exact in
+// f16; the products' free index order is used so that no operand needs a transpose
 // through shared memory:
-//   * S = Q K^T: lane (g, t) = (lane / 4, lane % 4) reads D/4 contiguous bytes of
-//     one key row, so a warp's load covers whole rows; the four k positions a
-//     lane feeds in step s are the dims t * D/4 + 4 s .. + 3, and the query
-//     fragments are loaded in that order.
-//   * O = P V: the softmax of S leaves P in the layout of an A operand.  The key
-//     behind column c of key tile j is 8 j + 4 (c & 1) + c / 2, so the four keys
-//     a lane feeds in a step are 16 s + t + {0, 4, 8, 12}: four rows in a row
-//     across t.  The lane reads D/8 contiguous bytes of each (dims g * D/8 ..)
-//     and pairs the keys' bytes with byte permutes.
+//   * S^T = K Q^T: lane (g, t) = (lane / 4, lane % 4) reads D/4 contiguous bytes of
+//     a key row, so a warp's load covers whole rows; the four k positions a lane
+//     feeds in step s are the dims t * D/4 + 4 s .. + 3, and the query fragments are
+//     loaded in that order.
+//   * O^T = V^T P^T: P leaves the softmax with keys along lanes and is turned by
+//     movmatrix, 8 x 8 at a time.  Row i of an 8-key group is its key
+//     4 (i & 1) + i / 2, so the four keys a lane feeds in a step are t + {0, 4, 8,
+//     12}: four rows in a row across t.  The lane reads D/8 contiguous bytes of each
+//     (dims g * D/8 ..) and pairs the keys' bytes with byte permutes.
 // Queries: a row is scaled by a power of two that brings its largest element to
 // [256, 512) and rounded to f16.  bf16 and f16 queries are exact in that (up to
 // 2^-33 of the row's largest element); float32 queries and their P are carried
-// as a head and a tail (about 22 bits), two products each.  f16 P (11 bits) for
-// 16-bit outputs adds less than the output's own rounding.
-// Softmax statistics, the sums over V and the joins of parts are float32.
+// as a head and a tail (about 22 bits), two products each, and each block's product
+// is added up in float32 registers.  f16 P (11 bits) for 16-bit outputs adds less
+// than the output's own rounding.
+// With x = S * a_b (a_b = row factor * block b's key scale, log2 units) and e_b the
+// exponent of its value scale, P = exp2(x + e_b - m') against m' = max (x + e_b):
+// P times the bare codes is the sum over values, its f16 rounding relative to what
+// the row adds up, whatever the blocks' scales.  The row's sum is
+// l = sum_b 2^-e_b sum P.  O is rescaled only when m' has grown by more than 2^12.
+// Softmax statistics and the joins of parts are float32.
 //
 // Work is dealt out by blocks of 64 keys: the visible blocks of all KV heads, one
 // after another, are cut into equal runs, one per CTA (with sequences of different
@@ -43,6 +51,7 @@ namespace cb {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr float kLazy = 12.0f;  // growth of the maximum, in powers of two, that O follows: f16 P ends at 2^16
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -72,45 +81,82 @@ __device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t (&w)[(N + 
   }
 }
 
-// Query rows row0 .. row0 + 15 of a KV head as A fragments: lane (g, t) holds
-// rows g and g + 8.  `back` gets the factor that undoes each row's power of two,
-// times scale * log2(e).  HL: the tails too.
-template <int D, bool HL>
-__device__ __forceinline__ void load_q(const AttendParams& p, int b, int hk, int row0, uint32_t (&qh)[D / 16][4],
-                                       uint32_t (&ql)[HL ? D / 16 : 1][4], float (&back)[2]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+// Query rows row0 .. row0 + 8 NT - 1 of a KV head as right operands: lane (g, t)
+// feeds row g of each eight.  `back`: the factors that undo the powers of two, times
+// scale * log2(e), of the rows 2 t and 2 t + 1 that the lane's scores belong to.
+// HL: the tails too.
+template <int D, bool HL, int NT>
+struct Query {
+  uint32_t h[NT][D / 16][2], l[HL ? NT : 1][HL ? D / 16 : 1][2];
+  float back[NT][2];
+  __device__ __forceinline__ void load(const AttendParams& p, int b, int hk, int row0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = row0 + g + 8 * half;
-    float x[D / 4];
-    float top = 0.0f;
-    const bool live = r < p.rows;
-    const int t = r / p.G, hq = hk * p.G + r % p.G;
-    const int64_t base = (int64_t)b * p.qs[0] + (int64_t)t * p.qs[1] + hq * p.qs[2] + t4 * (D / 4);
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row0 + 8 * nt + g;
+      float x[D / 4];
+      float top = 0.0f;
+      const bool live = r < p.rows;
+      const int t = r / p.G, hq = hk * p.G + r % p.G;
+      const int64_t base = (int64_t)b * p.qs[0] + (int64_t)t * p.qs[1] + hq * p.qs[2] + t4 * (D / 4);
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i) {
-      x[i] = live ? kv8_load(p.q, base + i, p.dtype) : 0.0f;
-      top = fmaxf(top, fabsf(x[i]));
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    int e = 0;  // top in [2^e, 2^(e+1)); rows of zeros, infinities and the ends of the range keep e = 0
-    if (top > 0.0f && top < INFINITY) e = min(max((__float_as_int(top) >> 23) - 127, -100), 100);
-    const float f = kv8_pow2(8 - e);
-    back[half] = kv8_pow2(e - 8) * p.scale * kLog2e;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float u = x[4 * s + 2 * i] * f, v = x[4 * s + 2 * i + 1] * f;
-        const __half2 h = __floats2half2_rn(u, v);
-        qh[s][half + 2 * i] = h2_bits(h);
-        if (HL) {
-          const float2 back2 = __half22float2(h);
-          ql[HL ? s : 0][half + 2 * i] = h2_bits(__floats2half2_rn(u - back2.x, v - back2.y));
-        }
+      for (int i = 0; i < D / 4; ++i) {
+        x[i] = live ? kv8_load(p.q, base + i, p.dtype) : 0.0f;
+        top = fmaxf(top, fabsf(x[i]));
       }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int e = 0;  // top in [2^e, 2^(e+1)); rows of zeros, infinities and the ends of the range keep e = 0
+      if (top > 0.0f && top < INFINITY) e = min(max((__float_as_int(top) >> 23) - 127, -100), 100);
+      const float f = copysignf(kv8_pow2(8 - e), p.scale), undo = kv8_pow2(e - 8) * fabsf(p.scale) * kLog2e;
+      back[nt][0] = __shfl_sync(0xffffffffu, undo, 8 * t4);
+      back[nt][1] = __shfl_sync(0xffffffffu, undo, 8 * t4 + 4);
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float u = x[4 * s + 2 * i] * f, v = x[4 * s + 2 * i + 1] * f;
+          const __half2 hd = __floats2half2_rn(u, v);
+          h[nt][s][i] = h2_bits(hd);
+          if (HL) {
+            const float2 hb = __half22float2(hd);
+            l[HL ? nt : 0][HL ? s : 0][i] = h2_bits(__floats2half2_rn(u - hb.x, v - hb.y));
+          }
+        }
+    }
   }
+};
+
+// Key (within 16) behind row g (+ 8) of a left operand of keys.
+__device__ __forceinline__ int key_row(int g) { return 4 * (g & 1) + (g >> 1); }
+
+// S^T of 16 keys (codes) against the query rows: c[nt] is (key g, rows 2t, 2t + 1),
+// (key g + 8, the same rows).
+template <int D, int FMT, bool HL, int NT>
+__device__ __forceinline__ void scores(const uint8_t* kb, const Query<D, HL, NT>& q, float (&c)[NT][4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  uint32_t w0[D / 16], w1[D / 16];
+  load_bytes<D / 4>(kb + key_row(g) * D + t4 * (D / 4), w0);
+  load_bytes<D / 4>(kb + (8 + key_row(g)) * D + t4 * (D / 4), w1);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    uint32_t a[4];
+    codes_to_h2<FMT>(w0[s], a[0], a[2]);
+    codes_to_h2<FMT>(w1[s], a[1], a[3]);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      mma16816(c[nt], a, q.h[nt][s][0], q.h[nt][s][1]);
+      if (HL) mma16816(c[nt], a, q.l[HL ? nt : 0][HL ? s : 0][0], q.l[HL ? nt : 0][HL ? s : 0][1]);
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t turn(uint32_t m) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(m));
+  return r;
 }
 
 // The last slot query row r sees; -1: none.
@@ -119,29 +165,6 @@ __device__ __forceinline__ int row_limit(const AttendParams& p, int r, int pos, 
   if (r >= p.rows || t >= cnt) return -1;
   return min(pos + t, p.limit - 1);
 }
-
-// S of 16 query rows against the 64 keys of a block (codes only): c[j] is key tile j.
-template <int D, int FMT, bool HL>
-__device__ __forceinline__ void scores(const uint8_t* kb, const uint32_t (&qh)[D / 16][4],
-                                       const uint32_t (&ql)[HL ? D / 16 : 1][4], float (&c)[8][4]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    uint32_t w[D / 16];
-    load_bytes<D / 4>(kb + (8 * j + (g & 1) * 4 + (g >> 1)) * D + t4 * (D / 4), w);
-    c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      uint32_t b0, b1;
-      codes_to_h2<FMT>(w[s], b0, b1);
-      mma16816(c[j], qh[s], b0, b1);
-      if (HL) mma16816(c[j], ql[HL ? s : 0], b0, b1);
-    }
-  }
-}
-
-// Key (within its block) behind element i of key tile j of this lane's S.
-__device__ __forceinline__ int key_of(int j, int i) { return 8 * j + 4 * (i & 1) + (threadIdx.x & 3); }
 
 // Writes the output and lse of one row's four dims: `o` is the sum against the
 // maximum mm, ll its weights' sum.
@@ -180,19 +203,22 @@ struct Cursor {
   int64_t left;    // blocks of the run in the heads after this one
 };
 
-template <int D, int FMT, bool HL>
+template <int D>
+constexpr int kRing = D == 128 ? 3 : 4;
+
+template <int D, int FMT, bool HL, int NT>
 __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_constant__ AttendParams p) {
-  constexpr int kSlot = kKv8Block * D, kSlots = D == 128 ? 3 : 4;
+  constexpr int kSlot = kKv8Block * D, kSlots = kRing<D>, kRows = 8 * NT;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) unsigned long long bars[kWarps][kSlots];
-  __shared__ float s_m[kWarps][16], s_l[kWarps][16];
-  __shared__ long long s_total;
+  __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
+  __shared__ int s_scan[kWarps];
+  __shared__ long long s_total, s_before;
   __shared__ int s_b, s_last;
-  __shared__ long long s_before;
-  float* s_join = reinterpret_cast<float*>(smem + kWarps * kSlots * kSlot);  // [2][16 * D]
+  float* s_join = reinterpret_cast<float*>(smem + kWarps * kSlots * kSlot);  // [2][kRows * D]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const int H = p.c.n_kv_heads, B = p.c.batch;
-  const int row0 = blockIdx.y * 16, rows_end = min(row0 + 16, p.rows);
+  const int row0 = blockIdx.y * kRows, rows_end = min(row0 + kRows, p.rows);
   const int64_t cta = blockIdx.x;
 
   // ------------------------------------------- this CTA's run of blocks
@@ -231,11 +257,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
       if (lane >= o) x += y;
     }
     __syncthreads();
-    if (lane == 31) s_m[warp][0] = __int_as_float(x);
+    if (lane == 31) s_scan[warp] = x;
     __syncthreads();
     long long before = base + x - mine, tile = 0;
     for (int w = 0; w < kWarps; ++w) {
-      const int n = __float_as_int(s_m[w][0]);
+      const int n = s_scan[w];
       before += w < warp ? n : 0;
       tile += n;
     }
@@ -280,7 +306,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
   __syncwarp();
   Cursor ahead = at;   // what is copied next: K of its block, then V
   bool more = true, ahead_v = false;
-  int put = 0;         // copies issued
+  int put = 0, put_at = 0;  // copies issued, and the next one's slot
   bool ok = true;
   auto find = [&] {    // to the warp's next block, if it has one left
     while (more && ahead.blk >= ahead.end) {
@@ -292,111 +318,159 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
     find();
     if (!more || !ok) return;
     if (lane == 0) {
-      const uint32_t bar = bar0 + 8 * (put % kSlots);
+      const uint32_t bar = bar0 + 8 * put_at;
       const uint8_t* src = (ahead_v ? p.c.v : p.c.k) +
                            (((int64_t)ahead.b * H + ahead.h) * p.c.max_len + (int64_t)ahead.blk * kKv8Block) * D;
       asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "n"(kSlot) : "memory");
       asm volatile(
           "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-              smem_u32(ring + put % kSlots * kSlot)),
+              smem_u32(ring) + put_at * kSlot),
           "l"(src), "n"(kSlot), "r"(bar)
           : "memory");
     }
     ++put;
+    if (++put_at == kSlots) put_at = 0;
     if (ahead_v) ahead.blk += kWarps;
     ahead_v = !ahead_v;
   };
   for (int i = 0; i < kSlots; ++i) copy();
-  int got = 0;  // copies waited for; after a wait that gave up, only those in flight
+  // copies waited for, the next one's slot and its phase; after a wait that gave up,
+  // only those in flight
+  int got = 0, got_at = 0, phase = 0;
   auto arrive = [&]() -> const uint8_t* {
-    if (got < put && !mbar_wait(bar0 + 8 * (got % kSlots), (got / kSlots) & 1)) ok = false;
-    return ring + got++ % kSlots * kSlot;
+    if (got < put && !mbar_wait(bar0 + 8 * got_at, phase)) ok = false;
+    const uint8_t* slot = ring + got_at * kSlot;
+    ++got;
+    if (++got_at == kSlots) got_at = 0, phase ^= 1;
+    return slot;
   };
 
   while (true) {
     const int64_t head = (int64_t)at.b * H + at.h;
     const int first = at.blk - warp, seg_end = at.end;  // the run's blocks in this head
     const int pos = p.pos[at.b], cnt = p.counts ? min(max(p.counts[at.b], 0), p.T) : p.T;
-    const int lim[2] = {row_limit(p, row0 + g, pos, cnt), row_limit(p, row0 + g + 8, pos, cnt)};
     const float* ksc = p.c.k_scale + head * (p.c.max_len / kKv8Block);
     const float* vsc = p.c.v_scale + head * (p.c.max_len / kKv8Block);
-    uint32_t qh[D / 16][4], ql[HL ? D / 16 : 1][4];
-    float back[2];
-    float ks = 0.0f, vs = 0.0f;
+    float ks = 0.0f, vs = 1.0f;
     if (at.blk < seg_end) {
       ks = __ldg(ksc + at.blk);
       vs = __ldg(vsc + at.blk);
     }
-    load_q<D, HL>(p, at.b, at.h, row0, qh, ql, back);
-    float o[D / 8][4] = {};
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    const int e_ref = kv8_exponent(vs);
+    Query<D, HL, NT> q;
+    q.load(p, at.b, at.h, row0);
+    float o[D / 16][NT][4] = {};
+    float m[NT][2], l[NT][2];  // of rows 2 t4, 2 t4 + 1; l: this lane's keys
+    int lim[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        m[nt][i] = -INFINITY;
+        l[nt][i] = 0.0f;
+        lim[nt][i] = row_limit(p, row0 + 8 * nt + 2 * t4 + i, pos, cnt);
+      }
 
     for (; at.blk < seg_end; at.blk += kWarps) {
-      const float f0 = back[0] * ks, f1 = back[1] * ks, vsn = vs;
+      const float kf = ks;
+      const int ev = kv8_exponent(vs);
       if (at.blk + kWarps < seg_end) {
         ks = __ldg(ksc + at.blk + kWarps);
         vs = __ldg(vsc + at.blk + kWarps);
       }
-      float c[8][4];
+      const int key0 = at.blk * kKv8Block;
+      float c[4][NT][4];
       const uint8_t* kb = arrive();
-      scores<D, FMT, HL>(kb, qh, ql, c);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) scores<D, FMT, HL, NT>(kb + 16 * mt * D, q, c[mt]);
       __syncwarp();
       copy();  // into the slot of these keys
-      const int key0 = at.blk * kKv8Block;
-      float top[2] = {-INFINITY, -INFINITY};
-      const bool whole = key0 + kKv8Block - 1 <= lim[0] && key0 + kKv8Block - 1 <= lim[1];
+      if (key0 + kKv8Block - 1 > pos + row0 / p.G || cnt < p.T || key0 + kKv8Block > p.limit) {
+        // the first row (or a row without a token) does not see all of the block
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+        for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int half = i >> 1;
-          c[j][i] *= half ? f1 : f0;
-          if (!whole && key0 + key_of(j, i) > lim[half]) c[j][i] = -INFINITY;
-          top[half] = fmaxf(top[half], c[j][i]);
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (key0 + 16 * mt + 8 * (i >> 1) + key_row(g) > lim[nt][i & 1]) c[mt][nt][i] = -INFINITY;
+      }
+      float a[NT][2];
+      bool any = false;
+      float now[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          a[nt][i] = fmaxf(q.back[nt][i] * kf, 1.2e-38f);  // above 0: a masked score times it stays -infinity
+          float t = fmaxf(c[0][nt][i], c[0][nt][i + 2]);
+#pragma unroll
+          for (int mt = 1; mt < 4; ++mt) t = fmaxf(fmaxf(t, c[mt][nt][i]), c[mt][nt][i + 2]);
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+          now[nt][i] = t > -INFINITY ? fmaf(t, a[nt][i], (float)ev) : -INFINITY;
+          any = any || now[nt][i] > m[nt][i] + kLazy || (m[nt][i] == -INFINITY && t > -INFINITY);
         }
       if (p.scores) {
         // log2 units, for the rows' attention weights
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-          if (row0 + g + 8 * half < p.rows) {
-            float* x = p.scores + (head * p.rows + row0 + g + 8 * half) * p.ld_scores + key0;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              x[key_of(j, 0)] = c[j][2 * half];
-              x[key_of(j, 1)] = c[j][2 * half + 1];
+          for (int i = 0; i < 2; ++i)
+            if (row0 + 8 * nt + 2 * t4 + i < p.rows) {
+              float* x = p.scores + (head * p.rows + row0 + 8 * nt + 2 * t4 + i) * p.ld_scores + key0 + key_row(g);
+#pragma unroll
+              for (int mt = 0; mt < 4; ++mt) {
+                x[16 * mt] = c[mt][nt][i] * a[nt][i];
+                x[16 * mt + 8] = c[mt][nt][i + 2] * a[nt][i];
+              }
             }
-          }
       }
-      float alpha[2];
+      if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
-        top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
-        const float now = fmaxf(m[half], top[half]);
-        alpha[half] = m[half] == -INFINITY ? 0.0f : exp2a(m[half] - now);
-        m[half] = now;
-        l[half] *= alpha[half];
+        for (int nt = 0; nt < NT; ++nt) {
+          float alpha[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float to = fmaxf(m[nt][i], now[nt][i]);
+            alpha[i] = m[nt][i] == -INFINITY ? 0.0f : exp2a(m[nt][i] - to);
+            m[nt][i] = to;
+            l[nt][i] *= alpha[i];
+          }
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[j][nt][i] *= alpha[i & 1];
+        }
       }
-      const float sub[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-      float pv[D / 8][4] = {};
+      const float back_l = kv8_pow2(min(max(e_ref - ev, -100), 100));
       const uint8_t* vb = arrive();
       const bool tail = key0 + kKv8Block > at.last + 1;  // the block ends past the last visible slot
+      float pv[HL ? D / 16 : 1][HL ? NT : 1][4] = {};
+      float sum[NT][2] = {};
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        uint32_t ph[4], pl[4];
+        uint32_t ph[NT][2], pl[HL ? NT : 1][2];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {  // A registers: (tile 2s, rows g / g+8), (tile 2s+1, rows g / g+8)
-          const int j = 2 * s + (q >> 1), half = q & 1;
-          const float e0 = exp2a(c[j][2 * half] - sub[half]), e1 = exp2a(c[j][2 * half + 1] - sub[half]);
-          l[half] += e0 + e1;
-          const __half2 h = __floats2half2_rn(e0, e1);
-          ph[q] = h2_bits(h);
-          if (HL) {
-            const float2 hb = __half22float2(h);
-            pl[q] = h2_bits(__floats2half2_rn(e0 - hb.x, e1 - hb.y));
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float e[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float add = (float)ev - (m[nt][i] == -INFINITY ? 0.0f : m[nt][i]);
+              e[i] = exp2a(fmaf(c[s][nt][2 * half + i], a[nt][i], add));
+              sum[nt][i] += e[i];
+            }
+            const __half2 h = __floats2half2_rn(e[0], e[1]);
+            ph[nt][half] = turn(h2_bits(h));
+            if (HL) {
+              const float2 hb = __half22float2(h);
+              pl[HL ? nt : 0][half] = turn(h2_bits(__floats2half2_rn(e[0] - hb.x, e[1] - hb.y)));
+            }
           }
-        }
-        constexpr int NB = D / 8;  // bytes of a row this lane feeds
+        constexpr int NB = D / 8;  // bytes of a key row this lane feeds
         uint32_t w[4][(NB + 3) / 4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -411,94 +485,112 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
         for (int z = 0; z < (NB + 3) / 4; ++z)
 #pragma unroll
           for (int y = 0; y < (NB < 4 ? 1 : 2); ++y) {
-            // keys' bytes side by side: dims 4z + 2y and 4z + 2y + 1
+            // keys' bytes side by side: dims 4z + 2y and 4z + 2y + 1, rows g and g + 8 of the operand
             const uint32_t sel = y ? 0x7362u : 0x5140u;
-            const uint32_t a = __byte_perm(w[0][z], w[1][z], sel), d = __byte_perm(w[2][z], w[3][z], sel);
-            uint32_t a0, a1, d0, d1;
-            codes_to_h2<FMT>(a, a0, a1);
-            codes_to_h2<FMT>(d, d0, d1);
-            const int n = 4 * z + 2 * y;
-            mma16816(pv[n], ph, a0, d0);
-            mma16816(pv[n + 1], ph, a1, d1);
-            if (HL) {
-              mma16816(pv[n], pl, a0, d0);
-              mma16816(pv[n + 1], pl, a1, d1);
+            uint32_t va[4];
+            codes_to_h2<FMT>(__byte_perm(w[0][z], w[1][z], sel), va[0], va[1]);
+            codes_to_h2<FMT>(__byte_perm(w[2][z], w[3][z], sel), va[2], va[3]);
+            const int j = 2 * z + y;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (HL) {
+                mma16816(pv[HL ? j : 0][HL ? nt : 0], va, ph[nt][0], ph[nt][1]);
+                mma16816(pv[HL ? j : 0][HL ? nt : 0], va, pl[HL ? nt : 0][0], pl[HL ? nt : 0][1]);
+              } else {
+                mma16816(o[j][nt], va, ph[nt][0], ph[nt][1]);
+              }
             }
           }
       }
       __syncwarp();
       copy();  // into the slot of these values
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n)
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][i] = fmaf(pv[n][i], vsn, o[n][i] * alpha[i >> 1]);
+        for (int i = 0; i < 2; ++i) l[nt][i] = fmaf(sum[nt][i], back_l, l[nt][i]);
+        if (HL)
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[j][nt][i] += pv[HL ? j : 0][HL ? nt : 0][i];
+      }
     }
 
     // join the warps: 2 and 3 into 0 and 1, then 1 into 0
+    const float undo = kv8_pow2(-e_ref);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-    }
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float v = l[nt][i] * undo;
+        v += __shfl_xor_sync(0xffffffffu, v, 4);
+        v += __shfl_xor_sync(0xffffffffu, v, 8);
+        l[nt][i] = v + __shfl_xor_sync(0xffffffffu, v, 16);
+      }
 #pragma unroll
     for (int step = kWarps / 2; step > 0; step >>= 1) {
       if (warp >= step && warp < 2 * step) {
-        float* to = s_join + (warp - step) * 16 * D;
+        float* to = s_join + (warp - step) * kRows * D;
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n)
+        for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) to[(n * 4 + i) * 32 + lane] = o[n][i];
-        if (t4 == 0) {
-          s_m[warp][g] = m[0], s_m[warp][g + 8] = m[1];
-          s_l[warp][g] = l[0], s_l[warp][g + 8] = l[1];
-        }
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[((j * NT + nt) * 4 + i) * 32 + lane] = o[j][nt][i];
+        if (g == 0)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              s_m[warp][8 * nt + 2 * t4 + i] = m[nt][i];
+              s_l[warp][8 * nt + 2 * t4 + i] = l[nt][i];
+            }
       }
       __syncthreads();
       if (warp < step) {
-        const float* from = s_join + warp * 16 * D;
-        float a[2], c[2];
+        const float* from = s_join + warp * kRows * D;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float om = s_m[warp + step][g + 8 * half], now = fmaxf(m[half], om);
-          a[half] = m[half] == -INFINITY ? 0.0f : exp2a(m[half] - now);
-          c[half] = om == -INFINITY ? 0.0f : exp2a(om - now);
-          l[half] = l[half] * a[half] + s_l[warp + step][g + 8 * half] * c[half];
-          m[half] = now;
+        for (int nt = 0; nt < NT; ++nt) {
+          float mine[2], theirs[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float om = s_m[warp + step][8 * nt + 2 * t4 + i], to = fmaxf(m[nt][i], om);
+            mine[i] = m[nt][i] == -INFINITY ? 0.0f : exp2a(m[nt][i] - to);
+            theirs[i] = om == -INFINITY ? 0.0f : exp2a(om - to);
+            l[nt][i] = l[nt][i] * mine[i] + s_l[warp + step][8 * nt + 2 * t4 + i] * theirs[i];
+            m[nt][i] = to;
+          }
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              o[j][nt][i] = o[j][nt][i] * mine[i & 1] + from[((j * NT + nt) * 4 + i) * 32 + lane] * theirs[i & 1];
         }
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            o[n][i] = o[n][i] * a[i >> 1] + from[(n * 4 + i) * 32 + lane] * c[i >> 1];
       }
       __syncthreads();
     }
     // parts of this head: from the CTA with its first block to the one with its last
     const int64_t head_u = u0 + (u1 - u0) - at.left - (seg_end - first) - first;  // its first block's number
     const int64_t c0 = ((head_u + 1) * ctas - 1) / all, c1 = ((head_u + at.blocks) * ctas - 1) / all;
-    const int64_t slot = (cta + head) * 16;
+    const int64_t slot = (int64_t)blockIdx.y * p.part_rows + (cta + head) * kRows;
     if (warp == 0) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int rr = g + 8 * half, r = row0 + rr;
-        if (r >= p.rows) continue;
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
+          const int rr = 8 * nt + 2 * t4 + i;
+          if (row0 + rr >= p.rows) continue;
+          float* to = p.part_o + (slot + rr) * D + g * (D / 8);
+          if constexpr (D >= 32) {
 #pragma unroll
-          for (int n = 0; n < D / 8; n += (D / 8 < 4 ? 2 : 4)) {
-            const int d = (2 * t4 + i) * (D / 8) + n;
-            if constexpr (D / 8 >= 4) {
-              const float4 v = make_float4(o[n][2 * half + i], o[n + 1][2 * half + i], o[n + 2][2 * half + i], o[n + 3][2 * half + i]);
-              *reinterpret_cast<float4*>(p.part_o + ((int64_t)blockIdx.y * p.part_rows + slot + rr) * D + d) = v;
-            } else {
-              *reinterpret_cast<float2*>(p.part_o + ((int64_t)blockIdx.y * p.part_rows + slot + rr) * D + d) =
-                  make_float2(o[n][2 * half + i], o[n + 1][2 * half + i]);
-            }
+            for (int j = 0; j < D / 16; j += 2)
+              *reinterpret_cast<float4*>(to + 2 * j) =
+                  make_float4(o[j][nt][i], o[j][nt][i + 2], o[j + 1][nt][i], o[j + 1][nt][i + 2]);
+          } else {
+            *reinterpret_cast<float2*>(to) = make_float2(o[0][nt][i], o[0][nt][i + 2]);
           }
-        if (t4 == 0)
-          *reinterpret_cast<float2*>(p.part_ml + ((int64_t)blockIdx.y * p.part_rows + slot + rr) * 2) =
-              make_float2(m[half], l[half]);
-      }
+          if (g == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + rr) * 2) = make_float2(m[nt][i], l[nt][i]);
+        }
       __threadfence();
     }
     __syncthreads();
@@ -511,19 +603,19 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
     __syncthreads();
     if (s_last) {
       __threadfence();
-      const int64_t part0 = (int64_t)blockIdx.y * p.part_rows + (c0 + head) * 16;
+      const int64_t part0 = (int64_t)blockIdx.y * p.part_rows + (c0 + head) * kRows;
       const int parts = (int)(c1 - c0) + 1, rows = rows_end - row0;
       for (int e = tid; e < rows * (D / 4); e += kWarps * 32) {
         const int rr = e / (D / 4), d = e % (D / 4) * 4;
         float mm = -INFINITY;
-        for (int q = 0; q < parts; ++q) mm = fmaxf(mm, __ldcg(p.part_ml + 2 * (part0 + 16 * q + rr)));
+        for (int k = 0; k < parts; ++k) mm = fmaxf(mm, __ldcg(p.part_ml + 2 * (part0 + kRows * k + rr)));
         float ll = 0.0f;
         float4 oo = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (mm > -INFINITY) {
 #pragma unroll 4
-          for (int q = 0; q < parts; ++q) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + part0 + 16 * q + rr);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (part0 + 16 * q + rr) * D + d));
+          for (int k = 0; k < parts; ++k) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + part0 + kRows * k + rr);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (part0 + kRows * k + rr) * D + d));
             const float f = exp2a(ml.x - mm);
             ll = fmaf(ml.y, f, ll);
             oo.x = fmaf(v.x, f, oo.x), oo.y = fmaf(v.y, f, oo.y);
@@ -573,7 +665,9 @@ __global__ void __launch_bounds__(256) kv8_scores_mass_kernel(const __grid_const
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int r = 0; r < p.rows; ++r) {
     const float lse = p.lse[((int64_t)b * p.T + r / p.G) * (p.G * p.c.n_kv_heads) + hk * p.G + r % p.G] * kLog2e;
-    if (lse == -INFINITY) continue;  // its scores were not all written
+    const int t = r / p.G;
+    // past a row's last slot its scores were not all written
+    if (key > p.pos[b] + t || t >= (p.counts ? min(p.counts[b], p.T) : p.T)) continue;
     const float4 x = *reinterpret_cast<const float4*>(p.scores + (head * p.rows + r) * p.ld_scores + key);
     sum.x += exp2a(x.x - lse), sum.y += exp2a(x.y - lse);
     sum.z += exp2a(x.z - lse), sum.w += exp2a(x.w - lse);
@@ -586,90 +680,98 @@ __global__ void __launch_bounds__(256) kv8_scores_mass_kernel(const __grid_const
 }
 
 // mass_j += sum_r exp(x[r][j] - lse_r): a warp owns a block of 64 keys and walks
-// the head's query rows 16 at a time, so every slot has one writer and one order.
-template <int D, int FMT, bool HL>
+// the head's query rows 8 NT at a time, so every slot has one writer and one order.
+template <int D, int FMT, bool HL, int NT>
 __global__ void __launch_bounds__(kWarps * 32) kv8_mass_kernel(const __grid_constant__ AttendParams p) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
   const int hk = blockIdx.y % p.c.n_kv_heads, b = blockIdx.y / p.c.n_kv_heads;
   const int pos = p.pos[b], cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
   const int last = cnt > 0 ? min(pos + cnt, p.limit) - 1 : -1;
   const int64_t head = (int64_t)b * p.c.n_kv_heads + hk;
-  for (int blk = blockIdx.x * kWarps + warp; blk * kKv8Block <= last; blk += gridDim.x * kWarps) {
-    const int key0 = blk * kKv8Block;
-    const uint8_t* kb = p.c.k + (head * p.c.max_len + key0) * D;
-    const float ks = p.c.k_scale[head * (p.c.max_len / kKv8Block) + blk];
-    float sum[8][2] = {};
-    const int first_t = max(0, key0 - pos);  // rows of earlier tokens do not see this block
-    for (int row0 = first_t * p.G / 16 * 16; row0 < cnt * p.G; row0 += 16) {
-      uint32_t qh[D / 16][4], ql[HL ? D / 16 : 1][4];
-      float back[2], lse[2];
-      load_q<D, HL>(p, b, hk, row0, qh, ql, back);
-      int lim[2];
+  const int blk = blockIdx.x * kWarps + warp, key0 = blk * kKv8Block;
+  if (key0 > last) return;
+  const uint8_t* kb = p.c.k + (head * p.c.max_len + key0) * D;
+  const float ks = p.c.k_scale[head * (p.c.max_len / kKv8Block) + blk];
+  float sum[4][2] = {};                    // keys g and g + 8 of each 16
+  const int first_t = max(0, key0 - pos);  // rows of earlier tokens do not see this block
+  for (int row0 = first_t * p.G / (8 * NT) * (8 * NT); row0 < cnt * p.G; row0 += 8 * NT) {
+    Query<D, HL, NT> q;
+    q.load(p, b, hk, row0);
+    float lse[NT][2];
+    int lim[NT][2];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = row0 + g + 8 * half;
-        lim[half] = row_limit(p, r, pos, cnt);
-        lse[half] = 0.0f;
-        if (lim[half] >= 0)
-          lse[half] = p.lse[((int64_t)b * p.T + r / p.G) * (p.G * p.c.n_kv_heads) + hk * p.G + r % p.G] * kLog2e;
-      }
-      float c[8][4];
-      scores<D, FMT, HL>(kb, qh, ql, c);
-      const float f[2] = {back[0] * ks, back[1] * ks};
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int half = i >> 1;
-          if (key0 + key_of(j, i) <= lim[half]) sum[j][i & 1] += exp2a(fmaf(c[j][i], f[half], -lse[half]));
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float v = sum[j][i];
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        const int key = key0 + key_of(j, i);
-        if (g == 0 && key <= last) p.c.mass[head * p.c.max_len + key] += v;
+        const int r = row0 + 8 * nt + 2 * t4 + i;
+        lim[nt][i] = row_limit(p, r, pos, cnt);
+        lse[nt][i] = 0.0f;
+        if (lim[nt][i] >= 0)
+          lse[nt][i] = p.lse[((int64_t)b * p.T + r / p.G) * (p.G * p.c.n_kv_heads) + hk * p.G + r % p.G] * kLog2e;
       }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      float c[NT][4];
+      scores<D, FMT, HL, NT>(kb + 16 * mt * D, q, c);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key0 + 16 * mt + 8 * (i >> 1) + key_row(g) <= lim[nt][i & 1])
+            sum[mt][i >> 1] += exp2a(fmaf(c[nt][i], q.back[nt][i & 1] * ks, -lse[nt][i & 1]));
+    }
   }
+#pragma unroll
+  for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float v = sum[mt][half];
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      const int key = key0 + 16 * mt + 8 * half + key_row(g);
+      if (t4 == 0 && key <= last) p.c.mass[head * p.c.max_len + key] += v;
+    }
 }
 
+// The decode form's kernels of a call, and their shared memory.
+struct Form {
+  void (*attend)(AttendParams);
+  void (*mass)(AttendParams);
+  int rows, smem;  // query rows of a CTA
+};
+
+template <int D, int FMT, bool HL, int NT>
+Form form_of() {
+  return {kv8_attend_kernel<D, FMT, HL, NT>, kv8_mass_kernel<D, FMT, HL, NT>, 8 * NT,
+          kWarps * kRing<D> * kKv8Block * D + 2 * 8 * NT * D * (int)sizeof(float)};
+}
+
+// As many query rows to a CTA as there are, up to what its registers hold: 32 rows
+// of 64 dims, 16 of 128 (half with heads and tails).
 template <int D, int FMT, bool HL>
-int launch_dfh(const AttendParams& p, int bh, int longest, cudaStream_t st) {
-  if (p.row_tiles > 0) {
-    if (const int rc = kv8_prompt_launch(p, bh, st)) return rc;
-    if (p.splits > 1) {
-      kv8_join_kernel<<<dim3(p.rows, bh), D / 4, 0, st>>>(p);
-      count_launch();
-    }
-    if (p.add_mass) return kv8_prompt_mass_launch(p, bh, longest, st);
-  } else {
-    const int smem = kWarps * (D == 128 ? 3 : 4) * kKv8Block * D + 2 * 16 * D * (int)sizeof(float);
-    auto fn = kv8_attend_kernel<D, FMT, HL>;
-    if (const int rc = ensure_smem_attr((const void*)fn, smem)) return rc;
-    fn<<<dim3(p.splits, ceil_div(p.rows, 16)), kWarps * 32, smem, st>>>(p);
-    count_launch();
-    if (p.scores) {
-      kv8_scores_mass_kernel<<<dim3(ceil_div(longest, 1024), bh), 256, 0, st>>>(p);
-      count_launch();
-    } else if (p.add_mass) {
-      kv8_mass_kernel<D, FMT, HL><<<dim3(ceil_div(longest, kWarps * kKv8Block), bh), kWarps * 32, 0, st>>>(p);
-      count_launch();
-    }
-  }
-  return cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
+Form form_of(int rows) {
+  constexpr int kMost = (D == 128 ? 2 : 4) / (HL && D >= 64 ? 2 : 1);
+  if constexpr (kMost >= 4)
+    if (rows > 16) return form_of<D, FMT, HL, 4>();
+  if constexpr (kMost >= 2)
+    if (rows > 8) return form_of<D, FMT, HL, 2>();
+  return form_of<D, FMT, HL, 1>();
 }
 
 template <int D>
-int launch_d(const AttendParams& p, int bh, int longest, cudaStream_t st) {
-  const bool e = p.c.format == CB_KV8_E4M3, hl = p.dtype == CB_F32;
-  if (e && hl) return launch_dfh<D, CB_KV8_E4M3, true>(p, bh, longest, st);
-  if (e) return launch_dfh<D, CB_KV8_E4M3, false>(p, bh, longest, st);
-  if (hl) return launch_dfh<D, CB_KV8_INT8, true>(p, bh, longest, st);
-  return launch_dfh<D, CB_KV8_INT8, false>(p, bh, longest, st);
+Form form_of(int format, bool hl, int rows) {
+  if (format == CB_KV8_E4M3) return hl ? form_of<D, CB_KV8_E4M3, true>(rows) : form_of<D, CB_KV8_E4M3, false>(rows);
+  return hl ? form_of<D, CB_KV8_INT8, true>(rows) : form_of<D, CB_KV8_INT8, false>(rows);
+}
+
+Form form_of(const CbKv8& c, int dtype, int rows) {
+  const bool hl = dtype == CB_F32;
+  switch (c.head_dim) {
+    case 16: return form_of<16>(c.format, hl, rows);
+    case 32: return form_of<32>(c.format, hl, rows);
+    case 64: return form_of<64>(c.format, hl, rows);
+    default: return form_of<128>(c.format, hl, rows);
+  }
 }
 
 // How a call is cut up, and where its parts lie in the scratch.  The counters come
@@ -705,13 +807,17 @@ Plan plan_of(const CbKv8& c, int dtype, int n_q_heads, int T, int longest, bool 
     }
     parts = (int64_t)bh * pl.rows * pl.splits;
   } else {
-    // CTAs that are resident at once (three to an SM of 48 KB rings, two of 96), at
-    // least one block of 64 keys for each warp, and no more than 48 parts a head
-    const int blocks = ceil_div(pl.rows, 16);
-    const int64_t fit = std::max(1, num_sms() * (c.head_dim == 128 ? 2 : 3) / blocks);
+    // CTAs that are resident at once, at least one block of 64 keys for each warp,
+    // and no more than 48 parts a head
+    const Form f = form_of(c, dtype, pl.rows);
+    int resident = 1;  // without a device: only the layout is asked for
+    if (ensure_smem_attr((const void*)f.attend, f.smem) == CB_OK)
+      resident = std::max(1, resident_ctas((const void*)f.attend, kWarps * 32, f.smem));
+    const int blocks = ceil_div(pl.rows, f.rows);
+    const int64_t fit = std::max(1, num_sms() * resident / blocks);
     const int64_t work = std::max<int64_t>(1, (int64_t)bh * ceil_div(longest, kKv8Block) / kWarps);
     pl.splits = (int)std::min(std::min(fit, work), (int64_t)bh * 48);
-    pl.part_rows = ((int64_t)bh + pl.splits) * 16;
+    pl.part_rows = ((int64_t)bh + pl.splits) * f.rows;
     parts = pl.part_rows * blocks;
     // rows' scores cost 8 bytes a key to write and read, taking them again head_dim
     if (add_mass && pl.rows * 8 <= c.head_dim) pl.ld_scores = ceil_div(longest, kKv8Block) * kKv8Block;
@@ -730,9 +836,9 @@ int check_call(const CbKv8* c, int dtype, int n_q_heads, int T, int longest) {
   if (n_q_heads <= 0 || n_q_heads % c->n_kv_heads) return CB_ERR_SHAPE;
   const int64_t rows = (int64_t)T * (n_q_heads / c->n_kv_heads);
   if (rows > 65535 * 16) return CB_ERR_SHAPE;
-  // a counter for each head and 16 rows
+  // a counter for each head and 8 rows
   if ((rows <= 32 || dtype == CB_F32 || c->head_dim < 64) &&
-      (rows + 15) / 16 * c->batch * c->n_kv_heads > (int64_t)kCounters)
+      (rows + 7) / 8 * c->batch * c->n_kv_heads > (int64_t)kCounters)
     return CB_ERR_SHAPE;
   return CB_OK;
 }
@@ -788,10 +894,25 @@ extern "C" int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const
   p.status = status;
   const int bh = c->batch * c->n_kv_heads;
   cudaStream_t st = (cudaStream_t)stream;
-  switch (c->head_dim) {
-    case 16: return launch_d<16>(p, bh, longest, st);
-    case 32: return launch_d<32>(p, bh, longest, st);
-    case 64: return launch_d<64>(p, bh, longest, st);
-    default: return launch_d<128>(p, bh, longest, st);
+  if (p.row_tiles > 0) {
+    if (const int rc = kv8_prompt_launch(p, bh, st)) return rc;
+    if (p.splits > 1) {
+      kv8_join_kernel<<<dim3(p.rows, bh), c->head_dim / 4, 0, st>>>(p);
+      count_launch();
+    }
+    if (p.add_mass) return kv8_prompt_mass_launch(p, bh, longest, st);
+  } else {
+    const Form f = form_of(*c, dtype, p.rows);
+    if (const int rc = ensure_smem_attr((const void*)f.attend, f.smem)) return rc;
+    f.attend<<<dim3(p.splits, ceil_div(p.rows, f.rows)), kWarps * 32, f.smem, st>>>(p);
+    count_launch();
+    if (p.scores) {
+      kv8_scores_mass_kernel<<<dim3(ceil_div(longest, 1024), bh), 256, 0, st>>>(p);
+      count_launch();
+    } else if (p.add_mass) {
+      f.mass<<<dim3(ceil_div(longest, kWarps * kKv8Block), bh), kWarps * 32, 0, st>>>(p);
+      count_launch();
+    }
   }
+  return cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
 }

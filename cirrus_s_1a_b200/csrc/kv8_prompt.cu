@@ -139,38 +139,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&u)[16]
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 16 codes as f16 operand values: int8 as they are, E4M3 divided by 256, which
-// moves its bits without arithmetic (the hardware converter shares its unit with
-// the exponentials).  Pieces that hold a NaN go through the converter.
+// 16 codes as f16 operand values.
 template <int FMT>
 __device__ __forceinline__ void to_operand(uint4 c, uint4& lo, uint4& hi) {
-  if (FMT == CB_KV8_INT8) {
-    codes_to_h2<FMT>(c.x, lo.x, lo.y);
-    codes_to_h2<FMT>(c.y, lo.z, lo.w);
-    codes_to_h2<FMT>(c.z, hi.x, hi.y);
-    codes_to_h2<FMT>(c.w, hi.z, hi.w);
-    return;
-  }
-  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-  uint32_t u[8], nan = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    nan |= (w[i] & 0x7F7F7F7Fu) + 0x01010101u;
-    const uint32_t x = __byte_perm(w[i], 0u, 0x1404), y = __byte_perm(w[i], 0u, 0x3424);
-    u[2 * i] = (x >> 1 & 0x3F803F80u) | (x & 0x80008000u);
-    u[2 * i + 1] = (y >> 1 & 0x3F803F80u) | (y & 0x80008000u);
-  }
-  if (nan & 0x80808080u) {
-    const __half2 f = __float2half2_rn(1.0f / 256.0f);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      codes_to_h2<FMT>(w[i], u[2 * i], u[2 * i + 1]);
-      u[2 * i] = h2_bits(__hmul2(bits_h2(u[2 * i]), f));
-      u[2 * i + 1] = h2_bits(__hmul2(bits_h2(u[2 * i + 1]), f));
-    }
-  }
-  lo = make_uint4(u[0], u[1], u[2], u[3]);
-  hi = make_uint4(u[4], u[5], u[6], u[7]);
+  codes_to_h2<FMT>(c.x, lo.x, lo.y);
+  codes_to_h2<FMT>(c.y, lo.z, lo.w);
+  codes_to_h2<FMT>(c.z, hi.x, hi.y);
+  codes_to_h2<FMT>(c.w, hi.z, hi.w);
 }
 
 // The last slot row r of a KV head sees (rows of padding tokens: -1).
@@ -301,8 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       const float* vsc = p.c.v_scale + head * (p.c.max_len / kKv8Block);
       const int vis = last / kKv8Block;  // the last block any row sees
       float m = -INFINITY, l = 0.0f;
-      constexpr float kCode = FMT == CB_KV8_E4M3 ? 256.0f : 1.0f;  // the operands hold codes / kCode
-      const int e_ref = n > 0 ? kv8_exponent(vsc[kHalves * beg] * kCode) : 0;
+      const int e_ref = n > 0 ? kv8_exponent(vsc[kHalves * beg]) : 0;
       float ks[kHalves], vs[kHalves];
       auto scales = [&](int j) {
 #pragma unroll
@@ -319,8 +293,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         int ev[kHalves];
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
-          a[h] = fmaxf(back * (ks[h] * kCode), 1.2e-38f);  // above 0: a masked score times it stays -infinity
-          ev[h] = kv8_exponent(vs[h] * kCode);
+          a[h] = fmaxf(back * ks[h], 1.2e-38f);  // above 0: a masked score times it stays -infinity
+          ev[h] = kv8_exponent(vs[h]);
         }
         if (j + 1 < n) scales(j + 1);
         if (!wait(s_full + 8 * tile, j)) break;
@@ -574,7 +548,6 @@ struct Mass {
 template <int D, int FMT>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __grid_constant__ AttendParams p) {
   using C = Mass<D>;
-  constexpr float kCode = FMT == CB_KV8_E4M3 ? 256.0f : 1.0f;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sk = smem_raw + (-smem_u32(smem_raw) & 1023);
   uint8_t* sq = sk + C::kQ;
@@ -635,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
   if (warp < kSoftWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     const int group = warp / 4, key = key0 + (warp % 4) * 32 + lane;
-    const float ks = p.c.k_scale[head * (p.c.max_len / kKv8Block) + min(key, last) / kKv8Block] * kCode;
+    const float ks = p.c.k_scale[head * (p.c.max_len / kKv8Block) + min(key, last) / kKv8Block];
     const f32x2 ks2 = pack2(ks, ks);
     f32x2 sum[2] = {0, 0};
     for (int k = group; k < n; k += 2) {
