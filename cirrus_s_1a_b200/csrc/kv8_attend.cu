@@ -204,10 +204,13 @@ struct Cursor {
 };
 
 template <int D>
-constexpr int kRing = D == 128 ? 3 : 4;
+constexpr int kRing = D == 128 ? 2 : 3;
+// CTAs of an SM to aim at
+template <int D, bool HL, int NT>
+constexpr int kResident = HL || NT == 4 ? 1 : D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
 
 template <int D, int FMT, bool HL, int NT>
-__global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_constant__ AttendParams p) {
+__global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_kernel(const __grid_constant__ AttendParams p) {
   constexpr int kSlot = kKv8Block * D, kSlots = kRing<D>, kRows = 8 * NT;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) unsigned long long bars[kWarps][kSlots];
@@ -308,19 +311,21 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
   bool more = true, ahead_v = false;
   int put = 0, put_at = 0;  // copies issued, and the next one's slot
   bool ok = true;
-  auto find = [&] {    // to the warp's next block, if it has one left
-    while (more && ahead.blk >= ahead.end) {
-      if (ahead.left > 0) next_head(ahead);
-      else more = false;
-    }
-  };
+  int64_t ahead_at = 0;  // its block in k and v
+  auto locate = [&] { ahead_at = (((int64_t)ahead.b * H + ahead.h) * p.c.max_len + (int64_t)ahead.blk * kKv8Block) * D; };
+  locate();
   auto copy = [&] {
-    find();
+    if (ahead.blk >= ahead.end) {  // to the warp's next block, if it has one left
+      while (more && ahead.blk >= ahead.end) {
+        if (ahead.left > 0) next_head(ahead);
+        else more = false;
+      }
+      locate();
+    }
     if (!more || !ok) return;
     if (lane == 0) {
       const uint32_t bar = bar0 + 8 * put_at;
-      const uint8_t* src = (ahead_v ? p.c.v : p.c.k) +
-                           (((int64_t)ahead.b * H + ahead.h) * p.c.max_len + (int64_t)ahead.blk * kKv8Block) * D;
+      const uint8_t* src = (ahead_v ? p.c.v : p.c.k) + ahead_at;
       asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "n"(kSlot) : "memory");
       asm volatile(
           "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -330,7 +335,10 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
     }
     ++put;
     if (++put_at == kSlots) put_at = 0;
-    if (ahead_v) ahead.blk += kWarps;
+    if (ahead_v) {
+      ahead.blk += kWarps;
+      ahead_at += kWarps * kSlot;
+    }
     ahead_v = !ahead_v;
   };
   for (int i = 0; i < kSlots; ++i) copy();
@@ -371,6 +379,8 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
         lim[nt][i] = row_limit(p, row0 + 8 * nt + 2 * t4 + i, pos, cnt);
       }
 
+    // blocks that end by here are seen whole by every row
+    const int seen = cnt < p.T ? -1 : min(pos + row0 / p.G, p.limit - 1);
     for (; at.blk < seg_end; at.blk += kWarps) {
       const float kf = ks;
       const int ev = kv8_exponent(vs);
@@ -385,7 +395,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
       for (int mt = 0; mt < 4; ++mt) scores<D, FMT, HL, NT>(kb + 16 * mt * D, q, c[mt]);
       __syncwarp();
       copy();  // into the slot of these keys
-      if (key0 + kKv8Block - 1 > pos + row0 / p.G || cnt < p.T || key0 + kKv8Block > p.limit) {
+      if (key0 + kKv8Block - 1 > seen) {
         // the first row (or a row without a token) does not see all of the block
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
@@ -395,9 +405,10 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
             for (int i = 0; i < 4; ++i)
               if (key0 + 16 * mt + 8 * (i >> 1) + key_row(g) > lim[nt][i & 1]) c[mt][nt][i] = -INFINITY;
       }
-      float a[NT][2];
+      // the largest x + e of this lane's keys: only where one passes m' by 2^kLazy do
+      // the lanes of a row compare
+      float a[NT][2], now[NT][2];
       bool any = false;
-      float now[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -406,11 +417,8 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
           float t = fmaxf(c[0][nt][i], c[0][nt][i + 2]);
 #pragma unroll
           for (int mt = 1; mt < 4; ++mt) t = fmaxf(fmaxf(t, c[mt][nt][i]), c[mt][nt][i + 2]);
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-          now[nt][i] = t > -INFINITY ? fmaf(t, a[nt][i], (float)ev) : -INFINITY;
-          any = any || now[nt][i] > m[nt][i] + kLazy || (m[nt][i] == -INFINITY && t > -INFINITY);
+          now[nt][i] = fmaf(t, a[nt][i], (float)ev);
+          any = any || now[nt][i] > m[nt][i] + kLazy;  // -infinity passes nothing, anything passes -infinity
         }
       if (p.scores) {
         // log2 units, for the rows' attention weights
@@ -433,7 +441,10 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
           float alpha[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float to = fmaxf(m[nt][i], now[nt][i]);
+            float to = now[nt][i];
+            to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 4));
+            to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 8));
+            to = fmaxf(m[nt][i], fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 16)));
             alpha[i] = m[nt][i] == -INFINITY ? 0.0f : exp2a(m[nt][i] - to);
             m[nt][i] = to;
             l[nt][i] *= alpha[i];
@@ -445,6 +456,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
         }
       }
       const float back_l = kv8_pow2(min(max(e_ref - ev, -100), 100));
+      float add[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) add[nt][i] = (float)ev - (m[nt][i] == -INFINITY ? 0.0f : m[nt][i]);
       const uint8_t* vb = arrive();
       const bool tail = key0 + kKv8Block > at.last + 1;  // the block ends past the last visible slot
       float pv[HL ? D / 16 : 1][HL ? NT : 1][4] = {};
@@ -459,8 +475,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attend_kernel(const __grid_co
             float e[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const float add = (float)ev - (m[nt][i] == -INFINITY ? 0.0f : m[nt][i]);
-              e[i] = exp2a(fmaf(c[s][nt][2 * half + i], a[nt][i], add));
+              e[i] = exp2a(fmaf(c[s][nt][2 * half + i], a[nt][i], add[nt][i]));
               sum[nt][i] += e[i];
             }
             const __half2 h = __floats2half2_rn(e[0], e[1]);
