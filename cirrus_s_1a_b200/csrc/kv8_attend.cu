@@ -99,11 +99,35 @@ struct Query {
       const bool live = r < p.rows;
       const int t = r / p.G, hq = hk * p.G + r % p.G;
       const int64_t base = (int64_t)b * p.qs[0] + (int64_t)t * p.qs[1] + hq * p.qs[2] + t4 * (D / 4);
+      if (D >= 32 && p.q_wide) {  // rows of 16-byte pieces
+        if (HL) {
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) {
-        x[i] = live ? kv8_load(p.q, base + i, p.dtype) : 0.0f;
-        top = fmaxf(top, fabsf(x[i]));
+          for (int i = 0; i < D / 16; ++i) {
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (live) v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + base) + i);
+            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+          }
+        } else {
+          uint32_t w[D / 8];
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (live) v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + base) + i);
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+          }
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const float2 f = p.dtype == CB_BF16 ? make_float2(bf16_to_f32(w[i]), __uint_as_float(w[i] & 0xFFFF0000u))
+                                                : __half22float2(bits_h2(w[i]));
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) x[i] = live ? kv8_load(p.q, base + i, p.dtype) : 0.0f;
       }
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       int e = 0;  // top in [2^e, 2^(e+1)); rows of zeros, infinities and the ends of the range keep e = 0
@@ -216,8 +240,8 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
   __shared__ __align__(8) unsigned long long bars[kWarps][kSlots];
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
   __shared__ int s_scan[kWarps];
-  __shared__ long long s_total, s_before;
-  __shared__ int s_b, s_last;
+  __shared__ long long s_before;
+  __shared__ int s_b, s_blocks, s_slot, s_last;
   float* s_join = reinterpret_cast<float*>(smem + kWarps * kSlots * kSlot);  // [2][kRows * D]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const int H = p.c.n_kv_heads, B = p.c.batch;
@@ -225,16 +249,36 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
   const int64_t cta = blockIdx.x;
 
   // ------------------------------------------- this CTA's run of blocks
-  if (tid == 0) s_total = 0;
-  __syncthreads();
-  {
-    long long mine = 0;
-    int last;
-    for (int b = tid; b < B; b += kWarps * 32) mine += visible_blocks(p, b, row0, rows_end, last);
-    if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(&s_total), (unsigned long long)mine);
+  // blocks (of one head) of the sequences before a thread's one in a tile of them
+  auto scan = [&](int mine, long long& tile) {
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) s_scan[warp] = x;
+    __syncthreads();
+    long long before = x - mine;
+    tile = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      const int n = s_scan[w];
+      before += w < warp ? n : 0;
+      tile += n;
+    }
+    return before;
+  };
+  long long total = 0, before = 0;
+  int mine = 0, mine_last = -1;
+  for (int b0 = 0; b0 < B; b0 += kWarps * 32) {
+    const int b = b0 + tid;
+    mine = b < B ? visible_blocks(p, b, row0, rows_end, mine_last) : 0;
+    long long tile;
+    before = total + scan(mine, tile);
+    total += tile;
   }
-  __syncthreads();
-  const int64_t all = s_total * H;  // every run holds a block: fewer CTAs work where there are fewer
+  const int64_t all = total * H;  // every run holds a block: fewer CTAs work where there are fewer
   const int64_t ctas = min((long long)gridDim.x, (long long)all);
   // heads without a visible slot belong to no run
   for (int b = (int)cta; b < B; b += (int)gridDim.x) {
@@ -248,38 +292,32 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
   if (cta >= ctas) return;
   const int64_t u0 = cta * all / ctas, u1 = (cta + 1) * all / ctas;
   // the sequence that holds block u0
-  long long base = 0;  // blocks (of one head) of the sequences before this tile of them
-  for (int b0 = 0; b0 < B; b0 += kWarps * 32) {
-    const int b = b0 + tid;
-    int last;
-    const int mine = b < B ? visible_blocks(p, b, row0, rows_end, last) : 0;
-    int x = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) s_scan[warp] = x;
-    __syncthreads();
-    long long before = base + x - mine, tile = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      const int n = s_scan[w];
-      before += w < warp ? n : 0;
-      tile += n;
-    }
+  auto found = [&](int b) {
     if (mine && before * H <= u0 && u0 < (before + mine) * H) {
       s_b = b;
+      s_blocks = mine;
+      s_slot = mine_last;
       s_before = before;
     }
-    base += tile;
-    if (base * H > u0) break;
+  };
+  if (B <= kWarps * 32) {
+    found(tid);
+  } else {
+    long long base = 0;
+    for (int b0 = 0; base * H <= u0; b0 += kWarps * 32) {
+      mine = b0 + tid < B ? visible_blocks(p, b0 + tid, row0, rows_end, mine_last) : 0;
+      long long tile;
+      before = base + scan(mine, tile);
+      base += tile;
+      found(b0 + tid);
+    }
   }
   __syncthreads();
 
   Cursor at;
   at.b = s_b;
-  at.blocks = visible_blocks(p, at.b, row0, rows_end, at.last);
+  at.blocks = s_blocks;
+  at.last = s_slot;
   {
     const int64_t in = u0 - s_before * H;  // blocks of this sequence's heads before the run
     at.h = (int)(in / at.blocks);
@@ -623,11 +661,12 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
       for (int e = tid; e < rows * (D / 4); e += kWarps * 32) {
         const int rr = e / (D / 4), d = e % (D / 4) * 4;
         float mm = -INFINITY;
+#pragma unroll 8
         for (int k = 0; k < parts; ++k) mm = fmaxf(mm, __ldcg(p.part_ml + 2 * (part0 + kRows * k + rr)));
         float ll = 0.0f;
         float4 oo = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (mm > -INFINITY) {
-#pragma unroll 4
+#pragma unroll 8
           for (int k = 0; k < parts; ++k) {
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + part0 + kRows * k + rr);
             const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (part0 + kRows * k + rr) * D + d));
@@ -884,7 +923,12 @@ extern "C" int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const
   p.c = *c;
   p.q = q;
   p.dtype = dtype;
-  for (int i = 0; i < 3; ++i) p.qs[i] = q_strides[i];
+  const int wide = dtype == CB_F32 ? 4 : 8;
+  p.q_wide = ((uintptr_t)q & 15) == 0;
+  for (int i = 0; i < 3; ++i) {
+    p.qs[i] = q_strides[i];
+    p.q_wide = p.q_wide && q_strides[i] % wide == 0;
+  }
   p.G = n_q_heads / c->n_kv_heads;
   p.T = T;
   p.rows = pl.rows;

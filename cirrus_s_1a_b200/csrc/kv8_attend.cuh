@@ -13,6 +13,7 @@ struct AttendParams {
   const void* q;
   int dtype;
   int64_t qs[3];        // element strides between sequences, tokens, heads
+  bool q_wide;          // q and its strides are multiples of 16 bytes
   int G, T, rows;       // query heads per KV head; rows = T * G of a KV head
   const int32_t* pos;
   const int32_t* counts;
