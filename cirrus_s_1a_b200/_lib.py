@@ -41,7 +41,8 @@ EXPORTS = ("cb_abi_version", "cb_status_string", "cb_nvfp4_quantize", "cb_nvfp4_
            "cb_workspace_layout", "cb_nvfp4_slice_bytes", "cb_nvfp4_pack_slices", "cb_prompt_lookup_draft",
            "cb_spec_accept", "cb_mtp_workspace_bytes", "cb_mtp_draft", "cb_gemm_nvfp4", "cb_gemm_scratch_bytes",
            "cb_stream_plan_bytes", "cb_stream_plan", "cb_weight_stream_nvfp4", "cb_kv8_append",
-           "cb_kv8_attend_scratch_bytes", "cb_kv8_attend", "cb_kv8_evict", "cb_token_logprobs")
+           "cb_kv8_attend_scratch_bytes", "cb_kv8_attend", "cb_kv8_evict", "cb_forward_kv8_workspace_bytes",
+           "cb_forward_kv8", "cb_token_logprobs")
 
 P = C.c_void_p
 I32 = C.c_int32
@@ -164,6 +165,10 @@ def lib() -> C.CDLL:
         L.cb_kv8_attend_scratch_bytes.argtypes = [P, I32, I32, I32, I32, I32]
         L.cb_kv8_attend.argtypes = [P, P, I32, P, I32, I32, P, P, I32, C.c_float, I32, P, P, P, C.c_size_t, P, P]
         L.cb_kv8_evict.argtypes = [P, P, I32, I32, P, P, P]
+        L.cb_forward_kv8_workspace_bytes.restype = C.c_size_t
+        L.cb_forward_kv8_workspace_bytes.argtypes = [C.POINTER(CbModel), P, I32]
+        L.cb_forward_kv8.argtypes = [C.POINTER(CbModel), C.POINTER(CbCache), P, P, I32, P, C.c_size_t, P, I32, I32, P,
+                                     P, P, P]
         L.cb_token_logprobs.argtypes = [P, I32, C.c_int64, I32, I32, P, I32, P, P, P, P, P, P, P]
         L.cb_read_trace.argtypes = [C.POINTER(CbModel), I32, I32, I32, P, P, I32, P]
         L.cb_launch_count.restype = C.c_int64
@@ -171,7 +176,7 @@ def lib() -> C.CDLL:
         for name in EXPORTS:
             if name not in ("cb_status_string", "cb_workspace_bytes", "cb_launch_count", "cb_nvfp4_slice_bytes",
                             "cb_mtp_workspace_bytes", "cb_gemm_scratch_bytes", "cb_stream_plan_bytes",
-                            "cb_kv8_attend_scratch_bytes"):
+                            "cb_kv8_attend_scratch_bytes", "cb_forward_kv8_workspace_bytes"):
                 getattr(L, name).restype = C.c_int
         if L.cb_abi_version() != 3:
             raise CbError("libcirrus_b200.so ABI version mismatch")

@@ -19,6 +19,7 @@
 #include "common.cuh"
 #include "gdn.cuh"
 #include "gemm.cuh"
+#include "kv8_model.cuh"
 #include "mk.cuh"
 #include "nvfp4.cuh"
 
@@ -282,12 +283,52 @@ static int launch_persistent(const CbModel& m, const CbCache& c, const Workspace
   return launch_mk(a, st);
 }
 
-static int validate(const CbModel& m, const CbCache& c) {
+// An 8-bit shared cache (cb_forward_kv8): what it needs of the workspace behind the
+// forward's own, ending with the attention's scratch.
+struct Kv8Run {
+  const CbKv8* kv = nullptr;
+  int32_t* slots = nullptr;
+  bool add_mass = false;
+  float* k = nullptr;       // [R][kv heads][hd]
+  void* q = nullptr;        // f16 [R][q heads][hd]
+  void* o = nullptr;        // f16 [R][q heads][hd]
+  float* lse = nullptr;     // [R][q heads]
+  int32_t* at = nullptr;    // [2][batch]: slots of the chunk's first token, of its first query
+  void* scratch = nullptr;
+  size_t scratch_off = 0, scratch_bytes = 0;
+};
+
+static Kv8Run kv8_carve(const CbModel& m, int batch, int T, size_t off, char* base) {
+  Kv8Run r;
+  const size_t R = (size_t)batch * chunk_tokens(m, T);
+  auto take = [&](size_t bytes) {
+    const size_t o = off;
+    off += align256(bytes);
+    return base ? base + o : nullptr;
+  };
+  r.k = (float*)take(R * m.n_kv_heads * m.head_dim * 4);
+  r.q = take(R * m.n_q_heads * m.head_dim * 2);
+  r.o = take(R * m.n_q_heads * m.head_dim * 2);
+  r.lse = (float*)take(R * m.n_q_heads * 4);
+  r.at = (int32_t*)take((size_t)batch * 2 * 4);
+  r.scratch_off = off;
+  r.scratch = base ? base + off : nullptr;
+  return r;
+}
+
+static int kv8_fits(const CbModel& m, const CbKv8* kv, int batch) {
+  if (const int rc = kv8_check(kv)) return rc;
+  if (m.sparse_topk > 0 || kv->batch != batch || kv->n_kv_heads != m.n_kv_heads || kv->head_dim != m.head_dim)
+    return CB_ERR_SHAPE;
+  return CB_OK;
+}
+
+static int validate(const CbModel& m, const CbCache& c, bool kv8) {
   if (m.n_self_layers <= 0 || m.n_self_layers > CB_MAX_SELF || m.n_cross_layers <= 0 ||
       m.n_cross_layers > CB_MAX_CROSS || m.d_model <= 0 || m.d_model % 16 || m.vocab_size <= 0)
     return CB_ERR_ARG;
   if (m.n_q_heads % m.n_kv_heads || m.head_dim % 8 || m.rot_dim > m.head_dim) return CB_ERR_SHAPE;
-  if (!c.pos || !c.kv_k || !c.kv_v || (m.sparse_topk > 0 && !c.kv_ik) || c.batch <= 0 || c.max_ctx <= 0)
+  if (!c.pos || (!kv8 && (!c.kv_k || !c.kv_v)) || (m.sparse_topk > 0 && !c.kv_ik) || c.batch <= 0 || c.max_ctx <= 0)
     return CB_ERR_ARG;
   if (c.swa_slots < m.swa_window + CB_SWA_EXTRA) return CB_ERR_SHAPE;
   if (!m.lm_head.tiles || !m.shared_proj.tiles || !m.inv_freq) return CB_ERR_ARG;
@@ -376,16 +417,25 @@ extern "C" int cb_clear_status(void* workspace, void* stream) {
   return cudaMemsetAsync(workspace, 0, sizeof(int32_t), (cudaStream_t)stream) == cudaSuccess ? CB_OK : CB_ERR_CUDA;
 }
 
-extern "C" int cb_forward(const CbModel* mp, const CbCache* cp, void* workspace, size_t workspace_bytes,
-                          const int64_t* ids, int32_t T, int32_t n_logits, float* logits, float* hidden,
-                          int32_t* argmax, void* stream) {
+static int forward(const CbModel* mp, const CbCache* cp, const Kv8Run* kv8_in, void* workspace, size_t workspace_bytes,
+                   const int64_t* ids, int32_t T, int32_t n_logits, float* logits, float* hidden, int32_t* argmax,
+                   void* stream) {
   if (!mp || !cp || !workspace || !ids || T <= 0) return CB_ERR_ARG;
   const CbModel& m = *mp;
   const CbCache& c = *cp;
-  CB_TRY(validate(m, c));
+  CB_TRY(validate(m, c, kv8_in != nullptr));
   const int B = c.batch;
   const Workspace w = carve(m, B, T, c.max_ctx, (char*)workspace);
   if (workspace_bytes < w.bytes) return CB_ERR_WORKSPACE;
+  Kv8Run kv8;
+  if (kv8_in) {
+    kv8 = kv8_carve(m, B, T, w.bytes, (char*)workspace);
+    kv8.kv = kv8_in->kv;
+    kv8.slots = kv8_in->slots;
+    kv8.add_mass = kv8_in->add_mass;
+    if (workspace_bytes < kv8.scratch_off) return CB_ERR_WORKSPACE;
+    kv8.scratch_bytes = workspace_bytes - kv8.scratch_off;
+  }
   cudaStream_t st = (cudaStream_t)stream;
   const int d = m.d_model;
   const int nq = (n_logits <= 0 || n_logits > T) ? T : n_logits;
@@ -399,7 +449,7 @@ extern "C" int cb_forward(const CbModel* mp, const CbCache* cp, void* workspace,
   const int64_t swa_layer = (int64_t)c.swa_slots * m.n_kv_heads * m.head_dim;
   const int64_t kv_seq = (int64_t)c.max_ctx * m.n_kv_heads * m.head_dim;
 
-  if (m.forward_path != CB_PATH_MULTI_KERNEL && T <= CB_MAX_T && mk_supported(m, c, T, nq)) {
+  if (!kv8.kv && m.forward_path != CB_PATH_MULTI_KERNEL && T <= CB_MAX_T && mk_supported(m, c, T, nq)) {
     const int rc = launch_persistent(m, c, w, ids, T, nq, logits, hidden, argmax, st);
     if (rc != CB_ERR_SHAPE) return rc;  // CB_ERR_SHAPE: not co-resident on this device, use one launch per op
   }
@@ -545,7 +595,28 @@ extern "C" int cb_forward(const CbModel* mp, const CbCache* cp, void* workspace,
     const int lds = w.ldp;
     CB_TRY(proj(w, m.shared_proj, w.h, d, R, m.shared_norm, m.norm_eps, PRE_RMSNORM, EPI_STORE, w.proj, lds,
                 m.shared_proj.rows, st));
-    {
+    if (kv8.kv) {
+      Kv8HeadsParams hp{};
+      hp.proj = w.proj;
+      hp.ldp = lds;
+      hp.src_T = tc;
+      hp.rows = R;
+      hp.T = tc;
+      hp.heads = m.n_kv_heads;
+      hp.hd = m.head_dim;
+      hp.rot2 = m.rot_dim / 2;
+      hp.pos = c.pos;
+      hp.offset = c0;
+      hp.norm = m.shared_k_norm;
+      hp.inv_freq = m.inv_freq;
+      hp.eps = m.norm_eps;
+      hp.out32 = kv8.k;
+      CB_TRY(launch_kv8_heads(hp, st));
+      CB_TRY(launch_kv8_slots(kv8.slots, B, c0, kv8.at, st));
+      const int64_t hd = m.head_dim, width = m.n_kv_heads * hd;
+      const int64_t ks[3] = {tc * width, width, hd}, vs[3] = {(int64_t)tc * lds, lds, hd};
+      CB_TRY(cb_kv8_append(kv8.kv, kv8.k, w.proj + width, CB_F32, ks, vs, tc, kv8.at, nullptr, w.status, st));
+    } else {
       HeadPrepParams hp{};
       hp.proj = w.proj;
       hp.ldp = lds;
@@ -611,6 +682,34 @@ extern "C" int cb_forward(const CbModel* mp, const CbCache* cp, void* workspace,
       const CbCrossLayer& L = m.cross_layers[j];
       const int ldc = L.q_gate.rows;
       CB_TRY(proj(w, L.q_gate, w.xc, d, RQ, L.norm1, m.norm_eps, PRE_RMSNORM, EPI_STORE, w.cproj, ldc, ldc, st));
+      if (kv8.kv) {
+        Kv8HeadsParams hp{};
+        hp.proj = w.cproj;
+        hp.ldp = ldc;
+        hp.src_T = nqc;
+        hp.rows = RQ;
+        hp.T = nqc;
+        hp.heads = m.n_q_heads;
+        hp.hd = m.head_dim;
+        hp.rot2 = m.rot_dim / 2;
+        hp.pos = c.pos;
+        hp.offset = c0 + t_off;
+        hp.norm = L.q_norm;
+        hp.inv_freq = m.inv_freq;
+        hp.eps = m.norm_eps;
+        hp.out16 = static_cast<__half*>(kv8.q);
+        CB_TRY(launch_kv8_heads(hp, st));
+        int32_t* at = kv8.at + B;
+        if (j == 0) CB_TRY(launch_kv8_slots(kv8.slots, B, c0 + t_off, at, st));
+        const int64_t hd = m.head_dim, width = m.n_q_heads * hd, qs[3] = {nqc * width, width, hd};
+        CB_TRY(cb_kv8_attend(kv8.kv, kv8.q, CB_F16, qs, m.n_q_heads, nqc, at, nullptr, kv8.kv->max_len,
+                             1.0f / sqrtf((float)m.head_dim), kv8.add_mass, kv8.o, kv8.lse, kv8.scratch,
+                             kv8.scratch_bytes, w.status, st));
+        CB_TRY(launch_kv8_gate(kv8.o, w.cproj + m.cr_off_gate, ldc, RQ, m.n_q_heads, m.head_dim, w.attn, w.att_ld, st));
+        CB_TRY(proj(w, L.o_proj, w.attn, w.att_ld, RQ, nullptr, 0.f, PRE_NONE, EPI_ADD, w.xc, d, d, st));
+        CB_TRY(ffn(L.gate_up, L.down, L.norm2, m, w.xc, RQ, w, st));
+        continue;
+      }
       CrossParams cpp{};
       cpp.proj = w.cproj;
       cpp.ldp = ldc;
@@ -673,5 +772,41 @@ extern "C" int cb_forward(const CbModel* mp, const CbCache* cp, void* workspace,
   }
   advance_pos_kernel<<<ceil_div(B, 128), 128, 0, st>>>(c.pos, B, T);
   count_launch();
+  if (kv8.kv) {
+    advance_pos_kernel<<<ceil_div(B, 128), 128, 0, st>>>(kv8.slots, B, T);
+    count_launch();
+  }
   return cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
+}
+
+extern "C" int cb_forward(const CbModel* m, const CbCache* c, void* workspace, size_t workspace_bytes,
+                          const int64_t* ids, int32_t T, int32_t n_logits, float* logits, float* hidden,
+                          int32_t* argmax, void* stream) {
+  return forward(m, c, nullptr, workspace, workspace_bytes, ids, T, n_logits, logits, hidden, argmax, stream);
+}
+
+extern "C" size_t cb_forward_kv8_workspace_bytes(const CbModel* m, const CbKv8* kv8, int32_t T) {
+  if (!m || T <= 0 || !kv8 || kv8_fits(*m, kv8, kv8->batch) != CB_OK) return 0;
+  const size_t own = carve(*m, kv8->batch, T, 1, nullptr).bytes;
+  const size_t off = kv8_carve(*m, kv8->batch, T, own, nullptr).scratch_off;
+  size_t scratch = 0;  // of any chunk's query count, with weights or without
+  for (int n = 1, most = chunk_tokens(*m, T); n <= most; ++n)
+    for (int mass = 0; mass < 2; ++mass)
+      scratch = std::max(scratch, cb_kv8_attend_scratch_bytes(kv8, CB_F16, m->n_q_heads, n, kv8->max_len, mass));
+  return scratch ? off + scratch : 0;
+}
+
+extern "C" int cb_forward_kv8(const CbModel* m, const CbCache* c, const CbKv8* kv8, int32_t* slots, int32_t add_mass,
+                              void* workspace, size_t workspace_bytes, const int64_t* ids, int32_t T, int32_t n_logits,
+                              float* logits, float* hidden, int32_t* argmax, void* stream) {
+  if (!m || !c || !kv8 || !slots) return CB_ERR_ARG;
+  CB_TRY(kv8_fits(*m, kv8, c->batch));
+  if (add_mass && !kv8->mass) return CB_ERR_ARG;
+  Kv8Run run;
+  run.kv = kv8;
+  run.slots = slots;
+  run.add_mass = add_mass != 0;
+  CbCache cache = *c;
+  cache.max_ctx = 1;  // sizes nothing here: no indexer scores, no rows by position
+  return forward(m, &cache, &run, workspace, workspace_bytes, ids, T, n_logits, logits, hidden, argmax, stream);
 }

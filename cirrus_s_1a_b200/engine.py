@@ -26,6 +26,7 @@ from cirrus_s_1a_b200 import _lib
 from cirrus_s_1a_b200._lib import (CB_LAYER_GDN, CB_LAYER_SWA, CB_MAX_T, CB_PREFILL_CHUNK, CB_SWA_EXTRA, CbCache,
                                    CbMatrix, CbModel,
                                    CbMtp, CbSliced)
+from cirrus_s_1a_b200.kv8 import Kv8Cache
 
 
 def pad16(n: int) -> int:
@@ -252,9 +253,16 @@ class DeviceCache:
     >= pos are scratch, so restoring a snapshot after a discarded verify
     forward (``generate.py:71-77``) is exact.  A clone and its source must not
     both be advanced past the fork point.
+
+    ``kv8="e4m3"`` or ``"int8"`` (models with dense cross attention): the shared K/V
+    is a ``Kv8Cache`` of ``max_ctx`` slots instead of bf16 rows by position;
+    ``slots_dev`` / ``slots_host`` count the slots in use and ``evict`` frees some, so
+    the text may be longer than the cache.  A clone then copies it (an append may
+    round older codes of its block again).
     """
 
-    def __init__(self, model: DeviceModel, batch: int, max_ctx: int, _share: "DeviceCache | None" = None):
+    def __init__(self, model: DeviceModel, batch: int, max_ctx: int, _share: "DeviceCache | None" = None,
+                 kv8: str | None = None, add_mass: bool = False):
         cfg, dev = model.cfg, model.device
         self.model, self.batch, self.max_ctx = model, batch, max_ctx
         # window + CB_PREFILL_CHUNK slots: a prompt chunk appends all its keys before its attention
@@ -269,9 +277,18 @@ class DeviceCache:
             self.swa_k = torch.zeros(batch, max(model.n_swa, 1), self.swa_slots, kvh, hd, dtype=torch.bfloat16,
                                      device=dev)
             self.swa_v = torch.zeros_like(self.swa_k)
-            self.kv_k = torch.zeros(batch, max_ctx, kvh, hd, dtype=torch.bfloat16, device=dev)
-            self.kv_v = torch.zeros_like(self.kv_k)
-            self.kv_ik = torch.zeros(batch, max_ctx, max(cfg.indexer_dim, 1), dtype=torch.uint8, device=dev)
+            self.kv8, self.add_mass = None, add_mass
+            if kv8 is not None:
+                if cfg.sparse_topk is not None:
+                    raise ValueError("an 8-bit shared cache needs dense cross attention (sparse_topk=None)")
+                self.kv8 = Kv8Cache(batch, kvh, hd, max_ctx, kv8, device=dev, mass=add_mass)
+                self.slots_dev = torch.zeros(batch, dtype=torch.int32, device=dev)
+                self.slots_host = [0] * batch
+                self.kv_k = self.kv_v = self.kv_ik = None
+            else:
+                self.kv_k = torch.zeros(batch, max_ctx, kvh, hd, dtype=torch.bfloat16, device=dev)
+                self.kv_v = torch.zeros_like(self.kv_k)
+                self.kv_ik = torch.zeros(batch, max_ctx, max(cfg.indexer_dim, 1), dtype=torch.uint8, device=dev)
             self.pos_host = [0] * batch
         else:
             self.pos_dev = _share.pos_dev.clone()
@@ -280,6 +297,11 @@ class DeviceCache:
             self.swa_k, self.swa_v = _share.swa_k, _share.swa_v
             self.kv_k, self.kv_v, self.kv_ik = _share.kv_k, _share.kv_v, _share.kv_ik
             self.pos_host = list(_share.pos_host)
+            self.kv8, self.add_mass = None, _share.add_mass
+            if _share.kv8 is not None:
+                self.kv8 = _share.kv8.clone()
+                self.slots_dev = _share.slots_dev.clone()
+                self.slots_host = list(_share.slots_host)
         self.snap_state = self.snap_conv = None
         self._struct = None
 
@@ -312,16 +334,29 @@ class DeviceCache:
             s.pos, s.gdn_state, s.gdn_conv = (self.pos_dev.data_ptr(), self.gdn_state.data_ptr(),
                                               self.gdn_conv.data_ptr())
             s.swa_k, s.swa_v = self.swa_k.data_ptr(), self.swa_v.data_ptr()
-            s.kv_k, s.kv_v, s.kv_ik = self.kv_k.data_ptr(), self.kv_v.data_ptr(), self.kv_ik.data_ptr()
+            if self.kv8 is None:
+                s.kv_k, s.kv_v, s.kv_ik = self.kv_k.data_ptr(), self.kv_v.data_ptr(), self.kv_ik.data_ptr()
             if self.snap_state is not None:
                 s.snap_state, s.snap_conv = self.snap_state.data_ptr(), self.snap_conv.data_ptr()
             self._struct = s
         return self._struct
 
+    def evict(self, keep: int, recent: int) -> torch.Tensor:
+        """Brings sequences of more than ``keep`` slots of the 8-bit cache down to
+        ``keep`` by accumulated attention weight (``Kv8Cache.evict``); positions go on
+        as before.  Returns the slots the kept tokens came from."""
+        if self.kv8 is None:
+            raise ValueError("only an 8-bit shared cache (kv8=...) can evict")
+        kept, self.slots_dev = self.kv8.evict(self.slots_dev, keep, recent)
+        self.slots_host = [min(n, keep) for n in self.slots_host]
+        return kept
+
     # ------------------------------------------------ reference-format view
     def to_reference(self, b: int = 0) -> dict:
         """The reference ``Cache`` contents of sequence ``b`` as CPU float32 tensors:
         ``{"layers": [...], "shared": {"k", "v", "ik"}, "pos": int}``."""
+        if self.kv8 is not None:
+            raise ValueError("an 8-bit shared cache has no reference form (its slots may be evicted)")
         cfg = self.model.cfg
         pos = self.pos_host[b]
         layers, gi, si = [], 0, 0
@@ -380,8 +415,12 @@ class CirrusB200:
         self._ws: dict = {}
 
     # ----------------------------------------------------------- helpers
-    def new_cache(self, batch: int = 1, max_ctx: int | None = None) -> DeviceCache:
-        return DeviceCache(self.model, batch, max_ctx or self.max_ctx)
+    def new_cache(self, batch: int = 1, max_ctx: int | None = None, kv8: str | None = None,
+                  add_mass: bool = False) -> DeviceCache:
+        """``kv8``: the shared K/V in 8 bits, ``max_ctx`` slots of it; ``add_mass``: each
+        forward adds the slots' attention weights up for ``DeviceCache.evict``."""
+        with torch.cuda.device(self.device):
+            return DeviceCache(self.model, batch, max_ctx or self.max_ctx, kv8=kv8, add_mass=add_mass)
 
     def workspace(self, batch: int, T: int, max_ctx: int) -> torch.Tensor:
         Tc = min(T, CB_PREFILL_CHUNK)  # cb_forward runs longer inputs in chunks of at most this many tokens
@@ -398,12 +437,31 @@ class CirrusB200:
     def launch(self, cache: DeviceCache, ids_dev: torch.Tensor, T: int, n_logits: int, logits, hidden, argmax,
                stream: int | None = None) -> None:
         """Enqueue one ``cb_forward`` (no synchronisation; capturable)."""
+        if cache.kv8 is not None:
+            self._launch_kv8(cache, ids_dev, T, n_logits, logits, hidden, argmax, stream)
+            return
         ws = self.workspace(cache.batch, T, cache.max_ctx)
         st = stream if stream is not None else _stream_ptr(self.device)
         rc = _lib.lib().cb_forward(C.byref(self.model.desc), C.byref(cache.struct()), ws.data_ptr(), ws.numel(),
                                    ids_dev.data_ptr(), T, n_logits, _lib.ptr(logits), _lib.ptr(hidden),
                                    _lib.ptr(argmax), st)
         _lib.check(rc, "cb_forward")
+
+    def _launch_kv8(self, cache, ids_dev, T, n_logits, logits, hidden, argmax, stream) -> None:
+        L = _lib.lib()
+        st = stream if stream is not None else _stream_ptr(self.device)
+        # the attention's counters in it are zero between calls: one workspace for each cache and length
+        Tc = min(T, CB_PREFILL_CHUNK)
+        ws = cache.kv8.workspaces.get(Tc)
+        if ws is None:
+            nbytes = L.cb_forward_kv8_workspace_bytes(C.byref(self.model.desc), cache.kv8._ref, Tc)
+            if nbytes == 0:
+                raise _lib.CbError("cb_forward_kv8_workspace_bytes: shape not supported")
+            ws = cache.kv8.workspaces[Tc] = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
+        rc = L.cb_forward_kv8(C.byref(self.model.desc), C.byref(cache.struct()), cache.kv8._ref,
+                              cache.slots_dev.data_ptr(), int(cache.add_mass), ws.data_ptr(), ws.numel(),
+                              ids_dev.data_ptr(), T, n_logits, _lib.ptr(logits), _lib.ptr(hidden), _lib.ptr(argmax), st)
+        _lib.check(rc, "cb_forward_kv8")
 
     def intermediates(self, cache: DeviceCache, T: int = 1) -> dict:
         """Views into the workspace of the last forward on this cache's shape
@@ -436,6 +494,9 @@ class CirrusB200:
         _lib.check(_lib.lib().cb_clear_status(ws.data_ptr(), _stream_ptr(self.device)), "cb_clear_status")
 
     def read_status(self, cache: DeviceCache, T: int = 1) -> int:
+        if cache.kv8 is not None:
+            ws = cache.kv8.workspaces.get(min(T, CB_PREFILL_CHUNK))
+            return 0 if ws is None else int(ws[:4].view(torch.int32).item())
         ws = self.workspace(cache.batch, T, cache.max_ctx)
         out = _lib.I32(0)
         _lib.check(_lib.lib().cb_read_status(ws.data_ptr(), C.byref(out), _stream_ptr(self.device)), "status")
@@ -502,7 +563,10 @@ class CirrusB200:
             cache = self.new_cache(B)
         elif cache.batch != B:
             raise ValueError(f"cache holds {cache.batch} sequences, input has {B}")
-        if max(cache.pos_host) + T > cache.max_ctx:
+        if cache.kv8 is not None:
+            if max(cache.slots_host) + T > cache.kv8.max_len:
+                raise _lib.CbError(f"context full: {max(cache.slots_host)} + {T} > {cache.kv8.max_len} slots")
+        elif max(cache.pos_host) + T > cache.max_ctx:
             raise _lib.CbError(f"context full: {max(cache.pos_host)} + {T} > max_ctx {cache.max_ctx}")
         nq = T if n_logits is None else max(1, min(n_logits, T))
         with torch.cuda.device(self.device):
@@ -511,6 +575,8 @@ class CirrusB200:
             hidden = torch.empty(B, nq, self.cfg.d_model, dtype=torch.float32, device=self.device)
             self.launch(cache, ids, T, nq, logits, hidden, None)
         cache.pos_host = [p + T for p in cache.pos_host]
+        if cache.kv8 is not None:
+            cache.slots_host = [n + T for n in cache.slots_host]
         return Output(logits=logits, hidden=hidden, cache=cache if want_cache else None)
 
     __call__ = forward
@@ -526,6 +592,8 @@ class DecodeGraph:
 
     def __init__(self, engine: CirrusB200, cache: DeviceCache, T: int = 1, n_logits: int = 1,
                  want_logits: bool = True):
+        if cache.kv8 is not None:
+            raise ValueError("DecodeGraph replays the bf16 shared cache")
         self.engine, self.cache, self.T, self.nq = engine, cache, T, n_logits
         dev = engine.device
         B = cache.batch

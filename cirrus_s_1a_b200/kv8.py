@@ -96,12 +96,17 @@ class Kv8Cache:
         self._ref = C.addressof(self._struct)
         self._lib = _lib.lib()
         self._scratch: dict = {}
+        self.workspaces: dict = {}  # of the model's forward over this cache, by chunk length
 
     # ------------------------------------------------------------- helpers
     @property
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale, self.mass)
                    if t is not None)
+
+    def clone(self) -> "Kv8Cache":
+        return Kv8Cache.from_tensors(*(None if t is None else t.clone()
+                                       for t in (self.k, self.v, self.k_scale, self.v_scale, self.mass)))
 
     def values(self) -> tuple:
         """(k, v) as float32 [B, H, L, D]: code * scale of every slot, in use or not."""

@@ -49,6 +49,8 @@ class SpecDecoder:
     def __init__(self, engine, cache, max_draft: int = 4, min_ngram: int = 2, max_ngram: int = 4):
         if max_draft < 0 or 1 + max_draft > _lib.CB_MAX_T:
             raise ValueError(f"max_draft must be in [0, {_lib.CB_MAX_T - 1}]")
+        if cache.kv8 is not None:
+            raise ValueError("SpecDecoder rewinds the bf16 shared cache; an 8-bit one is not supported")
         self.engine, self.cache = engine, cache
         self.max_draft, self.min_ngram, self.max_ngram = max_draft, min_ngram, max_ngram
         self.T = 1 + max_draft

@@ -463,6 +463,21 @@ int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const int64_t* q
 int cb_kv8_evict(const CbKv8* c, const int32_t* pos, int32_t keep, int32_t recent, int32_t* kept, int32_t* new_pos,
                  void* stream);
 
+/* cb_forward for a model with dense cross attention (sparse_topk 0) whose shared K/V
+ * is an 8-bit cache: the shared projection's keys (normed, RoPE at the tokens' true
+ * positions cache->pos) and values are appended at slots[b] (device int32, the slots
+ * of kv8 in use, <= pos[b] once slots have been evicted), every cross layer attends
+ * over kv8 (queries and outputs in f16), and slots[b] advances by T with pos[b].
+ * add_mass: each cross layer adds its attention weights to kv8->mass.  The cache's
+ * kv_k / kv_v / kv_ik are not used (null), its max_ctx does not bound positions;
+ * tokens past kv8->max_len are dropped and the status word receives
+ * CB_ERR_CTX_FULL.  workspace: cb_forward_kv8_workspace_bytes, zeroed once.
+ * Runs one launch per op.  head_dim 16, 32, 64 or 128 as the cache's. */
+size_t cb_forward_kv8_workspace_bytes(const CbModel* m, const CbKv8* kv8, int32_t T);
+int cb_forward_kv8(const CbModel* m, const CbCache* c, const CbKv8* kv8, int32_t* slots, int32_t add_mass,
+                   void* workspace, size_t workspace_bytes, const int64_t* ids, int32_t T, int32_t n_logits,
+                   float* logits, float* hidden, int32_t* argmax, void* stream);
+
 /* ------------------------------------------------- log probabilities */
 /* For each of `rows` rows of logits [rows][ld] (CB_F32 / CB_BF16 / CB_F16, V of
  * them): logprob = log softmax(x)[tokens[r]], entropy = -sum p log p (natural

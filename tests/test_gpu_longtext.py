@@ -1,0 +1,119 @@
+"""The 8-bit shared cache inside the model (cb_forward_kv8), with scoring and
+eviction: the operators run together as they are used."""
+
+from dataclasses import replace
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+def model(**kw):
+    from cirrus_s_1a_b200 import synthetic
+    from cirrus_s_1a_b200.config import get_config
+    from cirrus_s_1a_b200.engine import CirrusB200
+
+    cfg = replace(get_config("cirrus-s-1a-debug"), sparse_topk=None, **kw)
+    return cfg, CirrusB200(cfg, synthetic.random_state_dict(cfg, seed=3, norm_jitter=0.1), device=DEV, max_ctx=640)
+
+
+def text(cfg, n, batch=1, seed=5):
+    return torch.randint(0, cfg.vocab_size, (batch, n), generator=torch.Generator().manual_seed(seed))
+
+
+WIDE = dict(d_model=128, head_dim=64, n_q_heads=6, n_kv_heads=2, gdn_head_dim_k=64, gdn_head_dim_v=64, ffn_hidden=128)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("kw", [{}, WIDE], ids=["debug", "wide"])
+def test_steps_equal_the_bf16_path_on_the_same_keys_and_values(fmt, kw):
+    """Prompts (several chunk lengths), verify and decode steps.  The 8-bit cache's
+    values are exact in bf16, so the bf16 path can be given the same keys and values:
+    what is left is one step's own tokens (bf16 there, 8 bits here) and the rounding
+    of queries, probabilities and outputs to f16."""
+    cfg, eng = model(**kw)
+    B = 2
+    a, b = eng.new_cache(B, kv8=fmt, add_mass=True), eng.new_cache(B)
+    ids = text(cfg, 300, B)
+    at = 0
+    for T in (150, 1, 5, 40, 1, 1, 70):
+        step = ids[:, at:at + T]
+        x, y = eng(step, cache=a).logits, eng(step, cache=b).logits
+        at += T
+        # the first chunk differs by the quantisation of its own keys alone; later ones by their own tokens'
+        tol = 6e-2 if T > 8 else 2e-2
+        torch.testing.assert_close(x, y, rtol=tol, atol=tol)
+        k, v = a.kv8.values()
+        b.kv_k[:, :at] = k[:, :, :at].transpose(1, 2).bfloat16()
+        b.kv_v[:, :at] = v[:, :, :at].transpose(1, 2).bfloat16()
+        assert torch.equal(k, k.bfloat16().float())
+        assert a.slots_dev.tolist() == a.pos_dev.tolist() == [at] * B == a.slots_host
+    # every query row of every layer and head spreads a weight of 1
+    G = cfg.n_q_heads // cfg.n_kv_heads
+    want = float(at * G * cfg.n_cross_layers)
+    assert (a.kv8.mass.sum(-1) - want).abs().max() < 1e-3 * want
+    assert eng.read_status(a, 70) == 0
+
+
+def test_scoring_with_and_without_a_bound():
+    from cirrus_s_1a_b200.longtext import score_text
+
+    cfg, eng = model(**WIDE)
+    ids = text(cfg, 500)
+    full = score_text(eng, ids, eng.new_cache(), top=3)
+    assert full.logprob.shape == (1, 499) and full.top_token.shape == (1, 499, 3)
+    logits = eng(ids[:, :-1], use_cache=True).logits.double().log_softmax(-1)
+    want = logits.gather(2, ids[:, 1:, None].to(DEV))[..., 0]
+    assert (full.logprob - want).abs().max() < 1e-2
+    held = eng.new_cache(max_ctx=640, kv8="int8")
+    near = score_text(eng, ids, held)
+    assert (near.logprob - full.logprob).abs().max() < 0.1
+    cache = eng.new_cache(max_ctx=192 + 128, kv8="int8", add_mass=True)
+    bound = score_text(eng, ids, cache, keep=192, recent=64)
+    assert cache.slots_host == [192] and cache.pos == 499 and cache.slots_dev.tolist() == [192]
+    assert torch.equal(bound.logprob[:, :128], near.logprob[:, :128])  # nothing was evicted yet
+    assert torch.isfinite(bound.logprob).all()
+    assert (bound.logprob.mean() - near.logprob.mean()).abs() < 0.2
+    assert float(cache.kv8.mass[:, :, :192].min()) >= 0.0
+
+
+def test_clones_and_refusals():
+    from cirrus_s_1a_b200 import _lib
+    from cirrus_s_1a_b200.engine import CirrusB200, DecodeGraph
+    from cirrus_s_1a_b200.longtext import score_text
+    from cirrus_s_1a_b200.speculative import SpecDecoder
+    from cirrus_s_1a_b200 import synthetic
+    from cirrus_s_1a_b200.config import get_config
+
+    cfg, eng = model()
+    ids = text(cfg, 40)
+    cache = eng.new_cache(max_ctx=64, kv8="e4m3", add_mass=True)
+    eng(ids[:, :30], cache=cache)
+    fork = cache.clone()
+    x = eng(ids[:, 30:35], cache=cache).logits
+    y = eng(ids[:, 30:35], cache=fork).logits
+    assert torch.equal(x, y) and fork.slots_host == cache.slots_host == [35]
+    with pytest.raises(_lib.CbError):
+        eng(ids[:, :30], cache=cache)  # 35 + 30 > 64 slots
+    with pytest.raises(ValueError):
+        cache.to_reference()
+    with pytest.raises(ValueError):
+        DecodeGraph(eng, cache)
+    with pytest.raises(ValueError):
+        SpecDecoder(eng, cache)
+    plain = eng.new_cache()
+    with pytest.raises(ValueError):
+        plain.evict(4, 2)
+    with pytest.raises(ValueError):
+        score_text(eng, ids, plain, keep=8)
+    with pytest.raises(ValueError):
+        score_text(eng, ids, eng.new_cache(kv8="int8"), keep=8)
+    with pytest.raises(ValueError):
+        score_text(eng, ids[:, :1], plain)
+    sparse = get_config("cirrus-s-1a-debug")
+    other = CirrusB200(sparse, synthetic.random_state_dict(sparse, seed=0), device=DEV, max_ctx=64)
+    with pytest.raises(ValueError):
+        other.new_cache(kv8="int8")
