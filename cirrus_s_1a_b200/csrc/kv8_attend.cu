@@ -43,6 +43,7 @@
 // CTA that finishes a head last joins its parts in their order and writes the
 // output, so a call is one launch (two with attention weights).
 #include <algorithm>
+#include <climits>
 
 #include "kv8.cuh"
 #include "kv8_attend.cuh"
@@ -433,8 +434,8 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
       for (int mt = 0; mt < 4; ++mt) scores<D, FMT, HL, NT>(kb + 16 * mt * D, q, c[mt]);
       __syncwarp();
       copy();  // into the slot of these keys
-      if (key0 + kKv8Block - 1 > seen) {
-        // the first row (or a row without a token) does not see all of the block
+      const bool partly = key0 + kKv8Block - 1 > seen;  // the first row (or a row without a token) does not see all of it
+      if (partly) {
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
 #pragma unroll
         for (int i = 0; i < 2; ++i) add[nt][i] = (float)ev - (m[nt][i] == -INFINITY ? 0.0f : m[nt][i]);
       const uint8_t* vb = arrive();
-      const bool tail = key0 + kKv8Block > at.last + 1;  // the block ends past the last visible slot
+      int nan_key = INT_MAX;
       float pv[HL ? D / 16 : 1][HL ? NT : 1][4] = {};
       float sum[NT][2] = {};
 #pragma unroll
@@ -529,10 +530,19 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
         for (int u = 0; u < 4; ++u) {
           const int key = 16 * s + 4 * u + t4;
           load_bytes<NB>(vb + key * D + g * NB, w[u]);
-          // slots no row sees may hold anything, an E4M3 NaN too: 0 * NaN is not 0
-          if (tail && key0 + key > at.last)
+          if (partly) {
+            // 0 * NaN is not 0: slots no row sees may hold anything and read as 0, and an
+            // E4M3 NaN in a slot that some rows see makes NaN of those rows below
 #pragma unroll
-            for (int z = 0; z < (NB + 3) / 4; ++z) w[u][z] = 0u;
+            for (int z = 0; z < (NB + 3) / 4; ++z) {
+              if (key0 + key > at.last) w[u][z] = 0u;
+              if (FMT == CB_KV8_E4M3) {
+                const uint32_t nan = __vcmpeq4(w[u][z] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+                w[u][z] &= ~nan;
+                if (nan) nan_key = min(nan_key, key0 + key);
+              }
+            }
+          }
         }
 #pragma unroll
         for (int z = 0; z < (NB + 3) / 4; ++z)
@@ -557,6 +567,14 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
       }
       __syncwarp();
       copy();  // into the slot of these values
+      if (FMT == CB_KV8_E4M3 && partly) {
+        nan_key = __reduce_min_sync(0xffffffffu, nan_key);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (nan_key <= lim[nt][i]) sum[nt][i] = NAN;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll

@@ -7,6 +7,8 @@
 // are rewritten only when the scale grows (each is then rounded once more, onto
 // a grid 2^d times as coarse).  The result does not depend on the order of
 // anything: absmax is order-free and every division by a scale is exact.
+#include <type_traits>
+
 #include "kv8.cuh"
 #include "kv8_attend.cuh"
 
@@ -26,34 +28,78 @@ struct AppendParams {
   int32_t* status;
 };
 
-// Eight values of one token, from 16-byte vectors (VEC) or one by one.
-template <bool VEC>
-__device__ __forceinline__ void load8(const void* base, int64_t i, int dtype, float (&x)[8]) {
-  if (VEC && dtype == CB_F32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
-    const float4 a = __ldcs(p), b = __ldcs(p + 1);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else if (VEC) {
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// Eight values of one token as they come, widened where they are used (16-bit types
+// hold a third fewer registers that way, and more CTAs an SM).
+template <typename T>
+struct Eight {
+  uint4 v;
+  static __device__ __forceinline__ float2 widen(uint32_t w) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      return make_float2(bf16_to_f32(w), __uint_as_float(w & 0xFFFF0000u));
+    else
+      return __half22float2(bits_h2(w));
+  }
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* p) {
+    if (VEC) {
+      v = __ldcs(reinterpret_cast<const uint4*>(p));
+    } else {
+      const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+      uint32_t* w = &v.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = (uint32_t)u[2 * j] | (uint32_t)u[2 * j + 1] << 16;
+    }
+  }
+  __device__ __forceinline__ float2 pair(int j) const { return widen((&v.x)[j]); }
+};
+template <>
+struct Eight<float> {
+  float4 a, b;
+  template <bool VEC>
+  __device__ __forceinline__ void load(const float* p) {
+    if (VEC) {
+      a = __ldcs(reinterpret_cast<const float4*>(p));
+      b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+    } else {
+      a = make_float4(p[0], p[1], p[2], p[3]);
+      b = make_float4(p[4], p[5], p[6], p[7]);
+    }
+  }
+  __device__ __forceinline__ float2 pair(int j) const {
+    return j == 0 ? make_float2(a.x, a.y) : j == 1 ? make_float2(a.z, a.w) : j == 2 ? make_float2(b.x, b.y) : make_float2(b.z, b.w);
+  }
+};
+
+// Eight values times 1 / s as codes.  fast (int8): every |x / s| <= 127, and x / s +
+// 1.5 * 2^23 rounds to an integer (ties to even) whose low byte is the code.
+template <int FMT, typename T>
+__device__ __forceinline__ uint2 encode8(const Eight<T>& x, float inv, bool fast) {
+  uint32_t w[2] = {0u, 0u};
+  if (FMT == CB_KV8_INT8 && fast) {
+    uint32_t u[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (dtype == CB_BF16) {
-        x[2 * j] = bf16_to_f32(w[j]);
-        x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-        x[2 * j] = f.x;
-        x[2 * j + 1] = f.y;
-      }
+      const float2 f = x.pair(j);
+      u[2 * j] = __float_as_uint(fmaf(f.x, inv, 12582912.0f));
+      u[2 * j + 1] = __float_as_uint(fmaf(f.y, inv, 12582912.0f));
     }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      w[j] = __byte_perm(__byte_perm(u[4 * j], u[4 * j + 1], 0x0040), __byte_perm(u[4 * j + 2], u[4 * j + 3], 0x0040), 0x5410);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = kv8_load(base, i + j, dtype);
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = x.pair(j);
+      if (FMT == CB_KV8_E4M3)
+        w[j / 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f.x * inv, f.y * inv), __NV_SATFINITE, __NV_E4M3) << (16 * (j & 1));
+      else
+        w[j / 2] |= (kv8_encode<FMT>(f.x * inv) | kv8_encode<FMT>(f.y * inv) << 8) << (16 * (j & 1));
+    }
   }
+  return make_uint2(w[0], w[1]);
 }
 
-template <int D, int FMT, bool VEC>
+template <int D, int FMT, typename T, bool VEC>
 __global__ void __launch_bounds__(kAT) kv8_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int kPer = D / 8;                                     // 8-value pieces of one token
   constexpr int kPieces = kKv8Block * kPer;                       // of one block
@@ -71,22 +117,44 @@ __global__ void __launch_bounds__(kAT) kv8_append_kernel(const __grid_constant__
   const int lo = max(pos, first), hi = (int)min(end, (int64_t)min(first + kKv8Block, p.c.max_len));
   if (lo >= hi) return;
   const int64_t row = (int64_t)b * p.c.n_kv_heads + h;
-  const void* src = is_v ? p.v : p.k;
+  const T* src = static_cast<const T*>(is_v ? p.v : p.k);
   const int64_t* st = is_v ? p.vs : p.ks;
   uint8_t* codes = (is_v ? p.c.v : p.c.k) + (row * p.c.max_len + first) * D;
   float* scale = (is_v ? p.c.v_scale : p.c.k_scale) + row * (p.c.max_len / kKv8Block) + blk;
 
-  float x[kMine][8];
-  float top = 0.0f;
+  Eight<T> x[kMine];
+  float top = 0.0f, odd = 0.0f;  // odd: NaN where an infinity or a NaN passed
+  const T* from = src + (int64_t)b * st[0] + (int64_t)(first - pos) * st[1] + h * st[2];
+#pragma unroll
+  for (int m = 0; m < kMine; ++m) {
+    const int piece = threadIdx.x + m * kAT, slot = first + piece / kPer;
+    if (slot >= lo && slot < hi && piece < kPieces)
+      x[m].template load<VEC>(from + (int64_t)(piece / kPer) * st[1] + (piece % kPer) * 8);
+  }
 #pragma unroll
   for (int m = 0; m < kMine; ++m) {
     const int piece = threadIdx.x + m * kAT, slot = first + piece / kPer;
     if (slot < lo || slot >= hi || piece >= kPieces) continue;
-    load8<VEC>(src, (int64_t)b * st[0] + (int64_t)(slot - pos) * st[1] + h * st[2] + (piece % kPer) * 8, p.dtype, x[m]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float a = fabsf(x[m][j]);
-      if (a < INFINITY) top = fmaxf(top, a);  // infinities and NaN leave the scale alone
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = x[m].pair(j);
+      top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+      odd = fmaf(f.x, 0.0f, fmaf(f.y, 0.0f, odd));
+    }
+  }
+  const bool plain = odd == 0.0f;
+  if (!plain) {  // infinities and NaN leave the scale alone
+    top = 0.0f;
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const int piece = threadIdx.x + m * kAT, slot = first + piece / kPer;
+      if (slot < lo || slot >= hi || piece >= kPieces) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = x[m].pair(j);
+        if (fabsf(f.x) < INFINITY) top = fmaxf(top, fabsf(f.x));
+        if (fabsf(f.y) < INFINITY) top = fmaxf(top, fabsf(f.y));
+      }
     }
   }
   top = block_max(top, red);
@@ -103,29 +171,38 @@ __global__ void __launch_bounds__(kAT) kv8_append_kernel(const __grid_constant__
     const int piece = threadIdx.x + m * kAT, slot = first + piece / kPer;
     if (slot >= hi || piece >= kPieces || (slot < lo && !grow)) continue;
     uint2* dst = reinterpret_cast<uint2*>(codes + piece * 8);
-    uint32_t w[2] = {0u, 0u};
     if (slot < lo) {
       const uint2 c = *dst;
       const uint32_t was[2] = {c.x, c.y};
+      uint32_t w[2] = {0u, 0u};
       const float f = old * inv;  // 2^-d
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         w[j / 4] |= kv8_encode<FMT>(kv8_decode<FMT>(was[j / 4] >> (8 * (j & 3))) * f) << (8 * (j & 3));
+      *dst = make_uint2(w[0], w[1]);
     } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j / 4] |= kv8_encode<FMT>(x[m][j] * inv) << (8 * (j & 3));
+      *dst = encode8<FMT, T>(x[m], inv, plain && e < kKv8EMax);
     }
-    *dst = make_uint2(w[0], w[1]);
   }
+}
+
+template <int D, int FMT, typename T>
+void launch(const AppendParams& p, dim3 grid, bool vec, cudaStream_t st) {
+  if (vec) kv8_append_kernel<D, FMT, T, true><<<grid, kAT, 0, st>>>(p);
+  else kv8_append_kernel<D, FMT, T, false><<<grid, kAT, 0, st>>>(p);
+}
+
+template <int D, int FMT>
+void launch(const AppendParams& p, dim3 grid, bool vec, cudaStream_t st) {
+  if (p.dtype == CB_F32) launch<D, FMT, float>(p, grid, vec, st);
+  else if (p.dtype == CB_BF16) launch<D, FMT, __nv_bfloat16>(p, grid, vec, st);
+  else launch<D, FMT, __half>(p, grid, vec, st);
 }
 
 template <int D>
 void launch(const AppendParams& p, dim3 grid, bool vec, cudaStream_t st) {
-  const bool e4m3 = p.c.format == CB_KV8_E4M3;
-  if (e4m3 && vec) kv8_append_kernel<D, CB_KV8_E4M3, true><<<grid, kAT, 0, st>>>(p);
-  else if (e4m3) kv8_append_kernel<D, CB_KV8_E4M3, false><<<grid, kAT, 0, st>>>(p);
-  else if (vec) kv8_append_kernel<D, CB_KV8_INT8, true><<<grid, kAT, 0, st>>>(p);
-  else kv8_append_kernel<D, CB_KV8_INT8, false><<<grid, kAT, 0, st>>>(p);
+  if (p.c.format == CB_KV8_E4M3) launch<D, CB_KV8_E4M3>(p, grid, vec, st);
+  else launch<D, CB_KV8_INT8>(p, grid, vec, st);
 }
 
 }  // namespace

@@ -32,6 +32,8 @@
 // With several runs per row tile, kv8_join_kernel joins them (kv8_attend.cu).
 // Every wait is bounded (%globaltimer); a wait that gives up sets CB_ERR_TIMEOUT
 // in the status word, and the CTA ends without writing results.
+#include <climits>
+
 #include "kv8.cuh"
 #include "kv8_attend.cuh"
 
@@ -211,6 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   __shared__ __align__(8) unsigned long long bars[20];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
+  __shared__ int s_nan;  // the first E4M3 NaN among values that not all rows see
   uint8_t* sq = smem;
   uint8_t* sk = smem + kTiles * C::kQ;
   uint8_t* sv = sk + kStages * C::kKV;
@@ -244,6 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_abort = 0;
+    s_nan = INT_MAX;
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)));
@@ -377,7 +381,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       // results: O, m' and l (against e_ref).  (Products n - 2 and before are known done.)
       if (n > 0) wait(o_full + 8 * tile, n - 1);
       fence_after();
-      const float lsum = l * kv8_pow2(-e_ref);
+      float lsum = l * kv8_pow2(-e_ref);
+      if (FMT == CB_KV8_E4M3 && n > 0 && s_nan <= lim) lsum = NAN;
       const int t = r / p.G, hq = (int)(head % p.c.n_kv_heads) * p.G + r % p.G;
       const int64_t orow = ((int64_t)b * p.T + t) * (p.G * p.c.n_kv_heads) + hq;
       const int64_t at = (head * p.rows + r) * p.splits + split;
@@ -440,6 +445,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     };
     load(0, 0);
     load(1, 0);
+    // tiles that end by here are seen whole by every row
+    const int seen = row0 + tiles * kRows > cnt * p.G ? -1 : min(pos + row0 / p.G, p.limit - 1);
     for (int j = 0; j < n; ++j) {
       const int st = j & 1;
 #pragma unroll
@@ -450,6 +457,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         for (int i = 0; i < C::kPieces; ++i) {
           const int key = key_of(i), c = chunk_of(i);
           uint4 lo, hi;
+          if (FMT == CB_KV8_E4M3 && kv == 1 && (beg + j + 1) * kKeys - 1 > seen) {
+            // 0 * NaN is not 0: a NaN reads as 0 here, and makes NaN of the rows that see it at the end
+            uint32_t* w = &raw[kv][i].x;
+            uint32_t any = 0;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const uint32_t nan = __vcmpeq4(w[z] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+              w[z] &= ~nan;
+              any |= nan;
+            }
+            if (any) atomicMin(&s_nan, (beg + j) * kKeys + key);
+          }
           to_operand<FMT>(raw[kv][i], lo, hi);
           *reinterpret_cast<uint4*>(dst + swizzled<kKeys>(key, 2 * c)) = lo;
           *reinterpret_cast<uint4*>(dst + swizzled<kKeys>(key, 2 * c + 1)) = hi;

@@ -245,6 +245,21 @@ def test_nan_in_a_visible_key_reaches_its_rows_only():
     assert bool(torch.isfinite(out[0, :2]).all()) and bool(out[0, 2:].isnan().all()) and bool(lse[0, 2:].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,T", [(64, 4), (64, 140), (128, 140), (128, 1), (16, 5)])
+def test_nan_in_a_value_reaches_the_rows_that_see_it_only(D, T, dtype):
+    """A NaN value in a slot that later rows see and earlier ones do not (0 * NaN is not 0)."""
+    cache = filled(1, 1, D, 512, "e4m3")
+    q = torch.randn(1, T, 3, D, generator=torch.Generator().manual_seed(8)).to(TYPES[dtype]).to(DEV)
+    clean, clean_lse = cache.attend(q, ints([200]))
+    at = T // 2
+    cache.v.view(torch.uint8)[0, 0, 200 + at, 3] = 0xFF
+    cache.v.view(torch.uint8)[0, 0, 200 + T] = 0x7F  # no row sees this one
+    out, lse = cache.attend(q, ints([200]))
+    assert torch.equal(out[0, :at], clean[0, :at]) and torch.equal(lse[0, :at], clean_lse[0, :at])
+    assert bool(out[0, at:, :, 3].isnan().all())
+
+
 def test_query_strides_and_other_streams():
     cache = filled(2, 2, 64, 256, "int8")
     proj = torch.randn(2, 7, 6 * 64 + 13, generator=torch.Generator().manual_seed(4)).to(DEV)
