@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const __grid_constan
   const float tau = s_tau;
   float* out_lp = p.top_logprob + r * p.top;
   int32_t* out_tok = p.top_token + r * p.top;
-  const int per = (vecs + NT - 1) / NT;
+  const int per = (vecs + NT - 1) / NT, per_log2 = per > 1 ? 32 - __clz(per - 1) : 0;
   bool strict = tau == -INFINITY;
   int cands;
   while (true) {
@@ -342,20 +342,29 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const __grid_constan
     if (passes(mine_max)) s_thread[atomicAdd(&s_threads, 1)] = tid;
     if (edge_at >= 0 && passes(edge_x)) take(edge_x, edge_at);
     __syncthreads();
-    const int n = s_threads;
-    for (int k = warp; k < n; k += kWarps)
-      for (int u = lane; u < per; u += 32) {
-        const int j = s_thread[k] + u * NT;
-        if (j >= vecs) break;
-        const Vec<T> v = load_vec(body + (int64_t)j * N);
+    // (thread, vector) pairs over all threads, two reads ahead
+    const int jobs = s_threads << per_log2;
+    for (int job = tid; job < jobs; job += 2 * NT) {
+      int at[2];
+      Vec<T> v[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int jb = job + u * NT;
+        at[u] = jb < jobs ? s_thread[jb >> per_log2] + (jb & ((1 << per_log2) - 1)) * NT : vecs;
+        if (at[u] < vecs) v[u] = load_vec(body + (int64_t)at[u] * N);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (at[u] >= vecs) continue;
         unsigned which = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) which |= passes(v.get(i)) ? 1u << i : 0u;
+        for (int i = 0; i < N; ++i) which |= passes(v[u].get(i)) ? 1u << i : 0u;
         for (; which && s_cands <= kCand; which &= which - 1) {
-          const int i = head + j * N + __ffs(which) - 1;
+          const int i = head + at[u] * N + __ffs(which) - 1;
           take(to_f(row[i]), i);
         }
       }
+    }
     __syncthreads();
     cands = s_cands;
     if (cands <= kCand || strict) break;
