@@ -42,6 +42,14 @@
 // in a ring of slots of its own, two or three ahead, across the ends of heads.  The
 // CTA that finishes a head last joins its parts in their order and writes the
 // output, so a call is one launch (two with attention weights).
+//
+// Bound by memory in principle (2 D bytes a key for all rows of its head), by issue
+// and the latency of its chains in fact.  Measured: 64 sequences x 1 token at 32K,
+// 128 dims, E4M3, with weights 215 us, 5.2 TB/s in the attention itself (30 % of
+// issue slots); 16 x 5 tokens at up to 128K, 64 dims, int8 151 us, 4.3 TB/s (56 % of
+// issue slots, 51 % of the integer pipe: int8 codes take 5 instructions for four,
+// E4M3 two); one token at 32K 18 us, of which the blocks take 4, placing the CTA and
+// the query 4, and joining 48 parts the rest.
 #include <algorithm>
 #include <climits>
 
@@ -703,10 +711,12 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
   if (!ok) set_status(p.status, CB_ERR_TIMEOUT);
 }
 
-// Joins the runs' parts of one row of the prompt form, in order: one CTA of D threads per row.
-__global__ void kv8_join_kernel(const __grid_constant__ AttendParams p) {
-  const int D = p.c.head_dim, d = threadIdx.x;
-  const int r = blockIdx.x;
+// Joins the runs' parts of the prompt form's rows, in order: four dims a thread, 256
+// threads to a CTA (16000 rows of 128 dims in two parts: 9.7 us; a CTA for each row took 20, most of it launching).
+__global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ AttendParams p) {
+  const int lanes = p.c.head_dim / 4, d = threadIdx.x % lanes * 4;
+  const int r = blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+  if (r >= p.rows) return;
   const int64_t head = blockIdx.y;
   const int hk = (int)(head % p.c.n_kv_heads), b = (int)(head / p.c.n_kv_heads);
   const int64_t at = (head * p.rows + r) * p.splits;
@@ -717,12 +727,12 @@ __global__ void kv8_join_kernel(const __grid_constant__ AttendParams p) {
   if (mm > -INFINITY)
     for (int s = 0; s < p.splits; ++s) {
       const float f = exp2a(p.part_ml[2 * (at + s)] - mm);
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at + s) * D + 4 * d);
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at + s) * p.c.head_dim + d);
       ll = fmaf(p.part_ml[2 * (at + s) + 1], f, ll);
       oo.x = fmaf(v.x, f, oo.x), oo.y = fmaf(v.y, f, oo.y);
       oo.z = fmaf(v.z, f, oo.z), oo.w = fmaf(v.w, f, oo.w);
     }
-  write_row(p, b, hk, r, 4 * d, oo, mm, ll);
+  write_row(p, b, hk, r, d, oo, mm, ll);
 }
 
 // mass_j += sum_r exp(x[r][j] - lse_r) from the scores that the attention left: four
@@ -974,7 +984,7 @@ extern "C" int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const
   if (p.row_tiles > 0) {
     if (const int rc = kv8_prompt_launch(p, bh, st)) return rc;
     if (p.splits > 1) {
-      kv8_join_kernel<<<dim3(p.rows, bh), c->head_dim / 4, 0, st>>>(p);
+      kv8_join_kernel<<<dim3(ceil_div(p.rows, 1024 / c->head_dim), bh), 256, 0, st>>>(p);
       count_launch();
     }
     if (p.add_mass) return kv8_prompt_mass_launch(p, bh, longest, st);
