@@ -18,6 +18,11 @@
 //      barrier, arrived at when the round's copies have landed.
 // A new block takes the scale its values need; a code is rounded again only
 // where its scale grows, and copied as it is where the scale stays.
+// Bound by memory in principle (the weights once, each kept token read and written),
+// in fact by issue (52 % of the slots, 50 % of the integer pipe) and the rounds'
+// barriers.  Measured: 32 sequences of up to 64K down to 32K, 2 heads of 128 dims,
+// E4M3: 292 us = 2.5 TB/s (uniform lengths: 314 us = 3.6 TB/s); one sequence of 16.5K
+// down to 16K, 4 heads of 64: 33 us, the selection's dependent passes and the rounds' latency.
 #include <cooperative_groups.h>
 
 #include "kv8.cuh"
