@@ -10,7 +10,7 @@
 // and a run of key tiles (128 keys for 64 dims, 64 for 128).
 //   * 4 warps turn codes into f16 operands in shared memory (two stages each of K
 //     and V), exact; no scale is applied there.
-//   * one thread issues tcgen05.mma kind::f16: S = Q K^T into tensor memory, and
+//   * one thread (two for 128 dims) issues tcgen05.mma kind::f16: S = Q K^T into tensor memory, and
 //     O += P V with P read from tensor memory (V's dims are its contiguous
 //     direction, an MN-major operand).
 //   * two warpgroups, a thread per row, do the softmax.  With x = S * a_b
@@ -35,6 +35,8 @@
 // and slower: a share of the exponentials as a polynomial on the FMA units (636 to
 // 757 us, at 639 then), three row tiles of 64 keys (703; with strict turns at the
 // exponentials 696, turns passed on at half 624), Q K^T and P V issued by two warps (641).
+// For 128 dims, 2 x 1000 tokens at up to 8K (171 us then): tiles of 128 keys with P in
+// the columns of its scores (180), a second P a tile (171).
 // Every wait is bounded (%globaltimer); a wait that gives up sets CB_ERR_TIMEOUT
 // in the status word, and the CTA ends without writing results.
 #include <climits>
@@ -53,8 +55,8 @@ constexpr int kStages = 2;
 constexpr int kSoftWarps = 4 * kTiles;
 constexpr int kConvThreads = 128;
 constexpr int kThreads = kSoftWarps * 32 + kConvThreads + 128;
-// Registers a thread of the four warpgroups, out of the 128 at launch: two of
-// softmax, one that converts, one whose first warp issues the products.
+// Registers a thread of the four warpgroups, out of the 128 at launch, where a thread
+// holds 128 scores: two warpgroups of softmax, one that converts, one that issues the products.
 constexpr int kSoftRegs = 192, kConvRegs = 88, kMmaRegs = 40;
 static_assert(2 * kSoftRegs + kConvRegs + kMmaRegs <= 4 * 128, "the shares fit what the block was launched with");
 constexpr float kLazy = 15.0f;             // growth of the maximum, in powers of two, that O follows: f16 P ends at 2^16
@@ -205,6 +207,16 @@ struct Prompt {
   // tensor memory: S, P (f16, half as many columns) and O of both tiles
   static constexpr int kP = kTiles * kKeys, kO = 512 - kTiles * D;
   static_assert(kP + kTiles * kKeys / 2 <= kO, "S, P and O fit 512 columns");
+  // Warps that issue the products.  One keeps two tiles of 128 keys busy, in a fixed
+  // order that keeps the softmax warpgroups out of step (64 dims, 4096 tokens at 32K:
+  // 584 us, a warp to each tile 637).  With 64 keys its own waits and issue bounded a
+  // tile (128 dims, 2 x 1000 tokens at 8K with weights: 171 us
+  // with one warp, 161 with two; 2048 tokens at 32K: 341, 327).
+  static constexpr int kIssuers = D == 128 ? 2 : 1;
+  // With 64 scores a thread, the softmax leaves registers to the others.
+  static constexpr int kSoftRegs = D == 128 ? 160 : cb::kSoftRegs, kConvRegs = D == 128 ? 104 : cb::kConvRegs,
+                       kMmaRegs = D == 128 ? 88 : cb::kMmaRegs;
+  static_assert(2 * kSoftRegs + kConvRegs + kMmaRegs <= 4 * 128, "the shares fit what the block was launched with");
   static constexpr int kPieces = kKeys * D / 16 / kConvThreads;  // 16-byte pieces of a tile per converting thread
   static constexpr int kRow = D / 16;                            // of a key
 };
@@ -242,11 +254,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   const int beg = min(all, split * per), n = min(all, beg + per) - beg;
 
   if (tid == 0) {
-    const uint32_t one[] = {q_full, k_free, k_free + 8, v_free, v_free + 8, s_full, s_full + 8, o_full, o_full + 8, end};
+    const uint32_t one[] = {q_full, s_full, s_full + 8, o_full, o_full + 8, end, end + 8};
     for (uint32_t bar : one) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar));
     for (int i = 0; i < 2; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(k_full + 8 * i), "n"(kConvThreads));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(v_full + 8 * i), "n"(kConvThreads));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(k_free + 8 * i), "r"(min(tiles, C::kIssuers)));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(v_free + 8 * i), "r"(min(tiles, C::kIssuers)));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s_free + 8 * i), "n"(kRows));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(p_full + 8 * i), "n"(kRows));
     }
@@ -273,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 
   if (warp < kSoftWarps) {
     // ---------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
     const int tile = warp / 4, r = row0 + tile * kRows + (warp % 4) * 32 + lane;
     if (tile < tiles) {
       const uint32_t lanes = (uint32_t)(warp % 4) << 21;  // this warp's lanes of tensor memory (bits 16-31)
@@ -431,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     }
   } else if (warp < kSoftWarps + kConvThreads / 32) {
     // ------------------------------------------------- codes to operands
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kConvRegs));
     const int d = tid - kSoftWarps * 32;
     const uint8_t* src[2] = {p.c.k + head * p.c.max_len * D, p.c.v + head * p.c.max_len * D};
     uint4 raw[2][C::kPieces];
@@ -486,14 +500,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     }
   } else {
     // ---------------------------------------------------------- products
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
-    if (warp == kSoftWarps + kConvThreads / 32 && n > 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kMmaRegs));
+    const int issuer = warp - kSoftWarps - kConvThreads / 32;
+    if (issuer < C::kIssuers && issuer < tiles && n > 0) {
+      const int first = C::kIssuers > 1 ? issuer : 0;  // its row tiles: first, first + kIssuers ...
       // The whole warp walks the loop, so that addresses and descriptors stay in
       // uniform registers; one elected thread issues.  (A branch of one thread moved
       // them there for every instruction: 90 to 140 clocks each instead of 32 or 64.)
       const bool lead = elect_one();
       const uint32_t q_at = smem_u32(sq), k_at = smem_u32(sk), v_at = smem_u32(sv);
-      if (lead) {
+      if (lead && first == 0) {
         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(q_full), "r"(tiles * C::kQ) : "memory");
         asm volatile(
             "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(q_at),
@@ -510,24 +526,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             mma_ss(t * kKeys, qd + (s / 4 * (kRows * 128) + s % 4 * 32) / 16, kd + (s / 4 * (kKeys * 128) + s % 4 * 32) / 16,
                    kIdS, s > 0);
           commit(s_full + 8 * t);
+          if (t + C::kIssuers >= tiles) commit(k_free + 8 * st);
         }
       };
       bool go = all_wait(q_full, 0) && all_wait(k_full, 0);
-      if (go) {
-        for (int t = 0; t < tiles; ++t) qk(t, 0);
-        if (lead) commit(k_free);
-      }
+      if (go)
+        for (int t = first; t < tiles; t += C::kIssuers) qk(t, 0);
       for (int j = 0; j < n && go; ++j) {
         const int st = j & 1, next = (j + 1) & 1;
-        for (int t = 0; t < tiles && go; ++t) {
+        for (int t = first; t < tiles && go; t += C::kIssuers) {
           if (j + 1 < n) {
-            go = (t > 0 || all_wait(k_full + 8 * next, (j + 1) / 2)) && all_wait(s_free + 8 * t, j);
+            go = (t > first || all_wait(k_full + 8 * next, (j + 1) / 2)) && all_wait(s_free + 8 * t, j);
             if (!go) break;
             fence_after();
             qk(t, next);
-            if (lead && t + 1 == tiles) commit(k_free + 8 * next);
           }
-          go = all_wait(p_full + 8 * t, j) && (t > 0 || all_wait(v_full + 8 * st, j / 2));
+          go = all_wait(p_full + 8 * t, j) && (t > first || all_wait(v_full + 8 * st, j / 2));
           if (!go) break;
           fence_after();
           const uint64_t vd = mat_desc(v_at + st * C::kKV, kKeys * 128);
@@ -536,14 +550,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             for (int s = 0; s < kKeys / 16; ++s)
               mma_ts(C::kO + t * D, C::kP + t * (kKeys / 2) + s * 8, vd + s * 2048 / 16, kIdO, j > 0 || s > 0);
             commit(o_full + 8 * t);
-            if (t + 1 == tiles) commit(v_free + 8 * st);
+            if (t + C::kIssuers >= tiles) commit(v_free + 8 * st);
           }
         }
       }
       if (!go) {  // let the copy and the products in flight end before their memory goes
         mbar_wait(q_full, 0);
-        if (lead) commit(end);
-        mbar_wait(end, 0);
+        if (lead) commit(end + 8 * first);
+        mbar_wait(end + 8 * first, 0);
       }
     }
   }
