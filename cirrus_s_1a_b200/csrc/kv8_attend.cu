@@ -874,11 +874,11 @@ Plan plan_of(const CbKv8& c, int dtype, int n_q_heads, int T, int longest, bool 
   pl.ml = kCounters * sizeof(int);
   int64_t parts;
   // From 33 rows on the tensor cores' 128-row tiles pay for the rows they leave empty.
-  if (pl.rows > 32 && c.head_dim >= 64 && dtype != CB_F32) {
+  if (pl.rows > 32 && c.head_dim >= 64) {
     pl.row_tiles = ceil_div(pl.rows, 128);
     // runs of key tiles that leave the fewest tile times (and three more a CTA to
     // start and end) on the busiest SM
-    const int items = bh * ceil_div(pl.row_tiles, 2), tiles = ceil_div(longest, 8192 / c.head_dim);
+    const int items = bh * ceil_div(pl.row_tiles, 2), tiles = ceil_div(longest, dtype == CB_F32 ? 64 : 8192 / c.head_dim);
     long best = 0;
     for (int s = 1; s <= 32 && s <= ceil_div(tiles, 2); ++s) {
       const long cost = (long)ceil_div(items * s, num_sms()) * (ceil_div(tiles, s) + 3);
@@ -906,7 +906,7 @@ Plan plan_of(const CbKv8& c, int dtype, int n_q_heads, int T, int longest, bool 
   }
   pl.o = pl.ml + align256((size_t)parts * 2 * sizeof(float));
   pl.q16 = pl.o + align256((size_t)parts * c.head_dim * sizeof(float));
-  pl.back = pl.q16 + (size_t)bh * pl.row_tiles * 128 * c.head_dim * 2;
+  pl.back = pl.q16 + (size_t)bh * pl.row_tiles * 128 * c.head_dim * (dtype == CB_F32 ? 4 : 2);
   pl.scores = pl.back + (size_t)bh * pl.row_tiles * 128 * sizeof(float);
   pl.bytes = pl.scores + (size_t)bh * pl.rows * pl.ld_scores * sizeof(float);
   return pl;
@@ -919,7 +919,7 @@ int check_call(const CbKv8* c, int dtype, int n_q_heads, int T, int longest) {
   const int64_t rows = (int64_t)T * (n_q_heads / c->n_kv_heads);
   if (rows > 65535 * 16) return CB_ERR_SHAPE;
   // a counter for each head and 8 rows
-  if ((rows <= 32 || dtype == CB_F32 || c->head_dim < 64) &&
+  if ((rows <= 32 || c->head_dim < 64) &&
       (rows + 7) / 8 * c->batch * c->n_kv_heads > (int64_t)kCounters)
     return CB_ERR_SHAPE;
   return CB_OK;
@@ -987,7 +987,11 @@ extern "C" int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const
       kv8_join_kernel<<<dim3(ceil_div(p.rows, 1024 / c->head_dim), bh), 256, 0, st>>>(p);
       count_launch();
     }
-    if (p.add_mass) return kv8_prompt_mass_launch(p, bh, longest, st);
+    if (p.add_mass && dtype != CB_F32) return kv8_prompt_mass_launch(p, bh, longest, st);
+    if (p.add_mass) {  // float32 weights: on the warp-level form
+      form_of(*c, dtype, p.rows).mass<<<dim3(ceil_div(longest, kWarps * kKv8Block), bh), kWarps * 32, 0, st>>>(p);
+      count_launch();
+    }
   } else {
     const Form f = form_of(*c, dtype, p.rows);
     if (const int rc = ensure_smem_attr((const void*)f.attend, f.smem)) return rc;

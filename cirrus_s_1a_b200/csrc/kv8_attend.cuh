@@ -33,7 +33,7 @@ struct AttendParams {
   int64_t ld_scores;
   // the prompt form: query rows prepared in 128-row operand tiles, and the factors that undo their scaling
   int row_tiles;
-  uint8_t* q16;         // [batch * kv heads][row_tiles][128 * dim * 2 bytes]
+  uint8_t* q16;         // [batch * kv heads][row_tiles][128 * dim * 2 bytes, float32: twice, head and tail]
   float* q_back;        // [batch * kv heads][row_tiles * 128]
   int32_t* status;
 };

@@ -1,13 +1,13 @@
 // Attention of many query rows over the 8-bit K/V cache on the 5th-generation
-// tensor cores: the prompt form of cb_kv8_attend for head_dim 64 and 128 and
-// 16-bit queries.
+// tensor cores: the prompt form of cb_kv8_attend for head_dim 64 and 128.
 //
 // kv8_query_kernel prepares the query rows once: each scaled by a power of two
 // (largest element in [256, 512)), rounded to f16 and written as swizzled 128-row
-// operand tiles, with the factor that undoes the scaling.
+// operand tiles, with the factor that undoes the scaling; float32 rows as two such
+// tiles, the f16 head and what it leaves.
 //
 // kv8_prompt_kernel: a CTA owns 256 query rows of one KV head (two tiles of 128)
-// and a run of key tiles (128 keys for 64 dims, 64 for 128).
+// and a run of key tiles (128 keys for 64 dims, 64 for 128 and for float32).
 //   * 4 warps turn codes into f16 operands in shared memory (two stages each of K
 //     and V), exact; no scale is applied there.
 //   * one thread (two for 128 dims) issues tcgen05.mma kind::f16: S = Q K^T into tensor memory, and
@@ -37,6 +37,9 @@
 // exponentials 696, turns passed on at half 624), Q K^T and P V issued by two warps (641).
 // For 128 dims, 2 x 1000 tokens at up to 8K (171 us then): tiles of 128 keys with P in
 // the columns of its scores (180), a second P a tile (171).
+// float32, heads and tails of Q and of P as products of their own: 5 x 191 tokens at up
+// to 15.5K, 8 query heads of 128 dims 129 us, 4096 tokens behind 28600 as above 852 us
+// (twice the products; the warp-level form took 1345 us for the first).
 // Every wait is bounded (%globaltimer); a wait that gives up sets CB_ERR_TIMEOUT
 // in the status word, and the CTA ends without writing results.
 #include <climits>
@@ -166,7 +169,7 @@ __device__ __forceinline__ int row_limit(const AttendParams& p, int r, int pos, 
 
 // ------------------------------------------------------------------ queries
 // D/8 lanes per row, 8 elements each.
-template <int D>
+template <int D, int HL>
 __global__ void __launch_bounds__(256) kv8_query_kernel(const __grid_constant__ AttendParams p) {
   constexpr int kLanes = D / 8;
   const int64_t head = blockIdx.y;
@@ -188,42 +191,58 @@ __global__ void __launch_bounds__(256) kv8_query_kernel(const __grid_constant__ 
   int e = 0;
   if (top > 0.0f && top < INFINITY) e = min(max((__float_as_int(top) >> 23) - 127, -100), 100);
   const float f = copysignf(kv8_pow2(8 - e), p.scale);
-  uint32_t h[4];
+  uint8_t* tile = p.q16 + (head * p.row_tiles + r / kRows) * (int64_t)((1 + HL) * kRows * D * 2);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = h2_bits(__floats2half2_rn(x[2 * i] * f, x[2 * i + 1] * f));
-  uint8_t* tile = p.q16 + (head * p.row_tiles + r / kRows) * (int64_t)(kRows * D * 2);
-  *reinterpret_cast<uint4*>(tile + swizzled<kRows>(r % kRows, kb)) = make_uint4(h[0], h[1], h[2], h[3]);
+  for (int part = 0; part <= HL; ++part) {  // head, and what it leaves
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float y0 = part ? x[2 * i] : x[2 * i] * f, y1 = part ? x[2 * i + 1] : x[2 * i + 1] * f;
+      const __half2 y = __floats2half2_rn(y0, y1);
+      h[i] = h2_bits(y);
+      x[2 * i] = y0 - __low2float(y);
+      x[2 * i + 1] = y1 - __high2float(y);
+    }
+    *reinterpret_cast<uint4*>(tile + part * kRows * D * 2 + swizzled<kRows>(r % kRows, kb)) =
+        make_uint4(h[0], h[1], h[2], h[3]);
+  }
   if (kb == 0) p.q_back[head * p.row_tiles * kRows + r] = live ? kv8_pow2(e - 8) * fabsf(p.scale) * kLog2e : 0.0f;
 }
 
 // --------------------------------------------------------------- attention
-template <int D>
+// HL: float32 queries, carried as f16 head and tail, and so is P (22 bits).
+template <int D, int HL>
 struct Prompt {
-  static constexpr int kKeys = 8192 / D;        // of a key tile: S, P and O of two tiles fill tensor memory
+  static constexpr int kKeys = HL ? 64 : 8192 / D;  // of a key tile: S, P and O of two tiles fit tensor memory
   static constexpr int kHalves = kKeys / kKv8Block;
-  static constexpr int kQ = kRows * D * 2;      // bytes of a query tile
+  static constexpr int kHead = kRows * D * 2;
+  static constexpr int kQ = (1 + HL) * kHead;   // bytes of a query tile
   static constexpr int kKV = kKeys * D * 2;     // of a K or V tile
   static constexpr int kSmem = kTiles * kQ + 2 * kStages * kKV + 1024;
   // tensor memory: S, P (f16, half as many columns) and O of both tiles
+  static constexpr int kPCols = (1 + HL) * kKeys / 2;
   static constexpr int kP = kTiles * kKeys, kO = 512 - kTiles * D;
-  static_assert(kP + kTiles * kKeys / 2 <= kO, "S, P and O fit 512 columns");
+  static_assert(kP + kTiles * kPCols <= kO, "S, P and O fit 512 columns");
+  // What the row's largest P lies above 1, in powers of two: with a tail of P, its last
+  // bit (2^-24, the smallest f16) then is 2^-35 of the largest, and O follows growth by 2^4.
+  static constexpr float kLift = HL ? 11.0f : 0.0f;
   // Warps that issue the products.  One keeps two tiles of 128 keys busy, in a fixed
   // order that keeps the softmax warpgroups out of step (64 dims, 4096 tokens at 32K:
   // 584 us, a warp to each tile 637).  With 64 keys its own waits and issue bounded a
   // tile (128 dims, 2 x 1000 tokens at 8K with weights: 171 us
   // with one warp, 161 with two; 2048 tokens at 32K: 341, 327).
-  static constexpr int kIssuers = D == 128 ? 2 : 1;
+  static constexpr int kIssuers = kKeys == 64 ? 2 : 1;
   // With 64 scores a thread, the softmax leaves registers to the others.
-  static constexpr int kSoftRegs = D == 128 ? 160 : cb::kSoftRegs, kConvRegs = D == 128 ? 104 : cb::kConvRegs,
-                       kMmaRegs = D == 128 ? 88 : cb::kMmaRegs;
+  static constexpr int kSoftRegs = kKeys == 64 ? 160 : cb::kSoftRegs, kConvRegs = kKeys == 64 ? 104 : cb::kConvRegs,
+                       kMmaRegs = kKeys == 64 ? 88 : cb::kMmaRegs;
   static_assert(2 * kSoftRegs + kConvRegs + kMmaRegs <= 4 * 128, "the shares fit what the block was launched with");
   static constexpr int kPieces = kKeys * D / 16 / kConvThreads;  // 16-byte pieces of a tile per converting thread
   static constexpr int kRow = D / 16;                            // of a key
 };
 
-template <int D, int FMT>
+template <int D, int FMT, int HL>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_constant__ AttendParams p) {
-  using C = Prompt<D>;
+  using C = Prompt<D, HL>;
   constexpr int kKeys = C::kKeys, kHalves = C::kHalves;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);  // the swizzle counts from 1024-byte boundaries
@@ -291,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     const int tile = warp / 4, r = row0 + tile * kRows + (warp % 4) * 32 + lane;
     if (tile < tiles) {
       const uint32_t lanes = (uint32_t)(warp % 4) << 21;  // this warp's lanes of tensor memory (bits 16-31)
-      const uint32_t ts = tmem + lanes + tile * kKeys, tp = tmem + lanes + C::kP + tile * (kKeys / 2),
+      const uint32_t ts = tmem + lanes + tile * kKeys, tp = tmem + lanes + C::kP + tile * C::kPCols,
                      to = tmem + lanes + C::kO + tile * D;
       const int lim = row_limit(p, r, pos, cnt);
       const float back = p.q_back[head * p.row_tiles * kRows + r];
@@ -356,8 +375,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           fence_after();
         }
         if (__any_sync(0xffffffffu, grow)) {
-          const float alpha = !grow ? 1.0f : m > -INFINITY ? exp2a(m - now) : 0.0f;
-          if (grow) m = now;
+          const float ref = now - C::kLift, alpha = !grow ? 1.0f : m > -INFINITY ? exp2a(m - ref) : 0.0f;
+          if (grow) m = ref;
           l *= alpha;
           if (j > 0) {
 #pragma unroll
@@ -379,15 +398,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           f32x2 sum[2] = {0, 0};  // pairs of zeros
 #pragma unroll
           for (int q = 2 * h; q < 2 * h + 2; ++q) {
-            uint32_t ph[16];
+            uint32_t ph[16], pt[HL ? 16 : 1];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const float2 d = unpack2(fma2(pack2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), a2, c2));
               const float y0 = exp2a(d.x), y1 = exp2a(d.y);
               sum[i & 1] = add2(sum[i & 1], pack2(y0, y1));
-              ph[i] = h2_bits(__floats2half2_rn(y0, y1));
+              const __half2 y = __floats2half2_rn(y0, y1);
+              ph[i] = h2_bits(y);
+              if constexpr (HL > 0) pt[i] = h2_bits(__floats2half2_rn(y0 - __low2float(y), y1 - __high2float(y)));
             }
             tmem_st16(tp + q * 16, ph);
+            if constexpr (HL > 0) tmem_st16(tp + kKeys / 2 + q * 16, pt);
           }
           const float2 both = unpack2(add2(sum[0], sum[1]));
           sum_l = fmaf(both.x + both.y, kv8_pow2(min(max(e_ref - ev[h], -100), 100)), sum_l);
@@ -421,6 +443,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + c);
 #pragma unroll
           for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else if constexpr (HL > 0) {
+          float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + orow * D + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            dst[i] = make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
         } else {
           uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + orow * D + c);
           uint32_t u[16];
@@ -522,9 +549,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         const uint64_t qd = mat_desc(q_at + t * C::kQ, 16), kd = mat_desc(k_at + st * C::kKV, 16);
         if (lead) {
 #pragma unroll
-          for (int s = 0; s < D / 16; ++s)
-            mma_ss(t * kKeys, qd + (s / 4 * (kRows * 128) + s % 4 * 32) / 16, kd + (s / 4 * (kKeys * 128) + s % 4 * 32) / 16,
-                   kIdS, s > 0);
+          for (int s = 0; s < (1 + HL) * (D / 16); ++s) {
+            const int k = s % (D / 16);
+            mma_ss(t * kKeys, qd + (s / (D / 16) * C::kHead + k / 4 * (kRows * 128) + k % 4 * 32) / 16,
+                   kd + (k / 4 * (kKeys * 128) + k % 4 * 32) / 16, kIdS, s > 0);
+          }
           commit(s_full + 8 * t);
           if (t + C::kIssuers >= tiles) commit(k_free + 8 * st);
         }
@@ -547,8 +576,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           const uint64_t vd = mat_desc(v_at + st * C::kKV, kKeys * 128);
           if (lead) {
 #pragma unroll
-            for (int s = 0; s < kKeys / 16; ++s)
-              mma_ts(C::kO + t * D, C::kP + t * (kKeys / 2) + s * 8, vd + s * 2048 / 16, kIdO, j > 0 || s > 0);
+            for (int s = 0; s < C::kPCols / 8; ++s)
+              mma_ts(C::kO + t * D, C::kP + t * C::kPCols + s * 8, vd + s % (kKeys / 16) * 2048 / 16, kIdO, j > 0 || s > 0);
             commit(o_full + 8 * t);
             if (t + C::kIssuers >= tiles) commit(v_free + 8 * st);
           }
@@ -742,14 +771,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(s_tmem));
 }
 
-template <int D>
+template <int D, int HL>
 int launch_prompt(const AttendParams& p, int bh, cudaStream_t st) {
-  kv8_query_kernel<D><<<dim3(ceil_div(p.row_tiles * kRows * (D / 8), 256), bh), 256, 0, st>>>(p);
+  kv8_query_kernel<D, HL><<<dim3(ceil_div(p.row_tiles * kRows * (D / 8), 256), bh), 256, 0, st>>>(p);
   count_launch();
   const dim3 grid(ceil_div(p.row_tiles, kTiles) * p.splits, bh);
-  auto fn = p.c.format == CB_KV8_E4M3 ? kv8_prompt_kernel<D, CB_KV8_E4M3> : kv8_prompt_kernel<D, CB_KV8_INT8>;
-  if (const int rc = ensure_smem_attr((const void*)fn, Prompt<D>::kSmem)) return rc;
-  fn<<<grid, kThreads, Prompt<D>::kSmem, st>>>(p);
+  constexpr int kSmem = Prompt<D, HL>::kSmem;
+  auto fn = p.c.format == CB_KV8_E4M3 ? kv8_prompt_kernel<D, CB_KV8_E4M3, HL> : kv8_prompt_kernel<D, CB_KV8_INT8, HL>;
+  if (const int rc = ensure_smem_attr((const void*)fn, kSmem)) return rc;
+  fn<<<grid, kThreads, kSmem, st>>>(p);
   count_launch();
   return cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
 }
@@ -768,7 +798,8 @@ int kv8_prompt_mass_launch(const AttendParams& p, int bh, int longest, cudaStrea
 }
 
 int kv8_prompt_launch(const AttendParams& p, int bh, cudaStream_t st) {
-  return p.c.head_dim == 64 ? launch_prompt<64>(p, bh, st) : launch_prompt<128>(p, bh, st);
+  if (p.dtype == CB_F32) return p.c.head_dim == 64 ? launch_prompt<64, 1>(p, bh, st) : launch_prompt<128, 1>(p, bh, st);
+  return p.c.head_dim == 64 ? launch_prompt<64, 0>(p, bh, st) : launch_prompt<128, 0>(p, bh, st);
 }
 
 }  // namespace cb
