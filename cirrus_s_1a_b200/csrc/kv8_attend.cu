@@ -873,7 +873,9 @@ Plan plan_of(const CbKv8& c, int dtype, int n_q_heads, int T, int longest, bool 
   pl.rows = T * (n_q_heads / c.n_kv_heads);
   pl.ml = kCounters * sizeof(int);
   int64_t parts;
-  // From 33 rows on the tensor cores' 128-row tiles pay for the rows they leave empty.
+  // From 33 rows on the tensor cores' 128-row tiles pay for the rows they leave empty
+  // (float32, 128 dims: 16 sequences x 36 rows at 2K 29 us, 40 on the warp-level form; one
+  // of 80 rows at 32K 45 and 49, but of 36 rows 47 and 38).
   if (pl.rows > 32 && c.head_dim >= 64) {
     pl.row_tiles = ceil_div(pl.rows, 128);
     // runs of key tiles that leave the fewest tile times (and three more a CTA to
@@ -987,11 +989,7 @@ extern "C" int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const
       kv8_join_kernel<<<dim3(ceil_div(p.rows, 1024 / c->head_dim), bh), 256, 0, st>>>(p);
       count_launch();
     }
-    if (p.add_mass && dtype != CB_F32) return kv8_prompt_mass_launch(p, bh, longest, st);
-    if (p.add_mass) {  // float32 weights: on the warp-level form
-      form_of(*c, dtype, p.rows).mass<<<dim3(ceil_div(longest, kWarps * kKv8Block), bh), kWarps * 32, 0, st>>>(p);
-      count_launch();
-    }
+    if (p.add_mass) return kv8_prompt_mass_launch(p, bh, longest, st);
   } else {
     const Form f = form_of(*c, dtype, p.rows);
     if (const int rc = ensure_smem_attr((const void*)f.attend, f.smem)) return rc;

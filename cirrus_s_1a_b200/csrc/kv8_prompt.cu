@@ -38,8 +38,8 @@
 // For 128 dims, 2 x 1000 tokens at up to 8K (171 us then): tiles of 128 keys with P in
 // the columns of its scores (180), a second P a tile (171).
 // float32, heads and tails of Q and of P as products of their own: 5 x 191 tokens at up
-// to 15.5K, 8 query heads of 128 dims 129 us, 4096 tokens behind 28600 as above 852 us
-// (twice the products; the warp-level form took 1345 us for the first).
+// to 15.5K, 8 query heads of 128 dims 130 us, 4096 tokens behind 28600 as above 853 us
+// (twice the products; the warp-level form took 383 and 3287 us).
 // Every wait is bounded (%globaltimer); a wait that gives up sets CB_ERR_TIMEOUT
 // in the status word, and the CTA ends without writing results.
 #include <climits>
@@ -606,20 +606,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 // buffers of tensor memory, two warpgroups take them in turn.  Bound by the
 // exponentials and by whole CTAs to an SM: 2 x 1000 tokens at up to 8K, 8 query heads
 // of 128 dims: 69 us (206 key tiles on 148 SMs), the exponential unit 60 % busy.
-constexpr int kMassStages = 4;
-template <int D>
+// (float32 queries of 128 dims, with their tails: two stages and two buffers.)
+template <int D, int HL>
 struct Mass {
-  static constexpr int kQ = kRows * D * 2;
+  static constexpr int kStages = HL && D == 128 ? 2 : 4;
+  static constexpr int kHead = kRows * D * 2;
+  static constexpr int kQ = (1 + HL) * kHead;
   static constexpr int kInfo = kRows * 8;  // of each row: the factor of its scores, and -lse (log2 units)
-  static constexpr int kSmem = kQ + kMassStages * (kQ + kInfo) + 1024;
+  static constexpr int kSmem = kHead + kStages * (kQ + kInfo) + 1024;
 };
 
-template <int D, int FMT>
+template <int D, int FMT, int HL>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __grid_constant__ AttendParams p) {
-  using C = Mass<D>;
+  using C = Mass<D, HL>;
+  constexpr int kMassStages = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sk = smem_raw + (-smem_u32(smem_raw) & 1023);
-  uint8_t* sq = sk + C::kQ;
+  uint8_t* sq = sk + C::kHead;
   float* s_info = reinterpret_cast<float*>(sq + kMassStages * C::kQ);  // [stage][2][128]
   __shared__ __align__(8) unsigned long long bars[3 * kMassStages + 1];
   __shared__ uint32_t s_tmem;
@@ -749,9 +752,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
         const uint64_t kd = mat_desc(k_at, 16), qd = mat_desc(q_at + st * C::kQ, 16);
         if (lead) {
 #pragma unroll
-          for (int s = 0; s < D / 16; ++s)
-            mma_ss(st * kRows, kd + (s / 4 * (kRows * 128) + s % 4 * 32) / 16,
-                   qd + (s / 4 * (kRows * 128) + s % 4 * 32) / 16, idesc(kRows, kRows, false), s > 0);
+          for (int s = 0; s < (1 + HL) * (D / 16); ++s) {
+            const int k16 = s % (D / 16), at = k16 / 4 * (kRows * 128) + k16 % 4 * 32;
+            mma_ss(st * kRows, kd + at / 16, qd + (s / (D / 16) * C::kHead + at) / 16, idesc(kRows, kRows, false), s > 0);
+          }
           commit(s_full + 8 * st);
           commit(q_free + 8 * st);
         }
@@ -784,17 +788,23 @@ int launch_prompt(const AttendParams& p, int bh, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
 }
 
+template <int D, int HL>
+int launch_mass(const AttendParams& p, int bh, int longest, cudaStream_t st) {
+  constexpr int kSmem = Mass<D, HL>::kSmem;
+  auto fn = p.c.format == CB_KV8_E4M3 ? kv8_prompt_mass_kernel<D, CB_KV8_E4M3, HL>
+                                      : kv8_prompt_mass_kernel<D, CB_KV8_INT8, HL>;
+  if (const int rc = ensure_smem_attr((const void*)fn, kSmem)) return rc;
+  fn<<<dim3(ceil_div(longest, kRows), bh), kThreads, kSmem, st>>>(p);
+  count_launch();
+  return cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
+}
+
 }  // namespace
 
 int kv8_prompt_mass_launch(const AttendParams& p, int bh, int longest, cudaStream_t st) {
-  const bool e = p.c.format == CB_KV8_E4M3, narrow = p.c.head_dim == 64;
-  auto fn = narrow ? (e ? kv8_prompt_mass_kernel<64, CB_KV8_E4M3> : kv8_prompt_mass_kernel<64, CB_KV8_INT8>)
-                   : (e ? kv8_prompt_mass_kernel<128, CB_KV8_E4M3> : kv8_prompt_mass_kernel<128, CB_KV8_INT8>);
-  const int smem = narrow ? Mass<64>::kSmem : Mass<128>::kSmem;
-  if (const int rc = ensure_smem_attr((const void*)fn, smem)) return rc;
-  fn<<<dim3(ceil_div(longest, kRows), bh), kThreads, smem, st>>>(p);
-  count_launch();
-  return cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
+  if (p.dtype == CB_F32)
+    return p.c.head_dim == 64 ? launch_mass<64, 1>(p, bh, longest, st) : launch_mass<128, 1>(p, bh, longest, st);
+  return p.c.head_dim == 64 ? launch_mass<64, 0>(p, bh, longest, st) : launch_mass<128, 0>(p, bh, longest, st);
 }
 
 int kv8_prompt_launch(const AttendParams& p, int bh, cudaStream_t st) {
