@@ -31,7 +31,7 @@
 // clock take 1024 clocks, its products 512.
 // With several runs per row tile, kv8_join_kernel joins them (kv8_attend.cu).
 // Measured: 4096 tokens behind 28600, 12 query heads on 4 KV heads of 64 dims, E4M3:
-// 597 us = 646 TFLOP/s, the exponential unit 67 % busy, the tensor pipe 33 %.  Tried
+// 582 us = 663 TFLOP/s, the exponential unit 67 % busy, the tensor pipe 33 %.  Tried
 // and slower: a share of the exponentials as a polynomial on the FMA units (636 to
 // 757 us, at 639 then), three row tiles of 64 keys (703; with strict turns at the
 // exponentials 696, turns passed on at half 624), Q K^T and P V issued by two warps (641).

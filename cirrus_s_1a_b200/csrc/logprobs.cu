@@ -23,7 +23,7 @@
 //
 // Bound by memory in principle (the row once), by issue in fact (77 % of the slots;
 // the pass widens, compares, scales, exponentiates and adds each value).  Measured: 16384 rows of 32000 in bf16,
-// 20 alternatives: 248 to 265 us = 4.2 TB/s; without alternatives 197 us = 5.3 TB/s; five
+// 20 alternatives: 248 to 272 us = 4 TB/s; without alternatives 197 us = 5.3 TB/s; five
 // rows in float32: 17 us, the host's part of the call.
 #include "common.cuh"
 #include "kv8.cuh"
