@@ -61,22 +61,29 @@ __device__ __forceinline__ unsigned long long top_key(float v, int i) {
   return ((unsigned long long)score_key(v) << 32) | (uint32_t)~i;
 }
 
-// Running maximum m of one thread, and relative to c = m * log2(e) (rounded: every
-// term is taken against the rounded c, so its rounding cancels) the sums
-// l = sum 2^(x log2(e) - c) and t = sum of exponent * 2^exponent, each in two
-// halves.  Where |m| * log2(e) nears the end of float32 (kFar), c is 0 and the
-// exponents are (x - m) log2(e).
-constexpr float kFar = 2e38f, kFloor = -200.0f;
+// Running maximum m of one thread, and relative to a reference c near m * log2(e) the
+// sums l = sum 2^(x log2(e) - c) and t = sum of exponent * 2^exponent, each in two
+// halves.  Up to kFar, c is m * log2(e) rounded and every term is taken against the
+// rounded value by one fused operation, so what the rounding leaves (up to half an ulp of
+// c, 2^-4 there) is a factor common to all of them and cancels.  Beyond, that factor would
+// leave the range of float32, and values 150 below m are no longer told from m: c is
+// m * log2(e) itself and the exponents are (x - m) log2(e).
+constexpr float kFar = 1048576.0f, kFloor = -200.0f;
+constexpr float kHuge = 2e38f;  // from here on x * log2(e) overflows
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar; }
 struct Stat {
   float m = -INFINITY;
   f32x2 l = 0, t = 0;  // two zeros each
-  __device__ __forceinline__ bool far() const { return fabsf(m) > kFar; }
+  __device__ __forceinline__ bool far() const { return is_far(m); }
   __device__ __forceinline__ float c() const { return __fmul_rn(m, kLog2e); }
   __device__ __forceinline__ void raise(float top) {
     if (top > m) {
       if (m > -INFINITY) {
-        const bool exact = far() || fabsf(top) > kFar;
-        const float d = fmaxf(exact ? (m - top) * kLog2e : c() - __fmul_rn(top, kLog2e), kFloor), f = exp2a(d);
+        // from one reference to the other, whichever kind each is
+        const float to = __fmul_rn(top, kLog2e);
+        const float by = is_far(top) ? (far() ? (m - top) * kLog2e : -fmaf(top, kLog2e, -c()))
+                                     : (far() ? fmaf(m, kLog2e, -to) : c() - to);
+        const float d = fmaxf(by, kFloor), f = exp2a(d);
         t = mul2(fma2(pack2(d, d), l, t), pack2(f, f));
         l = mul2(l, pack2(f, f));
       }
@@ -166,9 +173,9 @@ struct Vec<__half> : Vec16<__half2> {
   __device__ __forceinline__ void above(float xt, Count& c) const { above2(__float2half2_rn(xt), c); }
 };
 
-// COUNT vectors, STEP values apart from `at` on, into a thread's sums.
-template <typename T, int COUNT, int STEP>
-__device__ __forceinline__ void add_vecs(const T* at, Vec<T> (&v)[COUNT], Stat& s, typename Vec<T>::Floor& floor) {
+// COUNT vectors into a thread's sums.
+template <typename T, int COUNT>
+__device__ __forceinline__ void add_vecs(Vec<T> (&v)[COUNT], Stat& s, typename Vec<T>::Floor& floor) {
   constexpr int N = Vec<T>::N;
   float top = v[0].max();
 #pragma unroll
@@ -191,9 +198,11 @@ __device__ __forceinline__ void add_vecs(const T* at, Vec<T> (&v)[COUNT], Stat& 
         s.t = fma2(d, e, s.t);
       }
     }
-  } else {  // nothing finite yet, or the far ends of the range
-#pragma unroll 1
-    for (int i = 0; i < COUNT * N; ++i) s.add(to_f(at[i / N * STEP + i % N]));
+  } else {  // nothing finite yet, far from zero, or a floor past the type's range
+#pragma unroll
+    for (int u = 0; u < COUNT; ++u)
+#pragma unroll
+      for (int i = 0; i < N; ++i) s.add(v[u].get(i));
   }
 }
 
@@ -247,12 +256,12 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const __grid_constan
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) v[u].above(xt, count);
     above += count.take();
-    add_vecs<T, kBatch, NT * N>(at, v, s, floor);
+    add_vecs<T, kBatch>(v, s, floor);
   }
   for (; j < vecs; j += NT, at += NT * N) {
     Vec<T> v[1] = {load_vec(at)};
     v[0].above(xt, count);
-    add_vecs<T, 1, 0>(at, v, s, floor);
+    add_vecs<T, 1>(v, s, floor);
   }
   above += count.take();
   // the edge goes to the last threads
@@ -317,7 +326,9 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const __grid_constan
   s.m = m;
   const float c0 = s.c();
   const bool far = s.far();
-  auto logp = [&](float x) { return far || fabsf(x) > kFar ? (x - m) - log2l * kLn2 : (fmaf(x, kLog2e, -c0) - log2l) * kLn2; };
+  auto logp = [&](float x) {
+    return far || fabsf(x) > kHuge ? (x - m) - log2l * kLn2 : (fmaf(x, kLog2e, -c0) - log2l) * kLn2;
+  };
   if (tid == 0) {
     int n = 0;
     for (int w = 0; w < kWarps; ++w) n += s_above[w];

@@ -75,6 +75,31 @@ def test_ties_masks_and_extremes(dtype, V):
     check(x, [V - 1, 0, 0, 0, 0, 0, 0, V - 1, 0], 32)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V", [32000, 777])
+def test_rows_far_from_zero(dtype, V):
+    """Masks by a finite value of any size, rows that hold nothing else, and logits around
+    2^20 and up to the ends of the range (the bounds of ``check`` hold over all of it)."""
+    g = torch.Generator().manual_seed(V + 1)
+    few = torch.rand(V, generator=g) < 0.02
+    few[V // 2] = True
+    rows = []
+    for mask in (-1e4, -1e9, -1e10, -1e20, -1e30, -3.3e38):
+        rows += [torch.where(few, torch.randn(V, generator=g) * 3, mask), torch.full((V,), mask)]
+    for peak in (2e9, 1e10, 1e30, 3.3e38):
+        one = torch.zeros(V)
+        one[V // 3] = peak
+        rows += [one, torch.full((V,), peak)]
+    for centre in (2.0 ** 10, -(2.0 ** 10), 2.0 ** 20, -(2.0 ** 20), 2.0 ** 24, -(2.0 ** 24)):
+        rows.append(centre + (torch.randn(V, generator=g) * 3).round())
+    x = torch.stack(rows)
+    top = torch.finfo(TYPES[dtype]).max
+    x = x.clamp(-top, top).to(TYPES[dtype])
+    tokens = [int(r.argmax()) if i % 2 else (V // 2 + i) % V for i, r in enumerate(x)]
+    check(x, tokens, 20)
+    check(x, tokens[::-1], 0)
+
+
 def test_rows_of_any_stride_and_alignment():
     g = torch.Generator().manual_seed(1)
     for dtype in TYPES.values():
