@@ -88,6 +88,24 @@ __device__ __forceinline__ float exp2a(float x) {
   return y;
 }
 
+// A sum of 2^x against a maximum, besides a row's own: rarely needed, so in shared memory.
+struct Aside {
+  float m, l;
+  __device__ __forceinline__ void clear() { m = -INFINITY, l = 0.0f; }
+  __device__ __forceinline__ void raise(float to) {
+    if (to > m) {
+      l *= exp2a(m - to);  // 0 of the 0 it starts with
+      m = to;
+    }
+  }
+  __device__ __forceinline__ void add(float ref, float sum) {  // sum * 2^ref
+    if (sum != 0.0f) {
+      raise(ref);
+      l = fmaf(sum, exp2a(ref - m), l);
+    }
+  }
+};
+
 // The larger of two; NaN if either is one.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;

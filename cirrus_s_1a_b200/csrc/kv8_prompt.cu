@@ -19,8 +19,10 @@
 //       P = exp2(x + e_b - m')
 //     so that P times the bare codes is the sum over values, and neither a block
 //     of tiny values nor one of huge ones costs the others precision: P's f16
-//     rounding is relative to what the row adds up.  The row's sum is
-//     l = sum_b 2^-e_b sum P (before P is rounded), the same in float32.
+//     rounding is relative to what the row adds up.  The row's sum (before P is rounded)
+//     is l = sum_b 2^(e_ref - e_b) sum P against m = m' - e_ref, with an e_ref near the
+//     blocks' exponents; blocks far below it (zeros) are summed for themselves (kNear).
+//     out = 2^(m' - m) O / l.
 //   * a thread reads its row of S into registers at once, so that the next tile's
 //     scores can follow, and takes P against the maximum so far.  Only where the
 //     tile's passes it by more than 2^15 (f16 P ends at 2^16) is it raised, and O
@@ -249,6 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   __shared__ __align__(8) unsigned long long bars[20];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
+  __shared__ Aside s_aside[kTiles * kRows];
   __shared__ int s_nan;  // the first E4M3 NaN among values that not all rows see
   uint8_t* sq = smem;
   uint8_t* sk = smem + kTiles * C::kQ;
@@ -318,7 +321,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       const float* vsc = p.c.v_scale + head * (p.c.max_len / kKv8Block);
       const int vis = last / kKv8Block;  // the last block any row sees
       float m = -INFINITY, l = 0.0f;
-      const int e_ref = n > 0 ? kv8_exponent(vsc[kHalves * beg]) : 0;
+      Aside& aside = s_aside[tid];
+      aside.clear();
+      // the run's largest value exponent, and whether any lies far below it
+      int e_ref = 0;
+      bool wide = false;
+      {
+        uint32_t most = 0u, least = ~0u;  // bits of positive floats
+        for (int blk = kHalves * beg + lane; blk <= min(vis, kHalves * (beg + n) - 1); blk += 32) {
+          const uint32_t u = __float_as_uint(__ldg(vsc + blk));
+          most = max(most, u), least = min(least, u);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        least = __reduce_min_sync(0xffffffffu, least);
+        if (n > 0) {
+          e_ref = kv8_exponent(__uint_as_float(most));
+          wide = kv8_exponent(__uint_as_float(least)) < e_ref - kNear;
+        }
+      }
       float ks[kHalves], vs[kHalves];
       auto scales = [&](int j) {
 #pragma unroll
@@ -341,6 +361,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         if (j + 1 < n) scales(j + 1);
         if (!wait(s_full + 8 * tile, j)) break;
         fence_after();
+        if (wide && min(ev[0], ev[kHalves - 1]) < e_ref - kNear) {
+#pragma unroll 1
+          for (int q = 0; q < kKeys / 16; ++q) {
+            const bool first = q < kKv8Block / 16;
+            if ((first ? ev[0] : ev[kHalves - 1]) >= e_ref - kNear) continue;
+            const float by = first ? a[0] : a[kHalves - 1];
+            uint32_t u[16];
+            tmem_ld16(ts + q * 16, u);
+            tmem_ld_wait();
+            float x = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (key0 + q * 16 + i > lim) u[i] = __float_as_uint(-INFINITY);
+              x = fmaxf(x, __uint_as_float(u[i]));
+            }
+            if (x > -INFINITY) {
+              aside.raise(x * by);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) aside.l += exp2a(fmaf(__uint_as_float(u[i]), by, -aside.m));
+            }
+            __syncwarp();
+          }
+        }
         const bool whole = __all_sync(0xffffffffu, lim >= key0 + kKeys - 1);
         float s[kKeys];
 #pragma unroll
@@ -412,22 +455,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             if constexpr (HL > 0) tmem_st16(tp + kKeys / 2 + q * 16, pt);
           }
           const float2 both = unpack2(add2(sum[0], sum[1]));
-          sum_l = fmaf(both.x + both.y, kv8_pow2(min(max(e_ref - ev[h], -100), 100)), sum_l);
+          const int d = e_ref - ev[h];  // 2^-127 is written as 0
+          sum_l = fmaf(both.x + both.y, kv8_pow2(d > kNear ? -127 : d), sum_l);
         }
         l += sum_l;
         tmem_st_wait();
         fence_before();
         mbar_arrive(p_full + 8 * tile);
       }
-      // results: O, m' and l (against e_ref).  (Products n - 2 and before are known done.)
+      // results: O, m', and l against mx.  (Products n - 2 and before are known done.)
       if (n > 0) wait(o_full + 8 * tile, n - 1);
       fence_after();
-      float lsum = l * kv8_pow2(-e_ref);
-      if (FMT == CB_KV8_E4M3 && n > 0 && s_nan <= lim) lsum = NAN;
+      float mx = m - (float)e_ref;
+      if (aside.l != 0.0f) {
+        aside.add(mx, l);
+        mx = aside.m;
+        l = aside.l;
+      }
+      if (FMT == CB_KV8_E4M3 && n > 0 && s_nan <= lim) l = NAN;
       const int t = r / p.G, hq = (int)(head % p.c.n_kv_heads) * p.G + r % p.G;
       const int64_t orow = ((int64_t)b * p.T + t) * (p.G * p.c.n_kv_heads) + hq;
       const int64_t at = (head * p.rows + r) * p.splits + split;
-      const float inv = m > -INFINITY ? 1.0f / lsum : 0.0f;
+      // 2^(m' - m) / l in two factors: an exponent of up to 135 times a small sum
+      const float half = mx > -INFINITY ? exp2a(0.5f * (m - mx)) : 0.0f, inv = mx > -INFINITY ? half / l : 0.0f;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         float o[32];
@@ -436,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           tmem_ld_wait();
         }
         if (r >= p.rows || !ok) continue;
-        if (m == -INFINITY)
+        if (mx == -INFINITY)
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0.0f;
         if (p.splits > 1) {
@@ -447,13 +497,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + orow * D + c);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            dst[i] = make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
+            dst[i] = make_float4(o[4 * i] * half * inv, o[4 * i + 1] * half * inv, o[4 * i + 2] * half * inv,
+                                 o[4 * i + 3] * half * inv);
         } else {
           uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + orow * D + c);
           uint32_t u[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float y0 = o[2 * i] * inv, y1 = o[2 * i + 1] * inv;
+            const float y0 = o[2 * i] * half * inv, y1 = o[2 * i + 1] * half * inv;
             u[i] = p.dtype == CB_BF16 ? (uint32_t)f32_to_bf16(y0) | (uint32_t)f32_to_bf16(y1) << 16
                                       : h2_bits(__floats2half2_rn(y0, y1));
           }
@@ -463,10 +514,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       }
       if (r < p.rows && ok) {
         if (p.splits > 1) {
-          p.part_ml[2 * at] = m;
-          p.part_ml[2 * at + 1] = lsum;
+          p.part_ml[at] = make_float4(m, mx, l, 0.0f);
         } else {
-          p.lse[orow] = m > -INFINITY ? (m + log2f(lsum)) * kLn2 : -INFINITY;
+          p.lse[orow] = mx > -INFINITY ? (mx + log2f(l)) * kLn2 : -INFINITY;
         }
       }
     }

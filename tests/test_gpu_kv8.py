@@ -226,6 +226,26 @@ def test_block_scales_twenty_octaves_apart(T):
     assert (out[:, :rows].cpu().double() - want[:, :rows]).abs().max() <= 127 * 2.0 ** -27 * 2.0 ** -10
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,T", [(64, 1), (64, 140), (128, 1), (128, 140), (16, 6)])
+@pytest.mark.parametrize("e", [1, 10, 30, 110])
+def test_value_blocks_of_zeros_beside_large_ones(fmt, dtype, D, T, e):
+    """A block of zero values has the scale 2^-100: its keys weigh as much as any others',
+    wherever it lies, and so do those of a block whose values are as small as that."""
+    cache = filled(1, 2, D, 704, fmt, seed=e)
+    for h, zero in ((0, (0, 4)), (1, (3, 7, 8))):
+        cache.v_scale[0, h] = torch.exp2(torch.randint(e - 2, e + 1, (11,), generator=torch.Generator().manual_seed(h)))
+        for blk in zero:
+            cache.v_scale[0, h, blk] = 2.0 ** -100
+            if blk != 7:
+                cache.v.view(torch.uint8)[0, h, 64 * blk:64 * blk + 64] = 0
+    q = (1.5 * torch.randn(1, T, 6, D, generator=torch.Generator().manual_seed(T))).to(TYPES[dtype])
+    check_attend(cache, q, [700 - T], dtype=dtype, add_mass=True)
+    # only keys of zero values, then one block of others
+    check_attend(cache, q, [max(63 - T, 0)], dtype=dtype, add_mass=True)
+
+
 @pytest.mark.parametrize("T", [1, 130])
 def test_peaked_and_extreme_scores(T):
     """Scores of thousands (one key takes all), queries of 1e-30 (all keys alike) and zeros."""
