@@ -94,8 +94,9 @@ __device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t (&w)[(N + 
 
 // Query rows row0 .. row0 + 8 NT - 1 of a KV head as right operands: lane (g, t)
 // feeds row g of each eight.  `back`: the factors that undo the powers of two, times
-// scale * log2(e), of the rows 2 t and 2 t + 1 that the lane's scores belong to.
-// HL: the tails too.
+// scale * log2(e), of the rows 2 t and 2 t + 1 that the lane's scores belong to.  A row with
+// a NaN or an infinity is taken as zeros with a NaN for its factor, which makes NaN of its
+// results.  HL: the tails too.
 template <int D, bool HL, int NT>
 struct Query {
   uint32_t h[NT][D / 16][2], l[HL ? NT : 1][HL ? D / 16 : 1][2];
@@ -138,19 +139,20 @@ struct Query {
         for (int i = 0; i < D / 4; ++i) x[i] = live ? kv8_load(p.q, base + i, p.dtype) : 0.0f;
       }
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      int e = 0;  // top in [2^e, 2^(e+1)); rows of zeros, infinities and the ends of the range keep e = 0
-      if (top > 0.0f && top < INFINITY) e = min(max((__float_as_int(top) >> 23) - 127, -100), 100);
-      const float f = copysignf(kv8_pow2(8 - e), p.scale), undo = kv8_pow2(e - 8) * fabsf(p.scale) * kLog2e;
+      for (int i = 0; i < D / 4; ++i) top = max_nan(top, fabsf(x[i]));
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const bool bad = !(top < INFINITY);
+      int e = 0;  // top in [2^e, 2^(e+1)); rows of zeros keep e = 0
+      if (top > 0.0f && !bad) e = min(max((__float_as_int(top) >> 23) - 127, -100), 100);
+      const float f = copysignf(kv8_pow2(8 - e), p.scale), undo = bad ? NAN : kv8_pow2(e - 8) * fabsf(p.scale) * kLog2e;
       back[nt][0] = __shfl_sync(0xffffffffu, undo, 8 * t4);
       back[nt][1] = __shfl_sync(0xffffffffu, undo, 8 * t4 + 4);
 #pragma unroll
       for (int s = 0; s < D / 16; ++s)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float u = x[4 * s + 2 * i] * f, v = x[4 * s + 2 * i + 1] * f;
+          const float u = bad ? 0.0f : x[4 * s + 2 * i] * f, v = bad ? 0.0f : x[4 * s + 2 * i + 1] * f;
           const __half2 hd = __floats2half2_rn(u, v);
           h[nt][s][i] = h2_bits(hd);
           if (HL) {
@@ -482,7 +484,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          a[nt][i] = fmaxf(q.back[nt][i] * kf, 1.2e-38f);  // above 0: a masked score times it stays -infinity
+          a[nt][i] = max_nan(q.back[nt][i] * kf, 1.2e-38f);  // above 0: a masked score times it stays -infinity
           float t = fmaxf(c[0][nt][i], c[0][nt][i + 2]);
 #pragma unroll
           for (int mt = 1; mt < 4; ++mt) t = fmaxf(fmaxf(t, c[mt][nt][i]), c[mt][nt][i + 2]);
@@ -653,6 +655,8 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
         v += __shfl_xor_sync(0xffffffffu, v, 4);
         v += __shfl_xor_sync(0xffffffffu, v, 8);
         l[nt][i] = v + __shfl_xor_sync(0xffffffffu, v, 16);
+        // NaN scores raise no maximum, but the row has seen something all the same
+        if (l[nt][i] != l[nt][i] && lim[nt][i] >= 0 && mx[nt][i] == -INFINITY) m[nt][i] = mx[nt][i] = 0.0f;
       }
 #pragma unroll
     for (int step = kWarps / 2; step > 0; step >>= 1) {
@@ -806,6 +810,14 @@ __global__ void __launch_bounds__(256) kv8_scores_mass_kernel(const __grid_const
     const int t = r / p.G;
     // past a row's last slot its scores were not all written
     if (key > p.pos[b] + t || t >= (p.counts ? min(p.counts[b], p.T) : p.T)) continue;
+    if (lse != lse) {  // every slot that the row sees
+      const int n = p.pos[b] + t - key;
+      sum.x = NAN;
+      if (n >= 1) sum.y = NAN;
+      if (n >= 2) sum.z = NAN;
+      if (n >= 3) sum.w = NAN;
+      continue;
+    }
     const float4 x = *reinterpret_cast<const float4*>(p.scores + (head * p.rows + r) * p.ld_scores + key);
     sum.x += exp2a(x.x - lse), sum.y += exp2a(x.y - lse);
     sum.z += exp2a(x.z - lse), sum.w += exp2a(x.w - lse);

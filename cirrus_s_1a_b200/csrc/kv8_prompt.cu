@@ -186,12 +186,17 @@ __global__ void __launch_bounds__(256) kv8_query_kernel(const __grid_constant__ 
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     x[i] = live ? kv8_load(p.q, base + i, p.dtype) : 0.0f;
-    top = fmaxf(top, fabsf(x[i]));
+    top = max_nan(top, fabsf(x[i]));
   }
 #pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = 1; o < kLanes; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  // a row with a NaN or an infinity: zeros, and a NaN for its factor
+  const bool bad = !(top < INFINITY);
+  if (bad)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
   int e = 0;
-  if (top > 0.0f && top < INFINITY) e = min(max((__float_as_int(top) >> 23) - 127, -100), 100);
+  if (top > 0.0f && !bad) e = min(max((__float_as_int(top) >> 23) - 127, -100), 100);
   const float f = copysignf(kv8_pow2(8 - e), p.scale);
   uint8_t* tile = p.q16 + (head * p.row_tiles + r / kRows) * (int64_t)((1 + HL) * kRows * D * 2);
 #pragma unroll
@@ -208,7 +213,7 @@ __global__ void __launch_bounds__(256) kv8_query_kernel(const __grid_constant__ 
     *reinterpret_cast<uint4*>(tile + part * kRows * D * 2 + swizzled<kRows>(r % kRows, kb)) =
         make_uint4(h[0], h[1], h[2], h[3]);
   }
-  if (kb == 0) p.q_back[head * p.row_tiles * kRows + r] = live ? kv8_pow2(e - 8) * fabsf(p.scale) * kLog2e : 0.0f;
+  if (kb == 0) p.q_back[head * p.row_tiles * kRows + r] = bad ? NAN : live ? kv8_pow2(e - 8) * fabsf(p.scale) * kLog2e : 0.0f;
 }
 
 // --------------------------------------------------------------- attention
@@ -355,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         int ev[kHalves];
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
-          a[h] = fmaxf(back * ks[h], 1.2e-38f);  // above 0: a masked score times it stays -infinity
+          a[h] = max_nan(back * ks[h], 1.2e-38f);  // above 0: a masked score times it stays -infinity
           ev[h] = kv8_exponent(vs[h]);
         }
         if (j + 1 < n) scales(j + 1);
@@ -476,8 +481,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       const int t = r / p.G, hq = (int)(head % p.c.n_kv_heads) * p.G + r % p.G;
       const int64_t orow = ((int64_t)b * p.T + t) * (p.G * p.c.n_kv_heads) + hq;
       const int64_t at = (head * p.rows + r) * p.splits + split;
+      // NaN scores raise no maximum, but the row has seen something all the same
+      const bool none = lim < 0 || l == 0.0f;
       // 2^(m' - m) / l in two factors: an exponent of up to 135 times a small sum
-      const float half = mx > -INFINITY ? exp2a(0.5f * (m - mx)) : 0.0f, inv = mx > -INFINITY ? half / l : 0.0f;
+      const float half = none ? 0.0f : exp2a(0.5f * (m - mx)), inv = none ? 0.0f : half / l;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         float o[32];
@@ -486,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           tmem_ld_wait();
         }
         if (r >= p.rows || !ok) continue;
-        if (mx == -INFINITY)
+        if (none)
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0.0f;
         if (p.splits > 1) {
@@ -514,9 +521,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       }
       if (r < p.rows && ok) {
         if (p.splits > 1) {
-          p.part_ml[at] = make_float4(m, mx, l, 0.0f);
+          p.part_ml[at] = make_float4(m, none ? -INFINITY : fmaxf(mx, -3e38f), none ? 0.0f : l, 0.0f);
         } else {
-          p.lse[orow] = mx > -INFINITY ? (mx + log2f(l)) * kLn2 : -INFINITY;
+          p.lse[orow] = none ? -INFINITY : (mx + log2f(l)) * kLn2;
         }
       }
     }
@@ -678,6 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ float s_sum[kRows];
+  __shared__ int s_nan_t;  // the last token with a row whose lse is NaN: every slot it sees is one too
   const uint32_t q_full = smem_u32(bars), q_free = q_full + 8 * kMassStages, s_full = q_free + 8 * kMassStages,
                  end = s_full + 8 * kMassStages;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -699,6 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(end));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_abort = 0;
+    s_nan_t = INT_MIN / 2;
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)));
@@ -777,11 +786,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
             "l"(p.q16 + (head * p.row_tiles + tile) * (int64_t)C::kQ), "r"(C::kQ), "r"(q_full + 8 * st)
             : "memory");
       }
-      // rows that see nothing: a factor that leaves any score finite, and -infinity
+      // rows that see nothing (or NaN): a factor that leaves any score finite, and -infinity
       float by = 1.2e-38f, sub = -INFINITY;
       if (t < cnt && pos + t >= 0) {
+        const float lse = p.lse[((int64_t)b * p.T + t) * (p.G * p.c.n_kv_heads) + hk * p.G + r % p.G];
         by = fmaxf(p.q_back[head * p.row_tiles * kRows + r], 1.2e-38f);
-        sub = -p.lse[((int64_t)b * p.T + t) * (p.G * p.c.n_kv_heads) + hk * p.G + r % p.G] * kLog2e;
+        sub = lse == lse ? -lse * kLog2e : -INFINITY;
+        if (lse != lse) atomicMax(&s_nan_t, t);
       }
       s_info[st * 2 * kRows + d] = by;
       s_info[st * 2 * kRows + kRows + d] = sub;
@@ -820,7 +831,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
   fence_before();
   __syncthreads();
   fence_after();
-  if (tid < kRows && key0 + tid <= last && !s_abort) p.c.mass[head * p.c.max_len + key0 + tid] += mine + s_sum[tid];
+  if (tid < kRows && key0 + tid <= last && !s_abort)
+    p.c.mass[head * p.c.max_len + key0 + tid] += key0 + tid <= pos + s_nan_t ? NAN : mine + s_sum[tid];
   if (tid == 0 && s_abort) set_status(p.status, CB_ERR_TIMEOUT);
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(s_tmem));
 }

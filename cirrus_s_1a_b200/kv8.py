@@ -176,7 +176,8 @@ class Kv8Cache:
         """Causal attention of the queries ``q`` [B, T, query heads, D] of the T
         tokens behind ``pos[b]``: row t sees slots up to ``pos[b] + t``.  Returns
         (out [B, T, query heads, D] in q's type, lse float32 [B, T, query heads]);
-        rows that see nothing give 0 and -inf.  ``scale`` defaults to D ** -0.5;
+        rows that see nothing give 0 and -inf, rows whose query is not finite or that see
+        a NaN key give NaN.  ``scale`` defaults to D ** -0.5;
         ``add_mass`` adds each slot's probabilities to ``mass``; ``longest`` bounds
         ``pos + T`` and sizes the launch (default ``max_len``) (``cb_kv8_attend``)."""
         T, heads, qs = self._rows(q, "q", None)

@@ -280,6 +280,47 @@ def test_nan_in_a_value_reaches_the_rows_that_see_it_only(D, T, dtype):
     assert bool(out[0, at:, :, 3].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,T", [(64, 1), (64, 2), (64, 4), (64, 140), (128, 140), (128, 1), (128, 5), (16, 5), (32, 60)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_query_that_is_not_finite_gives_nan(D, T, dtype, bad):
+    """Not the 0 and -infinity of a row that sees nothing.  The other rows, and the
+    weights of slots that the row does not see, are as they would be without it, up to
+    the roundings of two runs whose maxima rise at other keys: 2^-20 in the sums, and in
+    bf16 outputs that of the probabilities and of the output."""
+    cache = filled(1, 1, D, 512, "int8")
+    mass = cache.mass.clone()
+    q = torch.randn(1, T, 3, D, generator=torch.Generator().manual_seed(8)).to(TYPES[dtype]).to(DEV)
+    clean, clean_lse = cache.attend(q, ints([200]), add_mass=True)
+    clean_mass = cache.mass.clone()
+    at = T // 2
+    q[0, at, 1, D - 3] = bad
+    cache.mass.copy_(mass)
+    out, lse = cache.attend(q, ints([200]), add_mass=True)
+    rest = torch.ones(T, 3, dtype=torch.bool)
+    rest[at, 1] = False
+    assert bool(out[0, at, 1].isnan().all()) and bool(lse[0, at, 1].isnan())
+    near = 127 * float(cache.v_scale.max()) * (2.0 ** -7 if dtype == "bf16" else 2.0 ** -18)
+    assert (out[0][rest].float() - clean[0][rest].float()).abs().amax().le(near) 
+    assert torch.allclose(lse[0][rest], clean_lse[0][rest], rtol=2.0 ** -19, atol=2.0 ** -19)
+    assert bool(cache.mass[0, 0, :201 + at].isnan().all())
+    assert torch.allclose(cache.mass[0, 0, 201 + at:], clean_mass[0, 0, 201 + at:], rtol=2.0 ** -17, atol=0)
+
+
+@pytest.mark.parametrize("D,T", [(64, 1), (64, 4), (64, 140), (128, 140), (128, 1), (16, 5)])
+def test_a_row_that_sees_nan_keys_alone_gives_nan(D, T):
+    cache = filled(1, 1, D, 512, "e4m3")
+    cache.k.view(torch.uint8)[0, 0, 0, 5] = 0x7F
+    q = torch.randn(1, T, 3, D, generator=torch.Generator().manual_seed(8)).bfloat16().to(DEV)
+    out, lse = cache.attend(q, ints([0]), add_mass=True)
+    assert bool(out.isnan().all()) and bool(lse.isnan().all())  # every row sees slot 0
+    assert bool(cache.mass[0, 0, :T].isnan().all()) and bool(torch.isfinite(cache.mass[0, 0, T:]).all())
+    cache = filled(1, 1, D, 512, "e4m3")
+    cache.k.view(torch.uint8)[0, 0, :64, 5] = 0x7F  # a whole block, beside finite ones
+    out, lse = cache.attend(q, ints([300]))
+    assert bool(out.isnan().all()) and bool(lse.isnan().all())
+
+
 def test_query_strides_and_other_streams():
     cache = filled(2, 2, 64, 256, "int8")
     proj = torch.randn(2, 7, 6 * 64 + 13, generator=torch.Generator().manual_seed(4)).to(DEV)
