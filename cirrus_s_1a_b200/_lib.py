@@ -28,6 +28,7 @@ STATUS = {0: "ok", 1: "invalid argument", 2: "shape not supported", 3: "CUDA lau
 CB_PATH_AUTO, CB_PATH_MULTI_KERNEL = 0, 1
 CB_NOALLOC_MAX_SCORES = 1 << 20
 CB_KV8_BLOCK = 64
+CB_KV8_ZEROED = 262144
 CB_KV8_E4M3, CB_KV8_INT8 = 0, 1
 CB_F32, CB_BF16, CB_F16 = 0, 1, 2
 CB_LOGPROB_MAX_TOP, CB_LOGPROB_MAX_VOCAB = 32, 1 << 20

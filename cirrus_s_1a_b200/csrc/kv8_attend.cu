@@ -926,7 +926,7 @@ Form form_of(const CbKv8& c, int dtype, int rows) {
 
 // How a call is cut up, and where its parts lie in the scratch.  The counters come
 // first, in every call's layout: they are zero between calls.
-constexpr size_t kCounters = 65536;
+constexpr size_t kCounters = CB_KV8_ZEROED / sizeof(int);
 struct Plan {
   int rows = 0, row_tiles = 0, splits = 0;
   int64_t part_rows = 0, ld_scores = 0;

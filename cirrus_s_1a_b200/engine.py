@@ -454,6 +454,8 @@ class CirrusB200:
         Tc = min(T, CB_PREFILL_CHUNK)
         ws = cache.kv8.workspaces.get(Tc)
         if ws is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise _lib.CbError(f"run a forward of {Tc} tokens on this cache before one is captured")
             nbytes = L.cb_forward_kv8_workspace_bytes(C.byref(self.model.desc), cache.kv8._ref, Tc)
             if nbytes == 0:
                 raise _lib.CbError("cb_forward_kv8_workspace_bytes: shape not supported")

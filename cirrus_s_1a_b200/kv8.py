@@ -10,7 +10,8 @@ Keys and values are held as E4M3 or int8 codes with one scale, a power of two,
 for each block of 64 slots and KV head.  ``pos`` is a device int32 tensor: the
 slots of each sequence in use before the call.  Calls enqueue work on the
 current stream and do not synchronise.  The attention's scratch belongs to the
-cache and to one stream: calls of one cache from several streams get one each.
+cache and to one stream: calls of one cache from several streams get one each, and
+a call that a CUDA graph captures gets its own, from the graph's memory.
 
 The reference keeps the shared K/V in the model's type
 (``cirrus/model/model.py:41-51``); this is its bounded form for long texts.
@@ -95,7 +96,8 @@ class Kv8Cache:
                              v_scale.data_ptr(), _lib.ptr(mass))
         self._ref = C.addressof(self._struct)
         self._lib = _lib.lib()
-        self._scratch: dict = {}
+        self._scratch: dict = {}  # stream -> buffer; one serves every shape
+        self._sizes: dict = {}  # shape -> bytes
         self.workspaces: dict = {}  # of the model's forward over this cache, by chunk length
 
     # ------------------------------------------------------------- helpers
@@ -180,6 +182,9 @@ class Kv8Cache:
         a NaN key give NaN.  ``scale`` defaults to D ** -0.5;
         ``add_mass`` adds each slot's probabilities to ``mass``; ``longest`` bounds
         ``pos + T`` and sizes the launch (default ``max_len``) (``cb_kv8_attend``)."""
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.attend(q, pos, counts, scale=scale, add_mass=add_mass, longest=longest, out=out)
         T, heads, qs = self._rows(q, "q", None)
         if heads % self.n_kv_heads:
             raise ValueError(f"{heads} query heads do not divide among {self.n_kv_heads} KV heads")
@@ -193,29 +198,33 @@ class Kv8Cache:
             raise ValueError("out must be contiguous, of q's shape, type and device")
         lse = torch.empty(self.batch, T, heads, dtype=torch.float32, device=self.device)
         st = self._stream()
-        key = (st, dtype, heads, T, longest, add_mass)
-        scratch = self._scratch.get(key)
-        if scratch is None:
-            nbytes = self._lib.cb_kv8_attend_scratch_bytes(self._ref, dtype, heads, T, longest, int(add_mass))
-            if nbytes == 0:
-                raise _lib.CbError("cb_kv8_attend_scratch_bytes: shape not supported")
-            scratch = self._grow(st, nbytes)
-            self._scratch[key] = scratch
+        scratch = self._scratch_of(dtype, heads, T, longest, add_mass, st)
         self._call(self._lib.cb_kv8_attend, "cb_kv8_attend", self._ref, q.data_ptr(), dtype, qs, heads, T,
                    self._ints(pos, "pos"), self._ints(counts, "counts"), longest,
                    self.head_dim ** -0.5 if scale is None else float(scale), int(add_mass), out.data_ptr(),
                    lse.data_ptr(), scratch.data_ptr(), scratch.numel(), self.status.data_ptr(), st)
         return out, lse
 
-    def _grow(self, stream: int, nbytes: int) -> torch.Tensor:
-        """The stream's scratch, at least ``nbytes`` long: one buffer serves every shape on a stream."""
-        have = self._scratch.get(stream)
-        if have is None or have.numel() < nbytes:
-            have = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
-            for key in [k for k in self._scratch if k == stream or (isinstance(k, tuple) and k[0] == stream)]:
-                del self._scratch[key]
-            self._scratch[stream] = have
-        return have
+    def _scratch_of(self, dtype: int, heads: int, T: int, longest: int, add_mass: bool, stream: int) -> torch.Tensor:
+        key = (dtype, heads, T, longest, add_mass)
+        nbytes = self._sizes.get(key)
+        if nbytes is None:
+            nbytes = self._lib.cb_kv8_attend_scratch_bytes(self._ref, dtype, heads, T, longest, int(add_mass))
+            if nbytes == 0:
+                raise _lib.CbError("cb_kv8_attend_scratch_bytes: shape not supported")
+            if len(self._sizes) >= 256:  # a caller's ``longest`` may change with every token
+                self._sizes.clear()
+            self._sizes[key] = nbytes
+        if torch.cuda.is_current_stream_capturing():
+            # from the graph's pool, and zeroed by each replay: the stream's buffer may be replaced by a
+            # longer one, and what it holds is not zero before the graph's own first replay
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            scratch[:_lib.CB_KV8_ZEROED].zero_()
+            return scratch
+        scratch = self._scratch.get(stream)
+        if scratch is None or scratch.numel() < nbytes:
+            scratch = self._scratch[stream] = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
+        return scratch
 
     def evict(self, pos: torch.Tensor, keep: int, recent: int) -> tuple:
         """Brings every sequence of more than ``keep`` tokens down to ``keep``, per

@@ -403,6 +403,7 @@ int cb_spec_accept(const CbModel* m, const CbCache* c, const int32_t* argmax, co
  * 16-byte aligned.  The reference keeps the shared K/V in the model's type
  * (cirrus/model/model.py:41-51) and has no 8-bit cache. */
 #define CB_KV8_BLOCK 64
+#define CB_KV8_ZEROED 262144
 enum { CB_KV8_E4M3 = 0, CB_KV8_INT8 = 1 };
 enum { CB_F32 = 0, CB_BF16 = 1, CB_F16 = 2 };
 typedef struct CbKv8 {
@@ -440,9 +441,10 @@ int cb_kv8_append(const CbKv8* c, const void* k, const void* v, int32_t dtype, c
  * Sums are float32; 16-bit queries meet the codes exactly and the probabilities
  * are rounded to f16 for the product with v; float32 queries and probabilities
  * are carried in about 22 bits.  longest: a bound on pos[b] + T that sizes the
- * launch; slots from it on are not seen.  scratch: cb_kv8_attend_scratch_bytes(c, dtype, n_q_heads, T, longest,
- * add_mass) bytes, 16-byte aligned (as is out), zeroed once before its first use
- * (calls of any sizes may follow), not shared by calls that overlap.  status
+ * launch; slots from it on are not seen.  scratch: cb_kv8_attend_scratch_bytes(c,
+ * dtype, n_q_heads, T, longest, add_mass) bytes, 16-byte aligned (as is out), its first
+ * CB_KV8_ZEROED bytes zeroed once before its first use (calls of any sizes may follow),
+ * not shared by calls that overlap, kept as long as a graph that captured the call.  status
  * (device int32, may be null) receives CB_ERR_TIMEOUT if a bounded wait on the
  * tensor-core pipeline gives up.
  * Replaces the dense attention of CrossAttention.forward over the shared K/V

@@ -362,6 +362,62 @@ def test_results_repeat_and_replay_in_a_graph(T):
     assert torch.equal(d, e)
 
 
+def test_a_graph_keeps_its_scratch():
+    """A longer call on the capture's stream replaces the stream's buffer, not the graph's."""
+    cache = filled(2, 2, 64, 1024, "e4m3")
+    q = torch.randn(2, 1, 6, 64, generator=torch.Generator().manual_seed(1)).bfloat16().to(DEV)
+    long = torch.randn(2, 500, 6, 64, generator=torch.Generator().manual_seed(2)).bfloat16().to(DEV)
+    pos = ints([400, 333])
+    want, wlse = cache.attend(q, pos)
+    wlong, _ = cache.attend(long, pos)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.attend(q, pos)
+        with torch.cuda.graph(graph, stream=side):
+            out, lse = cache.attend(q, pos)
+        got, _ = cache.attend(long, pos)
+        held = [torch.full((1 << 20,), 7, dtype=torch.uint8, device=DEV) for _ in range(64)]  # where it may have been
+        for _ in range(3):
+            graph.replay()
+        again, _ = cache.attend(long, pos)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, want) and torch.equal(lse, wlse)
+    assert torch.equal(got, wlong) and torch.equal(again, wlong)
+    assert all(bool((h == 7).all()) for h in held)
+
+
+def test_graphs_captured_without_a_call_before_replay_in_any_order():
+    cache = filled(2, 2, 64, 1024, "e4m3")
+    pos = ints([400, 333])
+    qs = [torch.randn(2, T, 6, 64, generator=torch.Generator().manual_seed(T)).bfloat16().to(DEV) for T in (1, 5, 130)]
+    want = [cache.attend(q, pos) for q in qs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, got = [], []
+    for q in qs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            got.append(cache.attend(q, pos))
+    with torch.cuda.stream(side):
+        eager = cache.attend(qs[0], pos)  # between the captures and their first replay
+        for i in (2, 1, 0, 1, 2):
+            graphs[i].replay()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(eager[0], want[0][0])
+    for (a, la), (b, lb) in zip(got, want):
+        assert torch.equal(a, b) and torch.equal(la, lb)
+
+
+def test_lengths_that_change_with_every_token_keep_no_entry_each():
+    cache = filled(1, 1, 16, 1024, "int8")
+    q = torch.randn(1, 1, 1, 16).to(DEV)
+    for n in range(600):
+        cache.attend(q, ints([n]), longest=n + 1)
+    assert len(cache._sizes) <= 256 and len(cache._scratch) == 1
+
+
 def test_offsets_past_32_bits():
     """The last sequence of a cache whose codes pass 2^31 bytes."""
     from cirrus_s_1a_b200.kv8 import Kv8Cache

@@ -117,3 +117,31 @@ def test_clones_and_refusals():
     other = CirrusB200(sparse, synthetic.random_state_dict(sparse, seed=0), device=DEV, max_ctx=64)
     with pytest.raises(ValueError):
         other.new_cache(kv8="int8")
+
+
+def test_a_capture_wants_its_workspace_first():
+    """A workspace zeroed inside a capture would not be zero before the first replay."""
+    from cirrus_s_1a_b200 import _lib
+
+    cfg, eng = model()
+    cache = eng.new_cache(kv8="int8")
+    ids = text(cfg, 1).to(DEV)
+    logits = torch.empty(1, 1, cfg.vocab_size, device=DEV)
+    hidden = torch.empty(1, 1, cfg.d_model, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(_lib.CbError):
+        with torch.cuda.graph(graph):
+            torch.zeros(1, device=DEV)
+            eng.launch(cache, ids, 1, 1, logits, hidden, None)
+    eng(ids, cache=cache)
+    slots, state = cache.slots_dev.clone(), (cache.pos_dev.clone(), cache.gdn_state.clone(), cache.gdn_conv.clone())
+    eng.launch(cache, ids, 1, 1, logits, hidden, None)
+    want = logits.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        eng.launch(cache, ids, 1, 1, logits, hidden, None)
+    cache.slots_dev.copy_(slots)
+    for t, was in zip((cache.pos_dev, cache.gdn_state, cache.gdn_conv), state):
+        t.copy_(was)
+    graph.replay()
+    torch.testing.assert_close(logits, want, rtol=1e-4, atol=1e-4)
