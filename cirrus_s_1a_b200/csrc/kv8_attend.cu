@@ -33,7 +33,8 @@
 // the row adds up, whatever the blocks' scales.  The row's sum is
 // l = sum_b 2^(e_ref - e_b) sum P against m = m' - e_ref, with an e_ref near the blocks'
 // exponents; blocks far below it (zeros) are summed for themselves (kNear).
-// out = 2^(m' - m) O / l.  O is rescaled only when m' has grown by more than 2^12.
+// out = 2^(m' - m) O / l.  O is rescaled only when m' has grown by more than 2^12
+// (float32: 2^15, and m' is 11 powers below the maximum, for the tails).
 // Softmax statistics and the joins of parts are float32.
 //
 // Work is dealt out by blocks of 64 keys: the visible blocks of all KV heads, one
@@ -62,7 +63,12 @@ namespace cb {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr float kLazy = 12.0f;  // growth of the maximum, in powers of two, that O follows: f16 P ends at 2^16
+// Growth of the maximum, in powers of two, that O follows (f16 P ends at 2^16), and what a
+// row's largest P lies above 1 when it does: a tail of P then ends at 2^-35 of the largest.
+template <bool HL>
+constexpr float kLazy = HL ? 15.0f : 12.0f;
+template <bool HL>
+constexpr float kLift = HL ? 11.0f : 0.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -476,7 +482,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
             for (int i = 0; i < 4; ++i)
               if (key0 + 16 * mt + 8 * (i >> 1) + key_row(g) > lim[nt][i & 1]) c[mt][nt][i] = -INFINITY;
       }
-      // the largest x + e of this lane's keys: only where one passes m' by 2^kLazy do
+      // the largest x + e of this lane's keys: only where one passes m' by kLazy do
       // the lanes of a row compare
       float a[NT][2], now[NT][2];
       bool any = false;
@@ -489,7 +495,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
 #pragma unroll
           for (int mt = 1; mt < 4; ++mt) t = fmaxf(fmaxf(t, c[mt][nt][i]), c[mt][nt][i + 2]);
           now[nt][i] = fmaf(t, a[nt][i], (float)ev);
-          any = any || now[nt][i] > m[nt][i] + kLazy;  // -infinity passes nothing, anything passes -infinity
+          any = any || now[nt][i] > m[nt][i] + kLazy<HL>;  // -infinity passes nothing, anything passes -infinity
         }
       if (p.scores) {
         // log2 units, for the rows' attention weights
@@ -515,7 +521,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
             float to = now[nt][i];
             to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 4));
             to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 8));
-            to = fmaxf(m[nt][i], fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 16)));
+            to = fmaxf(m[nt][i], fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 16)) - kLift<HL>);
             alpha[i] = m[nt][i] == -INFINITY ? 0.0f : exp2a(m[nt][i] - to);
             m[nt][i] = to;
             l[nt][i] *= alpha[i];

@@ -246,6 +246,29 @@ def test_value_blocks_of_zeros_beside_large_ones(fmt, dtype, D, T, e):
     check_attend(cache, q, [max(63 - T, 0)], dtype=dtype, add_mass=True)
 
 
+@pytest.mark.parametrize("n", [64, 128, 32768])
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+def test_float32_keeps_small_probabilities(D, n):
+    """One key weighs 2^13 times as much as each of the others but its value is 0: head and tail
+    carry every probability to 2^-22 of itself, the exponential and the sums add 2^-20, truncated
+    products of 64 keys as much again: less than 2^-18 in all.  (The scores are exact.)"""
+    cache = filled(1, 1, D, n, "int8")
+    cache.k.zero_()
+    cache.k[0, 0, 50, 0] = 1
+    cache.k_scale.fill_(1.0)
+    v = torch.arange(D).remainder(127) + 1
+    cache.v.copy_(v.to(torch.int8).expand(1, 1, n, D))
+    cache.v[0, 0, 50] = 0
+    cache.v_scale.fill_(1.0)
+    for score in (9.125, 8.875, 9.25):
+        q = torch.zeros(1, 1, 1, D)
+        q[..., 0] = score
+        out, lse = cache.attend(q.to(DEV), ints([n - 1]), scale=1.0)
+        small = (n - 1) * math.exp(-score)
+        want = v.double() * small / (1 + small)
+        assert (out[0, 0, 0].cpu().double() / want - 1).abs().max() < 2.0 ** -18
+
+
 @pytest.mark.parametrize("T", [1, 130])
 def test_peaked_and_extreme_scores(T):
     """Scores of thousands (one key takes all), queries of 1e-30 (all keys alike) and zeros."""
