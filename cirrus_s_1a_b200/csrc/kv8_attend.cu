@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
 #pragma unroll
         for (int i = 0; i < 2; ++i) add[nt][i] = (float)ev - (m[nt][i] == -INFINITY ? 0.0f : m[nt][i]);
       const uint8_t* vb = arrive();
-      int nan_key = INT_MAX;
+      bool any_nan = false;
       float pv[HL ? D / 16 : 1][HL ? NT : 1][4] = {};
       float sum[NT][2] = {};
 #pragma unroll
@@ -583,15 +583,15 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
           const int key = 16 * s + 4 * u + t4;
           load_bytes<NB>(vb + key * D + g * NB, w[u]);
           if (partly) {
-            // 0 * NaN is not 0: slots no row sees may hold anything and read as 0, and an
-            // E4M3 NaN in a slot that some rows see makes NaN of those rows below
+            // 0 * NaN is not 0: slots no row sees may hold anything and read as 0, and so do
+            // E4M3 NaNs, which then reach the rows that see them below
 #pragma unroll
             for (int z = 0; z < (NB + 3) / 4; ++z) {
               if (key0 + key > at.last) w[u][z] = 0u;
               if (FMT == CB_KV8_E4M3) {
                 const uint32_t nan = __vcmpeq4(w[u][z] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
                 w[u][z] &= ~nan;
-                if (nan) nan_key = min(nan_key, key0 + key);
+                any_nan = any_nan || nan;
               }
             }
           }
@@ -617,16 +617,23 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
             }
           }
       }
+      if (FMT == CB_KV8_E4M3 && partly && __any_sync(0xffffffffu, any_nan)) {
+        // the first NaN of each of this lane's dims, for the rows that see it
+#pragma unroll
+        for (int y = 0; y < D / 8; ++y) {
+          int first = INT_MAX;
+#pragma unroll 1
+          for (int key = 63; key >= 0; --key)
+            if (key0 + key <= at.last && (vb[key * D + g * (D / 8) + y] & 0x7F) == 0x7F) first = key0 + key;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (first <= lim[nt][i]) o[y / 2][nt][2 * (y & 1) + i] = NAN;
+        }
+      }
       __syncwarp();
       copy();  // into the slot of these values
-      if (FMT == CB_KV8_E4M3 && partly) {
-        nan_key = __reduce_min_sync(0xffffffffu, nan_key);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (nan_key <= lim[nt][i]) sum[nt][i] = NAN;
-      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll

@@ -247,6 +247,32 @@ struct Prompt {
   static constexpr int kRow = D / 16;                            // of a key
 };
 
+// NaN over a row's results in the dims where a slot that it sees, from `first` on, holds a
+// NaN (thread for row, after the CTA's results).  Rarely called: it finds its place anew, so
+// that nothing is kept for it through the loops.
+template <int D, int HL>
+__device__ void nan_values(const AttendParams& p, int first, int end) {
+  uint32_t bx, by, tid;
+  asm volatile("mov.u32 %0, %%ctaid.x;\n\tmov.u32 %1, %%ctaid.y;\n\tmov.u32 %2, %%tid.x;" : "=r"(bx), "=r"(by), "=r"(tid));
+  const int64_t head = by;
+  const int hk = (int)(by % p.c.n_kv_heads), b = (int)(by / p.c.n_kv_heads);
+  const int split = bx % p.splits, r = bx / p.splits * kTiles * kRows + tid;
+  if (tid >= kTiles * kRows || r >= p.rows) return;
+  const int cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
+  const int lim = min(row_limit(p, r, p.pos[b], cnt), end - 1);
+  const int64_t at = p.splits > 1 ? (head * p.rows + r) * p.splits + split
+                                  : ((int64_t)b * p.T + r / p.G) * (p.G * p.c.n_kv_heads) + hk * p.G + r % p.G;
+#pragma unroll 1
+  for (int slot = first; slot <= lim; ++slot)
+#pragma unroll 1
+    for (int d = 0; d < D; ++d) {
+      if ((p.c.v[(head * p.c.max_len + slot) * D + d] & 0x7F) != 0x7F) continue;
+      if (p.splits > 1) p.part_o[at * D + d] = NAN;
+      else if (HL > 0) static_cast<float*>(p.out)[at * D + d] = NAN;
+      else static_cast<uint16_t*>(p.out)[at * D + d] = 0x7FFF;  // a NaN of either type
+    }
+}
+
 template <int D, int FMT, int HL>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_constant__ AttendParams p) {
   using C = Prompt<D, HL>;
@@ -257,7 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ Aside s_aside[kTiles * kRows];
-  __shared__ int s_nan;  // the first E4M3 NaN among values that not all rows see
+  __shared__ int s_nan;  // the first slot with an E4M3 NaN among values that not all rows see
+  __shared__ int s_end;  // the end of the run's slots
   uint8_t* sq = smem;
   uint8_t* sk = smem + kTiles * C::kQ;
   uint8_t* sv = sk + kStages * C::kKV;
@@ -294,6 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_abort = 0;
     s_nan = INT_MAX;
+    s_end = (beg + n) * kKeys;
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)));
@@ -477,7 +505,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         mx = aside.m;
         l = aside.l;
       }
-      if (FMT == CB_KV8_E4M3 && n > 0 && s_nan <= lim) l = NAN;
       const int t = r / p.G, hq = (int)(head % p.c.n_kv_heads) * p.G + r % p.G;
       const int64_t orow = ((int64_t)b * p.T + t) * (p.G * p.c.n_kv_heads) + hq;
       const int64_t at = (head * p.rows + r) * p.splits + split;
@@ -561,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           const int key = key_of(i), c = chunk_of(i);
           uint4 lo, hi;
           if (FMT == CB_KV8_E4M3 && kv == 1 && (beg + j + 1) * kKeys - 1 > seen) {
-            // 0 * NaN is not 0: a NaN reads as 0 here, and makes NaN of the rows that see it at the end
+            // 0 * NaN is not 0: a NaN reads as 0 here, and reaches the rows that see it at the end
             uint32_t* w = &raw[kv][i].x;
             uint32_t any = 0;
 #pragma unroll
@@ -650,6 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   fence_before();
   __syncthreads();
   fence_after();
+  if (FMT == CB_KV8_E4M3 && s_nan != INT_MAX && !s_abort) nan_values<D, HL>(p, s_nan, s_end);
   if (tid == 0 && s_abort) set_status(p.status, CB_ERR_TIMEOUT);
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(s_tmem));
 }

@@ -437,7 +437,8 @@ int cb_kv8_append(const CbKv8* c, const void* k, const void* v, int32_t dtype, c
  *   lse [batch][T][n_q_heads] float32: log of the softmax's sum (natural log)
  *   add_mass: mass[b][h][j] += the probabilities of slot j over the head's rows
  * Rows that see nothing (t >= counts[b], pos[b] + t < 0) give 0 and -infinity; a row
- * with a NaN or an infinity in its query, or that sees a NaN key, gives NaN.
+ * with a NaN or an infinity in its query, or that sees a NaN key, gives NaN, one that
+ * sees a NaN among the values gives NaN in its dim.
  * Sums are float32; 16-bit queries meet the codes exactly and the probabilities
  * are rounded to f16 for the product with v; float32 queries and probabilities
  * are carried in about 22 bits.  longest: a bound on pos[b] + T that sizes the

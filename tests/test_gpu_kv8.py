@@ -344,6 +344,30 @@ def test_a_row_that_sees_nan_keys_alone_gives_nan(D, T):
     assert bool(out.isnan().all()) and bool(lse.isnan().all())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,T", [(64, 4), (64, 140), (128, 140), (128, 1), (128, 9), (16, 5), (32, 50)])
+def test_a_nan_value_stays_in_its_dimension(D, T, dtype):
+    """In a block that every row sees and in one that some rows see in part: the other
+    dims, the sums and the weights do not change."""
+    cache = filled(1, 1, D, 512, "e4m3")
+    mass = cache.mass.clone()
+    q = torch.randn(1, T, 3, D, generator=torch.Generator().manual_seed(8)).to(TYPES[dtype]).to(DEV)
+    clean, clean_lse = cache.attend(q, ints([200]), add_mass=True)
+    clean_mass = cache.mass.clone()
+    at = T // 2
+    for slot, first in ((200 + at, at), (7, 0)):
+        codes = cache.v.view(torch.uint8)
+        was = codes[0, 0, slot].clone()
+        codes[0, 0, slot, 3], codes[0, 0, slot, D - 1] = 0xFF, 0x7F
+        cache.mass.copy_(mass)
+        out, lse = cache.attend(q, ints([200]), add_mass=True)
+        codes[0, 0, slot] = was
+        assert torch.equal(lse, clean_lse) and torch.equal(cache.mass, clean_mass)
+        assert bool(out[0, first:, :, [3, D - 1]].isnan().all())
+        out[0, first:, :, [3, D - 1]] = clean[0, first:, :, [3, D - 1]]
+        assert torch.equal(out, clean)
+
+
 def test_query_strides_and_other_streams():
     cache = filled(2, 2, 64, 256, "int8")
     proj = torch.randn(2, 7, 6 * 64 + 13, generator=torch.Generator().manual_seed(4)).to(DEV)
