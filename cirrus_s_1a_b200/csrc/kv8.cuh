@@ -88,21 +88,26 @@ __device__ __forceinline__ float exp2a(float x) {
   return y;
 }
 
-// A sum of 2^x against a maximum, besides a row's own: rarely needed, so in shared memory.
-struct Aside {
+// 1 / l for sums of 2^-135 to 2^115, in two factors.
+struct Inverse {
+  float f, inv;
+  __device__ __forceinline__ explicit Inverse(float l) : f(l < 1.0f ? 4294967296.0f : 2.3283064e-10f), inv(1.0f / (l * f)) {}
+  __device__ __forceinline__ float of(float o) const { return o * f * inv; }
+};
+
+// A softmax's sum l * 2^m, m = -infinity: nothing yet.  l may be 2^100 and its share of the
+// whole 1, so it is scaled in two steps of half the exponent.
+struct Sum {
   float m, l;
   __device__ __forceinline__ void clear() { m = -INFINITY, l = 0.0f; }
-  __device__ __forceinline__ void raise(float to) {
-    if (to > m) {
-      l *= exp2a(m - to);  // 0 of the 0 it starts with
-      m = to;
-    }
-  }
-  __device__ __forceinline__ void add(float ref, float sum) {  // sum * 2^ref
-    if (sum != 0.0f) {
-      raise(ref);
-      l = fmaf(sum, exp2a(ref - m), l);
-    }
+  // The root of the factor that takes what is against m to `to`.
+  static __device__ __forceinline__ float half(float m, float to) { return m == -INFINITY ? 0.0f : exp2a(0.5f * (m - to)); }
+  // Adds l2 * 2^m2; returns the factors that take what is against m and m2 to the new m.
+  __device__ __forceinline__ float2 add(float m2, float l2) {
+    const float to = fmaxf(m, m2), g = half(m, to), g2 = half(m2, to);
+    l = l * g * g + l2 * g2 * g2;
+    m = to;
+    return make_float2(g * g, g2 * g2);
   }
 };
 

@@ -31,9 +31,9 @@
 // exponent of its value scale, P = exp2(x + e_b - m') against m' = max (x + e_b):
 // P times the bare codes is the sum over values, its f16 rounding relative to what
 // the row adds up, whatever the blocks' scales.  The row's sum is
-// l = sum_b 2^(e_ref - e_b) sum P against m = m' - e_ref, with an e_ref near the blocks'
-// exponents; blocks far below it (zeros) are summed for themselves (kNear).
-// out = 2^(m' - m) O / l.  O is rescaled only when m' has grown by more than 2^12
+// l 2^m', l = sum_b 2^-e_b sum P, added up against an exponent e_ref near the blocks' own;
+// blocks far below it (zeros) are summed for themselves (kNear).
+// out = O / l.  O is rescaled only when m' has grown by more than 2^12
 // (float32: 2^15, and m' is 11 powers below the maximum, for the tails).
 // Softmax statistics and the joins of parts are float32.
 //
@@ -209,16 +209,13 @@ __device__ __forceinline__ int row_limit(const AttendParams& p, int r, int pos, 
   return min(pos + t, p.limit - 1);
 }
 
-// Writes the output and lse of one row's four dims: `o` is the sum against the maximum
-// mo of x + e, ll its weights' sum against the maximum mx of x.
-__device__ __forceinline__ void write_row(const AttendParams& p, int b, int hk, int r, int d, float4 o, float mo, float mx,
-                                          float ll) {
+// Writes the output and lse of one row's four dims: `o` against the sum's m.
+__device__ __forceinline__ void write_row(const AttendParams& p, int b, int hk, int r, int d, float4 o, Sum s) {
   const int64_t at = ((int64_t)b * p.T + r / p.G) * (p.G * p.c.n_kv_heads) + hk * p.G + r % p.G;
-  const bool none = mx == -INFINITY;
-  // 2^(mo - mx) / ll in two factors: an exponent of up to 135 times a small sum
-  const float half = none ? 0.0f : exp2a(0.5f * (mo - mx)), inv = none ? 0.0f : half / ll;
+  const bool none = s.m == -INFINITY;
+  const Inverse by(none ? 1.0f : s.l);
   if (none) o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  const float y[4] = {o.x * half * inv, o.y * half * inv, o.z * half * inv, o.w * half * inv};
+  const float y[4] = {by.of(o.x), by.of(o.y), by.of(o.z), by.of(o.w)};
   if (p.dtype == CB_F32) {
     *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at * p.c.head_dim + d) = make_float4(y[0], y[1], y[2], y[3]);
   } else {
@@ -230,7 +227,7 @@ __device__ __forceinline__ void write_row(const AttendParams& p, int b, int hk, 
       u = make_uint2(h2_bits(__floats2half2_rn(y[0], y[1])), h2_bits(__floats2half2_rn(y[2], y[3])));
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at * p.c.head_dim + d) = u;
   }
-  if (d == 0) p.lse[at] = none ? -INFINITY : (mx + log2f(ll)) * kLn2;
+  if (d == 0) p.lse[at] = none ? -INFINITY : (s.m + log2f(s.l)) * kLn2;
 }
 
 // Visible blocks of sequence b for the query rows up to last_row (exclusive).
@@ -260,8 +257,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
   constexpr int kSlot = kKv8Block * D, kSlots = kRing<D>, kRows = 8 * NT;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) unsigned long long bars[kWarps][kSlots];
-  __shared__ float s_m[kWarps][kRows], s_x[kWarps][kRows], s_l[kWarps][kRows];
-  __shared__ Aside s_aside[2 * NT][kWarps * 32];
+  __shared__ Sum s_sum[kWarps][kRows], s_aside[2 * NT][kWarps * 32];
   __shared__ int s_scan[kWarps];
   __shared__ long long s_before;
   __shared__ int s_b, s_blocks, s_slot, s_last;
@@ -309,7 +305,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
     if (visible_blocks(p, b, row0, rows_end, last) == 0)
       for (int e = tid; e < H * (rows_end - row0) * (D / 4); e += kWarps * 32) {
         const int h = e / ((rows_end - row0) * (D / 4)), r = row0 + e / (D / 4) % (rows_end - row0);
-        write_row(p, b, h, r, e % (D / 4) * 4, make_float4(0, 0, 0, 0), -INFINITY, -INFINITY, 0.0f);
+        write_row(p, b, h, r, e % (D / 4) * 4, make_float4(0, 0, 0, 0), Sum{-INFINITY, 0.0f});
       }
   }
   if (cta >= ctas) return;
@@ -451,10 +447,10 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            Aside& s = s_aside[2 * nt + i][tid];
+            Sum& s = s_aside[2 * nt + i][tid];
             if (!has_aside) s.clear();
             if (ev > e_ref) {
-              s.add(m[nt][i] - (float)e_ref, l[nt][i]);
+              s.add(m[nt][i], l[nt][i] * kv8_pow2(-e_ref));
               l[nt][i] = 0.0f;
             }
           }
@@ -539,11 +535,12 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
 #pragma unroll
           for (int i = 0; i < 2; ++i)
             if (now[nt][i] > -INFINITY) {
-              Aside& s = s_aside[2 * nt + i][tid];
-              s.raise(now[nt][i] - (float)ev);
+              const float add = (float)ev - now[nt][i];
+              float sum = 0.0f;
 #pragma unroll
               for (int mt = 0; mt < 4; ++mt)
-                s.l += exp2a(fmaf(c[mt][nt][i], a[nt][i], -s.m)) + exp2a(fmaf(c[mt][nt][i + 2], a[nt][i], -s.m));
+                sum += exp2a(fmaf(c[mt][nt][i], a[nt][i], add)) + exp2a(fmaf(c[mt][nt][i + 2], a[nt][i], add));
+              s_aside[2 * nt + i][tid].add(now[nt][i], sum * kv8_pow2(-ev));
             }
       }
       const float back_l = low ? 0.0f : kv8_pow2(e_ref - ev);
@@ -646,30 +643,24 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
       }
     }
 
-    // join the warps: 2 and 3 into 0 and 1, then 1 into 0; mx: what l is against
-    float mx[NT][2];
+    // join the warps: 2 and 3 into 0 and 1, then 1 into 0
+    const float undo = kv8_pow2(-e_ref);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        mx[nt][i] = m[nt][i] - (float)e_ref;
-        if (has_aside) {
-          Aside& s = s_aside[2 * nt + i][tid];
-          s.add(mx[nt][i], l[nt][i]);
-          float to = s.m;
-          to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 4));
-          to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 8));
-          to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 16));
-          s.raise(to);
-          mx[nt][i] = s.m;
-          l[nt][i] = s.l;
+        l[nt][i] *= undo;
+        if (has_aside) {  // (its m passes the row's by no more than a maximum lags)
+          const Sum s = s_aside[2 * nt + i][tid];
+          const float g = Sum::half(s.m, m[nt][i]);
+          l[nt][i] += s.l * g * g;
         }
         float v = l[nt][i];
         v += __shfl_xor_sync(0xffffffffu, v, 4);
         v += __shfl_xor_sync(0xffffffffu, v, 8);
         l[nt][i] = v + __shfl_xor_sync(0xffffffffu, v, 16);
         // NaN scores raise no maximum, but the row has seen something all the same
-        if (l[nt][i] != l[nt][i] && lim[nt][i] >= 0 && mx[nt][i] == -INFINITY) m[nt][i] = mx[nt][i] = 0.0f;
+        if (l[nt][i] != l[nt][i] && lim[nt][i] >= 0 && m[nt][i] == -INFINITY) m[nt][i] = 0.0f;
       }
 #pragma unroll
     for (int step = kWarps / 2; step > 0; step >>= 1) {
@@ -686,9 +677,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              s_m[warp][8 * nt + 2 * t4 + i] = m[nt][i];
-              s_x[warp][8 * nt + 2 * t4 + i] = mx[nt][i];
-              s_l[warp][8 * nt + 2 * t4 + i] = l[nt][i];
+              s_sum[warp][8 * nt + 2 * t4 + i] = Sum{m[nt][i], l[nt][i]};
             }
       }
       __syncthreads();
@@ -699,14 +688,13 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
           float mine[2], theirs[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float om = s_m[warp + step][8 * nt + 2 * t4 + i], to = fmaxf(m[nt][i], om);
-            mine[i] = m[nt][i] == -INFINITY ? 0.0f : exp2a(m[nt][i] - to);
-            theirs[i] = om == -INFINITY ? 0.0f : exp2a(om - to);
-            m[nt][i] = to;
-            const float ox = s_x[warp + step][8 * nt + 2 * t4 + i], x = fmaxf(mx[nt][i], ox);
-            l[nt][i] = l[nt][i] * (mx[nt][i] == -INFINITY ? 0.0f : exp2a(mx[nt][i] - x)) +
-                       s_l[warp + step][8 * nt + 2 * t4 + i] * (ox == -INFINITY ? 0.0f : exp2a(ox - x));
-            mx[nt][i] = x;
+            Sum s{m[nt][i], l[nt][i]};
+            const Sum other = s_sum[warp + step][8 * nt + 2 * t4 + i];
+            const float2 f = s.add(other.m, other.l);
+            mine[i] = f.x;
+            theirs[i] = f.y;
+            m[nt][i] = s.m;
+            l[nt][i] = s.l;
           }
 #pragma unroll
           for (int j = 0; j < D / 16; ++j)
@@ -737,7 +725,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
           } else {
             *reinterpret_cast<float2*>(to) = make_float2(o[0][nt][i], o[0][nt][i + 2]);
           }
-          if (g == 0) p.part_ml[slot + rr] = make_float4(m[nt][i], mx[nt][i], l[nt][i], 0.0f);
+          if (g == 0) p.part_ml[slot + rr] = Sum{m[nt][i], l[nt][i]};
         }
       __threadfence();
     }
@@ -755,26 +743,22 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
       const int parts = (int)(c1 - c0) + 1, rows = rows_end - row0;
       for (int e = tid; e < rows * (D / 4); e += kWarps * 32) {
         const int rr = e / (D / 4), d = e % (D / 4) * 4;
-        float mo = -INFINITY, top = -INFINITY;
+        Sum sum{-INFINITY, 0.0f};
 #pragma unroll 8
-        for (int k = 0; k < parts; ++k) {
-          const float2 both = __ldcg(reinterpret_cast<const float2*>(p.part_ml + part0 + kRows * k + rr));
-          mo = fmaxf(mo, both.x), top = fmaxf(top, both.y);
-        }
-        float ll = 0.0f;
+        for (int k = 0; k < parts; ++k) sum.m = fmaxf(sum.m, __ldcg(&p.part_ml[part0 + kRows * k + rr].m));
         float4 oo = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (top > -INFINITY) {
+        if (sum.m > -INFINITY) {
 #pragma unroll 8
           for (int k = 0; k < parts; ++k) {
-            const float4 ml = __ldcg(p.part_ml + part0 + kRows * k + rr);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + part0 + kRows * k + rr);
             const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + (part0 + kRows * k + rr) * D + d));
-            const float f = exp2a(ml.x - mo);
-            ll = fmaf(ml.z, exp2a(ml.y - top), ll);
+            const float g = exp2a(0.5f * (ml.x - sum.m)), f = g * g;
+            sum.l = fmaf(ml.y * g, g, sum.l);
             oo.x = fmaf(v.x, f, oo.x), oo.y = fmaf(v.y, f, oo.y);
             oo.z = fmaf(v.z, f, oo.z), oo.w = fmaf(v.w, f, oo.w);
           }
         }
-        write_row(p, at.b, at.h, row0 + rr, d, oo, mo, top, ll);
+        write_row(p, at.b, at.h, row0 + rr, d, oo, sum);
       }
     }
     if (at.left == 0) break;
@@ -792,20 +776,19 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ A
   const int64_t head = blockIdx.y;
   const int hk = (int)(head % p.c.n_kv_heads), b = (int)(head / p.c.n_kv_heads);
   const int64_t at = (head * p.rows + r) * p.splits;
-  float mo = -INFINITY, top = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) mo = fmaxf(mo, p.part_ml[at + s].x), top = fmaxf(top, p.part_ml[at + s].y);
-  float ll = 0.0f;
+  Sum sum{-INFINITY, 0.0f};
+  for (int s = 0; s < p.splits; ++s) sum.m = fmaxf(sum.m, p.part_ml[at + s].m);
   float4 oo = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (top > -INFINITY)
+  if (sum.m > -INFINITY)
     for (int s = 0; s < p.splits; ++s) {
-      const float4 ml = p.part_ml[at + s];
-      const float f = exp2a(ml.x - mo);
+      const Sum part = p.part_ml[at + s];
+      const float g = exp2a(0.5f * (part.m - sum.m)), f = g * g;
       const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at + s) * p.c.head_dim + d);
-      ll = fmaf(ml.z, exp2a(ml.y - top), ll);
+      sum.l = fmaf(part.l * g, g, sum.l);
       oo.x = fmaf(v.x, f, oo.x), oo.y = fmaf(v.y, f, oo.y);
       oo.z = fmaf(v.z, f, oo.z), oo.w = fmaf(v.w, f, oo.w);
     }
-  write_row(p, b, hk, r, d, oo, mo, top, ll);
+  write_row(p, b, hk, r, d, oo, sum);
 }
 
 // mass_j += sum_r exp(x[r][j] - lse_r) from the scores that the attention left: four
@@ -987,7 +970,7 @@ Plan plan_of(const CbKv8& c, int dtype, int n_q_heads, int T, int longest, bool 
     // rows' scores cost 8 bytes a key to write and read, taking them again head_dim
     if (add_mass && pl.rows * 8 <= c.head_dim) pl.ld_scores = ceil_div(longest, kKv8Block) * kKv8Block;
   }
-  pl.o = pl.ml + align256((size_t)parts * sizeof(float4));
+  pl.o = pl.ml + align256((size_t)parts * sizeof(Sum));
   pl.q16 = pl.o + align256((size_t)parts * c.head_dim * sizeof(float));
   pl.back = pl.q16 + (size_t)bh * pl.row_tiles * 128 * c.head_dim * (dtype == CB_F32 ? 4 : 2);
   pl.scores = pl.back + (size_t)bh * pl.row_tiles * 128 * sizeof(float);
@@ -1053,7 +1036,7 @@ extern "C" int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const
   p.splits = pl.splits;
   uint8_t* base = static_cast<uint8_t*>(scratch);
   p.arrived = reinterpret_cast<int*>(base);
-  p.part_ml = reinterpret_cast<float4*>(base + pl.ml);
+  p.part_ml = reinterpret_cast<Sum*>(base + pl.ml);
   p.part_rows = pl.part_rows;
   p.ld_scores = pl.ld_scores;
   p.scores = pl.ld_scores ? reinterpret_cast<float*>(base + pl.scores) : nullptr;

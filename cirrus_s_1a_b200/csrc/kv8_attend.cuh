@@ -8,6 +8,8 @@
 
 namespace cb {
 
+struct Sum;
+
 struct AttendParams {
   CbKv8 c;
   const void* q;
@@ -23,11 +25,10 @@ struct AttendParams {
   void* out;            // [batch][T][heads][dim], the queries' type
   float* lse;           // [batch][T][heads]
   int splits;           // runs: of all heads' blocks (decode form), of each row tile's keys (prompt form)
-  // parts: the maxima of x + e and of x (log2 units) and the sum, and values.  Decode form:
-  // [16 rows][run + head][16] rows, part_rows of them for each 16 query rows; prompt form:
-  // [head][rows][splits].
+  // parts: sums (Sum), and values against the same m'.  Decode form: [16 rows][run + head][16]
+  // rows, part_rows of them for each 16 query rows; prompt form: [head][rows][splits].
   int64_t part_rows;
-  float4* part_ml;      // [part]
+  Sum* part_ml;         // [part]
   float* part_o;        // [part][dim]
   int* arrived;         // [16 rows][head]: parts finished; zero between calls
   float* scores;        // [head][rows][ld_scores] in log2 units, or null
@@ -42,7 +43,7 @@ struct AttendParams {
 // A row's sum is taken from P against one value exponent e_ref as long as the blocks'
 // exponents lie within kNear of it; what is left of float32's range then holds every P that
 // matters to the sum.  A larger exponent becomes e_ref, what was summed so far is put aside
-// (Aside); blocks of smaller ones are summed there key by key, since their P may vanish
+// (shared memory: it is rarely needed); blocks of smaller ones are summed there key by key, since their P may vanish
 // beside the others' although their keys weigh as much (zeros have the exponent -100).
 constexpr int kNear = 28;
 

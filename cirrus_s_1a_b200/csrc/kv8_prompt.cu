@@ -20,9 +20,8 @@
 //     so that P times the bare codes is the sum over values, and neither a block
 //     of tiny values nor one of huge ones costs the others precision: P's f16
 //     rounding is relative to what the row adds up.  The row's sum (before P is rounded)
-//     is l = sum_b 2^(e_ref - e_b) sum P against m = m' - e_ref, with an e_ref near the
-//     blocks' exponents; blocks far below it (zeros) are summed for themselves (kNear).
-//     out = 2^(m' - m) O / l.
+//     is l 2^m', l = sum_b 2^-e_b sum P, added up against an exponent e_ref near the blocks'
+//     own; blocks far below it (zeros) are summed for themselves (kNear).  out = O / l.
 //   * a thread reads its row of S into registers at once, so that the next tile's
 //     scores can follow, and takes P against the maximum so far.  Only where the
 //     tile's passes it by more than 2^15 (f16 P ends at 2^16) is it raised, and O
@@ -282,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   __shared__ __align__(8) unsigned long long bars[20];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
-  __shared__ Aside s_aside[kTiles * kRows];
+  __shared__ Sum s_aside[kTiles * kRows];
   __shared__ int s_nan;  // the first slot with an E4M3 NaN among values that not all rows see
   __shared__ int s_end;  // the end of the run's slots
   uint8_t* sq = smem;
@@ -354,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       const float* vsc = p.c.v_scale + head * (p.c.max_len / kKv8Block);
       const int vis = last / kKv8Block;  // the last block any row sees
       float m = -INFINITY, l = 0.0f;
-      Aside& aside = s_aside[tid];
+      Sum& aside = s_aside[tid];
       aside.clear();
       // the run's largest value exponent, and whether any lies far below it
       int e_ref = 0;
@@ -410,9 +409,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
               x = fmaxf(x, __uint_as_float(u[i]));
             }
             if (x > -INFINITY) {
-              aside.raise(x * by);
+              const int e = first ? ev[0] : ev[kHalves - 1];
+              x = fmaf(x, by, (float)e);
+              float sum = 0.0f;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) aside.l += exp2a(fmaf(__uint_as_float(u[i]), by, -aside.m));
+              for (int i = 0; i < 16; ++i) sum += exp2a(fmaf(__uint_as_float(u[i]), by, (float)e - x));
+              aside.add(x, sum * kv8_pow2(-e));
             }
             __syncwarp();
           }
@@ -496,22 +498,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         fence_before();
         mbar_arrive(p_full + 8 * tile);
       }
-      // results: O, m', and l against mx.  (Products n - 2 and before are known done.)
+      // results: O, and the sum.  (Products n - 2 and before are known done.)
       if (n > 0) wait(o_full + 8 * tile, n - 1);
       fence_after();
-      float mx = m - (float)e_ref;
-      if (aside.l != 0.0f) {
-        aside.add(mx, l);
-        mx = aside.m;
-        l = aside.l;
+      l *= kv8_pow2(-e_ref);
+      if (wide) {  // (its m passes the row's by no more than a maximum lags)
+        const float g = Sum::half(aside.m, m);
+        l += aside.l * g * g;
       }
       const int t = r / p.G, hq = (int)(head % p.c.n_kv_heads) * p.G + r % p.G;
       const int64_t orow = ((int64_t)b * p.T + t) * (p.G * p.c.n_kv_heads) + hq;
       const int64_t at = (head * p.rows + r) * p.splits + split;
       // NaN scores raise no maximum, but the row has seen something all the same
       const bool none = lim < 0 || l == 0.0f;
-      // 2^(m' - m) / l in two factors: an exponent of up to 135 times a small sum
-      const float half = none ? 0.0f : exp2a(0.5f * (m - mx)), inv = none ? 0.0f : half / l;
+      const Inverse inv(none ? 1.0f : l);
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         float o[32];
@@ -531,14 +531,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + orow * D + c);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            dst[i] = make_float4(o[4 * i] * half * inv, o[4 * i + 1] * half * inv, o[4 * i + 2] * half * inv,
-                                 o[4 * i + 3] * half * inv);
+            dst[i] = make_float4(inv.of(o[4 * i]), inv.of(o[4 * i + 1]), inv.of(o[4 * i + 2]), inv.of(o[4 * i + 3]));
         } else {
           uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + orow * D + c);
           uint32_t u[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float y0 = o[2 * i] * half * inv, y1 = o[2 * i + 1] * half * inv;
+            const float y0 = inv.of(o[2 * i]), y1 = inv.of(o[2 * i + 1]);
             u[i] = p.dtype == CB_BF16 ? (uint32_t)f32_to_bf16(y0) | (uint32_t)f32_to_bf16(y1) << 16
                                       : h2_bits(__floats2half2_rn(y0, y1));
           }
@@ -548,9 +547,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       }
       if (r < p.rows && ok) {
         if (p.splits > 1) {
-          p.part_ml[at] = make_float4(m, none ? -INFINITY : fmaxf(mx, -3e38f), none ? 0.0f : l, 0.0f);
+          p.part_ml[at] = none ? Sum{-INFINITY, 0.0f} : Sum{fmaxf(m, -3e38f), l};
         } else {
-          p.lse[orow] = none ? -INFINITY : (mx + log2f(l)) * kLn2;
+          p.lse[orow] = none ? -INFINITY : (m + log2f(l)) * kLn2;
         }
       }
     }

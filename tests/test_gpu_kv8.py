@@ -269,6 +269,24 @@ def test_float32_keeps_small_probabilities(D, n):
         assert (out[0, 0, 0].cpu().double() / want - 1).abs().max() < 2.0 ** -18
 
 
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("T", [1, 130])
+def test_values_of_equal_keys_come_out_whatever_the_scores(D, T):
+    """Keys and values all alike: the output is the value.  Probabilities carry 2^-22, exponentials
+    and sums 2^-20, and up to 18 products of 16 keys a truncation of 2^-23 each: less than 2^-18.
+    (A score of 4095 has its last bit at 2^-12, but it is the same for all keys.)"""
+    cache = filled(1, 1, D, 192, "int8")
+    cache.k.fill_(1)
+    cache.v.fill_(93)
+    cache.k_scale.fill_(1.0)
+    for e in (-20, -6, 0, 9):
+        cache.v_scale.fill_(2.0 ** e)
+        for score in (0.0, 11.0, 2848.5, 2849.125, 2849.75, 2850.5, -2834.5, -2835.125, -2836.25, 90000.0):
+            q = torch.full((1, T, 1, D), score / D)
+            out, lse = cache.attend(q.to(DEV), ints([130 - T]), scale=1.0)
+            assert (out.cpu().double() / (93 * 2.0 ** e) - 1).abs().max() < 2.0 ** -18, (e, score)
+
+
 @pytest.mark.parametrize("T", [1, 130])
 def test_peaked_and_extreme_scores(T):
     """Scores of thousands (one key takes all), queries of 1e-30 (all keys alike) and zeros."""
