@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
   float* s_join = reinterpret_cast<float*>(smem + kWarps * kSlots * kSlot);  // [2][kRows * D]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const int H = p.c.n_kv_heads, B = p.c.batch;
-  const int row0 = blockIdx.y * kRows, rows_end = min(row0 + kRows, p.rows);
+  const int row0 = (p.block0 + blockIdx.y) * kRows, rows_end = min(row0 + kRows, p.rows);
   const int64_t cta = blockIdx.x;
 
   // ------------------------------------------- this CTA's run of blocks
@@ -921,10 +921,12 @@ Form form_of(const CbKv8& c, int dtype, int rows) {
 }
 
 // How a call is cut up, and where its parts lie in the scratch.  The counters come
-// first, in every call's layout: they are zero between calls.
+// first, in every call's layout: they are zero between calls.  A call with more 8-row
+// blocks over all heads than there are counters takes its rows in several launches.
 constexpr size_t kCounters = CB_KV8_ZEROED / sizeof(int);
 struct Plan {
   int rows = 0, row_tiles = 0, splits = 0;
+  int blocks = 0;  // of query rows, in a launch of the decode form
   int64_t part_rows = 0, ld_scores = 0;
   size_t ml = 0, o = 0, q16 = 0, back = 0, scores = 0, bytes = 0;
 };
@@ -961,12 +963,12 @@ Plan plan_of(const CbKv8& c, int dtype, int n_q_heads, int T, int longest, bool 
     int resident = 1;  // without a device: only the layout is asked for
     if (ensure_smem_attr((const void*)f.attend, f.smem) == CB_OK)
       resident = std::max(1, resident_ctas((const void*)f.attend, kWarps * 32, f.smem));
-    const int blocks = ceil_div(pl.rows, f.rows);
-    const int64_t fit = std::max(1, num_sms() * resident / blocks);
+    pl.blocks = std::min({ceil_div(pl.rows, f.rows), (int)kCounters / bh, 65535});
+    const int64_t fit = std::max(1, num_sms() * resident / pl.blocks);
     const int64_t work = std::max<int64_t>(1, (int64_t)bh * ceil_div(longest, kKv8Block) / kWarps);
     pl.splits = (int)std::min(std::min(fit, work), (int64_t)bh * 48);
     pl.part_rows = ((int64_t)bh + pl.splits) * f.rows;
-    parts = pl.part_rows * blocks;
+    parts = pl.part_rows * pl.blocks;
     // rows' scores cost 8 bytes a key to write and read, taking them again head_dim
     if (add_mass && pl.rows * 8 <= c.head_dim) pl.ld_scores = ceil_div(longest, kKv8Block) * kKv8Block;
   }
@@ -984,10 +986,6 @@ int check_call(const CbKv8* c, int dtype, int n_q_heads, int T, int longest) {
   if (n_q_heads <= 0 || n_q_heads % c->n_kv_heads) return CB_ERR_SHAPE;
   const int64_t rows = (int64_t)T * (n_q_heads / c->n_kv_heads);
   if (rows > 65535 * 16) return CB_ERR_SHAPE;
-  // a counter for each head and 8 rows
-  if ((rows <= 32 || c->head_dim < 64) &&
-      (rows + 7) / 8 * c->batch * c->n_kv_heads > (int64_t)kCounters)
-    return CB_ERR_SHAPE;
   return CB_OK;
 }
 
@@ -1057,8 +1055,10 @@ extern "C" int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const
   } else {
     const Form f = form_of(*c, dtype, p.rows);
     if (const int rc = ensure_smem_attr((const void*)f.attend, f.smem)) return rc;
-    f.attend<<<dim3(p.splits, ceil_div(p.rows, f.rows)), kWarps * 32, f.smem, st>>>(p);
-    count_launch();
+    for (const int all = ceil_div(p.rows, f.rows); p.block0 < all; p.block0 += pl.blocks) {
+      f.attend<<<dim3(p.splits, std::min(pl.blocks, all - p.block0)), kWarps * 32, f.smem, st>>>(p);
+      count_launch();
+    }
     if (p.scores) {
       kv8_scores_mass_kernel<<<dim3(ceil_div(longest, 1024), bh), 256, 0, st>>>(p);
       count_launch();

@@ -24,6 +24,7 @@ struct AttendParams {
   bool add_mass;
   void* out;            // [batch][T][heads][dim], the queries' type
   float* lse;           // [batch][T][heads]
+  int block0;           // decode form: the launch's first block of query rows
   int splits;           // runs: of all heads' blocks (decode form), of each row tile's keys (prompt form)
   // parts: sums (Sum), and values against the same m'.  Decode form: [16 rows][run + head][16]
   // rows, part_rows of them for each 16 query rows; prompt form: [head][rows][splits].

@@ -433,6 +433,7 @@ int cb_kv8_append(const CbKv8* c, const void* k, const void* v, int32_t dtype, c
  * have been appended with the same pos: row t of sequence b sees slots
  * j <= pos[b] + t.  q (its type and strides as k above) holds n_q_heads heads, a
  * multiple of n_kv_heads; query head i reads KV head i / (n_q_heads / n_kv_heads).
+ * T * n_q_heads / n_kv_heads, the query rows of a KV head, is at most 1048560.
  *   out [batch][T][n_q_heads][head_dim], q's type: softmax(scale * q . k) v
  *   lse [batch][T][n_q_heads] float32: log of the softmax's sum (natural log)
  *   add_mass: mass[b][h][j] += the probabilities of slot j over the head's rows

@@ -183,6 +183,29 @@ def test_attend_prompts(fmt, dtype, Hq, H, D, T, pos):
     check_attend(cache, q, pos, counts=[T - 9, 0], dtype=dtype, add_mass=True)
 
 
+@pytest.mark.parametrize("D,dtype", [(16, "bf16"), (32, "f32")])
+def test_long_prompts_of_many_sequences(D, dtype):
+    """More query rows over all heads than the scratch has counters for.  Against a call for
+    each sequence: the same scores, joined in other parts."""
+    from cirrus_s_1a_b200.kv8 import Kv8Cache
+
+    B, T = 33, 4096
+    big = filled(B, 2, D, T + 64, "int8")
+    q = torch.randn(B, T, 4, D, generator=torch.Generator().manual_seed(D)).to(TYPES[dtype]).to(DEV)
+    pos = ints([b % 7 for b in range(B)])
+    before = big.mass.clone()
+    out, lse = big.attend(q, pos, add_mass=True)
+    again, _ = big.attend(q, pos)
+    assert torch.equal(out, again)
+    for b in (0, 17, 32):
+        one = Kv8Cache.from_tensors(*(t[b:b + 1].contiguous() for t in (big.k, big.v, big.k_scale, big.v_scale, before)))
+        o, s = one.attend(q[b:b + 1].contiguous(), ints([b % 7]), add_mass=True)
+        near = 127 * float(big.v_scale.max()) * (2.0 ** -7 if dtype == "bf16" else 2.0 ** -17)
+        assert (o[0].float() - out[b].float()).abs().max() <= near
+        assert (s[0] - lse[b]).abs().max() < 2.0 ** -16
+        assert (one.mass[0] - big.mass[b]).abs().max() <= 2.0 ** -15 * one.mass.abs().max()
+
+
 def test_rows_that_see_nothing_give_zero_and_minus_infinity():
     cache = filled(4, 2, 64, 128, "e4m3")
     q = torch.randn(4, 3, 6, 64).bfloat16()
