@@ -290,8 +290,8 @@ struct Kv8Run {
   int32_t* slots = nullptr;
   bool add_mass = false;
   float* k = nullptr;       // [R][kv heads][hd]
-  void* q = nullptr;        // f16 [R][q heads][hd]
-  void* o = nullptr;        // f16 [R][q heads][hd]
+  float* q = nullptr;       // [R][q heads][hd]
+  float* o = nullptr;       // [R][q heads][hd]
   float* lse = nullptr;     // [R][q heads]
   int32_t* at = nullptr;    // [2][batch]: slots of the chunk's first token, of its first query
   void* scratch = nullptr;
@@ -307,8 +307,8 @@ static Kv8Run kv8_carve(const CbModel& m, int batch, int T, size_t off, char* ba
     return base ? base + o : nullptr;
   };
   r.k = (float*)take(R * m.n_kv_heads * m.head_dim * 4);
-  r.q = take(R * m.n_q_heads * m.head_dim * 2);
-  r.o = take(R * m.n_q_heads * m.head_dim * 2);
+  r.q = (float*)take(R * m.n_q_heads * m.head_dim * 4);
+  r.o = (float*)take(R * m.n_q_heads * m.head_dim * 4);
   r.lse = (float*)take(R * m.n_q_heads * 4);
   r.at = (int32_t*)take((size_t)batch * 2 * 4);
   r.scratch_off = off;
@@ -610,7 +610,7 @@ static int forward(const CbModel* mp, const CbCache* cp, const Kv8Run* kv8_in, v
       hp.norm = m.shared_k_norm;
       hp.inv_freq = m.inv_freq;
       hp.eps = m.norm_eps;
-      hp.out32 = kv8.k;
+      hp.out = kv8.k;
       CB_TRY(launch_kv8_heads(hp, st));
       CB_TRY(launch_kv8_slots(kv8.slots, B, c0, kv8.at, st));
       const int64_t hd = m.head_dim, width = m.n_kv_heads * hd;
@@ -697,12 +697,12 @@ static int forward(const CbModel* mp, const CbCache* cp, const Kv8Run* kv8_in, v
         hp.norm = L.q_norm;
         hp.inv_freq = m.inv_freq;
         hp.eps = m.norm_eps;
-        hp.out16 = static_cast<__half*>(kv8.q);
+        hp.out = kv8.q;
         CB_TRY(launch_kv8_heads(hp, st));
         int32_t* at = kv8.at + B;
         if (j == 0) CB_TRY(launch_kv8_slots(kv8.slots, B, c0 + t_off, at, st));
         const int64_t hd = m.head_dim, width = m.n_q_heads * hd, qs[3] = {nqc * width, width, hd};
-        CB_TRY(cb_kv8_attend(kv8.kv, kv8.q, CB_F16, qs, m.n_q_heads, nqc, at, nullptr, kv8.kv->max_len,
+        CB_TRY(cb_kv8_attend(kv8.kv, kv8.q, CB_F32, qs, m.n_q_heads, nqc, at, nullptr, kv8.kv->max_len,
                              1.0f / sqrtf((float)m.head_dim), kv8.add_mass, kv8.o, kv8.lse, kv8.scratch,
                              kv8.scratch_bytes, w.status, st));
         CB_TRY(launch_kv8_gate(kv8.o, w.cproj + m.cr_off_gate, ldc, RQ, m.n_q_heads, m.head_dim, w.attn, w.att_ld, st));
@@ -792,7 +792,7 @@ extern "C" size_t cb_forward_kv8_workspace_bytes(const CbModel* m, const CbKv8* 
   size_t scratch = 0;  // of any chunk's query count, with weights or without
   for (int n = 1, most = chunk_tokens(*m, T); n <= most; ++n)
     for (int mass = 0; mass < 2; ++mass)
-      scratch = std::max(scratch, cb_kv8_attend_scratch_bytes(kv8, CB_F16, m->n_q_heads, n, kv8->max_len, mass));
+      scratch = std::max(scratch, cb_kv8_attend_scratch_bytes(kv8, CB_F32, m->n_q_heads, n, kv8->max_len, mass));
   return scratch ? off + scratch : 0;
 }
 

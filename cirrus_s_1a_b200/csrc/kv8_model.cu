@@ -6,8 +6,7 @@
 namespace cb {
 namespace {
 
-// RMSNorm and RoPE of one head per warp (layers.py:72-82, 325-331), as float32 keys
-// or f16 queries (normed heads: far inside f16's range, 11 bits of each value).
+// RMSNorm and RoPE of one head per warp (layers.py:72-82, 325-331), keys or queries.
 __global__ void __launch_bounds__(256) kv8_heads_kernel(const __grid_constant__ Kv8HeadsParams p) {
   const int item = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (item >= p.rows * p.heads) return;
@@ -20,21 +19,17 @@ __global__ void __launch_bounds__(256) kv8_heads_kernel(const __grid_constant__ 
   for (int j = lane; j < p.hd / 2; j += 32) {
     float x1 = x[2 * j] * rn * p.norm[2 * j], x2 = x[2 * j + 1] * rn * p.norm[2 * j + 1];
     if (j < p.rot2) rope_pair(x1, x2, position, p.inv_freq[j]);
-    if (p.out16) {
-      reinterpret_cast<__half2*>(p.out16 + (int64_t)item * p.hd)[j] = __floats2half2_rn(x1, x2);
-    } else {
-      reinterpret_cast<float2*>(p.out32 + (int64_t)item * p.hd)[j] = make_float2(x1, x2);
-    }
+    reinterpret_cast<float2*>(p.out + (int64_t)item * p.hd)[j] = make_float2(x1, x2);
   }
 }
 
 // out[r][h][d] = o[r][h][d] * sigmoid(gate[r][h]) (layers.py:243)
-__global__ void __launch_bounds__(256) kv8_gate_kernel(const __half* __restrict__ o, const float* __restrict__ gate, int ldg,
+__global__ void __launch_bounds__(256) kv8_gate_kernel(const float* __restrict__ o, const float* __restrict__ gate, int ldg,
                                                        int rows, int heads, int hd, float* __restrict__ out, int ldo) {
   const int i = blockIdx.x * 256 + threadIdx.x, width = heads * hd;
   if (i >= rows * width) return;
   const int r = i / width, c = i % width;
-  out[(int64_t)r * ldo + c] = __half2float(o[i]) * sigmoid(gate[(int64_t)r * ldg + c / hd]);
+  out[(int64_t)r * ldo + c] = o[i] * sigmoid(gate[(int64_t)r * ldg + c / hd]);
 }
 
 // at[b] = slots[b] + offset
@@ -51,10 +46,9 @@ int launch_kv8_heads(const Kv8HeadsParams& p, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
 }
 
-int launch_kv8_gate(const void* o, const float* gate, int ldg, int rows, int heads, int hd, float* out, int ldo,
+int launch_kv8_gate(const float* o, const float* gate, int ldg, int rows, int heads, int hd, float* out, int ldo,
                     cudaStream_t st) {
-  kv8_gate_kernel<<<ceil_div(rows * heads * hd, 256), 256, 0, st>>>(static_cast<const __half*>(o), gate, ldg, rows, heads,
-                                                                    hd, out, ldo);
+  kv8_gate_kernel<<<ceil_div(rows * heads * hd, 256), 256, 0, st>>>(o, gate, ldg, rows, heads, hd, out, ldo);
   count_launch();
   return cudaGetLastError() == cudaSuccess ? CB_OK : CB_ERR_CUDA;
 }

@@ -6,8 +6,6 @@
 
 #include "cirrus_b200.h"
 
-struct __half;
-
 namespace cb {
 
 struct Kv8HeadsParams {
@@ -20,12 +18,11 @@ struct Kv8HeadsParams {
   const float* norm;
   const float* inv_freq;
   float eps;
-  float* out32;           // [rows][heads][hd], or
-  __half* out16;
+  float* out;             // [rows][heads][hd]
 };
 
 int launch_kv8_heads(const Kv8HeadsParams& p, cudaStream_t st);
-int launch_kv8_gate(const void* o, const float* gate, int ldg, int rows, int heads, int hd, float* out, int ldo,
+int launch_kv8_gate(const float* o, const float* gate, int ldg, int rows, int heads, int hd, float* out, int ldo,
                     cudaStream_t st);
 int launch_kv8_slots(const int32_t* slots, int batch, int offset, int32_t* at, cudaStream_t st);
 int kv8_check(const CbKv8* c);

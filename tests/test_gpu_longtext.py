@@ -145,3 +145,27 @@ def test_a_capture_wants_its_workspace_first():
         t.copy_(was)
     graph.replay()
     torch.testing.assert_close(logits, want, rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("kw", [{}, WIDE], ids=["debug", "wide"])
+def test_values_past_the_range_of_f16(kw):
+    """The 8-bit cache holds keys and values alone in fewer bits: values of 1e6 pass through
+    the attention as they do on the bf16 path."""
+    from cirrus_s_1a_b200 import synthetic
+    from cirrus_s_1a_b200.config import get_config
+    from cirrus_s_1a_b200.engine import CirrusB200
+
+    cfg = replace(get_config("cirrus-s-1a-debug"), sparse_topk=None, **kw)
+    sd = synthetic.random_state_dict(cfg, seed=3, norm_jitter=0.1)
+    name = [n for n in sd if "shared" in n and "norm" in n and "k_norm" not in n]
+    assert len(name) == 1, name
+    sd[name[0]] = sd[name[0]] * 1e6
+    eng = CirrusB200(cfg, sd, device=DEV, max_ctx=640)
+    ids = text(cfg, 22)
+    a, b = eng.new_cache(kv8="int8"), eng.new_cache()
+    for lo, hi in ((0, 16), (16, 17), (17, 22)):  # (the many-token GEMM takes inputs up to 65504)
+        x, y = eng(ids[:, lo:hi], cache=a).logits, eng(ids[:, lo:hi], cache=b).logits
+        assert float(a.kv8.values()[1].abs().max()) > 65504
+        # int8 values are within 2^-7 of their block's largest (1.6 % of a typical one); the
+        # layers behind may double that
+        assert float((x - y).norm() / y.norm()) < 0.1
