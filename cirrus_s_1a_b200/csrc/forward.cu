@@ -648,7 +648,8 @@ static int forward(const CbModel* mp, const CbCache* cp, const Kv8Run* kv8_in, v
     }
 
     // --------------------------------------------------- cross-decoder
-    const int nqc = std::max(0, std::min(tc, c0 + tc - (T - nq)));
+    const int asked = std::max(0, std::min(tc, c0 + tc - (T - nq)));  // rows with outputs
+    const int nqc = kv8.add_mass ? tc : asked;  // attention weights come from every token
     if (nqc == 0) continue;
     const int RQ = B * nqc, t_off = tc - nqc;
     gather_rows_kernel<<<RQ, 256, 0, st>>>(w.h, tc, t_off, nqc, d, w.xc);
@@ -744,28 +745,37 @@ static int forward(const CbModel* mp, const CbCache* cp, const Kv8Run* kv8_in, v
     }
 
     // --------------------------------------------------- LM head + outputs
+    if (asked == 0) continue;
+    float* xo = w.xc;
+    const int RO = B * asked;
+    if (asked < nqc) {
+      xo = w.h;  // this chunk is done with it
+      gather_rows_kernel<<<RO, 256, 0, st>>>(w.xc, nqc, nqc - asked, asked, d, xo);
+      count_launch();
+      if (cudaGetLastError() != cudaSuccess) return CB_ERR_CUDA;
+    }
     const int V = m.vocab_size;
-    const int out_off = c0 + t_off - (T - nq);  // first logits row of this chunk, per sequence
+    const int out_off = c0 + tc - asked - (T - nq);  // first logits row of this chunk, per sequence
     const bool direct = (tc == T) && logits != nullptr;
     float* lg = direct ? logits : w.logits;
-    CB_TRY(proj(w, m.lm_head, w.xc, d, RQ, m.final_norm, m.norm_eps, PRE_RMSNORM, EPI_STORE, lg, V, V, st));
+    CB_TRY(proj(w, m.lm_head, xo, d, RO, m.final_norm, m.norm_eps, PRE_RMSNORM, EPI_STORE, lg, V, V, st));
     if (logits && !direct) {
-      scatter_rows_kernel<float><<<RQ, 256, 0, st>>>(lg, V, nqc, nq, out_off, logits);
+      scatter_rows_kernel<float><<<RO, 256, 0, st>>>(lg, V, asked, nq, out_off, logits);
       count_launch();
       if (cudaGetLastError() != cudaSuccess) return CB_ERR_CUDA;
     }
     if (argmax) {
       if (tc == T) {
-        CB_TRY(launch_argmax(lg, RQ, V, V, argmax, st));
+        CB_TRY(launch_argmax(lg, RO, V, V, argmax, st));
       } else {
-        CB_TRY(launch_argmax(lg, RQ, V, V, w.amax, st));
-        scatter_rows_kernel<int32_t><<<RQ, 32, 0, st>>>(w.amax, 1, nqc, nq, out_off, argmax);
+        CB_TRY(launch_argmax(lg, RO, V, V, w.amax, st));
+        scatter_rows_kernel<int32_t><<<RO, 32, 0, st>>>(w.amax, 1, asked, nq, out_off, argmax);
         count_launch();
         if (cudaGetLastError() != cudaSuccess) return CB_ERR_CUDA;
       }
     }
     if (hidden) {
-      scatter_rows_kernel<float><<<RQ, 256, 0, st>>>(w.xc, d, nqc, nq, out_off, hidden);
+      scatter_rows_kernel<float><<<RO, 256, 0, st>>>(xo, d, asked, nq, out_off, hidden);
       count_launch();
       if (cudaGetLastError() != cudaSuccess) return CB_ERR_CUDA;
     }

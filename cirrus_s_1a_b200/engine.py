@@ -418,7 +418,8 @@ class CirrusB200:
     def new_cache(self, batch: int = 1, max_ctx: int | None = None, kv8: str | None = None,
                   add_mass: bool = False) -> DeviceCache:
         """``kv8``: the shared K/V in 8 bits, ``max_ctx`` slots of it; ``add_mass``: each
-        forward adds the slots' attention weights up for ``DeviceCache.evict``."""
+        forward adds the slots' attention weights up for ``DeviceCache.evict``, every token's
+        (also where ``n_logits`` asks for fewer, which then saves the LM head alone)."""
         with torch.cuda.device(self.device):
             return DeviceCache(self.model, batch, max_ctx or self.max_ctx, kv8=kv8, add_mass=add_mass)
 

@@ -473,7 +473,8 @@ int cb_kv8_evict(const CbKv8* c, const int32_t* pos, int32_t keep, int32_t recen
  * positions cache->pos) and values are appended at slots[b] (device int32, the slots
  * of kv8 in use, <= pos[b] once slots have been evicted), every cross layer attends
  * over kv8 (queries and outputs in float32), and slots[b] advances by T with pos[b].
- * add_mass: each cross layer adds its attention weights to kv8->mass.  The cache's
+ * add_mass: each cross layer adds its attention weights to kv8->mass, those of every
+ * token (the cross layers then run for all T, whatever n_logits is).  The cache's
  * kv_k / kv_v / kv_ik are not used (null), its max_ctx does not bound positions;
  * tokens past kv8->max_len are dropped and the status word receives
  * CB_ERR_CTX_FULL.  workspace: cb_forward_kv8_workspace_bytes, zeroed once.

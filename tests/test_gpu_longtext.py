@@ -169,3 +169,19 @@ def test_values_past_the_range_of_f16(kw):
         # int8 values are within 2^-7 of their block's largest (1.6 % of a typical one); the
         # layers behind may double that
         assert float((x - y).norm() / y.norm()) < 0.1
+
+
+@pytest.mark.parametrize("kw", [{}, WIDE], ids=["debug", "wide"])
+def test_weights_come_from_every_token_whatever_logits_are_asked_for(kw):
+    cfg, eng = model(**kw)
+    ids = text(cfg, 300, 2)
+    full, last = (eng.new_cache(2, kv8="int8", add_mass=True) for _ in range(2))
+    for lo, hi in ((0, 290), (290, 295), (295, 300)):
+        x = eng(ids[:, lo:hi], cache=full)
+        y = eng(ids[:, lo:hi], cache=last, n_logits=2)
+        assert y.logits.shape[1] == y.hidden.shape[1] == 2
+        assert torch.equal(x.hidden[:, -2:], y.hidden)
+        # the LM head of few rows runs on the GEMV, of many on the tensor cores (22-bit inputs)
+        torch.testing.assert_close(x.logits[:, -2:], y.logits, rtol=1e-4, atol=1e-4)
+        assert torch.equal(full.kv8.mass, last.kv8.mass)
+    assert torch.equal(full.evict(100, 20), last.evict(100, 20))
