@@ -471,6 +471,7 @@ class CirrusB200:
         (``cb_workspace_layout``): ``proj`` float32 [batch*Tc, ld] (the shared
         projection: k | v | idx_k | idx_q | idx_w), ``sel_idx`` int32 [rows, k+1]
         and ``sel_cnt`` int32 [rows] (the keys each query row selected)."""
+        self._bf16_only(cache, "intermediates")
         ws = self.workspace(cache.batch, T, cache.max_ctx)
         lay = _lib.CbWorkspaceLayout()
         _lib.check(_lib.lib().cb_workspace_layout(C.byref(self.model.desc), cache.batch, T, cache.max_ctx,
@@ -488,18 +489,31 @@ class CirrusB200:
         """Bounded-wait limit of the persistent kernel on this cache's workspace
         (``cb_set_wait_limit``; 0 = the default 200 ms).  ``stall_barrier`` > 0
         makes one barrier of every later launch incomplete (fault injection for tests)."""
+        self._bf16_only(cache, "set_wait_limit")
         ws = self.workspace(cache.batch, T, cache.max_ctx)
         _lib.check(_lib.lib().cb_set_wait_limit(ws.data_ptr(), int(limit_ns), int(stall_barrier),
                                                 _stream_ptr(self.device)), "cb_set_wait_limit")
 
+    @staticmethod
+    def _bf16_only(cache: DeviceCache, what: str) -> None:
+        if cache.kv8 is not None:
+            raise ValueError(f"{what} is about the workspace of the bf16 shared cache")
+
     def clear_status(self, cache: DeviceCache, T: int = 1) -> None:
+        """Clears the status of ``T``-token forwards; of an 8-bit cache, of all its calls."""
+        if cache.kv8 is not None:
+            for ws in (cache.kv8.status.view(torch.uint8), *cache.kv8.workspaces.values()):
+                ws[:4].zero_()
+            return
         ws = self.workspace(cache.batch, T, cache.max_ctx)
         _lib.check(_lib.lib().cb_clear_status(ws.data_ptr(), _stream_ptr(self.device)), "cb_clear_status")
 
     def read_status(self, cache: DeviceCache, T: int = 1) -> int:
+        """The status of ``T``-token forwards; of an 8-bit cache, of all its calls (the first that is
+        not 0).  Synchronises."""
         if cache.kv8 is not None:
-            ws = cache.kv8.workspaces.get(min(T, CB_PREFILL_CHUNK))
-            return 0 if ws is None else int(ws[:4].view(torch.int32).item())
+            words = [cache.kv8.status, *(ws[:4].view(torch.int32) for ws in cache.kv8.workspaces.values())]
+            return next((v for v in torch.cat(words).tolist() if v), 0)
         ws = self.workspace(cache.batch, T, cache.max_ctx)
         out = _lib.I32(0)
         _lib.check(_lib.lib().cb_read_status(ws.data_ptr(), C.byref(out), _stream_ptr(self.device)), "status")
@@ -508,6 +522,7 @@ class CirrusB200:
     def phase_trace(self, cache: DeviceCache, T: int = 1) -> list:
         """Per-phase timing of the last persistent launch on this cache's workspace:
         a list of (phase index, CTA-0 work us, barrier wait us) from %globaltimer stamps."""
+        self._bf16_only(cache, "phase_trace")
         ws = self.workspace(cache.batch, T, cache.max_ctx)
         buf = (C.c_uint64 * 512)()
         n = _lib.lib().cb_read_trace(C.byref(self.model.desc), cache.batch, min(T, CB_MAX_T), cache.max_ctx,

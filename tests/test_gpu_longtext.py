@@ -185,3 +185,22 @@ def test_weights_come_from_every_token_whatever_logits_are_asked_for(kw):
         torch.testing.assert_close(x.logits[:, -2:], y.logits, rtol=1e-4, atol=1e-4)
         assert torch.equal(full.kv8.mass, last.kv8.mass)
     assert torch.equal(full.evict(100, 20), last.evict(100, 20))
+
+
+def test_status_of_an_8_bit_cache_is_seen_and_cleared():
+    cfg, eng = model()
+    ids = text(cfg, 60)
+    cache = eng.new_cache(max_ctx=64, kv8="e4m3")
+    eng(ids[:, :40], cache=cache)
+    eng(ids[:, 40:41], cache=cache)
+    assert eng.read_status(cache) == 0
+    cache.slots_host = [0]  # the host's count does not stop it: the device drops the tokens and says so
+    eng(ids[:, :40], cache=cache)
+    assert eng.read_status(cache) == 5 and eng.read_status(cache, 40) == 5
+    eng.clear_status(cache)
+    assert eng.read_status(cache) == 0 and eng.read_status(cache, 40) == 0
+    held = len(eng._ws)
+    for wrong in (lambda: eng.intermediates(cache), lambda: eng.phase_trace(cache), lambda: eng.set_wait_limit(cache, 0)):
+        with pytest.raises(ValueError):
+            wrong()
+    assert len(eng._ws) == held
