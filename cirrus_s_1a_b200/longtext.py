@@ -27,6 +27,7 @@ from dataclasses import replace
 
 import torch
 
+from cirrus_s_1a_b200 import _lib
 from cirrus_s_1a_b200._lib import CB_PREFILL_CHUNK
 from cirrus_s_1a_b200.logprobs import TokenLogprobs, token_logprobs
 
@@ -37,7 +38,9 @@ def score_text(engine, tokens: torch.Tensor, cache, keep: int | None = None, rec
     """Scores ``tokens`` (int64 [B, N]) behind what ``cache`` holds: entry [b, t] is
     about token t + 1 given the tokens up to t (N - 1 of them; the arrays of
     ``TokenLogprobs`` with a leading [B, N - 1]).  ``keep`` (8-bit caches): after each
-    chunk sequences are brought down to ``keep`` slots, the ``recent`` last among them."""
+    chunk sequences are brought down to ``keep`` slots, the ``recent`` last among them.
+    Reads the device status at the end (and synchronises): a token outside the vocabulary,
+    a full cache or a wait that gave up is an error, with the status cleared."""
     B, N = tokens.shape
     if N < 2:
         raise ValueError("scoring needs at least two tokens")
@@ -46,14 +49,23 @@ def score_text(engine, tokens: torch.Tensor, cache, keep: int | None = None, rec
     if keep is not None and not cache.add_mass:
         raise ValueError("eviction goes by attention weights: a cache with add_mass=True")
     ids = tokens.to(engine.device, torch.int64)
-    follow = ids[:, 1:].to(torch.int32)
-    parts = []
+    vocab = engine.cfg.vocab_size
+    follow = ids[:, 1:]
+    follow = torch.where((follow >= 0) & (follow < vocab), follow, vocab).to(torch.int32)
+    status = torch.zeros(1, dtype=torch.int32, device=engine.device)
+    parts, lengths = [], set()
     for t in range(0, N - 1, chunk):
         n = min(chunk, N - 1 - t)
         out = engine(ids[:, t:t + n], cache=cache)
-        parts.append(token_logprobs(out.logits.flatten(0, 1), follow[:, t:t + n].reshape(-1).contiguous(), top))
+        parts.append(token_logprobs(out.logits.flatten(0, 1), follow[:, t:t + n].reshape(-1).contiguous(), top,
+                                    status))
+        lengths.add(n)
         if keep is not None:
             cache.evict(keep, recent)
+    rc = int(status) or next((r for r in (engine.read_status(cache, n) for n in lengths) if r), 0)
+    for n in lengths if rc else ():
+        engine.clear_status(cache, n)
+    _lib.check(rc, "score_text")
     return TokenLogprobs(*(torch.cat([x.unflatten(0, (B, -1)) for x in xs], 1) for xs in zip(*parts)))
 
 

@@ -204,3 +204,21 @@ def test_status_of_an_8_bit_cache_is_seen_and_cleared():
         with pytest.raises(ValueError):
             wrong()
     assert len(eng._ws) == held
+
+
+def test_scoring_reports_what_the_device_reports():
+    from cirrus_s_1a_b200 import _lib
+    from cirrus_s_1a_b200.longtext import score_text
+
+    cfg, eng = model()
+    ids = text(cfg, 60)
+    cache = eng.new_cache(max_ctx=64, kv8="e4m3")
+    cache.slots_dev.fill_(30)  # more than the host knows of
+    with pytest.raises(_lib.CbError):
+        score_text(eng, ids, cache)
+    for at, bad in ((50, cfg.vocab_size), (50, -1), (59, cfg.vocab_size), (59, -1), (59, 2 ** 32 + 5)):
+        wrong = ids.clone()
+        wrong[0, at] = bad
+        with pytest.raises(_lib.CbError):
+            score_text(eng, wrong, eng.new_cache())
+    assert bool(torch.isfinite(score_text(eng, ids, eng.new_cache()).logprob).all())
