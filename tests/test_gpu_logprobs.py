@@ -166,3 +166,15 @@ def test_refusals():
             token_logprobs(x, t, top)
     empty = token_logprobs(x[:0], t[:0], 2)
     assert empty.logprob.shape == (0,) and empty.top_token.shape == (0, 2)
+
+
+def test_the_status_is_checked():
+    from cirrus_s_1a_b200.logprobs import token_logprobs
+
+    x = torch.randn(3, 100, device=DEV)
+    t = torch.tensor([1, 2, 3], dtype=torch.int32, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for bad in (status.cpu(), status.long(), status[:0], torch.zeros(2, dtype=torch.int32, device=DEV)):
+        with pytest.raises(ValueError):
+            token_logprobs(x, t, 2, bad)
+    token_logprobs(x, t, 2, status)
