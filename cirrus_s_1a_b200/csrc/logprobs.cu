@@ -471,7 +471,7 @@ using namespace cb;
 extern "C" int cb_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t V,
                                  const int32_t* tokens, int32_t top, float* logprob, float* entropy, int32_t* rank,
                                  float* top_logprob, int32_t* top_token, int32_t* status, void* stream) {
-  if (!logits || !tokens || !logprob || !entropy || !rank || rows <= 0 || V <= 0 || ld < V) return CB_ERR_ARG;
+  if (!logits || !tokens || !logprob || !entropy || !rank || rows <= 0 || V <= 0 || (ld < V && ld != 0)) return CB_ERR_ARG;
   if (dtype != CB_F32 && dtype != CB_BF16 && dtype != CB_F16) return CB_ERR_ARG;
   if (top < 0 || top > V || (top > 0 && (!top_logprob || !top_token))) return CB_ERR_ARG;
   if (top > CB_LOGPROB_MAX_TOP || V > CB_LOGPROB_MAX_VOCAB) return CB_ERR_SHAPE;

@@ -28,14 +28,17 @@ class TokenLogprobs(NamedTuple):
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
                    status: torch.Tensor | None = None) -> TokenLogprobs:
-    """``logits`` [rows, vocab] (float32, bfloat16 or float16, rows of any stride),
-    ``tokens`` int32 [rows] (negative: no token).  ``status`` (int32 [1] on the logits' device)
-    receives 6 when a token is outside the vocabulary.  Runs on the current stream."""
+    """``logits`` [rows, vocab] (float32, bfloat16 or float16; rows at least ``vocab`` apart,
+    or one row expanded), ``tokens`` int32 [rows] (negative: no token).  ``status`` (int32
+    [1] on the logits' device) receives 6 when a token is outside the vocabulary.  Runs on
+    the current stream."""
     if logits.dim() != 2 or not logits.is_cuda:
         raise ValueError("logits must be [rows, vocab] on a CUDA device")
     R, V = logits.shape
     if R and V > 1 and logits.stride(1) != 1:
         raise ValueError("a row of logits must be contiguous")
+    if R > 1 and logits.stride(0) < V and logits.stride(0) != 0:
+        raise ValueError(f"rows of logits must be at least {V} apart (or one row expanded)")
     if status is not None and (status.dtype != torch.int32 or status.shape != (1,) or status.device != logits.device):
         raise ValueError(f"status must be an int32 tensor [1] on {logits.device}")
     if tokens.dtype != torch.int32 or tokens.shape != (R,) or tokens.device != logits.device \

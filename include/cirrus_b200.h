@@ -486,7 +486,7 @@ int cb_forward_kv8(const CbModel* m, const CbCache* c, const CbKv8* kv8, int32_t
 
 /* ------------------------------------------------- log probabilities */
 /* For each of `rows` rows of logits [rows][ld] (CB_F32 / CB_BF16 / CB_F16, V of
- * them): logprob = log softmax(x)[tokens[r]], entropy = -sum p log p (natural
+ * them; ld 0: one row for all): logprob = log softmax(x)[tokens[r]], entropy = -sum p log p (natural
  * log), rank = how many logits are larger than the token's, and the `top` largest
  * in order (ties to the lowest token) as top_logprob / top_token [rows][top].
  * tokens[r] < 0: no token (logprob 0, rank -1); tokens[r] >= V: the same, and

@@ -178,3 +178,16 @@ def test_the_status_is_checked():
         with pytest.raises(ValueError):
             token_logprobs(x, t, 2, bad)
     token_logprobs(x, t, 2, status)
+
+
+def test_rows_expanded_from_one():
+    from cirrus_s_1a_b200.logprobs import token_logprobs
+
+    x = torch.randn(3, 100, device=DEV)
+    t = torch.tensor([1, 2, 3], dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError):
+        token_logprobs(x.flatten().as_strided((3, 100), (50, 1)), t)  # rows over one another
+    one = x[:1].expand(3, 100)  # one row for several tokens
+    a, b = token_logprobs(one, t, 4), token_logprobs(one.contiguous(), t, 4)
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
