@@ -41,8 +41,8 @@
 // float32, heads and tails of Q and of P as products of their own: 5 x 191 tokens at up
 // to 15.5K, 8 query heads of 128 dims 130 us, 4096 tokens behind 28600 as above 853 us
 // (twice the products; the warp-level form took 383 and 3287 us).
-// Every wait is bounded (%globaltimer); a wait that gives up sets CB_ERR_TIMEOUT
-// in the status word, and the CTA ends without writing results.
+// Every wait is bounded (%globaltimer); one that gives up sets CB_ERR_TIMEOUT in the
+// status word, and the rows that waited are not written.
 #include <climits>
 
 #include "kv8.cuh"
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           ev[h] = kv8_exponent(vs[h]);
         }
         if (j + 1 < n) scales(j + 1);
-        if (!wait(s_full + 8 * tile, j)) break;
+        wait(s_full + 8 * tile, j);  // (where it gives up no lane leaves the loop: what follows takes whole warps)
         fence_after();
         if (wide && min(ev[0], ev[kHalves - 1]) < e_ref - kNear) {
 #pragma unroll 1
@@ -627,7 +627,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             : "memory");
       }
       constexpr uint32_t kIdS = idesc(kRows, kKeys, false), kIdO = idesc(kRows, D, true);
-      auto all_wait = [&](uint32_t bar, int phase) { return __all_sync(0xffffffffu, wait(bar, phase)); };
       auto qk = [&](int t, int st) {
         const uint64_t qd = mat_desc(q_at + t * C::kQ, 16), kd = mat_desc(k_at + st * C::kKV, 16);
         if (lead) {
@@ -641,6 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           if (t + C::kIssuers >= tiles) commit(k_free + 8 * st);
         }
       };
+      auto all_wait = [&](uint32_t bar, int phase) { return __all_sync(0xffffffffu, wait(bar, phase)); };
       bool go = all_wait(q_full, 0) && all_wait(k_full, 0);
       if (go)
         for (int t = first; t < tiles; t += C::kIssuers) qk(t, 0);
@@ -666,11 +666,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           }
         }
       }
-      if (!go) {  // let the copy and the products in flight end before their memory goes
-        mbar_wait(q_full, 0);
-        if (lead) commit(end + 8 * first);
-        mbar_wait(end + 8 * first, 0);
-      }
+      // the copy and the products in flight end before their memory goes
+      if (!go) mbar_wait(q_full, 0);
+      if (lead) commit(end + 8 * first);
+      mbar_wait(end + 8 * first, 0);
     }
   }
   fence_before();
@@ -771,7 +770,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
     f32x2 sum[2] = {0, 0};
     for (int k = group; k < n; k += 2) {
       const int st = k % kMassStages;
-      if (!wait(s_full + 8 * st, k / kMassStages)) break;
+      wait(s_full + 8 * st, k / kMassStages);  // (no lane leaves the loop alone)
       fence_after();
       float s[kRows];
 #pragma unroll
@@ -848,11 +847,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
           commit(q_free + 8 * st);
         }
       }
-      if (!go) {
-        if (lead) commit(end);
-        mbar_wait(end, 0);
-        for (int k = max(0, n - kMassStages); k < n; ++k) mbar_wait(q_full + 8 * (k % kMassStages), k / kMassStages & 1);
-      }
+      // the products and copies in flight end before their memory goes
+      if (lead) commit(end);
+      mbar_wait(end, 0);
+      for (int k = max(0, n - kMassStages); k < n && !go; ++k) mbar_wait(q_full + 8 * (k % kMassStages), k / kMassStages & 1);
     }
   }
   fence_before();
