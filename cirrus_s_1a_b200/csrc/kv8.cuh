@@ -118,6 +118,16 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return y;
 }
 
+// The smaller of two; NaN if either is one.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// An attention weight, 2^x: at most 1, also where scores are too coarse to say so.
+__device__ __forceinline__ float weight(float x) { return exp2a(min_nan(x, 0.0f)); }
+
 // Pairs of floats on the packed float32 units.
 using f32x2 = unsigned long long;
 __device__ __forceinline__ f32x2 pack2(float a, float b) {

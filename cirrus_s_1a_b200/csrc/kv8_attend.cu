@@ -150,7 +150,7 @@ struct Query {
       top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const bool bad = !(top < INFINITY);
       int e = 0;  // top in [2^e, 2^(e+1)); rows of zeros keep e = 0
-      if (top > 0.0f && !bad) e = min(max((__float_as_int(top) >> 23) - 127, -100), 100);
+      if (top > 0.0f && !bad) e = max((__float_as_int(top) >> 23) - 127, -100);
       const float f = copysignf(kv8_pow2(8 - e), p.scale), undo = bad ? NAN : kv8_pow2(e - 8) * fabsf(p.scale) * kLog2e;
       back[nt][0] = __shfl_sync(0xffffffffu, undo, 8 * t4);
       back[nt][1] = __shfl_sync(0xffffffffu, undo, 8 * t4 + 4);
@@ -227,7 +227,11 @@ __device__ __forceinline__ void write_row(const AttendParams& p, int b, int hk, 
       u = make_uint2(h2_bits(__floats2half2_rn(y[0], y[1])), h2_bits(__floats2half2_rn(y[2], y[3])));
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at * p.c.head_dim + d) = u;
   }
-  if (d == 0) p.lse[at] = none ? -INFINITY : (s.m + log2f(s.l)) * kLn2;
+  if (d == 0) {
+    const float lse2 = none ? -INFINITY : s.m + log2f(s.l);
+    p.lse[at] = lse2 * kLn2;
+    if (p.add_mass) p.lse2[((int64_t)b * p.c.n_kv_heads + hk) * p.rows + r] = lse2;
+  }
 }
 
 // Visible blocks of sequence b for the query rows up to last_row (exclusive).
@@ -425,7 +429,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
     q.load(p, at.b, at.h, row0);
     float o[D / 16][NT][4] = {};
     float m[NT][2], l[NT][2];  // of rows 2 t4, 2 t4 + 1; l: this lane's keys
-    bool has_aside = false;
+    bool has_aside = false, far = false;
     int e_ref = kv8_exponent(vs);
     int lim[NT][2];
 #pragma unroll
@@ -527,6 +531,10 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[j][nt][i] *= alpha[i & 1];
         }
+        bool any_far = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) any_far = any_far || fabsf(m[nt][0]) > kFarScore || fabsf(m[nt][1]) > kFarScore;
+        far = __any_sync(0xffffffffu, any_far);
       }
       const bool low = ev < e_ref - kNear;
       if (low) {
@@ -535,11 +543,11 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
 #pragma unroll
           for (int i = 0; i < 2; ++i)
             if (now[nt][i] > -INFINITY) {
-              const float add = (float)ev - now[nt][i];
               float sum = 0.0f;
 #pragma unroll
               for (int mt = 0; mt < 4; ++mt)
-                sum += exp2a(fmaf(c[mt][nt][i], a[nt][i], add)) + exp2a(fmaf(c[mt][nt][i + 2], a[nt][i], add));
+                sum += exp2a(fmaf(c[mt][nt][i], a[nt][i], (float)ev) - now[nt][i]) +
+                       exp2a(fmaf(c[mt][nt][i + 2], a[nt][i], (float)ev) - now[nt][i]);
               s_aside[2 * nt + i][tid].add(now[nt][i], sum * kv8_pow2(-ev));
             }
       }
@@ -549,6 +557,21 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<D, HL, NT>) kv8_attend_
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) add[nt][i] = (float)ev - (m[nt][i] == -INFINITY ? 0.0f : m[nt][i]);
+      if (far) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (m[nt][i] > -INFINITY) {
+#pragma unroll
+              for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                for (int half = 0; half < 4; half += 2)
+                  c[mt][nt][i + half] = min_nan(fmaf(c[mt][nt][i + half], a[nt][i], (float)ev) - m[nt][i], kFarMost);
+              a[nt][i] = 1.0f;
+              add[nt][i] = 0.0f;
+            }
+      }
       const uint8_t* vb = arrive();
       bool any_nan = false;
       float pv[HL ? D / 16 : 1][HL ? NT : 1][4] = {};
@@ -802,7 +825,7 @@ __global__ void __launch_bounds__(256) kv8_scores_mass_kernel(const __grid_const
   if (key > last) return;
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int r = 0; r < p.rows; ++r) {
-    const float lse = p.lse[((int64_t)b * p.T + r / p.G) * (p.G * p.c.n_kv_heads) + hk * p.G + r % p.G] * kLog2e;
+    const float lse = p.lse2[head * p.rows + r];
     const int t = r / p.G;
     // past a row's last slot its scores were not all written
     if (key > p.pos[b] + t || t >= (p.counts ? min(p.counts[b], p.T) : p.T)) continue;
@@ -815,8 +838,8 @@ __global__ void __launch_bounds__(256) kv8_scores_mass_kernel(const __grid_const
       continue;
     }
     const float4 x = *reinterpret_cast<const float4*>(p.scores + (head * p.rows + r) * p.ld_scores + key);
-    sum.x += exp2a(x.x - lse), sum.y += exp2a(x.y - lse);
-    sum.z += exp2a(x.z - lse), sum.w += exp2a(x.w - lse);
+    sum.x += weight(x.x - lse), sum.y += weight(x.y - lse);
+    sum.z += weight(x.z - lse), sum.w += weight(x.w - lse);
   }
   float* to = p.c.mass + head * p.c.max_len + key;
   const float v[4] = {sum.x, sum.y, sum.z, sum.w};
@@ -853,7 +876,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mass_kernel(const __grid_cons
         lim[nt][i] = row_limit(p, r, pos, cnt);
         lse[nt][i] = 0.0f;
         if (lim[nt][i] >= 0)
-          lse[nt][i] = p.lse[((int64_t)b * p.T + r / p.G) * (p.G * p.c.n_kv_heads) + hk * p.G + r % p.G] * kLog2e;
+          lse[nt][i] = p.lse2[head * p.rows + r];
       }
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
@@ -864,7 +887,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mass_kernel(const __grid_cons
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (key0 + 16 * mt + 8 * (i >> 1) + key_row(g) <= lim[nt][i & 1])
-            sum[mt][i >> 1] += exp2a(fmaf(c[nt][i], q.back[nt][i & 1] * ks, -lse[nt][i & 1]));
+            sum[mt][i >> 1] += weight(__fmul_rn(c[nt][i], q.back[nt][i & 1] * ks) - lse[nt][i & 1]);
     }
   }
 #pragma unroll
@@ -928,7 +951,7 @@ struct Plan {
   int rows = 0, row_tiles = 0, splits = 0;
   int blocks = 0;  // of query rows, in a launch of the decode form
   int64_t part_rows = 0, ld_scores = 0;
-  size_t ml = 0, o = 0, q16 = 0, back = 0, scores = 0, bytes = 0;
+  size_t ml = 0, o = 0, q16 = 0, back = 0, lse2 = 0, scores = 0, bytes = 0;
 };
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -975,7 +998,8 @@ Plan plan_of(const CbKv8& c, int dtype, int n_q_heads, int T, int longest, bool 
   pl.o = pl.ml + align256((size_t)parts * sizeof(Sum));
   pl.q16 = pl.o + align256((size_t)parts * c.head_dim * sizeof(float));
   pl.back = pl.q16 + (size_t)bh * pl.row_tiles * 128 * c.head_dim * (dtype == CB_F32 ? 4 : 2);
-  pl.scores = pl.back + (size_t)bh * pl.row_tiles * 128 * sizeof(float);
+  pl.lse2 = pl.back + (size_t)bh * pl.row_tiles * 128 * sizeof(float);
+  pl.scores = pl.lse2 + (add_mass ? align256((size_t)bh * pl.rows * sizeof(float)) : 0);
   pl.bytes = pl.scores + (size_t)bh * pl.rows * pl.ld_scores * sizeof(float);
   return pl;
 }
@@ -1042,6 +1066,7 @@ extern "C" int cb_kv8_attend(const CbKv8* c, const void* q, int32_t dtype, const
   p.row_tiles = pl.row_tiles;
   p.q16 = base + pl.q16;
   p.q_back = reinterpret_cast<float*>(base + pl.back);
+  p.lse2 = reinterpret_cast<float*>(base + pl.lse2);
   p.status = status;
   const int bh = c->batch * c->n_kv_heads;
   cudaStream_t st = (cudaStream_t)stream;

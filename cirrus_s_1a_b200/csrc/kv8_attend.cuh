@@ -24,6 +24,7 @@ struct AttendParams {
   bool add_mass;
   void* out;            // [batch][T][heads][dim], the queries' type
   float* lse;           // [batch][T][heads]
+  float* lse2;          // [head][rows], log2 units: for the weights
   int block0;           // decode form: the launch's first block of query rows
   int splits;           // runs: of all heads' blocks (decode form), of each row tile's keys (prompt form)
   // parts: sums (Sum), and values against the same m'.  Decode form: [16 rows][run + head][16]
@@ -47,6 +48,12 @@ struct AttendParams {
 // (shared memory: it is rarely needed); blocks of smaller ones are summed there key by key, since their P may vanish
 // beside the others' although their keys weigh as much (zeros have the exponent -100).
 constexpr int kNear = 28;
+
+// From here on what the rounding of m' leaves of x + e - m' (up to half its last bit, 2^-4
+// here, the same for all keys) would pass f16's range: x + e is rounded before m' is taken
+// off, and P ends at 2^kFarMost where the score's last bit is larger than the lags of m'.
+// Scores beyond 2^24 are coarser than the value exponents.
+constexpr float kFarScore = 1048576.0f, kFarMost = 15.0f;
 
 // Many query rows, head_dim 64 or 128, 16-bit queries (kv8_prompt.cu).  Writes out
 // and lse where splits is 1, parts otherwise.

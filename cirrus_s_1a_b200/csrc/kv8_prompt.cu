@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(256) kv8_query_kernel(const __grid_constant__ 
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0.0f;
   int e = 0;
-  if (top > 0.0f && !bad) e = min(max((__float_as_int(top) >> 23) - 127, -100), 100);
+  if (top > 0.0f && !bad) e = max((__float_as_int(top) >> 23) - 127, -100);
   const float f = copysignf(kv8_pow2(8 - e), p.scale);
   uint8_t* tile = p.q16 + (head * p.row_tiles + r / kRows) * (int64_t)((1 + HL) * kRows * D * 2);
 #pragma unroll
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
               x = fmaf(x, by, (float)e);
               float sum = 0.0f;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) sum += exp2a(fmaf(__uint_as_float(u[i]), by, (float)e - x));
+              for (int i = 0; i < 16; ++i) sum += exp2a(fmaf(__uint_as_float(u[i]), by, (float)e) - x);
               aside.add(x, sum * kv8_pow2(-e));
             }
             __syncwarp();
@@ -452,7 +452,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           wait(o_full + 8 * tile, j - 1);
           fence_after();
         }
-        if (__any_sync(0xffffffffu, grow)) {
+        float at_m = m == -INFINITY ? 0.0f : m;
+        if (__any_sync(0xffffffffu, grow || fabsf(at_m) > kFarScore)) {
           const float ref = now - C::kLift, alpha = !grow ? 1.0f : m > -INFINITY ? exp2a(m - ref) : 0.0f;
           if (grow) m = ref;
           l *= alpha;
@@ -467,11 +468,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
               tmem_st16(to + c, u);
             }
           }
+          at_m = m == -INFINITY ? 0.0f : m;
+          if (fabsf(at_m) > kFarScore) {
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i)
+              s[i] = min_nan(fmaf(s[i], a[i / 64], (float)ev[i / 64]) - at_m, kFarMost) - (float)ev[i / 64];
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) a[h] = 1.0f;
+            at_m = 0.0f;
+          }
         }
         float sum_l = 0.0f;
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
-          const float add = (float)ev[h] - (m == -INFINITY ? 0.0f : m);
+          const float add = (float)ev[h] - at_m;
           const f32x2 a2 = pack2(a[h], a[h]), c2 = pack2(add, add);
           f32x2 sum[2] = {0, 0};  // pairs of zeros
 #pragma unroll
@@ -549,7 +559,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         if (p.splits > 1) {
           p.part_ml[at] = none ? Sum{-INFINITY, 0.0f} : Sum{fmaxf(m, -3e38f), l};
         } else {
-          p.lse[orow] = none ? -INFINITY : (m + log2f(l)) * kLn2;
+          const float lse2 = none ? -INFINITY : m + log2f(l);
+          p.lse[orow] = lse2 * kLn2;
+          if (p.add_mass) p.lse2[head * p.rows + r] = lse2;
         }
       }
     }
@@ -716,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
                  end = s_full + 8 * kMassStages;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t head = blockIdx.y;
-  const int b = (int)(head / p.c.n_kv_heads), hk = (int)(head % p.c.n_kv_heads);
+  const int b = (int)(head / p.c.n_kv_heads);
   const int key0 = blockIdx.x * kRows;
   const int pos = p.pos[b], cnt = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
   const int last = cnt > 0 ? min(pos + cnt, p.limit) - 1 : -1;
@@ -788,10 +800,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
 #pragma unroll
       for (int i = 0; i < kRows; i += 4) {
         const float4 by = *reinterpret_cast<const float4*>(f + i), sub = *reinterpret_cast<const float4*>(f + kRows + i);
-        const float2 x = unpack2(fma2(mul2(pack2(s[i], s[i + 1]), ks2), pack2(by.x, by.y), pack2(sub.x, sub.y)));
-        const float2 y = unpack2(fma2(mul2(pack2(s[i + 2], s[i + 3]), ks2), pack2(by.z, by.w), pack2(sub.z, sub.w)));
-        sum[0] = add2(sum[0], pack2(exp2a(x.x), exp2a(x.y)));
-        sum[1] = add2(sum[1], pack2(exp2a(y.x), exp2a(y.y)));
+        const float2 x = unpack2(add2(mul2(mul2(pack2(s[i], s[i + 1]), ks2), pack2(by.x, by.y)), pack2(sub.x, sub.y)));
+        const float2 y = unpack2(add2(mul2(mul2(pack2(s[i + 2], s[i + 3]), ks2), pack2(by.z, by.w)), pack2(sub.z, sub.w)));
+        sum[0] = add2(sum[0], pack2(weight(x.x), weight(x.y)));
+        sum[1] = add2(sum[1], pack2(weight(y.x), weight(y.y)));
       }
       mbar_arrive(q_free + 8 * st);
     }
@@ -815,9 +827,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_mass_kernel(const __gr
       // rows that see nothing (or NaN): a factor that leaves any score finite, and -infinity
       float by = 1.2e-38f, sub = -INFINITY;
       if (t < cnt && pos + t >= 0) {
-        const float lse = p.lse[((int64_t)b * p.T + t) * (p.G * p.c.n_kv_heads) + hk * p.G + r % p.G];
+        const float lse = p.lse2[head * p.rows + r];
         by = fmaxf(p.q_back[head * p.row_tiles * kRows + r], 1.2e-38f);
-        sub = lse == lse ? -lse * kLog2e : -INFINITY;
+        sub = lse == lse ? -lse : -INFINITY;
         if (lse != lse) atomicMax(&s_nan_t, t);
       }
       s_info[st * 2 * kRows + d] = by;

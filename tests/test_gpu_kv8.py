@@ -321,6 +321,42 @@ def test_peaked_and_extreme_scores(T):
     check_attend(cache, q, [190 - T], dtype="f32", scale=0.7, longest=190)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,T", [(64, 1), (64, 130), (128, 5), (128, 130), (16, 3)])
+def test_scores_of_any_size(D, T, dtype):
+    """Queries up to the end of the range.  A key thousands ahead of the others takes the row:
+    its value comes out to the type's rounding and the 2^-20 of probabilities and sums, and
+    it takes each row's weight (to the 2 d of ``check_attend``, d the error of such a score).
+    Where float32 scores are too coarse to say which key does, outputs stay within the
+    values seen and weights within the number of rows."""
+    cache = filled(1, 1, D, 320, "e4m3")
+    cache.k.view(torch.uint8)[0, 0, :, 0] = 0x38  # 1
+    cache.k.view(torch.uint8)[0, 0, 20, 0] = 0x7E  # 448
+    cache.k_scale.fill_(2.0 ** -6)
+    cache.mass.zero_()
+    for size in (1e3, 1e6, 1e8, 1e9, 1e12, 1e30, 1e34):
+        q = torch.zeros(1, T, 3, D)
+        q[..., 0] = size
+        q = q.to(TYPES[dtype])
+        out, lse = cache.attend(q.to(DEV), ints([180 - T]), scale=0.5, add_mass=True)
+        score = float(q[0, 0, 0, 0].double()) * 7 * 0.5
+        want = cache.v[0, 0, 20].float() * cache.v_scale[0, 0, 0]
+        assert ((out.float() - want).abs() <= want.abs() * (2.0 ** -8 if dtype == "bf16" else 2.0 ** -19)).all(), size
+        assert (lse.double() / score - 1).abs().max() < 2.0 ** -20
+        d = score * (D * 2.0 ** -22 + 2.0 ** -21)
+        assert 3 * T * (1 - 2 * d - 2.0 ** -19) <= float(cache.mass[0, 0, 20]) <= 3 * T * (1 + 2.0 ** -19)
+        assert not cache.mass[0, 0, :20].any() and not cache.mass[0, 0, 21:].any()
+        cache.mass.zero_()
+    g = torch.Generator().manual_seed(1)
+    top = (cache.v.float() * cache.v_scale.repeat_interleave(64, -1)[..., None]).abs().max()
+    for size in (1e6, 1e9, 1e20, 1e34):
+        q = (torch.randn(1, T, 3, D, generator=g) * size).to(TYPES[dtype]).to(DEV)
+        out, lse = cache.attend(q, ints([180 - T]), add_mass=True)
+        assert bool(torch.isfinite(lse).all()) and bool((out.abs() <= top * 1.01).all())
+        assert bool((cache.mass >= 0).all()) and bool((cache.mass <= 3 * T * 1.01).all())
+        cache.mass.zero_()
+
+
 def test_nan_in_a_visible_key_reaches_its_rows_only():
     cache = filled(1, 1, 64, 128, "e4m3")
     cache.k.view(torch.uint8)[0, 0, 70, 5] = 0x7F
