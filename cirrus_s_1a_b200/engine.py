@@ -265,6 +265,8 @@ class DeviceCache:
                  kv8: str | None = None, add_mass: bool = False):
         cfg, dev = model.cfg, model.device
         self.model, self.batch, self.max_ctx = model, batch, max_ctx
+        if add_mass and kv8 is None and _share is None:
+            raise ValueError("add_mass: only an 8-bit shared cache (kv8=...) keeps attention weights")
         # window + CB_PREFILL_CHUNK slots: a prompt chunk appends all its keys before its attention
         self.swa_slots = cfg.swa_window + max(CB_SWA_EXTRA, CB_PREFILL_CHUNK)
         H, dk, dv, KC = cfg.gdn_heads, cfg.gdn_head_dim_k, cfg.gdn_head_dim_v, cfg.gdn_conv_size

@@ -222,3 +222,9 @@ def test_scoring_reports_what_the_device_reports():
         with pytest.raises(_lib.CbError):
             score_text(eng, wrong, eng.new_cache())
     assert bool(torch.isfinite(score_text(eng, ids, eng.new_cache()).logprob).all())
+
+
+def test_weights_without_an_8_bit_cache_are_refused():
+    cfg, eng = model()
+    with pytest.raises(ValueError):
+        eng.new_cache(add_mass=True)
