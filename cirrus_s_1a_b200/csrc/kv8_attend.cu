@@ -48,11 +48,12 @@
 //
 // Bound by memory in principle (2 D bytes a key for all rows of its head), by issue
 // and the latency of its chains in fact.  Measured: 64 sequences x 1 token at 32K,
-// 128 dims, E4M3, with weights 215 us, 5.2 TB/s in the attention itself (30 % of
-// issue slots); 16 x 5 tokens at up to 128K, 64 dims, int8 152 to 164 us, 4 TB/s (56 % of
-// issue slots, 51 % of the integer pipe: int8 codes take 5 instructions for four,
+// 128 dims, E4M3, with weights 221 us, 5 TB/s in the attention itself (30 % of
+// issue slots); 16 x 5 tokens at up to 128K, 64 dims, int8 155 to 172 us, 4 TB/s (53 % of
+// issue slots, 49 % of the integer pipe: int8 codes take 5 instructions for four,
 // E4M3 two); one token at 32K 18 us, of which the blocks take 4, placing the CTA and
-// the query 4, and joining 48 parts the rest.
+// the query 4, and joining 48 parts the rest.  Prompts of 16 and 32 dims: 1000 tokens at 8K,
+// 16 dims (2 heads, bf16) 38 us, with weights 218; 32 dims (4 heads, float32) 66 and 152.
 #include <algorithm>
 #include <climits>
 

@@ -27,12 +27,13 @@ struct AttendParams {
   float* lse2;          // [head][rows], log2 units: for the weights
   int block0;           // decode form: the launch's first block of query rows
   int splits;           // runs: of all heads' blocks (decode form), of each row tile's keys (prompt form)
-  // parts: sums (Sum), and values against the same m'.  Decode form: [16 rows][run + head][16]
-  // rows, part_rows of them for each 16 query rows; prompt form: [head][rows][splits].
+  // parts: sums (Sum), and values against the same m'.  Decode form: [row block][run + head][row],
+  // part_rows of them for each block (the 8, 16 or 32 query rows of a CTA); prompt form:
+  // [head][rows][splits].
   int64_t part_rows;
   Sum* part_ml;         // [part]
   float* part_o;        // [part][dim]
-  int* arrived;         // [16 rows][head]: parts finished; zero between calls
+  int* arrived;         // [row block of a launch][head]: parts finished; zero between calls
   float* scores;        // [head][rows][ld_scores] in log2 units, or null
   int64_t ld_scores;
   // the prompt form: query rows prepared in 128-row operand tiles, and the factors that undo their scaling
@@ -55,7 +56,7 @@ constexpr int kNear = 28;
 // Scores beyond 2^24 are coarser than the value exponents.
 constexpr float kFarScore = 1048576.0f, kFarMost = 15.0f;
 
-// Many query rows, head_dim 64 or 128, 16-bit queries (kv8_prompt.cu).  Writes out
+// Many query rows, head_dim 64 or 128, queries of any type (kv8_prompt.cu).  Writes out
 // and lse where splits is 1, parts otherwise.
 int kv8_prompt_launch(const AttendParams& p, int bh, cudaStream_t st);
 // The rows' attention weights into mass, after lse is complete.

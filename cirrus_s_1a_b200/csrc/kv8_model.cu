@@ -12,7 +12,7 @@ __global__ void __launch_bounds__(256) kv8_heads_kernel(const __grid_constant__ 
   if (item >= p.rows * p.heads) return;
   const int r = item / p.heads, h = item % p.heads, b = r / p.T, t = r % p.T;
   const int position = p.pos[b] + p.offset + t;
-  const float* x = p.proj + ((int64_t)b * p.src_T + p.src_off + t) * p.ldp + h * p.hd;
+  const float* x = p.proj + ((int64_t)b * p.src_T + t) * p.ldp + h * p.hd;
   float ss = 0.0f;
   for (int j = lane; j < p.hd; j += 32) ss += x[j] * x[j];
   const float rn = rsqrtf(warp_sum(ss) / (float)p.hd + p.eps);

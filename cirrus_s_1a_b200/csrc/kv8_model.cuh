@@ -9,8 +9,8 @@
 namespace cb {
 
 struct Kv8HeadsParams {
-  const float* proj;      // row b * src_T + src_off + t, heads from column 0
-  int ldp, src_T, src_off;
+  const float* proj;      // row b * src_T + t, heads from column 0
+  int ldp, src_T;
   int rows, T;            // rows b * T + t
   int heads, hd, rot2;
   const int32_t* pos;     // position pos[b] + offset + t

@@ -32,14 +32,14 @@
 // clock take 1024 clocks, its products 512.
 // With several runs per row tile, kv8_join_kernel joins them (kv8_attend.cu).
 // Measured: 4096 tokens behind 28600, 12 query heads on 4 KV heads of 64 dims, E4M3:
-// 582 us = 663 TFLOP/s, the exponential unit 67 % busy, the tensor pipe 33 %.  Tried
+// 593 us = 650 TFLOP/s, the exponential unit 66 % busy, the tensor pipe 33 %.  Tried
 // and slower: a share of the exponentials as a polynomial on the FMA units (636 to
 // 757 us, at 639 then), three row tiles of 64 keys (703; with strict turns at the
 // exponentials 696, turns passed on at half 624), Q K^T and P V issued by two warps (641).
 // For 128 dims, 2 x 1000 tokens at up to 8K (171 us then): tiles of 128 keys with P in
 // the columns of its scores (180), a second P a tile (171).
 // float32, heads and tails of Q and of P as products of their own: 5 x 191 tokens at up
-// to 15.5K, 8 query heads of 128 dims 130 us, 4096 tokens behind 28600 as above 853 us
+// to 15.5K, 8 query heads of 128 dims 134 us, 4096 tokens behind 28600 as above 865 us
 // (twice the products; the warp-level form took 383 and 3287 us).
 // Every wait is bounded (%globaltimer); one that gives up sets CB_ERR_TIMEOUT in the
 // status word, and the rows that waited are not written.
@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 // tiles and their rows' factors stream through four stages, the scores through four
 // buffers of tensor memory, two warpgroups take them in turn.  Bound by the
 // exponentials and by whole CTAs to an SM: 2 x 1000 tokens at up to 8K, 8 query heads
-// of 128 dims: 69 us (206 key tiles on 148 SMs), the exponential unit 60 % busy.
+// of 128 dims: 70 us (206 key tiles on 148 SMs), the exponential unit 59 % busy.
 // (float32 queries of 128 dims, with their tails: two stages and two buffers.)
 template <int D, int HL>
 struct Mass {

@@ -23,8 +23,10 @@
 //
 // Bound by memory in principle (the row once), by issue in fact (77 % of the slots;
 // the pass widens, compares, scales, exponentiates and adds each value).  Measured: 16384 rows of 32000 in bf16,
-// 20 alternatives: 248 to 272 us = 4 TB/s; without alternatives 197 us = 5.3 TB/s; five
-// rows in float32: 17 us, the host's part of the call.
+// 20 alternatives: 250 to 273 us = 4 TB/s (nine tenths masked by -1e9: 312); without
+// alternatives 200 us = 5.2 TB/s; five rows in float32: 17 us, the host's part of the call.
+// Rows with more than kCand equal negative values at the threshold (a finite mask that
+// leaves less than `top` tokens) take the one search per alternative, 0.5 us a row.
 #include "common.cuh"
 #include "kv8.cuh"
 

@@ -444,9 +444,11 @@ int cb_kv8_append(const CbKv8* c, const void* k, const void* v, int32_t dtype, c
  * are rounded to f16 for the product with v; float32 queries and probabilities
  * are carried in about 22 bits.  longest: a bound on pos[b] + T that sizes the
  * launch; slots from it on are not seen.  scratch: cb_kv8_attend_scratch_bytes(c,
- * dtype, n_q_heads, T, longest, add_mass) bytes, 16-byte aligned (as is out), its first
- * CB_KV8_ZEROED bytes zeroed once before its first use (calls of any sizes may follow),
- * not shared by calls that overlap, kept as long as a graph that captured the call.  status
+ * dtype, n_q_heads, T, longest, add_mass) bytes (with the weights of few rows it holds
+ * their scores, 4 bytes for each row and slot below longest: at most a quarter of the
+ * cache's own size), 16-byte aligned (as is out), its first CB_KV8_ZEROED bytes zeroed once
+ * before its first use (calls of any sizes may follow), not shared by calls that overlap,
+ * kept as long as a graph that captured the call.  status
  * (device int32, may be null) receives CB_ERR_TIMEOUT if a bounded wait on the
  * tensor-core pipeline gives up.
  * Replaces the dense attention of CrossAttention.forward over the shared K/V
