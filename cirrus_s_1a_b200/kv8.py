@@ -35,6 +35,9 @@ _Strides = C.c_int64 * 3
 
 #: device index -> the current stream's pointer (what ``torch.cuda.current_stream`` wraps, without the object)
 raw_stream = torch._C._cuda_getCurrentRawStream if torch.cuda.is_available() else None
+#: whether the current stream is being captured (``torch.cuda.is_current_stream_capturing`` without its wrapper)
+capturing = torch._C._cuda_isCurrentStreamCapturing if torch.cuda.is_available() else None
+current_device = torch._C._cuda_getDevice if torch.cuda.is_available() else None
 
 
 def _dtype(t: torch.Tensor, name: str) -> int:
@@ -98,6 +101,7 @@ class Kv8Cache:
         self._lib = _lib.lib()
         self._scratch: dict = {}  # stream -> buffer; one serves every shape
         self._sizes: dict = {}  # shape -> bytes
+        self._hits: dict = {}  # (stream, *shape) -> the stream's buffer, once it is known to be long enough
         self.workspaces: dict = {}  # of the model's forward over this cache, by chunk length
 
     # ------------------------------------------------------------- helpers
@@ -148,7 +152,7 @@ class Kv8Cache:
         return raw_stream(self.device.index)
 
     def _call(self, fn, what: str, *args) -> None:
-        if torch.cuda.current_device() == self.device.index:
+        if current_device() == self.device.index:
             rc = fn(*args)
         else:
             with torch.cuda.device(self.device):
@@ -182,7 +186,7 @@ class Kv8Cache:
         a NaN key give NaN.  ``scale`` defaults to D ** -0.5;
         ``add_mass`` adds each slot's probabilities to ``mass``; ``longest`` bounds
         ``pos + T`` and sizes the launch (default ``max_len``) (``cb_kv8_attend``)."""
-        if torch.cuda.current_device() != self.device.index:
+        if current_device() != self.device.index:
             with torch.cuda.device(self.device):
                 return self.attend(q, pos, counts, scale=scale, add_mass=add_mass, longest=longest, out=out)
         T, heads, qs = self._rows(q, "q", None)
@@ -198,14 +202,20 @@ class Kv8Cache:
             raise ValueError("out must be contiguous, of q's shape, type and device")
         lse = torch.empty(self.batch, T, heads, dtype=torch.float32, device=self.device)
         st = self._stream()
-        scratch = self._scratch_of(dtype, heads, T, longest, add_mass, st)
-        self._call(self._lib.cb_kv8_attend, "cb_kv8_attend", self._ref, q.data_ptr(), dtype, qs, heads, T,
-                   self._ints(pos, "pos"), self._ints(counts, "counts"), longest,
-                   self.head_dim ** -0.5 if scale is None else float(scale), int(add_mass), out.data_ptr(),
-                   lse.data_ptr(), scratch.data_ptr(), scratch.numel(), self.status.data_ptr(), st)
+        key = (st, dtype, heads, T, longest, add_mass)
+        scratch = None if capturing() else self._hits.get(key)
+        if scratch is None:
+            scratch = self._scratch_of(*key)
+        rc = self._lib.cb_kv8_attend(self._ref, q.data_ptr(), dtype, qs, heads, T, self._ints(pos, "pos"),
+                                     self._ints(counts, "counts"), longest,
+                                     self.head_dim ** -0.5 if scale is None else float(scale), int(add_mass),
+                                     out.data_ptr(), lse.data_ptr(), scratch.data_ptr(), scratch.numel(),
+                                     self.status.data_ptr(), st)
+        if rc:
+            _lib.check(rc, "cb_kv8_attend")
         return out, lse
 
-    def _scratch_of(self, dtype: int, heads: int, T: int, longest: int, add_mass: bool, stream: int) -> torch.Tensor:
+    def _scratch_of(self, stream: int, dtype: int, heads: int, T: int, longest: int, add_mass: bool) -> torch.Tensor:
         key = (dtype, heads, T, longest, add_mass)
         nbytes = self._sizes.get(key)
         if nbytes is None:
@@ -214,8 +224,9 @@ class Kv8Cache:
                 raise _lib.CbError("cb_kv8_attend_scratch_bytes: shape not supported")
             if len(self._sizes) >= 256:  # a caller's ``longest`` may change with every token
                 self._sizes.clear()
+                self._hits.clear()
             self._sizes[key] = nbytes
-        if torch.cuda.is_current_stream_capturing():
+        if capturing():
             # from the graph's pool, and zeroed by each replay: the stream's buffer may be replaced by a
             # longer one, and what it holds is not zero before the graph's own first replay
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
@@ -224,6 +235,8 @@ class Kv8Cache:
         scratch = self._scratch.get(stream)
         if scratch is None or scratch.numel() < nbytes:
             scratch = self._scratch[stream] = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
+            self._hits.clear()
+        self._hits[(stream, *key)] = scratch
         return scratch
 
     def evict(self, pos: torch.Tensor, keep: int, recent: int) -> tuple:
