@@ -32,6 +32,8 @@ CB_KV8_ZEROED = 262144
 CB_KV8_E4M3, CB_KV8_INT8 = 0, 1
 CB_F32, CB_BF16, CB_F16 = 0, 1, 2
 CB_LOGPROB_MAX_TOP, CB_LOGPROB_MAX_VOCAB = 32, 1 << 20
+CB_ENDS_MAX_ROWS, CB_ENDS_MAX_VOCAB, CB_ENDS_MAX_DIM = 1 << 24, 1 << 20, 65536
+CB_REDUCE_NONE, CB_REDUCE_MEAN, CB_REDUCE_SUM = 0, 1, 2
 CB_GEMM_PRE_NONE, CB_GEMM_PRE_RMSNORM = 0, 1
 CB_GEMM_EPI_STORE, CB_GEMM_EPI_ADD, CB_GEMM_EPI_SWIGLU = 0, 1, 2
 
@@ -43,7 +45,9 @@ EXPORTS = ("cb_abi_version", "cb_status_string", "cb_nvfp4_quantize", "cb_nvfp4_
            "cb_spec_accept", "cb_mtp_workspace_bytes", "cb_mtp_draft", "cb_gemm_nvfp4", "cb_gemm_scratch_bytes",
            "cb_stream_plan_bytes", "cb_stream_plan", "cb_weight_stream_nvfp4", "cb_kv8_append",
            "cb_kv8_attend_scratch_bytes", "cb_kv8_attend", "cb_kv8_evict", "cb_forward_kv8_workspace_bytes",
-           "cb_forward_kv8", "cb_token_logprobs")
+           "cb_forward_kv8", "cb_token_logprobs", "cb_embedding", "cb_embedding_grad_scratch_bytes", "cb_embedding_grad",
+           "cb_rms_norm", "cb_rms_norm_grad_scratch_bytes", "cb_rms_norm_grad", "cb_linear_ce_scratch_bytes",
+           "cb_linear_ce", "cb_linear_ce_grad")
 
 P = C.c_void_p
 I32 = C.c_int32
@@ -171,13 +175,28 @@ def lib() -> C.CDLL:
         L.cb_forward_kv8.argtypes = [C.POINTER(CbModel), C.POINTER(CbCache), P, P, I32, P, C.c_size_t, P, I32, I32, P,
                                      P, P, P]
         L.cb_token_logprobs.argtypes = [P, I32, C.c_int64, I32, I32, P, I32, P, P, P, P, P, P, P]
+        I64, F32, N = C.c_int64, C.c_float, C.c_size_t
+        L.cb_embedding.argtypes = [P, I32, I64, I32, I32, P, I32, I64, F32, P, P, P]
+        L.cb_embedding_grad_scratch_bytes.argtypes = [I64, I32, I32]
+        L.cb_embedding_grad.argtypes = [P, I32, I64, P, I32, I64, I32, I32, F32, P, P, N, P]
+        L.cb_rms_norm.argtypes = [P, I32, I64, P, I32, I32, I32, F32, P, P]
+        L.cb_rms_norm_grad_scratch_bytes.argtypes = [I32, I32]
+        L.cb_rms_norm_grad.argtypes = [P, I32, I64, P, I64, P, I32, I32, I32, F32, P, P, P, N, P]
+        L.cb_linear_ce_scratch_bytes.argtypes = [I32] * 6
+        L.cb_linear_ce.argtypes = [P, I32, I64, P, I32, I64, I32, I32, I32, P, I32, I32, P, P, P, P, N, P, P]
+        L.cb_linear_ce_grad.argtypes = [P, I32, I64, P, I32, I64, I32, I32, I32, P, I32, I32, P, P, P, I64, P, I64, P, P,
+                                        P, N, P, P]
+        for fn in (L.cb_embedding_grad_scratch_bytes, L.cb_rms_norm_grad_scratch_bytes, L.cb_linear_ce_scratch_bytes):
+            fn.restype = N
         L.cb_read_trace.argtypes = [C.POINTER(CbModel), I32, I32, I32, P, P, I32, P]
         L.cb_launch_count.restype = C.c_int64
         L.cb_launch_count.argtypes = []
         for name in EXPORTS:
             if name not in ("cb_status_string", "cb_workspace_bytes", "cb_launch_count", "cb_nvfp4_slice_bytes",
                             "cb_mtp_workspace_bytes", "cb_gemm_scratch_bytes", "cb_stream_plan_bytes",
-                            "cb_kv8_attend_scratch_bytes", "cb_forward_kv8_workspace_bytes"):
+                            "cb_kv8_attend_scratch_bytes", "cb_forward_kv8_workspace_bytes",
+                            "cb_embedding_grad_scratch_bytes", "cb_rms_norm_grad_scratch_bytes",
+                            "cb_linear_ce_scratch_bytes"):
                 getattr(L, name).restype = C.c_int
         if L.cb_abi_version() != 3:
             raise CbError("libcirrus_b200.so ABI version mismatch")

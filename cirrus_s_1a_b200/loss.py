@@ -1,0 +1,107 @@
+"""Softmax cross entropy over the vocabulary from hidden rows, without keeping the
+logits, and its gradient (``cb_linear_ce``, ``cb_linear_ce_grad``).
+
+    r = linear_cross_entropy(hidden, weight, targets)      # hidden [N, d], weight [V, d]
+    r.loss.backward()                                      # hidden.grad, weight.grad
+
+Neither direction ever holds the [N, V] logits: the forward keeps each row's maximum and
+sum, the backward takes the logits again for a piece of the vocabulary at a time.
+
+The reference computes the same loss from its head's logits, in chunks
+(``cirrus/model/model.py:176-228``).
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from cirrus_s_1a_b200 import _lib, _rows
+
+REDUCTIONS = {"none": _lib.CB_REDUCE_NONE, "mean": _lib.CB_REDUCE_MEAN, "sum": _lib.CB_REDUCE_SUM}
+
+
+class CrossEntropy(NamedTuple):
+    loss: torch.Tensor  # float32: a scalar, or [N] with reduction "none" (0 where a row has no target)
+    lse: torch.Tensor   # float32 [N]: log of each row's softmax sum (natural log)
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, reduction: str = "mean",
+                         status: torch.Tensor | None = None) -> CrossEntropy:
+    """``logsumexp(x) - x[target]`` with ``x = hidden @ weight.T`` for ``hidden`` [N, d]
+    and ``weight`` [V, d]: one type for both (float32, bfloat16 or float16), or float32
+    against bfloat16.  ``targets`` int64 or int32 [N]; a negative one means the row has
+    none.  ``reduction`` "mean" is over the rows that have a target (0 where none has).
+    Both results are differentiable: ``r.loss + z * r.lse.square().mean()`` is a loss too.
+    ``status`` (int32 [1] on the device) receives 6 when a target is outside the
+    vocabulary, which then counts as none, and 8 when a bounded wait in a kernel gave up.
+    Runs on the current stream."""
+    _check(hidden, weight, targets, reduction, status)
+    if _rows.wants_grad(hidden, weight):
+        return CrossEntropy(*_LinearCE.apply(hidden, weight, targets, reduction, status))
+    return CrossEntropy(*_forward(hidden, weight, targets, reduction, status)[:2])
+
+
+def _check(hidden, weight, targets, reduction, status) -> tuple:
+    """The leading arguments of both entry points, and (N, V, d) with the type codes."""
+    N, D, ldh, h_code = _rows.matrix(hidden, "hidden")
+    V, Dw, ldw, w_code = _rows.vocabulary(weight, "weight", hidden.device)
+    if Dw != D:
+        raise ValueError(f"weight must have {D} columns as hidden, not {Dw}")
+    if hidden.dtype != weight.dtype and not (hidden.dtype == torch.float32 and weight.dtype == torch.bfloat16):
+        raise ValueError(f"hidden and weight must have one type, or float32 and bfloat16, not {hidden.dtype} and "
+                         f"{weight.dtype}")
+    if targets.shape != (N,):
+        raise ValueError(f"targets must be [{N}]")
+    wide = _rows.ids(targets, "targets", hidden.device)
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"unknown reduction {reduction!r}; choose from {sorted(REDUCTIONS)}")
+    _rows.status(status, hidden.device)
+    return (hidden.data_ptr(), h_code, ldh, weight.data_ptr(), w_code, ldw, N, V, D, targets.data_ptr(), wide,
+            REDUCTIONS[reduction]), (h_code, w_code, N, V, D)
+
+
+def _forward(hidden, weight, targets, reduction, status) -> tuple:
+    args, shape = _check(hidden, weight, targets, reduction, status)
+    dev, N = hidden.device, shape[2]
+    lse = torch.empty(N, dtype=torch.float32, device=dev)
+    if N == 0:
+        return torch.zeros(() if reduction != "none" else 0, device=dev), lse, None
+    loss = torch.empty(N if reduction == "none" else (), dtype=torch.float32, device=dev)
+    count = None if reduction == "none" else torch.empty(1, dtype=torch.int32, device=dev)
+    scratch = _rows.scratch(dev, "cb_linear_ce_scratch_bytes", *shape, 0)
+    _rows.call(dev, "cb_linear_ce", *args, loss.data_ptr(), lse.data_ptr(), _lib.ptr(count), scratch.data_ptr(),
+               scratch.numel(), _rows.status(status, dev))
+    return loss, lse, count
+
+
+class _LinearCE(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, reduction, status):
+        loss, lse, count = _forward(hidden, weight, targets, reduction, status)
+        ctx.save_for_backward(hidden, weight, targets, lse, count)
+        ctx.reduction, ctx.status = reduction, status
+        ctx.set_materialize_grads(False)
+        return loss, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_loss, g_lse):
+        hidden, weight, targets, lse, count = ctx.saved_tensors
+        want_h, want_w = ctx.needs_input_grad[:2]
+        if g_loss is None and g_lse is None:
+            return None, None, None, None, None
+        args, shape = _check(hidden, weight, targets, ctx.reduction, ctx.status)
+        dev, (_, _, N, V, D) = hidden.device, shape
+        dh = torch.empty(N, D, dtype=hidden.dtype, device=dev) if want_h else None
+        if N == 0:
+            return dh, torch.zeros(V, D, dtype=weight.dtype, device=dev) if want_w else None, None, None, None
+        dw = torch.empty(V, D, dtype=weight.dtype, device=dev) if want_w else None
+        scratch = _rows.scratch(dev, "cb_linear_ce_scratch_bytes", *shape, 1)
+        step = lambda g: g.stride(0) if g is not None and g.dim() else 0  # noqa: E731
+        _rows.call(dev, "cb_linear_ce_grad", *args, lse.data_ptr(), _lib.ptr(count), _lib.ptr(g_loss), step(g_loss),
+                   _lib.ptr(g_lse), step(g_lse), _lib.ptr(dh), _lib.ptr(dw), scratch.data_ptr(), scratch.numel(),
+                   _rows.status(ctx.status, dev))
+        return dh, dw, None, None, None

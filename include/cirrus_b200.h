@@ -502,6 +502,68 @@ int cb_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int32_t row
                       int32_t top, float* logprob, float* entropy, int32_t* rank, float* top_logprob,
                       int32_t* top_token, int32_t* status, void* stream);
 
+/* ------------------------------------------- the ends of a model, trained */
+/* The embedding lookup, the RMSNorm of rows and the cross entropy over the vocabulary,
+ * each with its gradient.  Matrices are CB_F32 / CB_BF16 / CB_F16 with contiguous rows,
+ * `ld` elements apart (0: one row for all, but not for a table or a vocabulary); outputs
+ * are contiguous.  Sums are float32 or wider and their order does not depend on timing:
+ * the same call gives the same bits.  Token ids and targets are int32, or int64 where
+ * `_64` is 1; a negative one means no token; one of V or more is taken as none, and *status (device
+ * int32, may be null) receives CB_ERR_TOKEN.  Scratch is 16-byte aligned, holds nothing
+ * between calls and is not shared by calls that overlap; it needs no initial value.
+ * At most CB_ENDS_MAX_ROWS rows or tokens, CB_ENDS_MAX_VOCAB vocabulary rows and
+ * CB_ENDS_MAX_DIM columns. */
+#define CB_ENDS_MAX_ROWS (1 << 24)
+#define CB_ENDS_MAX_VOCAB (1 << 20)
+#define CB_ENDS_MAX_DIM 65536
+enum { CB_REDUCE_NONE = 0, CB_REDUCE_MEAN = 1, CB_REDUCE_SUM = 2 };
+
+/* out [n][d] = scale * table[ids[i]], zeros where there is no token.  Replaces nn.Embedding
+ * (cirrus/model/model.py:124) for a dense table; cb_embed reads the NVFP4 one. */
+int cb_embedding(const void* table, int32_t dtype, int64_t ld, int32_t V, int32_t d, const void* ids, int32_t ids_64,
+                 int64_t n, float scale, void* out, int32_t* status, void* stream);
+
+/* dtable [V][d] = scale * the sum, over the tokens with id v in their order, of g [n][ldg];
+ * zeros for rows without a token. */
+size_t cb_embedding_grad_scratch_bytes(int64_t n, int32_t V, int32_t d);
+int cb_embedding_grad(const void* g, int32_t dtype, int64_t ldg, const void* ids, int32_t ids_64, int64_t n, int32_t V,
+                      int32_t d, float scale, void* dtable, void* scratch, size_t scratch_bytes, void* stream);
+
+/* y [rows][d] = x * rsqrt(mean(x^2) + eps) * w; w [d] float32 or x's type.  Replaces RMSNorm
+ * (cirrus/model/layers.py:33-44). */
+int cb_rms_norm(const void* x, int32_t dtype, int64_t ld, const void* w, int32_t w_dtype, int32_t rows, int32_t d,
+                float eps, void* y, void* stream);
+
+/* Its gradient for g [rows][ldg] (x's type): dx [rows][d] in x's type, dw [d] in w's. */
+size_t cb_rms_norm_grad_scratch_bytes(int32_t rows, int32_t d);
+int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const void* g, int64_t ldg, const void* w,
+                     int32_t w_dtype, int32_t rows, int32_t d, float eps, void* dx, void* dw, void* scratch,
+                     size_t scratch_bytes, void* stream);
+
+/* Cross entropy of the rows h [N][ldh] over the vocabulary rows w [V][ldw], without keeping
+ * the logits x = h w^T: lse [N] = log sum exp x (natural log), and per row lse - x[target],
+ * 0 where there is no target.  loss: that for each row [N] (CB_REDUCE_NONE), or its mean
+ * over the rows with a target (0 when none has one) or its sum, [1], with their number in
+ * count [1].  h and w have one type, or h is CB_F32 and w CB_BF16.  16-bit products are
+ * exact and float32 ones carried in about 24 bits, both summed in float32.
+ * Replaces lm_head + the loss of CirrusModel.forward (cirrus/model/model.py:176-228). */
+size_t cb_linear_ce_scratch_bytes(int32_t h_dtype, int32_t w_dtype, int32_t N, int32_t V, int32_t d, int32_t backward);
+int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype, int64_t ldw, int32_t N,
+                 int32_t V, int32_t d, const void* targets, int32_t targets_64, int32_t reduction, float* loss,
+                 float* lse, int32_t* count, void* scratch, size_t scratch_bytes, int32_t* status, void* stream);
+
+/* Its gradient: with G = (g_loss + g_lse) p - g_loss [v = target], p = exp(x - lse),
+ * dh [N][d] = G w in h's type and dw [V][d] = G^T h in w's (either may be null).  g_loss and
+ * g_lse (either null for zeros) are float32, of row n at n * step (step 0: one for all);
+ * for a reduced loss g_loss is [1].  lse and count are the forward's.  A row without a
+ * gradient (no target and g_lse 0) adds nothing, whatever it holds.  G is rounded to the
+ * 16-bit type before the products; for float32 it is carried in about 24 bits. */
+int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype, int64_t ldw,
+                      int32_t N, int32_t V, int32_t d, const void* targets, int32_t targets_64, int32_t reduction,
+                      const float* lse, const int32_t* count, const float* g_loss, int64_t g_loss_step,
+                      const float* g_lse, int64_t g_lse_step, void* dh, void* dw, void* scratch, size_t scratch_bytes,
+                      int32_t* status, void* stream);
+
 /* Copy the workspace's device status word into *status (synchronises on the stream). */
 int cb_read_status(const void* workspace, int32_t* status, void* stream);
 /* Clear the status word (stream-ordered). */
