@@ -182,7 +182,7 @@ def lib() -> C.CDLL:
         L.cb_rms_norm.argtypes = [P, I32, I64, P, I32, I32, I32, F32, P, P]
         L.cb_rms_norm_grad_scratch_bytes.argtypes = [I32, I32]
         L.cb_rms_norm_grad.argtypes = [P, I32, I64, P, I64, P, I32, I32, I32, F32, P, P, P, N, P]
-        L.cb_linear_ce_scratch_bytes.argtypes = [I32] * 6
+        L.cb_linear_ce_scratch_bytes.argtypes = [P, I32, I64, P, I32, I64, I32, I32, I32, P, I32]
         L.cb_linear_ce.argtypes = [P, I32, I64, P, I32, I64, I32, I32, I32, P, I32, I32, P, P, P, P, N, P, P]
         L.cb_linear_ce_grad.argtypes = [P, I32, I64, P, I32, I64, I32, I32, I32, P, I32, I32, P, P, P, I64, P, I64, P, P,
                                         P, N, P, P]

@@ -4,20 +4,637 @@
 //   G_nv = a_n p_nv - b_n [v = t(n)],  p = exp(x - lse),  a = dL/dloss + dL/dlse,  b = dL/dloss
 //   dh = G W        dW = G^T h
 //
-// Forward: each tile of logits leaves its rows' maximum and sum, which a second kernel
-// joins in the order of the vocabulary.  Backward: the logits are taken again for a piece
-// of the vocabulary at a time, and G of that piece goes into both products.
+// Bound by the matrix products: 2 N V d operations forward, 6 N V d backward (the logits
+// again, and two products), against N d + V d elements read.  All of them run in one
+// kernel on the 5th-generation tensor cores:
+//   * a pair of CTAs (cta_group::2) owns a 256 x 256 tile: each holds 128 of its rows, the
+//     accumulator in tensor memory (two of them, so that a tile's products run under the
+//     last tile's epilogue), and brings half of the columns' operand;
+//   * a thread of each CTA copies 64-wide steps of K by TMA into six stages, one of the pair
+//     issues tcgen05.mma, eight warps a CTA take the accumulators out of tensor memory;
+//   * operands lie as the caller has them: logits read h and W along K; dh reads W, and dW
+//     reads G and h, across it (MN-major operands), so that nothing is transposed.
+// Forward: a pair takes a run of tiles along the vocabulary and keeps its rows' maximum and
+// sum over them; a second kernel joins the runs in order.  Backward: G of a piece of the
+// vocabulary goes to memory in the operands' type, both products of the piece follow in one
+// launch; dh adds the pieces up in float32.
+// float32 operands are three bf16 parts each (8 + 8 + 8 bits, and float32's range), six
+// products of parts (what is left out is below 2^-24 of a product), three against bf16.
+// Every wait is bounded (%globaltimer); one that gives up sets CB_ERR_TIMEOUT.
+#include <cuda.h>
+
+#include <algorithm>
+#include <climits>
+
 #include "ends.cuh"
 
 namespace cb {
 namespace {
 
-constexpr int kTile = 64, kStep = 16, kThreads = 256;
-constexpr int kPiece = 2048;  // vocabulary rows whose G is held at a time
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTileM = 256, kTileN = 256;  // of a pair
+constexpr int kStep = 64;                  // of K: 128 bytes, a swizzled row
+constexpr int kStages = 6;
+constexpr int kHalfBytes = 128 * kStep * 2;  // one CTA's rows of one operand's step
+constexpr int kStageBytes = 2 * kHalfBytes;
+constexpr int kOutBytes = 128 * 128;  // a box on its way out: 128 rows of 128 bytes, one for each half of the columns
+constexpr int kSmem = kStages * kStageBytes + 2 * kOutBytes + 1024;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = kEpiWarps * 32 + 64;
+constexpr int kMaxPasses = 6;
+// Sums in tensor memory are cut off, not rounded, after every 16 products: over 48 of them a
+// row's lse was 5e-7 off, over 1500 the gradients 4e-5.  So a span of K is added up there,
+// and the spans in registers, rounded: 1024 of K, or 256 where float32 parts are multiplied.
+constexpr int kSpan16 = 16, kSpan32 = 4;
+constexpr uint64_t kWaitNs = 2000000000ull, kDrainNs = 10000000ull;
 
+enum { STATS = 0, GRAD = 1, PRODUCTS = 2 };
+enum { OUT_STORE = 0, OUT_ADD = 1 };
+
+// One matrix product D[m][n] = sum over passes and k of A[m][k] B[n][k].  An operand is a
+// 16-bit matrix read along K (its rows are m or n) or across it (its rows are k); pass i
+// adds a_part[i] / b_part[i] to the column it is read at, the place of a part of its values.
+struct alignas(64) Gemm {
+  CUtensorMap a, b, out;
+  int a_mn, b_mn;                  // read across K
+  int a_base, b_base;              // added to the row it is read at
+  int passes;
+  int a_part[kMaxPasses], b_part[kMaxPasses];
+  int m_tiles, n_tiles, k_steps;   // k_steps of a pass
+  int span;                        // steps of K that are added up in tensor memory
+  int splits;                      // of K, each with an output of its own
+  int out_f32, out_mode;
+  int out_rows;                    // between the splits' outputs
+  const float* scale;              // the output's, in memory (PRODUCTS; null: none), times scale_by
+  float scale_by;
+};
+
+struct alignas(64) Args {
+  Gemm g[2];
+  int n1, n2, extra, pairs;        // PRODUCTS: items of g[0] and of g[1] (see item_of)
+  uint32_t kind;                   // instruction descriptor without sizes and directions
+  int tile_n;                      // STATS, GRAD
+  // STATS and GRAD: rows, vocabulary rows, the vocabulary row that the tiles start at, and how many
+  int N, V, v0, vp;
+  Ids targets;
+  int slots;                       // STATS: parts of a row's sum
+  float2* part;                    // [slots][2][N]
+  float* xt;                       // [N]
+  uint32_t* counter;               // set to 0
+  const float4* rows;              // GRAD: (a, b, lse, -) of each row
+  const float* top;                // and their largest factor
+  int g_parts, g_cols;             // of G: columns of one part
+  int is_f16;
+  int32_t* status;
+};
+
+// ------------------------------------------------------------- primitives
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, "
+      "p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+__device__ __noinline__ bool slow_wait(uint32_t bar, uint32_t parity, uint64_t limit) {
+  const uint64_t end = now_ns() + limit;
+  while (!try_wait(bar, parity))
+    if (now_ns() > end) return false;
+  return true;
+}
+__device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, uint64_t limit) {
+  for (int i = 0; i < 64; ++i)
+    if (try_wait(bar, parity)) return true;
+  return slow_wait(bar, parity, limit);
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
+}
+// Whether any of the 128 threads of a half of the epilogue says so; a barrier of theirs.
+__device__ __forceinline__ bool any_of_half(int half, bool is) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"((uint32_t)is), "r"(half + 1)
+      : "memory");
+  return any != 0;
+}
+__device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void copy_in(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void copy_out(const CUtensorMap* map, int x, int y, uint32_t src, int mode) {
+  if (mode == OUT_ADD)
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map),
+                 "r"(src), "r"(x), "r"(y)
+                 : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src),
+                 "r"(x), "r"(y)
+                 : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// The pair's products issued so far arrive at this barrier of both CTAs.
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"((uint32_t)add)
+      : "memory");
+}
+// Operand of 128-byte swizzled rows (2 at bits 61-63, version 1 at bits 46-47), 8-row groups
+// 1024 bytes apart; read across K, its 64-element column blocks lie a step's rows apart.
+__device__ __forceinline__ uint64_t operand(uint32_t saddr) {
+  constexpr uint32_t kBlock = kStep * 128;
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(kBlock >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void load32(uint32_t addr, float* v) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void load16(uint32_t addr, float* v) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void loads_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two float32 operations in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two values in 16 bits, the first in the low half.
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// G is held in units of the largest |a| or |b| of the call, `top`: a mean's G is p - [v = t]
+// itself, whose largest entries lie below 1, where their rounding is smallest against them.
+// float16, whose range ends soon: G of row n is held times 2^(13 + e), e >= 0 the exponent
+// by which the row's |a| + |b| falls behind the largest it can be, so that it stays below
+// 2^15 and a probability of 2^-26 is a normal number; dh is scaled back by rows, for dW the
+// row of h is multiplied by 2^-e.
+constexpr int kF16Shift = 13;
+__device__ __forceinline__ bool has_gradient(float4 row) { return row.x != 0.0f || row.y != 0.0f; }
+__device__ __forceinline__ float scale_of(float top) { return top > 0.0f ? top : 1.0f; }
+// -e; 0 for rows whose factors are not finite.
+__device__ __forceinline__ int row_exponent(float4 row, float top) {
+  const float size = (fabsf(row.x) + fabsf(row.y)) / scale_of(top);
+  int e = 0;
+  if (size > 0.0f && size < INFINITY) frexpf(size, &e);
+  return min(max(e - 2, -100), 0);
+}
+
+// ------------------------------------------------------------------- work
+struct Item {
+  int gemm, m0, n0, first, steps, split;  // steps `first` .. of K; times the passes
+  int tile;                               // along n
+};
+
+// The i-th tile of a pair.  STATS and GRAD: a run of equal length of all tiles, rows after
+// rows of tiles.  PRODUCTS: items of g[0], the longer ones, are dealt in turn; the pairs that
+// get one less take `extra` items of g[1] in its place, and the rest are dealt in turn.
+template <int MODE>
+__device__ __forceinline__ bool item_of(const Args& p, int pair, int i, Item& it) {
+  if (MODE != PRODUCTS) {
+    const Gemm& g = p.g[0];
+    const int64_t all = (int64_t)g.m_tiles * g.n_tiles;
+    const int64_t u = all * pair / p.pairs + i;
+    if (u >= all * (pair + 1) / p.pairs) return false;
+    it.gemm = 0;
+    it.m0 = (int)(u / g.n_tiles) * kTileM;
+    it.tile = (int)(u % g.n_tiles);
+    it.n0 = it.tile * p.tile_n;
+    it.first = 0;
+    it.steps = g.k_steps;
+    it.split = 0;
+    return true;
+  }
+  const int odd = p.n1 % p.pairs;  // pairs with one item of g[0] more than the others
+  const int longs = (p.n1 - pair + p.pairs - 1) / p.pairs;
+  int idx;
+  if (i < longs) {
+    idx = pair + i * p.pairs;
+  } else {
+    i -= longs;
+    int mine = 0;
+    if (pair >= odd && p.extra > pair - odd) mine = (p.extra - (pair - odd) + p.pairs - odd - 1) / (p.pairs - odd);
+    if (i < mine) {
+      idx = p.n1 + (pair - odd) + i * (p.pairs - odd);
+    } else {
+      const int at = p.extra + (pair - odd + p.pairs) % p.pairs + (i - mine) * p.pairs;
+      if (at >= p.n2) return false;
+      idx = p.n1 + at;
+    }
+  }
+  it.gemm = idx >= p.n1;
+  const Gemm& g = p.g[it.gemm];
+  if (it.gemm) idx -= p.n1;
+  it.split = idx % g.splits;
+  idx /= g.splits;
+  it.tile = idx % g.n_tiles;
+  it.n0 = it.tile * kTileN;
+  it.m0 = idx / g.n_tiles * kTileM;
+  it.first = (int)((int64_t)g.k_steps * it.split / g.splits);
+  it.steps = (int)((int64_t)g.k_steps * (it.split + 1) / g.splits) - it.first;
+  return true;
+}
+
+// One 128-byte row of a box, word j of which is f(j): eight 16-byte pieces, piece c at c ^ (row % 8).
+template <typename F>
+__device__ __forceinline__ void put_row(uint32_t box, int row, F&& f) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const uint32_t u0 = f(4 * c), u1 = f(4 * c + 1), u2 = f(4 * c + 2), u3 = f(4 * c + 3);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + row * 128 + ((c ^ (row & 7)) << 4)), "r"(u0),
+                 "r"(u1), "r"(u2), "r"(u3)
+                 : "memory");
+  }
+}
+
+template <int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ Args p) {
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t bars[2 * kStages + 4];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1;
+  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
+  const uint32_t out_at = base + kStages * kStageBytes;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, done = empty + 8 * kStages, freed = done + 16;
+
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full + 8 * i));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(empty + 8 * i));
+    }
+    for (int i = 0; i < 2; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(done + 8 * i));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(freed + 8 * i), "n"(2 * kEpiWarps));
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_abort = 0;
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  if (MODE == STATS && blockIdx.x == 0 && tid == 32) *p.counter = 0;
+  fence_before();
+  __syncthreads();
+  cluster_sync();
+  fence_after();
+  const uint32_t tmem = s_tmem;
+  volatile int* abort_flag = &s_abort;
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (*abort_flag) return false;
+    if (bounded_wait(bar, parity, kWaitNs)) return true;
+    *abort_flag = 1;
+    return false;
+  };
+
+  if (warp == kEpiWarps) {
+    // ---------------------------------------------------------- copies in
+    if (elect_one()) {
+      int n = 0;  // steps so far
+      Item it;
+      bool go = true;
+      for (int i = 0; go && item_of<MODE>(p, pair, i, it); ++i) {
+        const Gemm& g = p.g[MODE == PRODUCTS ? it.gemm : 0];
+        const int n_rows = MODE == PRODUCTS ? kTileN / 2 : p.tile_n / 2;
+        const int m = it.m0 + rank * 128, c = it.n0 + rank * n_rows;
+        const uint32_t bytes = 2 * (kHalfBytes + n_rows * 128);
+        // a span of K at a time, all passes over it
+        for (int from = 0; go && from < it.steps; from += g.span)
+          for (int pass = 0; go && pass < g.passes; ++pass) {
+            const int ap = g.a_part[pass], bp = g.b_part[pass], end = min(from + g.span, it.steps);
+            for (int k = from; k < end; ++k, ++n) {
+              const int st = n % kStages, k0 = (it.first + k) * kStep;
+              if (n >= kStages && !wait(empty + 8 * st, (n / kStages - 1) & 1)) {
+                go = false;
+                break;
+              }
+              const uint32_t bar = in_leader(full + 8 * st), at = base + st * kStageBytes, bt = at + kHalfBytes;
+              if (rank == 0)
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full + 8 * st), "r"(bytes)
+                             : "memory");
+              if (MODE == PRODUCTS && g.a_mn) {
+                copy_in(at, &g.a, m + ap, g.a_base + k0, bar);
+                copy_in(at + kHalfBytes / 2, &g.a, m + 64 + ap, g.a_base + k0, bar);
+              } else {
+                copy_in(at, &g.a, k0 + ap, g.a_base + m, bar);
+              }
+              if (MODE == PRODUCTS) {  // both products read their second operand across K
+                copy_in(bt, &g.b, c + bp, g.b_base + k0, bar);
+                copy_in(bt + kHalfBytes / 2, &g.b, c + 64 + bp, g.b_base + k0, bar);
+              } else {
+                copy_in(bt, &g.b, k0 + bp, g.b_base + c, bar);
+              }
+            }
+          }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kEpiWarps + 1) {
+    // ----------------------------------------------------------- products
+    if (rank == 0) {
+      const bool lead = elect_one();
+      int n = 0, sums = 0;
+      Item it;
+      bool go = true;
+      for (int i = 0; go && item_of<MODE>(p, pair, i, it); ++i) {
+        const Gemm& g = p.g[MODE == PRODUCTS ? it.gemm : 0];
+        const bool a_mn = MODE == PRODUCTS && g.a_mn;
+        const uint32_t id = p.kind | (a_mn ? 1u << 15 : 0u) | (MODE == PRODUCTS ? 1u << 16 : 0u) |
+                            (uint32_t)((MODE == PRODUCTS ? kTileN : p.tile_n) >> 3) << 17 | (uint32_t)(kTileM >> 4) << 24;
+        // 16 of K: 32 bytes of a row, or 16 rows
+        const uint32_t a_step = a_mn ? 2048 / 16 : 2, b_step = MODE == PRODUCTS ? 2048 / 16 : 2;
+        for (int from = 0; go && from < it.steps; from += g.span, ++sums) {
+          const int acc = sums & 1, steps = min(g.span, it.steps - from) * g.passes;
+          if (sums >= 2) go = __all_sync(0xffffffffu, wait(freed + 8 * acc, (sums / 2 - 1) & 1));
+          fence_after();
+          const uint32_t d = tmem + acc * kTileN;
+          for (int k = 0; k < steps && go; ++k, ++n) {
+            const int st = n % kStages;
+            go = __all_sync(0xffffffffu, wait(full + 8 * st, (n / kStages) & 1));
+            if (!go) break;
+            fence_after();
+            if (lead) {
+              const uint64_t a = operand(base + st * kStageBytes), b = operand(base + st * kStageBytes + kHalfBytes);
+#pragma unroll
+              for (int s = 0; s < kStep / 16; ++s) mma(d, a + s * a_step, b + s * b_step, id, k > 0 || s > 0);
+              commit(empty + 8 * st);
+            }
+            __syncwarp();
+          }
+          if (go && lead) commit(done + 8 * acc);
+          __syncwarp();
+        }
+      }
+      if (!go) {  // what is in flight ends before the memory goes
+        for (int k = 0; k < kStages; ++k) {
+          const int last = n - 1 - k;
+          if (last >= 0) bounded_wait(empty + 8 * (last % kStages), (last / kStages) & 1, kDrainNs);
+        }
+        for (int k = 0; k < kStages; ++k) bounded_wait(full + 8 * ((n + k) % kStages), ((n + k) / kStages) & 1, kDrainNs);
+      }
+    }
+  } else {
+    // ----------------------------------------------------------- epilogue
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t box = out_at + half * kOutBytes;
+    const bool lead = (warp & 3) == 0 && lane == 0;  // issues the half's copies out
+    const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
+    auto half_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(half + 1) : "memory"); };
+    // the rows' 128 bytes go out as one box
+    auto send = [&](const CUtensorMap* map, int x, int y, int mode, auto&& word) {
+      if (lead) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      half_sync();
+      put_row(box, row, word);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      half_sync();
+      if (lead) copy_out(map, x, y, box, mode);
+    };
+    float m = -INFINITY, l = 0.0f;  // STATS: of the row over the run
+    int run = -1, slot = 0;
+    int64_t target = -1;
+    float4 f = make_float4(0, 0, 0, 0);
+    auto leave = [&] {  // STATS: the run's part of the row's sum
+      if (run >= 0 && run + rank * 128 + row < p.N)
+        p.part[((int64_t)slot * 2 + half) * p.N + run + rank * 128 + row] = make_float2(m, l);
+    };
+    Item it;
+    int sums = 0;
+    for (int i = 0; item_of<MODE>(p, pair, i, it); ++i) {
+      const int n = it.m0 + rank * 128 + row;
+      const bool live = MODE != PRODUCTS && n < p.N;
+      if (MODE != PRODUCTS && it.m0 != run) {
+        if (MODE == STATS) leave();
+        run = it.m0;
+        m = -INFINITY;
+        l = 0.0f;
+        target = live ? p.targets[n] : -1;
+        if (target >= p.V) target = -1;
+        if (MODE == GRAD) {
+          f = live ? p.rows[n] : make_float4(0, 0, 0, 0);
+          const float by = p.is_f16 ? ldexpf(1.0f, kF16Shift - row_exponent(f, *p.top)) : 1.0f;
+          f.x = f.x / scale_of(*p.top) * by;
+          f.y = f.y / scale_of(*p.top) * by;
+        }
+        if (MODE == STATS) {
+          // which of the runs over these rows this one is
+          const int64_t all = (int64_t)p.g[0].m_tiles * p.g[0].n_tiles, from = (int64_t)(it.m0 / kTileM) * p.g[0].n_tiles;
+          slot = pair - (int)(((from + 1) * p.pairs - 1) / all);
+        }
+      }
+      float x[128];
+      const int cols = MODE == PRODUCTS ? 128 : min(128, p.tile_n - half * 128);
+      const int span = p.g[MODE == PRODUCTS ? it.gemm : 0].span;
+      bool go = true;
+      for (int from = 0; from < it.steps; from += span, ++sums) {
+        const int acc = sums & 1;
+        // the half's four waits agree, or its barriers would not
+        go = !any_of_half(half, !wait(done + 8 * acc, (sums / 2) & 1));
+        if (!go) break;
+        fence_after();
+        const uint32_t at = tmem + lane_at + acc * kTileN + half * 128;
+        if (from == 0) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c * 32 < cols) load32(at + c * 32, x + c * 32);
+          loads_done();
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            if (c * 16 < cols) {
+              float y[16];
+              load16(at + c * 16, y);
+              loads_done();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) x[c * 16 + j] += y[j];
+            }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_leader(freed + 8 * acc))
+                       : "memory");
+      }
+      if (!go) break;
+      const int v = it.n0 + half * 128;  // of the piece, or of d
+      const int at = (int)(target - p.v0 - v);  // the target's column
+      const bool hit = MODE != PRODUCTS && target >= 0 && at >= 0 && at < cols;
+      if constexpr (MODE == PRODUCTS) {
+        const Gemm& g = p.g[it.gemm];
+        const int y = it.m0 + rank * 128 + it.split * g.out_rows;
+        if (g.scale) {
+          const float s = scale_of(*g.scale) * g.scale_by;
+#pragma unroll
+          for (int c = 0; c < 128; ++c) x[c] *= s;
+        }
+        if (g.out_f32) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            send(&g.out, v + c * 32, y, g.out_mode, [&](int j) { return __float_as_uint(x[c * 32 + j]); });
+        } else {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            send(&g.out, v + c * 64, y, OUT_STORE, [&](int j) {
+              const float lo = x[c * 64 + 2 * j], hi = x[c * 64 + 2 * j + 1];
+              return p.is_f16 ? pack_f16(lo, hi) : pack_bf16(lo, hi);
+            });
+        }
+      }
+      if constexpr (MODE == STATS) {
+        if (v + cols > p.vp)  // the last tile
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (v + c >= p.vp) x[c] = -INFINITY;
+        if (__any_sync(0xffffffffu, hit)) {
+          float t = 0.0f;
+#pragma unroll
+          for (int c = 0; c < 128; ++c) t = c == at ? x[c] : t;
+          if (hit) p.xt[n] = t;
+        }
+        float top[4] = {m, m, m, m};
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (g * 32 < cols)
+#pragma unroll
+            for (int c = g * 32; c < g * 32 + 32; c += 2) top[c / 2 & 3] = max3(top[c / 2 & 3], x[c], x[c + 1]);
+        const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const float ref = t == -INFINITY ? 0.0f : t;
+        const float2 off = make_float2(-ref, -ref), scale = make_float2(kLog2e, kLog2e);
+        float2 s[4] = {};
+        s[0].x = l * exp2_of((m - ref) * kLog2e);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (g * 32 < cols)
+#pragma unroll
+            for (int c = g * 32; c < g * 32 + 32; c += 2) {
+              const float2 e = mul2(add2(make_float2(x[c], x[c + 1]), off), scale);
+              s[c / 2 & 3] = add2(s[c / 2 & 3], make_float2(exp2_of(e.x), exp2_of(e.y)));
+            }
+        const float2 both = add2(add2(s[0], s[1]), add2(s[2], s[3]));
+        l = both.x + both.y;
+        m = t;
+      }
+      if constexpr (MODE == GRAD) {
+        const float2 off = make_float2(-f.z, -f.z), scale = make_float2(kLog2e, kLog2e), by = make_float2(f.x, f.x);
+#pragma unroll
+        for (int c = 0; c < 128; c += 2) {
+          const float2 e = mul2(add2(make_float2(x[c], x[c + 1]), off), scale);
+          const float2 g = mul2(make_float2(exp2_of(e.x), exp2_of(e.y)), by);
+          x[c] = g.x;
+          x[c + 1] = g.y;
+        }
+        if (__any_sync(0xffffffffu, hit)) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c) x[c] = hit && c == at ? x[c] - f.y : x[c];
+        }
+        if (v + cols > p.vp)
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (v + c >= p.vp) x[c] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (v + c * 64 >= p.g_cols) continue;
+          for (int part = 0; part < p.g_parts; ++part)
+            send(&p.g[0].out, part * p.g_cols + v + c * 64, it.m0 + rank * 128, OUT_STORE, [&](int j) {
+              float &lo = x[c * 64 + 2 * j], &hi = x[c * 64 + 2 * j + 1];
+              if (p.is_f16) return pack_f16(lo, hi);
+              const uint32_t u = pack_bf16(lo, hi);
+              lo -= __uint_as_float(u << 16);  // what is left for the next part
+              hi -= __uint_as_float(u & 0xFFFF0000u);
+              return u;
+            });
+        }
+      }
+    }
+    if (MODE == STATS) leave();
+    if (lead) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while the pair's products or arrivals may reach it
+  fence_after();
+  if (tid == 0 && s_abort) set_status(p.status, CB_ERR_TIMEOUT);
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// --------------------------------------------------------- before and after
 struct Problem {
-  const void *h, *w;
-  int64_t ldh, ldw;
   int N, V, d;
   Ids targets;
 };
@@ -27,98 +644,66 @@ __device__ __forceinline__ int64_t target_of(const Problem& p, int n) {
   return t >= 0 && t < p.V ? t : -1;
 }
 
-// acc[i][j] = sum_k A[r0 + ty * 4 + i][k] * B[c0 + tx * 4 + j][k], with A and B given as functions of (row, k).
-template <typename FA, typename FB>
-__device__ __forceinline__ void tile_product(float (&acc)[4][4], int K, FA&& a, FB&& b) {
-  __shared__ float As[kStep][kTile + 1], Bs[kStep][kTile + 1];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  for (int k0 = 0; k0 < K; k0 += kStep) {
-    __syncthreads();
-    for (int e = tid; e < kTile * kStep; e += kThreads) {
-      const int k = e % kStep, r = e / kStep;
-      As[k][r] = k0 + k < K ? a(r, k0 + k) : 0.0f;
-      Bs[k][r] = k0 + k < K ? b(r, k0 + k) : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kStep; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(As[k][ty * 4 + i], Bs[k][tx * 4 + j], acc[i][j]);
-  }
-}
+constexpr int kRowThreads = 256;
 
-// part[tile][n] = (maximum, sum of exponentials against it) of the row's logits in the tile; xt[n] the target's logit.
-template <typename TH, typename TW>
-__global__ void __launch_bounds__(kThreads) stats_kernel(Problem p, float2* part, float* xt) {
-  const int n0 = blockIdx.x * kTile, v0 = blockIdx.y * kTile;
-  float x[4][4] = {};
-  tile_product(
-      x, p.d,
-      [&](int r, int k) { return n0 + r < p.N ? Elem<TH>::get(static_cast<const TH*>(p.h)[(n0 + r) * p.ldh + k]) : 0.0f; },
-      [&](int r, int k) { return v0 + r < p.V ? Elem<TW>::get(static_cast<const TW*>(p.w)[(v0 + r) * p.ldw + k]) : 0.0f; });
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int n = n0 + ty * 4 + i;
-    const int64_t t = n < p.N ? target_of(p, n) : -1;
+// Joins the runs' parts of a row's sum, a warp to a row; the last CTA adds the losses up.
+__global__ void __launch_bounds__(kRowThreads) join_kernel(Problem p, int n_tiles, int m_tiles, int pairs, const float2* part,
+                                                           const float* xt, float* rows, float* lse, int reduction,
+                                                           float* loss, int32_t* count, uint32_t* counter,
+                                                           int32_t* status) {
+  const int lane = threadIdx.x & 31, n = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+  if (n < p.N) {
+    const int64_t all = (int64_t)m_tiles * n_tiles, from = (int64_t)(n / kTileM) * n_tiles;
+    const int parts = 2 * ((int)(((from + n_tiles) * pairs - 1) / all) - (int)(((from + 1) * pairs - 1) / all) + 1);
     float m = -INFINITY, l = 0.0f;
-    bool nan = false;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (v0 + tx * 4 + j < p.V) {
-        m = fmaxf(m, x[i][j]);
-        nan |= x[i][j] != x[i][j];
-        if (v0 + tx * 4 + j == t) xt[n] = x[i][j];
-      }
-    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (v0 + tx * 4 + j < p.V && m > -INFINITY) l += expf(x[i][j] - m);
-    if (nan) l = NAN;
-    for (int o = 8; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (tx == 0 && n < p.N) part[(int64_t)blockIdx.y * p.N + n] = make_float2(m, l);
+    for (int i = lane; i < parts; i += 32) {
+      const float2 q = part[(int64_t)i * p.N + n];
+      const float t = fmaxf(m, q.x), ref = t == -INFINITY ? 0.0f : t;
+      l = l * expf(m - ref) + q.y * expf(q.x - ref);
+      m = t;
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+      const float qm = __shfl_xor_sync(0xffffffffu, m, o), ql = __shfl_xor_sync(0xffffffffu, l, o);
+      const float t = fmaxf(m, qm), ref = t == -INFINITY ? 0.0f : t;
+      l = l * expf(m - ref) + ql * expf(qm - ref);
+      m = t;
+    }
+    if (lane == 0) {
+      lse[n] = m + logf(l);
+      rows[n] = target_of(p, n) >= 0 ? (m - xt[n]) + logf(l) : 0.0f;
+      if (p.targets[n] >= p.V) set_status(status, CB_ERR_TOKEN);
+    }
   }
-}
-
-__global__ void __launch_bounds__(kThreads) join_kernel(Problem p, const float2* part, int tiles, const float* xt,
-                                                        float* loss, float* lse, int32_t* status) {
-  const int n = blockIdx.x * kThreads + threadIdx.x;
-  if (n >= p.N) return;
-  float m = -INFINITY, l = 0.0f;
-  for (int i = 0; i < tiles; ++i) m = fmaxf(m, part[(int64_t)i * p.N + n].x);
-  for (int i = 0; i < tiles; ++i) {
-    const float2 q = part[(int64_t)i * p.N + n];
-    l += q.y == 0.0f ? 0.0f : q.y * expf(q.x - m);
+  if (reduction == CB_REDUCE_NONE) return;
+  __shared__ int s_last;
+  __shared__ double s_sum[kRowThreads];
+  __shared__ int s_count[kRowThreads];
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    s_last = atomicAdd(counter, 1u) == gridDim.x - 1;
   }
-  lse[n] = m + logf(l);
-  const int64_t t = target_of(p, n);
-  loss[n] = t >= 0 ? (m - xt[n]) + logf(l) : 0.0f;
-  if (p.targets[n] >= p.V) set_status(status, CB_ERR_TOKEN);
-}
-
-__global__ void __launch_bounds__(1024) reduce_kernel(Problem p, const float* loss, int mean, float* out, int32_t* count) {
-  __shared__ double sums[1024];
-  __shared__ int counts[1024];
-  double s = 0.0;
-  int c = 0;
-  for (int n = threadIdx.x; n < p.N; n += 1024) {
-    c += target_of(p, n) >= 0;
-    s += loss[n];
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  double sum = 0.0;
+  int has = 0;
+  for (int i = threadIdx.x; i < p.N; i += kRowThreads) {
+    sum += __ldcg(rows + i);
+    has += target_of(p, i) >= 0;
   }
-  sums[threadIdx.x] = s;
-  counts[threadIdx.x] = c;
-  for (int o = 512; o > 0; o >>= 1) {
+  s_sum[threadIdx.x] = sum;
+  s_count[threadIdx.x] = has;
+  for (int o = kRowThreads / 2; o > 0; o >>= 1) {
     __syncthreads();
     if (threadIdx.x < o) {
-      sums[threadIdx.x] += sums[threadIdx.x + o];
-      counts[threadIdx.x] += counts[threadIdx.x + o];
+      s_sum[threadIdx.x] += s_sum[threadIdx.x + o];
+      s_count[threadIdx.x] += s_count[threadIdx.x + o];
     }
   }
   if (threadIdx.x == 0) {
-    *out = (float)(mean ? sums[0] / max(counts[0], 1) : sums[0]);
-    *count = counts[0];
+    *loss = (float)(reduction == CB_REDUCE_MEAN ? s_sum[0] / max(s_count[0], 1) : s_sum[0]);
+    *count = s_count[0];
   }
 }
 
@@ -129,92 +714,102 @@ struct Upstream {
   int reduction;
 };
 
-__global__ void __launch_bounds__(kThreads) factors_kernel(Problem p, Upstream u, float2* ab) {
-  const int n = blockIdx.x * kThreads + threadIdx.x;
-  if (n >= p.N) return;
-  float b = 0.0f;
-  if (u.loss && target_of(p, n) >= 0) {
-    b = u.loss[u.reduction == CB_REDUCE_NONE ? n * u.loss_step : 0];
-    if (u.reduction == CB_REDUCE_MEAN) b /= (float)max(*u.count, 1);
+// rows[n] = (a, b, lse, -) as they come from above, and *top = the largest |a| or |b|.
+// (*top starts at 0; a maximum does not depend on the order it is taken in.)
+__global__ void __launch_bounds__(kRowThreads) factors_kernel(Problem p, Upstream u, const float* lse, float4* rows, float* top) {
+  const int n = blockIdx.x * kRowThreads + threadIdx.x;
+  float size = 0.0f;
+  if (n < p.N) {
+    float b = 0.0f;
+    if (u.loss && target_of(p, n) >= 0) {
+      b = u.loss[u.reduction == CB_REDUCE_NONE ? n * u.loss_step : 0];
+      if (u.reduction == CB_REDUCE_MEAN) b /= (float)max(*u.count, 1);
+    }
+    const float a = b + (u.lse ? u.lse[n * u.lse_step] : 0.0f);
+    // (a row without a gradient is read as zeros, and its G is 0 whatever its own lse is)
+    rows[n] = make_float4(a, b, a == 0.0f && b == 0.0f ? 0.0f : lse[n], 0.0f);
+    size = fmaxf(fabsf(a), fabsf(b));
+    if (!(size < INFINITY)) size = 0.0f;
   }
-  ab[n] = make_float2(b + (u.lse ? u.lse[n * u.lse_step] : 0.0f), b);
+  size = warp_max(size);
+  if ((threadIdx.x & 31) == 0 && size > 0.0f) atomicMax(reinterpret_cast<int*>(top), __float_as_int(size));
 }
 
-__device__ __forceinline__ bool dead(float2 ab) { return ab.x == 0.0f && ab.y == 0.0f; }
-
-// G[n][v - v0] of the vocabulary rows v0 .. v0 + vp; a row without a gradient is 0 whatever it holds.
-template <typename TH, typename TW>
-__global__ void __launch_bounds__(kThreads) grad_kernel(Problem p, const float2* ab, const float* lse, int v0, int vp,
-                                                        float* G) {
-  const int n0 = blockIdx.x * kTile, c0 = blockIdx.y * kTile;
-  float x[4][4] = {};
-  tile_product(
-      x, p.d,
-      [&](int r, int k) { return n0 + r < p.N ? Elem<TH>::get(static_cast<const TH*>(p.h)[(n0 + r) * p.ldh + k]) : 0.0f; },
-      [&](int r, int k) {
-        return c0 + r < vp ? Elem<TW>::get(static_cast<const TW*>(p.w)[(v0 + c0 + r) * p.ldw + k]) : 0.0f;
-      });
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+// Rows as operands: 16-bit ones as they are, float32 ones as `parts` bf16 parts of dp columns
+// each.  rows given: rows without a gradient become zeros; top given: the others are
+// multiplied by 2^exponent of RowScale.
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads) operand_kernel(const T* x, int64_t ld, int64_t n_rows, int d, int dp,
+                                                              int parts, const float4* rows, const float* top,
+                                                              uint16_t* out) {
+  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
+  const int64_t n = i / (dp / 8);
+  if (n >= n_rows) return;
+  const int j0 = (int)(i % (dp / 8)) * 8;
+  const bool live = !rows || has_gradient(rows[n]);
+  const float by = top && live ? ldexpf(1.0f, row_exponent(rows[n], *top)) : 1.0f;
+  uint4 o[3];
+  uint16_t(*u)[8] = reinterpret_cast<uint16_t(*)[8]>(o);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int n = n0 + ty * 4 + i;
-    if (n >= p.N) continue;
-    const int64_t t = target_of(p, n);
-    const float2 f = ab[n];
+  for (int j = 0; j < 8; ++j) {
+    T v = Elem<T>::put(0.0f);
+    if (j0 + j < d && live) v = x[n * ld + j0 + j];
+    if (sizeof(T) == 4) {
+      float r = Elem<T>::get(v);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = c0 + tx * 4 + j;
-      if (c >= vp) continue;
-      G[(int64_t)n * vp + c] = dead(f) ? 0.0f : f.x * expf(x[i][j] - lse[n]) - (v0 + c == t ? f.y : 0.0f);
+      for (int k = 0; k < 3; ++k) {
+        u[k][j] = f32_to_bf16(r);
+        r -= bf16_to_f32(u[k][j]);
+      }
+    } else {
+      if (top) v = Elem<T>::put(Elem<T>::get(v) * by);
+      u[0][j] = *reinterpret_cast<uint16_t*>(&v);
     }
   }
+  for (int k = 0; k < parts; ++k) *reinterpret_cast<uint4*>(out + (n * parts + k) * dp + j0) = o[k];
 }
 
-// acc (+)= G W of a piece.
-template <typename TW>
-__global__ void __launch_bounds__(kThreads) dh_kernel(Problem p, const float* G, int v0, int vp, float* acc) {
-  const int n0 = blockIdx.x * kTile, c0 = blockIdx.y * kTile;
-  float x[4][4] = {};
-  tile_product(
-      x, vp, [&](int r, int k) { return n0 + r < p.N ? G[(int64_t)(n0 + r) * vp + k] : 0.0f; },
-      [&](int r, int k) {
-        return c0 + r < p.d ? Elem<TW>::get(static_cast<const TW*>(p.w)[(v0 + k) * p.ldw + c0 + r]) : 0.0f;
-      });
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + ty * 4 + i, c = c0 + tx * 4 + j;
-      if (n < p.N && c < p.d) acc[(int64_t)n * p.d + c] = (v0 ? acc[(int64_t)n * p.d + c] : 0.0f) + x[i][j];
-    }
+// out[r][j] = the sum of the splits' results, scaled back; 0 in a row without a gradient.
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads) finish_kernel(const float* acc, int splits, int64_t split_rows, int da,
+                                                             int64_t n_rows, int d, const float4* rows, const float* top,
+                                                             int f16, T* out) {
+  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
+  if (i >= n_rows * d) return;
+  const int64_t n = i / d, j = i % d;
+  float s = 0.0f;
+  for (int k = 0; k < splits; ++k) s += acc[(k * split_rows + n) * da + j];
+  if (f16) s = ldexpf(s, (rows ? row_exponent(rows[n], *top) : 0) - kF16Shift);
+  s *= scale_of(*top);
+  if (rows && !has_gradient(rows[n])) s = 0.0f;
+  out[i] = Elem<T>::put(s);
 }
 
-template <typename TH>
-__global__ void __launch_bounds__(kThreads) dh_out_kernel(Problem p, const float2* ab, const float* acc, TH* dh) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= (int64_t)p.N * p.d) return;
-  dh[i] = Elem<TH>::put(dead(ab[i / p.d]) ? 0.0f : acc[i]);
+// ------------------------------------------------------------------- host
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder() {
+  static const EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult how;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &how) != cudaSuccess ||
+        how != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
 }
 
-// dW = G^T h of a piece; rows without a gradient are left out, whatever they hold.
-template <typename TH, typename TW>
-__global__ void __launch_bounds__(kThreads) dw_kernel(Problem p, const float2* ab, const float* G, int v0, int vp, TW* dw) {
-  const int r0 = blockIdx.x * kTile, c0 = blockIdx.y * kTile;
-  float x[4][4] = {};
-  tile_product(
-      x, p.N, [&](int r, int k) { return r0 + r < vp ? G[(int64_t)k * vp + r0 + r] : 0.0f; },
-      [&](int r, int k) {
-        return c0 + r < p.d && !dead(ab[k]) ? Elem<TH>::get(static_cast<const TH*>(p.h)[k * p.ldh + c0 + r]) : 0.0f;
-      });
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = r0 + ty * 4 + i, c = c0 + tx * 4 + j;
-      if (r < vp && c < p.d) dw[(int64_t)(v0 + r) * p.d + c] = Elem<TW>::put(x[i][j]);
-    }
+// A matrix of rows `ld` elements apart, in boxes of 128 bytes x box_rows.
+bool map_of(CUtensorMap* map, const void* at, CUtensorMapDataType type, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  const int size = type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(ld * size)};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows}, steps[2] = {1, 1};
+  return encoder() && encoder()(map, type, 2, const_cast<void*>(at), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 bool bad(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype, int64_t ldw, int32_t N, int32_t V,
@@ -230,24 +825,226 @@ bool too_large(int32_t N, int32_t V, int32_t d) {
   return N > CB_ENDS_MAX_ROWS || V > CB_ENDS_MAX_VOCAB || d > CB_ENDS_MAX_DIM;
 }
 
-size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-template <typename F>
-int with_types(int32_t h_dtype, int32_t w_dtype, F&& f) {
-  if (h_dtype == CB_F32) return w_dtype == CB_F32 ? f(float{}, float{}) : f(float{}, __nv_bfloat16{});
-  return with_type(h_dtype, [&](auto t) { return f(t, t); });
+// Whether a 16-bit matrix can be copied by TMA where it lies.
+bool direct(const void* x, int32_t dtype, int64_t ld, int64_t rows) {
+  return dtype != CB_F32 && aligned_to(x, 16) && (rows == 1 || (ld % 8 == 0 && ld > 0));
 }
+
+// Vocabulary rows whose G is held at a time: whole tiles, 256 MiB of G at most.
+int piece_of(int32_t N, int32_t V, int parts) {
+  const int64_t most = std::max<int64_t>(kTileM, (int64_t)(256 << 20) / ((int64_t)N * parts * 2) / kTileM * kTileM);
+  const int pieces = (int)((V + most - 1) / most);
+  return (int)up((V + pieces - 1) / pieces, kTileM);
+}
+
+// The products of parts that matter, the smallest first: what tensor memory cuts off a sum
+// (below) is in proportion to the sum so far.
+int passes_of(int a_parts, int b_parts, int a_cols, int b_cols, Gemm& g) {
+  g.passes = 0;
+  for (int both = 2; both >= 0; --both)
+    for (int i = std::min(both, a_parts - 1); i >= 0 && both - i < b_parts; --i) {
+      g.a_part[g.passes] = i * a_cols;
+      g.b_part[g.passes++] = (both - i) * b_cols;
+    }
+  g.span = g.passes == 1 ? kSpan16 : kSpan32;
+  return g.passes;
+}
+
+struct Split {
+  int h, w;        // of K of the two products
+  int extra;       // see item_of
+  bool dh_first;   // the longer items
+};
+
+// How K of the two products is split over the pairs: the split whose longest pair ends
+// first, counted in steps of K, with what a tile costs beside them and what the splits'
+// results cost in memory.
+Split split_of(int pairs, int h_tiles, int h_steps, int w_tiles, int w_steps, int passes_h, int passes_w, double h_bytes,
+               double w_bytes, int h_most, int w_most) {
+  constexpr int kTileCost = 6;             // of filling and emptying, in steps
+  constexpr double kBytesPerStep = 900e3;  // written and read back in a step's time by the whole device
+  Split best{1, 1, 0, true};
+  double least = 1e30;
+  for (int sh = 1; sh <= 32 && sh <= h_steps && sh <= h_most; sh *= 2)
+    for (int sw = 1; sw <= 32 && sw <= w_steps && sw <= w_most; sw *= 2) {
+      const double lh = (double)h_steps * passes_h / sh + kTileCost, lw = (double)w_steps * passes_w / sw + kTileCost;
+      const int nh = h_tiles * sh, nw = w_tiles * sw;
+      const bool first = nw == 0 || (nh > 0 && lh >= lw);
+      const int n1 = first ? nh : nw, n2 = first ? nw : nh;
+      const double l1 = first ? lh : lw, l2 = first ? lw : lh;
+      const int odd = n1 % pairs, extra = odd ? (int)std::min<int64_t>(n2, (int64_t)(pairs - odd) * (int)(l1 / l2)) : 0;
+      const double a = (n1 / pairs + (odd > 0)) * l1, b = (n1 / pairs) * l1 + (odd ? ceil_div(extra, pairs - odd) * l2 : 0.0);
+      double t = std::max(a, b) + ceil_div(n2 - extra, pairs) * l2;
+      if (nh) t += sh * h_bytes / kBytesPerStep;
+      if (nw && sw > 1) t += sw * w_bytes / kBytesPerStep;
+      if (t < least * 0.999) {
+        least = t;
+        best = Split{sh, sw, extra, first};
+      }
+      if (w_tiles == 0) break;
+    }
+  return best;
+}
+
+struct Shape {
+  int N, V, d, dp;          // dp: columns of a part
+  int h_parts, w_parts, g_parts;
+  CUtensorMapDataType type;  // of operands
+  int f16;
+  int pairs;                // on this device
+  int piece;                // backward
+  Shape(int32_t h_dtype, int32_t w_dtype, int N_, int V_, int d_) : N(N_), V(V_), d(d_), dp((int)up(d_, kStep)) {
+    h_parts = h_dtype == CB_F32 ? 3 : 1;
+    w_parts = w_dtype == CB_F32 ? 3 : 1;
+    g_parts = h_parts;
+    f16 = h_dtype == CB_F16;
+    type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    pairs = std::max(1, num_sms() / 2);
+    piece = piece_of(N, V, g_parts);
+  }
+  uint32_t kind() const { return 1u << 4 | (f16 ? 0u : 1u << 7 | 1u << 10); }
+  int da() const { return (int)up(d, 4); }  // columns of a float32 result
+};
+
+// The splits of a piece; those of the first, the largest, are what scratch is laid out for.
+Split splits(const Shape& s, bool dh, bool dw, int vp, int h_most, int w_most) {
+  Gemm t;
+  const int nt = ceil_div(s.d, kTileN);
+  return split_of(s.pairs, dh ? ceil_div(s.N, kTileM) * nt : 0, ceil_div(vp, kStep), dw ? ceil_div(vp, kTileM) * nt : 0,
+                  ceil_div(s.N, kStep), passes_of(s.g_parts, s.w_parts, 0, 0, t), passes_of(s.g_parts, s.h_parts, 0, 0, t),
+                  2.0 * s.N * s.d * 4, 2.0 * vp * s.d * 4, h_most, w_most);
+}
+
+// Scratch, part by part; `at` null only counts.
+struct Layout {
+  char* at;
+  size_t used = 0;
+  template <typename T>
+  T* take(int64_t n) {
+    T* p = reinterpret_cast<T*>(at + used);
+    used += (size_t)up(n * (int64_t)sizeof(T), 256);
+    return p;
+  }
+};
+
+struct Forward {
+  uint16_t *h, *w;
+  float2* part;
+  float *xt, *rows;
+  uint32_t* counter;
+  int tile_n, m_tiles, n_tiles, pairs, slots;
+  Forward(Layout& a, const Shape& s, bool h_direct, bool w_direct) {
+    // the width that leaves the pairs' last round fullest: 32000 columns for one tile of
+    // rows take two rounds of 74 either way, of 256 or of 224 columns
+    m_tiles = ceil_div(s.N, kTileM);
+    int64_t least = INT64_MAX;
+    tile_n = kTileN;
+    for (int t = kTileN; t >= 192; t -= 32) {
+      const int64_t all = (int64_t)m_tiles * ceil_div(s.V, t), cost = (all + s.pairs - 1) / s.pairs * t;
+      if (cost * 33 < least * 32) {
+        least = cost;
+        tile_n = t;
+      }
+    }
+    n_tiles = ceil_div(s.V, tile_n);
+    pairs = (int)std::min<int64_t>(s.pairs, (int64_t)m_tiles * n_tiles);
+    slots = ceil_div(pairs, m_tiles) + 1;
+    h = h_direct ? nullptr : a.take<uint16_t>((int64_t)s.N * s.h_parts * s.dp);
+    w = w_direct ? nullptr : a.take<uint16_t>((int64_t)s.V * s.w_parts * s.dp);
+    part = a.take<float2>((int64_t)slots * 2 * s.N);
+    xt = a.take<float>(s.N);
+    rows = a.take<float>(s.N);
+    counter = a.take<uint32_t>(1);
+  }
+};
+
+struct Backward {
+  float4* rows;
+  float* top;
+  uint16_t *h, *hs, *w, *G;
+  float *acc, *dw;
+  Split split;
+  int dw_direct;
+  Backward(Layout& a, const Shape& s, bool w_direct, bool want_h, bool want_w, bool dw_aligned) {
+    const int vp = std::min(s.piece, s.V);
+    split = splits(s, want_h, want_w, vp, 32, 32);
+    dw_direct = dw_aligned && split.w == 1;
+    rows = a.take<float4>(s.N);
+    top = a.take<float>(1);
+    h = a.take<uint16_t>((int64_t)s.N * s.h_parts * s.dp);
+    hs = s.f16 && want_w ? a.take<uint16_t>((int64_t)s.N * s.dp) : h;
+    w = w_direct ? nullptr : a.take<uint16_t>((int64_t)s.V * s.w_parts * s.dp);
+    G = a.take<uint16_t>((int64_t)s.N * s.g_parts * up(vp, kStep));
+    acc = want_h ? a.take<float>((int64_t)split.h * up(s.N, kTileM) * s.da()) : nullptr;
+    dw = want_w && !dw_direct ? a.take<float>((int64_t)split.w * up(vp, kTileM) * s.da()) : nullptr;
+  }
+};
+
+template <int MODE>
+int launch(const Args& p, cudaStream_t st) {
+  if (int rc = ensure_smem_attr((const void*)gemm_kernel<MODE>, kSmem)) return rc;
+  gemm_kernel<MODE><<<2 * p.pairs, kThreads, kSmem, st>>>(p);
+  return launched();
+}
+
+template <typename T>
+int make_operand(const void* x, int64_t ld, int64_t n_rows, const Shape& s, int parts, const float4* rows, const float* top,
+                 uint16_t* out, cudaStream_t st) {
+  const int64_t n = n_rows * (s.dp / 8);
+  operand_kernel<T><<<(unsigned)((n + kRowThreads - 1) / kRowThreads), kRowThreads, 0, st>>>(
+      static_cast<const T*>(x), ld, n_rows, s.d, s.dp, parts, rows, top, out);
+  return launched();
+}
+
+int make_operand(int32_t dtype, const void* x, int64_t ld, int64_t n_rows, const Shape& s, int parts, const float4* rows,
+                 const float* top, uint16_t* out, cudaStream_t st) {
+  return with_type(dtype, [&](auto t) { return make_operand<decltype(t)>(x, ld, n_rows, s, parts, rows, top, out, st); });
+}
+
+template <typename T>
+int finish(const float* acc, int splits, int64_t split_rows, const Shape& s, int64_t n_rows, const float4* rows,
+           const float* top, T* out, cudaStream_t st) {
+  finish_kernel<T><<<(unsigned)((n_rows * s.d + kRowThreads - 1) / kRowThreads), kRowThreads, 0, st>>>(
+      acc, splits, split_rows, s.da(), n_rows, s.d, rows, top, s.f16, out);
+  return launched();
+}
+
+// An operand in memory: the caller's matrix, or one made from it.
+struct Operand {
+  const void* at;
+  int64_t cols, ld;
+  Operand(const void* x, int64_t ld_, int64_t rows, const uint16_t* made, int parts, const Shape& s) {
+    at = made ? made : x;
+    cols = made ? (int64_t)parts * s.dp : s.d;
+    ld = made ? cols : rows == 1 ? up(s.d, 8) : ld_;
+  }
+};
 
 }  // namespace
 }  // namespace cb
 
 using namespace cb;
 
-extern "C" size_t cb_linear_ce_scratch_bytes(int32_t h_dtype, int32_t w_dtype, int32_t N, int32_t V, int32_t d,
-                                             int32_t backward) {
+extern "C" size_t cb_linear_ce_scratch_bytes(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype,
+                                             int64_t ldw, int32_t N, int32_t V, int32_t d, const void* dw, int32_t backward) {
   if (N <= 0 || V <= 0 || d <= 0 || too_large(N, V, d) || !is_dtype(h_dtype) || !is_dtype(w_dtype)) return 0;
-  if (!backward) return up16((size_t)N * ceil_div(V, kTile) * sizeof(float2)) + up16((size_t)N * 4) * 2;
-  return up16((size_t)N * sizeof(float2)) + up16((size_t)N * min(V, kPiece) * 4) + up16((size_t)N * d * 4);
+  const Shape s(h_dtype, w_dtype, N, V, d);
+  Layout a{nullptr};
+  if (!backward) {
+    Forward f(a, s, direct(h, h_dtype, ldh, N), direct(w, w_dtype, ldw, V));
+  } else {
+    // the larger of what the gradients together and each alone take
+    size_t most = 0;
+    for (int want = 1; want < 4; ++want) {
+      Layout b{nullptr};
+      Backward f(b, s, direct(w, w_dtype, ldw, V), want & 1, want & 2, aligned_to(dw, 16) && d * dtype_size(w_dtype) % 16 == 0);
+      most = std::max(most, b.used);
+    }
+    return most;
+  }
+  return a.used;
 }
 
 extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype, int64_t ldw,
@@ -255,27 +1052,42 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
                             float* loss, float* lse, int32_t* count, void* scratch, size_t scratch_bytes,
                             int32_t* status, void* stream) {
   if (bad(h, h_dtype, ldh, w, w_dtype, ldw, N, V, d, targets, targets_64, reduction) || !loss || !lse || !scratch ||
-      !aligned_to(scratch, 16) || (reduction != CB_REDUCE_NONE && !count))
+      !aligned_to(scratch, 256) || (reduction != CB_REDUCE_NONE && !count))
     return CB_ERR_ARG;
   if (too_large(N, V, d)) return CB_ERR_SHAPE;
-  if (scratch_bytes < cb_linear_ce_scratch_bytes(h_dtype, w_dtype, N, V, d, 0)) return CB_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
-  const Problem p{h, w, ldh, ldw, N, V, d, Ids{targets, targets_64}};
-  const int tiles = ceil_div(V, kTile);
-  float2* part = static_cast<float2*>(scratch);
-  float* xt = reinterpret_cast<float*>(static_cast<char*>(scratch) + up16((size_t)N * tiles * sizeof(float2)));
-  float* rows = reduction == CB_REDUCE_NONE ? loss : xt + up16((size_t)N * 4) / 4;
-  return with_types(h_dtype, w_dtype, [&](auto t, auto u) {
-    using TH = decltype(t);
-    using TW = decltype(u);
-    stats_kernel<TH, TW><<<dim3(ceil_div(N, kTile), tiles), kThreads, 0, st>>>(p, part, xt);
-    if (int rc = launched()) return rc;
-    join_kernel<<<ceil_div(N, kThreads), kThreads, 0, st>>>(p, part, tiles, xt, rows, lse, status);
-    if (int rc = launched()) return rc;
-    if (reduction == CB_REDUCE_NONE) return (int)CB_OK;
-    reduce_kernel<<<1, 1024, 0, st>>>(p, rows, reduction == CB_REDUCE_MEAN, loss, count);
-    return launched();
-  });
+  const Shape s(h_dtype, w_dtype, N, V, d);
+  Layout a{static_cast<char*>(scratch)};
+  const Forward f(a, s, direct(h, h_dtype, ldh, N), direct(w, w_dtype, ldw, V));
+  if (scratch_bytes < a.used) return CB_ERR_WORKSPACE;
+  if (f.h)
+    if (int rc = make_operand(h_dtype, h, ldh, N, s, s.h_parts, nullptr, nullptr, f.h, st)) return rc;
+  if (f.w)
+    if (int rc = make_operand(w_dtype, w, ldw, V, s, s.w_parts, nullptr, nullptr, f.w, st)) return rc;
+  const Operand ho(h, ldh, N, f.h, s.h_parts, s), wo(w, ldw, V, f.w, s.w_parts, s);
+  Args p{};
+  Gemm& g = p.g[0];
+  if (!map_of(&g.a, ho.at, s.type, N, ho.cols, ho.ld, 128) || !map_of(&g.b, wo.at, s.type, V, wo.cols, wo.ld, f.tile_n / 2))
+    return CB_ERR_CUDA;
+  passes_of(s.h_parts, s.w_parts, s.dp, s.dp, g);
+  g.m_tiles = f.m_tiles;
+  g.n_tiles = f.n_tiles;
+  g.k_steps = s.dp / kStep;
+  p.pairs = f.pairs;
+  p.kind = s.kind();
+  p.tile_n = f.tile_n;
+  p.N = N;
+  p.V = p.vp = V;
+  p.targets = Ids{targets, targets_64};
+  p.part = f.part;
+  p.xt = f.xt;
+  p.counter = f.counter;
+  p.status = status;
+  if (int rc = launch<STATS>(p, st)) return rc;
+  join_kernel<<<ceil_div(N, kRowThreads / 32), kRowThreads, 0, st>>>(
+      Problem{N, V, d, p.targets}, f.n_tiles, f.m_tiles, f.pairs, f.part, f.xt, reduction == CB_REDUCE_NONE ? loss : f.rows,
+      lse, reduction, loss, count, f.counter, status);
+  return launched();
 }
 
 extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype,
@@ -283,42 +1095,125 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
                                  int32_t reduction, const float* lse, const int32_t* count, const float* g_loss,
                                  int64_t g_loss_step, const float* g_lse, int64_t g_lse_step, void* dh, void* dw,
                                  void* scratch, size_t scratch_bytes, int32_t* status, void* stream) {
-  (void)status;
   if (bad(h, h_dtype, ldh, w, w_dtype, ldw, N, V, d, targets, targets_64, reduction) || !lse || !scratch ||
-      !aligned_to(scratch, 16) || (reduction == CB_REDUCE_MEAN && !count) || g_loss_step < 0 || g_lse_step < 0 ||
-      (!dh && !dw) || (dh && !aligned_to(dh, dtype_size(h_dtype))) || (dw && !aligned_to(dw, dtype_size(w_dtype))))
+      !aligned_to(scratch, 256) || (reduction == CB_REDUCE_MEAN && !count) || g_loss_step < 0 || g_lse_step < 0 ||
+      (!dh && !dw) || !aligned_to(dh, dtype_size(h_dtype)) || !aligned_to(dw, dtype_size(w_dtype)))
     return CB_ERR_ARG;
   if (too_large(N, V, d)) return CB_ERR_SHAPE;
-  if (scratch_bytes < cb_linear_ce_scratch_bytes(h_dtype, w_dtype, N, V, d, 1)) return CB_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
-  const Problem p{h, w, ldh, ldw, N, V, d, Ids{targets, targets_64}};
-  char* at = static_cast<char*>(scratch);
-  float2* ab = reinterpret_cast<float2*>(at);
-  float* G = reinterpret_cast<float*>(at += up16((size_t)N * sizeof(float2)));
-  float* acc = reinterpret_cast<float*>(at + up16((size_t)N * min(V, kPiece) * 4));
-  factors_kernel<<<ceil_div(N, kThreads), kThreads, 0, st>>>(
-      p, Upstream{g_loss, g_lse, g_loss_step, g_lse_step, count, reduction}, ab);
+  const Shape s(h_dtype, w_dtype, N, V, d);
+  const bool dw_aligned = aligned_to(dw, 16) && d * dtype_size(w_dtype) % 16 == 0;
+  Layout a{static_cast<char*>(scratch)};
+  const Backward f(a, s, direct(w, w_dtype, ldw, V), dh != nullptr, dw != nullptr, dw_aligned);
+  if (scratch_bytes < a.used) return CB_ERR_WORKSPACE;
+  const Problem pb{N, V, d, Ids{targets, targets_64}};
+  const Upstream u{g_loss, g_lse, g_loss_step, g_lse_step, count, reduction};
+  if (cudaMemsetAsync(f.top, 0, sizeof(float), st) != cudaSuccess) return CB_ERR_CUDA;
+  factors_kernel<<<ceil_div(N, kRowThreads), kRowThreads, 0, st>>>(pb, u, lse, f.rows, f.top);
   if (int rc = launched()) return rc;
-  return with_types(h_dtype, w_dtype, [&](auto t, auto u) {
-    using TH = decltype(t);
-    using TW = decltype(u);
-    for (int v0 = 0; v0 < V; v0 += kPiece) {
-      const int vp = min(kPiece, V - v0);
-      grad_kernel<TH, TW><<<dim3(ceil_div(N, kTile), ceil_div(vp, kTile)), kThreads, 0, st>>>(p, ab, lse, v0, vp, G);
-      if (int rc = launched()) return rc;
-      if (dh) {
-        dh_kernel<TW><<<dim3(ceil_div(N, kTile), ceil_div(d, kTile)), kThreads, 0, st>>>(p, G, v0, vp, acc);
-        if (int rc = launched()) return rc;
-      }
-      if (dw) {
-        dw_kernel<TH, TW><<<dim3(ceil_div(vp, kTile), ceil_div(d, kTile)), kThreads, 0, st>>>(p, ab, G, v0, vp,
-                                                                                            static_cast<TW*>(dw));
-        if (int rc = launched()) return rc;
-      }
+  if (int rc = make_operand(h_dtype, h, ldh, N, s, s.h_parts, f.rows, nullptr, f.h, st)) return rc;
+  if (f.hs != f.h)
+    if (int rc = make_operand(h_dtype, h, ldh, N, s, 1, f.rows, f.top, f.hs, st)) return rc;
+  if (f.w)
+    if (int rc = make_operand(w_dtype, w, ldw, V, s, s.w_parts, nullptr, nullptr, f.w, st)) return rc;
+  const Operand wo(w, ldw, V, f.w, s.w_parts, s);
+  const int64_t h_cols = (int64_t)s.h_parts * s.dp;
+  const int nt = ceil_div(d, kTileN), m_tiles = ceil_div(N, kTileM);
+
+  Args q{};  // G of a piece
+  Gemm& g = q.g[0];
+  if (!map_of(&g.a, f.h, s.type, N, h_cols, h_cols, 128) || !map_of(&g.b, wo.at, s.type, V, wo.cols, wo.ld, kTileN / 2))
+    return CB_ERR_CUDA;
+  passes_of(s.h_parts, s.w_parts, s.dp, s.dp, g);
+  g.m_tiles = m_tiles;
+  g.k_steps = s.dp / kStep;
+  q.kind = s.kind();
+  q.tile_n = kTileN;
+  q.N = N;
+  q.V = V;
+  q.targets = pb.targets;
+  q.rows = f.rows;
+  q.top = f.top;
+  q.g_parts = s.g_parts;
+  q.is_f16 = s.f16;
+  q.status = status;
+  Args r{};  // both products of a piece
+  r.kind = q.kind;
+  r.is_f16 = s.f16;
+  r.status = status;
+  for (int v0 = 0; v0 < V; v0 += s.piece) {
+    const int vp = std::min(s.piece, V - v0), cols = (int)up(vp, kStep);
+    const int64_t g_ld = (int64_t)s.g_parts * cols;
+    if (!map_of(&g.out, f.G, s.type, N, g_ld, g_ld, 128)) return CB_ERR_CUDA;
+    g.b_base = q.v0 = v0;
+    g.n_tiles = ceil_div(vp, kTileN);
+    q.vp = vp;
+    q.g_cols = cols;
+    q.pairs = (int)std::min<int64_t>(s.pairs, (int64_t)m_tiles * g.n_tiles);
+    if (int rc = launch<GRAD>(q, st)) return rc;
+
+    const Split sp = v0 ? splits(s, dh != nullptr, dw != nullptr, vp, f.split.h, f.split.w) : f.split;
+    Gemm& gh = r.g[sp.dh_first ? 0 : 1];
+    Gemm& gw = r.g[sp.dh_first ? 1 : 0];
+    gh = gw = Gemm{};
+    int nh = 0, nw = 0;
+    if (dh) {
+      if (!map_of(&gh.a, f.G, s.type, N, g_ld, g_ld, 128) || !map_of(&gh.b, wo.at, s.type, V, wo.cols, wo.ld, 64) ||
+          !map_of(&gh.out, f.acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.split.h * up(N, kTileM), s.da(), s.da(), 128))
+        return CB_ERR_CUDA;
+      passes_of(s.g_parts, s.w_parts, cols, s.dp, gh);
+      gh.b_mn = 1;
+      gh.b_base = v0;
+      gh.m_tiles = m_tiles;
+      gh.n_tiles = nt;
+      gh.k_steps = cols / kStep;
+      gh.splits = sp.h;
+      gh.out_f32 = 1;
+      gh.out_mode = v0 ? OUT_ADD : OUT_STORE;
+      gh.out_rows = (int)up(N, kTileM);
+      nh = m_tiles * nt * sp.h;
     }
-    if (!dh) return (int)CB_OK;
-    dh_out_kernel<TH><<<(unsigned)(((int64_t)N * d + kThreads - 1) / kThreads), kThreads, 0, st>>>(p, ab, acc,
-                                                                                                  static_cast<TH*>(dh));
-    return launched();
+    if (dw) {
+      if (!map_of(&gw.a, f.G, s.type, N, g_ld, g_ld, 64) ||
+          !map_of(&gw.b, s.f16 ? f.hs : f.h, s.type, N, s.f16 ? s.dp : h_cols, s.f16 ? s.dp : h_cols, 64))
+        return CB_ERR_CUDA;
+      const bool ok =
+          f.dw_direct
+              ? map_of(&gw.out, static_cast<char*>(dw) + (int64_t)v0 * d * dtype_size(w_dtype),
+                       w_dtype == CB_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : s.type, vp, d, d, 128)
+              : map_of(&gw.out, f.dw, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.split.w * up(std::min(s.piece, V), kTileM), s.da(),
+                       s.da(), 128);
+      if (!ok) return CB_ERR_CUDA;
+      passes_of(s.g_parts, s.h_parts, cols, s.dp, gw);
+      gw.a_mn = gw.b_mn = 1;
+      gw.m_tiles = ceil_div(vp, kTileM);
+      gw.n_tiles = nt;
+      gw.k_steps = ceil_div(N, kStep);
+      gw.splits = sp.w;
+      gw.out_f32 = !f.dw_direct || w_dtype == CB_F32;
+      gw.out_rows = (int)up(std::min(s.piece, V), kTileM);
+      if (f.dw_direct) {
+        gw.scale = f.top;
+        gw.scale_by = s.f16 ? 1.0f / (1 << kF16Shift) : 1.0f;
+      }
+      nw = gw.m_tiles * nt * sp.w;
+    }
+    r.n1 = sp.dh_first ? nh : nw;
+    r.n2 = sp.dh_first ? nw : nh;
+    r.pairs = std::min(s.pairs, r.n1 + r.n2);
+    r.extra = r.pairs == s.pairs ? sp.extra : 0;
+    if (int rc = launch<PRODUCTS>(r, st)) return rc;
+    if (dw && !f.dw_direct)
+      if (int rc = with_type(w_dtype, [&](auto t) {
+            using T = decltype(t);
+            return finish<T>(f.dw, sp.w, up(std::min(s.piece, V), kTileM), s, vp, nullptr, f.top,
+                             static_cast<T*>(dw) + (int64_t)v0 * d, st);
+          }))
+        return rc;
+  }
+  if (!dh) return CB_OK;
+  return with_type(h_dtype, [&](auto t) {
+    using T = decltype(t);
+    return finish<T>(f.acc, f.split.h, up(N, kTileM), s, N, f.rows, f.top, static_cast<T*>(dh), st);
   });
 }

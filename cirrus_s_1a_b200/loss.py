@@ -45,7 +45,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
 
 
 def _check(hidden, weight, targets, reduction, status) -> tuple:
-    """The leading arguments of both entry points, and (N, V, d) with the type codes."""
+    """The leading arguments of both entry points, and (N, V, d)."""
     N, D, ldh, h_code = _rows.matrix(hidden, "hidden")
     V, Dw, ldw, w_code = _rows.vocabulary(weight, "weight", hidden.device)
     if Dw != D:
@@ -60,18 +60,18 @@ def _check(hidden, weight, targets, reduction, status) -> tuple:
         raise ValueError(f"unknown reduction {reduction!r}; choose from {sorted(REDUCTIONS)}")
     _rows.status(status, hidden.device)
     return (hidden.data_ptr(), h_code, ldh, weight.data_ptr(), w_code, ldw, N, V, D, targets.data_ptr(), wide,
-            REDUCTIONS[reduction]), (h_code, w_code, N, V, D)
+            REDUCTIONS[reduction]), (N, V, D)
 
 
 def _forward(hidden, weight, targets, reduction, status) -> tuple:
     args, shape = _check(hidden, weight, targets, reduction, status)
-    dev, N = hidden.device, shape[2]
+    dev, N = hidden.device, shape[0]
     lse = torch.empty(N, dtype=torch.float32, device=dev)
     if N == 0:
         return torch.zeros(() if reduction != "none" else 0, device=dev), lse, None
     loss = torch.empty(N if reduction == "none" else (), dtype=torch.float32, device=dev)
     count = None if reduction == "none" else torch.empty(1, dtype=torch.int32, device=dev)
-    scratch = _rows.scratch(dev, "cb_linear_ce_scratch_bytes", *shape, 0)
+    scratch = _rows.scratch(dev, "cb_linear_ce_scratch_bytes", *args[:9], None, 0)
     _rows.call(dev, "cb_linear_ce", *args, loss.data_ptr(), lse.data_ptr(), _lib.ptr(count), scratch.data_ptr(),
                scratch.numel(), _rows.status(status, dev))
     return loss, lse, count
@@ -94,12 +94,12 @@ class _LinearCE(torch.autograd.Function):
         if g_loss is None and g_lse is None:
             return None, None, None, None, None
         args, shape = _check(hidden, weight, targets, ctx.reduction, ctx.status)
-        dev, (_, _, N, V, D) = hidden.device, shape
+        dev, (N, V, D) = hidden.device, shape
         dh = torch.empty(N, D, dtype=hidden.dtype, device=dev) if want_h else None
         if N == 0:
             return dh, torch.zeros(V, D, dtype=weight.dtype, device=dev) if want_w else None, None, None, None
         dw = torch.empty(V, D, dtype=weight.dtype, device=dev) if want_w else None
-        scratch = _rows.scratch(dev, "cb_linear_ce_scratch_bytes", *shape, 1)
+        scratch = _rows.scratch(dev, "cb_linear_ce_scratch_bytes", *args[:9], _lib.ptr(dw), 1)
         step = lambda g: g.stride(0) if g is not None and g.dim() else 0  # noqa: E731
         _rows.call(dev, "cb_linear_ce_grad", *args, lse.data_ptr(), _lib.ptr(count), _lib.ptr(g_loss), step(g_loss),
                    _lib.ptr(g_lse), step(g_lse), _lib.ptr(dh), _lib.ptr(dw), scratch.data_ptr(), scratch.numel(),

@@ -43,7 +43,8 @@ def test_entry_points_refuse_bad_arguments_without_launching(built_lib):  # noqa
         256, 1, 8, 256, 1, 8, 3, 4, 8, 256, 1, red, lse, count, gl, s1, None, 0, dh, dw, s, nb, None, None)
     assert cg(lse=None) == 1 and cg(red=1, count=None) == 1 and cg(s1=-1) == 1 and cg(dh=None, dw=None) == 1
     assert cg(dh=257) == 1 and cg(dw=257) == 1 and cg(s=None) == 1 and cg(nb=0) == 4
-    assert L.cb_linear_ce_scratch_bytes(7, 1, 3, 4, 8, 0) == 0 and L.cb_linear_ce_scratch_bytes(1, 1, 3, 4, 8, 1) > 0
+    need = lambda hd, back: L.cb_linear_ce_scratch_bytes(256, hd, 8, 256, 1, 8, 3, 4, 8, 256, back)  # noqa: E731
+    assert need(7, 0) == 0 and need(1, 0) > 0 and need(1, 1) > 0 and need(0, 1) > need(1, 1)
     assert L.cb_launch_count() == before
 
 
