@@ -2,44 +2,357 @@
 //
 //   y[n] = scale * table[id_n]                dtable[v] = scale * sum of g[n] over the n with id_n = v
 //
-// Both are bound by memory.  The gradient is written by vocabulary rows, so that every
-// row has one owner and its sum one order, that of the tokens, whatever their number.
+// Both are bound by memory: a row read and a row written for each token, and every row of
+// dtable.  The gradient sorts the tokens by id, so that every row has one owner and its sum
+// one order, that of the tokens:
+//   * sort_kernel: a cluster of up to 16 CTAs sorts up to 131072 (id, token) pairs by 8-bit
+//     digits, stable, exchanging counts and pairs through distributed shared memory;
+//   * sum_kernel: a warp sums 32 sorted tokens over 512 bytes of columns, however the tokens
+//     fall to rows, so that a frequent token is spread over many warps; a row whose tokens
+//     end within them is written, one that goes on leaves its part (float32) in scratch;
+//     other warps write the rows without a token;
+//   * join_kernel: adds the parts of such rows in order.
+// More tokens are taken in batches, added up in float32.
+#include <algorithm>
+#include <type_traits>
+
 #include "ends.cuh"
 
 namespace cb {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kPerCta = 8192, kMaxCluster = 16;
+constexpr int64_t kBatch = (int64_t)kPerCta * kMaxCluster;
+constexpr int kChunk = 32;  // sorted tokens of a warp
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) embedding_kernel(const T* table, int64_t ld, int V, int d, Ids ids,
-                                                             float scale, T* out, int32_t* status) {
-  const int64_t n = blockIdx.x;
+// ----------------------------------------------------------------- lookup
+// 16 bytes of a row to a thread, or one element where rows are not 16-byte aligned.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Vec {
+  T v[VEC];
+};
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) embedding_kernel(const T* table, int64_t ld, int V, int vecs, Ids ids,
+                                                             int64_t all, float scale, T* out, int32_t* status) {
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= all) return;
+  const int64_t n = i / vecs;
+  const int j = (int)(i - n * vecs);
   const int64_t id = ids[n];
-  const bool has = id >= 0 && id < V;
-  if (id >= V && threadIdx.x == 0) set_status(status, CB_ERR_TOKEN);
-  for (int j = threadIdx.x; j < d; j += kThreads)
-    out[n * d + j] = has ? Elem<T>::put(Elem<T>::get(table[id * ld + j]) * scale) : Elem<T>::put(0.0f);
+  Vec<T, VEC> x;
+  if (id >= 0 && id < V) {
+    x = *reinterpret_cast<const Vec<T, VEC>*>(table + id * ld + j * VEC);
+    if (scale != 1.0f)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x.v[k] = Elem<T>::put(Elem<T>::get(x.v[k]) * scale);
+  } else {
+    if (id >= V && j == 0) set_status(status, CB_ERR_TOKEN);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) x.v[k] = Elem<T>::put(0.0f);
+  }
+  *reinterpret_cast<Vec<T, VEC>*>(out + i * VEC) = x;
 }
 
-// A warp to 32 columns of a vocabulary row: it reads all ids in order.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) embedding_grad_kernel(const T* g, int64_t ldg, Ids ids, int64_t n, int V,
-                                                                  int d, float scale, T* dtable) {
+// ------------------------------------------------------------------- sort
+struct SortShared {
+  uint2 pairs[2][kPerCta];  // (key, token)
+  uint16_t rank[kPerCta];   // of a pair among its digit's in its warp's segment
+  uint16_t count[kSortWarps][256];
+  uint32_t total[256], base[256], warp_sum[8];
+};
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t at_rank(const void* p, int rank) {
+  uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+
+// Tokens [0, n) of the batch by id, those without one (as id V) last: keys and order.
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(Ids ids, int64_t first, int n, int V, int passes, uint32_t* keys,
+                                                            uint32_t* order) {
+  extern __shared__ SortShared sort_shared[];
+  SortShared& s = *sort_shared;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = blockIdx.x, ctas = gridDim.x;  // one cluster
+  const int per = (n + ctas - 1) / ctas, mine = max(0, min(per, n - rank * per));
+  // a warp's segment
+  const int seg = ((per + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
+  const int from = min(mine, warp * seg), to = min(mine, from + seg);
+  for (int i = tid; i < mine; i += kSortThreads) {
+    const int64_t id = ids[first + rank * per + i];
+    s.pairs[0][i] = make_uint2(id >= 0 && id < V ? (uint32_t)id : (uint32_t)V, (uint32_t)(rank * per + i));
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const uint2* in = s.pairs[pass & 1];
+    uint2* out = s.pairs[(pass & 1) ^ 1];
+    const int shift = pass * 8;
+    for (int i = lane; i < 256; i += 32) s.count[warp][i] = 0;
+    __syncthreads();
+    for (int i = from + lane; i - lane < to; i += 32) {
+      const bool is = i < to;
+      const uint32_t digit = is ? in[i].x >> shift & 255 : 256;
+      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      const int before = __popc(same & ((1u << lane) - 1));
+      const int at = is ? s.count[warp][digit] : 0;
+      __syncwarp();
+      if (is) {
+        s.rank[i] = (uint16_t)(at + before);
+        if (before == 0) s.count[warp][digit] = (uint16_t)(at + __popc(same));
+      }
+      __syncwarp();
+    }
+    __syncthreads();
+    if (tid < 256) {  // counts of the warps before, for each digit
+      uint32_t sum = 0;
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = s.count[w][tid];
+        s.count[w][tid] = (uint16_t)sum;
+        sum += c;
+      }
+      s.total[tid] = sum;
+    }
+    cluster_sync();
+    uint32_t before = 0, all = 0, scan = 0;
+    if (tid < 256) {
+      for (int r = 0; r < ctas; ++r) {
+        uint32_t c;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(at_rank(&s.total[tid], r)));
+        before += r < rank ? c : 0;
+        all += c;
+      }
+      scan = all;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += v;
+      }
+      if (lane == 31) s.warp_sum[warp] = scan;
+    }
+    __syncthreads();
+    if (tid < 256) {
+      for (int w = 0; w < warp; ++w) scan += s.warp_sum[w];
+      s.base[tid] = scan - all + before;
+    }
+    __syncthreads();
+    const bool last = pass == passes - 1;
+    for (int i = from + lane; i < to; i += 32) {
+      const uint2 p = in[i];
+      const uint32_t digit = p.x >> shift & 255, at = s.base[digit] + s.count[warp][digit] + s.rank[i];
+      if (last) {
+        keys[at] = p.x;
+        order[at] = p.y;
+      } else {
+        const uint32_t cta = at / per;
+        asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at_rank(out + (at - cta * per), cta)), "r"(p.x), "r"(p.y)
+                     : "memory");
+      }
+    }
+    cluster_sync();  // pairs have arrived, and totals may be replaced
+  }
+}
+
+// ------------------------------------------------------------------- sums
+// What a row's sum goes to: the table itself, or the batches' float32 sums.
+template <typename T, int VEC>
+__device__ __forceinline__ void write_row(T* dtable, float* total, int64_t at, const float* sum, float scale) {
+  if (total) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) total[at + k] += sum[k];
+  } else {
+    Vec<T, VEC> x;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) x.v[k] = Elem<T>::put(sum[k] * scale);
+    *reinterpret_cast<Vec<T, VEC>*>(dtable + at) = x;
+  }
+}
+
+// part[chunk][which][d]: 0 the sum of the tokens of the row that began before the chunk, 1 of
+// one that begins in it and goes on.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) sum_kernel(const T* g, int64_t ldg, const uint32_t* keys, const uint32_t* order,
+                                                       int n, int V, int d, int slabs, float scale, T* dtable, float* total,
+                                                       float* part) {
   const int lane = threadIdx.x & 31;
-  const int64_t v = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (v >= V) return;
-  const int j = blockIdx.y * 32 + lane;
-  float sum = 0.0f;
-  for (int64_t i = 0; i < n; i += 32) {
-    uint32_t hits = __ballot_sync(0xffffffffu, i + lane < n && ids[i + lane] == v);
-    while (hits) {
-      const int at = __ffs(hits) - 1;
-      hits &= hits - 1;
-      if (j < d) sum += Elem<T>::get(g[(i + at) * ldg + j]);
+  const int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const int chunks = (n + kChunk - 1) / kChunk;
+  const int64_t sums = (int64_t)chunks * slabs;
+  if (w >= sums) {
+    // rows without a token, 32 at a time
+    const int64_t v0 = (w - sums) * 32;
+    if (total || v0 >= V) return;
+    const uint32_t v = (uint32_t)v0 + lane;
+    int lo = 0, hi = n;  // the first key of v or more
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (keys[mid] < v) lo = mid + 1;
+      else hi = mid;
+    }
+    uint32_t none = __ballot_sync(0xffffffffu, v < (uint32_t)V && (lo >= n || keys[lo] != v));
+    Vec<T, VEC> zero;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) zero.v[k] = Elem<T>::put(0.0f);
+    while (none) {
+      const int64_t row = v0 + __ffs(none) - 1;
+      none &= none - 1;
+      for (int j = lane * VEC; j < d; j += 32 * VEC) *reinterpret_cast<Vec<T, VEC>*>(dtable + row * d + j) = zero;
+    }
+    return;
+  }
+  const int chunk = (int)(w / slabs), j = ((int)(w % slabs) * 32 + lane) * VEC;
+  const int first = chunk * kChunk, count = min(kChunk, n - first);
+  const bool live = j < d;
+  const uint32_t my_key = lane < count ? keys[first + lane] : (uint32_t)V;
+  const uint32_t my_row = lane < count ? order[first + lane] : 0;
+  const uint32_t prev = first > 0 ? keys[first - 1] : (uint32_t)V, next = first + count < n ? keys[first + count] : (uint32_t)V;
+  float sum[VEC] = {};
+  constexpr int kAhead = 8;  // rows in flight
+  for (int i0 = 0; i0 < count; i0 += kAhead) {
+    Vec<T, VEC> x[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const uint32_t key = __shfl_sync(0xffffffffu, my_key, i0 + i);
+      const int64_t row = __shfl_sync(0xffffffffu, my_row, i0 + i);
+      if (live && key < (uint32_t)V) x[i] = *reinterpret_cast<const Vec<T, VEC>*>(g + row * ldg + j);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = i0 + i;
+      const uint32_t key = __shfl_sync(0xffffffffu, my_key, at);
+      if (key >= (uint32_t)V) break;  // the tokens without an id are the last
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sum[k] += Elem<T>::get(x[i].v[k]);
+      const uint32_t after = at + 1 < count ? __shfl_sync(0xffffffffu, my_key, (at + 1) & 31) : next;
+      if (after == key && at + 1 < count) continue;
+      const bool began = key == prev && __shfl_sync(0xffffffffu, my_key, 0) == key;  // before the chunk
+      const bool goes_on = after == key;
+      if (live) {
+        if (began || goes_on) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) part[((int64_t)chunk * 2 + (began ? 0 : 1)) * d + j + k] = sum[k];
+        } else {
+          write_row<T, VEC>(dtable, total, (int64_t)key * d + j, sum, scale);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sum[k] = 0.0f;
     }
   }
-  if (j < d) dtable[v * d + j] = Elem<T>::put(sum * scale);
+}
+
+// A warp to 512 bytes of columns of a chunk whose last row goes on: the row's parts in order.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) join_kernel(const uint32_t* keys, int n, int V, int d, int slabs, float scale,
+                                                        T* dtable, float* total, const float* part) {
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const int chunk = (int)(w / slabs), j = ((int)(w % slabs) * 32 + lane) * VEC;
+  const int end = (chunk + 1) * kChunk;
+  if (end >= n || j >= d) return;
+  const uint32_t key = keys[end - 1];
+  if (key >= (uint32_t)V || keys[end] != key) return;
+  const int first = chunk * kChunk;
+  if (keys[first] == key && first > 0 && keys[first - 1] == key) return;  // it began before
+  float sum[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) sum[k] = part[((int64_t)chunk * 2 + 1) * d + j + k];
+  constexpr int kAhead = 8;
+  for (int64_t c = chunk + 1; c * kChunk < n && keys[c * kChunk] == key; c += kAhead) {
+    float x[kAhead][VEC];
+    bool is[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      is[i] = (c + i) * kChunk < n && keys[(c + i) * kChunk] == key;
+      if (is[i])
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) x[i][k] = part[(c + i) * 2 * d + j + k];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (is[i])
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sum[k] += x[i][k];
+  }
+  write_row<T, VEC>(dtable, total, (int64_t)key * d + j, sum, scale);
+}
+
+// The batches' sums in the table's type.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) scale_kernel(const float* total, int64_t all, float scale, T* dtable) {
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kThreads)
+    dtable[i] = Elem<T>::put(total[i] * scale);
+}
+
+// ------------------------------------------------------------------- host
+struct Scratch {
+  uint32_t *keys, *order;
+  float *part, *total;
+  size_t used = 0;
+  Scratch(void* at, int64_t n, int32_t V, int32_t d) {
+    const int64_t batch = std::min(n, kBatch);
+    auto take = [&](int64_t bytes) {
+      char* p = static_cast<char*>(at) + used;
+      used += (size_t)((bytes + 15) / 16 * 16);
+      return p;
+    };
+    keys = reinterpret_cast<uint32_t*>(take(batch * 4));
+    order = reinterpret_cast<uint32_t*>(take(batch * 4));
+    part = reinterpret_cast<float*>(take((batch + kChunk - 1) / kChunk * 2 * d * 4));
+    total = n > kBatch ? reinterpret_cast<float*>(take((int64_t)V * d * 4)) : nullptr;
+  }
+};
+
+int launch_sort(Ids ids, int64_t first, int n, int V, const Scratch& s, cudaStream_t st) {
+  int bits = 1;
+  while (V >> bits) ++bits;  // keys go up to V
+  // 2048 tokens a CTA where there are few: 5000 tokens in one CTA took 15 us instead of 11
+  int ctas = 1;
+  while (ctas < kMaxCluster && ctas * 2048 < n) ctas *= 2;
+  const void* fn = (const void*)sort_kernel;
+  if (int rc = ensure_smem_attr(fn, sizeof(SortShared))) return rc;
+  if (ctas > 8 && cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    return CB_ERR_CUDA;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = sizeof(SortShared);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ctas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, sort_kernel, ids, first, n, V, (bits + 7) / 8, s.keys, s.order) != cudaSuccess)
+    return CB_ERR_CUDA;
+  count_launch();
+  return CB_OK;
+}
+
+template <typename T, int VEC>
+int grad(const T* g, int64_t ldg, Ids ids, int64_t n, int V, int d, float scale, T* dtable, const Scratch& s, cudaStream_t st) {
+  if (s.total && cudaMemsetAsync(s.total, 0, (size_t)V * d * 4, st) != cudaSuccess) return CB_ERR_CUDA;
+  const int slabs = ceil_div(d, 32 * VEC);
+  for (int64_t first = 0; first < n; first += kBatch) {
+    const int m = (int)std::min(kBatch, n - first);
+    if (int rc = launch_sort(ids, first, m, V, s, st)) return rc;
+    const int64_t sums = (int64_t)ceil_div(m, kChunk) * slabs, warps = sums + (s.total ? 0 : ceil_div(V, 32));
+    constexpr int kWarps = kThreads / 32;
+    sum_kernel<T, VEC><<<(unsigned)((warps + kWarps - 1) / kWarps), kThreads, 0, st>>>(
+        g + first * ldg, ldg, s.keys, s.order, m, V, d, slabs, scale, dtable, s.total, s.part);
+    if (int rc = launched()) return rc;
+    if (m <= kChunk) continue;
+    join_kernel<T, VEC><<<(unsigned)((sums + kWarps - 1) / kWarps), kThreads, 0, st>>>(s.keys, m, V, d, slabs, scale, dtable,
+                                                                                       s.total, s.part);
+    if (int rc = launched()) return rc;
+  }
+  if (!s.total) return CB_OK;
+  scale_kernel<T><<<8 * num_sms(), kThreads, 0, st>>>(s.total, (int64_t)V * d, scale, dtable);
+  return launched();
 }
 
 }  // namespace
@@ -50,37 +363,45 @@ using namespace cb;
 extern "C" int cb_embedding(const void* table, int32_t dtype, int64_t ld, int32_t V, int32_t d, const void* ids,
                             int32_t ids_64, int64_t n, float scale, void* out, int32_t* status, void* stream) {
   if (!table || !ids || !out || V <= 0 || d <= 0 || n <= 0 || (V > 1 && ld < d) || !is_dtype(dtype)) return CB_ERR_ARG;
-  if (!aligned_to(table, dtype_size(dtype)) || !aligned_to(out, dtype_size(dtype)) || !aligned_to(ids, ids_64 ? 8 : 4))
-    return CB_ERR_ARG;
+  const int size = dtype_size(dtype);
+  if (!aligned_to(table, size) || !aligned_to(out, size) || !aligned_to(ids, ids_64 ? 8 : 4)) return CB_ERR_ARG;
   if (n > CB_ENDS_MAX_ROWS || V > CB_ENDS_MAX_VOCAB || d > CB_ENDS_MAX_DIM) return CB_ERR_SHAPE;
+  const bool wide = aligned_to(table, 16) && aligned_to(out, 16) && d * size % 16 == 0 && (V == 1 || ld * size % 16 == 0);
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    embedding_kernel<T><<<(unsigned)n, kThreads, 0, (cudaStream_t)stream>>>(
-        static_cast<const T*>(table), ld, V, d, Ids{ids, ids_64}, scale, static_cast<T*>(out), status);
-    return launched();
+    auto go = [&](auto vec) {
+      constexpr int VEC = decltype(vec)::value;
+      const int64_t all = n * (d / VEC);
+      embedding_kernel<T, VEC><<<(unsigned)((all + kThreads - 1) / kThreads), kThreads, 0, (cudaStream_t)stream>>>(
+          static_cast<const T*>(table), ld, V, d / VEC, Ids{ids, ids_64}, all, scale, static_cast<T*>(out), status);
+      return launched();
+    };
+    return wide ? go(std::integral_constant<int, 16 / sizeof(T)>{}) : go(std::integral_constant<int, 1>{});
   });
 }
 
 extern "C" size_t cb_embedding_grad_scratch_bytes(int64_t n, int32_t V, int32_t d) {
   if (n <= 0 || V <= 0 || d <= 0 || n > CB_ENDS_MAX_ROWS || V > CB_ENDS_MAX_VOCAB || d > CB_ENDS_MAX_DIM) return 0;
-  return 16;
+  return Scratch(nullptr, n, V, d).used;
 }
 
 extern "C" int cb_embedding_grad(const void* g, int32_t dtype, int64_t ldg, const void* ids, int32_t ids_64, int64_t n,
                                  int32_t V, int32_t d, float scale, void* dtable, void* scratch, size_t scratch_bytes,
                                  void* stream) {
   if (!g || !ids || !dtable || !scratch || V <= 0 || d <= 0 || n <= 0 || ldg < 0 || !is_dtype(dtype)) return CB_ERR_ARG;
-  if (!aligned_to(g, dtype_size(dtype)) || !aligned_to(dtable, dtype_size(dtype)) || !aligned_to(ids, ids_64 ? 8 : 4) ||
-      !aligned_to(scratch, 16))
+  const int size = dtype_size(dtype);
+  if (!aligned_to(g, size) || !aligned_to(dtable, size) || !aligned_to(ids, ids_64 ? 8 : 4) || !aligned_to(scratch, 16))
     return CB_ERR_ARG;
-  const size_t need = cb_embedding_grad_scratch_bytes(n, V, d);
-  if (!need) return CB_ERR_SHAPE;
-  if (scratch_bytes < need) return CB_ERR_WORKSPACE;
+  if (!cb_embedding_grad_scratch_bytes(n, V, d)) return CB_ERR_SHAPE;
+  const Scratch s(scratch, n, V, d);
+  if (scratch_bytes < s.used) return CB_ERR_WORKSPACE;
+  const bool wide = aligned_to(g, 16) && aligned_to(dtable, 16) && d * size % 16 == 0 && ldg * size % 16 == 0;
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const dim3 grid((unsigned)ceil_div(V, kThreads / 32), (unsigned)ceil_div(d, 32));
-    embedding_grad_kernel<T><<<grid, kThreads, 0, (cudaStream_t)stream>>>(static_cast<const T*>(g), ldg, Ids{ids, ids_64},
-                                                                          n, V, d, scale, static_cast<T*>(dtable));
-    return launched();
+    auto go = [&](auto vec) {
+      return grad<T, decltype(vec)::value>(static_cast<const T*>(g), ldg, Ids{ids, ids_64}, n, V, d, scale,
+                                           static_cast<T*>(dtable), s, (cudaStream_t)stream);
+    };
+    return wide ? go(std::integral_constant<int, 16 / sizeof(T)>{}) : go(std::integral_constant<int, 1>{});
   });
 }

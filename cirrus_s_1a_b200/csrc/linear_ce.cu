@@ -41,7 +41,7 @@ constexpr int kOutBytes = 128 * 128;  // a box on its way out: 128 rows of 128 b
 constexpr int kSmem = kStages * kStageBytes + 2 * kOutBytes + 1024;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = kEpiWarps * 32 + 64;
-constexpr int kMaxPasses = 6;
+constexpr int kMaxPasses = 6, kMaxPairs = 128;
 // Sums in tensor memory are cut off, not rounded, after every 16 products: over 48 of them a
 // row's lse was 5e-7 off, over 1500 the gradients 4e-5.  So a span of K is added up there,
 // and the spans in registers, rounded: 1024 of K, or 256 where float32 parts are multiplied.
@@ -63,15 +63,17 @@ struct alignas(64) Gemm {
   int m_tiles, n_tiles, k_steps;   // k_steps of a pass
   int span;                        // steps of K that are added up in tensor memory
   int splits;                      // of K, each with an output of its own
-  int out_f32, out_mode;
+  int out_f32, out_mode, split_mode;  // of the first split and of the others
   int out_rows;                    // between the splits' outputs
   const float* scale;              // the output's, in memory (PRODUCTS; null: none), times scale_by
   float scale_by;
 };
 
 struct alignas(64) Args {
-  Gemm g[2];
-  int n1, n2, extra, pairs;        // PRODUCTS: items of g[0] and of g[1] (see item_of)
+  Gemm g[2];                       // STATS, GRAD: one; PRODUCTS: dW, dh
+  int pairs;
+  int whole;                       // PRODUCTS: items of dW, dealt in turn
+  int from[kMaxPairs + 1];         // and where each pair's steps of dh begin
   uint32_t kind;                   // instruction descriptor without sizes and directions
   int tile_n;                      // STATS, GRAD
   // STATS and GRAD: rows, vocabulary rows, the vocabulary row that the tiles start at, and how many
@@ -261,9 +263,10 @@ struct Item {
   int tile;                               // along n
 };
 
-// The i-th tile of a pair.  STATS and GRAD: a run of equal length of all tiles, rows after
-// rows of tiles.  PRODUCTS: items of g[0], the longer ones, are dealt in turn; the pairs that
-// get one less take `extra` items of g[1] in its place, and the rest are dealt in turn.
+// The i-th item of a pair.  STATS and GRAD: a run of equal length of all tiles, rows after
+// rows of tiles.  PRODUCTS: tiles of dW (or splits of them), dealt in turn, and then a run of
+// all steps of all tiles of dh, as long as what it takes for all pairs to end together; a
+// tile that lies in several runs has its sum in parts, in slots of their own.
 template <int MODE>
 __device__ __forceinline__ bool item_of(const Args& p, int pair, int i, Item& it) {
   if (MODE != PRODUCTS) {
@@ -280,33 +283,29 @@ __device__ __forceinline__ bool item_of(const Args& p, int pair, int i, Item& it
     it.split = 0;
     return true;
   }
-  const int odd = p.n1 % p.pairs;  // pairs with one item of g[0] more than the others
-  const int longs = (p.n1 - pair + p.pairs - 1) / p.pairs;
-  int idx;
-  if (i < longs) {
-    idx = pair + i * p.pairs;
-  } else {
-    i -= longs;
-    int mine = 0;
-    if (pair >= odd && p.extra > pair - odd) mine = (p.extra - (pair - odd) + p.pairs - odd - 1) / (p.pairs - odd);
-    if (i < mine) {
-      idx = p.n1 + (pair - odd) + i * (p.pairs - odd);
-    } else {
-      const int at = p.extra + (pair - odd + p.pairs) % p.pairs + (i - mine) * p.pairs;
-      if (at >= p.n2) return false;
-      idx = p.n1 + at;
-    }
-  }
-  it.gemm = idx >= p.n1;
+  const int mine = (p.whole - pair + p.pairs - 1) / p.pairs;
+  it.gemm = i >= mine;
   const Gemm& g = p.g[it.gemm];
-  if (it.gemm) idx -= p.n1;
-  it.split = idx % g.splits;
-  idx /= g.splits;
-  it.tile = idx % g.n_tiles;
+  int tile;
+  if (!it.gemm) {
+    const int idx = pair + i * p.pairs;
+    it.split = idx % g.splits;
+    tile = idx / g.splits;
+    it.first = (int)((int64_t)g.k_steps * it.split / g.splits);
+    it.steps = (int)((int64_t)g.k_steps * (it.split + 1) / g.splits) - it.first;
+  } else {
+    const int begin = p.from[pair], end = p.from[pair + 1];
+    tile = begin / max(g.k_steps, 1) + i - mine;
+    const int tile_at = tile * g.k_steps, at = max(begin, tile_at);
+    if (at >= end) return false;
+    it.first = at - tile_at;
+    it.steps = min(end, tile_at + g.k_steps) - at;
+    it.split = 0;
+    for (int c = pair; p.from[c] > tile_at && at == begin; --c) it.split += p.from[c] > p.from[c - 1];
+  }
+  it.tile = tile % g.n_tiles;
   it.n0 = it.tile * kTileN;
-  it.m0 = idx / g.n_tiles * kTileM;
-  it.first = (int)((int64_t)g.k_steps * it.split / g.splits);
-  it.steps = (int)((int64_t)g.k_steps * (it.split + 1) / g.splits) - it.first;
+  it.m0 = tile / g.n_tiles * kTileM;
   return true;
 }
 
@@ -546,7 +545,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         if (g.out_f32) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            send(&g.out, v + c * 32, y, g.out_mode, [&](int j) { return __float_as_uint(x[c * 32 + j]); });
+            send(&g.out, v + c * 32, y, it.split ? g.split_mode : g.out_mode, [&](int j) { return __float_as_uint(x[c * 32 + j]); });
         } else {
 #pragma unroll
           for (int c = 0; c < 2; ++c)
@@ -852,39 +851,55 @@ int passes_of(int a_parts, int b_parts, int a_cols, int b_cols, Gemm& g) {
   return g.passes;
 }
 
-struct Split {
-  int h, w;        // of K of the two products
-  int extra;       // see item_of
-  bool dh_first;   // the longer items
+// How the two products are dealt: dW's tiles split `w` times along K, and the steps of dh
+// that go to each pair.
+struct Deal {
+  int w, h_slots;
+  int from[kMaxPairs + 1];
 };
 
-// How K of the two products is split over the pairs: the split whose longest pair ends
-// first, counted in steps of K, with what a tile costs beside them and what the splits'
-// results cost in memory.
-Split split_of(int pairs, int h_tiles, int h_steps, int w_tiles, int w_steps, int passes_h, int passes_w, double h_bytes,
-               double w_bytes, int h_most, int w_most) {
+// dh's steps fill what dW's items, dealt in turn, leave of a common end.
+double fill(Deal& o, int pairs, int items, double cost, int64_t steps, int step_cost, int k_steps) {
+  const int odd = items % pairs, low = items / pairs;  // `odd` pairs have one item more
+  const double work = (double)steps * step_cost;
+  double end = low * cost + work / (pairs - odd);  // if only the others get steps
+  if (end > (low + 1) * cost || odd == 0) end = (items * cost + work) / pairs;
+  const double most = std::max(end, items ? (low + (odd > 0)) * cost : 0.0);
+  double sum = 0.0;
+  for (int c = 0; c <= pairs; ++c) {
+    o.from[c] = c == pairs ? (int)steps : (int)std::min((double)steps, sum / step_cost);
+    sum += std::max(0.0, end - (low + (c < odd)) * cost);
+  }
+  // the most parts that a tile of dh lies in
+  o.h_slots = 1;
+  for (int c = 0, parts = 1; c < pairs && steps; ++c) {
+    if (o.from[c] == o.from[c + 1]) continue;
+    parts = o.from[c] % k_steps == 0 ? 1 : parts + 1;
+    o.h_slots = std::max(o.h_slots, parts);
+    if (o.from[c + 1] / k_steps > o.from[c] / k_steps) parts = 1;
+  }
+  return most;
+}
+
+// dW's split is the one whose pairs end first, counted in steps of K, with what a tile costs
+// beside them and what the splits' float32 results cost in memory.
+Deal deal(int pairs, int h_tiles, int h_steps, int h_passes, int w_tiles, int w_steps, int w_passes, double w_bytes,
+          int w_most) {
   constexpr int kTileCost = 6;             // of filling and emptying, in steps
   constexpr double kBytesPerStep = 900e3;  // written and read back in a step's time by the whole device
-  Split best{1, 1, 0, true};
+  Deal best{}, o{};
   double least = 1e30;
-  for (int sh = 1; sh <= 32 && sh <= h_steps && sh <= h_most; sh *= 2)
-    for (int sw = 1; sw <= 32 && sw <= w_steps && sw <= w_most; sw *= 2) {
-      const double lh = (double)h_steps * passes_h / sh + kTileCost, lw = (double)w_steps * passes_w / sw + kTileCost;
-      const int nh = h_tiles * sh, nw = w_tiles * sw;
-      const bool first = nw == 0 || (nh > 0 && lh >= lw);
-      const int n1 = first ? nh : nw, n2 = first ? nw : nh;
-      const double l1 = first ? lh : lw, l2 = first ? lw : lh;
-      const int odd = n1 % pairs, extra = odd ? (int)std::min<int64_t>(n2, (int64_t)(pairs - odd) * (int)(l1 / l2)) : 0;
-      const double a = (n1 / pairs + (odd > 0)) * l1, b = (n1 / pairs) * l1 + (odd ? ceil_div(extra, pairs - odd) * l2 : 0.0);
-      double t = std::max(a, b) + ceil_div(n2 - extra, pairs) * l2;
-      if (nh) t += sh * h_bytes / kBytesPerStep;
-      if (nw && sw > 1) t += sw * w_bytes / kBytesPerStep;
-      if (t < least * 0.999) {
-        least = t;
-        best = Split{sh, sw, extra, first};
-      }
-      if (w_tiles == 0) break;
+  for (int w = 1; w <= 64 && w <= w_steps && w <= w_most; w *= 2) {
+    o.w = w;
+    double t = fill(o, pairs, w_tiles * w, (double)w_steps * w_passes / w + kTileCost, (int64_t)h_tiles * h_steps, h_passes,
+                    std::max(h_steps, 1));
+    if (w > 1) t += w * w_bytes / kBytesPerStep;
+    if (t < least * 0.99) {
+      least = t;
+      best = o;
     }
+    if (w_tiles == 0) break;
+  }
   return best;
 }
 
@@ -901,20 +916,20 @@ struct Shape {
     g_parts = h_parts;
     f16 = h_dtype == CB_F16;
     type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    pairs = std::max(1, num_sms() / 2);
+    pairs = std::min(std::max(1, num_sms() / 2), kMaxPairs);
     piece = piece_of(N, V, g_parts);
   }
   uint32_t kind() const { return 1u << 4 | (f16 ? 0u : 1u << 7 | 1u << 10); }
   int da() const { return (int)up(d, 4); }  // columns of a float32 result
 };
 
-// The splits of a piece; those of the first, the largest, are what scratch is laid out for.
-Split splits(const Shape& s, bool dh, bool dw, int vp, int h_most, int w_most) {
+// How a piece is dealt; scratch is laid out for the first, the largest.
+Deal deal_of(const Shape& s, bool dh, bool dw, int vp, int w_most) {
   Gemm t;
   const int nt = ceil_div(s.d, kTileN);
-  return split_of(s.pairs, dh ? ceil_div(s.N, kTileM) * nt : 0, ceil_div(vp, kStep), dw ? ceil_div(vp, kTileM) * nt : 0,
-                  ceil_div(s.N, kStep), passes_of(s.g_parts, s.w_parts, 0, 0, t), passes_of(s.g_parts, s.h_parts, 0, 0, t),
-                  2.0 * s.N * s.d * 4, 2.0 * vp * s.d * 4, h_most, w_most);
+  return deal(s.pairs, dh ? ceil_div(s.N, kTileM) * nt : 0, ceil_div(vp, kStep), passes_of(s.g_parts, s.w_parts, 0, 0, t),
+              dw ? ceil_div(vp, kTileM) * nt : 0, ceil_div(s.N, kStep), passes_of(s.g_parts, s.h_parts, 0, 0, t),
+              2.0 * vp * s.d * 4, w_most);
 }
 
 // Scratch, part by part; `at` null only counts.
@@ -965,20 +980,22 @@ struct Backward {
   float* top;
   uint16_t *h, *hs, *w, *G;
   float *acc, *dw;
-  Split split;
-  int dw_direct;
+  Deal first;
+  int h_slots, dw_direct;
   Backward(Layout& a, const Shape& s, bool w_direct, bool want_h, bool want_w, bool dw_aligned) {
     const int vp = std::min(s.piece, s.V);
-    split = splits(s, want_h, want_w, vp, 32, 32);
-    dw_direct = dw_aligned && split.w == 1;
+    first = deal_of(s, want_h, want_w, vp, 64);
+    dw_direct = dw_aligned && first.w == 1;
+    h_slots = first.h_slots;
+    if (s.V % s.piece) h_slots = std::max(h_slots, deal_of(s, want_h, want_w, s.V % s.piece, first.w).h_slots);
     rows = a.take<float4>(s.N);
     top = a.take<float>(1);
     h = a.take<uint16_t>((int64_t)s.N * s.h_parts * s.dp);
     hs = s.f16 && want_w ? a.take<uint16_t>((int64_t)s.N * s.dp) : h;
     w = w_direct ? nullptr : a.take<uint16_t>((int64_t)s.V * s.w_parts * s.dp);
     G = a.take<uint16_t>((int64_t)s.N * s.g_parts * up(vp, kStep));
-    acc = want_h ? a.take<float>((int64_t)split.h * up(s.N, kTileM) * s.da()) : nullptr;
-    dw = want_w && !dw_direct ? a.take<float>((int64_t)split.w * up(vp, kTileM) * s.da()) : nullptr;
+    acc = want_h ? a.take<float>((int64_t)h_slots * up(s.N, kTileM) * s.da()) : nullptr;
+    dw = want_w && !dw_direct ? a.take<float>((int64_t)first.w * up(vp, kTileM) * s.da()) : nullptr;
   }
 };
 
@@ -1141,6 +1158,9 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   r.kind = q.kind;
   r.is_f16 = s.f16;
   r.status = status;
+  const int64_t slot = up(N, kTileM) * s.da();  // floats of one of dh's
+  if (dh && f.h_slots > 1 && cudaMemsetAsync(f.acc + slot, 0, (f.h_slots - 1) * slot * sizeof(float), st) != cudaSuccess)
+    return CB_ERR_CUDA;
   for (int v0 = 0; v0 < V; v0 += s.piece) {
     const int vp = std::min(s.piece, V - v0), cols = (int)up(vp, kStep);
     const int64_t g_ld = (int64_t)s.g_parts * cols;
@@ -1152,14 +1172,14 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
     q.pairs = (int)std::min<int64_t>(s.pairs, (int64_t)m_tiles * g.n_tiles);
     if (int rc = launch<GRAD>(q, st)) return rc;
 
-    const Split sp = v0 ? splits(s, dh != nullptr, dw != nullptr, vp, f.split.h, f.split.w) : f.split;
-    Gemm& gh = r.g[sp.dh_first ? 0 : 1];
-    Gemm& gw = r.g[sp.dh_first ? 1 : 0];
+    const Deal sp = vp == std::min(s.piece, V) ? f.first : deal_of(s, dh != nullptr, dw != nullptr, vp, f.first.w);
+    Gemm &gw = r.g[0], &gh = r.g[1];
     gh = gw = Gemm{};
-    int nh = 0, nw = 0;
+    r.whole = 0;
+    std::copy(sp.from, sp.from + kMaxPairs + 1, r.from);
     if (dh) {
       if (!map_of(&gh.a, f.G, s.type, N, g_ld, g_ld, 128) || !map_of(&gh.b, wo.at, s.type, V, wo.cols, wo.ld, 64) ||
-          !map_of(&gh.out, f.acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.split.h * up(N, kTileM), s.da(), s.da(), 128))
+          !map_of(&gh.out, f.acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.h_slots * up(N, kTileM), s.da(), s.da(), 128))
         return CB_ERR_CUDA;
       passes_of(s.g_parts, s.w_parts, cols, s.dp, gh);
       gh.b_mn = 1;
@@ -1167,11 +1187,10 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
       gh.m_tiles = m_tiles;
       gh.n_tiles = nt;
       gh.k_steps = cols / kStep;
-      gh.splits = sp.h;
       gh.out_f32 = 1;
       gh.out_mode = v0 ? OUT_ADD : OUT_STORE;
+      gh.split_mode = OUT_ADD;
       gh.out_rows = (int)up(N, kTileM);
-      nh = m_tiles * nt * sp.h;
     }
     if (dw) {
       if (!map_of(&gw.a, f.G, s.type, N, g_ld, g_ld, 64) ||
@@ -1181,7 +1200,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
           f.dw_direct
               ? map_of(&gw.out, static_cast<char*>(dw) + (int64_t)v0 * d * dtype_size(w_dtype),
                        w_dtype == CB_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : s.type, vp, d, d, 128)
-              : map_of(&gw.out, f.dw, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.split.w * up(std::min(s.piece, V), kTileM), s.da(),
+              : map_of(&gw.out, f.dw, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.first.w * up(std::min(s.piece, V), kTileM), s.da(),
                        s.da(), 128);
       if (!ok) return CB_ERR_CUDA;
       passes_of(s.g_parts, s.h_parts, cols, s.dp, gw);
@@ -1196,12 +1215,9 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
         gw.scale = f.top;
         gw.scale_by = s.f16 ? 1.0f / (1 << kF16Shift) : 1.0f;
       }
-      nw = gw.m_tiles * nt * sp.w;
+      r.whole = gw.m_tiles * nt * sp.w;
     }
-    r.n1 = sp.dh_first ? nh : nw;
-    r.n2 = sp.dh_first ? nw : nh;
-    r.pairs = std::min(s.pairs, r.n1 + r.n2);
-    r.extra = r.pairs == s.pairs ? sp.extra : 0;
+    r.pairs = s.pairs;
     if (int rc = launch<PRODUCTS>(r, st)) return rc;
     if (dw && !f.dw_direct)
       if (int rc = with_type(w_dtype, [&](auto t) {
@@ -1214,6 +1230,6 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   if (!dh) return CB_OK;
   return with_type(h_dtype, [&](auto t) {
     using T = decltype(t);
-    return finish<T>(f.acc, f.split.h, up(N, kTileM), s, N, f.rows, f.top, static_cast<T*>(dh), st);
+    return finish<T>(f.acc, f.h_slots, up(N, kTileM), s, N, f.rows, f.top, static_cast<T*>(dh), st);
   });
 }
