@@ -34,26 +34,37 @@ struct alignas(sizeof(T) * VEC) Vec {
   T v[VEC];
 };
 
+constexpr int kPieces = 4;  // of a thread, in flight together
+
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) embedding_kernel(const T* table, int64_t ld, int V, int vecs, Ids ids,
                                                              int64_t all, float scale, T* out, int32_t* status) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= all) return;
-  const int64_t n = i / vecs;
-  const int j = (int)(i - n * vecs);
-  const int64_t id = ids[n];
-  Vec<T, VEC> x;
-  if (id >= 0 && id < V) {
-    x = *reinterpret_cast<const Vec<T, VEC>*>(table + id * ld + j * VEC);
+  const int64_t first = (int64_t)blockIdx.x * (kPieces * kThreads) + threadIdx.x;
+  Vec<T, VEC> x[kPieces];
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p) {
+    const int64_t i = first + p * kThreads;
+    if (i >= all) break;
+    const int64_t n = all < (1ll << 31) ? (int64_t)((uint32_t)i / (uint32_t)vecs) : i / vecs;
+    const int j = (int)(i - n * vecs);
+    const int64_t id = ids[n];
+    if (id >= 0 && id < V) {
+      x[p] = *reinterpret_cast<const Vec<T, VEC>*>(table + id * ld + j * VEC);
+    } else {
+      if (id >= V && j == 0) set_status(status, CB_ERR_TOKEN);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[p].v[k] = Elem<T>::put(0.0f);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p) {
+    const int64_t i = first + p * kThreads;
+    if (i >= all) break;
     if (scale != 1.0f)
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x.v[k] = Elem<T>::put(Elem<T>::get(x.v[k]) * scale);
-  } else {
-    if (id >= V && j == 0) set_status(status, CB_ERR_TOKEN);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) x.v[k] = Elem<T>::put(0.0f);
+      for (int k = 0; k < VEC; ++k) x[p].v[k] = Elem<T>::put(Elem<T>::get(x[p].v[k]) * scale);
+    *reinterpret_cast<Vec<T, VEC>*>(out + i * VEC) = x[p];
   }
-  *reinterpret_cast<Vec<T, VEC>*>(out + i * VEC) = x;
 }
 
 // ------------------------------------------------------------------- sort
@@ -120,11 +131,16 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(Ids ids, int64_t fir
     cluster_sync();
     uint32_t before = 0, all = 0, scan = 0;
     if (tid < 256) {
-      for (int r = 0; r < ctas; ++r) {
-        uint32_t c;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(at_rank(&s.total[tid], r)));
-        before += r < rank ? c : 0;
-        all += c;
+      uint32_t c[kMaxCluster];
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        c[r] = 0;
+        if (r < ctas) asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c[r]) : "r"(at_rank(&s.total[tid], r)));
+      }
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        before += r < rank ? c[r] : 0;
+        all += c[r];
       }
       scan = all;
       for (int o = 1; o < 32; o <<= 1) {
@@ -244,6 +260,17 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const T* g, int64_t ldg, 
   }
 }
 
+template <int VEC>
+__device__ __forceinline__ void load_sum(const float* at, float (&x)[VEC]) {
+  constexpr int kN = VEC < 4 ? VEC : 4;
+#pragma unroll
+  for (int i = 0; i < VEC; i += kN) {
+    const Vec<float, kN> v = *reinterpret_cast<const Vec<float, kN>*>(at + i);
+#pragma unroll
+    for (int k = 0; k < kN; ++k) x[i + k] = v.v[k];
+  }
+}
+
 // A warp to 512 bytes of columns of a chunk whose last row goes on: the row's parts in order.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) join_kernel(const uint32_t* keys, int n, int V, int d, int slabs, float scale,
@@ -252,32 +279,31 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const uint32_t* keys, in
   const int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   const int chunk = (int)(w / slabs), j = ((int)(w % slabs) * 32 + lane) * VEC;
   const int end = (chunk + 1) * kChunk;
-  if (end >= n || j >= d) return;
+  if (end >= n) return;
   const uint32_t key = keys[end - 1];
   if (key >= (uint32_t)V || keys[end] != key) return;
   const int first = chunk * kChunk;
   if (keys[first] == key && first > 0 && keys[first - 1] == key) return;  // it began before
   float sum[VEC];
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) sum[k] = part[((int64_t)chunk * 2 + 1) * d + j + k];
+  if (j < d) load_sum<VEC>(part + ((int64_t)chunk * 2 + 1) * d + j, sum);
   constexpr int kAhead = 8;
-  for (int64_t c = chunk + 1; c * kChunk < n && keys[c * kChunk] == key; c += kAhead) {
-    float x[kAhead][VEC];
-    bool is[kAhead];
+  for (int c = chunk + 1, more = 32; more == 32; c += 32) {
+    // how many of the next 32 chunks begin with the row
+    const int at = c + lane;
+    more = __popc(__ballot_sync(0xffffffffu, (int64_t)at * kChunk < n && keys[at * kChunk] == key));
+    for (int i0 = 0; i0 < more; i0 += kAhead) {
+      float x[kAhead][VEC];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      is[i] = (c + i) * kChunk < n && keys[(c + i) * kChunk] == key;
-      if (is[i])
+      for (int i = 0; i < kAhead; ++i)
+        if (i0 + i < more && j < d) load_sum<VEC>(part + (int64_t)(c + i0 + i) * 2 * d + j, x[i]);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) x[i][k] = part[(c + i) * 2 * d + j + k];
+      for (int i = 0; i < kAhead; ++i)
+        if (i0 + i < more)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) sum[k] += x[i][k];
     }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-      if (is[i])
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) sum[k] += x[i][k];
   }
-  write_row<T, VEC>(dtable, total, (int64_t)key * d + j, sum, scale);
+  if (j < d) write_row<T, VEC>(dtable, total, (int64_t)key * d + j, sum, scale);
 }
 
 // The batches' sums in the table's type.
@@ -372,7 +398,7 @@ extern "C" int cb_embedding(const void* table, int32_t dtype, int64_t ld, int32_
     auto go = [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
       const int64_t all = n * (d / VEC);
-      embedding_kernel<T, VEC><<<(unsigned)((all + kThreads - 1) / kThreads), kThreads, 0, (cudaStream_t)stream>>>(
+      embedding_kernel<T, VEC><<<(unsigned)((all + kPieces * kThreads - 1) / (kPieces * kThreads)), kThreads, 0, (cudaStream_t)stream>>>(
           static_cast<const T*>(table), ld, V, d / VEC, Ids{ids, ids_64}, all, scale, static_cast<T*>(out), status);
       return launched();
     };

@@ -3,15 +3,172 @@
 //   y = x r w, r = (mean x^2 + eps)^-1/2
 //   dx = r (g w - x r mean(g w x r))          dw = sum over rows of g x r
 //
-// Bound by memory.  Sums are float32; dw is summed over fixed groups of rows, then over
-// the groups, so that its order does not depend on timing.
+// Bound by memory: a row is read once and held in a warp's registers while its sums are
+// taken.  The gradient's warps go through rows in turn and add their part of dw up as they
+// do; the parts of a CTA's warps, then of the CTAs, are added in order, so that the sum does
+// not depend on timing.  Rows that do not fit (more than 2048 columns) or are not 16-byte
+// aligned are taken by a CTA each, read twice, with dw over fixed groups of rows.
+#include <algorithm>
+#include <type_traits>
+
 #include "ends.cuh"
 
 namespace cb {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kGroup = 64;  // rows whose part of dw one CTA sums
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kGroup = 64;  // rows whose part of dw one CTA sums (rows taken by CTAs)
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Vec {
+  T v[VEC];
+};
+// A thread's elements of w beside VEC of x.
+template <typename W, int VEC>
+__device__ __forceinline__ void load_w(const W* w, float (&o)[VEC]) {
+  constexpr int kN = std::min(VEC, 16 / (int)sizeof(W));
+#pragma unroll
+  for (int i = 0; i < VEC; i += kN) {
+    const Vec<W, kN> v = *reinterpret_cast<const Vec<W, kN>*>(w + i);
+#pragma unroll
+    for (int k = 0; k < kN; ++k) o[i + k] = Elem<W>::get(v.v[k]);
+  }
+}
+
+// A warp to a row: NV pieces of 16 bytes a lane.
+template <typename T, typename W, int NV>
+__global__ void __launch_bounds__(kThreads) rms_norm_warp_kernel(const T* x, int64_t ld, const W* w, int rows, int d,
+                                                                 float eps, T* y) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, n = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (n >= rows) return;
+  Vec<T, VEC> v[NV];
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = (i * 32 + lane) * VEC;
+    if (j < d) v[i] = *reinterpret_cast<const Vec<T, VEC>*>(x + n * ld + j);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if ((i * 32 + lane) * VEC < d)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s += Elem<T>::get(v[i].v[k]) * Elem<T>::get(v[i].v[k]);
+  const float r = rsqrtf(warp_sum(s) / d + eps);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = (i * 32 + lane) * VEC;
+    if (j >= d) continue;
+    float u[VEC];
+    load_w<W, VEC>(w + j, u);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[i].v[k] = Elem<T>::put(Elem<T>::get(v[i].v[k]) * r * u[k]);
+    *reinterpret_cast<Vec<T, VEC>*>(y + (int64_t)n * d + j) = v[i];
+  }
+}
+
+// part[cta][d], or dw itself where there is one CTA.
+template <typename T, typename W, int NV>
+__global__ void __launch_bounds__(kThreads) rms_norm_grad_warp_kernel(const T* x, int64_t ld, const T* g, int64_t ldg,
+                                                                      const W* w, int rows, int d, float eps, T* dx,
+                                                                      float* part, W* dw) {
+  constexpr int VEC = 16 / sizeof(T);
+  constexpr int kWide = NV * VEC * 32;   // columns of NV pieces a lane, d of them or more
+  __shared__ float s_part[kWarps / 2][kWide];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float acc[NV][VEC] = {};
+  for (int n = blockIdx.x * kWarps + warp; n < rows; n += gridDim.x * kWarps) {
+    Vec<T, VEC> v[NV], up[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * 32 + lane) * VEC;
+      if (j < d) {
+        v[i] = *reinterpret_cast<const Vec<T, VEC>*>(x + n * ld + j);
+        up[i] = *reinterpret_cast<const Vec<T, VEC>*>(g + n * ldg + j);
+      }
+    }
+    float s = 0.0f, c = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * 32 + lane) * VEC;
+      if (j >= d) continue;
+      float u[VEC];
+      load_w<W, VEC>(w + j, u);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float a = Elem<T>::get(v[i].v[k]);
+        s += a * a;
+        c += Elem<T>::get(up[i].v[k]) * u[k] * a;
+      }
+    }
+    const float r = rsqrtf(warp_sum(s) / d + eps);
+    const float m = warp_sum(c) * r / d * r;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * 32 + lane) * VEC;
+      if (j >= d) continue;
+      float u[VEC];
+      load_w<W, VEC>(w + j, u);
+      Vec<T, VEC> o;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float a = Elem<T>::get(v[i].v[k]), b = Elem<T>::get(up[i].v[k]);
+        o.v[k] = Elem<T>::put(r * (b * u[k] - a * m));
+        acc[i][k] += b * (a * r);
+      }
+      *reinterpret_cast<Vec<T, VEC>*>(dx + (int64_t)n * d + j) = o;
+    }
+  }
+  // the warps' parts, halved until one is left
+  for (int half = kWarps / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (warp >= half && warp < 2 * half)
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          s_part[warp - half][(i * VEC + k) * 32 + lane] = acc[i][k];
+    __syncthreads();
+    if (warp < half)
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          acc[i][k] += s_part[warp][(i * VEC + k) * 32 + lane];
+  }
+  if (warp > 0) return;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const int j = (i * 32 + lane) * VEC + k;
+      if (j >= d) continue;
+      if (gridDim.x == 1) dw[j] = Elem<W>::put(acc[i][k]);
+      else part[(int64_t)blockIdx.x * d + j] = acc[i][k];
+    }
+}
+
+// dw = the sum of `parts` rows: 32 columns a CTA, its warps' sums added in order.
+template <typename W>
+__global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* part, int parts, int d, W* dw) {
+  __shared__ float s_sum[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
+  float s[4] = {};
+  if (j < d) {
+    int i = warp;
+    for (; i + 96 < parts; i += 128)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[k] += part[(int64_t)(i + 32 * k) * d + j];
+    for (; i < parts; i += 32) s[0] += part[(int64_t)i * d + j];
+  }
+  s_sum[warp][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (warp == 0 && j < d) {
+    float t = 0.0f;
+    for (int k = 0; k < 32; ++k) t += s_sum[k][lane];
+    dw[j] = Elem<W>::put(t);
+  }
+}
 
 template <typename T, typename W>
 __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const T* x, int64_t ld, const W* w, int d, float eps, T* y) {
@@ -59,14 +216,27 @@ __global__ void __launch_bounds__(kThreads) rms_norm_dw_part_kernel(const T* x, 
   part[(int64_t)blockIdx.x * d + j] = s;
 }
 
-template <typename W>
-__global__ void __launch_bounds__(kThreads) rms_norm_dw_kernel(const float* part, int parts, int d, W* dw) {
-  const int j = blockIdx.x * kThreads + threadIdx.x;
-  if (j >= d) return;
-  float s = 0.0f;
-  for (int64_t i = 0; i < parts; ++i) s += part[i * d + j];
-  dw[j] = Elem<W>::put(s);
+// f(number of 16-byte pieces a lane) for rows of d columns.
+template <typename T, typename F>
+int with_pieces(int d, F&& f) {
+  const int n = ceil_div(d, 32 * 16 / (int)sizeof(T));
+  if (n <= 1) return f(std::integral_constant<int, 1>{});
+  if (n <= 2) return f(std::integral_constant<int, 2>{});
+  if (n <= 3) return f(std::integral_constant<int, 3>{});
+  if (n <= 4) return f(std::integral_constant<int, 4>{});
+  if (n <= 6) return f(std::integral_constant<int, 6>{});
+  if (n <= 8 || sizeof(T) == 2) return f(std::integral_constant<int, 8>{});
+  return f(std::integral_constant<int, sizeof(T) == 4 ? 16 : 8>{});
 }
+
+// Whether a warp can hold a row: 16-byte pieces, 2048 columns.
+bool in_a_warp(const void* x, int64_t ld, int rows, int d, int size) {
+  return d <= 2048 && d * size % 16 == 0 && aligned_to(x, 16) && (rows == 1 || ld * size % 16 == 0);
+}
+
+// CTAs of the gradient's warps: 16 rows or fewer to one (dw then needs no second kernel), at
+// most three to an SM.
+int grad_ctas(int rows) { return rows <= 2 * kWarps ? 1 : std::min(ceil_div(rows, kWarps), 3 * num_sms()); }
 
 template <typename F>
 int with_types(int32_t dtype, int32_t w_dtype, F&& f) {
@@ -87,19 +257,28 @@ extern "C" int cb_rms_norm(const void* x, int32_t dtype, int64_t ld, const void*
                            int32_t d, float eps, void* y, void* stream) {
   if (bad(x, dtype, ld, w, w_dtype, rows, d) || !y || !aligned_to(y, dtype_size(dtype))) return CB_ERR_ARG;
   if (rows > CB_ENDS_MAX_ROWS || d > CB_ENDS_MAX_DIM) return CB_ERR_SHAPE;
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool warps = in_a_warp(x, ld, rows, d, dtype_size(dtype)) && aligned_to(y, 16) && aligned_to(w, 16);
   return with_types(dtype, w_dtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
-    rms_norm_kernel<T, W><<<rows, kThreads, 0, (cudaStream_t)stream>>>(static_cast<const T*>(x), ld,
-                                                                       static_cast<const W*>(w), d, eps,
-                                                                       static_cast<T*>(y));
-    return launched();
+    const T* in = static_cast<const T*>(x);
+    const W* weight = static_cast<const W*>(w);
+    if (!warps) {
+      rms_norm_kernel<T, W><<<rows, kThreads, 0, st>>>(in, ld, weight, d, eps, static_cast<T*>(y));
+      return launched();
+    }
+    return with_pieces<T>(d, [&](auto nv) {
+      rms_norm_warp_kernel<T, W, decltype(nv)::value><<<ceil_div(rows, kWarps), kThreads, 0, st>>>(
+          in, ld, weight, rows, d, eps, static_cast<T*>(y));
+      return launched();
+    });
   });
 }
 
 extern "C" size_t cb_rms_norm_grad_scratch_bytes(int32_t rows, int32_t d) {
   if (rows <= 0 || d <= 0 || rows > CB_ENDS_MAX_ROWS || d > CB_ENDS_MAX_DIM) return 0;
-  return ((size_t)rows + (size_t)ceil_div(rows, kGroup) * d) * sizeof(float);
+  return ((size_t)rows + (size_t)std::max(ceil_div(rows, kGroup), grad_ctas(rows)) * d) * sizeof(float);
 }
 
 extern "C" int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const void* g, int64_t ldg, const void* w,
@@ -113,19 +292,34 @@ extern "C" int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const 
   if (!need) return CB_ERR_SHAPE;
   if (scratch_bytes < need) return CB_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
+  const int size = dtype_size(dtype);
+  const bool warps = in_a_warp(x, ld, rows, d, size) && in_a_warp(g, ldg, rows, d, size) && aligned_to(dx, 16) &&
+                     aligned_to(w, 16);
   return with_types(dtype, w_dtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
+    const T *in = static_cast<const T*>(x), *up = static_cast<const T*>(g);
+    const W* weight = static_cast<const W*>(w);
     float* rstd = static_cast<float*>(scratch);
     float* part = rstd + rows;
-    const int parts = ceil_div(rows, kGroup);
-    rms_norm_dx_kernel<T, W><<<rows, kThreads, 0, st>>>(static_cast<const T*>(x), ld, static_cast<const T*>(g), ldg,
-                                                        static_cast<const W*>(w), d, eps, static_cast<T*>(dx), rstd);
-    if (int rc = launched()) return rc;
-    rms_norm_dw_part_kernel<T><<<dim3(parts, ceil_div(d, kThreads)), kThreads, 0, st>>>(
-        static_cast<const T*>(x), ld, static_cast<const T*>(g), ldg, rstd, rows, d, part);
-    if (int rc = launched()) return rc;
-    rms_norm_dw_kernel<W><<<ceil_div(d, kThreads), kThreads, 0, st>>>(part, parts, d, static_cast<W*>(dw));
+    int parts;
+    if (warps) {
+      part = rstd;
+      parts = grad_ctas(rows);
+      const int rc = with_pieces<T>(d, [&](auto nv) {
+        auto* fn = rms_norm_grad_warp_kernel<T, W, decltype(nv)::value>;
+        fn<<<parts, kThreads, 0, st>>>(in, ld, up, ldg, weight, rows, d, eps, static_cast<T*>(dx), part, static_cast<W*>(dw));
+        return launched();
+      });
+      if (rc || parts == 1) return rc;
+    } else {
+      parts = ceil_div(rows, kGroup);
+      rms_norm_dx_kernel<T, W><<<rows, kThreads, 0, st>>>(in, ld, up, ldg, weight, d, eps, static_cast<T*>(dx), rstd);
+      if (int rc = launched()) return rc;
+      rms_norm_dw_part_kernel<T><<<dim3(parts, ceil_div(d, kThreads)), kThreads, 0, st>>>(in, ld, up, ldg, rstd, rows, d, part);
+      if (int rc = launched()) return rc;
+    }
+    rms_norm_dw_kernel<W><<<ceil_div(d, 32), 1024, 0, st>>>(part, parts, d, static_cast<W*>(dw));
     return launched();
   });
 }
