@@ -6,7 +6,7 @@ from __future__ import annotations
 import torch
 
 from cirrus_s_1a_b200 import _lib
-from cirrus_s_1a_b200.kv8 import _dtype, current_device, raw_stream
+from cirrus_s_1a_b200.kv8 import DTYPES, current_device, raw_stream
 
 
 def matrix(t: torch.Tensor, name: str, device=None) -> tuple:
@@ -18,9 +18,13 @@ def matrix(t: torch.Tensor, name: str, device=None) -> tuple:
     R, D = t.shape
     if not 0 < D <= _lib.CB_ENDS_MAX_DIM or R > _lib.CB_ENDS_MAX_ROWS:
         raise ValueError(f"{name} must have 1 to {_lib.CB_ENDS_MAX_DIM} columns and at most {_lib.CB_ENDS_MAX_ROWS} rows")
-    if R and D > 1 and t.stride(1) != 1:
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
+    ld, step = t.stride()
+    if step != 1 and R and D > 1:
         raise ValueError(f"a row of {name} must be contiguous")
-    return R, D, t.stride(0) if R > 1 else D, _dtype(t, name)
+    return R, D, ld if R > 1 else D, code
 
 
 def vocabulary(t: torch.Tensor, name: str, device=None) -> tuple:
@@ -31,18 +35,24 @@ def vocabulary(t: torch.Tensor, name: str, device=None) -> tuple:
     return V, D, ld, code
 
 
-def upstream(g: torch.Tensor) -> torch.Tensor:
-    """A gradient as the kernels read it: rows of any distance (0 where it was expanded), contiguous in themselves."""
-    return g if g.stride(-1) == 1 or g.shape[-1] == 1 else g.contiguous()
+def upstream(g: torch.Tensor, D: int) -> tuple:
+    """A gradient [rows, D] as the kernels read it, and the elements between its rows (0
+    where one row was expanded); one whose rows are not contiguous is copied."""
+    ld, step = g.stride()
+    if step != 1 and D > 1:
+        g = g.contiguous()
+        ld = D
+    return g, ld if g.shape[0] > 1 else D
 
 
 def ids(t: torch.Tensor, name: str, device) -> int:
     """1 for int64 ids, 0 for int32."""
-    if t.dtype not in (torch.int64, torch.int32) or t.device != device or not t.is_contiguous():
+    wide = t.dtype == torch.int64
+    if not (wide or t.dtype == torch.int32) or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int64 or int32 ids on {device}")
     if t.numel() > _lib.CB_ENDS_MAX_ROWS:
         raise ValueError(f"at most {_lib.CB_ENDS_MAX_ROWS} {name}")
-    return int(t.dtype == torch.int64)
+    return int(wide)
 
 
 def status(t: torch.Tensor | None, device) -> int | None:
@@ -53,25 +63,40 @@ def status(t: torch.Tensor | None, device) -> int | None:
     return t.data_ptr()
 
 
-def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+def once() -> None:
+    """Called in a backward pass: what it returns has no gradient of its own."""
+    if torch.is_grad_enabled():  # only under create_graph
+        raise RuntimeError("the gradient of this operator is not differentiable (create_graph=True)")
+
+
+_fns: dict = {}
+_sizes: dict = {}
 
 
 def call(device, name: str, *args) -> None:
     """One entry point on ``device``'s current stream."""
-    fn = getattr(_lib.lib(), name)
-    if current_device() == device.index:
-        rc = fn(*args, raw_stream(device.index))
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_lib.lib(), name)
+    index = device.index
+    if current_device() == index:
+        rc = fn(*args, raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, raw_stream(device.index))
+            rc = fn(*args, raw_stream(index))
     if rc:
         _lib.check(rc, name)
 
 
-def scratch(device, name: str, *shape) -> torch.Tensor:
-    """Scratch of a call, from the stream's (or the capture's) own memory."""
-    n = getattr(_lib.lib(), name)(*shape)
-    if n == 0:
-        raise _lib.CbError(f"{name}: shape not supported")
+def scratch(device, name: str, key: tuple, *args) -> torch.Tensor:
+    """Scratch of a call, from the stream's (or the capture's) own memory; its size, which
+    ``args`` give, is looked up by ``key``."""
+    n = _sizes.get((name, key))
+    if n is None:
+        n = getattr(_lib.lib(), name)(*args)
+        if n == 0:
+            raise _lib.CbError(f"{name}: shape not supported")
+        if len(_sizes) >= 1024:  # a caller's rows may change with every call
+            _sizes.clear()
+        _sizes[(name, key)] = n
     return torch.empty(n, dtype=torch.uint8, device=device)

@@ -28,17 +28,13 @@ constexpr int64_t kBatch = (int64_t)kPerCta * kMaxCluster;
 constexpr int kChunk = 32;  // sorted tokens of a warp
 
 // ----------------------------------------------------------------- lookup
-// 16 bytes of a row to a thread, or one element where rows are not 16-byte aligned.
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Vec {
-  T v[VEC];
-};
-
 constexpr int kPieces = 4;  // of a thread, in flight together
 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) embedding_kernel(const T* table, int64_t ld, int V, int vecs, Ids ids,
                                                              int64_t all, float scale, T* out, int32_t* status) {
+  await_before();
+  start_next();
   const int64_t first = (int64_t)blockIdx.x * (kPieces * kThreads) + threadIdx.x;
   Vec<T, VEC> x[kPieces];
 #pragma unroll
@@ -91,6 +87,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(Ids ids, int64_t fir
   SortShared& s = *sort_shared;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x, ctas = gridDim.x;  // one cluster
+  await_before();
+  start_next();
   const int per = (n + ctas - 1) / ctas, mine = max(0, min(per, n - rank * per));
   // a warp's segment
   const int seg = ((per + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
@@ -195,6 +193,8 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const T* g, int64_t ldg, 
                                                        float* part) {
   const int lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  await_before();
+  start_next();
   const int chunks = (n + kChunk - 1) / kChunk;
   const int64_t sums = (int64_t)chunks * slabs;
   if (w >= sums) {
@@ -279,6 +279,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const uint32_t* keys, in
   const int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   const int chunk = (int)(w / slabs), j = ((int)(w % slabs) * 32 + lane) * VEC;
   const int end = (chunk + 1) * kChunk;
+  await_before();
+  start_next();
   if (end >= n) return;
   const uint32_t key = keys[end - 1];
   if (key >= (uint32_t)V || keys[end] != key) return;
@@ -309,6 +311,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const uint32_t* keys, in
 // The batches' sums in the table's type.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) scale_kernel(const float* total, int64_t all, float scale, T* dtable) {
+  await_before();
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kThreads)
     dtable[i] = Elem<T>::put(total[i] * scale);
 }
@@ -347,12 +350,14 @@ int launch_sort(Ids ids, int64_t first, int n, int V, const Scratch& s, cudaStre
   cfg.blockDim = dim3(kSortThreads);
   cfg.dynamicSmemBytes = sizeof(SortShared);
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = ctas;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, sort_kernel, ids, first, n, V, (bits + 7) / 8, s.keys, s.order) != cudaSuccess)
     return CB_ERR_CUDA;
   count_launch();
@@ -368,17 +373,16 @@ int grad(const T* g, int64_t ldg, Ids ids, int64_t n, int V, int d, float scale,
     if (int rc = launch_sort(ids, first, m, V, s, st)) return rc;
     const int64_t sums = (int64_t)ceil_div(m, kChunk) * slabs, warps = sums + (s.total ? 0 : ceil_div(V, 32));
     constexpr int kWarps = kThreads / 32;
-    sum_kernel<T, VEC><<<(unsigned)((warps + kWarps - 1) / kWarps), kThreads, 0, st>>>(
-        g + first * ldg, ldg, s.keys, s.order, m, V, d, slabs, scale, dtable, s.total, s.part);
-    if (int rc = launched()) return rc;
+    if (int rc = launch_after(sum_kernel<T, VEC>, dim3((unsigned)((warps + kWarps - 1) / kWarps)), kThreads, 0, st,
+                              g + first * ldg, ldg, s.keys, s.order, m, V, d, slabs, scale, dtable, s.total, s.part))
+      return rc;
     if (m <= kChunk) continue;
-    join_kernel<T, VEC><<<(unsigned)((sums + kWarps - 1) / kWarps), kThreads, 0, st>>>(s.keys, m, V, d, slabs, scale, dtable,
-                                                                                       s.total, s.part);
-    if (int rc = launched()) return rc;
+    if (int rc = launch_after(join_kernel<T, VEC>, dim3((unsigned)((sums + kWarps - 1) / kWarps)), kThreads, 0, st, s.keys, m,
+                              V, d, slabs, scale, dtable, s.total, s.part))
+      return rc;
   }
   if (!s.total) return CB_OK;
-  scale_kernel<T><<<8 * num_sms(), kThreads, 0, st>>>(s.total, (int64_t)V * d, scale, dtable);
-  return launched();
+  return launch_after(scale_kernel<T>, dim3(8 * num_sms()), kThreads, 0, st, s.total, (int64_t)V * d, scale, dtable);
 }
 
 }  // namespace
@@ -398,9 +402,9 @@ extern "C" int cb_embedding(const void* table, int32_t dtype, int64_t ld, int32_
     auto go = [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
       const int64_t all = n * (d / VEC);
-      embedding_kernel<T, VEC><<<(unsigned)((all + kPieces * kThreads - 1) / (kPieces * kThreads)), kThreads, 0, (cudaStream_t)stream>>>(
-          static_cast<const T*>(table), ld, V, d / VEC, Ids{ids, ids_64}, all, scale, static_cast<T*>(out), status);
-      return launched();
+      return launch_after(embedding_kernel<T, VEC>, dim3((unsigned)((all + kPieces * kThreads - 1) / (kPieces * kThreads))),
+                          kThreads, 0, (cudaStream_t)stream, static_cast<const T*>(table), ld, V, d / VEC, Ids{ids, ids_64},
+                          all, scale, static_cast<T*>(out), status);
     };
     return wide ? go(std::integral_constant<int, 16 / sizeof(T)>{}) : go(std::integral_constant<int, 1>{});
   });

@@ -349,11 +349,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
-  if (MODE == STATS && blockIdx.x == 0 && tid == 32) *p.counter = 0;
   fence_before();
   __syncthreads();
   cluster_sync();
   fence_after();
+  await_before();
+  start_next();
+  if (MODE == STATS && blockIdx.x == 0 && tid == 0) *p.counter = 0;
   const uint32_t tmem = s_tmem;
   volatile int* abort_flag = &s_abort;
   auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -645,64 +647,92 @@ __device__ __forceinline__ int64_t target_of(const Problem& p, int n) {
 
 constexpr int kRowThreads = 256;
 
-// Joins the runs' parts of a row's sum, a warp to a row; the last CTA adds the losses up.
+// Joins the runs' parts of a row's sum, LANES threads to a row (32 where few rows are in many
+// parts).  A reduced loss: the CTAs' sums, which the last CTA adds up in order.
+template <int LANES>
 __global__ void __launch_bounds__(kRowThreads) join_kernel(Problem p, int n_tiles, int m_tiles, int pairs, const float2* part,
                                                            const float* xt, float* rows, float* lse, int reduction,
-                                                           float* loss, int32_t* count, uint32_t* counter,
+                                                           float* loss, int32_t* count, double2* sums, uint32_t* counter,
                                                            int32_t* status) {
-  const int lane = threadIdx.x & 31, n = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
-  if (n < p.N) {
-    const int64_t all = (int64_t)m_tiles * n_tiles, from = (int64_t)(n / kTileM) * n_tiles;
-    const int parts = 2 * ((int)(((from + n_tiles) * pairs - 1) / all) - (int)(((from + 1) * pairs - 1) / all) + 1);
-    float m = -INFINITY, l = 0.0f;
-    for (int i = lane; i < parts; i += 32) {
-      const float2 q = part[(int64_t)i * p.N + n];
-      const float t = fmaxf(m, q.x), ref = t == -INFINITY ? 0.0f : t;
-      l = l * expf(m - ref) + q.y * expf(q.x - ref);
-      m = t;
+  __shared__ double s_sum[kRowThreads / 32], s_count[kRowThreads / 32];
+  __shared__ int s_last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = (blockIdx.x * kRowThreads + threadIdx.x) / LANES;
+  await_before();
+  start_next();
+  double sum = 0.0, has = 0.0;
+  const int64_t all = (int64_t)m_tiles * n_tiles, from = (int64_t)(n / kTileM) * n_tiles;
+  const int parts =
+      n < p.N ? 2 * ((int)(((from + n_tiles) * pairs - 1) / all) - (int)(((from + 1) * pairs - 1) / all) + 1) : 0;
+  float m = -INFINITY, l = 0.0f;
+  for (int i = threadIdx.x % LANES; i < parts; i += LANES) {
+    const float2 q = part[(int64_t)i * p.N + n];
+    const float t = fmaxf(m, q.x), ref = t == -INFINITY ? 0.0f : t;
+    l = l * expf(m - ref) + q.y * expf(q.x - ref);
+    m = t;
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    const float qm = __shfl_xor_sync(0xffffffffu, m, o), ql = __shfl_xor_sync(0xffffffffu, l, o);
+    const float t = fmaxf(m, qm), ref = t == -INFINITY ? 0.0f : t;
+    l = l * expf(m - ref) + ql * expf(qm - ref);
+    m = t;
+  }
+  if (n < p.N && threadIdx.x % LANES == 0) {
+    lse[n] = m + logf(l);
+    const int64_t t = p.targets[n];
+    float row = 0.0f;
+    if (t >= p.V) set_status(status, CB_ERR_TOKEN);
+    if (t >= 0 && t < p.V) {
+      row = (m - xt[n]) + logf(l);
+      sum = row;
+      has = 1.0;
     }
-    for (int o = 16; o > 0; o >>= 1) {
-      const float qm = __shfl_xor_sync(0xffffffffu, m, o), ql = __shfl_xor_sync(0xffffffffu, l, o);
-      const float t = fmaxf(m, qm), ref = t == -INFINITY ? 0.0f : t;
-      l = l * expf(m - ref) + ql * expf(qm - ref);
-      m = t;
-    }
-    if (lane == 0) {
-      lse[n] = m + logf(l);
-      rows[n] = target_of(p, n) >= 0 ? (m - xt[n]) + logf(l) : 0.0f;
-      if (p.targets[n] >= p.V) set_status(status, CB_ERR_TOKEN);
-    }
+    if (reduction == CB_REDUCE_NONE) rows[n] = row;
   }
   if (reduction == CB_REDUCE_NONE) return;
-  __shared__ int s_last;
-  __shared__ double s_sum[kRowThreads];
-  __shared__ int s_count[kRowThreads];
-  __syncthreads();
+  auto block_add = [&] {  // to thread 0
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      has += __shfl_xor_sync(0xffffffffu, has, o);
+    }
+    if (lane == 0) {
+      s_sum[warp] = sum;
+      s_count[warp] = has;
+    }
+    __syncthreads();
+    sum = has = 0.0;
+    if (threadIdx.x == 0)
+      for (int w = 0; w < kRowThreads / 32; ++w) {
+        sum += s_sum[w];
+        has += s_count[w];
+      }
+  };
+  block_add();
   if (threadIdx.x == 0) {
-    __threadfence();
-    s_last = atomicAdd(counter, 1u) == gridDim.x - 1;
+    if (gridDim.x > 1) {
+      sums[blockIdx.x] = make_double2(sum, has);
+      __threadfence();
+      s_last = atomicAdd(counter, 1u) == gridDim.x - 1;
+      __threadfence();
+    } else {
+      s_last = 1;
+    }
   }
   __syncthreads();
   if (!s_last) return;
-  __threadfence();
-  double sum = 0.0;
-  int has = 0;
-  for (int i = threadIdx.x; i < p.N; i += kRowThreads) {
-    sum += __ldcg(rows + i);
-    has += target_of(p, i) >= 0;
-  }
-  s_sum[threadIdx.x] = sum;
-  s_count[threadIdx.x] = has;
-  for (int o = kRowThreads / 2; o > 0; o >>= 1) {
-    __syncthreads();
-    if (threadIdx.x < o) {
-      s_sum[threadIdx.x] += s_sum[threadIdx.x + o];
-      s_count[threadIdx.x] += s_count[threadIdx.x + o];
+  if (gridDim.x > 1) {
+    sum = has = 0.0;
+    for (int i = threadIdx.x; i < gridDim.x; i += kRowThreads) {
+      const double2 q = __ldcg(sums + i);
+      sum += q.x;
+      has += q.y;
     }
+    block_add();
   }
   if (threadIdx.x == 0) {
-    *loss = (float)(reduction == CB_REDUCE_MEAN ? s_sum[0] / max(s_count[0], 1) : s_sum[0]);
-    *count = s_count[0];
+    *loss = (float)(reduction == CB_REDUCE_MEAN ? sum / fmax(has, 1.0) : sum);
+    *count = (int)has;
   }
 }
 
@@ -713,75 +743,115 @@ struct Upstream {
   int reduction;
 };
 
-// rows[n] = (a, b, lse, -) as they come from above, and *top = the largest |a| or |b|.
-// (*top starts at 0; a maximum does not depend on the order it is taken in.)
+// rows[n] = (a, b, lse, -) as they come from above, and *top = the largest |a| or |b|: one
+// for all rows of a reduced loss; else a maximum (which does not depend on the order it is
+// taken in), *top starting at 0.
 __global__ void __launch_bounds__(kRowThreads) factors_kernel(Problem p, Upstream u, const float* lse, float4* rows, float* top) {
   const int n = blockIdx.x * kRowThreads + threadIdx.x;
+  const bool common = u.reduction != CB_REDUCE_NONE && !u.lse;
+  await_before();
+  start_next();
+  float one = u.loss && u.reduction != CB_REDUCE_NONE ? *u.loss : 0.0f;
+  if (u.reduction == CB_REDUCE_MEAN) one /= (float)max(*u.count, 1);
+  if (common && n == 0) *top = fabsf(one) < INFINITY ? fabsf(one) : 0.0f;
   float size = 0.0f;
   if (n < p.N) {
     float b = 0.0f;
-    if (u.loss && target_of(p, n) >= 0) {
-      b = u.loss[u.reduction == CB_REDUCE_NONE ? n * u.loss_step : 0];
-      if (u.reduction == CB_REDUCE_MEAN) b /= (float)max(*u.count, 1);
-    }
+    if (u.loss && target_of(p, n) >= 0) b = u.reduction == CB_REDUCE_NONE ? u.loss[n * u.loss_step] : one;
     const float a = b + (u.lse ? u.lse[n * u.lse_step] : 0.0f);
     // (a row without a gradient is read as zeros, and its G is 0 whatever its own lse is)
     rows[n] = make_float4(a, b, a == 0.0f && b == 0.0f ? 0.0f : lse[n], 0.0f);
     size = fmaxf(fabsf(a), fabsf(b));
     if (!(size < INFINITY)) size = 0.0f;
   }
+  if (common) return;
   size = warp_max(size);
   if ((threadIdx.x & 31) == 0 && size > 0.0f) atomicMax(reinterpret_cast<int*>(top), __float_as_int(size));
 }
 
-// Rows as operands: 16-bit ones as they are, float32 ones as `parts` bf16 parts of dp columns
-// each.  rows given: rows without a gradient become zeros; top given: the others are
-// multiplied by 2^exponent of RowScale.
-template <typename T>
+// Rows as operands: 16-bit ones as they are, float32 ones as three bf16 parts of dp columns
+// each.  rows given: rows without a gradient become zeros; scaled given: a second copy, the
+// others multiplied by 2^row_exponent.  WIDE: rows are 16-byte aligned and d a multiple of 8.
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kRowThreads) operand_kernel(const T* x, int64_t ld, int64_t n_rows, int d, int dp,
-                                                              int parts, const float4* rows, const float* top,
-                                                              uint16_t* out) {
+                                                              const float4* rows, const float* top, uint16_t* out,
+                                                              uint16_t* scaled) {
+  constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
   const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  const int64_t n = i / (dp / 8);
+  const uint32_t pieces = dp / 8;
+  const int64_t n = i < (1ll << 32) ? (int64_t)((uint32_t)i / pieces) : i / pieces;
+  await_before();
+  start_next();
   if (n >= n_rows) return;
-  const int j0 = (int)(i % (dp / 8)) * 8;
-  const bool live = !rows || has_gradient(rows[n]);
-  const float by = top && live ? ldexpf(1.0f, row_exponent(rows[n], *top)) : 1.0f;
-  uint4 o[3];
-  uint16_t(*u)[8] = reinterpret_cast<uint16_t(*)[8]>(o);
+  const int j0 = (int)(i - n * pieces) * 8;
+  const float4 row = rows ? rows[n] : make_float4(1.0f, 0.0f, 0.0f, 0.0f);
+  Vec<T, 8> v;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    T v = Elem<T>::put(0.0f);
-    if (j0 + j < d && live) v = x[n * ld + j0 + j];
-    if (sizeof(T) == 4) {
-      float r = Elem<T>::get(v);
+  for (int j = 0; j < 8; ++j) v.v[j] = Elem<T>::put(0.0f);
+  if (has_gradient(row)) {
+    const T* at = x + n * ld + j0;
+    if (WIDE) {
+      if (j0 < d)
 #pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        u[k][j] = f32_to_bf16(r);
-        r -= bf16_to_f32(u[k][j]);
-      }
+        for (int k = 0; k < kParts; k += 2)
+          *reinterpret_cast<uint4*>(&v.v[k * 2]) = *reinterpret_cast<const uint4*>(at + k * 2);
     } else {
-      if (top) v = Elem<T>::put(Elem<T>::get(v) * by);
-      u[0][j] = *reinterpret_cast<uint16_t*>(&v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j0 + j < d) v.v[j] = at[j];
     }
   }
-  for (int k = 0; k < parts; ++k) *reinterpret_cast<uint4*>(out + (n * parts + k) * dp + j0) = o[k];
+  if (sizeof(T) == 2) {
+    *reinterpret_cast<uint4*>(out + n * dp + j0) = *reinterpret_cast<const uint4*>(&v);
+    if (!scaled) return;
+    const float by = ldexpf(1.0f, row_exponent(row, *top));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v.v[j] = Elem<T>::put(Elem<T>::get(v.v[j]) * by);
+    *reinterpret_cast<uint4*>(scaled + n * dp + j0) = *reinterpret_cast<const uint4*>(&v);
+    return;
+  }
+  float r[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = Elem<T>::get(v.v[j]);
+#pragma unroll
+  for (int k = 0; k < kParts; ++k) {
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u[j] = pack_bf16(r[2 * j], r[2 * j + 1]);
+      r[2 * j] -= __uint_as_float(u[j] << 16);
+      r[2 * j + 1] -= __uint_as_float(u[j] & 0xFFFF0000u);
+    }
+    *reinterpret_cast<uint4*>(out + (n * kParts + k) * dp + j0) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
 }
 
 // out[r][j] = the sum of the splits' results, scaled back; 0 in a row without a gradient.
-template <typename T>
+// VEC columns a thread: 4 where d is a multiple of it.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(kRowThreads) finish_kernel(const float* acc, int splits, int64_t split_rows, int da,
                                                              int64_t n_rows, int d, const float4* rows, const float* top,
                                                              int f16, T* out) {
   const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  if (i >= n_rows * d) return;
-  const int64_t n = i / d, j = i % d;
-  float s = 0.0f;
-  for (int k = 0; k < splits; ++k) s += acc[(k * split_rows + n) * da + j];
-  if (f16) s = ldexpf(s, (rows ? row_exponent(rows[n], *top) : 0) - kF16Shift);
-  s *= scale_of(*top);
-  if (rows && !has_gradient(rows[n])) s = 0.0f;
-  out[i] = Elem<T>::put(s);
+  const uint32_t pieces = d / VEC;
+  const int64_t n = i < (1ll << 32) ? (int64_t)((uint32_t)i / pieces) : i / pieces;
+  await_before();
+  start_next();
+  if (n >= n_rows) return;
+  const int j = (int)(i - n * pieces) * VEC;
+  float s[VEC] = {};
+  for (int k = 0; k < splits; ++k) {
+    const Vec<float, VEC> q = *reinterpret_cast<const Vec<float, VEC>*>(acc + (k * split_rows + n) * da + j);
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) s[c] += q.v[c];
+  }
+  const bool live = !rows || has_gradient(rows[n]);
+  float by = scale_of(*top);
+  if (f16) by = ldexpf(by, (rows ? row_exponent(rows[n], *top) : 0) - kF16Shift);
+  Vec<T, VEC> o;
+#pragma unroll
+  for (int c = 0; c < VEC; ++c) o.v[c] = Elem<T>::put(live ? s[c] * by : 0.0f);
+  *reinterpret_cast<Vec<T, VEC>*>(out + n * d + j) = o;
 }
 
 // ------------------------------------------------------------------- host
@@ -831,6 +901,9 @@ bool direct(const void* x, int32_t dtype, int64_t ld, int64_t rows) {
   return dtype != CB_F32 && aligned_to(x, 16) && (rows == 1 || (ld % 8 == 0 && ld > 0));
 }
 
+// Whether TMA can write contiguous rows of d columns there.
+bool tma_rows(const void* x, int32_t dtype, int d) { return aligned_to(x, 16) && d * dtype_size(dtype) % 16 == 0; }
+
 // Vocabulary rows whose G is held at a time: whole tiles, 256 MiB of G at most.
 int piece_of(int32_t N, int32_t V, int parts) {
   const int64_t most = std::max<int64_t>(kTileM, (int64_t)(256 << 20) / ((int64_t)N * parts * 2) / kTileM * kTileM);
@@ -858,27 +931,16 @@ struct Deal {
   int from[kMaxPairs + 1];
 };
 
-// dh's steps fill what dW's items, dealt in turn, leave of a common end.
-double fill(Deal& o, int pairs, int items, double cost, int64_t steps, int step_cost, int k_steps) {
+// When the last pair ends, if dh's steps fill what dW's items, dealt in turn, leave of a
+// common end, and that end.
+struct End {
+  double last, common;
+};
+End end_of(int pairs, int items, double cost, double work) {
   const int odd = items % pairs, low = items / pairs;  // `odd` pairs have one item more
-  const double work = (double)steps * step_cost;
-  double end = low * cost + work / (pairs - odd);  // if only the others get steps
-  if (end > (low + 1) * cost || odd == 0) end = (items * cost + work) / pairs;
-  const double most = std::max(end, items ? (low + (odd > 0)) * cost : 0.0);
-  double sum = 0.0;
-  for (int c = 0; c <= pairs; ++c) {
-    o.from[c] = c == pairs ? (int)steps : (int)std::min((double)steps, sum / step_cost);
-    sum += std::max(0.0, end - (low + (c < odd)) * cost);
-  }
-  // the most parts that a tile of dh lies in
-  o.h_slots = 1;
-  for (int c = 0, parts = 1; c < pairs && steps; ++c) {
-    if (o.from[c] == o.from[c + 1]) continue;
-    parts = o.from[c] % k_steps == 0 ? 1 : parts + 1;
-    o.h_slots = std::max(o.h_slots, parts);
-    if (o.from[c + 1] / k_steps > o.from[c] / k_steps) parts = 1;
-  }
-  return most;
+  double common = low * cost + work / (pairs - odd);   // if only the others get steps
+  if (common > (low + 1) * cost || odd == 0) common = (items * cost + work) / pairs;
+  return {std::max(common, items ? (low + (odd > 0)) * cost : 0.0), common};
 }
 
 // dW's split is the one whose pairs end first, counted in steps of K, with what a tile costs
@@ -887,20 +949,32 @@ Deal deal(int pairs, int h_tiles, int h_steps, int h_passes, int w_tiles, int w_
           int w_most) {
   constexpr int kTileCost = 6;             // of filling and emptying, in steps
   constexpr double kBytesPerStep = 900e3;  // written and read back in a step's time by the whole device
-  Deal best{}, o{};
+  const double steps = (double)h_tiles * h_steps, work = steps * h_passes;
+  Deal o;
+  o.w = 1;
   double least = 1e30;
-  for (int w = 1; w <= 64 && w <= w_steps && w <= w_most; w *= 2) {
-    o.w = w;
-    double t = fill(o, pairs, w_tiles * w, (double)w_steps * w_passes / w + kTileCost, (int64_t)h_tiles * h_steps, h_passes,
-                    std::max(h_steps, 1));
-    if (w > 1) t += w * w_bytes / kBytesPerStep;
+  auto cost = [&](int w) { return (double)w_steps * w_passes / w + kTileCost; };
+  for (int w = 1; w_tiles && w <= 64 && w <= w_steps && w <= w_most; w *= 2) {
+    const double t = end_of(pairs, w_tiles * w, cost(w), work).last + (w > 1 ? w * w_bytes / kBytesPerStep : 0.0);
     if (t < least * 0.99) {
       least = t;
-      best = o;
+      o.w = w;
     }
-    if (w_tiles == 0) break;
   }
-  return best;
+  const int items = w_tiles * o.w, odd = items % pairs, low = items / pairs;
+  const double end = end_of(pairs, items, cost(o.w), work).common;
+  const double most = std::max(0.0, end - low * cost(o.w)) / h_passes, less = std::max(0.0, end - (low + 1) * cost(o.w)) / h_passes;
+  for (int c = 0; c < pairs; ++c) o.from[c] = (int)std::min(steps, c < odd ? c * less : odd * less + (c - odd) * most);
+  o.from[pairs] = (int)steps;
+  // the most parts that a tile of dh lies in
+  o.h_slots = 1;
+  for (int c = 0, parts = 1; c < pairs && h_tiles; ++c) {
+    if (o.from[c] == o.from[c + 1]) continue;
+    parts = o.from[c] % h_steps == 0 ? 1 : parts + 1;
+    o.h_slots = std::max(o.h_slots, parts);
+    if (o.from[c + 1] / h_steps > o.from[c] / h_steps) parts = 1;
+  }
+  return o;
 }
 
 struct Shape {
@@ -947,7 +1021,8 @@ struct Layout {
 struct Forward {
   uint16_t *h, *w;
   float2* part;
-  float *xt, *rows;
+  float* xt;
+  double2* sums;
   uint32_t* counter;
   int tile_n, m_tiles, n_tiles, pairs, slots;
   Forward(Layout& a, const Shape& s, bool h_direct, bool w_direct) {
@@ -970,9 +1045,11 @@ struct Forward {
     w = w_direct ? nullptr : a.take<uint16_t>((int64_t)s.V * s.w_parts * s.dp);
     part = a.take<float2>((int64_t)slots * 2 * s.N);
     xt = a.take<float>(s.N);
-    rows = a.take<float>(s.N);
+    sums = a.take<double2>(join_ctas(s.N));
     counter = a.take<uint32_t>(1);
   }
+  int lanes() const { return 2 * slots > 16 ? 32 : 4; }  // of a row's parts
+  int join_ctas(int N) const { return ceil_div(N, kRowThreads / lanes()); }
 };
 
 struct Backward {
@@ -1002,30 +1079,31 @@ struct Backward {
 template <int MODE>
 int launch(const Args& p, cudaStream_t st) {
   if (int rc = ensure_smem_attr((const void*)gemm_kernel<MODE>, kSmem)) return rc;
-  gemm_kernel<MODE><<<2 * p.pairs, kThreads, kSmem, st>>>(p);
-  return launched();
+  return launch_after(gemm_kernel<MODE>, dim3(2 * p.pairs), kThreads, kSmem, st, p);
 }
 
-template <typename T>
-int make_operand(const void* x, int64_t ld, int64_t n_rows, const Shape& s, int parts, const float4* rows, const float* top,
-                 uint16_t* out, cudaStream_t st) {
+int make_operand(int32_t dtype, const void* x, int64_t ld, int64_t n_rows, const Shape& s, const float4* rows,
+                 const float* top, uint16_t* out, uint16_t* scaled, cudaStream_t st) {
   const int64_t n = n_rows * (s.dp / 8);
-  operand_kernel<T><<<(unsigned)((n + kRowThreads - 1) / kRowThreads), kRowThreads, 0, st>>>(
-      static_cast<const T*>(x), ld, n_rows, s.d, s.dp, parts, rows, top, out);
-  return launched();
+  const bool wide = s.d % 8 == 0 && aligned_to(x, 16) && ld * dtype_size(dtype) % 16 == 0;
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    return launch_after(wide ? operand_kernel<T, true> : operand_kernel<T, false>,
+                        dim3((unsigned)((n + kRowThreads - 1) / kRowThreads)), kRowThreads, 0, st, static_cast<const T*>(x),
+                        ld, n_rows, s.d, s.dp, rows, top, out, scaled);
+  });
 }
 
-int make_operand(int32_t dtype, const void* x, int64_t ld, int64_t n_rows, const Shape& s, int parts, const float4* rows,
-                 const float* top, uint16_t* out, cudaStream_t st) {
-  return with_type(dtype, [&](auto t) { return make_operand<decltype(t)>(x, ld, n_rows, s, parts, rows, top, out, st); });
-}
-
-template <typename T>
-int finish(const float* acc, int splits, int64_t split_rows, const Shape& s, int64_t n_rows, const float4* rows,
-           const float* top, T* out, cudaStream_t st) {
-  finish_kernel<T><<<(unsigned)((n_rows * s.d + kRowThreads - 1) / kRowThreads), kRowThreads, 0, st>>>(
-      acc, splits, split_rows, s.da(), n_rows, s.d, rows, top, s.f16, out);
-  return launched();
+int finish(int32_t dtype, const float* acc, int splits, int64_t split_rows, const Shape& s, int64_t n_rows, const float4* rows,
+           const float* top, void* out, cudaStream_t st) {
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const bool wide = s.d % 4 == 0 && aligned_to(out, 4 * sizeof(T));
+    const int64_t n = n_rows * (wide ? s.d / 4 : s.d);
+    return launch_after(wide ? finish_kernel<T, 4> : finish_kernel<T, 1>,
+                        dim3((unsigned)((n + kRowThreads - 1) / kRowThreads)), kRowThreads, 0, st, acc, splits, split_rows,
+                        s.da(), n_rows, s.d, rows, top, s.f16, static_cast<T*>(out));
+  });
 }
 
 // An operand in memory: the caller's matrix, or one made from it.
@@ -1045,21 +1123,17 @@ struct Operand {
 using namespace cb;
 
 extern "C" size_t cb_linear_ce_scratch_bytes(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype,
-                                             int64_t ldw, int32_t N, int32_t V, int32_t d, const void* dw, int32_t backward) {
-  if (N <= 0 || V <= 0 || d <= 0 || too_large(N, V, d) || !is_dtype(h_dtype) || !is_dtype(w_dtype)) return 0;
+                                             int64_t ldw, int32_t N, int32_t V, int32_t d, const void* dw, int32_t gradients) {
+  if (N <= 0 || V <= 0 || d <= 0 || too_large(N, V, d) || !is_dtype(h_dtype) || !is_dtype(w_dtype) || gradients < 0 ||
+      gradients > 3)
+    return 0;
   const Shape s(h_dtype, w_dtype, N, V, d);
   Layout a{nullptr};
-  if (!backward) {
-    Forward f(a, s, direct(h, h_dtype, ldh, N), direct(w, w_dtype, ldw, V));
+  const bool w_direct = direct(w, w_dtype, ldw, V);
+  if (!gradients) {
+    Forward f(a, s, direct(h, h_dtype, ldh, N), w_direct);
   } else {
-    // the larger of what the gradients together and each alone take
-    size_t most = 0;
-    for (int want = 1; want < 4; ++want) {
-      Layout b{nullptr};
-      Backward f(b, s, direct(w, w_dtype, ldw, V), want & 1, want & 2, aligned_to(dw, 16) && d * dtype_size(w_dtype) % 16 == 0);
-      most = std::max(most, b.used);
-    }
-    return most;
+    Backward f(a, s, w_direct, gradients & 1, gradients & 2, tma_rows(dw, w_dtype, d));
   }
   return a.used;
 }
@@ -1078,9 +1152,9 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   const Forward f(a, s, direct(h, h_dtype, ldh, N), direct(w, w_dtype, ldw, V));
   if (scratch_bytes < a.used) return CB_ERR_WORKSPACE;
   if (f.h)
-    if (int rc = make_operand(h_dtype, h, ldh, N, s, s.h_parts, nullptr, nullptr, f.h, st)) return rc;
+    if (int rc = make_operand(h_dtype, h, ldh, N, s, nullptr, nullptr, f.h, nullptr, st)) return rc;
   if (f.w)
-    if (int rc = make_operand(w_dtype, w, ldw, V, s, s.w_parts, nullptr, nullptr, f.w, st)) return rc;
+    if (int rc = make_operand(w_dtype, w, ldw, V, s, nullptr, nullptr, f.w, nullptr, st)) return rc;
   const Operand ho(h, ldh, N, f.h, s.h_parts, s), wo(w, ldw, V, f.w, s.w_parts, s);
   Args p{};
   Gemm& g = p.g[0];
@@ -1101,10 +1175,10 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   p.counter = f.counter;
   p.status = status;
   if (int rc = launch<STATS>(p, st)) return rc;
-  join_kernel<<<ceil_div(N, kRowThreads / 32), kRowThreads, 0, st>>>(
-      Problem{N, V, d, p.targets}, f.n_tiles, f.m_tiles, f.pairs, f.part, f.xt, reduction == CB_REDUCE_NONE ? loss : f.rows,
-      lse, reduction, loss, count, f.counter, status);
-  return launched();
+  const int lanes = f.lanes();
+  return launch_after(lanes == 32 ? join_kernel<32> : join_kernel<4>, dim3(f.join_ctas(N)), kRowThreads, 0, st,
+                      Problem{N, V, d, p.targets}, f.n_tiles, f.m_tiles, f.pairs, f.part, f.xt, loss, lse, reduction, loss,
+                      count, f.sums, f.counter, status);
 }
 
 extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype,
@@ -1119,20 +1193,17 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   if (too_large(N, V, d)) return CB_ERR_SHAPE;
   cudaStream_t st = (cudaStream_t)stream;
   const Shape s(h_dtype, w_dtype, N, V, d);
-  const bool dw_aligned = aligned_to(dw, 16) && d * dtype_size(w_dtype) % 16 == 0;
   Layout a{static_cast<char*>(scratch)};
-  const Backward f(a, s, direct(w, w_dtype, ldw, V), dh != nullptr, dw != nullptr, dw_aligned);
+  const Backward f(a, s, direct(w, w_dtype, ldw, V), dh != nullptr, dw != nullptr, tma_rows(dw, w_dtype, d));
   if (scratch_bytes < a.used) return CB_ERR_WORKSPACE;
   const Problem pb{N, V, d, Ids{targets, targets_64}};
   const Upstream u{g_loss, g_lse, g_loss_step, g_lse_step, count, reduction};
-  if (cudaMemsetAsync(f.top, 0, sizeof(float), st) != cudaSuccess) return CB_ERR_CUDA;
-  factors_kernel<<<ceil_div(N, kRowThreads), kRowThreads, 0, st>>>(pb, u, lse, f.rows, f.top);
-  if (int rc = launched()) return rc;
-  if (int rc = make_operand(h_dtype, h, ldh, N, s, s.h_parts, f.rows, nullptr, f.h, st)) return rc;
-  if (f.hs != f.h)
-    if (int rc = make_operand(h_dtype, h, ldh, N, s, 1, f.rows, f.top, f.hs, st)) return rc;
+  if ((reduction == CB_REDUCE_NONE || g_lse) && cudaMemsetAsync(f.top, 0, sizeof(float), st) != cudaSuccess) return CB_ERR_CUDA;
+  if (int rc = launch_after(factors_kernel, dim3(ceil_div(N, kRowThreads)), kRowThreads, 0, st, pb, u, lse, f.rows, f.top))
+    return rc;
+  if (int rc = make_operand(h_dtype, h, ldh, N, s, f.rows, f.top, f.h, f.hs != f.h ? f.hs : nullptr, st)) return rc;
   if (f.w)
-    if (int rc = make_operand(w_dtype, w, ldw, V, s, s.w_parts, nullptr, nullptr, f.w, st)) return rc;
+    if (int rc = make_operand(w_dtype, w, ldw, V, s, nullptr, nullptr, f.w, nullptr, st)) return rc;
   const Operand wo(w, ldw, V, f.w, s.w_parts, s);
   const int64_t h_cols = (int64_t)s.h_parts * s.dp;
   const int nt = ceil_div(d, kTileN), m_tiles = ceil_div(N, kTileM);
@@ -1176,7 +1247,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
     Gemm &gw = r.g[0], &gh = r.g[1];
     gh = gw = Gemm{};
     r.whole = 0;
-    std::copy(sp.from, sp.from + kMaxPairs + 1, r.from);
+    std::copy(sp.from, sp.from + s.pairs + 1, r.from);
     if (dh) {
       if (!map_of(&gh.a, f.G, s.type, N, g_ld, g_ld, 128) || !map_of(&gh.b, wo.at, s.type, V, wo.cols, wo.ld, 64) ||
           !map_of(&gh.out, f.acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.h_slots * up(N, kTileM), s.da(), s.da(), 128))
@@ -1220,16 +1291,10 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
     r.pairs = s.pairs;
     if (int rc = launch<PRODUCTS>(r, st)) return rc;
     if (dw && !f.dw_direct)
-      if (int rc = with_type(w_dtype, [&](auto t) {
-            using T = decltype(t);
-            return finish<T>(f.dw, sp.w, up(std::min(s.piece, V), kTileM), s, vp, nullptr, f.top,
-                             static_cast<T*>(dw) + (int64_t)v0 * d, st);
-          }))
+      if (int rc = finish(w_dtype, f.dw, sp.w, up(std::min(s.piece, V), kTileM), s, vp, nullptr, f.top,
+                          static_cast<char*>(dw) + (int64_t)v0 * d * dtype_size(w_dtype), st))
         return rc;
   }
   if (!dh) return CB_OK;
-  return with_type(h_dtype, [&](auto t) {
-    using T = decltype(t);
-    return finish<T>(f.acc, f.h_slots, up(N, kTileM), s, N, f.rows, f.top, static_cast<T*>(dh), st);
-  });
+  return finish(h_dtype, f.acc, f.h_slots, up(N, kTileM), s, N, f.rows, f.top, dh, st);
 }

@@ -19,10 +19,6 @@ namespace {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kGroup = 64;  // rows whose part of dw one CTA sums (rows taken by CTAs)
 
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Vec {
-  T v[VEC];
-};
 // A thread's elements of w beside VEC of x.
 template <typename W, int VEC>
 __device__ __forceinline__ void load_w(const W* w, float (&o)[VEC]) {
@@ -41,6 +37,8 @@ __global__ void __launch_bounds__(kThreads) rms_norm_warp_kernel(const T* x, int
                                                                  float eps, T* y) {
   constexpr int VEC = 16 / sizeof(T);
   const int lane = threadIdx.x & 31, n = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  await_before();
+  start_next();
   if (n >= rows) return;
   Vec<T, VEC> v[NV];
   float s = 0.0f;
@@ -77,6 +75,8 @@ __global__ void __launch_bounds__(kThreads) rms_norm_grad_warp_kernel(const T* x
   __shared__ float s_part[kWarps / 2][kWide];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float acc[NV][VEC] = {};
+  await_before();
+  start_next();
   for (int n = blockIdx.x * kWarps + warp; n < rows; n += gridDim.x * kWarps) {
     Vec<T, VEC> v[NV], up[NV];
 #pragma unroll
@@ -154,6 +154,8 @@ __global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* part, in
   __shared__ float s_sum[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
   float s[4] = {};
+  await_before();
+  start_next();
   if (j < d) {
     int i = warp;
     for (; i + 96 < parts; i += 128)
@@ -173,6 +175,8 @@ __global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* part, in
 template <typename T, typename W>
 __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const T* x, int64_t ld, const W* w, int d, float eps, T* y) {
   __shared__ float red[33];
+  await_before();
+  start_next();
   const T* row = x + blockIdx.x * ld;
   float s = 0.0f;
   for (int j = threadIdx.x; j < d; j += kThreads) {
@@ -188,6 +192,8 @@ template <typename T, typename W>
 __global__ void __launch_bounds__(kThreads) rms_norm_dx_kernel(const T* x, int64_t ld, const T* g, int64_t ldg,
                                                                const W* w, int d, float eps, T* dx, float* rstd) {
   __shared__ float red[33];
+  await_before();
+  start_next();
   const T* row = x + blockIdx.x * ld;
   const T* up = g + blockIdx.x * ldg;
   float s = 0.0f, c = 0.0f;
@@ -208,6 +214,8 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) rms_norm_dw_part_kernel(const T* x, int64_t ld, const T* g, int64_t ldg,
                                                                     const float* rstd, int rows, int d, float* part) {
   const int j = blockIdx.y * kThreads + threadIdx.x;
+  await_before();
+  start_next();
   if (j >= d) return;
   const int64_t from = (int64_t)blockIdx.x * kGroup;
   const int64_t to = min(from + kGroup, (int64_t)rows);
@@ -265,13 +273,11 @@ extern "C" int cb_rms_norm(const void* x, int32_t dtype, int64_t ld, const void*
     const T* in = static_cast<const T*>(x);
     const W* weight = static_cast<const W*>(w);
     if (!warps) {
-      rms_norm_kernel<T, W><<<rows, kThreads, 0, st>>>(in, ld, weight, d, eps, static_cast<T*>(y));
-      return launched();
+      return launch_after(rms_norm_kernel<T, W>, dim3(rows), kThreads, 0, st, in, ld, weight, d, eps, static_cast<T*>(y));
     }
     return with_pieces<T>(d, [&](auto nv) {
-      rms_norm_warp_kernel<T, W, decltype(nv)::value><<<ceil_div(rows, kWarps), kThreads, 0, st>>>(
-          in, ld, weight, rows, d, eps, static_cast<T*>(y));
-      return launched();
+      return launch_after(rms_norm_warp_kernel<T, W, decltype(nv)::value>, dim3(ceil_div(rows, kWarps)), kThreads, 0, st, in,
+                          ld, weight, rows, d, eps, static_cast<T*>(y));
     });
   });
 }
@@ -307,19 +313,19 @@ extern "C" int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const 
       part = rstd;
       parts = grad_ctas(rows);
       const int rc = with_pieces<T>(d, [&](auto nv) {
-        auto* fn = rms_norm_grad_warp_kernel<T, W, decltype(nv)::value>;
-        fn<<<parts, kThreads, 0, st>>>(in, ld, up, ldg, weight, rows, d, eps, static_cast<T*>(dx), part, static_cast<W*>(dw));
-        return launched();
+        return launch_after(rms_norm_grad_warp_kernel<T, W, decltype(nv)::value>, dim3(parts), kThreads, 0, st, in, ld, up,
+                            ldg, weight, rows, d, eps, static_cast<T*>(dx), part, static_cast<W*>(dw));
       });
       if (rc || parts == 1) return rc;
     } else {
       parts = ceil_div(rows, kGroup);
-      rms_norm_dx_kernel<T, W><<<rows, kThreads, 0, st>>>(in, ld, up, ldg, weight, d, eps, static_cast<T*>(dx), rstd);
-      if (int rc = launched()) return rc;
-      rms_norm_dw_part_kernel<T><<<dim3(parts, ceil_div(d, kThreads)), kThreads, 0, st>>>(in, ld, up, ldg, rstd, rows, d, part);
-      if (int rc = launched()) return rc;
+      if (int rc = launch_after(rms_norm_dx_kernel<T, W>, dim3(rows), kThreads, 0, st, in, ld, up, ldg, weight, d, eps,
+                                static_cast<T*>(dx), rstd))
+        return rc;
+      if (int rc = launch_after(rms_norm_dw_part_kernel<T>, dim3(parts, ceil_div(d, kThreads)), kThreads, 0, st, in, ld, up,
+                                ldg, rstd, rows, d, part))
+        return rc;
     }
-    rms_norm_dw_kernel<W><<<ceil_div(d, 32), 1024, 0, st>>>(part, parts, d, static_cast<W*>(dw));
-    return launched();
+    return launch_after(rms_norm_dw_kernel<W>, dim3(ceil_div(d, 32)), 1024, 0, st, part, parts, d, static_cast<W*>(dw));
   });
 }

@@ -11,9 +11,9 @@ tied to its head.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from cirrus_s_1a_b200 import _rows
+from cirrus_s_1a_b200.kv8 import DTYPES
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
@@ -24,45 +24,44 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     when an id is outside the table, which then counts as negative.  The table's gradient
     has its type, with sums in float32 in the order of the tokens.  Runs on the current
     stream."""
-    _rows.vocabulary(table, "table")
-    _rows.ids(ids, "ids", table.device)
-    _rows.status(status, table.device)
-    if _rows.wants_grad(table):
+    if table.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(ids, table, float(scale), status)
-    return _lookup(ids, table, float(scale), status)
+    return _lookup(ids, table, float(scale), status)[0]
 
 
-def _lookup(ids, table, scale, status):
+def _lookup(ids, table, scale, status) -> tuple:
+    """(the rows, whether ids are 64 bits wide)"""
     V, D, ld, code = _rows.vocabulary(table, "table")
-    out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
-    if ids.numel():
-        _rows.call(table.device, "cb_embedding", table.data_ptr(), code, ld, V, D, ids.data_ptr(),
-                   _rows.ids(ids, "ids", table.device), ids.numel(), scale, out.data_ptr(),
-                   _rows.status(status, table.device))
-    return out
+    dev = table.device
+    wide = _rows.ids(ids, "ids", dev)
+    flag = _rows.status(status, dev)
+    out = torch.empty(*ids.shape, D, dtype=table.dtype, device=dev)
+    n = ids.numel()
+    if n:
+        _rows.call(dev, "cb_embedding", table.data_ptr(), code, ld, V, D, ids.data_ptr(), wide, n, scale, out.data_ptr(),
+                   flag)
+    return out, wide
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale, status):
         ctx.save_for_backward(ids)
-        ctx.scale, ctx.shape, ctx.dtype = scale, table.shape, table.dtype
-        return _lookup(ids, table, scale, status)
+        out, wide = _lookup(ids, table, scale, status)
+        ctx.args = scale, table.shape, table.dtype, wide
+        return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        _rows.once()
         ids, = ctx.saved_tensors
-        V, D = ctx.shape
-        n = ids.numel()
+        scale, (V, D), dtype, wide = ctx.args
+        n, dev = ids.numel(), ids.device
         if n == 0:
-            return None, torch.zeros(V, D, dtype=ctx.dtype, device=ids.device), None, None
-        g = g.reshape(n, D)
-        g = _rows.upstream(g)
-        out = torch.empty(V, D, dtype=ctx.dtype, device=ids.device)
-        scratch = _rows.scratch(ids.device, "cb_embedding_grad_scratch_bytes", n, V, D)
-        _, _, ldg, code = _rows.matrix(g, "the gradient")
-        _rows.call(ids.device, "cb_embedding_grad", g.data_ptr(), code, ldg, ids.data_ptr(),
-                   _rows.ids(ids, "ids", ids.device), n, V, D, ctx.scale, out.data_ptr(), scratch.data_ptr(),
-                   scratch.numel())
+            return None, torch.zeros(V, D, dtype=dtype, device=dev), None, None
+        g, ldg = _rows.upstream(g.reshape(n, D), D)
+        out = torch.empty(V, D, dtype=dtype, device=dev)
+        scratch = _rows.scratch(dev, "cb_embedding_grad_scratch_bytes", (n, V, D), n, V, D)
+        _rows.call(dev, "cb_embedding_grad", g.data_ptr(), DTYPES[dtype], ldg, ids.data_ptr(), wide, n, V, D, scale,
+                   out.data_ptr(), scratch.data_ptr(), scratch.numel())
         return None, out, None, None

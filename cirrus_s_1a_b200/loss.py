@@ -16,7 +16,6 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from cirrus_s_1a_b200 import _lib, _rows
 
@@ -38,70 +37,77 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     ``status`` (int32 [1] on the device) receives 6 when a target is outside the
     vocabulary, which then counts as none, and 8 when a bounded wait in a kernel gave up.
     Runs on the current stream."""
-    _check(hidden, weight, targets, reduction, status)
-    if _rows.wants_grad(hidden, weight):
+    if (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
         return CrossEntropy(*_LinearCE.apply(hidden, weight, targets, reduction, status))
     return CrossEntropy(*_forward(hidden, weight, targets, reduction, status)[:2])
 
 
-def _check(hidden, weight, targets, reduction, status) -> tuple:
-    """The leading arguments of both entry points, and (N, V, d)."""
+def _forward(hidden, weight, targets, reduction, status) -> tuple:
+    """(loss, lse, count, the leading arguments of both entry points)"""
     N, D, ldh, h_code = _rows.matrix(hidden, "hidden")
-    V, Dw, ldw, w_code = _rows.vocabulary(weight, "weight", hidden.device)
+    dev = hidden.device
+    V, Dw, ldw, w_code = _rows.vocabulary(weight, "weight", dev)
     if Dw != D:
         raise ValueError(f"weight must have {D} columns as hidden, not {Dw}")
-    if hidden.dtype != weight.dtype and not (hidden.dtype == torch.float32 and weight.dtype == torch.bfloat16):
+    if h_code != w_code and not (h_code == _lib.CB_F32 and w_code == _lib.CB_BF16):
         raise ValueError(f"hidden and weight must have one type, or float32 and bfloat16, not {hidden.dtype} and "
                          f"{weight.dtype}")
     if targets.shape != (N,):
         raise ValueError(f"targets must be [{N}]")
-    wide = _rows.ids(targets, "targets", hidden.device)
-    if reduction not in REDUCTIONS:
+    wide = _rows.ids(targets, "targets", dev)
+    code = REDUCTIONS.get(reduction)
+    if code is None:
         raise ValueError(f"unknown reduction {reduction!r}; choose from {sorted(REDUCTIONS)}")
-    _rows.status(status, hidden.device)
-    return (hidden.data_ptr(), h_code, ldh, weight.data_ptr(), w_code, ldw, N, V, D, targets.data_ptr(), wide,
-            REDUCTIONS[reduction]), (N, V, D)
-
-
-def _forward(hidden, weight, targets, reduction, status) -> tuple:
-    args, shape = _check(hidden, weight, targets, reduction, status)
-    dev, N = hidden.device, shape[0]
+    flag = _rows.status(status, dev)
+    args = (hidden.data_ptr(), h_code, ldh, weight.data_ptr(), w_code, ldw, N, V, D, targets.data_ptr(), wide, code)
     lse = torch.empty(N, dtype=torch.float32, device=dev)
     if N == 0:
-        return torch.zeros(() if reduction != "none" else 0, device=dev), lse, None
+        return torch.zeros(() if reduction != "none" else 0, device=dev), lse, None, args
     loss = torch.empty(N if reduction == "none" else (), dtype=torch.float32, device=dev)
     count = None if reduction == "none" else torch.empty(1, dtype=torch.int32, device=dev)
-    scratch = _rows.scratch(dev, "cb_linear_ce_scratch_bytes", *args[:9], None, 0)
+    scratch = _scratch(dev, args, None, 0)
     _rows.call(dev, "cb_linear_ce", *args, loss.data_ptr(), lse.data_ptr(), _lib.ptr(count), scratch.data_ptr(),
-               scratch.numel(), _rows.status(status, dev))
-    return loss, lse, count
+               scratch.numel(), flag)
+    return loss, lse, count, args
+
+
+def _scratch(dev, args, dw, gradients) -> torch.Tensor:
+    h, h_code, ldh, w, w_code, ldw, N, V, D = args[:9]
+    at = None if dw is None else dw.data_ptr()
+    # what the size goes by, beside the shape: which matrices can be read and written where they lie
+    key = (dev, h_code, w_code, N, V, D, ldh % 8, ldh > 0, ldw % 8, h % 16, w % 16, (at or 0) % 16, gradients)
+    return _rows.scratch(dev, "cb_linear_ce_scratch_bytes", key, *args[:9], at, gradients)
 
 
 class _LinearCE(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, reduction, status):
-        loss, lse, count = _forward(hidden, weight, targets, reduction, status)
+        loss, lse, count, ctx.args = _forward(hidden, weight, targets, reduction, status)
         ctx.save_for_backward(hidden, weight, targets, lse, count)
-        ctx.reduction, ctx.status = reduction, status
+        ctx.status = status
         ctx.set_materialize_grads(False)
         return loss, lse
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_loss, g_lse):
+        _rows.once()
         hidden, weight, targets, lse, count = ctx.saved_tensors
         want_h, want_w = ctx.needs_input_grad[:2]
         if g_loss is None and g_lse is None:
             return None, None, None, None, None
-        args, shape = _check(hidden, weight, targets, ctx.reduction, ctx.status)
-        dev, (N, V, D) = hidden.device, shape
+        dev = hidden.device
+        N, V, D = ctx.args[6:9]
         dh = torch.empty(N, D, dtype=hidden.dtype, device=dev) if want_h else None
         if N == 0:
             return dh, torch.zeros(V, D, dtype=weight.dtype, device=dev) if want_w else None, None, None, None
         dw = torch.empty(V, D, dtype=weight.dtype, device=dev) if want_w else None
-        scratch = _rows.scratch(dev, "cb_linear_ce_scratch_bytes", *args[:9], _lib.ptr(dw), 1)
-        step = lambda g: g.stride(0) if g is not None and g.dim() else 0  # noqa: E731
-        _rows.call(dev, "cb_linear_ce_grad", *args, lse.data_ptr(), _lib.ptr(count), _lib.ptr(g_loss), step(g_loss),
-                   _lib.ptr(g_lse), step(g_lse), _lib.ptr(dh), _lib.ptr(dw), scratch.data_ptr(), scratch.numel(),
-                   _rows.status(ctx.status, dev))
+        scratch = _scratch(dev, ctx.args, dw, want_h + 2 * want_w)
+        _rows.call(dev, "cb_linear_ce_grad", *ctx.args, lse.data_ptr(), _lib.ptr(count), _lib.ptr(g_loss), _step(g_loss),
+                   _lib.ptr(g_lse), _step(g_lse), _lib.ptr(dh), _lib.ptr(dw), scratch.data_ptr(), scratch.numel(),
+                   _lib.ptr(ctx.status))
         return dh, dw, None, None, None
+
+
+def _step(g) -> int:
+    """Elements between the rows of a gradient (0: one for all)."""
+    return 0 if g is None or g.dim() == 0 else g.stride(0)

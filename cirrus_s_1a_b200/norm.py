@@ -9,56 +9,52 @@ is fused into the products that follow.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from cirrus_s_1a_b200 import _rows
-from cirrus_s_1a_b200.kv8 import _dtype
+from cirrus_s_1a_b200.kv8 import DTYPES
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
     """``x * rsqrt(mean(x^2) + eps) * weight`` for the rows of ``x`` [rows, d] (float32,
     bfloat16 or float16, rows at any distance) and ``weight`` [d] (float32 or x's type),
     in x's type; gradients in x's and the weight's.  Runs on the current stream."""
-    _check(x, weight)
-    if _rows.wants_grad(x, weight):
+    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
         return _RMSNorm.apply(x, weight, float(eps))
-    return _norm(x, weight, float(eps))
+    return _norm(x, weight, float(eps))[0]
 
 
-def _check(x, weight) -> tuple:
+def _norm(x, weight, eps) -> tuple:
+    """(y, the arguments that both entry points share)"""
     R, D, ld, code = _rows.matrix(x, "x")
-    if weight.shape != (D,) or weight.device != x.device or not weight.is_contiguous() \
+    dev = x.device
+    if weight.shape != (D,) or weight.device != dev or not weight.is_contiguous() \
             or weight.dtype not in (torch.float32, x.dtype):
-        raise ValueError(f"weight must be contiguous, float32 or {x.dtype}, [{D}] on {x.device}")
-    return R, D, ld, code, _dtype(weight, "weight")
-
-
-def _norm(x, weight, eps):
-    R, D, ld, code, w_code = _check(x, weight)
-    y = torch.empty(R, D, dtype=x.dtype, device=x.device)
+        raise ValueError(f"weight must be contiguous, float32 or {x.dtype}, [{D}] on {dev}")
+    w_code = DTYPES[weight.dtype]
+    y = torch.empty(R, D, dtype=x.dtype, device=dev)
     if R:
-        _rows.call(x.device, "cb_rms_norm", x.data_ptr(), code, ld, weight.data_ptr(), w_code, R, D, eps, y.data_ptr())
-    return y
+        _rows.call(dev, "cb_rms_norm", x.data_ptr(), code, ld, weight.data_ptr(), w_code, R, D, eps, y.data_ptr())
+    return y, (R, D, ld, code, w_code, eps)
 
 
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps):
         ctx.save_for_backward(x, weight)
-        ctx.eps = eps
-        return _norm(x, weight, eps)
+        y, ctx.args = _norm(x, weight, eps)
+        return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        _rows.once()
         x, weight = ctx.saved_tensors
-        R, D, ld, code, w_code = _check(x, weight)
+        R, D, ld, code, w_code, eps = ctx.args
+        dev = x.device
         if R == 0:
             return torch.zeros_like(x), torch.zeros_like(weight), None
-        g = _rows.upstream(g)
-        dx, dw = torch.empty(R, D, dtype=x.dtype, device=x.device), torch.empty_like(weight)
-        scratch = _rows.scratch(x.device, "cb_rms_norm_grad_scratch_bytes", R, D)
-        _, _, ldg, _ = _rows.matrix(g, "the gradient")
-        _rows.call(x.device, "cb_rms_norm_grad", x.data_ptr(), code, ld, g.data_ptr(), ldg, weight.data_ptr(), w_code, R,
-                   D, ctx.eps, dx.data_ptr(), dw.data_ptr(), scratch.data_ptr(), scratch.numel())
+        g, ldg = _rows.upstream(g, D)
+        dx, dw = torch.empty(R, D, dtype=x.dtype, device=dev), torch.empty_like(weight)
+        scratch = _rows.scratch(dev, "cb_rms_norm_grad_scratch_bytes", (R, D), R, D)
+        _rows.call(dev, "cb_rms_norm_grad", x.data_ptr(), code, ld, g.data_ptr(), ldg, weight.data_ptr(), w_code, R, D, eps,
+                   dx.data_ptr(), dw.data_ptr(), scratch.data_ptr(), scratch.numel())
         return dx, dw, None

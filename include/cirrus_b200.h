@@ -546,12 +546,12 @@ int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const void* g, in
  * over the rows with a target (0 when none has one) or its sum, [1], with their number in
  * count [1].  h and w have one type, or h is CB_F32 and w CB_BF16.  16-bit products are
  * exact and float32 ones carried in about 24 bits, both summed in float32.
- * Scratch: cb_linear_ce_scratch_bytes of the same arguments bytes (backward 1, with dw, for
- * the gradient), 256-byte aligned.  *status also receives CB_ERR_TIMEOUT when a bounded
+ * Scratch, 256-byte aligned: cb_linear_ce_scratch_bytes of the same arguments, for the
+ * gradient with 1 for dh + 2 for dw in `gradients`, and dw.  *status also receives CB_ERR_TIMEOUT when a bounded
  * wait in a kernel gave up.
  * Replaces lm_head + the loss of CirrusModel.forward (cirrus/model/model.py:176-228). */
 size_t cb_linear_ce_scratch_bytes(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype, int64_t ldw,
-                                  int32_t N, int32_t V, int32_t d, const void* dw, int32_t backward);
+                                  int32_t N, int32_t V, int32_t d, const void* dw, int32_t gradients);
 int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype, int64_t ldw, int32_t N,
                  int32_t V, int32_t d, const void* targets, int32_t targets_64, int32_t reduction, float* loss,
                  float* lse, int32_t* count, void* scratch, size_t scratch_bytes, int32_t* status, void* stream);
