@@ -34,7 +34,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTileM = 256, kTileN = 256;  // of a pair
 constexpr int kStep = 64;                  // of K: 128 bytes, a swizzled row
-constexpr int kStages = 6;
+constexpr int kStages = 6, kMaxStages = 12;
 constexpr int kHalfBytes = 128 * kStep * 2;  // one CTA's rows of one operand's step
 constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kOutBytes = 128 * 128;  // a box on its way out: 128 rows of 128 bytes, one for each half of the columns
@@ -48,7 +48,10 @@ constexpr int kMaxPasses = 6, kMaxPairs = 128;
 constexpr int kSpan16 = 16, kSpan32 = 4;
 constexpr uint64_t kWaitNs = 2000000000ull, kDrainNs = 10000000ull;
 
-enum { STATS = 0, GRAD = 1, PRODUCTS = 2 };
+// Rows up to which the forward has them as columns and the vocabulary as rows of its tiles.
+constexpr int kFew = 128;
+
+enum { STATS = 0, FEW = 1, GRAD = 2, PRODUCTS = 3 };
 enum { OUT_STORE = 0, OUT_ADD = 1 };
 
 // One matrix product D[m][n] = sum over passes and k of A[m][k] B[n][k].  An operand is a
@@ -75,12 +78,15 @@ struct alignas(64) Args {
   int whole;                       // PRODUCTS: items of dW, dealt in turn
   int from[kMaxPairs + 1];         // and where each pair's steps of dh begin
   uint32_t kind;                   // instruction descriptor without sizes and directions
-  int tile_n;                      // STATS, GRAD
-  // STATS and GRAD: rows, vocabulary rows, the vocabulary row that the tiles start at, and how many
+  int tile_m, tile_n;              // rows and columns of a tile (PRODUCTS: kTileM, kTileN)
+  int share;                       // FEW: parts of the rows' operand that a step of the vocabulary's meets
+  int part_cols;                   // and the columns between them
+  int stages, stage_bytes;         // FEW
+  // STATS, FEW and GRAD: rows, vocabulary rows, the vocabulary row that the tiles start at, and how many
   int N, V, v0, vp;
   Ids targets;
   int slots;                       // STATS: parts of a row's sum
-  float2* part;                    // [slots][2][N]
+  float2* part;                    // STATS: [slots][2][N]; FEW: [tiles][2][N]
   float* xt;                       // [N]
   uint32_t* counter;               // set to 0
   const float4* rows;              // GRAD: (a, b, lse, -) of each row
@@ -275,7 +281,7 @@ __device__ __forceinline__ bool item_of(const Args& p, int pair, int i, Item& it
     const int64_t u = all * pair / p.pairs + i;
     if (u >= all * (pair + 1) / p.pairs) return false;
     it.gemm = 0;
-    it.m0 = (int)(u / g.n_tiles) * kTileM;
+    it.m0 = (int)(u / g.n_tiles) * p.tile_m;
     it.tile = (int)(u % g.n_tiles);
     it.n0 = it.tile * p.tile_n;
     it.first = 0;
@@ -324,17 +330,19 @@ __device__ __forceinline__ void put_row(uint32_t box, int row, F&& f) {
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ Args p) {
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t bars[2 * kStages + 4];
+  __shared__ uint64_t bars[2 * kMaxStages + 4];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1;
   const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
   const uint32_t out_at = base + kStages * kStageBytes;
-  const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, done = empty + 8 * kStages, freed = done + 16;
+  const int stages = MODE == FEW ? p.stages : kStages, stage_bytes = MODE == FEW ? p.stage_bytes : kStageBytes;
+  const int a_bytes = MODE == FEW ? p.tile_m * 64 : kHalfBytes;  // of a stage
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kMaxStages, done = empty + 8 * kMaxStages, freed = done + 16;
 
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kMaxStages; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full + 8 * i));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(empty + 8 * i));
     }
@@ -355,7 +363,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   fence_after();
   await_before();
   start_next();
-  if (MODE == STATS && blockIdx.x == 0 && tid == 0) *p.counter = 0;
+  if (MODE <= FEW && blockIdx.x == 0 && tid == 0) *p.counter = 0;
   const uint32_t tmem = s_tmem;
   volatile int* abort_flag = &s_abort;
   auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -373,20 +381,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       bool go = true;
       for (int i = 0; go && item_of<MODE>(p, pair, i, it); ++i) {
         const Gemm& g = p.g[MODE == PRODUCTS ? it.gemm : 0];
-        const int n_rows = MODE == PRODUCTS ? kTileN / 2 : p.tile_n / 2;
-        const int m = it.m0 + rank * 128, c = it.n0 + rank * n_rows;
-        const uint32_t bytes = 2 * (kHalfBytes + n_rows * 128);
+        const int n_rows = MODE == PRODUCTS ? kTileN / 2 : p.tile_n / 2, m_rows = MODE == FEW ? p.tile_m / 2 : 128;
+        const int m = it.m0 + rank * m_rows, c = it.n0 + rank * n_rows;
+        const uint32_t bytes = 2 * (m_rows + (MODE == FEW ? p.share : 1) * n_rows) * 128;
         // a span of K at a time, all passes over it
         for (int from = 0; go && from < it.steps; from += g.span)
           for (int pass = 0; go && pass < g.passes; ++pass) {
             const int ap = g.a_part[pass], bp = g.b_part[pass], end = min(from + g.span, it.steps);
             for (int k = from; k < end; ++k, ++n) {
-              const int st = n % kStages, k0 = (it.first + k) * kStep;
-              if (n >= kStages && !wait(empty + 8 * st, (n / kStages - 1) & 1)) {
+              const int st = n % stages, k0 = (it.first + k) * kStep;
+              if (n >= stages && !wait(empty + 8 * st, (n / stages - 1) & 1)) {
                 go = false;
                 break;
               }
-              const uint32_t bar = in_leader(full + 8 * st), at = base + st * kStageBytes, bt = at + kHalfBytes;
+              const uint32_t bar = in_leader(full + 8 * st), at = base + st * stage_bytes, bt = at + a_bytes;
               if (rank == 0)
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full + 8 * st), "r"(bytes)
                              : "memory");
@@ -401,6 +409,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
                 copy_in(bt + kHalfBytes / 2, &g.b, c + 64 + bp, g.b_base + k0, bar);
               } else {
                 copy_in(bt, &g.b, k0 + bp, g.b_base + c, bar);
+                for (int j = 1; j < (MODE == FEW ? p.share : 1); ++j)
+                  copy_in(bt + j * n_rows * 128, &g.b, k0 + j * p.part_cols, c, bar);
               }
             }
           }
@@ -427,14 +437,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           fence_after();
           const uint32_t d = tmem + acc * kTileN;
           for (int k = 0; k < steps && go; ++k, ++n) {
-            const int st = n % kStages;
-            go = __all_sync(0xffffffffu, wait(full + 8 * st, (n / kStages) & 1));
+            const int st = n % stages;
+            go = __all_sync(0xffffffffu, wait(full + 8 * st, (n / stages) & 1));
             if (!go) break;
             fence_after();
             if (lead) {
-              const uint64_t a = operand(base + st * kStageBytes), b = operand(base + st * kStageBytes + kHalfBytes);
+              const uint64_t a = operand(base + st * stage_bytes), b = operand(base + st * stage_bytes + a_bytes);
 #pragma unroll
               for (int s = 0; s < kStep / 16; ++s) mma(d, a + s * a_step, b + s * b_step, id, k > 0 || s > 0);
+              for (int j = 1; j < (MODE == FEW ? p.share : 1); ++j)
+#pragma unroll
+                for (int s = 0; s < kStep / 16; ++s) mma(d, a + s * a_step, b + j * p.tile_n * 4 + s * b_step, id, true);
               commit(empty + 8 * st);
             }
             __syncwarp();
@@ -444,11 +457,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         }
       }
       if (!go) {  // what is in flight ends before the memory goes
-        for (int k = 0; k < kStages; ++k) {
+        for (int k = 0; k < stages; ++k) {
           const int last = n - 1 - k;
-          if (last >= 0) bounded_wait(empty + 8 * (last % kStages), (last / kStages) & 1, kDrainNs);
+          if (last >= 0) bounded_wait(empty + 8 * (last % stages), (last / stages) & 1, kDrainNs);
         }
-        for (int k = 0; k < kStages; ++k) bounded_wait(full + 8 * ((n + k) % kStages), ((n + k) / kStages) & 1, kDrainNs);
+        for (int k = 0; k < stages; ++k) bounded_wait(full + 8 * ((n + k) % stages), ((n + k) / stages) & 1, kDrainNs);
       }
     }
   } else {
@@ -480,7 +493,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     for (int i = 0; item_of<MODE>(p, pair, i, it); ++i) {
       const int n = it.m0 + rank * 128 + row;
       const bool live = MODE != PRODUCTS && n < p.N;
-      if (MODE != PRODUCTS && it.m0 != run) {
+      if ((MODE == STATS || MODE == GRAD) && it.m0 != run) {
         if (MODE == STATS) leave();
         run = it.m0;
         m = -INFINITY;
@@ -499,8 +512,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           slot = pair - (int)(((from + 1) * p.pairs - 1) / all);
         }
       }
-      float x[128];
-      const int cols = MODE == PRODUCTS ? 128 : min(128, p.tile_n - half * 128);
+      constexpr int kCols = MODE == FEW ? kFew / 2 : 128;  // a thread's
+      float x[kCols];
+      // this half's columns
+      const int cols = MODE == PRODUCTS ? 128 : MODE == FEW ? p.tile_n / 2 : min(128, p.tile_n - half * 128);
       const int span = p.g[MODE == PRODUCTS ? it.gemm : 0].span;
       bool go = true;
       for (int from = 0; from < it.steps; from += span, ++sums) {
@@ -509,15 +524,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         go = !any_of_half(half, !wait(done + 8 * acc, (sums / 2) & 1));
         if (!go) break;
         fence_after();
-        const uint32_t at = tmem + lane_at + acc * kTileN + half * 128;
+        const uint32_t at = tmem + lane_at + acc * kTileN + half * (MODE == FEW ? cols : 128);
         if (from == 0) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < kCols / 32; ++c)
             if (c * 32 < cols) load32(at + c * 32, x + c * 32);
           loads_done();
         } else {
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
+          for (int c = 0; c < kCols / 16; ++c)
             if (c * 16 < cols) {
               float y[16];
               load16(at + c * 16, y);
@@ -535,7 +550,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       if (!go) break;
       const int v = it.n0 + half * 128;  // of the piece, or of d
       const int at = (int)(target - p.v0 - v);  // the target's column
-      const bool hit = MODE != PRODUCTS && target >= 0 && at >= 0 && at < cols;
+      const bool hit = (MODE == STATS || MODE == GRAD) && target >= 0 && at >= 0 && at < cols;
       if constexpr (MODE == PRODUCTS) {
         const Gemm& g = p.g[it.gemm];
         const int y = it.m0 + rank * 128 + it.split * g.out_rows;
@@ -555,6 +570,62 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
               const float lo = x[c * 64 + 2 * j], hi = x[c * 64 + 2 * j + 1];
               return p.is_f16 ? pack_f16(lo, hi) : pack_bf16(lo, hi);
             });
+        }
+      }
+      if constexpr (MODE == FEW) {
+        // Lanes hold vocabulary rows, columns the few rows.  Turned over in shared memory, 32
+        // columns at a time (word j * 128 + (row ^ j), free of bank conflicts both ways), a
+        // thread takes a quarter of the tile's logits of one row, a warp joins the quarters.
+        const int m_rows = p.tile_m / 2, v0 = it.m0 + rank * m_rows, valid = min(m_rows, p.V - v0);
+        const int quarter = warp & 3;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          if (b * 32 >= cols) break;
+          const int r = half * cols + b * 32 + lane;  // this thread's row
+          const bool is = b * 32 + lane < cols && r < p.N;
+          half_sync();
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (b * 32 + (j & 16) < cols)
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(box + (j * 128 + (row ^ j)) * 4), "f"(x[b * 32 + j]) : "memory");
+          half_sync();
+          float t = -INFINITY, s = 0.0f;
+          if (is) {
+            float y[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y[k]) : "r"(box + (lane * 128 + ((quarter * 32 + k) ^ lane)) * 4));
+              if (quarter * 32 + k >= valid) y[k] = -INFINITY;
+            }
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) t = max3(t, y[k], y[k + 1]);
+            const float ref = t == -INFINITY ? 0.0f : t;
+            float e[4] = {};
+#pragma unroll
+            for (int k = 0; k < 32; ++k) e[k & 3] += exp2_of((y[k] - ref) * kLog2e);
+            s = (e[0] + e[1]) + (e[2] + e[3]);
+            const int64_t own = p.targets[r] - v0;
+            if (own >= quarter * 32 && own < min(valid, quarter * 32 + 32)) {
+              float at_target;
+              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(at_target) : "r"(box + (lane * 128 + ((int)own ^ lane)) * 4));
+              p.xt[r] = at_target;
+            }
+          }
+          half_sync();
+          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(box + (quarter * 32 + lane) * 8), "f"(t), "f"(s) : "memory");
+          half_sync();
+          if (quarter == 0 && is) {
+            float2 q[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(q[k].x), "=f"(q[k].y) : "r"(box + (k * 32 + lane) * 8));
+            t = fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x));
+            const float ref = t == -INFINITY ? 0.0f : t;
+            s = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s += q[k].y * exp2_of((q[k].x - ref) * kLog2e);
+            p.part[(int64_t)(it.m0 / p.tile_m * 2 + rank) * p.N + r] = make_float2(t, s);
+          }
         }
       }
       if constexpr (MODE == STATS) {
@@ -650,7 +721,7 @@ constexpr int kRowThreads = 256;
 // Joins the runs' parts of a row's sum, LANES threads to a row (32 where few rows are in many
 // parts).  A reduced loss: the CTAs' sums, which the last CTA adds up in order.
 template <int LANES>
-__global__ void __launch_bounds__(kRowThreads) join_kernel(Problem p, int n_tiles, int m_tiles, int pairs, const float2* part,
+__global__ void __launch_bounds__(kRowThreads) join_kernel(Problem p, int few, int n_tiles, int m_tiles, int pairs, const float2* part,
                                                            const float* xt, float* rows, float* lse, int reduction,
                                                            float* loss, int32_t* count, double2* sums, uint32_t* counter,
                                                            int32_t* status) {
@@ -662,12 +733,19 @@ __global__ void __launch_bounds__(kRowThreads) join_kernel(Problem p, int n_tile
   double sum = 0.0, has = 0.0;
   const int64_t all = (int64_t)m_tiles * n_tiles, from = (int64_t)(n / kTileM) * n_tiles;
   const int parts =
-      n < p.N ? 2 * ((int)(((from + n_tiles) * pairs - 1) / all) - (int)(((from + 1) * pairs - 1) / all) + 1) : 0;
+      n >= p.N ? 0
+      : few    ? 2 * m_tiles
+               : 2 * ((int)(((from + n_tiles) * pairs - 1) / all) - (int)(((from + 1) * pairs - 1) / all) + 1);
   float m = -INFINITY, l = 0.0f;
-  for (int i = threadIdx.x % LANES; i < parts; i += LANES) {
-    const float2 q = part[(int64_t)i * p.N + n];
-    const float t = fmaxf(m, q.x), ref = t == -INFINITY ? 0.0f : t;
-    l = l * expf(m - ref) + q.y * expf(q.x - ref);
+  for (int i = threadIdx.x % LANES; i < parts; i += 4 * LANES) {
+    float2 q[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      q[k] = i + k * LANES < parts ? part[(int64_t)(i + k * LANES) * p.N + n] : make_float2(-INFINITY, 0.0f);
+    const float t = fmaxf(m, fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x))), ref = t == -INFINITY ? 0.0f : t;
+    l *= expf(m - ref);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) l += q[k].y * expf(q[k].x - ref);
     m = t;
   }
 #pragma unroll
@@ -1024,23 +1102,34 @@ struct Forward {
   float* xt;
   double2* sums;
   uint32_t* counter;
-  int tile_n, m_tiles, n_tiles, pairs, slots;
+  int few, tile_m, tile_n, m_tiles, n_tiles, pairs, slots;
   Forward(Layout& a, const Shape& s, bool h_direct, bool w_direct) {
-    // the width that leaves the pairs' last round fullest: 32000 columns for one tile of
-    // rows take two rounds of 74 either way, of 256 or of 224 columns
-    m_tiles = ceil_div(s.N, kTileM);
-    int64_t least = INT64_MAX;
-    tile_n = kTileN;
-    for (int t = kTileN; t >= 192; t -= 32) {
-      const int64_t all = (int64_t)m_tiles * ceil_div(s.V, t), cost = (all + s.pairs - 1) / s.pairs * t;
-      if (cost * 33 < least * 32) {
-        least = cost;
-        tile_n = t;
+    few = s.N <= kFew;
+    if (few) {
+      // the vocabulary in as many tiles as there are CTAs, or twice, .. as many, of equal height
+      const int rounds = ceil_div(s.V, 256 * s.pairs);
+      tile_m = 2 * std::min(128, (int)up(ceil_div(s.V, 2 * s.pairs * rounds), 8));
+      tile_n = (int)up(s.N, 32);
+      m_tiles = ceil_div(s.V, tile_m);
+      n_tiles = 1;
+      slots = m_tiles;
+    } else {
+      // the width that leaves the pairs' last round fullest: 32000 columns for one tile of
+      // rows take two rounds of 74 either way, of 256 or of 224 columns
+      tile_m = tile_n = kTileM;
+      m_tiles = ceil_div(s.N, kTileM);
+      int64_t least = INT64_MAX;
+      for (int t = kTileN; t >= 192; t -= 32) {
+        const int64_t all = (int64_t)m_tiles * ceil_div(s.V, t), cost = (all + s.pairs - 1) / s.pairs * t;
+        if (cost * 33 < least * 32) {
+          least = cost;
+          tile_n = t;
+        }
       }
+      n_tiles = ceil_div(s.V, tile_n);
     }
-    n_tiles = ceil_div(s.V, tile_n);
     pairs = (int)std::min<int64_t>(s.pairs, (int64_t)m_tiles * n_tiles);
-    slots = ceil_div(pairs, m_tiles) + 1;
+    if (!few) slots = ceil_div(pairs, m_tiles) + 1;
     h = h_direct ? nullptr : a.take<uint16_t>((int64_t)s.N * s.h_parts * s.dp);
     w = w_direct ? nullptr : a.take<uint16_t>((int64_t)s.V * s.w_parts * s.dp);
     part = a.take<float2>((int64_t)slots * 2 * s.N);
@@ -1158,14 +1247,30 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   const Operand ho(h, ldh, N, f.h, s.h_parts, s), wo(w, ldw, V, f.w, s.w_parts, s);
   Args p{};
   Gemm& g = p.g[0];
-  if (!map_of(&g.a, ho.at, s.type, N, ho.cols, ho.ld, 128) || !map_of(&g.b, wo.at, s.type, V, wo.cols, wo.ld, f.tile_n / 2))
+  const Operand &ao = f.few ? wo : ho, &bo = f.few ? ho : wo;
+  if (!map_of(&g.a, ao.at, s.type, f.few ? V : N, ao.cols, ao.ld, f.tile_m / 2) ||
+      !map_of(&g.b, bo.at, s.type, f.few ? N : V, bo.cols, bo.ld, f.tile_n / 2))
     return CB_ERR_CUDA;
-  passes_of(s.h_parts, s.w_parts, s.dp, s.dp, g);
+  p.share = 1;
+  if (!f.few) {
+    passes_of(s.h_parts, s.w_parts, s.dp, s.dp, g);
+  } else if (s.w_parts == 1 && s.h_parts > 1) {
+    // the rows' parts meet a step of the vocabulary together, which is then read once
+    passes_of(1, 1, 0, 0, g);
+    g.span = kSpan32;
+    p.share = s.h_parts;
+  } else {
+    passes_of(s.w_parts, s.h_parts, s.dp, s.dp, g);
+  }
+  p.part_cols = s.dp;
+  p.stage_bytes = f.tile_m * 64 + p.share * f.tile_n * 64;
+  p.stages = std::min(kMaxStages, kStages * kStageBytes / p.stage_bytes);
   g.m_tiles = f.m_tiles;
   g.n_tiles = f.n_tiles;
   g.k_steps = s.dp / kStep;
   p.pairs = f.pairs;
   p.kind = s.kind();
+  p.tile_m = f.tile_m;
   p.tile_n = f.tile_n;
   p.N = N;
   p.V = p.vp = V;
@@ -1174,10 +1279,10 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   p.xt = f.xt;
   p.counter = f.counter;
   p.status = status;
-  if (int rc = launch<STATS>(p, st)) return rc;
+  if (int rc = f.few ? launch<FEW>(p, st) : launch<STATS>(p, st)) return rc;
   const int lanes = f.lanes();
   return launch_after(lanes == 32 ? join_kernel<32> : join_kernel<4>, dim3(f.join_ctas(N)), kRowThreads, 0, st,
-                      Problem{N, V, d, p.targets}, f.n_tiles, f.m_tiles, f.pairs, f.part, f.xt, loss, lse, reduction, loss,
+                      Problem{N, V, d, p.targets}, f.few, f.n_tiles, f.m_tiles, f.pairs, f.part, f.xt, loss, lse, reduction, loss,
                       count, f.sums, f.counter, status);
 }
 
@@ -1216,6 +1321,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   g.m_tiles = m_tiles;
   g.k_steps = s.dp / kStep;
   q.kind = s.kind();
+  q.tile_m = kTileM;
   q.tile_n = kTileN;
   q.N = N;
   q.V = V;
