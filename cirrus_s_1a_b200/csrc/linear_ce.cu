@@ -18,8 +18,11 @@
 // sum over them; a second kernel joins the runs in order.  Backward: G of a piece of the
 // vocabulary goes to memory in the operands' type, both products of the piece follow in one
 // launch; dh adds the pieces up in float32.
-// float32 operands are three bf16 parts each (8 + 8 + 8 bits, and float32's range), six
-// products of parts (what is left out is below 2^-24 of a product), three against bf16.
+// float32 operands are two f16 parts each (11 + 11 bits, of the value times 2^8), three
+// products of parts (what is left out is below 2^-24 of a product), where the values lie in
+// the range that this is right for, which the kernel that makes the parts finds out; else
+// three bf16 parts (8 + 8 + 8 bits, and float32's range), six products.  Against bf16: three
+// bf16 parts, three products.
 // Every wait is bounded (%globaltimer); one that gives up sets CB_ERR_TIMEOUT.
 #include <cuda.h>
 
@@ -61,25 +64,28 @@ struct alignas(64) Gemm {
   CUtensorMap a, b, out;
   int a_mn, b_mn;                  // read across K
   int a_base, b_base;              // added to the row it is read at
-  int passes;
-  int a_part[kMaxPasses], b_part[kMaxPasses];
+  // for operands in bf16 (or 16 bits as they came), and for float32 ones in f16
+  int passes[2], a_part[2][kMaxPasses], b_part[2][kMaxPasses];
+  int span[2];                     // steps of K that are added up in tensor memory
   int m_tiles, n_tiles, k_steps;   // k_steps of a pass
-  int span;                        // steps of K that are added up in tensor memory
   int splits;                      // of K, each with an output of its own
   int out_f32, out_mode, split_mode;  // of the first split and of the others
   int out_rows;                    // between the splits' outputs
-  const float* scale;              // the output's, in memory (PRODUCTS; null: none), times scale_by
-  float scale_by;
+  const float* top;                // PRODUCTS: the output is final, G's units to be multiplied in (null: not yet)
 };
+
+constexpr uint32_t kKindF16 = 1u << 4, kKindBf16 = 1u << 4 | 1u << 7 | 1u << 10;  // D float32; A and B
 
 struct alignas(64) Args {
   Gemm g[2];                       // STATS, GRAD: one; PRODUCTS: dW, dh
   int pairs;
   int whole;                       // PRODUCTS: items of dW, dealt in turn
   int from[kMaxPairs + 1];         // and where each pair's steps of dh begin
+  const uint32_t* wide;            // float32 pairs: 0 where their parts are f16 (null: other types)
   uint32_t kind;                   // instruction descriptor without sizes and directions
   int tile_m, tile_n;              // rows and columns of a tile (PRODUCTS: kTileM, kTileN)
-  int share;                       // FEW: parts of the rows' operand that a step of the vocabulary's meets
+  int share;                       // FEW: parts of the rows' operand that a step of the vocabulary's meets, the
+                                   // smaller ones in an accumulator kFew columns further
   int part_cols;                   // and the columns between them
   int stages, stage_bytes;         // FEW
   // STATS, FEW and GRAD: rows, vocabulary rows, the vocabulary row that the tiles start at, and how many
@@ -89,10 +95,11 @@ struct alignas(64) Args {
   float2* part;                    // STATS: [slots][2][N]; FEW: [tiles][2][N]
   float* xt;                       // [N]
   uint32_t* counter;               // set to 0
-  const float4* rows;              // GRAD: (a, b, lse, -) of each row
+  const float* row_scale;          // STATS, FEW, f16 parts: what a row's logits are multiplied by
+  const float4* rows;              // GRAD: (a, b, lse, that) of each row
   const float* top;                // and their largest factor
   int g_parts, g_cols;             // of G: columns of one part
-  int is_f16;
+  int is_f16;                      // 16-bit operands are f16
   int32_t* status;
 };
 
@@ -246,6 +253,18 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return r;
 }
 
+__device__ __forceinline__ float2 unpack_bf16(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t u) { return __half22float2(reinterpret_cast<const __half2&>(u)); }
+
+// float32 as two f16 parts.  W, and h as dW's operand: of the value times 2^8, right for
+// values below 255 in rows whose largest is 2^-10 or more, against which what lies below
+// f16's range, 2^-33, is 2^-23.  h in front of the logits: of the row times the power of two
+// that brings its largest value to [2^14, 2^15), so that no row depends on another.
+constexpr int kNarrowShift = 8;
+constexpr float kNarrowMost = 255.0f, kNarrowLeast = 1.0f / 1024;
+
 // G is held in units of the largest |a| or |b| of the call, `top`: a mean's G is p - [v = t]
 // itself, whose largest entries lie below 1, where their rounding is smallest against them.
 // float16, whose range ends soon: G of row n is held times 2^(13 + e), e >= 0 the exponent
@@ -261,6 +280,10 @@ __device__ __forceinline__ int row_exponent(float4 row, float top) {
   int e = 0;
   if (size > 0.0f && size < INFINITY) frexpf(size, &e);
   return min(max(e - 2, -100), 0);
+}
+// What a product of G (16 bits or parts of float32) is multiplied by, beside top and rows' exponents.
+__device__ __forceinline__ float product_scale(bool f16, bool narrow) {
+  return f16 ? 1.0f / (1 << (kF16Shift + (narrow ? kNarrowShift : 0))) : 1.0f;
 }
 
 // ------------------------------------------------------------------- work
@@ -365,6 +388,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   start_next();
   if (MODE <= FEW && blockIdx.x == 0 && tid == 0) *p.counter = 0;
   const uint32_t tmem = s_tmem;
+  const bool narrow = p.wide && *p.wide == 0;  // float32 in f16 parts
   volatile int* abort_flag = &s_abort;
   auto wait = [&](uint32_t bar, uint32_t parity) {
     if (*abort_flag) return false;
@@ -385,9 +409,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         const int m = it.m0 + rank * m_rows, c = it.n0 + rank * n_rows;
         const uint32_t bytes = 2 * (m_rows + (MODE == FEW ? p.share : 1) * n_rows) * 128;
         // a span of K at a time, all passes over it
-        for (int from = 0; go && from < it.steps; from += g.span)
-          for (int pass = 0; go && pass < g.passes; ++pass) {
-            const int ap = g.a_part[pass], bp = g.b_part[pass], end = min(from + g.span, it.steps);
+        const int span = g.span[narrow], passes = g.passes[narrow];
+        for (int from = 0; go && from < it.steps; from += span)
+          for (int pass = 0; go && pass < passes; ++pass) {
+            const int ap = g.a_part[narrow][pass], bp = g.b_part[narrow][pass], end = min(from + span, it.steps);
             for (int k = from; k < end; ++k, ++n) {
               const int st = n % stages, k0 = (it.first + k) * kStep;
               if (n >= stages && !wait(empty + 8 * st, (n / stages - 1) & 1)) {
@@ -427,12 +452,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       for (int i = 0; go && item_of<MODE>(p, pair, i, it); ++i) {
         const Gemm& g = p.g[MODE == PRODUCTS ? it.gemm : 0];
         const bool a_mn = MODE == PRODUCTS && g.a_mn;
-        const uint32_t id = p.kind | (a_mn ? 1u << 15 : 0u) | (MODE == PRODUCTS ? 1u << 16 : 0u) |
+        const uint32_t id = (narrow ? kKindF16 : p.kind) | (a_mn ? 1u << 15 : 0u) | (MODE == PRODUCTS ? 1u << 16 : 0u) |
                             (uint32_t)((MODE == PRODUCTS ? kTileN : p.tile_n) >> 3) << 17 | (uint32_t)(kTileM >> 4) << 24;
         // 16 of K: 32 bytes of a row, or 16 rows
         const uint32_t a_step = a_mn ? 2048 / 16 : 2, b_step = MODE == PRODUCTS ? 2048 / 16 : 2;
-        for (int from = 0; go && from < it.steps; from += g.span, ++sums) {
-          const int acc = sums & 1, steps = min(g.span, it.steps - from) * g.passes;
+        const int span = g.span[narrow];
+        for (int from = 0; go && from < it.steps; from += span, ++sums) {
+          const int acc = sums & 1, steps = min(span, it.steps - from) * g.passes[narrow];
           if (sums >= 2) go = __all_sync(0xffffffffu, wait(freed + 8 * acc, (sums / 2 - 1) & 1));
           fence_after();
           const uint32_t d = tmem + acc * kTileN;
@@ -447,7 +473,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
               for (int s = 0; s < kStep / 16; ++s) mma(d, a + s * a_step, b + s * b_step, id, k > 0 || s > 0);
               for (int j = 1; j < (MODE == FEW ? p.share : 1); ++j)
 #pragma unroll
-                for (int s = 0; s < kStep / 16; ++s) mma(d, a + s * a_step, b + j * p.tile_n * 4 + s * b_step, id, true);
+                for (int s = 0; s < kStep / 16; ++s)
+                  mma(d + kFew, a + s * a_step, b + j * p.tile_n * 4 + s * b_step, id, k > 0 || j > 1 || s > 0);
               commit(empty + 8 * st);
             }
             __syncwarp();
@@ -467,6 +494,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   } else {
     // ----------------------------------------------------------- epilogue
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const bool f16 = p.is_f16 || narrow;
     const uint32_t box = out_at + half * kOutBytes;
     const bool lead = (warp & 3) == 0 && lane == 0;  // issues the half's copies out
     const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
@@ -502,11 +530,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         if (target >= p.V) target = -1;
         if (MODE == GRAD) {
           f = live ? p.rows[n] : make_float4(0, 0, 0, 0);
-          const float by = p.is_f16 ? ldexpf(1.0f, kF16Shift - row_exponent(f, *p.top)) : 1.0f;
+          const float by = f16 ? ldexpf(1.0f, kF16Shift - row_exponent(f, *p.top)) : 1.0f;
           f.x = f.x / scale_of(*p.top) * by;
           f.y = f.y / scale_of(*p.top) * by;
         }
         if (MODE == STATS) {
+          f.w = live && narrow ? p.row_scale[n] : 1.0f;
           // which of the runs over these rows this one is
           const int64_t all = (int64_t)p.g[0].m_tiles * p.g[0].n_tiles, from = (int64_t)(it.m0 / kTileM) * p.g[0].n_tiles;
           slot = pair - (int)(((from + 1) * p.pairs - 1) / all);
@@ -516,7 +545,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       float x[kCols];
       // this half's columns
       const int cols = MODE == PRODUCTS ? 128 : MODE == FEW ? p.tile_n / 2 : min(128, p.tile_n - half * 128);
-      const int span = p.g[MODE == PRODUCTS ? it.gemm : 0].span;
+      const int span = p.g[MODE == PRODUCTS ? it.gemm : 0].span[narrow];
       bool go = true;
       for (int from = 0; from < it.steps; from += span, ++sums) {
         const int acc = sums & 1;
@@ -530,12 +559,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           for (int c = 0; c < kCols / 32; ++c)
             if (c * 32 < cols) load32(at + c * 32, x + c * 32);
           loads_done();
-        } else {
+        }
+        for (int more = from == 0; more < (MODE == FEW && p.share > 1 ? 2 : 1); ++more) {
 #pragma unroll
           for (int c = 0; c < kCols / 16; ++c)
             if (c * 16 < cols) {
               float y[16];
-              load16(at + c * 16, y);
+              load16(at + more * kFew + c * 16, y);
               loads_done();
 #pragma unroll
               for (int j = 0; j < 16; ++j) x[c * 16 + j] += y[j];
@@ -548,14 +578,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
                        : "memory");
       }
       if (!go) break;
+      if ((MODE == STATS || MODE == GRAD) && narrow)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) x[c] *= f.w;
       const int v = it.n0 + half * 128;  // of the piece, or of d
       const int at = (int)(target - p.v0 - v);  // the target's column
       const bool hit = (MODE == STATS || MODE == GRAD) && target >= 0 && at >= 0 && at < cols;
       if constexpr (MODE == PRODUCTS) {
         const Gemm& g = p.g[it.gemm];
         const int y = it.m0 + rank * 128 + it.split * g.out_rows;
-        if (g.scale) {
-          const float s = scale_of(*g.scale) * g.scale_by;
+        if (g.top) {
+          const float s = scale_of(*g.top) * product_scale(f16, narrow);
 #pragma unroll
           for (int c = 0; c < 128; ++c) x[c] *= s;
         }
@@ -591,11 +624,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           half_sync();
           float t = -INFINITY, s = 0.0f;
           if (is) {
+            const float unit = narrow ? p.row_scale[r] : 1.0f;
             float y[32];
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
               asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y[k]) : "r"(box + (lane * 128 + ((quarter * 32 + k) ^ lane)) * 4));
-              if (quarter * 32 + k >= valid) y[k] = -INFINITY;
+              y[k] = quarter * 32 + k < valid ? y[k] * unit : -INFINITY;
             }
 #pragma unroll
             for (int k = 0; k < 32; k += 2) t = max3(t, y[k], y[k + 1]);
@@ -608,7 +642,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
             if (own >= quarter * 32 && own < min(valid, quarter * 32 + 32)) {
               float at_target;
               asm volatile("ld.shared.f32 %0, [%1];" : "=f"(at_target) : "r"(box + (lane * 128 + ((int)own ^ lane)) * 4));
-              p.xt[r] = at_target;
+              p.xt[r] = at_target * unit;
             }
           }
           half_sync();
@@ -682,13 +716,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if (v + c * 64 >= p.g_cols) continue;
-          for (int part = 0; part < p.g_parts; ++part)
+          const int parts = narrow ? 2 : p.g_parts;
+          for (int part = 0; part < parts; ++part)
             send(&p.g[0].out, part * p.g_cols + v + c * 64, it.m0 + rank * 128, OUT_STORE, [&](int j) {
               float &lo = x[c * 64 + 2 * j], &hi = x[c * 64 + 2 * j + 1];
-              if (p.is_f16) return pack_f16(lo, hi);
-              const uint32_t u = pack_bf16(lo, hi);
-              lo -= __uint_as_float(u << 16);  // what is left for the next part
-              hi -= __uint_as_float(u & 0xFFFF0000u);
+              const uint32_t u = f16 ? pack_f16(lo, hi) : pack_bf16(lo, hi);
+              const float2 is = f16 ? unpack_f16(u) : unpack_bf16(u);
+              lo -= is.x;  // what is left for the next part
+              hi -= is.y;
               return u;
             });
         }
@@ -824,11 +859,13 @@ struct Upstream {
 // rows[n] = (a, b, lse, -) as they come from above, and *top = the largest |a| or |b|: one
 // for all rows of a reduced loss; else a maximum (which does not depend on the order it is
 // taken in), *top starting at 0.
-__global__ void __launch_bounds__(kRowThreads) factors_kernel(Problem p, Upstream u, const float* lse, float4* rows, float* top) {
+__global__ void __launch_bounds__(kRowThreads) factors_kernel(Problem p, Upstream u, const float* lse, float4* rows, float* top,
+                                                              uint32_t* wide) {
   const int n = blockIdx.x * kRowThreads + threadIdx.x;
   const bool common = u.reduction != CB_REDUCE_NONE && !u.lse;
   await_before();
   start_next();
+  if (wide && n == 0) *wide = 0;
   float one = u.loss && u.reduction != CB_REDUCE_NONE ? *u.loss : 0.0f;
   if (u.reduction == CB_REDUCE_MEAN) one /= (float)max(*u.count, 1);
   if (common && n == 0) *top = fabsf(one) < INFINITY ? fabsf(one) : 0.0f;
@@ -847,61 +884,161 @@ __global__ void __launch_bounds__(kRowThreads) factors_kernel(Problem p, Upstrea
   if ((threadIdx.x & 31) == 0 && size > 0.0f) atomicMax(reinterpret_cast<int*>(top), __float_as_int(size));
 }
 
-// Rows as operands: 16-bit ones as they are, float32 ones as three bf16 parts of dp columns
-// each.  rows given: rows without a gradient become zeros; scaled given: a second copy, the
-// others multiplied by 2^row_exponent.  WIDE: rows are 16-byte aligned and d a multiple of 8.
+// A matrix to be made an operand: rows of dp columns a part.  rows given: rows without a
+// gradient become zeros.  scaled given: a second copy for dW, in f16 with row n multiplied by
+// 2^row_exponent.  unit given: h in f16 parts, scaled by rows; what its logits are to be
+// multiplied by.
+struct Source {
+  const void* x;
+  int64_t ld, n;
+  float4* rows;
+  uint16_t *out, *scaled;
+  float* unit;
+  int64_t unit_step;
+};
+struct Sources {
+  Source s[2];
+  int d, dp;
+  const float* top;
+  uint32_t* wide;  // float32 pairs
+};
+
+// Eight columns of a row.  WIDE: rows are 16-byte aligned and d a multiple of 8.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kRowThreads) operand_kernel(const T* x, int64_t ld, int64_t n_rows, int d, int dp,
-                                                              const float4* rows, const float* top, uint16_t* out,
-                                                              uint16_t* scaled) {
-  constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
-  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  const uint32_t pieces = dp / 8;
-  const int64_t n = i < (1ll << 32) ? (int64_t)((uint32_t)i / pieces) : i / pieces;
-  await_before();
-  start_next();
-  if (n >= n_rows) return;
-  const int j0 = (int)(i - n * pieces) * 8;
-  const float4 row = rows ? rows[n] : make_float4(1.0f, 0.0f, 0.0f, 0.0f);
+__device__ __forceinline__ Vec<T, 8> load8(const T* row, int j0, int d) {
   Vec<T, 8> v;
 #pragma unroll
   for (int j = 0; j < 8; ++j) v.v[j] = Elem<T>::put(0.0f);
-  if (has_gradient(row)) {
-    const T* at = x + n * ld + j0;
-    if (WIDE) {
-      if (j0 < d)
+  if (WIDE) {
+    if (j0 < d)
 #pragma unroll
-        for (int k = 0; k < kParts; k += 2)
-          *reinterpret_cast<uint4*>(&v.v[k * 2]) = *reinterpret_cast<const uint4*>(at + k * 2);
+      for (int k = 0; k < 8; k += 16 / sizeof(T)) *reinterpret_cast<uint4*>(&v.v[k]) = *reinterpret_cast<const uint4*>(row + j0 + k);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j0 + j < d) v.v[j] = row[j0 + j];
+  }
+  return v;
+}
+
+// 16-bit rows as they are, float32 ones as three bf16 parts (for pairs of float32 matrices:
+// only where *wide is set).
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kRowThreads) operand_kernel(Sources p, int64_t first, int64_t blocks) {
+  constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
+  await_before();
+  start_next();
+  if (p.wide && *p.wide == 0) return;
+  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+    const bool second = block >= first;
+    const Source& s = p.s[second];
+    const int64_t i = (block - (second ? first : 0)) * kRowThreads + threadIdx.x;
+    const uint32_t pieces = p.dp / 8;
+    const int64_t n = i < (1ll << 32) ? (int64_t)((uint32_t)i / pieces) : i / pieces;
+    if (n >= s.n) continue;
+    const int j0 = (int)(i - n * pieces) * 8;
+    const float4 row = s.rows ? s.rows[n] : make_float4(1.0f, 0.0f, 0.0f, 0.0f);
+    Vec<T, 8> v = load8<T, WIDE>(static_cast<const T*>(s.x) + n * s.ld, j0, has_gradient(row) ? p.d : 0);
+    if constexpr (kParts == 1) {
+      *reinterpret_cast<uint4*>(s.out + n * p.dp + j0) = *reinterpret_cast<const uint4*>(&v);
+      if (!s.scaled) continue;
+      const float by = ldexpf(1.0f, row_exponent(row, *p.top));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v.v[j] = Elem<T>::put(Elem<T>::get(v.v[j]) * by);
+      *reinterpret_cast<uint4*>(s.scaled + n * p.dp + j0) = *reinterpret_cast<const uint4*>(&v);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j0 + j < d) v.v[j] = at[j];
+      for (int k = 0; k < kParts; ++k) {
+        uint32_t u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          u[j] = pack_bf16(v.v[2 * j], v.v[2 * j + 1]);
+          const float2 is = unpack_bf16(u[j]);
+          v.v[2 * j] -= is.x;
+          v.v[2 * j + 1] -= is.y;
+        }
+        const int64_t at = (n * kParts + k) * p.dp + j0;
+        *reinterpret_cast<uint4*>(s.out + at) = make_uint4(u[0], u[1], u[2], u[3]);
+        if (s.scaled) *reinterpret_cast<uint4*>(s.scaled + at) = make_uint4(u[0], u[1], u[2], u[3]);
+      }
     }
   }
-  if (sizeof(T) == 2) {
-    *reinterpret_cast<uint4*>(out + n * dp + j0) = *reinterpret_cast<const uint4*>(&v);
-    if (!scaled) return;
-    const float by = ldexpf(1.0f, row_exponent(row, *top));
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v.v[j] = Elem<T>::put(Elem<T>::get(v.v[j]) * by);
-    *reinterpret_cast<uint4*>(scaled + n * dp + j0) = *reinterpret_cast<const uint4*>(&v);
-    return;
-  }
+}
+
+// Eight float32 values, times `by`, as two f16 parts dp columns apart.
+__device__ __forceinline__ void put_parts(uint16_t* out, int dp, const Vec<float, 8>& v, float by) {
   float r[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) r[j] = Elem<T>::get(v.v[j]);
+  for (int j = 0; j < 8; ++j) r[j] = v.v[j] * by;
 #pragma unroll
-  for (int k = 0; k < kParts; ++k) {
+  for (int k = 0; k < 2; ++k) {
     uint32_t u[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      u[j] = pack_bf16(r[2 * j], r[2 * j + 1]);
-      r[2 * j] -= __uint_as_float(u[j] << 16);
-      r[2 * j + 1] -= __uint_as_float(u[j] & 0xFFFF0000u);
+      u[j] = pack_f16(r[2 * j], r[2 * j + 1]);
+      const float2 part = unpack_f16(u[j]);
+      r[2 * j] -= part.x;
+      r[2 * j + 1] -= part.y;
     }
-    *reinterpret_cast<uint4*>(out + (n * kParts + k) * dp + j0) = make_uint4(u[0], u[1], u[2], u[3]);
+    *reinterpret_cast<uint4*>(out + k * dp) = make_uint4(u[0], u[1], u[2], u[3]);
   }
+}
+
+// float32 rows as two f16 parts (in rows laid out for three), LANES threads to a row; sets
+// *wide where values of W, or of a row of h that counts for dW, do not fit (one that is not
+// finite makes its sums NaN in any form, and is left to).
+template <bool WIDE, int LANES>
+__global__ void __launch_bounds__(kRowThreads) narrow_kernel(Sources p, int64_t first) {
+  const bool second = blockIdx.x >= first;
+  const Source& s = p.s[second];
+  const int lane = threadIdx.x % LANES;
+  const int64_t n = ((blockIdx.x - (second ? first : 0)) * kRowThreads + threadIdx.x) / LANES;
+  await_before();
+  start_next();
+  const bool is = n < s.n;
+  const float4 row = is && s.rows ? s.rows[n] : make_float4(1.0f, 0.0f, 0.0f, 0.0f);
+  const int d = is && has_gradient(row) ? p.d : 0, dp = is ? p.dp : 0;
+  const float* x = static_cast<const float*>(s.x) + n * s.ld;
+  uint16_t* out = s.out + n * 3 * p.dp;
+  constexpr int kAhead = 3;  // pieces in flight: a row of 768
+  float top = 0.0f;
+  auto reduce_top = [&] {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  };
+  float by = 1 << kNarrowShift;
+  if (s.unit) {
+    for (int j0 = lane * 8; j0 < dp; j0 += LANES * 8) {
+      const Vec<float, 8> v = load8<float, WIDE>(x, j0, d);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v.v[j]));
+    }
+    reduce_top();
+    int e = 0;
+    if (top > 0.0f && top < INFINITY) frexpf(top, &e);
+    e = min(max(e, -100), 128);
+    by = ldexpf(1.0f, 15 - e);
+    if (is && lane == 0) s.unit[n * s.unit_step] = ldexpf(1.0f, e - 15 - kNarrowShift);
+  }
+  const float dw_by = is && s.scaled ? ldexpf(1.0f, kNarrowShift + row_exponent(row, *p.top)) : 1.0f;
+  for (int j0 = lane * 8; j0 < dp; j0 += kAhead * LANES * 8) {
+    Vec<float, 8> v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) v[i] = load8<float, WIDE>(x, j0 + i * LANES * 8, d);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = j0 + i * LANES * 8;
+      if (j >= dp) break;
+      if (!s.unit)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[i].v[k]));
+      put_parts(out + j, p.dp, v[i], by);
+      if (s.scaled) put_parts(s.scaled + n * 3 * p.dp + j, p.dp, v[i], dw_by);
+    }
+  }
+  if (!s.unit) reduce_top();
+  if (lane == 0 && (!s.unit || s.scaled) && top < INFINITY && (top >= kNarrowMost || (top > 0.0f && top < kNarrowLeast)))
+    *p.wide = 1;
 }
 
 // out[r][j] = the sum of the splits' results, scaled back; 0 in a row without a gradient.
@@ -909,7 +1046,7 @@ __global__ void __launch_bounds__(kRowThreads) operand_kernel(const T* x, int64_
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kRowThreads) finish_kernel(const float* acc, int splits, int64_t split_rows, int da,
                                                              int64_t n_rows, int d, const float4* rows, const float* top,
-                                                             int f16, T* out) {
+                                                             int f16, const uint32_t* wide, T* out) {
   const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
   const uint32_t pieces = d / VEC;
   const int64_t n = i < (1ll << 32) ? (int64_t)((uint32_t)i / pieces) : i / pieces;
@@ -924,8 +1061,9 @@ __global__ void __launch_bounds__(kRowThreads) finish_kernel(const float* acc, i
     for (int c = 0; c < VEC; ++c) s[c] += q.v[c];
   }
   const bool live = !rows || has_gradient(rows[n]);
-  float by = scale_of(*top);
-  if (f16) by = ldexpf(by, (rows ? row_exponent(rows[n], *top) : 0) - kF16Shift);
+  const bool narrow = wide && *wide == 0;
+  float by = scale_of(*top) * product_scale(f16 || narrow, narrow);
+  if (rows && (f16 || narrow)) by = ldexpf(by, row_exponent(rows[n], *top));
   Vec<T, VEC> o;
 #pragma unroll
   for (int c = 0; c < VEC; ++c) o.v[c] = Elem<T>::put(live ? s[c] * by : 0.0f);
@@ -989,17 +1127,19 @@ int piece_of(int32_t N, int32_t V, int parts) {
   return (int)up((V + pieces - 1) / pieces, kTileM);
 }
 
-// The products of parts that matter, the smallest first: what tensor memory cuts off a sum
-// (below) is in proportion to the sum so far.
-int passes_of(int a_parts, int b_parts, int a_cols, int b_cols, Gemm& g) {
-  g.passes = 0;
-  for (int both = 2; both >= 0; --both)
+// The products of parts that matter, those of a smaller part first: what tensor memory cuts
+// off a sum is in proportion to the sum so far.  `least`: the orders of parts, the two added,
+// that are left in.
+int passes_of(Gemm& g, int narrow, int a_parts, int b_parts, int a_cols, int b_cols, int least = 2) {
+  int n = 0;
+  for (int both = least; both >= 0; --both)
     for (int i = std::min(both, a_parts - 1); i >= 0 && both - i < b_parts; --i) {
-      g.a_part[g.passes] = i * a_cols;
-      g.b_part[g.passes++] = (both - i) * b_cols;
+      g.a_part[narrow][n] = i * a_cols;
+      g.b_part[narrow][n++] = (both - i) * b_cols;
     }
-  g.span = g.passes == 1 ? kSpan16 : kSpan32;
-  return g.passes;
+  g.passes[narrow] = n;
+  g.span[narrow] = n == 1 ? kSpan16 : kSpan32;
+  return n;
 }
 
 // How the two products are dealt: dW's tiles split `w` times along K, and the steps of dh
@@ -1058,6 +1198,7 @@ Deal deal(int pairs, int h_tiles, int h_steps, int h_passes, int w_tiles, int w_
 struct Shape {
   int N, V, d, dp;          // dp: columns of a part
   int h_parts, w_parts, g_parts;
+  bool pair;                // both are float32: tried in f16 parts
   CUtensorMapDataType type;  // of operands
   int f16;
   int pairs;                // on this device
@@ -1066,12 +1207,21 @@ struct Shape {
     h_parts = h_dtype == CB_F32 ? 3 : 1;
     w_parts = w_dtype == CB_F32 ? 3 : 1;
     g_parts = h_parts;
+    pair = w_parts == 3;
     f16 = h_dtype == CB_F16;
     type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     pairs = std::min(std::max(1, num_sms() / 2), kMaxPairs);
     piece = piece_of(N, V, g_parts);
   }
-  uint32_t kind() const { return 1u << 4 | (f16 ? 0u : 1u << 7 | 1u << 10); }
+  uint32_t kind() const { return f16 ? kKindF16 : kKindBf16; }
+  // The passes of a product of these parts; float32 pairs: also of their f16 parts.  Returns
+  // how many there will be, as a rule.
+  int passes(Gemm& g, int a_parts, int b_parts, int a_cols, int b_cols, int least = 2) const {
+    const int n = passes_of(g, 0, a_parts, b_parts, a_cols, b_cols, least);
+    return pair ? passes_of(g, 1, 2, 2, a_cols, b_cols, 1) : n;
+  }
+  // dW = G^T h: of h's three parts two where dW has 16 bits
+  int dw_passes(Gemm& g, int g_cols) const { return passes(g, g_parts, h_parts, g_cols, dp, w_parts == 1 ? 1 : 2); }
   int da() const { return (int)up(d, 4); }  // columns of a float32 result
 };
 
@@ -1079,8 +1229,8 @@ struct Shape {
 Deal deal_of(const Shape& s, bool dh, bool dw, int vp, int w_most) {
   Gemm t;
   const int nt = ceil_div(s.d, kTileN);
-  return deal(s.pairs, dh ? ceil_div(s.N, kTileM) * nt : 0, ceil_div(vp, kStep), passes_of(s.g_parts, s.w_parts, 0, 0, t),
-              dw ? ceil_div(vp, kTileM) * nt : 0, ceil_div(s.N, kStep), passes_of(s.g_parts, s.h_parts, 0, 0, t),
+  return deal(s.pairs, dh ? ceil_div(s.N, kTileM) * nt : 0, ceil_div(vp, kStep), s.passes(t, s.g_parts, s.w_parts, 0, 0),
+              dw ? ceil_div(vp, kTileM) * nt : 0, ceil_div(s.N, kStep), s.dw_passes(t, 0),
               2.0 * vp * s.d * 4, w_most);
 }
 
@@ -1101,7 +1251,8 @@ struct Forward {
   float2* part;
   float* xt;
   double2* sums;
-  uint32_t* counter;
+  uint32_t *counter, *wide;
+  float* unit;
   int few, tile_m, tile_n, m_tiles, n_tiles, pairs, slots;
   Forward(Layout& a, const Shape& s, bool h_direct, bool w_direct) {
     few = s.N <= kFew;
@@ -1136,6 +1287,8 @@ struct Forward {
     xt = a.take<float>(s.N);
     sums = a.take<double2>(join_ctas(s.N));
     counter = a.take<uint32_t>(1);
+    wide = s.pair ? a.take<uint32_t>(1) : nullptr;
+    unit = s.pair ? a.take<float>(s.N) : nullptr;
   }
   int lanes() const { return 2 * slots > 16 ? 32 : 4; }  // of a row's parts
   int join_ctas(int N) const { return ceil_div(N, kRowThreads / lanes()); }
@@ -1144,6 +1297,7 @@ struct Forward {
 struct Backward {
   float4* rows;
   float* top;
+  uint32_t* wide;
   uint16_t *h, *hs, *w, *G;
   float *acc, *dw;
   Deal first;
@@ -1157,7 +1311,8 @@ struct Backward {
     rows = a.take<float4>(s.N);
     top = a.take<float>(1);
     h = a.take<uint16_t>((int64_t)s.N * s.h_parts * s.dp);
-    hs = s.f16 && want_w ? a.take<uint16_t>((int64_t)s.N * s.dp) : h;
+    wide = s.pair ? a.take<uint32_t>(1) : nullptr;
+    hs = (s.f16 || s.pair) && want_w ? a.take<uint16_t>((int64_t)s.N * s.h_parts * s.dp) : h;
     w = w_direct ? nullptr : a.take<uint16_t>((int64_t)s.V * s.w_parts * s.dp);
     G = a.take<uint16_t>((int64_t)s.N * s.g_parts * up(vp, kStep));
     acc = want_h ? a.take<float>((int64_t)h_slots * up(s.N, kTileM) * s.da()) : nullptr;
@@ -1171,27 +1326,40 @@ int launch(const Args& p, cudaStream_t st) {
   return launch_after(gemm_kernel<MODE>, dim3(2 * p.pairs), kThreads, kSmem, st, p);
 }
 
-int make_operand(int32_t dtype, const void* x, int64_t ld, int64_t n_rows, const Shape& s, const float4* rows,
-                 const float* top, uint16_t* out, uint16_t* scaled, cudaStream_t st) {
-  const int64_t n = n_rows * (s.dp / 8);
-  const bool wide = s.d % 8 == 0 && aligned_to(x, 16) && ld * dtype_size(dtype) % 16 == 0;
+// Operands from up to two matrices of a type.
+int make_operands(int32_t dtype, const Shape& s, const Source& one, const Source& two, const float* top, uint32_t* wide,
+                  cudaStream_t st) {
+  const int size = dtype_size(dtype);
+  auto pieces = [&](const Source& x) { return !x.n || (aligned_to(x.x, 16) && x.ld * size % 16 == 0); };
+  const bool aligned = s.d % 8 == 0 && pieces(one) && pieces(two);
+  const Sources p{{one, two}, s.d, s.dp, top, wide};
+  if (wide) {
+    const int lanes = s.dp <= 64 ? 8 : 32;
+    auto ctas = [&](const Source& x) { return (x.n * lanes + kRowThreads - 1) / kRowThreads; };
+    auto* fn = lanes == 8 ? (aligned ? narrow_kernel<true, 8> : narrow_kernel<false, 8>)
+                          : (aligned ? narrow_kernel<true, 32> : narrow_kernel<false, 32>);
+    if (int rc = launch_after(fn, dim3((unsigned)(ctas(one) + ctas(two))), kRowThreads, 0, st, p, ctas(one))) return rc;
+  }
+  auto ctas = [&](const Source& x) { return (x.n * (s.dp / 8) + kRowThreads - 1) / kRowThreads; };
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    return launch_after(wide ? operand_kernel<T, true> : operand_kernel<T, false>,
-                        dim3((unsigned)((n + kRowThreads - 1) / kRowThreads)), kRowThreads, 0, st, static_cast<const T*>(x),
-                        ld, n_rows, s.d, s.dp, rows, top, out, scaled);
+    const int64_t blocks = ctas(one) + ctas(two);
+    // the float32 pairs' rarely has anything to do
+    const unsigned grid = (unsigned)(wide ? std::min<int64_t>(blocks, 8 * num_sms()) : blocks);
+    return launch_after(aligned ? operand_kernel<T, true> : operand_kernel<T, false>, dim3(grid), kRowThreads, 0, st, p,
+                        ctas(one), blocks);
   });
 }
 
 int finish(int32_t dtype, const float* acc, int splits, int64_t split_rows, const Shape& s, int64_t n_rows, const float4* rows,
-           const float* top, void* out, cudaStream_t st) {
+           const float* top, const uint32_t* wide, void* out, cudaStream_t st) {
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const bool wide = s.d % 4 == 0 && aligned_to(out, 4 * sizeof(T));
-    const int64_t n = n_rows * (wide ? s.d / 4 : s.d);
-    return launch_after(wide ? finish_kernel<T, 4> : finish_kernel<T, 1>,
+    const bool vecs = s.d % 4 == 0 && aligned_to(out, 4 * sizeof(T));
+    const int64_t n = n_rows * (vecs ? s.d / 4 : s.d);
+    return launch_after(vecs ? finish_kernel<T, 4> : finish_kernel<T, 1>,
                         dim3((unsigned)((n + kRowThreads - 1) / kRowThreads)), kRowThreads, 0, st, acc, splits, split_rows,
-                        s.da(), n_rows, s.d, rows, top, s.f16, static_cast<T*>(out));
+                        s.da(), n_rows, s.d, rows, top, s.f16, wide, static_cast<T*>(out));
   });
 }
 
@@ -1240,10 +1408,16 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   Layout a{static_cast<char*>(scratch)};
   const Forward f(a, s, direct(h, h_dtype, ldh, N), direct(w, w_dtype, ldw, V));
   if (scratch_bytes < a.used) return CB_ERR_WORKSPACE;
-  if (f.h)
-    if (int rc = make_operand(h_dtype, h, ldh, N, s, nullptr, nullptr, f.h, nullptr, st)) return rc;
-  if (f.w)
-    if (int rc = make_operand(w_dtype, w, ldw, V, s, nullptr, nullptr, f.w, nullptr, st)) return rc;
+  const Source none{}, hs{h, ldh, N, nullptr, f.h, nullptr, f.unit, 1}, ws{w, ldw, V, nullptr, f.w, nullptr, nullptr, 0};
+  if (s.pair) {
+    if (cudaMemsetAsync(f.wide, 0, sizeof(uint32_t), st) != cudaSuccess) return CB_ERR_CUDA;
+    if (int rc = make_operands(CB_F32, s, ws, hs, nullptr, f.wide, st)) return rc;
+  } else {
+    if (f.h)
+      if (int rc = make_operands(h_dtype, s, hs, none, nullptr, nullptr, st)) return rc;
+    if (f.w)
+      if (int rc = make_operands(w_dtype, s, ws, none, nullptr, nullptr, st)) return rc;
+  }
   const Operand ho(h, ldh, N, f.h, s.h_parts, s), wo(w, ldw, V, f.w, s.w_parts, s);
   Args p{};
   Gemm& g = p.g[0];
@@ -1253,14 +1427,14 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
     return CB_ERR_CUDA;
   p.share = 1;
   if (!f.few) {
-    passes_of(s.h_parts, s.w_parts, s.dp, s.dp, g);
+    s.passes(g, s.h_parts, s.w_parts, s.dp, s.dp);
   } else if (s.w_parts == 1 && s.h_parts > 1) {
     // the rows' parts meet a step of the vocabulary together, which is then read once
-    passes_of(1, 1, 0, 0, g);
-    g.span = kSpan32;
+    s.passes(g, 1, 1, 0, 0);
+    g.span[0] = kSpan32;
     p.share = s.h_parts;
   } else {
-    passes_of(s.w_parts, s.h_parts, s.dp, s.dp, g);
+    s.passes(g, s.w_parts, s.h_parts, s.dp, s.dp);
   }
   p.part_cols = s.dp;
   p.stage_bytes = f.tile_m * 64 + p.share * f.tile_n * 64;
@@ -1278,6 +1452,8 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   p.part = f.part;
   p.xt = f.xt;
   p.counter = f.counter;
+  p.wide = f.wide;
+  p.row_scale = f.unit;
   p.status = status;
   if (int rc = f.few ? launch<FEW>(p, st) : launch<STATS>(p, st)) return rc;
   const int lanes = f.lanes();
@@ -1304,11 +1480,16 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   const Problem pb{N, V, d, Ids{targets, targets_64}};
   const Upstream u{g_loss, g_lse, g_loss_step, g_lse_step, count, reduction};
   if ((reduction == CB_REDUCE_NONE || g_lse) && cudaMemsetAsync(f.top, 0, sizeof(float), st) != cudaSuccess) return CB_ERR_CUDA;
-  if (int rc = launch_after(factors_kernel, dim3(ceil_div(N, kRowThreads)), kRowThreads, 0, st, pb, u, lse, f.rows, f.top))
+  if (int rc = launch_after(factors_kernel, dim3(ceil_div(N, kRowThreads)), kRowThreads, 0, st, pb, u, lse, f.rows, f.top,
+                            f.wide))
     return rc;
-  if (int rc = make_operand(h_dtype, h, ldh, N, s, f.rows, f.top, f.h, f.hs != f.h ? f.hs : nullptr, st)) return rc;
-  if (f.w)
-    if (int rc = make_operand(w_dtype, w, ldw, V, s, nullptr, nullptr, f.w, nullptr, st)) return rc;
+  const Source none{}, ws{w, ldw, V, nullptr, f.w, nullptr, nullptr, 0};
+  const Source hs{h, ldh, N, f.rows, f.h, f.hs != f.h ? f.hs : nullptr, s.pair ? &f.rows->w : nullptr, 4};
+  if (int rc = s.pair ? make_operands(CB_F32, s, ws, hs, f.top, f.wide, st)
+                      : make_operands(h_dtype, s, hs, none, f.top, nullptr, st))
+    return rc;
+  if (f.w && !s.pair)
+    if (int rc = make_operands(w_dtype, s, ws, none, nullptr, nullptr, st)) return rc;
   const Operand wo(w, ldw, V, f.w, s.w_parts, s);
   const int64_t h_cols = (int64_t)s.h_parts * s.dp;
   const int nt = ceil_div(d, kTileN), m_tiles = ceil_div(N, kTileM);
@@ -1317,7 +1498,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   Gemm& g = q.g[0];
   if (!map_of(&g.a, f.h, s.type, N, h_cols, h_cols, 128) || !map_of(&g.b, wo.at, s.type, V, wo.cols, wo.ld, kTileN / 2))
     return CB_ERR_CUDA;
-  passes_of(s.h_parts, s.w_parts, s.dp, s.dp, g);
+  s.passes(g, s.h_parts, s.w_parts, s.dp, s.dp);
   g.m_tiles = m_tiles;
   g.k_steps = s.dp / kStep;
   q.kind = s.kind();
@@ -1330,10 +1511,12 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   q.top = f.top;
   q.g_parts = s.g_parts;
   q.is_f16 = s.f16;
+  q.wide = f.wide;
   q.status = status;
   Args r{};  // both products of a piece
   r.kind = q.kind;
   r.is_f16 = s.f16;
+  r.wide = f.wide;
   r.status = status;
   const int64_t slot = up(N, kTileM) * s.da();  // floats of one of dh's
   if (dh && f.h_slots > 1 && cudaMemsetAsync(f.acc + slot, 0, (f.h_slots - 1) * slot * sizeof(float), st) != cudaSuccess)
@@ -1358,7 +1541,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
       if (!map_of(&gh.a, f.G, s.type, N, g_ld, g_ld, 128) || !map_of(&gh.b, wo.at, s.type, V, wo.cols, wo.ld, 64) ||
           !map_of(&gh.out, f.acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.h_slots * up(N, kTileM), s.da(), s.da(), 128))
         return CB_ERR_CUDA;
-      passes_of(s.g_parts, s.w_parts, cols, s.dp, gh);
+      s.passes(gh, s.g_parts, s.w_parts, cols, s.dp);
       gh.b_mn = 1;
       gh.b_base = v0;
       gh.m_tiles = m_tiles;
@@ -1371,7 +1554,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
     }
     if (dw) {
       if (!map_of(&gw.a, f.G, s.type, N, g_ld, g_ld, 64) ||
-          !map_of(&gw.b, s.f16 ? f.hs : f.h, s.type, N, s.f16 ? s.dp : h_cols, s.f16 ? s.dp : h_cols, 64))
+          !map_of(&gw.b, f.hs, s.type, N, h_cols, h_cols, 64))
         return CB_ERR_CUDA;
       const bool ok =
           f.dw_direct
@@ -1380,7 +1563,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
               : map_of(&gw.out, f.dw, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.first.w * up(std::min(s.piece, V), kTileM), s.da(),
                        s.da(), 128);
       if (!ok) return CB_ERR_CUDA;
-      passes_of(s.g_parts, s.h_parts, cols, s.dp, gw);
+      s.dw_passes(gw, cols);
       gw.a_mn = gw.b_mn = 1;
       gw.m_tiles = ceil_div(vp, kTileM);
       gw.n_tiles = nt;
@@ -1388,19 +1571,16 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
       gw.splits = sp.w;
       gw.out_f32 = !f.dw_direct || w_dtype == CB_F32;
       gw.out_rows = (int)up(std::min(s.piece, V), kTileM);
-      if (f.dw_direct) {
-        gw.scale = f.top;
-        gw.scale_by = s.f16 ? 1.0f / (1 << kF16Shift) : 1.0f;
-      }
+      if (f.dw_direct) gw.top = f.top;
       r.whole = gw.m_tiles * nt * sp.w;
     }
     r.pairs = s.pairs;
     if (int rc = launch<PRODUCTS>(r, st)) return rc;
     if (dw && !f.dw_direct)
-      if (int rc = finish(w_dtype, f.dw, sp.w, up(std::min(s.piece, V), kTileM), s, vp, nullptr, f.top,
+      if (int rc = finish(w_dtype, f.dw, sp.w, up(std::min(s.piece, V), kTileM), s, vp, nullptr, f.top, f.wide,
                           static_cast<char*>(dw) + (int64_t)v0 * d * dtype_size(w_dtype), st))
         return rc;
   }
   if (!dh) return CB_OK;
-  return finish(h_dtype, f.acc, f.h_slots, up(N, kTileM), s, N, f.rows, f.top, dh, st);
+  return finish(h_dtype, f.acc, f.h_slots, up(N, kTileM), s, N, f.rows, f.top, f.wide, dh, st);
 }
