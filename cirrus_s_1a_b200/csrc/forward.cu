@@ -758,7 +758,8 @@ static int forward(const CbModel* mp, const CbCache* cp, const Kv8Run* kv8_in, v
     const int out_off = c0 + tc - asked - (T - nq);  // first logits row of this chunk, per sequence
     const bool direct = (tc == T) && logits != nullptr;
     float* lg = direct ? logits : w.logits;
-    CB_TRY(proj(w, m.lm_head, xo, d, RO, m.final_norm, m.norm_eps, PRE_RMSNORM, EPI_STORE, lg, V, V, st));
+    if (logits || argmax)
+      CB_TRY(proj(w, m.lm_head, xo, d, RO, m.final_norm, m.norm_eps, PRE_RMSNORM, EPI_STORE, lg, V, V, st));
     if (logits && !direct) {
       scatter_rows_kernel<float><<<RO, 256, 0, st>>>(lg, V, asked, nq, out_off, logits);
       count_launch();

@@ -27,6 +27,8 @@ from cirrus_s_1a_b200._lib import (CB_LAYER_GDN, CB_LAYER_SWA, CB_MAX_T, CB_PREF
                                    CbMatrix, CbModel,
                                    CbMtp, CbSliced)
 from cirrus_s_1a_b200.kv8 import Kv8Cache
+from cirrus_s_1a_b200.loss import CrossEntropy, linear_cross_entropy
+from cirrus_s_1a_b200.norm import rms_norm
 
 
 def pad16(n: int) -> int:
@@ -214,7 +216,8 @@ class DeviceModel:
             L.down = pack(p + "ffn.down.weight").struct()
             L.down_ks = sliced(p + "ffn.down.weight", 16)
             L.q_norm = keep(sd[p + "mixer.q_norm.weight"])
-        m.final_norm = keep(sd["final_norm.weight"])
+        self.final_norm = f32(sd["final_norm.weight"])
+        m.final_norm = self.final_norm.data_ptr()
         self.lm_head = pack("lm_head.weight")
         m.lm_head = self.lm_head.struct()
         self.desc = m
@@ -415,6 +418,7 @@ class CirrusB200:
             self.model = DeviceModel(cfg, state_dict, self.device, tensor_scale, path)
         self.draft_ids = state_dict.get("draft_ids", torch.arange(min(cfg.mtp_draft_vocab, cfg.vocab_size)))
         self._ws: dict = {}
+        self._head: torch.Tensor | None = None
 
     # ----------------------------------------------------------- helpers
     def new_cache(self, batch: int = 1, max_ctx: int | None = None, kv8: str | None = None,
@@ -572,9 +576,13 @@ class CirrusB200:
     @torch.no_grad()
     def forward(self, input_ids: torch.Tensor, cache: DeviceCache | None = None, use_cache: bool = False,
                 labels=None, n_logits: int | None = None, **unused) -> Output:
-        """``CirrusModel.forward`` for inference (``model.py:99-176``)."""
+        """``CirrusModel.forward`` for inference (``model.py:99-176``); ``loss`` is its loss
+        on given targets."""
         if labels is not None:
             raise NotImplementedError("training (labels) is outside the B200 decode path")
+        return self._forward(input_ids, cache, use_cache, n_logits, True)
+
+    def _forward(self, input_ids, cache, use_cache, n_logits, want_logits: bool) -> Output:
         if input_ids.dim() != 2:
             raise ValueError("input_ids must be [B, T]")
         B, T = input_ids.shape
@@ -591,7 +599,8 @@ class CirrusB200:
         nq = T if n_logits is None else max(1, min(n_logits, T))
         with torch.cuda.device(self.device):
             ids = input_ids.to(self.device, torch.int64, non_blocking=True).contiguous()
-            logits = torch.empty(B, nq, self.cfg.vocab_size, dtype=torch.float32, device=self.device)
+            logits = (torch.empty(B, nq, self.cfg.vocab_size, dtype=torch.float32, device=self.device)
+                      if want_logits else None)
             hidden = torch.empty(B, nq, self.cfg.d_model, dtype=torch.float32, device=self.device)
             self.launch(cache, ids, T, nq, logits, hidden, None)
         cache.pos_host = [p + T for p in cache.pos_host]
@@ -600,6 +609,39 @@ class CirrusB200:
         return Output(logits=logits, hidden=hidden, cache=cache if want_cache else None)
 
     __call__ = forward
+
+    # ----------------------------------------------------------- loss
+    def dense_head(self) -> torch.Tensor:
+        """The LM head's (and embedding's) quantised weights as a matrix [vocab, d], made once:
+        bfloat16 where that holds them exactly, as it does unless ``tensor_scale`` is odd,
+        else float32."""
+        if self._head is None:
+            V, d = self.cfg.vocab_size, self.cfg.d_model
+            with torch.cuda.device(self.device):
+                ids = torch.arange(V, device=self.device)
+                w = torch.empty(V, d, dtype=torch.float32, device=self.device)
+                _lib.check(_lib.lib().cb_embed(C.byref(self.model.desc.lm_head), ids.data_ptr(), V, w.data_ptr(), None,
+                                               _stream_ptr(self.device)), "cb_embed")
+                short = w.bfloat16()
+                self._head = short if torch.equal(short.float(), w) else w
+        return self._head
+
+    @torch.no_grad()
+    def loss(self, input_ids: torch.Tensor, targets: torch.Tensor, cache: DeviceCache | None = None,
+             reduction: str = "mean", status: torch.Tensor | None = None) -> CrossEntropy:
+        """Cross entropy of ``targets`` [B, T], the token that follows each of ``input_ids``
+        (negative: none), behind what ``cache`` holds, from the hidden states alone: the
+        logits are not kept (``linear_cross_entropy`` over the final norm's output and
+        ``dense_head``).  ``loss`` is [B, T] with reduction "none", ``lse`` always."""
+        if targets.shape != input_ids.shape:
+            raise ValueError(f"targets must be {tuple(input_ids.shape)}, one for each input token")
+        with torch.cuda.device(self.device):
+            out = self._forward(input_ids, cache, cache is not None, None, False)
+            h = rms_norm(out.hidden.flatten(0, 1), self.model.final_norm, self.cfg.norm_eps)
+            t = targets.to(self.device, non_blocking=True).reshape(-1).contiguous()
+            r = linear_cross_entropy(h, self.dense_head(), t, reduction, status)
+        loss = r.loss.view(targets.shape) if reduction == "none" else r.loss
+        return CrossEntropy(loss, r.lse.view(targets.shape))
 
     def eval(self):
         return self

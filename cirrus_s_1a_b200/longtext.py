@@ -12,9 +12,13 @@ by their weight (``Kv8Cache.evict``).  A bf16 cache (``engine.new_cache()``) wor
 the same way without eviction, so the two scores of one text say what the 8 bits
 and the bound cost.
 
+Where only the mean counts, ``mean_loss`` gives it from the hidden states, without the
+logits of a chunk.
+
     python -m cirrus_s_1a_b200.longtext --tokens 8192 --keep 2048
 
-runs a model of random weights both ways and prints the comparison.
+runs a model of random weights both ways and prints the comparison; ``--mean-only`` takes the
+mean alone.
 
 The reference scores a text through its training loss (``cirrus/model/model.py:176-228``).
 """
@@ -44,10 +48,7 @@ def score_text(engine, tokens: torch.Tensor, cache, keep: int | None = None, rec
     B, N = tokens.shape
     if N < 2:
         raise ValueError("scoring needs at least two tokens")
-    if keep is not None and cache.kv8 is None:
-        raise ValueError("keep needs an 8-bit shared cache (kv8=...)")
-    if keep is not None and not cache.add_mass:
-        raise ValueError("eviction goes by attention weights: a cache with add_mass=True")
+    _check_eviction(cache, keep)
     ids = tokens.to(engine.device, torch.int64)
     vocab = engine.cfg.vocab_size
     follow = ids[:, 1:]
@@ -62,11 +63,47 @@ def score_text(engine, tokens: torch.Tensor, cache, keep: int | None = None, rec
         lengths.add(n)
         if keep is not None:
             cache.evict(keep, recent)
+    _check_status(engine, cache, status, lengths, "score_text")
+    return TokenLogprobs(*(torch.cat([x.unflatten(0, (B, -1)) for x in xs], 1) for xs in zip(*parts)))
+
+
+@torch.no_grad()
+def mean_loss(engine, tokens: torch.Tensor, cache, keep: int | None = None, recent: int = 0,
+              chunk: int = CB_PREFILL_CHUNK) -> torch.Tensor:
+    """The mean of -log p over what ``score_text`` scores, as a float32 scalar on the device
+    (``CirrusB200.loss`` for each chunk); ``keep`` and errors as there."""
+    B, N = tokens.shape
+    if N < 2:
+        raise ValueError("scoring needs at least two tokens")
+    _check_eviction(cache, keep)
+    ids = tokens.to(engine.device, torch.int64)
+    status = torch.zeros(1, dtype=torch.int32, device=engine.device)
+    total, lengths = torch.zeros((), dtype=torch.float64, device=engine.device), set()
+    for t in range(0, N - 1, chunk):
+        n = min(chunk, N - 1 - t)
+        # (a token below 0 is one outside the vocabulary, as it is for the model)
+        follow = ids[:, t + 1:t + 1 + n]
+        follow = torch.where(follow < 0, engine.cfg.vocab_size, follow)
+        total += engine.loss(ids[:, t:t + n], follow, cache, reduction="sum", status=status).loss
+        lengths.add(n)
+        if keep is not None:
+            cache.evict(keep, recent)
+    _check_status(engine, cache, status, lengths, "mean_loss")
+    return (total / (B * (N - 1))).float()
+
+
+def _check_eviction(cache, keep) -> None:
+    if keep is not None and cache.kv8 is None:
+        raise ValueError("keep needs an 8-bit shared cache (kv8=...)")
+    if keep is not None and not cache.add_mass:
+        raise ValueError("eviction goes by attention weights: a cache with add_mass=True")
+
+
+def _check_status(engine, cache, status, lengths, what) -> None:
     rc = int(status) or next((r for r in (engine.read_status(cache, n) for n in lengths) if r), 0)
     for n in lengths if rc else ():
         engine.clear_status(cache, n)
-    _lib.check(rc, "score_text")
-    return TokenLogprobs(*(torch.cat([x.unflatten(0, (B, -1)) for x in xs], 1) for xs in zip(*parts)))
+    _lib.check(rc, what)
 
 
 def main() -> None:
@@ -79,6 +116,7 @@ def main() -> None:
     ap.add_argument("--keep", type=int, default=2048, help="slots of the 8-bit cache after each chunk")
     ap.add_argument("--recent", type=int, default=512, help="of them the last ones")
     ap.add_argument("--fmt", choices=("e4m3", "int8"), default="e4m3")
+    ap.add_argument("--mean-only", action="store_true", help="the mean alone, without the logits")
     a = ap.parse_args()
     cfg = replace(baseline_config(), sparse_topk=None)
     engine = CirrusB200(cfg, synthetic.random_state_dict(cfg, seed=0), max_ctx=a.tokens + CB_PREFILL_CHUNK)
@@ -88,13 +126,17 @@ def main() -> None:
               (f"{a.fmt}, {a.keep} slots", engine.new_cache(max_ctx=a.keep + CB_PREFILL_CHUNK, kv8=a.fmt, add_mass=True),
                a.keep))
     first = None
+    score = mean_loss if a.mean_only else score_text
     for name, cache, keep in caches:
-        score_text(engine, text[:, :2 * CB_PREFILL_CHUNK], cache.clone(), keep=keep, recent=min(a.recent, keep or 0))
+        score(engine, text[:, :2 * CB_PREFILL_CHUNK], cache.clone(), keep=keep, recent=min(a.recent, keep or 0))
         torch.cuda.synchronize()
         t0 = time.perf_counter()
-        s = score_text(engine, text, cache, keep=keep, recent=min(a.recent, keep or 0))
+        s = score(engine, text, cache, keep=keep, recent=min(a.recent, keep or 0))
         torch.cuda.synchronize()
         dt = time.perf_counter() - t0
+        if a.mean_only:
+            print(f"{name:>18}: mean log p {-s:.5f}, {(a.tokens - 1) / dt:.0f} tokens/s")
+            continue
         nbytes = cache.kv8.nbytes if cache.kv8 else 2 * cache.kv_k.numel() * 2
         first = s.logprob if first is None else first
         print(f"{name:>18}: mean log p {s.logprob.mean():.5f}, entropy {s.entropy.mean():.5f}, "
