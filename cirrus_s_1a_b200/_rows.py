@@ -91,12 +91,14 @@ def call(device, name: str, *args) -> None:
 def scratch(device, name: str, key: tuple, *args) -> torch.Tensor:
     """Scratch of a call, from the stream's (or the capture's) own memory; its size, which
     ``args`` give, is looked up by ``key``."""
-    n = _sizes.get((name, key))
+    key = (name, device, key)
+    n = _sizes.get(key)
     if n is None:
-        n = getattr(_lib.lib(), name)(*args)
+        with torch.cuda.device(device):
+            n = getattr(_lib.lib(), name)(*args)
         if n == 0:
             raise _lib.CbError(f"{name}: shape not supported")
         if len(_sizes) >= 1024:  # a caller's rows may change with every call
             _sizes.clear()
-        _sizes[(name, key)] = n
+        _sizes[key] = n
     return torch.empty(n, dtype=torch.uint8, device=device)

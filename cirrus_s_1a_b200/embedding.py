@@ -26,11 +26,10 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     stream."""
     if table.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(ids, table, float(scale), status)
-    return _lookup(ids, table, float(scale), status)[0]
+    return _lookup(ids, table, float(scale), status)
 
 
-def _lookup(ids, table, scale, status) -> tuple:
-    """(the rows, whether ids are 64 bits wide)"""
+def _lookup(ids, table, scale, status):
     V, D, ld, code = _rows.vocabulary(table, "table")
     dev = table.device
     wide = _rows.ids(ids, "ids", dev)
@@ -40,23 +39,23 @@ def _lookup(ids, table, scale, status) -> tuple:
     if n:
         _rows.call(dev, "cb_embedding", table.data_ptr(), code, ld, V, D, ids.data_ptr(), wide, n, scale, out.data_ptr(),
                    flag)
-    return out, wide
+    return out
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale, status):
         ctx.save_for_backward(ids)
-        out, wide = _lookup(ids, table, scale, status)
-        ctx.args = scale, table.shape, table.dtype, wide
-        return out
+        ctx.args = scale, table.shape, table.dtype
+        return _lookup(ids, table, scale, status)
 
     @staticmethod
     def backward(ctx, g):
         _rows.once()
         ids, = ctx.saved_tensors
-        scale, (V, D), dtype, wide = ctx.args
+        scale, (V, D), dtype = ctx.args
         n, dev = ids.numel(), ids.device
+        wide = _rows.ids(ids, "ids", dev)
         if n == 0:
             return None, torch.zeros(V, D, dtype=dtype, device=dev), None, None
         g, ldg = _rows.upstream(g.reshape(n, D), D)

@@ -42,8 +42,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     return CrossEntropy(*_forward(hidden, weight, targets, reduction, status)[:2])
 
 
-def _forward(hidden, weight, targets, reduction, status) -> tuple:
-    """(loss, lse, count, the leading arguments of both entry points)"""
+def _arguments(hidden, weight, targets, reduction) -> tuple:
+    """The leading arguments of both entry points."""
     N, D, ldh, h_code = _rows.matrix(hidden, "hidden")
     dev = hidden.device
     V, Dw, ldw, w_code = _rows.vocabulary(weight, "weight", dev)
@@ -58,33 +58,39 @@ def _forward(hidden, weight, targets, reduction, status) -> tuple:
     code = REDUCTIONS.get(reduction)
     if code is None:
         raise ValueError(f"unknown reduction {reduction!r}; choose from {sorted(REDUCTIONS)}")
+    return hidden.data_ptr(), h_code, ldh, weight.data_ptr(), w_code, ldw, N, V, D, targets.data_ptr(), wide, code
+
+
+def _forward(hidden, weight, targets, reduction, status) -> tuple:
+    """(loss, lse, count)"""
+    args = _arguments(hidden, weight, targets, reduction)
+    dev, N = hidden.device, args[6]
     flag = _rows.status(status, dev)
-    args = (hidden.data_ptr(), h_code, ldh, weight.data_ptr(), w_code, ldw, N, V, D, targets.data_ptr(), wide, code)
     lse = torch.empty(N, dtype=torch.float32, device=dev)
     if N == 0:
-        return torch.zeros(() if reduction != "none" else 0, device=dev), lse, None, args
+        return torch.zeros(() if reduction != "none" else 0, device=dev), lse, None
     loss = torch.empty(N if reduction == "none" else (), dtype=torch.float32, device=dev)
     count = None if reduction == "none" else torch.empty(1, dtype=torch.int32, device=dev)
     scratch = _scratch(dev, args, None, 0)
     _rows.call(dev, "cb_linear_ce", *args, loss.data_ptr(), lse.data_ptr(), _lib.ptr(count), scratch.data_ptr(),
                scratch.numel(), flag)
-    return loss, lse, count, args
+    return loss, lse, count
 
 
 def _scratch(dev, args, dw, gradients) -> torch.Tensor:
     h, h_code, ldh, w, w_code, ldw, N, V, D = args[:9]
     at = None if dw is None else dw.data_ptr()
     # what the size goes by, beside the shape: which matrices can be read and written where they lie
-    key = (dev, h_code, w_code, N, V, D, ldh % 8, ldh > 0, ldw % 8, h % 16, w % 16, (at or 0) % 16, gradients)
+    key = (h_code, w_code, N, V, D, ldh % 8, ldh > 0, ldw % 8, h % 16, w % 16, (at or 0) % 16, gradients)
     return _rows.scratch(dev, "cb_linear_ce_scratch_bytes", key, *args[:9], at, gradients)
 
 
 class _LinearCE(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, reduction, status):
-        loss, lse, count, ctx.args = _forward(hidden, weight, targets, reduction, status)
+        loss, lse, count = _forward(hidden, weight, targets, reduction, status)
         ctx.save_for_backward(hidden, weight, targets, lse, count)
-        ctx.status = status
+        ctx.reduction, ctx.status = reduction, status
         ctx.set_materialize_grads(False)
         return loss, lse
 
@@ -95,14 +101,15 @@ class _LinearCE(torch.autograd.Function):
         want_h, want_w = ctx.needs_input_grad[:2]
         if g_loss is None and g_lse is None:
             return None, None, None, None, None
-        dev = hidden.device
-        N, V, D = ctx.args[6:9]
+        # of the tensors as they come back: hooks may have moved them in between
+        args = _arguments(hidden, weight, targets, ctx.reduction)
+        dev, (N, V, D) = hidden.device, args[6:9]
         dh = torch.empty(N, D, dtype=hidden.dtype, device=dev) if want_h else None
         if N == 0:
             return dh, torch.zeros(V, D, dtype=weight.dtype, device=dev) if want_w else None, None, None, None
         dw = torch.empty(V, D, dtype=weight.dtype, device=dev) if want_w else None
-        scratch = _scratch(dev, ctx.args, dw, want_h + 2 * want_w)
-        _rows.call(dev, "cb_linear_ce_grad", *ctx.args, lse.data_ptr(), _lib.ptr(count), _lib.ptr(g_loss), _step(g_loss),
+        scratch = _scratch(dev, args, dw, want_h + 2 * want_w)
+        _rows.call(dev, "cb_linear_ce_grad", *args, lse.data_ptr(), _lib.ptr(count), _lib.ptr(g_loss), _step(g_loss),
                    _lib.ptr(g_lse), _step(g_lse), _lib.ptr(dh), _lib.ptr(dw), scratch.data_ptr(), scratch.numel(),
                    _lib.ptr(ctx.status))
         return dh, dw, None, None, None

@@ -20,41 +20,46 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.
     in x's type; gradients in x's and the weight's.  Runs on the current stream."""
     if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
         return _RMSNorm.apply(x, weight, float(eps))
-    return _norm(x, weight, float(eps))[0]
+    return _norm(x, weight, float(eps))
 
 
-def _norm(x, weight, eps) -> tuple:
-    """(y, the arguments that both entry points share)"""
+def _arguments(x, weight) -> tuple:
+    """(rows, columns, elements between rows, both type codes)"""
     R, D, ld, code = _rows.matrix(x, "x")
-    dev = x.device
-    if weight.shape != (D,) or weight.device != dev or not weight.is_contiguous() \
+    if weight.shape != (D,) or weight.device != x.device or not weight.is_contiguous() \
             or weight.dtype not in (torch.float32, x.dtype):
-        raise ValueError(f"weight must be contiguous, float32 or {x.dtype}, [{D}] on {dev}")
-    w_code = DTYPES[weight.dtype]
+        raise ValueError(f"weight must be contiguous, float32 or {x.dtype}, [{D}] on {x.device}")
+    return R, D, ld, code, DTYPES[weight.dtype]
+
+
+def _norm(x, weight, eps):
+    R, D, ld, code, w_code = _arguments(x, weight)
+    dev = x.device
     y = torch.empty(R, D, dtype=x.dtype, device=dev)
     if R:
         _rows.call(dev, "cb_rms_norm", x.data_ptr(), code, ld, weight.data_ptr(), w_code, R, D, eps, y.data_ptr())
-    return y, (R, D, ld, code, w_code, eps)
+    return y
 
 
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps):
         ctx.save_for_backward(x, weight)
-        y, ctx.args = _norm(x, weight, eps)
-        return y
+        ctx.eps = eps
+        return _norm(x, weight, eps)
 
     @staticmethod
     def backward(ctx, g):
         _rows.once()
         x, weight = ctx.saved_tensors
-        R, D, ld, code, w_code, eps = ctx.args
+        # of the tensors as they come back: hooks may have moved them in between
+        R, D, ld, code, w_code = _arguments(x, weight)
         dev = x.device
         if R == 0:
             return torch.zeros_like(x), torch.zeros_like(weight), None
         g, ldg = _rows.upstream(g, D)
         dx, dw = torch.empty(R, D, dtype=x.dtype, device=dev), torch.empty_like(weight)
         scratch = _rows.scratch(dev, "cb_rms_norm_grad_scratch_bytes", (R, D), R, D)
-        _rows.call(dev, "cb_rms_norm_grad", x.data_ptr(), code, ld, g.data_ptr(), ldg, weight.data_ptr(), w_code, R, D, eps,
-                   dx.data_ptr(), dw.data_ptr(), scratch.data_ptr(), scratch.numel())
+        _rows.call(dev, "cb_rms_norm_grad", x.data_ptr(), code, ld, g.data_ptr(), ldg, weight.data_ptr(), w_code, R, D,
+                   ctx.eps, dx.data_ptr(), dw.data_ptr(), scratch.data_ptr(), scratch.numel())
         return dx, dw, None

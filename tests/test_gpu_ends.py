@@ -92,6 +92,38 @@ def test_a_captured_training_step_and_an_eager_one():
         assert all(torch.equal(x, y) for x, y in zip(outs[:3], want[:3])) and torch.equal(tab, want[3])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_saved_tensors_that_a_hook_moves(dtype):
+    """Tensors kept on the host between forward and backward come back elsewhere, and rows of a
+    wider matrix come back contiguous."""
+    g = torch.Generator().manual_seed(2)
+    big = (torch.randn(300, 100, generator=g) / 8).to(TYPES[dtype]).to(DEV)
+    ids, targets = (torch.randint(0, 300, (200,), generator=g).to(DEV) for _ in range(2))
+    norm = torch.ones(64, device=DEV)
+
+    def step():
+        table, w = big[:, 8:72].detach().requires_grad_(), norm.detach().requires_grad_()
+        with torch.autograd.graph.save_on_cpu() if moved else torch.enable_grad():
+            loss = chain(ids + 0, table, w, targets + 0, 1.0, ours())
+        torch.full((1 << 22,), 7.0, device=DEV)  # over what has been freed
+        return loss, *torch.autograd.grad(loss, (table, w))
+
+    moved = False
+    want = step()
+    moved = True
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+def test_a_gradient_of_a_gradient_is_refused():
+    table = torch.randn(20, 16, device=DEV, requires_grad=True)
+    norm = torch.ones(16, device=DEV, requires_grad=True)
+    ids = torch.arange(10, device=DEV)
+    embed, rms, ce = ours()
+    for out in (embed(ids, table), rms(table, norm), ce(table, table, torch.arange(20, device=DEV))):
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(out.sum(), table, create_graph=True)
+
+
 def engine(**kw):
     from cirrus_s_1a_b200 import synthetic
     from cirrus_s_1a_b200.config import get_config
