@@ -10,7 +10,7 @@
 //   * a pair of CTAs (cta_group::2) owns a 256 x 256 tile: each holds 128 of its rows, the
 //     accumulator in tensor memory (two of them, so that a tile's products run under the
 //     last tile's epilogue), and brings half of the columns' operand;
-//   * a thread of each CTA copies 64-wide steps of K by TMA into six stages, one of the pair
+//   * a thread of each CTA copies 64-wide steps of K by TMA into five stages or more, one of the pair
 //     issues tcgen05.mma, eight warps a CTA take the accumulators out of tensor memory;
 //   * operands lie as the caller has them: logits read h and W along K; dh reads W, and dW
 //     reads G and h, across it (MN-major operands), so that nothing is transposed.
@@ -37,12 +37,12 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTileM = 256, kTileN = 256;  // of a pair
 constexpr int kStep = 64;                  // of K: 128 bytes, a swizzled row
-constexpr int kStages = 6, kMaxStages = 12;
+constexpr int kMaxStages = 12;
 constexpr int kHalfBytes = 128 * kStep * 2;  // one CTA's rows of one operand's step
 constexpr int kStageBytes = 2 * kHalfBytes;
-constexpr int kOutBytes = 128 * 128;  // a box on its way out: 128 rows of 128 bytes, one for each half of the columns
-constexpr int kSmem = kStages * kStageBytes + 2 * kOutBytes + 1024;
 constexpr int kEpiWarps = 8;
+constexpr int kBoxBytes = 32 * 128;  // a box on its way out: a warp's 32 rows, 128 bytes of each
+constexpr int kSmem = 7 * kStageBytes + 1024;
 constexpr int kThreads = kEpiWarps * 32 + 64;
 constexpr int kMaxPasses = 6, kMaxPairs = 128;
 // Sums in tensor memory are cut off, not rounded, after every 16 products: over 48 of them a
@@ -56,6 +56,10 @@ constexpr int kFew = 128;
 
 enum { STATS = 0, FEW = 1, GRAD = 2, PRODUCTS = 3 };
 enum { OUT_STORE = 0, OUT_ADD = 1 };
+// Stages of 32 KiB out of seven; the last is for what goes out.  (Two boxes a warp and five
+// stages: 159 us instead of 152 for G of 16384 x 8192 x 768, the copies in are what waits.)
+constexpr int stages_of(int mode) { return mode == STATS ? 7 : 6; }
+static_assert(kEpiWarps * kBoxBytes == kStageBytes, "a box for each warp takes a stage");
 
 // One matrix product D[m][n] = sum over passes and k of A[m][k] B[n][k].  An operand is a
 // 16-bit matrix read along K (its rows are m or n) or across it (its rows are k); pass i
@@ -332,9 +336,11 @@ __device__ __forceinline__ bool item_of(const Args& p, int pair, int i, Item& it
     it.split = 0;
     for (int c = pair; p.from[c] > tile_at && at == begin; --c) it.split += p.from[c] > p.from[c - 1];
   }
-  it.tile = tile % g.n_tiles;
+  // dW's tiles go by rows of tiles, in turn: pairs that work at one time share their rows of
+  // G^T.  dh's go by columns: the pairs a column of tiles apart share their rows of G.
+  it.tile = it.gemm ? tile / g.m_tiles : tile % g.n_tiles;
   it.n0 = it.tile * kTileN;
-  it.m0 = tile / g.n_tiles * kTileM;
+  it.m0 = (it.gemm ? tile % g.m_tiles : tile / g.n_tiles) * kTileM;
   return true;
 }
 
@@ -359,8 +365,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1;
   const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
-  const uint32_t out_at = base + kStages * kStageBytes;
-  const int stages = MODE == FEW ? p.stages : kStages, stage_bytes = MODE == FEW ? p.stage_bytes : kStageBytes;
+  const uint32_t out_at = base + stages_of(MODE) * kStageBytes;
+  const int stages = MODE == FEW ? p.stages : stages_of(MODE), stage_bytes = MODE == FEW ? p.stage_bytes : kStageBytes;
   const int a_bytes = MODE == FEW ? p.tile_m * 64 : kHalfBytes;  // of a stage
   const uint32_t full = smem_u32(bars), empty = full + 8 * kMaxStages, done = empty + 8 * kMaxStages, freed = done + 16;
 
@@ -495,18 +501,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     // ----------------------------------------------------------- epilogue
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const bool f16 = p.is_f16 || narrow;
-    const uint32_t box = out_at + half * kOutBytes;
-    const bool lead = (warp & 3) == 0 && lane == 0;  // issues the half's copies out
     const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
     auto half_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(half + 1) : "memory"); };
-    // the rows' 128 bytes go out as one box
+    auto warp_bar = [&] { asm volatile("bar.sync %0, 32;" ::"r"(warp + 3) : "memory"); };
+    // the warp's rows, 128 bytes of each, go out as a box
     auto send = [&](const CUtensorMap* map, int x, int y, int mode, auto&& word) {
-      if (lead) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-      half_sync();
-      put_row(box, row, word);
+      const uint32_t box = out_at + warp * kBoxBytes;
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      warp_bar();
+      put_row(box, lane, word);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      half_sync();
-      if (lead) copy_out(map, x, y, box, mode);
+      warp_bar();
+      if (lane == 0) copy_out(map, x, y + (warp & 3) * 32, box, mode);
     };
     float m = -INFINITY, l = 0.0f;  // STATS: of the row over the run
     int run = -1, slot = 0;
@@ -611,6 +617,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         // thread takes a quarter of the tile's logits of one row, a warp joins the quarters.
         const int m_rows = p.tile_m / 2, v0 = it.m0 + rank * m_rows, valid = min(m_rows, p.V - v0);
         const int quarter = warp & 3;
+        const uint32_t box = out_at + half * 4 * kBoxBytes;  // [32][128] logits
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           if (b * 32 >= cols) break;
@@ -716,9 +723,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if (v + c * 64 >= p.g_cols) continue;
-          const int parts = narrow ? 2 : p.g_parts;
-          for (int part = 0; part < parts; ++part)
-            send(&p.g[0].out, part * p.g_cols + v + c * 64, it.m0 + rank * 128, OUT_STORE, [&](int j) {
+          const int parts = narrow ? 2 : p.g_parts, y = it.m0 + rank * 128;
+          int at_part = v + c * 64;
+          for (int part = 1; part < parts; ++part, at_part += p.g_cols)
+            send(&p.g[0].out, at_part, y, OUT_STORE, [&](int j) {
               float &lo = x[c * 64 + 2 * j], &hi = x[c * 64 + 2 * j + 1];
               const uint32_t u = f16 ? pack_f16(lo, hi) : pack_bf16(lo, hi);
               const float2 is = f16 ? unpack_f16(u) : unpack_bf16(u);
@@ -726,11 +734,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
               hi -= is.y;
               return u;
             });
+          if (f16)
+            send(&p.g[0].out, at_part, y, OUT_STORE, [&](int j) { return pack_f16(x[c * 64 + 2 * j], x[c * 64 + 2 * j + 1]); });
+          else
+            send(&p.g[0].out, at_part, y, OUT_STORE, [&](int j) { return pack_bf16(x[c * 64 + 2 * j], x[c * 64 + 2 * j + 1]); });
         }
       }
     }
     if (MODE == STATS) leave();
-    if (lead) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   fence_before();
   __syncthreads();
@@ -1165,7 +1177,7 @@ End end_of(int pairs, int items, double cost, double work) {
 // beside them and what the splits' float32 results cost in memory.
 Deal deal(int pairs, int h_tiles, int h_steps, int h_passes, int w_tiles, int w_steps, int w_passes, double w_bytes,
           int w_most) {
-  constexpr int kTileCost = 6;             // of filling and emptying, in steps
+  constexpr int kTileCost = 2;             // of filling and emptying, in steps
   constexpr double kBytesPerStep = 900e3;  // written and read back in a step's time by the whole device
   const double steps = (double)h_tiles * h_steps, work = steps * h_passes;
   Deal o;
@@ -1435,10 +1447,11 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
     p.share = s.h_parts;
   } else {
     s.passes(g, s.w_parts, s.h_parts, s.dp, s.dp);
+    if (s.pair) g.span[0] = g.span[1] = kSpan32 / 2;  // (the tiles are small)
   }
   p.part_cols = s.dp;
   p.stage_bytes = f.tile_m * 64 + p.share * f.tile_n * 64;
-  p.stages = std::min(kMaxStages, kStages * kStageBytes / p.stage_bytes);
+  p.stages = std::min(kMaxStages, stages_of(FEW) * kStageBytes / p.stage_bytes);
   g.m_tiles = f.m_tiles;
   g.n_tiles = f.n_tiles;
   g.k_steps = s.dp / kStep;
@@ -1524,7 +1537,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   for (int v0 = 0; v0 < V; v0 += s.piece) {
     const int vp = std::min(s.piece, V - v0), cols = (int)up(vp, kStep);
     const int64_t g_ld = (int64_t)s.g_parts * cols;
-    if (!map_of(&g.out, f.G, s.type, N, g_ld, g_ld, 128)) return CB_ERR_CUDA;
+    if (!map_of(&g.out, f.G, s.type, N, g_ld, g_ld, 32)) return CB_ERR_CUDA;
     g.b_base = q.v0 = v0;
     g.n_tiles = ceil_div(vp, kTileN);
     q.vp = vp;
@@ -1539,7 +1552,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
     std::copy(sp.from, sp.from + s.pairs + 1, r.from);
     if (dh) {
       if (!map_of(&gh.a, f.G, s.type, N, g_ld, g_ld, 128) || !map_of(&gh.b, wo.at, s.type, V, wo.cols, wo.ld, 64) ||
-          !map_of(&gh.out, f.acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.h_slots * up(N, kTileM), s.da(), s.da(), 128))
+          !map_of(&gh.out, f.acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.h_slots * up(N, kTileM), s.da(), s.da(), 32))
         return CB_ERR_CUDA;
       s.passes(gh, s.g_parts, s.w_parts, cols, s.dp);
       gh.b_mn = 1;
@@ -1559,9 +1572,9 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
       const bool ok =
           f.dw_direct
               ? map_of(&gw.out, static_cast<char*>(dw) + (int64_t)v0 * d * dtype_size(w_dtype),
-                       w_dtype == CB_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : s.type, vp, d, d, 128)
+                       w_dtype == CB_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : s.type, vp, d, d, 32)
               : map_of(&gw.out, f.dw, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.first.w * up(std::min(s.piece, V), kTileM), s.da(),
-                       s.da(), 128);
+                       s.da(), 32);
       if (!ok) return CB_ERR_CUDA;
       s.dw_passes(gw, cols);
       gw.a_mn = gw.b_mn = 1;
