@@ -391,7 +391,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   cluster_sync();
   fence_after();
   await_before();
-  start_next();
   if (MODE <= FEW && blockIdx.x == 0 && tid == 0) *p.counter = 0;
   const uint32_t tmem = s_tmem;
   const bool narrow = p.wide && *p.wide == 0;  // float32 in f16 parts
@@ -744,6 +743,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     if (MODE == STATS) leave();
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
+  start_next();  // (at the start it would have small kernels wait beside these CTAs: 33 us instead of 27 for 128 rows of float32)
   fence_before();
   __syncthreads();
   cluster_sync();  // no CTA leaves while the pair's products or arrivals may reach it
@@ -1267,7 +1267,9 @@ struct Forward {
   float* unit;
   int few, tile_m, tile_n, m_tiles, n_tiles, pairs, slots;
   Forward(Layout& a, const Shape& s, bool h_direct, bool w_direct) {
-    few = s.N <= kFew;
+    // Float32 rows against bf16 meet each step of the vocabulary once (128 rows, 32000 x 768: 27 us, 34 as rows of a
+    // tile, three passes); otherwise only the fewest gain (5 rows of bf16: 17 and 19 us; 64 rows, 8192 x 1024: 16 and 13).
+    few = s.N <= (s.h_parts > s.w_parts ? kFew : 16);
     if (few) {
       // the vocabulary in as many tiles as there are CTAs, or twice, .. as many, of equal height
       const int rounds = ceil_div(s.V, 256 * s.pairs);
@@ -1277,18 +1279,9 @@ struct Forward {
       n_tiles = 1;
       slots = m_tiles;
     } else {
-      // the width that leaves the pairs' last round fullest: 32000 columns for one tile of
-      // rows take two rounds of 74 either way, of 256 or of 224 columns
-      tile_m = tile_n = kTileM;
+      tile_m = kTileM;
+      tile_n = kTileN;
       m_tiles = ceil_div(s.N, kTileM);
-      int64_t least = INT64_MAX;
-      for (int t = kTileN; t >= 192; t -= 32) {
-        const int64_t all = (int64_t)m_tiles * ceil_div(s.V, t), cost = (all + s.pairs - 1) / s.pairs * t;
-        if (cost * 33 < least * 32) {
-          least = cost;
-          tile_n = t;
-        }
-      }
       n_tiles = ceil_div(s.V, tile_n);
     }
     pairs = (int)std::min<int64_t>(s.pairs, (int64_t)m_tiles * n_tiles);

@@ -243,8 +243,8 @@ bool in_a_warp(const void* x, int64_t ld, int rows, int d, int size) {
 }
 
 // CTAs of the gradient's warps: 16 rows or fewer to one (dw then needs no second kernel), at
-// most three to an SM.
-int grad_ctas(int rows) { return rows <= 2 * kWarps ? 1 : std::min(ceil_div(rows, kWarps), 3 * num_sms()); }
+// most two to an SM (bf16, 65537 x 768 with the forward: 103 us, 121 with three).
+int grad_ctas(int rows) { return rows <= 2 * kWarps ? 1 : std::min(ceil_div(rows, kWarps), 2 * num_sms()); }
 
 template <typename F>
 int with_types(int32_t dtype, int32_t w_dtype, F&& f) {
