@@ -85,7 +85,7 @@ struct alignas(64) Args {
   int pairs;
   int whole;                       // PRODUCTS: items of dW, dealt in turn
   int from[kMaxPairs + 1];         // and where each pair's steps of dh begin
-  const uint32_t* wide;            // float32 pairs: 0 where their parts are f16 (null: other types)
+  const uint32_t* wide;            // 0 where the parts are f16 (null: not tried)
   uint32_t kind;                   // instruction descriptor without sizes and directions
   int tile_m, tile_n;              // rows and columns of a tile (PRODUCTS: kTileM, kTileN)
   int share;                       // FEW: parts of the rows' operand that a step of the vocabulary's meets, the
@@ -912,7 +912,7 @@ struct Sources {
   Source s[2];
   int d, dp;
   const float* top;
-  uint32_t* wide;  // float32 pairs
+  uint32_t* wide;  // set where f16 parts do not fit (null: not tried)
 };
 
 // Eight columns of a row.  WIDE: rows are 16-byte aligned and d a multiple of 8.
@@ -933,8 +933,8 @@ __device__ __forceinline__ Vec<T, 8> load8(const T* row, int j0, int d) {
   return v;
 }
 
-// 16-bit rows as they are, float32 ones as three bf16 parts (for pairs of float32 matrices:
-// only where *wide is set).
+// 16-bit rows as they are, float32 ones as three bf16 parts; after a try in f16 parts only
+// where *wide is set.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kRowThreads) operand_kernel(Sources p, int64_t first, int64_t blocks) {
   constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
@@ -977,13 +977,15 @@ __global__ void __launch_bounds__(kRowThreads) operand_kernel(Sources p, int64_t
   }
 }
 
-// Eight float32 values, times `by`, as two f16 parts dp columns apart.
-__device__ __forceinline__ void put_parts(uint16_t* out, int dp, const Vec<float, 8>& v, float by) {
+// Eight values, times `by`, as f16 parts dp columns apart: two of float32, one of bf16, which
+// f16 holds whole.
+template <typename T>
+__device__ __forceinline__ void put_parts(uint16_t* out, int dp, const Vec<T, 8>& v, float by) {
   float r[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) r[j] = v.v[j] * by;
+  for (int j = 0; j < 8; ++j) r[j] = Elem<T>::get(v.v[j]) * by;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < (int)sizeof(T) / 2; ++k) {
     uint32_t u[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -996,10 +998,10 @@ __device__ __forceinline__ void put_parts(uint16_t* out, int dp, const Vec<float
   }
 }
 
-// float32 rows as two f16 parts (in rows laid out for three), LANES threads to a row; sets
-// *wide where values of W, or of a row of h that counts for dW, do not fit (one that is not
+// float32 rows as two f16 parts (in rows laid out for three), bf16 rows as one, LANES threads
+// to a row; sets *wide where values of W, or of a row of h that counts for dW, do not fit (one that is not
 // finite makes its sums NaN in any form, and is left to).
-template <bool WIDE, int LANES>
+template <typename T, bool WIDE, int LANES>
 __global__ void __launch_bounds__(kRowThreads) narrow_kernel(Sources p, int64_t first) {
   const bool second = blockIdx.x >= first;
   const Source& s = p.s[second];
@@ -1010,8 +1012,9 @@ __global__ void __launch_bounds__(kRowThreads) narrow_kernel(Sources p, int64_t 
   const bool is = n < s.n;
   const float4 row = is && s.rows ? s.rows[n] : make_float4(1.0f, 0.0f, 0.0f, 0.0f);
   const int d = is && has_gradient(row) ? p.d : 0, dp = is ? p.dp : 0;
-  const float* x = static_cast<const float*>(s.x) + n * s.ld;
-  uint16_t* out = s.out + n * 3 * p.dp;
+  constexpr int kLaid = sizeof(T) == 4 ? 3 : 1;
+  const T* x = static_cast<const T*>(s.x) + n * s.ld;
+  uint16_t* out = s.out + n * kLaid * p.dp;
   constexpr int kAhead = 3;  // pieces in flight: a row of 768
   float top = 0.0f;
   auto reduce_top = [&] {
@@ -1021,9 +1024,9 @@ __global__ void __launch_bounds__(kRowThreads) narrow_kernel(Sources p, int64_t 
   float by = 1 << kNarrowShift;
   if (s.unit) {
     for (int j0 = lane * 8; j0 < dp; j0 += LANES * 8) {
-      const Vec<float, 8> v = load8<float, WIDE>(x, j0, d);
+      const Vec<T, 8> v = load8<T, WIDE>(x, j0, d);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v.v[j]));
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(Elem<T>::get(v.v[j])));
     }
     reduce_top();
     int e = 0;
@@ -1034,18 +1037,18 @@ __global__ void __launch_bounds__(kRowThreads) narrow_kernel(Sources p, int64_t 
   }
   const float dw_by = is && s.scaled ? ldexpf(1.0f, kNarrowShift + row_exponent(row, *p.top)) : 1.0f;
   for (int j0 = lane * 8; j0 < dp; j0 += kAhead * LANES * 8) {
-    Vec<float, 8> v[kAhead];
+    Vec<T, 8> v[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) v[i] = load8<float, WIDE>(x, j0 + i * LANES * 8, d);
+    for (int i = 0; i < kAhead; ++i) v[i] = load8<T, WIDE>(x, j0 + i * LANES * 8, d);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int j = j0 + i * LANES * 8;
       if (j >= dp) break;
       if (!s.unit)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[i].v[k]));
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(Elem<T>::get(v[i].v[k])));
       put_parts(out + j, p.dp, v[i], by);
-      if (s.scaled) put_parts(s.scaled + n * 3 * p.dp + j, p.dp, v[i], dw_by);
+      if (s.scaled) put_parts(s.scaled + n * kLaid * p.dp + j, p.dp, v[i], dw_by);
     }
   }
   if (!s.unit) reduce_top();
@@ -1210,7 +1213,7 @@ Deal deal(int pairs, int h_tiles, int h_steps, int h_passes, int w_tiles, int w_
 struct Shape {
   int N, V, d, dp;          // dp: columns of a part
   int h_parts, w_parts, g_parts;
-  bool pair;                // both are float32: tried in f16 parts
+  bool tried;               // float32 rows, in f16 parts if they fit
   CUtensorMapDataType type;  // of operands
   int f16;
   int pairs;                // on this device
@@ -1219,21 +1222,30 @@ struct Shape {
     h_parts = h_dtype == CB_F32 ? 3 : 1;
     w_parts = w_dtype == CB_F32 ? 3 : 1;
     g_parts = h_parts;
-    pair = w_parts == 3;
+    // bf16 W would be read where it lies for bf16 parts: worth a copy in f16 for many rows (the loss of 1100 rows, 32000
+    // x 768: 110 us, 121 in bf16 parts; of 16384 1310 and 2050)
+    tried = w_parts == 3 || (h_parts == 3 && N > 1024);
     f16 = h_dtype == CB_F16;
     type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     pairs = std::min(std::max(1, num_sms() / 2), kMaxPairs);
     piece = piece_of(N, V, g_parts);
   }
   uint32_t kind() const { return f16 ? kKindF16 : kKindBf16; }
-  // The passes of a product of these parts; float32 pairs: also of their f16 parts.  Returns
-  // how many there will be, as a rule.
-  int passes(Gemm& g, int a_parts, int b_parts, int a_cols, int b_cols, int least = 2) const {
-    const int n = passes_of(g, 0, a_parts, b_parts, a_cols, b_cols, least);
-    return pair ? passes_of(g, 1, 2, 2, a_cols, b_cols, 1) : n;
+  // The passes of a product of these parts, and of the f16 parts that take their place (two of
+  // float32, one of bf16).  Returns how many there will be, as a rule.
+  int passes(Gemm& g, int a_parts, int b_parts, int a_cols, int b_cols) const {
+    const int n = passes_of(g, 0, a_parts, b_parts, a_cols, b_cols);
+    return tried ? passes_of(g, 1, std::min(a_parts, 2), std::min(b_parts, 2), a_cols, b_cols, 1) : n;
   }
-  // dW = G^T h: of h's three parts two where dW has 16 bits
-  int dw_passes(Gemm& g, int g_cols) const { return passes(g, g_parts, h_parts, g_cols, dp, w_parts == 1 ? 1 : 2); }
+  // dW = G^T h; where dW is bf16, two of three bf16 parts will do
+  int dw_passes(Gemm& g, int g_cols) const {
+    const int n = passes(g, g_parts, h_parts, g_cols, dp);
+    if (w_parts == h_parts) return n;
+    passes_of(g, 0, g_parts, h_parts, g_cols, dp, 1);
+    return g.passes[tried];
+  }
+  // whether W is read where it lies
+  bool reads_w(const void* w, int32_t w_dtype, int64_t ldw) const { return !tried && direct(w, w_dtype, ldw, V); }
   int da() const { return (int)up(d, 4); }  // columns of a float32 result
 };
 
@@ -1292,8 +1304,8 @@ struct Forward {
     xt = a.take<float>(s.N);
     sums = a.take<double2>(join_ctas(s.N));
     counter = a.take<uint32_t>(1);
-    wide = s.pair ? a.take<uint32_t>(1) : nullptr;
-    unit = s.pair ? a.take<float>(s.N) : nullptr;
+    wide = s.tried ? a.take<uint32_t>(1) : nullptr;
+    unit = s.tried ? a.take<float>(s.N) : nullptr;
   }
   int lanes() const { return 2 * slots > 16 ? 32 : 4; }  // of a row's parts
   int join_ctas(int N) const { return ceil_div(N, kRowThreads / lanes()); }
@@ -1316,8 +1328,8 @@ struct Backward {
     rows = a.take<float4>(s.N);
     top = a.take<float>(1);
     h = a.take<uint16_t>((int64_t)s.N * s.h_parts * s.dp);
-    wide = s.pair ? a.take<uint32_t>(1) : nullptr;
-    hs = (s.f16 || s.pair) && want_w ? a.take<uint16_t>((int64_t)s.N * s.h_parts * s.dp) : h;
+    wide = s.tried ? a.take<uint32_t>(1) : nullptr;
+    hs = (s.f16 || s.tried) && want_w ? a.take<uint16_t>((int64_t)s.N * s.h_parts * s.dp) : h;
     w = w_direct ? nullptr : a.take<uint16_t>((int64_t)s.V * s.w_parts * s.dp);
     G = a.take<uint16_t>((int64_t)s.N * s.g_parts * up(vp, kStep));
     acc = want_h ? a.take<float>((int64_t)h_slots * up(s.N, kTileM) * s.da()) : nullptr;
@@ -1331,29 +1343,61 @@ int launch(const Args& p, cudaStream_t st) {
   return launch_after(gemm_kernel<MODE>, dim3(2 * p.pairs), kThreads, kSmem, st, p);
 }
 
-// Operands from up to two matrices of a type.
-int make_operands(int32_t dtype, const Shape& s, const Source& one, const Source& two, const float* top, uint32_t* wide,
-                  cudaStream_t st) {
-  const int size = dtype_size(dtype);
-  auto pieces = [&](const Source& x) { return !x.n || (aligned_to(x.x, 16) && x.ld * size % 16 == 0); };
-  const bool aligned = s.d % 8 == 0 && pieces(one) && pieces(two);
-  const Sources p{{one, two}, s.d, s.dp, top, wide};
-  if (wide) {
-    const int lanes = s.dp <= 64 ? 8 : 32;
-    auto ctas = [&](const Source& x) { return (x.n * lanes + kRowThreads - 1) / kRowThreads; };
-    auto* fn = lanes == 8 ? (aligned ? narrow_kernel<true, 8> : narrow_kernel<false, 8>)
-                          : (aligned ? narrow_kernel<true, 32> : narrow_kernel<false, 32>);
-    if (int rc = launch_after(fn, dim3((unsigned)(ctas(one) + ctas(two))), kRowThreads, 0, st, p, ctas(one))) return rc;
+template <typename F>
+int with_f32_or_bf16(int32_t dtype, F&& f) {
+  return dtype == CB_F32 ? f(float{}) : f(__nv_bfloat16{});
+}
+
+// Up to two matrices of a type, and whether their rows can be read 16 bytes at a time.
+struct Made {
+  Sources p;
+  int32_t dtype;
+  bool aligned;
+  Made(int32_t dtype_, const Shape& s, const Source& one, const Source& two, const float* top, uint32_t* wide)
+      : p{{one, two}, s.d, s.dp, top, wide}, dtype(dtype_) {
+    auto pieces = [&](const Source& x) { return !x.n || (aligned_to(x.x, 16) && x.ld * dtype_size(dtype) % 16 == 0); };
+    aligned = s.d % 8 == 0 && pieces(one) && pieces(two);
   }
-  auto ctas = [&](const Source& x) { return (x.n * (s.dp / 8) + kRowThreads - 1) / kRowThreads; };
-  return with_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    const int64_t blocks = ctas(one) + ctas(two);
-    // the float32 pairs' rarely has anything to do
-    const unsigned grid = (unsigned)(wide ? std::min<int64_t>(blocks, 8 * num_sms()) : blocks);
-    return launch_after(aligned ? operand_kernel<T, true> : operand_kernel<T, false>, dim3(grid), kRowThreads, 0, st, p,
-                        ctas(one), blocks);
-  });
+  // in f16 parts
+  int narrow(cudaStream_t st) const {
+    const int lanes = p.dp <= 64 ? 8 : 32;
+    auto ctas = [&](const Source& x) { return (x.n * lanes + kRowThreads - 1) / kRowThreads; };
+    return with_f32_or_bf16(dtype, [&](auto t) {
+      using T = decltype(t);
+      auto* fn = lanes == 8 ? (aligned ? narrow_kernel<T, true, 8> : narrow_kernel<T, false, 8>)
+                            : (aligned ? narrow_kernel<T, true, 32> : narrow_kernel<T, false, 32>);
+      return launch_after(fn, dim3((unsigned)(ctas(p.s[0]) + ctas(p.s[1]))), kRowThreads, 0, st, p, ctas(p.s[0]));
+    });
+  }
+  // as they are, or in bf16 parts; after a try in f16 parts there is rarely anything to do
+  int whole(cudaStream_t st) const {
+    auto ctas = [&](const Source& x) { return (x.n * (p.dp / 8) + kRowThreads - 1) / kRowThreads; };
+    const int64_t blocks = ctas(p.s[0]) + ctas(p.s[1]);
+    const unsigned grid = (unsigned)(p.wide ? std::min<int64_t>(blocks, 8 * num_sms()) : blocks);
+    return with_type(dtype, [&](auto t) {
+      using T = decltype(t);
+      return launch_after(aligned ? operand_kernel<T, true> : operand_kernel<T, false>, dim3(grid), kRowThreads, 0, st, p,
+                          ctas(p.s[0]), blocks);
+    });
+  }
+};
+
+// h's and W's operands, as far as they have to be made.  f16 parts are tried for both before
+// either is made in another form: one matrix that does not fit decides for both.
+int make_operands(int32_t h_dtype, int32_t w_dtype, const Shape& s, const Source& h, const Source& w, const float* top,
+                  uint32_t* wide, cudaStream_t st) {
+  const bool together = h_dtype == w_dtype && h.out && w.out;
+  const Made first(w_dtype, s, w, together ? h : Source{}, top, wide), second(h_dtype, s, h, Source{}, top, wide);
+  const bool has_first = w.out, has_second = h.out && !together;
+  if (wide) {
+    if (has_first)
+      if (int rc = first.narrow(st)) return rc;
+    if (has_second)
+      if (int rc = second.narrow(st)) return rc;
+  }
+  if (has_first)
+    if (int rc = first.whole(st)) return rc;
+  return has_second ? second.whole(st) : (int)CB_OK;
 }
 
 int finish(int32_t dtype, const float* acc, int splits, int64_t split_rows, const Shape& s, int64_t n_rows, const float4* rows,
@@ -1391,7 +1435,7 @@ extern "C" size_t cb_linear_ce_scratch_bytes(const void* h, int32_t h_dtype, int
     return 0;
   const Shape s(h_dtype, w_dtype, N, V, d);
   Layout a{nullptr};
-  const bool w_direct = direct(w, w_dtype, ldw, V);
+  const bool w_direct = s.reads_w(w, w_dtype, ldw);
   if (!gradients) {
     Forward f(a, s, direct(h, h_dtype, ldh, N), w_direct);
   } else {
@@ -1411,18 +1455,11 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   cudaStream_t st = (cudaStream_t)stream;
   const Shape s(h_dtype, w_dtype, N, V, d);
   Layout a{static_cast<char*>(scratch)};
-  const Forward f(a, s, direct(h, h_dtype, ldh, N), direct(w, w_dtype, ldw, V));
+  const Forward f(a, s, direct(h, h_dtype, ldh, N), s.reads_w(w, w_dtype, ldw));
   if (scratch_bytes < a.used) return CB_ERR_WORKSPACE;
-  const Source none{}, hs{h, ldh, N, nullptr, f.h, nullptr, f.unit, 1}, ws{w, ldw, V, nullptr, f.w, nullptr, nullptr, 0};
-  if (s.pair) {
-    if (cudaMemsetAsync(f.wide, 0, sizeof(uint32_t), st) != cudaSuccess) return CB_ERR_CUDA;
-    if (int rc = make_operands(CB_F32, s, ws, hs, nullptr, f.wide, st)) return rc;
-  } else {
-    if (f.h)
-      if (int rc = make_operands(h_dtype, s, hs, none, nullptr, nullptr, st)) return rc;
-    if (f.w)
-      if (int rc = make_operands(w_dtype, s, ws, none, nullptr, nullptr, st)) return rc;
-  }
+  const Source hs{h, ldh, N, nullptr, f.h, nullptr, f.unit, 1}, ws{w, ldw, V, nullptr, f.w, nullptr, nullptr, 0};
+  if (s.tried && cudaMemsetAsync(f.wide, 0, sizeof(uint32_t), st) != cudaSuccess) return CB_ERR_CUDA;
+  if (int rc = make_operands(h_dtype, w_dtype, s, hs, ws, nullptr, f.wide, st)) return rc;
   const Operand ho(h, ldh, N, f.h, s.h_parts, s), wo(w, ldw, V, f.w, s.w_parts, s);
   Args p{};
   Gemm& g = p.g[0];
@@ -1440,7 +1477,7 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
     p.share = s.h_parts;
   } else {
     s.passes(g, s.w_parts, s.h_parts, s.dp, s.dp);
-    if (s.pair) g.span[0] = g.span[1] = kSpan32 / 2;  // (the tiles are small)
+    if (s.tried) g.span[0] = g.span[1] = kSpan32 / 2;  // (the tiles are small)
   }
   p.part_cols = s.dp;
   p.stage_bytes = f.tile_m * 64 + p.share * f.tile_n * 64;
@@ -1481,7 +1518,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   cudaStream_t st = (cudaStream_t)stream;
   const Shape s(h_dtype, w_dtype, N, V, d);
   Layout a{static_cast<char*>(scratch)};
-  const Backward f(a, s, direct(w, w_dtype, ldw, V), dh != nullptr, dw != nullptr, tma_rows(dw, w_dtype, d));
+  const Backward f(a, s, s.reads_w(w, w_dtype, ldw), dh != nullptr, dw != nullptr, tma_rows(dw, w_dtype, d));
   if (scratch_bytes < a.used) return CB_ERR_WORKSPACE;
   const Problem pb{N, V, d, Ids{targets, targets_64}};
   const Upstream u{g_loss, g_lse, g_loss_step, g_lse_step, count, reduction};
@@ -1489,13 +1526,9 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   if (int rc = launch_after(factors_kernel, dim3(ceil_div(N, kRowThreads)), kRowThreads, 0, st, pb, u, lse, f.rows, f.top,
                             f.wide))
     return rc;
-  const Source none{}, ws{w, ldw, V, nullptr, f.w, nullptr, nullptr, 0};
-  const Source hs{h, ldh, N, f.rows, f.h, f.hs != f.h ? f.hs : nullptr, s.pair ? &f.rows->w : nullptr, 4};
-  if (int rc = s.pair ? make_operands(CB_F32, s, ws, hs, f.top, f.wide, st)
-                      : make_operands(h_dtype, s, hs, none, f.top, nullptr, st))
-    return rc;
-  if (f.w && !s.pair)
-    if (int rc = make_operands(w_dtype, s, ws, none, nullptr, nullptr, st)) return rc;
+  const Source ws{w, ldw, V, nullptr, f.w, nullptr, nullptr, 0};
+  const Source hs{h, ldh, N, f.rows, f.h, f.hs != f.h ? f.hs : nullptr, s.tried ? &f.rows->w : nullptr, 4};
+  if (int rc = make_operands(h_dtype, w_dtype, s, hs, ws, f.top, f.wide, st)) return rc;
   const Operand wo(w, ldw, V, f.w, s.w_parts, s);
   const int64_t h_cols = (int64_t)s.h_parts * s.dp;
   const int nt = ceil_div(d, kTileN), m_tiles = ceil_div(N, kTileM);

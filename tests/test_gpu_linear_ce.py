@@ -212,6 +212,26 @@ def test_float32_of_any_size():
     check(h, w, t, "none", torch.ones(32))
 
 
+@pytest.mark.parametrize("weight", ["f32", "bf16"])
+@pytest.mark.parametrize("what", ["fits", "large row", "small row", "large vocabulary row", "small vocabulary row"])
+def test_float32_in_two_parts_or_three(weight, what):
+    """Rows enough for the two-part form against either weight; values just in its range, and
+    one row or vocabulary row out of it."""
+    h, w, t = inputs(1100, 200, 72, ("f32", weight), seed=21)
+    h[7] *= 250 / h[7].abs().max()
+    w[9] *= 2.0 ** -9 / w[9].abs().max()
+    if what == "large row":
+        h[50] *= 3e4
+    elif what == "small row":
+        h[50] *= 1e-9
+    elif what == "large vocabulary row":
+        w[60] *= 1e4
+    elif what == "small vocabulary row":
+        w[60] *= 1e-9
+    check(h, w, t, "none", torch.linspace(0.2, 1, 1100))
+    check(h, w, t, "mean")
+
+
 @pytest.mark.parametrize("pair", PAIRS)
 def test_strides_and_alignment(pair):
     g = torch.Generator().manual_seed(11)
