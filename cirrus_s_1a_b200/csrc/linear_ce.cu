@@ -10,24 +10,27 @@
 //   * a pair of CTAs (cta_group::2) owns a 256 x 256 tile: each holds 128 of its rows, the
 //     accumulator in tensor memory (two of them, so that a tile's products run under the
 //     last tile's epilogue), and brings half of the columns' operand;
-//   * a thread of each CTA copies 64-wide steps of K by TMA into five stages or more, one of the pair
-//     issues tcgen05.mma, eight warps a CTA take the accumulators out of tensor memory;
+//   * a thread of each CTA copies 64-wide steps of K by TMA into six or seven stages, one of
+//     the pair issues tcgen05.mma, eight warps a CTA take the accumulators out of tensor
+//     memory;
 //   * operands lie as the caller has them: logits read h and W along K; dh reads W, and dW
 //     reads G and h, across it (MN-major operands), so that nothing is transposed.
 // Forward: a pair takes a run of tiles along the vocabulary and keeps its rows' maximum and
 // sum over them; a second kernel joins the runs in order.  Backward: G of a piece of the
 // vocabulary goes to memory in the operands' type, both products of the piece follow in one
 // launch; dh adds the pieces up in float32.
-// float32 operands are two f16 parts each (11 + 11 bits, of the value times 2^8), three
-// products of parts (what is left out is below 2^-24 of a product), where the values lie in
-// the range that this is right for, which the kernel that makes the parts finds out; else
-// three bf16 parts (8 + 8 + 8 bits, and float32's range), six products.  Against bf16: three
-// bf16 parts, three products.
+// float32 operands are two f16 parts each (11 + 11 bits, of the value times a power of two),
+// three products of parts (what is left out is below 2^-24 of a product), where the values
+// lie in the range that this is right for, which the kernel that makes the parts finds out;
+// else three bf16 parts (8 + 8 + 8 bits, and float32's range), six products.  Against bf16,
+// which is one part: two products and three.
+// Measured, 16384 x 32000 x 768 in bf16: loss 545 us = 1.48 PFLOP/s (tensor pipe 88 %),
+// with the gradient 2665 us = 1.21 PFLOP/s, at the power limit (G of a quarter of the
+// vocabulary 140 us, both its products 250 us, tensor pipe 77 and 90 %).
 // Every wait is bounded (%globaltimer); one that gives up sets CB_ERR_TIMEOUT.
 #include <cuda.h>
 
 #include <algorithm>
-#include <climits>
 
 #include "ends.cuh"
 
@@ -66,11 +69,12 @@ static_assert(kEpiWarps * kBoxBytes == kStageBytes, "a box for each warp takes a
 // adds a_part[i] / b_part[i] to the column it is read at, the place of a part of its values.
 struct alignas(64) Gemm {
   CUtensorMap a, b, out;
-  int a_mn, b_mn;                  // read across K
+  int a_mn;                        // PRODUCTS: A is read across K, as B always is there
   int a_base, b_base;              // added to the row it is read at
   // for operands in bf16 (or 16 bits as they came), and for float32 ones in f16
   int passes[2], a_part[2][kMaxPasses], b_part[2][kMaxPasses];
   int span[2];                     // steps of K that are added up in tensor memory
+  int by_step;                     // bf16 parts: all passes over a step of K before the next step, not over a span
   int m_tiles, n_tiles, k_steps;   // k_steps of a pass
   int splits;                      // of K, each with an output of its own
   int out_f32, out_mode, split_mode;  // of the first split and of the others
@@ -88,20 +92,19 @@ struct alignas(64) Args {
   const uint32_t* wide;            // 0 where the parts are f16 (null: not tried)
   uint32_t kind;                   // instruction descriptor without sizes and directions
   int tile_m, tile_n;              // rows and columns of a tile (PRODUCTS: kTileM, kTileN)
-  int share;                       // FEW: parts of the rows' operand that a step of the vocabulary's meets, the
-                                   // smaller ones in an accumulator kFew columns further
+  int share;                       // FEW: parts of the rows' operand that a step of the vocabulary's meets
   int part_cols;                   // and the columns between them
   int stages, stage_bytes;         // FEW
   // STATS, FEW and GRAD: rows, vocabulary rows, the vocabulary row that the tiles start at, and how many
   int N, V, v0, vp;
   Ids targets;
-  int slots;                       // STATS: parts of a row's sum
-  float2* part;                    // STATS: [slots][2][N]; FEW: [tiles][2][N]
+  float2* part;                    // of a row's sum.  STATS: [run][2][N]; FEW: [tile][2][N]
   float* xt;                       // [N]
   uint32_t* counter;               // set to 0
   const float* row_scale;          // STATS, FEW, f16 parts: what a row's logits are multiplied by
   const float4* rows;              // GRAD: (a, b, lse, that) of each row
   const float* top;                // and their largest factor
+  const float* common;             // PRODUCTS, f16 parts: the largest value of h as dW's operand
   int g_parts, g_cols;             // of G: columns of one part
   int is_f16;                      // 16-bit operands are f16
   int32_t* status;
@@ -262,12 +265,21 @@ __device__ __forceinline__ float2 unpack_bf16(uint32_t u) {
 }
 __device__ __forceinline__ float2 unpack_f16(uint32_t u) { return __half22float2(reinterpret_cast<const __half2&>(u)); }
 
-// float32 as two f16 parts.  W, and h as dW's operand: of the value times 2^8, right for
-// values below 255 in rows whose largest is 2^-10 or more, against which what lies below
-// f16's range, 2^-33, is 2^-23.  h in front of the logits: of the row times the power of two
-// that brings its largest value to [2^14, 2^15), so that no row depends on another.
+// float32 as two f16 parts.  W: of the value times 2^8, right for values below 255 in rows
+// whose largest is 2^-10 or more, against which what lies below f16's range, 2^-33, is 2^-23;
+// W alone decides, so that both directions take the logits alike (a logit of thousands that
+// came out another way would not be the one its lse is of).  h in front of the logits: of the
+// row times the power of two that brings its largest value to [2^14, 2^15), so that no row
+// depends on another.  h as dW's operand: of the rows times one power of two, that of their
+// largest value (rows more than 2^17 below it lose bits of their part of dW).
 constexpr int kNarrowShift = 8;
 constexpr float kNarrowMost = 255.0f, kNarrowLeast = 1.0f / 1024;
+// The exponent that brings `top` to [2^14, 2^15).
+__device__ __forceinline__ int exponent_to_15(float top) {
+  int e = 0;
+  if (top > 0.0f && top < INFINITY) frexpf(top, &e);
+  return 15 - min(max(e, -100), 128);
+}
 
 // G is held in units of the largest |a| or |b| of the call, `top`: a mean's G is p - [v = t]
 // itself, whose largest entries lie below 1, where their rounding is smallest against them.
@@ -285,9 +297,11 @@ __device__ __forceinline__ int row_exponent(float4 row, float top) {
   if (size > 0.0f && size < INFINITY) frexpf(size, &e);
   return min(max(e - 2, -100), 0);
 }
-// What a product of G (16 bits or parts of float32) is multiplied by, beside top and rows' exponents.
-__device__ __forceinline__ float product_scale(bool f16, bool narrow) {
-  return f16 ? 1.0f / (1 << (kF16Shift + (narrow ? kNarrowShift : 0))) : 1.0f;
+// What a product of G (16 bits or parts of float32) is multiplied by, beside top and rows'
+// exponents; common: of h as dW's operand (null: of W).
+__device__ __forceinline__ float product_scale(bool f16, bool narrow, const float* common) {
+  if (!f16) return 1.0f;
+  return ldexpf(1.0f, -kF16Shift - (!narrow ? 0 : common ? exponent_to_15(*common) : kNarrowShift));
 }
 
 // ------------------------------------------------------------------- work
@@ -359,7 +373,9 @@ __device__ __forceinline__ void put_row(uint32_t box, int row, F&& f) {
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ Args p) {
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t bars[2 * kMaxStages + 4];
+  // of 128 or 256 columns (128 float32 rows: 31.0 us, with two 31.9)
+  constexpr int kAccs = MODE == FEW ? 4 : 2;
+  __shared__ uint64_t bars[2 * kMaxStages + 2 * kAccs];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -368,14 +384,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   const uint32_t out_at = base + stages_of(MODE) * kStageBytes;
   const int stages = MODE == FEW ? p.stages : stages_of(MODE), stage_bytes = MODE == FEW ? p.stage_bytes : kStageBytes;
   const int a_bytes = MODE == FEW ? p.tile_m * 64 : kHalfBytes;  // of a stage
-  const uint32_t full = smem_u32(bars), empty = full + 8 * kMaxStages, done = empty + 8 * kMaxStages, freed = done + 16;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kMaxStages, done = empty + 8 * kMaxStages, freed = done + 8 * kAccs;
 
   if (tid == 0) {
     for (int i = 0; i < kMaxStages; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full + 8 * i));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(empty + 8 * i));
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kAccs; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(done + 8 * i));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(freed + 8 * i), "n"(2 * kEpiWarps));
     }
@@ -415,32 +431,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         const uint32_t bytes = 2 * (m_rows + (MODE == FEW ? p.share : 1) * n_rows) * 128;
         // a span of K at a time, all passes over it
         const int span = g.span[narrow], passes = g.passes[narrow];
+        const bool by_step = g.by_step && !narrow;
         for (int from = 0; go && from < it.steps; from += span)
-          for (int pass = 0; go && pass < passes; ++pass) {
-            const int ap = g.a_part[narrow][pass], bp = g.b_part[narrow][pass], end = min(from + span, it.steps);
-            for (int k = from; k < end; ++k, ++n) {
-              const int st = n % stages, k0 = (it.first + k) * kStep;
-              if (n >= stages && !wait(empty + 8 * st, (n / stages - 1) & 1)) {
-                go = false;
-                break;
-              }
-              const uint32_t bar = in_leader(full + 8 * st), at = base + st * stage_bytes, bt = at + a_bytes;
-              if (rank == 0)
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full + 8 * st), "r"(bytes)
-                             : "memory");
-              if (MODE == PRODUCTS && g.a_mn) {
-                copy_in(at, &g.a, m + ap, g.a_base + k0, bar);
-                copy_in(at + kHalfBytes / 2, &g.a, m + 64 + ap, g.a_base + k0, bar);
+          for (int k = 0, pass = 0, end = min(span, it.steps - from); k < end && pass < passes; ++n) {
+            const int ap = g.a_part[narrow][pass], bp = g.b_part[narrow][pass];
+            const int st = n % stages, k0 = (it.first + from + k) * kStep;
+            if (n >= stages && !wait(empty + 8 * st, (n / stages - 1) & 1)) {
+              go = false;
+              break;
+            }
+            const uint32_t bar = in_leader(full + 8 * st), at = base + st * stage_bytes, bt = at + a_bytes;
+            if (rank == 0)
+              asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full + 8 * st), "r"(bytes)
+                           : "memory");
+            if (MODE == PRODUCTS && g.a_mn) {
+              copy_in(at, &g.a, m + ap, g.a_base + k0, bar);
+              copy_in(at + kHalfBytes / 2, &g.a, m + 64 + ap, g.a_base + k0, bar);
+            } else {
+              copy_in(at, &g.a, k0 + ap, g.a_base + m, bar);
+            }
+            if (MODE == PRODUCTS) {  // both products read their second operand across K
+              copy_in(bt, &g.b, c + bp, g.b_base + k0, bar);
+              copy_in(bt + kHalfBytes / 2, &g.b, c + 64 + bp, g.b_base + k0, bar);
+            } else {
+              copy_in(bt, &g.b, k0 + bp, g.b_base + c, bar);
+              for (int q = 1; q < (MODE == FEW ? p.share : 1); ++q)
+                copy_in(bt + q * n_rows * 128, &g.b, k0 + q * p.part_cols, c, bar);
+            }
+            if (by_step ? ++pass == passes : ++k == end) {
+              if (by_step) {
+                pass = 0;
+                ++k;
               } else {
-                copy_in(at, &g.a, k0 + ap, g.a_base + m, bar);
-              }
-              if (MODE == PRODUCTS) {  // both products read their second operand across K
-                copy_in(bt, &g.b, c + bp, g.b_base + k0, bar);
-                copy_in(bt + kHalfBytes / 2, &g.b, c + 64 + bp, g.b_base + k0, bar);
-              } else {
-                copy_in(bt, &g.b, k0 + bp, g.b_base + c, bar);
-                for (int j = 1; j < (MODE == FEW ? p.share : 1); ++j)
-                  copy_in(bt + j * n_rows * 128, &g.b, k0 + j * p.part_cols, c, bar);
+                k = 0;
+                ++pass;
               }
             }
           }
@@ -463,10 +487,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         const uint32_t a_step = a_mn ? 2048 / 16 : 2, b_step = MODE == PRODUCTS ? 2048 / 16 : 2;
         const int span = g.span[narrow];
         for (int from = 0; go && from < it.steps; from += span, ++sums) {
-          const int acc = sums & 1, steps = min(span, it.steps - from) * g.passes[narrow];
-          if (sums >= 2) go = __all_sync(0xffffffffu, wait(freed + 8 * acc, (sums / 2 - 1) & 1));
+          const int acc = sums % kAccs, steps = min(span, it.steps - from) * g.passes[narrow];
+          if (sums >= kAccs) go = __all_sync(0xffffffffu, wait(freed + 8 * acc, (sums / kAccs - 1) & 1));
           fence_after();
-          const uint32_t d = tmem + acc * kTileN;
+          const uint32_t d = tmem + acc * (512 / kAccs);
           for (int k = 0; k < steps && go; ++k, ++n) {
             const int st = n % stages;
             go = __all_sync(0xffffffffu, wait(full + 8 * st, (n / stages) & 1));
@@ -474,12 +498,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
             fence_after();
             if (lead) {
               const uint64_t a = operand(base + st * stage_bytes), b = operand(base + st * stage_bytes + a_bytes);
-#pragma unroll
-              for (int s = 0; s < kStep / 16; ++s) mma(d, a + s * a_step, b + s * b_step, id, k > 0 || s > 0);
-              for (int j = 1; j < (MODE == FEW ? p.share : 1); ++j)
+              // (parts that share a step: the smaller ones first, as one after the other)
+              const int last = MODE == FEW ? p.share - 1 : 0;
+              for (int j = last; j > 0; --j)
 #pragma unroll
                 for (int s = 0; s < kStep / 16; ++s)
-                  mma(d + kFew, a + s * a_step, b + j * p.tile_n * 4 + s * b_step, id, k > 0 || j > 1 || s > 0);
+                  mma(d, a + s * a_step, b + j * p.tile_n * 4 + s * b_step, id, k > 0 || j < last || s > 0);
+#pragma unroll
+              for (int s = 0; s < kStep / 16; ++s) mma(d, a + s * a_step, b + s * b_step, id, k > 0 || last > 0 || s > 0);
               commit(empty + 8 * st);
             }
             __syncwarp();
@@ -553,24 +579,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       const int span = p.g[MODE == PRODUCTS ? it.gemm : 0].span[narrow];
       bool go = true;
       for (int from = 0; from < it.steps; from += span, ++sums) {
-        const int acc = sums & 1;
-        // the half's four waits agree, or its barriers would not
-        go = !any_of_half(half, !wait(done + 8 * acc, (sums / 2) & 1));
+        const int acc = sums % kAccs;
+        go = __all_sync(0xffffffffu, wait(done + 8 * acc, (sums / kAccs) & 1));
         if (!go) break;
         fence_after();
-        const uint32_t at = tmem + lane_at + acc * kTileN + half * (MODE == FEW ? cols : 128);
+        const uint32_t at = tmem + lane_at + acc * (512 / kAccs) + half * (MODE == FEW ? cols : 128);
         if (from == 0) {
 #pragma unroll
           for (int c = 0; c < kCols / 32; ++c)
             if (c * 32 < cols) load32(at + c * 32, x + c * 32);
           loads_done();
-        }
-        for (int more = from == 0; more < (MODE == FEW && p.share > 1 ? 2 : 1); ++more) {
+        } else {
 #pragma unroll
           for (int c = 0; c < kCols / 16; ++c)
             if (c * 16 < cols) {
               float y[16];
-              load16(at + more * kFew + c * 16, y);
+              load16(at + c * 16, y);
               loads_done();
 #pragma unroll
               for (int j = 0; j < 16; ++j) x[c * 16 + j] += y[j];
@@ -582,7 +606,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_leader(freed + 8 * acc))
                        : "memory");
       }
-      if (!go) break;
+      // the half's four warps agree, or its barriers would not
+      if (any_of_half(half, !go)) break;
       if ((MODE == STATS || MODE == GRAD) && narrow)
 #pragma unroll
         for (int c = 0; c < kCols; ++c) x[c] *= f.w;
@@ -593,7 +618,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         const Gemm& g = p.g[it.gemm];
         const int y = it.m0 + rank * 128 + it.split * g.out_rows;
         if (g.top) {
-          const float s = scale_of(*g.top) * product_scale(f16, narrow);
+          const float s = scale_of(*g.top) * product_scale(f16, narrow, p.common);
 #pragma unroll
           for (int c = 0; c < 128; ++c) x[c] *= s;
         }
@@ -872,15 +897,16 @@ struct Upstream {
 // for all rows of a reduced loss; else a maximum (which does not depend on the order it is
 // taken in), *top starting at 0.
 __global__ void __launch_bounds__(kRowThreads) factors_kernel(Problem p, Upstream u, const float* lse, float4* rows, float* top,
-                                                              uint32_t* wide) {
+                                                              float* common, uint32_t* wide) {
   const int n = blockIdx.x * kRowThreads + threadIdx.x;
-  const bool common = u.reduction != CB_REDUCE_NONE && !u.lse;
+  const bool one_top = u.reduction != CB_REDUCE_NONE && !u.lse;
   await_before();
   start_next();
   if (wide && n == 0) *wide = 0;
+  if (common && n == 0) *common = 0.0f;
   float one = u.loss && u.reduction != CB_REDUCE_NONE ? *u.loss : 0.0f;
   if (u.reduction == CB_REDUCE_MEAN) one /= (float)max(*u.count, 1);
-  if (common && n == 0) *top = fabsf(one) < INFINITY ? fabsf(one) : 0.0f;
+  if (one_top && n == 0) *top = fabsf(one) < INFINITY ? fabsf(one) : 0.0f;
   float size = 0.0f;
   if (n < p.N) {
     float b = 0.0f;
@@ -891,27 +917,29 @@ __global__ void __launch_bounds__(kRowThreads) factors_kernel(Problem p, Upstrea
     size = fmaxf(fabsf(a), fabsf(b));
     if (!(size < INFINITY)) size = 0.0f;
   }
-  if (common) return;
+  if (one_top) return;
   size = warp_max(size);
   if ((threadIdx.x & 31) == 0 && size > 0.0f) atomicMax(reinterpret_cast<int*>(top), __float_as_int(size));
 }
 
 // A matrix to be made an operand: rows of dp columns a part.  rows given: rows without a
-// gradient become zeros.  scaled given: a second copy for dW, in f16 with row n multiplied by
-// 2^row_exponent.  unit given: h in f16 parts, scaled by rows; what its logits are to be
-// multiplied by.
+// gradient become zeros.  scaled given: a second copy for dW, f16 rows multiplied by
+// 2^row_exponent.
+enum { SCALE_FIXED = 0, SCALE_ROW = 1, SCALE_COMMON = 2 };  // of f16 parts of float32, see kNarrowShift
 struct Source {
   const void* x;
   int64_t ld, n;
   float4* rows;
   uint16_t *out, *scaled;
-  float* unit;
+  int scale;
+  float* unit;  // SCALE_ROW: what the row's logits are to be multiplied by
   int64_t unit_step;
 };
 struct Sources {
   Source s[2];
   int d, dp;
   const float* top;
+  float* common;   // SCALE_ROW: raised to the rows' largest value; SCALE_COMMON: that (null: not wanted)
   uint32_t* wide;  // set where f16 parts do not fit (null: not tried)
 };
 
@@ -999,10 +1027,11 @@ __device__ __forceinline__ void put_parts(uint16_t* out, int dp, const Vec<T, 8>
 }
 
 // float32 rows as two f16 parts (in rows laid out for three), bf16 rows as one, LANES threads
-// to a row; sets *wide where values of W, or of a row of h that counts for dW, do not fit (one that is not
-// finite makes its sums NaN in any form, and is left to).
+// to a row; sets *wide where values of W do not fit.  (A value that is not finite makes its
+// sums NaN in any form, and is left to.)
 template <typename T, bool WIDE, int LANES>
 __global__ void __launch_bounds__(kRowThreads) narrow_kernel(Sources p, int64_t first) {
+  constexpr int kLaid = sizeof(T) == 4 ? 3 : 1;
   const bool second = blockIdx.x >= first;
   const Source& s = p.s[second];
   const int lane = threadIdx.x % LANES;
@@ -1010,9 +1039,9 @@ __global__ void __launch_bounds__(kRowThreads) narrow_kernel(Sources p, int64_t 
   await_before();
   start_next();
   const bool is = n < s.n;
+  if (s.scale == SCALE_COMMON && *p.wide) return;  // dW takes the bf16 parts
   const float4 row = is && s.rows ? s.rows[n] : make_float4(1.0f, 0.0f, 0.0f, 0.0f);
   const int d = is && has_gradient(row) ? p.d : 0, dp = is ? p.dp : 0;
-  constexpr int kLaid = sizeof(T) == 4 ? 3 : 1;
   const T* x = static_cast<const T*>(s.x) + n * s.ld;
   uint16_t* out = s.out + n * kLaid * p.dp;
   constexpr int kAhead = 3;  // pieces in flight: a row of 768
@@ -1021,21 +1050,23 @@ __global__ void __launch_bounds__(kRowThreads) narrow_kernel(Sources p, int64_t 
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   };
-  float by = 1 << kNarrowShift;
-  if (s.unit) {
+  int e = kNarrowShift;
+  if (s.scale == SCALE_ROW) {
     for (int j0 = lane * 8; j0 < dp; j0 += LANES * 8) {
       const Vec<T, 8> v = load8<T, WIDE>(x, j0, d);
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(Elem<T>::get(v.v[j])));
     }
     reduce_top();
-    int e = 0;
-    if (top > 0.0f && top < INFINITY) frexpf(top, &e);
-    e = min(max(e, -100), 128);
-    by = ldexpf(1.0f, 15 - e);
-    if (is && lane == 0) s.unit[n * s.unit_step] = ldexpf(1.0f, e - 15 - kNarrowShift);
+    e = exponent_to_15(top);
+    if (is && lane == 0) {
+      s.unit[n * s.unit_step] = ldexpf(1.0f, -e - kNarrowShift);
+      const float mine = p.common && top < INFINITY ? ldexpf(top, row_exponent(row, *p.top)) : 0.0f;
+      if (mine > 0.0f) atomicMax(reinterpret_cast<int*>(p.common), __float_as_int(mine));
+    }
   }
-  const float dw_by = is && s.scaled ? ldexpf(1.0f, kNarrowShift + row_exponent(row, *p.top)) : 1.0f;
+  if (s.scale == SCALE_COMMON) e = exponent_to_15(*p.common) + row_exponent(row, *p.top);
+  const float by = ldexpf(1.0f, e);
   for (int j0 = lane * 8; j0 < dp; j0 += kAhead * LANES * 8) {
     Vec<T, 8> v[kAhead];
 #pragma unroll
@@ -1044,16 +1075,15 @@ __global__ void __launch_bounds__(kRowThreads) narrow_kernel(Sources p, int64_t 
     for (int i = 0; i < kAhead; ++i) {
       const int j = j0 + i * LANES * 8;
       if (j >= dp) break;
-      if (!s.unit)
+      if (s.scale == SCALE_FIXED)
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(Elem<T>::get(v[i].v[k])));
       put_parts(out + j, p.dp, v[i], by);
-      if (s.scaled) put_parts(s.scaled + n * kLaid * p.dp + j, p.dp, v[i], dw_by);
     }
   }
-  if (!s.unit) reduce_top();
-  if (lane == 0 && (!s.unit || s.scaled) && top < INFINITY && (top >= kNarrowMost || (top > 0.0f && top < kNarrowLeast)))
-    *p.wide = 1;
+  if (s.scale != SCALE_FIXED) return;
+  reduce_top();
+  if (lane == 0 && top < INFINITY && (top >= kNarrowMost || (top > 0.0f && top < kNarrowLeast))) *p.wide = 1;
 }
 
 // out[r][j] = the sum of the splits' results, scaled back; 0 in a row without a gradient.
@@ -1061,7 +1091,7 @@ __global__ void __launch_bounds__(kRowThreads) narrow_kernel(Sources p, int64_t 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kRowThreads) finish_kernel(const float* acc, int splits, int64_t split_rows, int da,
                                                              int64_t n_rows, int d, const float4* rows, const float* top,
-                                                             int f16, const uint32_t* wide, T* out) {
+                                                             const float* common, int f16, const uint32_t* wide, T* out) {
   const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
   const uint32_t pieces = d / VEC;
   const int64_t n = i < (1ll << 32) ? (int64_t)((uint32_t)i / pieces) : i / pieces;
@@ -1077,7 +1107,7 @@ __global__ void __launch_bounds__(kRowThreads) finish_kernel(const float* acc, i
   }
   const bool live = !rows || has_gradient(rows[n]);
   const bool narrow = wide && *wide == 0;
-  float by = scale_of(*top) * product_scale(f16 || narrow, narrow);
+  float by = scale_of(*top) * product_scale(f16 || narrow, narrow, common);
   if (rows && (f16 || narrow)) by = ldexpf(by, row_exponent(rows[n], *top));
   Vec<T, VEC> o;
 #pragma unroll
@@ -1231,6 +1261,18 @@ struct Shape {
     piece = piece_of(N, V, g_parts);
   }
   uint32_t kind() const { return f16 ? kKindF16 : kKindBf16; }
+  // The logits' passes.  Of float32 against bf16 all parts of a step follow each other, as they
+  // do where few rows share it: every form of the forward and the backward pass adds alike.
+  // (Sums that are large while the small parts come are cut off more: in spans of 256 of K by
+  // twice as much, 1.1e-7 of a sum of 768 magnitudes, at 29.4 us instead of 31.0 for 128 rows.)
+  void logit_passes(Gemm& g, bool swapped) const {
+    passes(g, h_parts, w_parts, dp, dp);
+    if (h_parts > w_parts) {
+      g.by_step = 1;
+      g.span[0] = kSpan32 / 2;
+    }
+    if (swapped) std::swap(g.a_part, g.b_part);
+  }
   // The passes of a product of these parts, and of the f16 parts that take their place (two of
   // float32, one of bf16).  Returns how many there will be, as a rule.
   int passes(Gemm& g, int a_parts, int b_parts, int a_cols, int b_cols) const {
@@ -1313,7 +1355,7 @@ struct Forward {
 
 struct Backward {
   float4* rows;
-  float* top;
+  float *top, *common;
   uint32_t* wide;
   uint16_t *h, *hs, *w, *G;
   float *acc, *dw;
@@ -1327,6 +1369,7 @@ struct Backward {
     if (s.V % s.piece) h_slots = std::max(h_slots, deal_of(s, want_h, want_w, s.V % s.piece, first.w).h_slots);
     rows = a.take<float4>(s.N);
     top = a.take<float>(1);
+    common = s.tried && want_w ? a.take<float>(1) : nullptr;
     h = a.take<uint16_t>((int64_t)s.N * s.h_parts * s.dp);
     wide = s.tried ? a.take<uint32_t>(1) : nullptr;
     hs = (s.f16 || s.tried) && want_w ? a.take<uint16_t>((int64_t)s.N * s.h_parts * s.dp) : h;
@@ -1353,8 +1396,8 @@ struct Made {
   Sources p;
   int32_t dtype;
   bool aligned;
-  Made(int32_t dtype_, const Shape& s, const Source& one, const Source& two, const float* top, uint32_t* wide)
-      : p{{one, two}, s.d, s.dp, top, wide}, dtype(dtype_) {
+  Made(int32_t dtype_, const Shape& s, const Source& one, const Source& two, const float* top, float* common, uint32_t* wide)
+      : p{{one, two}, s.d, s.dp, top, common, wide}, dtype(dtype_) {
     auto pieces = [&](const Source& x) { return !x.n || (aligned_to(x.x, 16) && x.ld * dtype_size(dtype) % 16 == 0); };
     aligned = s.d % 8 == 0 && pieces(one) && pieces(two);
   }
@@ -1385,15 +1428,22 @@ struct Made {
 // h's and W's operands, as far as they have to be made.  f16 parts are tried for both before
 // either is made in another form: one matrix that does not fit decides for both.
 int make_operands(int32_t h_dtype, int32_t w_dtype, const Shape& s, const Source& h, const Source& w, const float* top,
-                  uint32_t* wide, cudaStream_t st) {
+                  float* common, uint32_t* wide, cudaStream_t st) {
   const bool together = h_dtype == w_dtype && h.out && w.out;
-  const Made first(w_dtype, s, w, together ? h : Source{}, top, wide), second(h_dtype, s, h, Source{}, top, wide);
+  const Made first(w_dtype, s, w, together ? h : Source{}, top, common, wide);
+  const Made second(h_dtype, s, h, Source{}, top, common, wide);
   const bool has_first = w.out, has_second = h.out && !together;
   if (wide) {
     if (has_first)
       if (int rc = first.narrow(st)) return rc;
     if (has_second)
       if (int rc = second.narrow(st)) return rc;
+    if (h.scaled) {
+      Source dw = h;
+      dw.out = h.scaled;
+      dw.scale = SCALE_COMMON;
+      if (int rc = Made(h_dtype, s, dw, Source{}, top, common, wide).narrow(st)) return rc;
+    }
   }
   if (has_first)
     if (int rc = first.whole(st)) return rc;
@@ -1401,14 +1451,14 @@ int make_operands(int32_t h_dtype, int32_t w_dtype, const Shape& s, const Source
 }
 
 int finish(int32_t dtype, const float* acc, int splits, int64_t split_rows, const Shape& s, int64_t n_rows, const float4* rows,
-           const float* top, const uint32_t* wide, void* out, cudaStream_t st) {
+           const float* top, const float* common, const uint32_t* wide, void* out, cudaStream_t st) {
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     const bool vecs = s.d % 4 == 0 && aligned_to(out, 4 * sizeof(T));
     const int64_t n = n_rows * (vecs ? s.d / 4 : s.d);
     return launch_after(vecs ? finish_kernel<T, 4> : finish_kernel<T, 1>,
                         dim3((unsigned)((n + kRowThreads - 1) / kRowThreads)), kRowThreads, 0, st, acc, splits, split_rows,
-                        s.da(), n_rows, s.d, rows, top, s.f16, wide, static_cast<T*>(out));
+                        s.da(), n_rows, s.d, rows, top, common, s.f16, wide, static_cast<T*>(out));
   });
 }
 
@@ -1457,9 +1507,9 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   Layout a{static_cast<char*>(scratch)};
   const Forward f(a, s, direct(h, h_dtype, ldh, N), s.reads_w(w, w_dtype, ldw));
   if (scratch_bytes < a.used) return CB_ERR_WORKSPACE;
-  const Source hs{h, ldh, N, nullptr, f.h, nullptr, f.unit, 1}, ws{w, ldw, V, nullptr, f.w, nullptr, nullptr, 0};
+  const Source hs{h, ldh, N, nullptr, f.h, nullptr, SCALE_ROW, f.unit, 1}, ws{w, ldw, V, nullptr, f.w};
   if (s.tried && cudaMemsetAsync(f.wide, 0, sizeof(uint32_t), st) != cudaSuccess) return CB_ERR_CUDA;
-  if (int rc = make_operands(h_dtype, w_dtype, s, hs, ws, nullptr, f.wide, st)) return rc;
+  if (int rc = make_operands(h_dtype, w_dtype, s, hs, ws, nullptr, nullptr, f.wide, st)) return rc;
   const Operand ho(h, ldh, N, f.h, s.h_parts, s), wo(w, ldw, V, f.w, s.w_parts, s);
   Args p{};
   Gemm& g = p.g[0];
@@ -1468,16 +1518,12 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
       !map_of(&g.b, bo.at, s.type, f.few ? N : V, bo.cols, bo.ld, f.tile_n / 2))
     return CB_ERR_CUDA;
   p.share = 1;
-  if (!f.few) {
-    s.passes(g, s.h_parts, s.w_parts, s.dp, s.dp);
-  } else if (s.w_parts == 1 && s.h_parts > 1) {
+  s.logit_passes(g, f.few);
+  if (f.few && s.h_parts > s.w_parts) {
     // the rows' parts meet a step of the vocabulary together, which is then read once
-    s.passes(g, 1, 1, 0, 0);
-    g.span[0] = kSpan32;
+    g.passes[0] = 1;
+    g.b_part[0][0] = 0;
     p.share = s.h_parts;
-  } else {
-    s.passes(g, s.w_parts, s.h_parts, s.dp, s.dp);
-    if (s.tried) g.span[0] = g.span[1] = kSpan32 / 2;  // (the tiles are small)
   }
   p.part_cols = s.dp;
   p.stage_bytes = f.tile_m * 64 + p.share * f.tile_n * 64;
@@ -1524,11 +1570,11 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   const Upstream u{g_loss, g_lse, g_loss_step, g_lse_step, count, reduction};
   if ((reduction == CB_REDUCE_NONE || g_lse) && cudaMemsetAsync(f.top, 0, sizeof(float), st) != cudaSuccess) return CB_ERR_CUDA;
   if (int rc = launch_after(factors_kernel, dim3(ceil_div(N, kRowThreads)), kRowThreads, 0, st, pb, u, lse, f.rows, f.top,
-                            f.wide))
+                            f.common, f.wide))
     return rc;
-  const Source ws{w, ldw, V, nullptr, f.w, nullptr, nullptr, 0};
-  const Source hs{h, ldh, N, f.rows, f.h, f.hs != f.h ? f.hs : nullptr, s.tried ? &f.rows->w : nullptr, 4};
-  if (int rc = make_operands(h_dtype, w_dtype, s, hs, ws, f.top, f.wide, st)) return rc;
+  const Source ws{w, ldw, V, nullptr, f.w};
+  const Source hs{h, ldh, N, f.rows, f.h, f.hs != f.h ? f.hs : nullptr, SCALE_ROW, s.tried ? &f.rows->w : nullptr, 4};
+  if (int rc = make_operands(h_dtype, w_dtype, s, hs, ws, f.top, f.common, f.wide, st)) return rc;
   const Operand wo(w, ldw, V, f.w, s.w_parts, s);
   const int64_t h_cols = (int64_t)s.h_parts * s.dp;
   const int nt = ceil_div(d, kTileN), m_tiles = ceil_div(N, kTileM);
@@ -1537,7 +1583,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   Gemm& g = q.g[0];
   if (!map_of(&g.a, f.h, s.type, N, h_cols, h_cols, 128) || !map_of(&g.b, wo.at, s.type, V, wo.cols, wo.ld, kTileN / 2))
     return CB_ERR_CUDA;
-  s.passes(g, s.h_parts, s.w_parts, s.dp, s.dp);
+  s.logit_passes(g, false);
   g.m_tiles = m_tiles;
   g.k_steps = s.dp / kStep;
   q.kind = s.kind();
@@ -1556,6 +1602,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   r.kind = q.kind;
   r.is_f16 = s.f16;
   r.wide = f.wide;
+  r.common = f.common;
   r.status = status;
   const int64_t slot = up(N, kTileM) * s.da();  // floats of one of dh's
   if (dh && f.h_slots > 1 && cudaMemsetAsync(f.acc + slot, 0, (f.h_slots - 1) * slot * sizeof(float), st) != cudaSuccess)
@@ -1581,7 +1628,6 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
           !map_of(&gh.out, f.acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, f.h_slots * up(N, kTileM), s.da(), s.da(), 32))
         return CB_ERR_CUDA;
       s.passes(gh, s.g_parts, s.w_parts, cols, s.dp);
-      gh.b_mn = 1;
       gh.b_base = v0;
       gh.m_tiles = m_tiles;
       gh.n_tiles = nt;
@@ -1603,7 +1649,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
                        s.da(), 32);
       if (!ok) return CB_ERR_CUDA;
       s.dw_passes(gw, cols);
-      gw.a_mn = gw.b_mn = 1;
+      gw.a_mn = 1;
       gw.m_tiles = ceil_div(vp, kTileM);
       gw.n_tiles = nt;
       gw.k_steps = ceil_div(N, kStep);
@@ -1616,10 +1662,10 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
     r.pairs = s.pairs;
     if (int rc = launch<PRODUCTS>(r, st)) return rc;
     if (dw && !f.dw_direct)
-      if (int rc = finish(w_dtype, f.dw, sp.w, up(std::min(s.piece, V), kTileM), s, vp, nullptr, f.top, f.wide,
+      if (int rc = finish(w_dtype, f.dw, sp.w, up(std::min(s.piece, V), kTileM), s, vp, nullptr, f.top, f.common, f.wide,
                           static_cast<char*>(dw) + (int64_t)v0 * d * dtype_size(w_dtype), st))
         return rc;
   }
   if (!dh) return CB_OK;
-  return finish(h_dtype, f.acc, f.h_slots, up(N, kTileM), s, N, f.rows, f.top, f.wide, dh, st);
+  return finish(h_dtype, f.acc, f.h_slots, up(N, kTileM), s, N, f.rows, f.top, nullptr, f.wide, dh, st);
 }

@@ -529,7 +529,8 @@ size_t cb_embedding_grad_scratch_bytes(int64_t n, int32_t V, int32_t d);
 int cb_embedding_grad(const void* g, int32_t dtype, int64_t ldg, const void* ids, int32_t ids_64, int64_t n, int32_t V,
                       int32_t d, float scale, void* dtable, void* scratch, size_t scratch_bytes, void* stream);
 
-/* y [rows][d] = x * rsqrt(mean(x^2) + eps) * w; w [d] float32 or x's type.  Replaces RMSNorm
+/* y [rows][d] = x * rsqrt(mean(x^2) + eps) * w; w [d] float32 or x's type.  (Squares are
+ * float32: values past 2^63 give 0 or NaN.)  Replaces RMSNorm
  * (cirrus/model/layers.py:33-44). */
 int cb_rms_norm(const void* x, int32_t dtype, int64_t ld, const void* w, int32_t w_dtype, int32_t rows, int32_t d,
                 float eps, void* y, void* stream);
@@ -545,7 +546,7 @@ int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const void* g, in
  * 0 where there is no target.  loss: that for each row [N] (CB_REDUCE_NONE), or its mean
  * over the rows with a target (0 when none has one) or its sum, [1], with their number in
  * count [1].  h and w have one type, or h is CB_F32 and w CB_BF16.  16-bit products are
- * exact and float32 ones carried in about 24 bits, both summed in float32.
+ * exact and float32 ones carried in about 22 bits, both summed in float32.
  * Scratch, 256-byte aligned: cb_linear_ce_scratch_bytes of the same arguments, for the
  * gradient with 1 for dh + 2 for dw in `gradients`, and dw.  *status also receives CB_ERR_TIMEOUT when a bounded
  * wait in a kernel gave up.
@@ -561,7 +562,11 @@ int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int
  * g_lse (either null for zeros) are float32, of row n at n * step (step 0: one for all);
  * for a reduced loss g_loss is [1].  lse and count are the forward's.  A row without a
  * gradient (no target and g_lse 0) adds nothing, whatever it holds.  G is rounded to the
- * 16-bit type before the products; for float32 it is carried in about 24 bits. */
+ * 16-bit type before the products; for float32 it is carried in about 22 bits, and what lies
+ * below 2^-38 of the largest |g_loss + g_lse| or |g_loss| may be taken as 0 (in float16
+ * too, of the row's own); in dw also what lies below 2^-39 of the largest value of float32 h.
+ * x here has the bits that it had in the forward pass, so that G is 0 where the target has
+ * all the probability; lse is rounded to float32, G's relative error is not below that. */
 int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype, int64_t ldw,
                       int32_t N, int32_t V, int32_t d, const void* targets, int32_t targets_64, int32_t reduction,
                       const float* lse, const int32_t* count, const float* g_loss, int64_t g_loss_step,

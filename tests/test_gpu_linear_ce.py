@@ -203,6 +203,48 @@ def test_peaked_and_far_rows(pair, centre):
     check(h, w, t, "none", torch.linspace(0.1, 1, 36))
 
 
+@pytest.mark.parametrize("pair", PAIRS)
+@pytest.mark.parametrize("N", [1, 5, 16, 17, 45, 129, 300, 1100])
+@pytest.mark.parametrize("parts", ["two", "three"])
+def test_both_directions_take_a_logit_alike(pair, N, parts):
+    """A word that has all the probability, with a logit of 2000 and more: loss and gradients
+    are exactly 0, for every other exponential is, unless the backward pass's logit differs by
+    a bit from the one that lse is.  (Another word's logit is below 3 * 26 * 8 + 30 = 660 in
+    magnitude, with 8 deviations and all that the rows add.)"""
+    g = torch.Generator().manual_seed(N)
+    V, d = 270, 700
+    w = torch.randn(V, d, generator=g)
+    w[3, 5] = 1.0 if parts == "two" else 300.0
+    w = w.to(TYPES[pair[1]])
+    t = torch.randint(4, V, (N,), generator=g)
+    h = 3 * w[t].float() * (1 + torch.rand(N, 1, generator=g)) + 0.01 * torch.randn(N, d, generator=g)
+    h[:, 5] = 0.0
+    h = h.to(TYPES[pair[0]])
+    got = call(h.to(DEV), w.to(DEV), t.to(DEV), "none", torch.linspace(0.5, 2, N))
+    for n in ("loss", "dh", "dw"):
+        assert got[n].eq(0).all(), (n, float(got[n].abs().max()))
+    x = (h.double() * w.double()[t]).sum(1)
+    assert (got["lse"].cpu().double() - x).abs().le(x * ((d / 8 + 8) * 2.0 ** -23 + 2.0 ** -22)).all()
+
+
+@pytest.mark.parametrize("N", [1, 3, 40, 1030])
+@pytest.mark.parametrize("pair", PAIRS)
+def test_a_vocabulary_of_one(pair, N):
+    h, w, t = inputs(N, 1, 1500, pair, seed=N, masked=0.0, gain=30.0)
+    got = call(h.to(DEV), w.to(DEV), t.to(DEV), "sum", torch.ones(()))
+    assert all(got[n].eq(0).all() for n in ("loss", "dh", "dw"))
+
+
+@pytest.mark.parametrize("weight", ["f32", "bf16"])
+def test_rows_of_very_different_size(weight):
+    """Rows of 2^-8 to 2^9 with weights to match, whose logits are ordinary ones: every row has
+    its part in dw."""
+    h, w, t = inputs(1100, 200, 72, ("f32", weight), seed=23, gain=2.0 ** -6)
+    h *= torch.exp2(torch.arange(1100) % 18 - 8.0)[:, None]
+    check(h, w, t, "none", torch.linspace(0.2, 1, 1100))
+    check(h, w, t, "none", torch.linspace(0.2, 1, 1100) * torch.exp2(8 - torch.arange(1100) % 18))
+
+
 def test_float32_of_any_size():
     """No common scale: tiny rows keep their bits beside huge ones."""
     h, w, t = inputs(32, 200, 64, ("f32", "f32"), seed=10, masked=0.0)
