@@ -74,7 +74,7 @@ struct alignas(64) Gemm {
   // for operands in bf16 (or 16 bits as they came), and for float32 ones in f16
   int passes[2], a_part[2][kMaxPasses], b_part[2][kMaxPasses];
   int span[2];                     // steps of K that are added up in tensor memory
-  int by_step;                     // bf16 parts: all passes over a step of K before the next step, not over a span
+  int apart;                       // bf16 parts: the passes before the last, step by step, are a sum of their own
   int m_tiles, n_tiles, k_steps;   // k_steps of a pass
   int splits;                      // of K, each with an output of its own
   int out_f32, out_mode, split_mode;  // of the first split and of the others
@@ -92,7 +92,7 @@ struct alignas(64) Args {
   const uint32_t* wide;            // 0 where the parts are f16 (null: not tried)
   uint32_t kind;                   // instruction descriptor without sizes and directions
   int tile_m, tile_n;              // rows and columns of a tile (PRODUCTS: kTileM, kTileN)
-  int share;                       // FEW: parts of the rows' operand that a step of the vocabulary's meets
+  int share;                       // FEW: parts of the rows' operand that a step of the vocabulary's meets, 1 or 3
   int part_cols;                   // and the columns between them
   int stages, stage_bytes;         // FEW
   // STATS, FEW and GRAD: rows, vocabulary rows, the vocabulary row that the tiles start at, and how many
@@ -373,9 +373,7 @@ __device__ __forceinline__ void put_row(uint32_t box, int row, F&& f) {
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ Args p) {
   extern __shared__ uint8_t raw[];
-  // of 128 or 256 columns (128 float32 rows: 31.0 us, with two 31.9)
-  constexpr int kAccs = MODE == FEW ? 4 : 2;
-  __shared__ uint64_t bars[2 * kMaxStages + 2 * kAccs];
+  __shared__ uint64_t bars[2 * kMaxStages + 4];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -384,14 +382,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   const uint32_t out_at = base + stages_of(MODE) * kStageBytes;
   const int stages = MODE == FEW ? p.stages : stages_of(MODE), stage_bytes = MODE == FEW ? p.stage_bytes : kStageBytes;
   const int a_bytes = MODE == FEW ? p.tile_m * 64 : kHalfBytes;  // of a stage
-  const uint32_t full = smem_u32(bars), empty = full + 8 * kMaxStages, done = empty + 8 * kMaxStages, freed = done + 8 * kAccs;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kMaxStages, done = empty + 8 * kMaxStages, freed = done + 16;
 
   if (tid == 0) {
     for (int i = 0; i < kMaxStages; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full + 8 * i));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(empty + 8 * i));
     }
-    for (int i = 0; i < kAccs; ++i) {
+    for (int i = 0; i < 2; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(done + 8 * i));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(freed + 8 * i), "n"(2 * kEpiWarps));
     }
@@ -429,11 +427,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         const int n_rows = MODE == PRODUCTS ? kTileN / 2 : p.tile_n / 2, m_rows = MODE == FEW ? p.tile_m / 2 : 128;
         const int m = it.m0 + rank * m_rows, c = it.n0 + rank * n_rows;
         const uint32_t bytes = 2 * (m_rows + (MODE == FEW ? p.share : 1) * n_rows) * 128;
-        // a span of K at a time, all passes over it
+        // a span of K at a time, all passes over it, or those apart and then the last
         const int span = g.span[narrow], passes = g.passes[narrow];
-        const bool by_step = g.by_step && !narrow;
+        const bool apart = (MODE == STATS || MODE == GRAD) && g.apart && !narrow;
         for (int from = 0; go && from < it.steps; from += span)
-          for (int k = 0, pass = 0, end = min(span, it.steps - from); k < end && pass < passes; ++n) {
+          for (int k = 0, pass = 0, end = min(span, it.steps - from); pass < passes; ++n) {
             const int ap = g.a_part[narrow][pass], bp = g.b_part[narrow][pass];
             const int st = n % stages, k0 = (it.first + from + k) * kStep;
             if (n >= stages && !wait(empty + 8 * st, (n / stages - 1) & 1)) {
@@ -454,18 +452,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
               copy_in(bt, &g.b, c + bp, g.b_base + k0, bar);
               copy_in(bt + kHalfBytes / 2, &g.b, c + 64 + bp, g.b_base + k0, bar);
             } else {
-              copy_in(bt, &g.b, k0 + bp, g.b_base + c, bar);
-              for (int q = 1; q < (MODE == FEW ? p.share : 1); ++q)
-                copy_in(bt + q * n_rows * 128, &g.b, k0 + q * p.part_cols, c, bar);
-            }
-            if (by_step ? ++pass == passes : ++k == end) {
-              if (by_step) {
-                pass = 0;
-                ++k;
-              } else {
-                k = 0;
-                ++pass;
+              const bool shared = MODE == FEW && p.share > 1;
+              copy_in(shared ? bt + rank * n_rows * 128 : bt, &g.b, k0 + bp, g.b_base + c, bar);
+              if (shared) {
+                copy_in(bt + (rank ^ 1) * n_rows * 128, &g.b, k0 + p.part_cols, c, bar);
+                copy_in(bt + 2 * n_rows * 128, &g.b, k0 + 2 * p.part_cols, c, bar);
               }
+            }
+            if (apart && pass < passes - 1) {
+              if (++pass < passes - 1) continue;
+              pass = ++k < end ? 0 : passes - 1;
+              if (k == end) k = 0;
+            } else if (++k == end) {
+              k = 0;
+              ++pass;
             }
           }
       }
@@ -485,12 +485,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
                             (uint32_t)((MODE == PRODUCTS ? kTileN : p.tile_n) >> 3) << 17 | (uint32_t)(kTileM >> 4) << 24;
         // 16 of K: 32 bytes of a row, or 16 rows
         const uint32_t a_step = a_mn ? 2048 / 16 : 2, b_step = MODE == PRODUCTS ? 2048 / 16 : 2;
-        const int span = g.span[narrow];
-        for (int from = 0; go && from < it.steps; from += span, ++sums) {
-          const int acc = sums % kAccs, steps = min(span, it.steps - from) * g.passes[narrow];
-          if (sums >= kAccs) go = __all_sync(0xffffffffu, wait(freed + 8 * acc, (sums / kAccs - 1) & 1));
+        const int span = g.span[narrow], passes = g.passes[narrow];
+        const int apart = (MODE == STATS || MODE == GRAD) && g.apart && !narrow;
+        for (int from = 0, last = !apart; go && from < it.steps; from += last ? span : 0, last = !apart || !last, ++sums) {
+          const int acc = sums & 1, steps = min(span, it.steps - from) * (!apart ? passes : last ? 1 : passes - 1);
+          if (sums >= 2) go = __all_sync(0xffffffffu, wait(freed + 8 * acc, (sums / 2 - 1) & 1));
           fence_after();
-          const uint32_t d = tmem + acc * (512 / kAccs);
+          const uint32_t d = tmem + acc * kTileN;
           for (int k = 0; k < steps && go; ++k, ++n) {
             const int st = n % stages;
             go = __all_sync(0xffffffffu, wait(full + 8 * st, (n / stages) & 1));
@@ -498,14 +499,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
             fence_after();
             if (lead) {
               const uint64_t a = operand(base + st * stage_bytes), b = operand(base + st * stage_bytes + a_bytes);
-              // (parts that share a step: the smaller ones first, as one after the other)
-              const int last = MODE == FEW ? p.share - 1 : 0;
-              for (int j = last; j > 0; --j)
+              // Parts that share a step: the first two in one product of twice the columns, the
+              // third on to the second's, which lie side by side: half a product's columns come
+              // from either CTA, and the right one holds the two parts the other way round.
+              const bool shared = MODE == FEW && p.share > 1;
+              const uint32_t id0 = shared ? id + ((uint32_t)(p.tile_n >> 3) << 17) : id;
+#pragma unroll
+              for (int s = 0; s < kStep / 16; ++s) mma(d, a + s * a_step, b + s * b_step, id0, k > 0 || s > 0);
+              if (shared)
 #pragma unroll
                 for (int s = 0; s < kStep / 16; ++s)
-                  mma(d, a + s * a_step, b + j * p.tile_n * 4 + s * b_step, id, k > 0 || j < last || s > 0);
-#pragma unroll
-              for (int s = 0; s < kStep / 16; ++s) mma(d, a + s * a_step, b + s * b_step, id, k > 0 || last > 0 || s > 0);
+                  mma(d + p.tile_n / 2, a + s * a_step, b + 2 * p.tile_n * 4 + s * b_step, id, true);
               commit(empty + 8 * st);
             }
             __syncwarp();
@@ -547,6 +551,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       if (run >= 0 && run + rank * 128 + row < p.N)
         p.part[((int64_t)slot * 2 + half) * p.N + run + rank * 128 + row] = make_float2(m, l);
     };
+    // FEW: the thread's one or two rows, over a quarter of each tile
+    const int quarter = warp & 3;
+    const uint32_t few_box = out_at + half * 4 * kBoxBytes;  // [32][128] logits
+    int few_row[2], few_target[2];
+    float few_unit[2], few_m[2] = {-INFINITY, -INFINITY}, few_l[2] = {};
+    if constexpr (MODE == FEW)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int c = b * 32 + lane, r = half * (p.tile_n / 2) + c;
+        few_row[b] = c < p.tile_n / 2 && r < p.N ? r : -1;
+        const int64_t t = few_row[b] >= 0 ? p.targets[r] : -1;
+        few_target[b] = t < p.V ? (int)t : -1;
+        few_unit[b] = few_row[b] >= 0 && narrow ? p.row_scale[r] : 1.0f;
+      }
     Item it;
     int sums = 0;
     for (int i = 0; item_of<MODE>(p, pair, i, it); ++i) {
@@ -576,30 +594,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       float x[kCols];
       // this half's columns
       const int cols = MODE == PRODUCTS ? 128 : MODE == FEW ? p.tile_n / 2 : min(128, p.tile_n - half * 128);
-      const int span = p.g[MODE == PRODUCTS ? it.gemm : 0].span[narrow];
+      const Gemm& mine = p.g[MODE == PRODUCTS ? it.gemm : 0];
+      const int spans = (it.steps + mine.span[narrow] - 1) / mine.span[narrow];
       bool go = true;
-      for (int from = 0; from < it.steps; from += span, ++sums) {
-        const int acc = sums % kAccs;
-        go = __all_sync(0xffffffffu, wait(done + 8 * acc, (sums / kAccs) & 1));
+      for (int q = (MODE == STATS || MODE == GRAD) && mine.apart && !narrow ? 2 * spans : spans, first = 1; q > 0;
+           --q, first = 0, ++sums) {
+        const int acc = sums & 1;
+        go = __all_sync(0xffffffffu, wait(done + 8 * acc, (sums / 2) & 1));
         if (!go) break;
         fence_after();
-        const uint32_t at = tmem + lane_at + acc * (512 / kAccs) + half * (MODE == FEW ? cols : 128);
-        if (from == 0) {
+        // the half's columns; of parts that share a step the small ones' first, then the large one's
+        const bool shared = MODE == FEW && p.share > 1;
+        const uint32_t acc_at = tmem + lane_at + acc * kTileN;
+        const uint32_t at = acc_at + (shared ? (1 + half) * cols : half * (MODE == FEW ? cols : 128));
+        if (first) {
 #pragma unroll
           for (int c = 0; c < kCols / 32; ++c)
             if (c * 32 < cols) load32(at + c * 32, x + c * 32);
           loads_done();
-        } else {
+        }
+        constexpr int kAtOnce = MODE == FEW ? 32 : 16;
+        for (int more = first; more < (shared ? 2 : 1); ++more)
 #pragma unroll
-          for (int c = 0; c < kCols / 16; ++c)
-            if (c * 16 < cols) {
-              float y[16];
-              load16(at + c * 16, y);
+          for (int c = 0; c < kCols / kAtOnce; ++c)
+            if (c * kAtOnce < cols) {
+              float y[kAtOnce];
+              if constexpr (MODE == FEW)
+                load32((more ? acc_at + half * 3 * cols : at) + c * 32, y);
+              else
+                load16(at + c * 16, y);
               loads_done();
 #pragma unroll
-              for (int j = 0; j < 16; ++j) x[c * 16 + j] += y[j];
+              for (int j = 0; j < kAtOnce; ++j) x[c * kAtOnce + j] += y[j];
             }
-        }
         fence_before();
         __syncwarp();
         if (lane == 0)
@@ -638,58 +665,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       if constexpr (MODE == FEW) {
         // Lanes hold vocabulary rows, columns the few rows.  Turned over in shared memory, 32
         // columns at a time (word j * 128 + (row ^ j), free of bank conflicts both ways), a
-        // thread takes a quarter of the tile's logits of one row, a warp joins the quarters.
-        const int m_rows = p.tile_m / 2, v0 = it.m0 + rank * m_rows, valid = min(m_rows, p.V - v0);
-        const int quarter = warp & 3;
-        const uint32_t box = out_at + half * 4 * kBoxBytes;  // [32][128] logits
+        // thread takes a quarter of the tile's logits of one row.
+        const int v0 = it.m0 + rank * (p.tile_m / 2), valid = min(p.tile_m / 2, p.V - v0);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           if (b * 32 >= cols) break;
-          const int r = half * cols + b * 32 + lane;  // this thread's row
-          const bool is = b * 32 + lane < cols && r < p.N;
-          half_sync();
+          if (b) half_sync();
 #pragma unroll
           for (int j = 0; j < 32; ++j)
             if (b * 32 + (j & 16) < cols)
-              asm volatile("st.shared.f32 [%0], %1;" ::"r"(box + (j * 128 + (row ^ j)) * 4), "f"(x[b * 32 + j]) : "memory");
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(few_box + (j * 128 + (row ^ j)) * 4), "f"(x[b * 32 + j]) : "memory");
           half_sync();
-          float t = -INFINITY, s = 0.0f;
-          if (is) {
-            const float unit = narrow ? p.row_scale[r] : 1.0f;
-            float y[32];
+          if (few_row[b] < 0) continue;
+          float y[32], t = few_m[b];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y[k]) : "r"(box + (lane * 128 + ((quarter * 32 + k) ^ lane)) * 4));
-              y[k] = quarter * 32 + k < valid ? y[k] * unit : -INFINITY;
-            }
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) t = max3(t, y[k], y[k + 1]);
-            const float ref = t == -INFINITY ? 0.0f : t;
-            float e[4] = {};
-#pragma unroll
-            for (int k = 0; k < 32; ++k) e[k & 3] += exp2_of((y[k] - ref) * kLog2e);
-            s = (e[0] + e[1]) + (e[2] + e[3]);
-            const int64_t own = p.targets[r] - v0;
-            if (own >= quarter * 32 && own < min(valid, quarter * 32 + 32)) {
-              float at_target;
-              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(at_target) : "r"(box + (lane * 128 + ((int)own ^ lane)) * 4));
-              p.xt[r] = at_target * unit;
-            }
+          for (int k = 0; k < 32; ++k) {
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y[k]) : "r"(few_box + (lane * 128 + ((quarter * 32 + k) ^ lane)) * 4));
+            y[k] = quarter * 32 + k < valid ? y[k] * few_unit[b] : -INFINITY;
           }
-          half_sync();
-          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(box + (quarter * 32 + lane) * 8), "f"(t), "f"(s) : "memory");
-          half_sync();
-          if (quarter == 0 && is) {
-            float2 q[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(q[k].x), "=f"(q[k].y) : "r"(box + (k * 32 + lane) * 8));
-            t = fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x));
-            const float ref = t == -INFINITY ? 0.0f : t;
-            s = 0.0f;
+          for (int k = 0; k < 32; k += 2) t = max3(t, y[k], y[k + 1]);
+          const float ref = t == -INFINITY ? 0.0f : t;
+          float e[4] = {few_l[b] * exp2_of((few_m[b] - ref) * kLog2e)};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s += q[k].y * exp2_of((q[k].x - ref) * kLog2e);
-            p.part[(int64_t)(it.m0 / p.tile_m * 2 + rank) * p.N + r] = make_float2(t, s);
+          for (int k = 0; k < 32; ++k) e[k & 3] += exp2_of((y[k] - ref) * kLog2e);
+          few_l[b] = (e[0] + e[1]) + (e[2] + e[3]);
+          few_m[b] = t;
+          const int own = few_target[b] - v0;
+          if (few_target[b] >= 0 && own >= quarter * 32 && own < min(valid, quarter * 32 + 32)) {
+            float at_target;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(at_target) : "r"(few_box + (lane * 128 + (own ^ lane)) * 4));
+            p.xt[few_row[b]] = at_target * few_unit[b];
           }
         }
       }
@@ -766,6 +772,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       }
     }
     if (MODE == STATS) leave();
+    if constexpr (MODE == FEW) {  // a warp joins the quarters
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        half_sync();
+        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(few_box + (quarter * 32 + lane) * 8), "f"(few_m[b]), "f"(few_l[b])
+                     : "memory");
+        half_sync();
+        if (quarter == 0 && few_row[b] >= 0) {
+          float2 q[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(q[k].x), "=f"(q[k].y) : "r"(few_box + (k * 32 + lane) * 8));
+          const float t = fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x)), ref = t == -INFINITY ? 0.0f : t;
+          float sum = 0.0f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sum += q[k].y * exp2_of((q[k].x - ref) * kLog2e);
+          p.part[((int64_t)pair * 2 + rank) * p.N + few_row[b]] = make_float2(t, sum);
+        }
+      }
+    }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   start_next();  // (at the start it would have small kernels wait beside these CTAs: 33 us instead of 27 for 128 rows of float32)
@@ -806,7 +832,7 @@ __global__ void __launch_bounds__(kRowThreads) join_kernel(Problem p, int few, i
   const int64_t all = (int64_t)m_tiles * n_tiles, from = (int64_t)(n / kTileM) * n_tiles;
   const int parts =
       n >= p.N ? 0
-      : few    ? 2 * m_tiles
+      : few    ? 2 * pairs
                : 2 * ((int)(((from + n_tiles) * pairs - 1) / all) - (int)(((from + 1) * pairs - 1) / all) + 1);
   float m = -INFINITY, l = 0.0f;
   for (int i = threadIdx.x % LANES; i < parts; i += 4 * LANES) {
@@ -1261,16 +1287,13 @@ struct Shape {
     piece = piece_of(N, V, g_parts);
   }
   uint32_t kind() const { return f16 ? kKindF16 : kKindBf16; }
-  // The logits' passes.  Of float32 against bf16 all parts of a step follow each other, as they
-  // do where few rows share it: every form of the forward and the backward pass adds alike.
-  // (Sums that are large while the small parts come are cut off more: in spans of 256 of K by
-  // twice as much, 1.1e-7 of a sum of 768 magnitudes, at 29.4 us instead of 31.0 for 128 rows.)
+  // The logits' passes.  Of float32 against bf16 the smaller parts of a step follow each other,
+  // as they do where few rows share it: every form of the forward and the backward pass adds
+  // alike.
   void logit_passes(Gemm& g, bool swapped) const {
     passes(g, h_parts, w_parts, dp, dp);
-    if (h_parts > w_parts) {
-      g.by_step = 1;
-      g.span[0] = kSpan32 / 2;
-    }
+    g.apart = h_parts > w_parts;
+    if (g.apart) std::swap(g.a_part[0][0], g.a_part[0][1]);
     if (swapped) std::swap(g.a_part, g.b_part);
   }
   // The passes of a product of these parts, and of the f16 parts that take their place (two of
@@ -1321,9 +1344,11 @@ struct Forward {
   float* unit;
   int few, tile_m, tile_n, m_tiles, n_tiles, pairs, slots;
   Forward(Layout& a, const Shape& s, bool h_direct, bool w_direct) {
-    // Float32 rows against bf16 meet each step of the vocabulary once (128 rows, 32000 x 768: 27 us, 34 as rows of a
-    // tile, three passes); otherwise only the fewest gain (5 rows of bf16: 17 and 19 us; 64 rows, 8192 x 1024: 16 and 13).
-    few = s.N <= (s.h_parts > s.w_parts ? kFew : 16);
+    // Float32 rows against bf16 meet each step of the vocabulary once (128 rows, 32000 x 768: 27 us, 36 as rows of a
+    // tile, three passes).  Otherwise it is read at memory's speed by tiles enough, with a quarter of the columns or
+    // less (64 rows of bf16: 24000 x 768 16 us, as rows of a tile 18, 152000 x 1024 60 and 63; but 8192 x 1024 16 and
+    // 13; 128 rows, 32000 x 768: 19 and 18.5).
+    few = s.N <= (s.h_parts > s.w_parts ? kFew : s.V > 192 * s.pairs ? 64 : 16);
     if (few) {
       // the vocabulary in as many tiles as there are CTAs, or twice, .. as many, of equal height
       const int rounds = ceil_div(s.V, 256 * s.pairs);
@@ -1331,7 +1356,6 @@ struct Forward {
       tile_n = (int)up(s.N, 32);
       m_tiles = ceil_div(s.V, tile_m);
       n_tiles = 1;
-      slots = m_tiles;
     } else {
       tile_m = kTileM;
       tile_n = kTileN;
@@ -1339,7 +1363,7 @@ struct Forward {
       n_tiles = ceil_div(s.V, tile_n);
     }
     pairs = (int)std::min<int64_t>(s.pairs, (int64_t)m_tiles * n_tiles);
-    if (!few) slots = ceil_div(pairs, m_tiles) + 1;
+    slots = few ? pairs : ceil_div(pairs, m_tiles) + 1;
     h = h_direct ? nullptr : a.take<uint16_t>((int64_t)s.N * s.h_parts * s.dp);
     w = w_direct ? nullptr : a.take<uint16_t>((int64_t)s.V * s.w_parts * s.dp);
     part = a.take<float2>((int64_t)slots * 2 * s.N);
@@ -1522,7 +1546,7 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   if (f.few && s.h_parts > s.w_parts) {
     // the rows' parts meet a step of the vocabulary together, which is then read once
     g.passes[0] = 1;
-    g.b_part[0][0] = 0;
+    g.b_part[0][0] = g.apart = 0;
     p.share = s.h_parts;
   }
   p.part_cols = s.dp;

@@ -100,6 +100,15 @@ def test_matches_oracle(pair, N, V, d):
 
 
 @pytest.mark.parametrize("pair", PAIRS)
+@pytest.mark.parametrize("N,V,d", [(17, 15001, 72), (32, 19200, 40), (33, 40000, 24), (64, 20000, 300), (65, 15001, 64)])
+def test_some_rows_over_a_large_vocabulary(pair, N, V, d):
+    """Few rows as columns of tiles of the vocabulary, one, two and three tiles a CTA, and the
+    first number of rows that is not."""
+    h, w, t = inputs(N, V, d, pair, seed=N)
+    check(h, w, t, "none")
+
+
+@pytest.mark.parametrize("pair", PAIRS)
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 def test_reductions_and_gradients_from_above(pair, reduction):
     h, w, t = inputs(70, 333, 96, pair, seed=3)
