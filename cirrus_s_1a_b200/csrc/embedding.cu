@@ -391,8 +391,10 @@ int launch_sort(Ids ids, int64_t first, int n, int V, const Scratch& s, cudaStre
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, sort_kernel, ids, first, n, V, (bits + 7) / 8, s.keys, s.order) != cudaSuccess)
+  if (cudaLaunchKernelEx(&cfg, sort_kernel, ids, first, n, V, (bits + 7) / 8, s.keys, s.order) != cudaSuccess) {
+    (void)cudaGetLastError();
     return CB_ERR_CUDA;
+  }
   count_launch();
   return CB_OK;
 }

@@ -3,13 +3,14 @@
 //   y = x r w, r = (mean x^2 + eps)^-1/2
 //   dx = r (g w - x r mean(g w x r))          dw = sum over rows of g x r
 //
-// Bound by memory: a row is read once and held in a warp's registers while its sums are
-// taken.  The gradient's warps go through rows in turn and add their part of dw up as they
-// do; the parts of a CTA's warps, then of the CTAs, are added in order, so that the sum does
-// not depend on timing.  Rows that do not fit (more than 2048 columns) or are not 16-byte
-// aligned are taken by a CTA each, read twice, with dw over fixed groups of rows.
+// Bound by memory: a row is read once and held in the registers of a warp, or where rows are
+// few or long of a CTA, while its sums are taken.  The gradient's warps or CTAs go through
+// rows in turn and add their part of dw up as they do; the parts of a CTA's warps, then of the
+// CTAs, are added in order, so that the sum does not depend on timing.  Rows that are not
+// 16-byte aligned are taken by single elements.  Rows too long to be held (more than 8192
+// columns, 4096 of single elements) are read twice, with dw over fixed groups of rows.
 // Measured, 65537 x 1024 in float32: 78 us (6.9 TB/s) and, the gradient, 125 us (6.4 TB/s);
-// 16384 x 768 in bf16, both, 33 us.
+// 16384 x 768 in bf16, both, 33 us; 16384 x 4096 in bf16, both, 160 us (5.0 TB/s), x 769 80 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -33,11 +34,10 @@ __device__ __forceinline__ void load_w(const W* w, float (&o)[VEC]) {
   }
 }
 
-// A warp to a row: NV pieces of 16 bytes a lane.
-template <typename T, typename W, int NV>
+// A warp to a row: NV pieces of VEC elements a lane, 16 bytes or one element.
+template <typename T, typename W, int VEC, int NV>
 __global__ void __launch_bounds__(kThreads) rms_norm_warp_kernel(const T* x, int64_t ld, const W* w, int rows, int d,
                                                                  float eps, T* y) {
-  constexpr int VEC = 16 / sizeof(T);
   const int lane = threadIdx.x & 31, n = blockIdx.x * kWarps + (threadIdx.x >> 5);
   await_before();
   start_next();
@@ -67,12 +67,11 @@ __global__ void __launch_bounds__(kThreads) rms_norm_warp_kernel(const T* x, int
   }
 }
 
-// part[cta][d], or dw itself where there is one CTA.
-template <typename T, typename W, int NV>
+// part[cta][d]
+template <typename T, typename W, int VEC, int NV>
 __global__ void __launch_bounds__(kThreads) rms_norm_grad_warp_kernel(const T* x, int64_t ld, const T* g, int64_t ldg,
                                                                       const W* w, int rows, int d, float eps, T* dx,
-                                                                      float* part, W* dw) {
-  constexpr int VEC = 16 / sizeof(T);
+                                                                      float* part) {
   constexpr int kWide = NV * VEC * 32;   // columns of NV pieces a lane, d of them or more
   __shared__ float s_part[kWarps / 2][kWide];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -144,9 +143,7 @@ __global__ void __launch_bounds__(kThreads) rms_norm_grad_warp_kernel(const T* x
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
       const int j = (i * 32 + lane) * VEC + k;
-      if (j >= d) continue;
-      if (gridDim.x == 1) dw[j] = Elem<W>::put(acc[i][k]);
-      else part[(int64_t)blockIdx.x * d + j] = acc[i][k];
+      if (j < d) part[(int64_t)blockIdx.x * d + j] = acc[i][k];
     }
 }
 
@@ -174,6 +171,108 @@ __global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* part, in
   }
 }
 
+// A CTA to a row that it holds: NV pieces of VEC elements a thread.
+template <typename T, typename W, int VEC, int NV>
+__global__ void __launch_bounds__(kThreads) rms_norm_cta_kernel(const T* x, int64_t ld, const W* w, int d, float eps, T* y) {
+  __shared__ float red[33];
+  await_before();
+  start_next();
+  Vec<T, VEC> v[NV];
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = (i * kThreads + threadIdx.x) * VEC;
+    if (j < d) v[i] = *reinterpret_cast<const Vec<T, VEC>*>(x + blockIdx.x * ld + j);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if ((i * kThreads + threadIdx.x) * VEC < d)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s += Elem<T>::get(v[i].v[k]) * Elem<T>::get(v[i].v[k]);
+  const float r = rsqrtf(block_sum(s, red) / d + eps);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = (i * kThreads + threadIdx.x) * VEC;
+    if (j >= d) continue;
+    float u[VEC];
+    load_w<W, VEC>(w + j, u);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[i].v[k] = Elem<T>::put(Elem<T>::get(v[i].v[k]) * r * u[k]);
+    *reinterpret_cast<Vec<T, VEC>*>(y + (int64_t)blockIdx.x * d + j) = v[i];
+  }
+}
+
+// CTAs take rows in turn.  part[cta][d]
+template <typename T, typename W, int VEC, int NV>
+__global__ void __launch_bounds__(kThreads) rms_norm_grad_cta_kernel(const T* x, int64_t ld, const T* g, int64_t ldg, const W* w,
+                                                                     int rows, int d, float eps, T* dx, float* part) {
+  __shared__ float2 s_sum[2][kWarps];  // one is read while the next row's is written
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float acc[NV][VEC] = {};
+  int which = 0;
+  await_before();
+  start_next();
+  for (int n = blockIdx.x; n < rows; n += gridDim.x, which ^= 1) {
+    Vec<T, VEC> v[NV], up[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * kThreads + threadIdx.x) * VEC;
+      if (j < d) {
+        v[i] = *reinterpret_cast<const Vec<T, VEC>*>(x + n * ld + j);
+        up[i] = *reinterpret_cast<const Vec<T, VEC>*>(g + n * ldg + j);
+      }
+    }
+    float s = 0.0f, c = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * kThreads + threadIdx.x) * VEC;
+      if (j >= d) continue;
+      float u[VEC];
+      load_w<W, VEC>(w + j, u);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float a = Elem<T>::get(v[i].v[k]);
+        s += a * a;
+        c += Elem<T>::get(up[i].v[k]) * u[k] * a;
+      }
+    }
+    s = warp_sum(s);
+    c = warp_sum(c);
+    if (lane == 0) s_sum[which][warp] = make_float2(s, c);
+    __syncthreads();
+    s = c = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+      s += s_sum[which][k].x;
+      c += s_sum[which][k].y;
+    }
+    const float r = rsqrtf(s / d + eps), m = c * r / d * r;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * kThreads + threadIdx.x) * VEC;
+      if (j >= d) continue;
+      float u[VEC];
+      load_w<W, VEC>(w + j, u);
+      Vec<T, VEC> o;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float a = Elem<T>::get(v[i].v[k]), b = Elem<T>::get(up[i].v[k]);
+        o.v[k] = Elem<T>::put(r * (b * u[k] - a * m));
+        acc[i][k] += b * (a * r);
+      }
+      *reinterpret_cast<Vec<T, VEC>*>(dx + (int64_t)n * d + j) = o;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const int j = (i * kThreads + threadIdx.x) * VEC + k;
+      if (j < d) part[(int64_t)blockIdx.x * d + j] = acc[i][k];
+    }
+}
+
+// Rows of any length, read twice.
 template <typename T, typename W>
 __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const T* x, int64_t ld, const W* w, int d, float eps, T* y) {
   __shared__ float red[33];
@@ -226,27 +325,49 @@ __global__ void __launch_bounds__(kThreads) rms_norm_dw_part_kernel(const T* x, 
   part[(int64_t)blockIdx.x * d + j] = s;
 }
 
-// f(number of 16-byte pieces a lane) for rows of d columns.
+// Whether a row's pieces can be 16 bytes.
+bool in_pieces(const void* x, int64_t ld, int rows, int d, int size) {
+  return d * size % 16 == 0 && aligned_to(x, 16) && (rows == 1 || ld * size % 16 == 0);
+}
+
+// Whether warps take a row each: enough rows (768 columns of float32: 300 rows 2.5 us, by CTAs
+// 1.8, 2400 rows 2.9 and 3.9; both directions 300 rows 7.7 and 6.5, 600 rows 8.2 and 9.9) of up
+// to 4096 bytes, in the gradient 1024 columns, whose sums fill the registers (16384 x 1536 in
+// bf16 87 us, by CTAs 74, in float32 140 and 93; x 1024 39 and 62, 61 and 76), and 512 of
+// single elements (16384 x 255 24 us, by CTAs 61; x 769 122 and 78).
+bool in_a_warp(int rows, int d, int size, bool pieces, bool grad) {
+  return rows > (grad ? 3 : 6) * num_sms() && (!pieces ? d <= 512 : grad ? d <= 1024 : d * size <= 4096);
+}
+// Whether CTAs hold a row each.
+bool in_a_cta(int d, bool pieces) { return d <= (pieces ? 8192 : 4096); }
+
+// f(elements of a piece, pieces a thread): the first of NV that holds n pieces.
+template <int VEC, int NV, int... MORE, typename F>
+int first_of(int n, F&& f) {
+  if constexpr (sizeof...(MORE) > 0)
+    if (n > NV) return first_of<VEC, MORE...>(n, f);
+  return f(std::integral_constant<int, VEC>{}, std::integral_constant<int, NV>{});
+}
 template <typename T, typename F>
-int with_pieces(int d, F&& f) {
-  const int n = ceil_div(d, 32 * 16 / (int)sizeof(T));
-  if (n <= 1) return f(std::integral_constant<int, 1>{});
-  if (n <= 2) return f(std::integral_constant<int, 2>{});
-  if (n <= 3) return f(std::integral_constant<int, 3>{});
-  if (n <= 4) return f(std::integral_constant<int, 4>{});
-  if (n <= 6) return f(std::integral_constant<int, 6>{});
-  if (n <= 8 || sizeof(T) == 2) return f(std::integral_constant<int, 8>{});
-  return f(std::integral_constant<int, sizeof(T) == 4 ? 16 : 8>{});
+int warp_pieces(int d, bool pieces, F&& f) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int n = ceil_div(d, 32 * (pieces ? VEC : 1));
+  if (!pieces) return first_of<1, 4, 8, 16>(n, f);
+  return first_of<VEC, 1, 2, 3, 4, 6, 8>(n, f);
+}
+template <typename T, typename F>
+int cta_pieces(int d, bool pieces, F&& f) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int n = ceil_div(d, kThreads * (pieces ? VEC : 1));
+  if (!pieces) return first_of<1, 3, 4, 6, 8, 16>(n, f);
+  if constexpr (sizeof(T) == 4) return first_of<VEC, 2, 4, 8>(n, f);
+  else return first_of<VEC, 1, 2, 4>(n, f);
 }
 
-// Whether a warp can hold a row: 16-byte pieces, 2048 columns.
-bool in_a_warp(const void* x, int64_t ld, int rows, int d, int size) {
-  return d <= 2048 && d * size % 16 == 0 && aligned_to(x, 16) && (rows == 1 || ld * size % 16 == 0);
-}
-
-// CTAs of the gradient's warps: 16 rows or fewer to one (dw then needs no second kernel), at
-// most two to an SM (bf16, 65537 x 768 with the forward: 103 us, 121 with three).
-int grad_ctas(int rows) { return rows <= 2 * kWarps ? 1 : std::min(ceil_div(rows, kWarps), 2 * num_sms()); }
+// CTAs of the gradient: of warps at most two to an SM (bf16, 65537 x 768 with the forward: 103
+// us, 121 with three), of those that hold a row four.
+int warp_ctas(int rows) { return std::min(ceil_div(rows, kWarps), 2 * num_sms()); }
+int row_ctas(int rows) { return std::min(rows, 4 * num_sms()); }
 
 template <typename F>
 int with_types(int32_t dtype, int32_t w_dtype, F&& f) {
@@ -268,17 +389,22 @@ extern "C" int cb_rms_norm(const void* x, int32_t dtype, int64_t ld, const void*
   if (bad(x, dtype, ld, w, w_dtype, rows, d) || !y || !aligned_to(y, dtype_size(dtype))) return CB_ERR_ARG;
   if (rows > CB_ENDS_MAX_ROWS || d > CB_ENDS_MAX_DIM) return CB_ERR_SHAPE;
   cudaStream_t st = (cudaStream_t)stream;
-  const bool warps = in_a_warp(x, ld, rows, d, dtype_size(dtype)) && aligned_to(y, 16) && aligned_to(w, 16);
+  const bool pieces = in_pieces(x, ld, rows, d, dtype_size(dtype)) && aligned_to(y, 16) && aligned_to(w, 16);
   return with_types(dtype, w_dtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
     const T* in = static_cast<const T*>(x);
     const W* weight = static_cast<const W*>(w);
-    if (!warps) {
+    if (!in_a_cta(d, pieces)) {
       return launch_after(rms_norm_kernel<T, W>, dim3(rows), kThreads, 0, st, in, ld, weight, d, eps, static_cast<T*>(y));
     }
-    return with_pieces<T>(d, [&](auto nv) {
-      return launch_after(rms_norm_warp_kernel<T, W, decltype(nv)::value>, dim3(ceil_div(rows, kWarps)), kThreads, 0, st, in,
+    if (!in_a_warp(rows, d, dtype_size(dtype), pieces, false))
+      return cta_pieces<T>(d, pieces, [&](auto vec, auto nv) {
+        return launch_after(rms_norm_cta_kernel<T, W, decltype(vec)::value, decltype(nv)::value>, dim3(rows), kThreads, 0, st,
+                            in, ld, weight, d, eps, static_cast<T*>(y));
+      });
+    return warp_pieces<T>(d, pieces, [&](auto vec, auto nv) {
+      return launch_after(rms_norm_warp_kernel<T, W, decltype(vec)::value, decltype(nv)::value>, dim3(ceil_div(rows, kWarps)), kThreads, 0, st, in,
                           ld, weight, rows, d, eps, static_cast<T*>(y));
     });
   });
@@ -286,7 +412,7 @@ extern "C" int cb_rms_norm(const void* x, int32_t dtype, int64_t ld, const void*
 
 extern "C" size_t cb_rms_norm_grad_scratch_bytes(int32_t rows, int32_t d) {
   if (rows <= 0 || d <= 0 || rows > CB_ENDS_MAX_ROWS || d > CB_ENDS_MAX_DIM) return 0;
-  return ((size_t)rows + (size_t)std::max(ceil_div(rows, kGroup), grad_ctas(rows)) * d) * sizeof(float);
+  return ((size_t)rows + (size_t)std::max(ceil_div(rows, kGroup), row_ctas(rows)) * d) * sizeof(float);
 }
 
 extern "C" int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const void* g, int64_t ldg, const void* w,
@@ -301,8 +427,8 @@ extern "C" int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const 
   if (scratch_bytes < need) return CB_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
   const int size = dtype_size(dtype);
-  const bool warps = in_a_warp(x, ld, rows, d, size) && in_a_warp(g, ldg, rows, d, size) && aligned_to(dx, 16) &&
-                     aligned_to(w, 16);
+  const bool pieces = in_pieces(x, ld, rows, d, size) && in_pieces(g, ldg, rows, d, size) && aligned_to(dx, 16) &&
+                      aligned_to(w, 16);
   return with_types(dtype, w_dtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
@@ -311,14 +437,22 @@ extern "C" int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const 
     float* rstd = static_cast<float*>(scratch);
     float* part = rstd + rows;
     int parts;
-    if (warps) {
+    if (in_a_warp(rows, d, size, pieces, true)) {
       part = rstd;
-      parts = grad_ctas(rows);
-      const int rc = with_pieces<T>(d, [&](auto nv) {
-        return launch_after(rms_norm_grad_warp_kernel<T, W, decltype(nv)::value>, dim3(parts), kThreads, 0, st, in, ld, up,
-                            ldg, weight, rows, d, eps, static_cast<T*>(dx), part, static_cast<W*>(dw));
+      parts = warp_ctas(rows);
+      const int rc = warp_pieces<T>(d, pieces, [&](auto vec, auto nv) {
+        return launch_after(rms_norm_grad_warp_kernel<T, W, decltype(vec)::value, decltype(nv)::value>, dim3(parts), kThreads,
+                            0, st, in, ld, up, ldg, weight, rows, d, eps, static_cast<T*>(dx), part);
       });
-      if (rc || parts == 1) return rc;
+      if (rc) return rc;
+    } else if (in_a_cta(d, pieces)) {
+      part = rstd;
+      parts = row_ctas(rows);
+      const int rc = cta_pieces<T>(d, pieces, [&](auto vec, auto nv) {
+        return launch_after(rms_norm_grad_cta_kernel<T, W, decltype(vec)::value, decltype(nv)::value>, dim3(parts), kThreads, 0,
+                            st, in, ld, up, ldg, weight, rows, d, eps, static_cast<T*>(dx), part);
+      });
+      if (rc) return rc;
     } else {
       parts = ceil_div(rows, kGroup);
       if (int rc = launch_after(rms_norm_dx_kernel<T, W>, dim3(rows), kThreads, 0, st, in, ld, up, ldg, weight, d, eps,

@@ -59,6 +59,28 @@ def test_matches_oracle(pair, R, d):
 
 
 @pytest.mark.parametrize("pair", PAIRS)
+@pytest.mark.parametrize("R,d", [(1, 33), (16, 127), (1500, 127), (17, 129), (600, 255), (1200, 257), (40, 511), (1001, 512),
+                                 (2500, 513), (50, 769), (1, 1023), (20, 1025), (2500, 1031), (9, 2047), (700, 4095),
+                                 (5, 4097)])
+def test_rows_of_single_elements(pair, R, d):
+    """Widths at both ends of each number of elements a thread, and past the last."""
+    check(*case(R, d, pair, seed=R + d))
+
+
+@pytest.mark.parametrize("pair", PAIRS)
+@pytest.mark.parametrize("R,d", [(1, 2056), (700, 4096), (3, 4104), (40, 6152), (601, 8192), (5, 8200)])
+def test_long_rows(pair, R, d):
+    check(*case(R, d, pair, seed=R + d))
+
+
+@pytest.mark.parametrize("pair", PAIRS)
+@pytest.mark.parametrize("R,d", [(1500, 8), (1200, 264), (1000, 512), (999, 768), (1300, 1024), (1300, 1032), (1000, 2048)])
+def test_many_rows(pair, R, d):
+    """Rows enough for a warp each, at the ends of each number of pieces a lane."""
+    check(*case(R, d, pair, seed=R + d))
+
+
+@pytest.mark.parametrize("pair", PAIRS)
 def test_strides_and_alignment(pair):
     X, W, G = case(50, 300, pair, seed=1)
     Xd, Wd, Gd = X.to(DEV), W.to(DEV), G.to(DEV)
