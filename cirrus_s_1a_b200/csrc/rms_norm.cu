@@ -10,7 +10,7 @@
 // 16-byte aligned are taken by single elements.  Rows too long to be held (more than 8192
 // columns, 4096 of single elements) are read twice, with dw over fixed groups of rows.
 // Measured, 65537 x 1024 in float32: 78 us (6.9 TB/s) and, the gradient, 125 us (6.4 TB/s);
-// 16384 x 768 in bf16, both, 33 us; 16384 x 4096 in bf16, both, 160 us (5.0 TB/s), x 769 80 us.
+// 16384 x 768 in bf16, both, 33 us; 16384 x 4096 in bf16, both, 139 us (4.8 TB/s), x 769 63 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -202,9 +202,11 @@ __global__ void __launch_bounds__(kThreads) rms_norm_cta_kernel(const T* x, int6
   }
 }
 
-// CTAs take rows in turn.  part[cta][d]
+// CTAs take rows in turn, row_ctas (for so many columns a thread) to an SM: 16384 x 4096 in bf16
+// 139 us, 160 with registers for three.  part[cta][d]
+constexpr int row_ctas(int columns) { return columns <= 16 ? 4 : 2; }
 template <typename T, typename W, int VEC, int NV>
-__global__ void __launch_bounds__(kThreads) rms_norm_grad_cta_kernel(const T* x, int64_t ld, const T* g, int64_t ldg, const W* w,
+__global__ void __launch_bounds__(kThreads, row_ctas(NV * VEC)) rms_norm_grad_cta_kernel(const T* x, int64_t ld, const T* g, int64_t ldg, const W* w,
                                                                      int rows, int d, float eps, T* dx, float* part) {
   __shared__ float2 s_sum[2][kWarps];  // one is read while the next row's is written
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -212,15 +214,31 @@ __global__ void __launch_bounds__(kThreads) rms_norm_grad_cta_kernel(const T* x,
   int which = 0;
   await_before();
   start_next();
-  for (int n = blockIdx.x; n < rows; n += gridDim.x, which ^= 1) {
-    Vec<T, VEC> v[NV], up[NV];
+  // The next row is on its way meanwhile where registers allow (16384 x 2047 in float32 131 us,
+  // with it 114; 16 columns a thread: x 4096 213 and 284).
+  constexpr bool kNext = NV * VEC <= 8;
+  Vec<T, VEC> v[NV], up[NV], next_v[kNext ? NV : 1], next_up[kNext ? NV : 1];
+  auto load = [&](int n, auto& to_v, auto& to_up) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = (i * kThreads + threadIdx.x) * VEC;
-      if (j < d) {
-        v[i] = *reinterpret_cast<const Vec<T, VEC>*>(x + n * ld + j);
-        up[i] = *reinterpret_cast<const Vec<T, VEC>*>(g + n * ldg + j);
+      if (n < rows && j < d) {
+        to_v[i] = *reinterpret_cast<const Vec<T, VEC>*>(x + n * ld + j);
+        to_up[i] = *reinterpret_cast<const Vec<T, VEC>*>(g + n * ldg + j);
       }
+    }
+  };
+  if constexpr (kNext) load(blockIdx.x, next_v, next_up);
+  for (int n = blockIdx.x; n < rows; n += gridDim.x, which ^= 1) {
+    if constexpr (kNext) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        v[i] = next_v[i];
+        up[i] = next_up[i];
+      }
+      load(n + gridDim.x, next_v, next_up);
+    } else {
+      load(n, v, up);
     }
     float s = 0.0f, c = 0.0f;
 #pragma unroll
@@ -334,7 +352,7 @@ bool in_pieces(const void* x, int64_t ld, int rows, int d, int size) {
 // 1.8, 2400 rows 2.9 and 3.9; both directions 300 rows 7.7 and 6.5, 600 rows 8.2 and 9.9) of up
 // to 4096 bytes, in the gradient 1024 columns, whose sums fill the registers (16384 x 1536 in
 // bf16 87 us, by CTAs 74, in float32 140 and 93; x 1024 39 and 62, 61 and 76), and 512 of
-// single elements (16384 x 255 24 us, by CTAs 61; x 769 122 and 78).
+// single elements (16384 x 255 24 us, by CTAs 61; x 769 122 and 64).
 bool in_a_warp(int rows, int d, int size, bool pieces, bool grad) {
   return rows > (grad ? 3 : 6) * num_sms() && (!pieces ? d <= 512 : grad ? d <= 1024 : d * size <= 4096);
 }
@@ -365,9 +383,9 @@ int cta_pieces(int d, bool pieces, F&& f) {
 }
 
 // CTAs of the gradient: of warps at most two to an SM (bf16, 65537 x 768 with the forward: 103
-// us, 121 with three), of those that hold a row four.
+// us, 121 with three), of those that hold a row two or four.
 int warp_ctas(int rows) { return std::min(ceil_div(rows, kWarps), 2 * num_sms()); }
-int row_ctas(int rows) { return std::min(rows, 4 * num_sms()); }
+int row_ctas(int rows, int columns) { return std::min(rows, row_ctas(columns) * num_sms()); }
 
 template <typename F>
 int with_types(int32_t dtype, int32_t w_dtype, F&& f) {
@@ -412,7 +430,7 @@ extern "C" int cb_rms_norm(const void* x, int32_t dtype, int64_t ld, const void*
 
 extern "C" size_t cb_rms_norm_grad_scratch_bytes(int32_t rows, int32_t d) {
   if (rows <= 0 || d <= 0 || rows > CB_ENDS_MAX_ROWS || d > CB_ENDS_MAX_DIM) return 0;
-  return ((size_t)rows + (size_t)std::max(ceil_div(rows, kGroup), row_ctas(rows)) * d) * sizeof(float);
+  return ((size_t)rows + (size_t)std::max(ceil_div(rows, kGroup), row_ctas(rows, 1)) * d) * sizeof(float);
 }
 
 extern "C" int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const void* g, int64_t ldg, const void* w,
@@ -447,8 +465,8 @@ extern "C" int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const 
       if (rc) return rc;
     } else if (in_a_cta(d, pieces)) {
       part = rstd;
-      parts = row_ctas(rows);
       const int rc = cta_pieces<T>(d, pieces, [&](auto vec, auto nv) {
+        parts = row_ctas(rows, vec * nv);
         return launch_after(rms_norm_grad_cta_kernel<T, W, decltype(vec)::value, decltype(nv)::value>, dim3(parts), kThreads, 0,
                             st, in, ld, up, ldg, weight, rows, d, eps, static_cast<T*>(dx), part);
       });
