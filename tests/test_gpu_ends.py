@@ -59,6 +59,37 @@ def test_tied_table_gets_both_gradients(dtype, n, V, d):
         assert (got.cpu().double() - ref).norm() <= 8 * u * ref.norm() + 1e-12
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_threads_on_streams_of_their_own(dtype):
+    """Calls at the same time have their own scratch and give the bits of one alone."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    g = torch.Generator().manual_seed(8)
+    ids = [torch.randint(0, 2500, (n,), generator=g).to(DEV) for n in (900, 40)]
+    targets = [torch.randint(-1, 2500, (len(i),), generator=g).to(DEV) for i in ids]
+    table = (torch.randn(2500, 128, generator=g) / 8).to(TYPES[dtype]).to(DEV)
+    norm = torch.ones(128, dtype=TYPES[dtype], device=DEV)
+
+    def step(k):
+        t, n = table.detach().requires_grad_(), norm.detach().requires_grad_()
+        loss = chain(ids[k], t, n, targets[k], 2.0, ours())
+        return loss.detach(), *torch.autograd.grad(loss, (t, n))
+
+    def many(k):
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            out = [step(k) for _ in range(20)]
+        side.synchronize()
+        return out
+
+    alone = [step(k) for k in range(2)]
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(2) as pool:
+        for k, runs in enumerate(pool.map(many, range(2))):
+            for out in runs:
+                assert all(torch.equal(a, b) for a, b in zip(out, alone[k]))
+
+
 def test_a_captured_training_step_and_an_eager_one():
     """A step of plain descent on the tied table, captured while an eager graph of the same
     table has lived: replays equal the eager steps bit for bit."""

@@ -109,6 +109,13 @@ def test_some_rows_over_a_large_vocabulary(pair, N, V, d):
 
 
 @pytest.mark.parametrize("pair", PAIRS)
+@pytest.mark.parametrize("N,V", [(3, 40), (270, 5)])
+def test_widest_rows(pair, N, V):
+    h, w, t = inputs(N, V, 65536, pair, seed=N)
+    check(h, w, t, "sum")
+
+
+@pytest.mark.parametrize("pair", PAIRS)
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 def test_reductions_and_gradients_from_above(pair, reduction):
     h, w, t = inputs(70, 333, 96, pair, seed=3)

@@ -68,7 +68,7 @@ def test_rows_of_single_elements(pair, R, d):
 
 
 @pytest.mark.parametrize("pair", PAIRS)
-@pytest.mark.parametrize("R,d", [(1, 2056), (700, 4096), (3, 4104), (40, 6152), (601, 8192), (5, 8200)])
+@pytest.mark.parametrize("R,d", [(1, 2056), (700, 4096), (3, 4104), (40, 6152), (601, 8192), (5, 8200), (3, 65536)])
 def test_long_rows(pair, R, d):
     check(*case(R, d, pair, seed=R + d))
 
