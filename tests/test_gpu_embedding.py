@@ -55,6 +55,14 @@ def test_matches_oracle(dtype, n, V, d):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [2, 6, 12, 70, 100, 258, 516, 771])
+def test_widths_of_smaller_pieces(dtype, d):
+    """Rows whose pieces are 8 or 4 bytes or one element."""
+    ids, table, g = case(700, 60, d, dtype, seed=d)
+    check(ids, table, g, scale=1.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_one_token_many_times_and_none_at_all(dtype):
     ids, table, g = case(4097, 50, 72, dtype, seed=1, padded=0.0)
     check(torch.full_like(ids, 49), table, g)
