@@ -26,7 +26,7 @@
 // which is one part: two products and three.
 // Measured, 16384 x 32000 x 768 in bf16: loss 545 us = 1.48 PFLOP/s (tensor pipe 88 %),
 // with the gradient 2665 us = 1.21 PFLOP/s, at the power limit (G of a quarter of the
-// vocabulary 140 us, both its products 250 us, tensor pipe 77 and 90 %).  5 rows 16 us,
+// vocabulary 140 us, both its products 250 us, tensor pipe 77 and 90 %).  5 rows 17 us,
 // 128 rows of float32 against bf16 25 us, of which one read of W is 7.5.
 // Every wait is bounded (%globaltimer); one that gives up sets CB_ERR_TIMEOUT.
 #include <cuda.h>
@@ -52,7 +52,10 @@ constexpr int kMaxPasses = 6, kMaxPairs = 128;
 // Sums in tensor memory are cut off, not rounded, after every 16 products: over 48 of them a
 // row's lse was 5e-7 off, over 1500 the gradients 4e-5.  So a span of K is added up there,
 // and the spans in registers, rounded: 1024 of K, or 256 where float32 parts are multiplied.
-constexpr int kSpan16 = 16, kSpan32 = 4;
+// 256 also in the logits of up to 64 16-bit rows, which wait for W (5 rows of 768 columns are 8e-8
+// off instead of 2.4e-7, the plain float32 form 4e-8, in 17.5 us instead of 16.5; 16384 rows would
+// take 610 us instead of 545).
+constexpr int kSpan16 = 16, kSpan32 = 4, kSpan32Rows = 64;
 constexpr uint64_t kWaitNs = 2000000000ull, kDrainNs = 10000000ull;
 
 // Rows up to which the forward has them as columns and the vocabulary as rows of its tiles.
@@ -1293,6 +1296,7 @@ struct Shape {
   // alike.
   void logit_passes(Gemm& g, bool swapped) const {
     passes(g, h_parts, w_parts, dp, dp);
+    if (N <= kSpan32Rows) g.span[0] = kSpan32;
     g.apart = h_parts > w_parts;
     if (g.apart) std::swap(g.a_part[0][0], g.a_part[0][1]);
     if (swapped) std::swap(g.a_part, g.b_part);
