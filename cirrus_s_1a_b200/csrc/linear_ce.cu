@@ -58,6 +58,14 @@ constexpr int kMaxPasses = 6, kMaxPairs = 128;
 constexpr int kSpan16 = 16, kSpan32 = 4, kSpan32Rows = 64;
 constexpr uint64_t kWaitNs = 2000000000ull, kDrainNs = 10000000ull;
 
+// 16-bit rows up to which the backward pass holds G in two parts.  One part is off by half a
+// step, as the results' own rounding is: over many rows their errors come to 1.2 to 1.4 of what
+// rounding the results alone gives, but of few rows single roundings show (3 rows of f16, dW 1.7
+// times).  The second part takes 8 to 14 % of the loss with its gradient up to 128 rows (32000 x
+// 768 in bf16: 3 rows 80 us and 89, 128 rows 86 and 97), 18 to 45 % of 256 to 1001 rows (256 rows
+// 92 and 108, over 200000 x 1024 461 and 664; 1001 rows 184 and 269).
+constexpr int kTwoRows = 128;
+
 // Rows up to which the forward has them as columns and the vocabulary as rows of its tiles.
 constexpr int kFew = 128;
 
@@ -1281,7 +1289,7 @@ struct Shape {
   Shape(int32_t h_dtype, int32_t w_dtype, int N_, int V_, int d_) : N(N_), V(V_), d(d_), dp((int)up(d_, kStep)) {
     h_parts = h_dtype == CB_F32 ? 3 : 1;
     w_parts = w_dtype == CB_F32 ? 3 : 1;
-    g_parts = h_parts;
+    g_parts = h_parts == 1 && N <= kTwoRows ? 2 : h_parts;
     // bf16 W would be read where it lies for bf16 parts: worth a copy in f16 for many rows (the loss of 1100 rows, 32000
     // x 768: 110 us, 121 in bf16 parts; of 16384 1310 and 2050)
     tried = w_parts == 3 || (h_parts == 3 && N > 1024);

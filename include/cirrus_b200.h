@@ -562,7 +562,8 @@ int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int
  * g_lse (either null for zeros) are float32, of row n at n * step (step 0: one for all);
  * for a reduced loss g_loss is [1].  lse and count are the forward's.  A row without a
  * gradient (no target and g_lse 0) adds nothing, whatever it holds.  G is rounded to the
- * 16-bit type before the products; for float32 it is carried in about 22 bits, and what lies
+ * 16-bit type before the products (of up to 128 rows it is held in two parts, the second of
+ * what the first leaves out); for float32 it is carried in about 22 bits, and what lies
  * below 2^-38 of the largest |g_loss + g_lse| or |g_loss| may be taken as 0 (in float16
  * too, of the row's own); in dw also what lies below 2^-39 of the largest value of float32 h.
  * x here has the bits that it had in the forward pass, so that G is 0 where the target has
