@@ -35,3 +35,29 @@ def test_gradients_of_few_16_bit_rows_are_rounded_once(pair, N, V, d):
         err = (got[n].cpu().double() - r[n]).abs()
         tol = tol * 1.01 + r[n].abs() * half_step(h.dtype) * (1 + half_step(h.dtype)) + smallest(h.dtype)
         assert (err <= tol).all(), (n, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("N", [5, 18944])
+def test_the_sum_over_a_long_vocabulary(N):
+    """Logits that are exact (multiples of 2^-7), so that the sum alone is off.  18944 rows are
+    as many tiles as there are pairs of CTAs: a run goes over all 4096 tiles of 256 vocabulary
+    rows.  Each addition of a tile's sum to the run's is off by at most 2^-24 of what there is
+    by then, evenly: over T of them, growing evenly, 2^-24 sqrt(T) / 3 in the mean square.
+    Beside it 2^-21 for the exponentials and a tile's own additions, in the mean over so many,
+    and 2^-21 for the join and the logarithm."""
+    from cirrus_s_1a_b200.loss import linear_cross_entropy
+
+    V, d = 1 << 20, 8
+    g = torch.Generator(device=DEV).manual_seed(N)
+    h = torch.randint(-8, 9, (N, d), generator=g, device=DEV) / 8
+    w = torch.randint(-32, 33, (V, d), generator=g, device=DEV) / 16
+    h[:, 7], w[:, 7] = 1.0, -14.0  # lse near 0, so that its own rounding is small
+    t = torch.randint(0, V, (N,), generator=g, device=DEV)
+    r = linear_cross_entropy(h.bfloat16(), w.bfloat16(), t, "none")
+    some = torch.arange(0, N, max(1, N // 1024), device=DEV)
+    lse = torch.cat([torch.logsumexp(h[i].double() @ w.double().T, 1) for i in some.split(64)])
+    x = (h[some].double() * w[t[some]].double()).sum(1)
+    tol = 2.0 ** -24 * math.sqrt(V / 256) / 3 + 2 * 2.0 ** -21
+    for got, want in ((r.lse[some], lse), (r.loss[some], lse - x)):
+        off = float((got.double() - want).square().mean().sqrt())
+        assert off <= tol + 2.0 ** -24 * float(want.abs().max()), (off, tol)
