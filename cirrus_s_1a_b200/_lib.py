@@ -47,7 +47,7 @@ EXPORTS = ("cb_abi_version", "cb_status_string", "cb_nvfp4_quantize", "cb_nvfp4_
            "cb_kv8_attend_scratch_bytes", "cb_kv8_attend", "cb_kv8_evict", "cb_forward_kv8_workspace_bytes",
            "cb_forward_kv8", "cb_token_logprobs", "cb_embedding", "cb_embedding_grad_scratch_bytes", "cb_embedding_grad",
            "cb_rms_norm", "cb_rms_norm_grad_scratch_bytes", "cb_rms_norm_grad", "cb_linear_ce_scratch_bytes",
-           "cb_linear_ce", "cb_linear_ce_grad")
+           "cb_linear_ce", "cb_linear_ce_grad", "cb_linear_ce_set_wait_limit")
 
 P = C.c_void_p
 I32 = C.c_int32
@@ -186,6 +186,7 @@ def lib() -> C.CDLL:
         L.cb_linear_ce.argtypes = [P, I32, I64, P, I32, I64, I32, I32, I32, P, I32, I32, P, P, P, P, N, P, P]
         L.cb_linear_ce_grad.argtypes = [P, I32, I64, P, I32, I64, I32, I32, I32, P, I32, I32, P, P, P, I64, P, I64, P, P,
                                         P, N, P, P]
+        L.cb_linear_ce_set_wait_limit.argtypes = [C.c_uint64, I32]
         for fn in (L.cb_embedding_grad_scratch_bytes, L.cb_rms_norm_grad_scratch_bytes, L.cb_linear_ce_scratch_bytes):
             fn.restype = N
         L.cb_read_trace.argtypes = [C.POINTER(CbModel), I32, I32, I32, P, P, I32, P]

@@ -28,10 +28,12 @@
 // with the gradient 2665 us = 1.21 PFLOP/s, at the power limit (G of a quarter of the
 // vocabulary 140 us, both its products 250 us, tensor pipe 77 and 90 %).  5 rows 17 us,
 // 128 rows of float32 against bf16 25 us, of which one read of W is 7.5.
-// Every wait is bounded (%globaltimer); one that gives up sets CB_ERR_TIMEOUT.
+// Every wait is bounded (%globaltimer).  One that gives up sets CB_ERR_TIMEOUT, and what its
+// CTA had still to give is NaN, so that a caller without a status word sees it too.
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "ends.cuh"
 
@@ -57,6 +59,9 @@ constexpr int kMaxPasses = 6, kMaxPairs = 128;
 // take 610 us instead of 545).
 constexpr int kSpan16 = 16, kSpan32 = 4, kSpan32Rows = 64;
 constexpr uint64_t kWaitNs = 2000000000ull, kDrainNs = 10000000ull;
+// cb_linear_ce_set_wait_limit's
+std::atomic<uint64_t> wait_limit{kWaitNs};
+std::atomic<int32_t> stalled_pair{-1};
 
 // 16-bit rows up to which the backward pass holds G in two parts.  One part is off by half a
 // step, as the results' own rounding is: over many rows their errors come to 1.2 to 1.4 of what
@@ -120,6 +125,8 @@ struct alignas(64) Args {
   int g_parts, g_cols;             // of G: columns of one part
   int is_f16;                      // 16-bit operands are f16
   int32_t* status;
+  uint64_t wait_ns;                // limit of a wait
+  int stalled;                     // the pair that copies nothing (tests; none: -1)
 };
 
 // ------------------------------------------------------------- primitives
@@ -423,7 +430,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   volatile int* abort_flag = &s_abort;
   auto wait = [&](uint32_t bar, uint32_t parity) {
     if (*abort_flag) return false;
-    if (bounded_wait(bar, parity, kWaitNs)) return true;
+    if (bounded_wait(bar, parity, p.wait_ns)) return true;
     *abort_flag = 1;
     return false;
   };
@@ -433,7 +440,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     if (elect_one()) {
       int n = 0;  // steps so far
       Item it;
-      bool go = true;
+      bool go = pair != p.stalled;
       for (int i = 0; go && item_of<MODE>(p, pair, i, it); ++i) {
         const Gemm& g = p.g[MODE == PRODUCTS ? it.gemm : 0];
         const int n_rows = MODE == PRODUCTS ? kTileN / 2 : p.tile_n / 2, m_rows = MODE == FEW ? p.tile_m / 2 : 128;
@@ -645,8 +652,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_leader(freed + 8 * acc))
                        : "memory");
       }
-      // the half's four warps agree, or its barriers would not
-      if (any_of_half(half, !go)) break;
+      // The half's four warps agree.  After a wait that gave up all that follow do at once, and
+      // what the CTA has still to give is NaN.
+      if (any_of_half(half, !go))
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) x[c] = NAN;
       if ((MODE == STATS || MODE == GRAD) && narrow)
 #pragma unroll
         for (int c = 0; c < kCols; ++c) x[c] *= f.w;
@@ -1419,7 +1429,9 @@ struct Backward {
 };
 
 template <int MODE>
-int launch(const Args& p, cudaStream_t st) {
+int launch(Args& p, cudaStream_t st) {
+  p.wait_ns = wait_limit;
+  p.stalled = stalled_pair;
   if (int rc = ensure_smem_attr((const void*)gemm_kernel<MODE>, kSmem)) return rc;
   return launch_after(gemm_kernel<MODE>, dim3(2 * p.pairs), kThreads, kSmem, st, p);
 }
@@ -1706,4 +1718,11 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   }
   if (!dh) return CB_OK;
   return finish(h_dtype, f.acc, f.h_slots, up(N, kTileM), s, N, f.rows, f.top, nullptr, f.wide, dh, st);
+}
+
+extern "C" int cb_linear_ce_set_wait_limit(uint64_t limit_ns, int32_t stall_pair) {
+  if (stall_pair < 0) return CB_ERR_ARG;
+  wait_limit = limit_ns ? limit_ns : kWaitNs;
+  stalled_pair = stall_pair - 1;
+  return CB_OK;
 }

@@ -35,7 +35,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     none.  ``reduction`` "mean" is over the rows that have a target (0 where none has).
     Both results are differentiable: ``r.loss + z * r.lse.square().mean()`` is a loss too.
     ``status`` (int32 [1] on the device) receives 6 when a target is outside the
-    vocabulary, which then counts as none, and 8 when a bounded wait in a kernel gave up.
+    vocabulary, which then counts as none, and 8 when a bounded wait in a kernel gave up,
+    which also makes the results that it would have gone into NaN.
     Runs on the current stream."""
     if (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
         return CrossEntropy(*_LinearCE.apply(hidden, weight, targets, reduction, status))

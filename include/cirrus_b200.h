@@ -548,8 +548,8 @@ int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const void* g, in
  * count [1].  h and w have one type, or h is CB_F32 and w CB_BF16.  16-bit products are
  * exact and float32 ones carried in about 22 bits, both summed in float32.
  * Scratch, 256-byte aligned: cb_linear_ce_scratch_bytes of the same arguments, for the
- * gradient with 1 for dh + 2 for dw in `gradients`, and dw.  *status also receives CB_ERR_TIMEOUT when a bounded
- * wait in a kernel gave up.
+ * gradient with 1 for dh + 2 for dw in `gradients`, and dw.  When a bounded wait in a kernel gave up, *status
+ * receives CB_ERR_TIMEOUT and the results that it would have gone into are NaN.
  * Replaces lm_head + the loss of CirrusModel.forward (cirrus/model/model.py:176-228). */
 size_t cb_linear_ce_scratch_bytes(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype, int64_t ldw,
                                   int32_t N, int32_t V, int32_t d, const void* dw, int32_t gradients);
@@ -573,6 +573,11 @@ int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, const void* w
                       const float* lse, const int32_t* count, const float* g_loss, int64_t g_loss_step,
                       const float* g_lse, int64_t g_lse_step, void* dh, void* dw, void* scratch, size_t scratch_bytes,
                       int32_t* status, void* stream);
+
+/* Limit of the bounded waits of cb_linear_ce's and cb_linear_ce_grad's later launches in this
+ * process (0 = the default, 2 s).  stall_pair > 0: that pair of CTAs, from 1, brings nothing
+ * in, so that every wait for it runs out (fault injection for tests; 0 = off). */
+int cb_linear_ce_set_wait_limit(uint64_t limit_ns, int32_t stall_pair);
 
 /* Copy the workspace's device status word into *status (synchronises on the stream). */
 int cb_read_status(const void* workspace, int32_t* status, void* stream);
