@@ -27,7 +27,7 @@ from cirrus_s_1a_b200._lib import (CB_LAYER_GDN, CB_LAYER_SWA, CB_MAX_T, CB_PREF
                                    CbMatrix, CbModel,
                                    CbMtp, CbSliced)
 from cirrus_s_1a_b200.kv8 import Kv8Cache
-from cirrus_s_1a_b200.loss import CrossEntropy, linear_cross_entropy
+from cirrus_s_1a_b200.loss import CrossEntropy, check_call, linear_cross_entropy
 from cirrus_s_1a_b200.norm import rms_norm
 
 
@@ -636,10 +636,13 @@ class CirrusB200:
         if targets.shape != input_ids.shape:
             raise ValueError(f"targets must be {tuple(input_ids.shape)}, one for each input token")
         with torch.cuda.device(self.device):
+            # (what may be refused is, before the cache takes the tokens)
+            t = targets.to(self.device, non_blocking=True).reshape(-1).contiguous()
+            check_call(t, reduction, status, self.device)
+            head = self.dense_head()
             out = self._forward(input_ids, cache, cache is not None, None, False)
             h = rms_norm(out.hidden.flatten(0, 1), self.model.final_norm, self.cfg.norm_eps)
-            t = targets.to(self.device, non_blocking=True).reshape(-1).contiguous()
-            r = linear_cross_entropy(h, self.dense_head(), t, reduction, status)
+            r = linear_cross_entropy(h, head, t, reduction, status)
         loss = r.loss.view(targets.shape) if reduction == "none" else r.loss
         return CrossEntropy(loss, r.lse.view(targets.shape))
 

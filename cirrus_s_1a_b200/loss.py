@@ -43,8 +43,16 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     return CrossEntropy(*_forward(hidden, weight, targets, reduction, status)[:2])
 
 
-def _arguments(hidden, weight, targets, reduction) -> tuple:
-    """The leading arguments of both entry points."""
+def check_call(targets, reduction, status, device) -> tuple:
+    """(1 for int64 targets, the reduction's code, the status word's address), or ValueError."""
+    code = REDUCTIONS.get(reduction)
+    if code is None:
+        raise ValueError(f"unknown reduction {reduction!r}; choose from {sorted(REDUCTIONS)}")
+    return _rows.ids(targets, "targets", device), code, _rows.status(status, device)
+
+
+def _arguments(hidden, weight, targets, reduction, status) -> tuple:
+    """The leading arguments of both entry points, and the status word's address."""
     N, D, ldh, h_code = _rows.matrix(hidden, "hidden")
     dev = hidden.device
     V, Dw, ldw, w_code = _rows.vocabulary(weight, "weight", dev)
@@ -55,18 +63,14 @@ def _arguments(hidden, weight, targets, reduction) -> tuple:
                          f"{weight.dtype}")
     if targets.shape != (N,):
         raise ValueError(f"targets must be [{N}]")
-    wide = _rows.ids(targets, "targets", dev)
-    code = REDUCTIONS.get(reduction)
-    if code is None:
-        raise ValueError(f"unknown reduction {reduction!r}; choose from {sorted(REDUCTIONS)}")
-    return hidden.data_ptr(), h_code, ldh, weight.data_ptr(), w_code, ldw, N, V, D, targets.data_ptr(), wide, code
+    wide, code, flag = check_call(targets, reduction, status, dev)
+    return (hidden.data_ptr(), h_code, ldh, weight.data_ptr(), w_code, ldw, N, V, D, targets.data_ptr(), wide, code), flag
 
 
 def _forward(hidden, weight, targets, reduction, status) -> tuple:
     """(loss, lse, count)"""
-    args = _arguments(hidden, weight, targets, reduction)
+    args, flag = _arguments(hidden, weight, targets, reduction, status)
     dev, N = hidden.device, args[6]
-    flag = _rows.status(status, dev)
     lse = torch.empty(N, dtype=torch.float32, device=dev)
     if N == 0:
         return torch.zeros(() if reduction != "none" else 0, device=dev), lse, None
@@ -103,7 +107,7 @@ class _LinearCE(torch.autograd.Function):
         if g_loss is None and g_lse is None:
             return None, None, None, None, None
         # of the tensors as they come back: hooks may have moved them in between
-        args = _arguments(hidden, weight, targets, ctx.reduction)
+        args, flag = _arguments(hidden, weight, targets, ctx.reduction, ctx.status)
         dev, (N, V, D) = hidden.device, args[6:9]
         dh = torch.empty(N, D, dtype=hidden.dtype, device=dev) if want_h else None
         if N == 0:
@@ -112,7 +116,7 @@ class _LinearCE(torch.autograd.Function):
         scratch = _scratch(dev, args, dw, want_h + 2 * want_w)
         _rows.call(dev, "cb_linear_ce_grad", *args, lse.data_ptr(), _lib.ptr(count), _lib.ptr(g_loss), _step(g_loss),
                    _lib.ptr(g_lse), _step(g_lse), _lib.ptr(dh), _lib.ptr(dw), scratch.data_ptr(), scratch.numel(),
-                   _lib.ptr(ctx.status))
+                   flag)
         return dh, dw, None, None, None
 
 

@@ -1,0 +1,30 @@
+"""Calls of the operators at the ends of a model that are refused, and what they leave as it was."""
+
+import pytest
+import torch
+
+from test_gpu_ends import DEV, engine
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kv8", [None, "e4m3"])
+@pytest.mark.parametrize("T", [5, 150])
+def test_a_refused_loss_leaves_the_cache(kv8, T):
+    cfg, eng = engine()
+    ids = torch.randint(0, cfg.vocab_size, (2, T + 1), generator=torch.Generator().manual_seed(T))
+    x, targets = ids[:, :T], ids[:, 1:]
+    kw = dict(max_ctx=256, kv8=kv8) if kv8 else {}
+    cache, clean = eng.new_cache(2, **kw), eng.new_cache(2, **kw)
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for kwargs in (dict(targets=targets, reduction="median"), dict(targets=targets.short()), dict(targets=targets.float()),
+                   dict(targets=targets, status=torch.zeros(2, dtype=torch.int32, device=DEV)),
+                   dict(targets=targets, status=word.long()), dict(targets=targets, status=word.cpu()),
+                   dict(targets=targets[:1])):
+        with pytest.raises(ValueError):
+            eng.loss(x, cache=cache, **kwargs)
+    with pytest.raises(ValueError):
+        eng.loss(x.repeat(2, 1), targets.repeat(2, 1), cache)
+    assert cache.pos == 0 and cache.pos_dev.tolist() == [0, 0]
+    assert torch.equal(eng.loss(x, targets, cache).lse, eng.loss(x, targets, clean).lse)
+    assert cache.pos == clean.pos == T
