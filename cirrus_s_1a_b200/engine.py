@@ -617,6 +617,8 @@ class CirrusB200:
         else float32."""
         if self._head is None:
             V, d = self.cfg.vocab_size, self.cfg.d_model
+            if torch.cuda.is_current_stream_capturing():
+                raise _lib.CbError("call dense_head() before a loss is captured")
             with torch.cuda.device(self.device):
                 ids = torch.arange(V, device=self.device)
                 w = torch.empty(V, d, dtype=torch.float32, device=self.device)

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from cirrus_s_1a_b200 import _lib
 from test_gpu_ends import DEV, engine
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +29,22 @@ def test_a_refused_loss_leaves_the_cache(kv8, T):
     assert cache.pos == 0 and cache.pos_dev.tolist() == [0, 0]
     assert torch.equal(eng.loss(x, targets, cache).lse, eng.loss(x, targets, clean).lse)
     assert cache.pos == clean.pos == T
+
+
+def test_a_captured_loss_wants_the_head_first():
+    cfg, eng = engine()
+    ids = torch.randint(0, cfg.vocab_size, (1, 6), device=DEV)
+    cache = eng.new_cache(1)
+    x, targets = ids[:, :5].contiguous(), ids[:, 1:].contiguous()
+    eng(x, cache=cache.clone())  # the workspace
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(_lib.CbError):
+            eng.loss(x, targets, cache)
+    assert cache.pos == 0 and cache.pos_dev.tolist() == [0]
+    eng.dense_head()
+    want = eng.loss(x, targets, cache.clone(), "none")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = eng.loss(x, targets, cache, "none")
+    graph.replay()
+    assert torch.equal(got.loss, want.loss) and torch.equal(got.lse, want.lse)
