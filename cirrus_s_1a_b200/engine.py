@@ -525,6 +525,12 @@ class CirrusB200:
         _lib.check(_lib.lib().cb_read_status(ws.data_ptr(), C.byref(out), _stream_ptr(self.device)), "status")
         return int(out.value)
 
+    def _status_word(self, cache: DeviceCache, T: int) -> torch.Tensor:
+        """The word that a forward of ``T`` tokens has just used, int32 [1]."""
+        ws = (self.workspace(cache.batch, T, cache.max_ctx) if cache.kv8 is None
+              else cache.kv8.workspaces[min(T, CB_PREFILL_CHUNK)])
+        return ws[:4].view(torch.int32)
+
     def phase_trace(self, cache: DeviceCache, T: int = 1) -> list:
         """Per-phase timing of the last persistent launch on this cache's workspace:
         a list of (phase index, CTA-0 work us, barrier wait us) from %globaltimer stamps."""
@@ -634,7 +640,9 @@ class CirrusB200:
         """Cross entropy of ``targets`` [B, T], the token that follows each of ``input_ids``
         (negative: none), behind what ``cache`` holds, from the hidden states alone: the
         logits are not kept (``linear_cross_entropy`` over the final norm's output and
-        ``dense_head``).  ``loss`` is [B, T] with reduction "none", ``lse`` always."""
+        ``dense_head``).  ``loss`` is [B, T] with reduction "none", ``lse`` always.  Without
+        ``status`` a target outside the vocabulary and a wait that gave up are noted where the
+        forward's errors are (``read_status`` of the cache and T)."""
         if targets.shape != input_ids.shape:
             raise ValueError(f"targets must be {tuple(input_ids.shape)}, one for each input token")
         with torch.cuda.device(self.device):
@@ -642,7 +650,9 @@ class CirrusB200:
             t = targets.to(self.device, non_blocking=True).reshape(-1).contiguous()
             check_call(t, reduction, status, self.device)
             head = self.dense_head()
-            out = self._forward(input_ids, cache, cache is not None, None, False)
+            out = self._forward(input_ids, cache, True, None, False)
+            if status is None:
+                status = self._status_word(out.cache, input_ids.shape[1])
             h = rms_norm(out.hidden.flatten(0, 1), self.model.final_norm, self.cfg.norm_eps)
             r = linear_cross_entropy(h, head, t, reduction, status)
         loss = r.loss.view(targets.shape) if reduction == "none" else r.loss

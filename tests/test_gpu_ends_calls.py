@@ -48,3 +48,28 @@ def test_a_captured_loss_wants_the_head_first():
         got = eng.loss(x, targets, cache, "none")
     graph.replay()
     assert torch.equal(got.loss, want.loss) and torch.equal(got.lse, want.lse)
+
+
+@pytest.mark.parametrize("kv8", [None, "e4m3"])
+@pytest.mark.parametrize("T", [5, 150])
+def test_a_loss_notes_targets_outside_where_the_forward_notes_tokens(kv8, T):
+    cfg, eng = engine()
+    ids = torch.randint(0, cfg.vocab_size, (2, T + 1), generator=torch.Generator().manual_seed(T))
+    x, targets = ids[:, :T], ids[:, 1:].clone()
+    make = lambda: eng.new_cache(2, **(dict(max_ctx=256, kv8=kv8) if kv8 else {}))  # noqa: E731
+    targets[1, 2] = -1
+    cache = make()
+    want = eng.loss(x, targets, cache, "none")
+    assert eng.read_status(cache, T) == 0
+    targets[1, 2] = cfg.vocab_size
+    cache = make()
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert torch.equal(eng.loss(x, targets, cache.clone(), "none", word).loss, want.loss)
+    assert int(word) == 6 and eng.read_status(cache, T) == 0  # the word that is given is the one that is used
+    assert torch.equal(eng.loss(x, targets, cache, "none").loss, want.loss)
+    assert eng.read_status(cache, T) == 6
+    eng.clear_status(cache, T)
+    assert eng.read_status(cache, T) == 0
+    if not kv8:  # without a cache: that of any cache of this size
+        eng.loss(x, targets)
+        assert eng.read_status(eng.new_cache(2), T) == 6
