@@ -4,6 +4,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from cirrus_s_1a_b200 import _lib
 from cirrus_s_1a_b200.kv8 import DTYPES, current_device, raw_stream
@@ -63,10 +64,23 @@ def status(t: torch.Tensor | None, device) -> int | None:
     return t.data_ptr()
 
 
-def once() -> None:
-    """Called in a backward pass: what it returns has no gradient of its own."""
+def wants_grad(*tensors) -> bool:
+    """Whether results are to have a gradient; derivatives in forward mode are refused."""
+    no_tangent(*tensors)
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+def no_tangent(*tensors) -> None:
+    for t in tensors:
+        if t is not None and unpack_dual(t).tangent is not None:
+            raise RuntimeError("this operator has no derivative in forward mode")
+
+
+def once(*grads) -> None:
+    """Called in a backward pass: what it returns has no derivative of its own."""
     if torch.is_grad_enabled():  # only under create_graph
         raise RuntimeError("the gradient of this operator is not differentiable (create_graph=True)")
+    no_tangent(*grads)
 
 
 _fns: dict = {}

@@ -24,7 +24,7 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     when an id is outside the table, which then counts as negative.  The table's gradient
     has its type, with sums in float32 in the order of the tokens.  Runs on the current
     stream."""
-    if table.requires_grad and torch.is_grad_enabled():
+    if _rows.wants_grad(table):
         return _Embedding.apply(ids, table, float(scale), status)
     return _lookup(ids, table, float(scale), status)
 
@@ -51,7 +51,7 @@ class _Embedding(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        _rows.once()
+        _rows.once(g)
         ids, = ctx.saved_tensors
         scale, (V, D), dtype = ctx.args
         n, dev = ids.numel(), ids.device

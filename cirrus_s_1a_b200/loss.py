@@ -38,7 +38,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     vocabulary, which then counts as none, and 8 when a bounded wait in a kernel gave up,
     which also makes the results that it would have gone into NaN.
     Runs on the current stream."""
-    if (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
+    if _rows.wants_grad(hidden, weight):
         return CrossEntropy(*_LinearCE.apply(hidden, weight, targets, reduction, status))
     return CrossEntropy(*_forward(hidden, weight, targets, reduction, status)[:2])
 
@@ -101,7 +101,7 @@ class _LinearCE(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_loss, g_lse):
-        _rows.once()
+        _rows.once(g_loss, g_lse)
         hidden, weight, targets, lse, count = ctx.saved_tensors
         want_h, want_w = ctx.needs_input_grad[:2]
         if g_loss is None and g_lse is None:

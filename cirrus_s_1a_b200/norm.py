@@ -18,7 +18,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.
     """``x * rsqrt(mean(x^2) + eps) * weight`` for the rows of ``x`` [rows, d] (float32,
     bfloat16 or float16, rows at any distance) and ``weight`` [d] (float32 or x's type),
     in x's type; gradients in x's and the weight's.  Runs on the current stream."""
-    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
+    if _rows.wants_grad(x, weight):
         return _RMSNorm.apply(x, weight, float(eps))
     return _norm(x, weight, float(eps))
 
@@ -50,7 +50,7 @@ class _RMSNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        _rows.once()
+        _rows.once(g)
         x, weight = ctx.saved_tensors
         # of the tensors as they come back: hooks may have moved them in between
         R, D, ld, code, w_code = _arguments(x, weight)

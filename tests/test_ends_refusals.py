@@ -1,5 +1,10 @@
 """CPU tests of what the operators at the ends of a model refuse, beside ``test_ends_host``."""
 
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
+from cirrus_s_1a_b200 import _rows
 from test_host import built_lib  # noqa: F401
 
 
@@ -7,3 +12,21 @@ def test_wait_limit_refuses_a_negative_pair(built_lib):  # noqa: F811
     L = built_lib
     assert L.cb_linear_ce_set_wait_limit(0, -1) == 1 and L.cb_linear_ce_set_wait_limit(1000, 3) == 0
     assert L.cb_linear_ce_set_wait_limit(0, 0) == 0
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost: no autograd function is entered where nothing requires grad."""
+    from cirrus_s_1a_b200.embedding import embedding
+    from cirrus_s_1a_b200.loss import linear_cross_entropy
+    from cirrus_s_1a_b200.norm import rms_norm
+
+    x, t, w = torch.ones(4, 8), torch.zeros(4, dtype=torch.int64), torch.ones(8)
+    with fw.dual_level():
+        dual, dual_w = fw.make_dual(x, torch.ones(4, 8)), fw.make_dual(w, torch.ones(8))
+        for call in (lambda: embedding(t, dual), lambda: rms_norm(dual, w), lambda: rms_norm(x, dual_w),
+                     lambda: linear_cross_entropy(dual, x, t), lambda: linear_cross_entropy(x, dual, t)):
+            with pytest.raises(RuntimeError, match="forward mode"):
+                call()
+    with pytest.raises(RuntimeError, match="forward mode"):
+        torch.func.jvp(lambda a: rms_norm(a, w), (x,), (x,))
+    assert _rows.wants_grad(x) is False and _rows.wants_grad(x, w.requires_grad_()) is True

@@ -2,9 +2,10 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from cirrus_s_1a_b200 import _lib
-from test_gpu_ends import DEV, engine
+from test_gpu_ends import DEV, engine, ours
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +74,19 @@ def test_a_loss_notes_targets_outside_where_the_forward_notes_tokens(kv8, T):
     if not kv8:  # without a cache: that of any cache of this size
         eng.loss(x, targets)
         assert eng.read_status(eng.new_cache(2), T) == 6
+
+
+def test_forward_mode_is_refused_on_the_device_and_of_gradients_from_above():
+    embed, rms, ce = ours()
+    table = torch.randn(20, 16, device=DEV)
+    norm = torch.ones(16, device=DEV)
+    ids = torch.arange(10, device=DEV)
+    calls = (lambda x: embed(ids, x), lambda x: rms(x, norm), lambda x: ce(x, table, torch.arange(20, device=DEV)))
+    for call in calls:
+        with fw.dual_level():
+            with pytest.raises(RuntimeError):
+                call(fw.make_dual(table, torch.ones_like(table)))
+            x = table.clone().requires_grad_()
+            y = call(x)
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(y, x, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
