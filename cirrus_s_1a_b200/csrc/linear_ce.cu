@@ -1206,9 +1206,10 @@ bool too_large(int32_t N, int32_t V, int32_t d) {
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// Whether a 16-bit matrix can be copied by TMA where it lies.
-bool direct(const void* x, int32_t dtype, int64_t ld, int64_t rows) {
-  return dtype != CB_F32 && aligned_to(x, 16) && (rows == 1 || (ld % 8 == 0 && ld > 0));
+// Whether a 16-bit matrix can be copied by TMA where it lies: a tensor map's rows are aligned
+// and do not overlap.
+bool direct(const void* x, int32_t dtype, int64_t ld, int64_t rows, int d) {
+  return dtype != CB_F32 && aligned_to(x, 16) && (rows == 1 || (ld % 8 == 0 && ld >= d));
 }
 
 // Whether TMA can write contiguous rows of d columns there.
@@ -1334,7 +1335,7 @@ struct Shape {
     return g.passes[tried];
   }
   // whether W is read where it lies
-  bool reads_w(const void* w, int32_t w_dtype, int64_t ldw) const { return !tried && direct(w, w_dtype, ldw, V); }
+  bool reads_w(const void* w, int32_t w_dtype, int64_t ldw) const { return !tried && direct(w, w_dtype, ldw, V, d); }
   int da() const { return (int)up(d, 4); }  // columns of a float32 result
 };
 
@@ -1537,7 +1538,7 @@ extern "C" size_t cb_linear_ce_scratch_bytes(const void* h, int32_t h_dtype, int
   Layout a{nullptr};
   const bool w_direct = s.reads_w(w, w_dtype, ldw);
   if (!gradients) {
-    Forward f(a, s, direct(h, h_dtype, ldh, N), w_direct);
+    Forward f(a, s, direct(h, h_dtype, ldh, N, d), w_direct);
   } else {
     Backward f(a, s, w_direct, gradients & 1, gradients & 2, tma_rows(dw, w_dtype, d));
   }
@@ -1555,7 +1556,7 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   cudaStream_t st = (cudaStream_t)stream;
   const Shape s(h_dtype, w_dtype, N, V, d);
   Layout a{static_cast<char*>(scratch)};
-  const Forward f(a, s, direct(h, h_dtype, ldh, N), s.reads_w(w, w_dtype, ldw));
+  const Forward f(a, s, direct(h, h_dtype, ldh, N, d), s.reads_w(w, w_dtype, ldw));
   if (scratch_bytes < a.used) return CB_ERR_WORKSPACE;
   const Source hs{h, ldh, N, nullptr, f.h, nullptr, SCALE_ROW, f.unit, 1}, ws{w, ldw, V, nullptr, f.w};
   if (s.tried && cudaMemsetAsync(f.wide, 0, sizeof(uint32_t), st) != cudaSuccess) return CB_ERR_CUDA;

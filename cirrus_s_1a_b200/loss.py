@@ -86,7 +86,7 @@ def _scratch(dev, args, dw, gradients) -> torch.Tensor:
     h, h_code, ldh, w, w_code, ldw, N, V, D = args[:9]
     at = None if dw is None else dw.data_ptr()
     # what the size goes by, beside the shape: which matrices can be read and written where they lie
-    key = (h_code, w_code, N, V, D, ldh % 8, ldh > 0, ldw % 8, h % 16, w % 16, (at or 0) % 16, gradients)
+    key = (h_code, w_code, N, V, D, ldh % 8, ldh >= D, ldw % 8, h % 16, w % 16, (at or 0) % 16, gradients)
     return _rows.scratch(dev, "cb_linear_ce_scratch_bytes", key, *args[:9], at, gradients)
 
 

@@ -6,6 +6,7 @@ import torch.autograd.forward_ad as fw
 
 from cirrus_s_1a_b200 import _lib
 from test_gpu_ends import DEV, engine, ours
+from test_gpu_linear_ce import PAIRS, TYPES, check, inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +91,16 @@ def test_forward_mode_is_refused_on_the_device_and_of_gradients_from_above():
             y = call(x)
             with pytest.raises(RuntimeError):
                 torch.autograd.grad(y, x, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.parametrize("pair", PAIRS)
+@pytest.mark.parametrize("N,V,d", [(5, 300, 64), (200, 515, 72), (300, 90, 33)])
+@pytest.mark.parametrize("step", [8, 16, 24, 1])
+def test_hidden_rows_that_overlap(pair, N, V, d, step):
+    """Rows closer together than they are long, as ``unfold`` gives."""
+    _, w, t = inputs(N, V, d, pair, seed=N + step)
+    line = torch.randn(N * step + d, generator=torch.Generator().manual_seed(step)).to(TYPES[pair[0]])
+    h = line.unfold(0, d, step)[:N]
+    hd = line.to(DEV).unfold(0, d, step)[:N]
+    assert hd.stride() == (step, 1)
+    check(h, w, t, dev=(hd, w.to(DEV)))
