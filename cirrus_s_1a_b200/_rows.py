@@ -83,6 +83,13 @@ def once(*grads) -> None:
     no_tangent(*grads)
 
 
+def given(t: torch.Tensor | None, name: str, shape: tuple, dtype, device) -> None:
+    """What a backward pass is handed or has kept has to be what goes with its other tensors:
+    hooks on saved tensors may have given back another."""
+    if t is not None and (t.shape != shape or t.dtype != dtype or t.device != device):
+        raise ValueError(f"{name} must be {dtype} {list(shape)} on {device}, not {t.dtype} {list(t.shape)} on {t.device}")
+
+
 _fns: dict = {}
 _sizes: dict = {}
 

@@ -54,7 +54,7 @@ class _Embedding(torch.autograd.Function):
         _rows.once(g)
         ids, = ctx.saved_tensors
         scale, (V, D), dtype = ctx.args
-        n, dev = ids.numel(), ids.device
+        n, dev = ids.numel(), g.device
         wide = _rows.ids(ids, "ids", dev)
         if n == 0:
             return None, torch.zeros(V, D, dtype=dtype, device=dev), None, None

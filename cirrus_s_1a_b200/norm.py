@@ -55,6 +55,7 @@ class _RMSNorm(torch.autograd.Function):
         # of the tensors as they come back: hooks may have moved them in between
         R, D, ld, code, w_code = _arguments(x, weight)
         dev = x.device
+        _rows.given(g, "the result's gradient", (R, D), x.dtype, dev)
         if R == 0:
             return torch.zeros_like(x), torch.zeros_like(weight), None
         g, ldg = _rows.upstream(g, D)

@@ -5,6 +5,7 @@ import torch
 import torch.autograd.forward_ad as fw
 
 from cirrus_s_1a_b200 import _lib
+from cirrus_s_1a_b200.loss import linear_cross_entropy
 from test_gpu_ends import DEV, engine, ours
 from test_gpu_linear_ce import PAIRS, TYPES, check, inputs
 
@@ -104,3 +105,32 @@ def test_hidden_rows_that_overlap(pair, N, V, d, step):
     hd = line.to(DEV).unfold(0, d, step)[:N]
     assert hd.stride() == (step, 1)
     check(h, w, t, dev=(hd, w.to(DEV)))
+
+
+def test_saved_tensors_that_come_back_changed():
+    """A hook that gives back another device's, type's or length's tensor: refused before a kernel
+    reads it as what was saved."""
+    embed, rms, _ = ours()
+    table = torch.randn(20, 16, device=DEV)
+    norm = torch.ones(16, device=DEV)
+    ids = torch.arange(10, device=DEV)
+    t = torch.arange(20, device=DEV)
+    calls = {"embed": (1, lambda x: embed(ids + 0, x)), "norm": (2, lambda x: rms(x, norm + 0)),
+             "mean": (5, lambda x: linear_cross_entropy(x, table + 0, t + 0).loss),
+             "none": (4, lambda x: linear_cross_entropy(x, table + 0, t + 0, "none").loss)}
+    for name, (saved, call) in calls.items():
+        for which in range(saved):
+            for change in (lambda x: x.cpu(), lambda x: x.to(torch.float16), lambda x: x[:-1]):
+                seen = []
+
+                def unpack(x):
+                    seen.append(x)
+                    return change(x) if len(seen) == which + 1 else x
+
+                x = table.clone().requires_grad_()
+                with torch.autograd.graph.saved_tensors_hooks(lambda x: x, unpack):
+                    y = call(x)
+                with pytest.raises((ValueError, RuntimeError)):
+                    torch.autograd.grad(y, x, torch.ones_like(y))
+                assert len(seen) == saved, name
+    torch.cuda.synchronize()
