@@ -18,6 +18,7 @@
 // Measured, 131072 tokens, 32768 x 1024 in float32: lookup 104 us (5.9 TB/s), sort 30, sums
 // 110 (5.3 TB/s), join 26; 16384 tokens, 32000 x 768 in bf16: 11, 14, 20 and 7.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "ends.cuh"
@@ -439,7 +440,8 @@ using namespace cb;
 
 extern "C" int cb_embedding(const void* table, int32_t dtype, int64_t ld, int32_t V, int32_t d, const void* ids,
                             int32_t ids_64, int64_t n, float scale, void* out, int32_t* status, void* stream) {
-  if (!table || !ids || !out || V <= 0 || d <= 0 || n <= 0 || (V > 1 && ld < d) || !is_dtype(dtype)) return CB_ERR_ARG;
+  if (!table || !ids || !out || V <= 0 || d <= 0 || n <= 0 || (V > 1 && ld < d) || !is_dtype(dtype) || !std::isfinite(scale))
+    return CB_ERR_ARG;
   const int size = dtype_size(dtype);
   if (!aligned_to(table, size) || !aligned_to(out, size) || !aligned_to(ids, ids_64 ? 8 : 4)) return CB_ERR_ARG;
   if (n > CB_ENDS_MAX_ROWS || V > CB_ENDS_MAX_VOCAB || d > CB_ENDS_MAX_DIM) return CB_ERR_SHAPE;
@@ -464,7 +466,9 @@ extern "C" size_t cb_embedding_grad_scratch_bytes(int64_t n, int32_t V, int32_t 
 extern "C" int cb_embedding_grad(const void* g, int32_t dtype, int64_t ldg, const void* ids, int32_t ids_64, int64_t n,
                                  int32_t V, int32_t d, float scale, void* dtable, void* scratch, size_t scratch_bytes,
                                  void* stream) {
-  if (!g || !ids || !dtable || !scratch || V <= 0 || d <= 0 || n <= 0 || ldg < 0 || !is_dtype(dtype)) return CB_ERR_ARG;
+  if (!g || !ids || !dtable || !scratch || V <= 0 || d <= 0 || n <= 0 || ldg < 0 || !is_dtype(dtype) ||
+      !std::isfinite(scale))
+    return CB_ERR_ARG;
   const int size = dtype_size(dtype);
   if (!aligned_to(g, size) || !aligned_to(dtable, size) || !aligned_to(ids, ids_64 ? 8 : 4) || !aligned_to(scratch, 16))
     return CB_ERR_ARG;

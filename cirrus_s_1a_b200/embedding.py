@@ -10,6 +10,8 @@ tied to its head.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from cirrus_s_1a_b200 import _rows
@@ -19,11 +21,13 @@ from cirrus_s_1a_b200.kv8 import DTYPES
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
               status: torch.Tensor | None = None) -> torch.Tensor:
     """``scale * table[ids]`` for ``table`` [V, d] (float32, bfloat16 or float16; rows at
-    least d apart) and contiguous int64 or int32 ``ids`` of any shape; a negative id gives
-    a zero row and no gradient.  ``status`` (int32 [1] on the table's device) receives 6
-    when an id is outside the table, which then counts as negative.  The table's gradient
-    has its type, with sums in float32 in the order of the tokens.  Runs on the current
-    stream."""
+    least d apart), a finite ``scale`` and contiguous int64 or int32 ``ids`` of any shape; a
+    negative id gives a zero row and no gradient.  ``status`` (int32 [1] on the table's
+    device) receives 6 when an id is outside the table, which then counts as negative.  The
+    table's gradient has its type, with sums in float32 in the order of the tokens.  Runs on
+    the current stream."""
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, not {scale}")
     if _rows.wants_grad(table):
         return _Embedding.apply(ids, table, float(scale), status)
     return _lookup(ids, table, float(scale), status)

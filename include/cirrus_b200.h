@@ -518,7 +518,7 @@ int cb_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int32_t row
 #define CB_ENDS_MAX_DIM 65536
 enum { CB_REDUCE_NONE = 0, CB_REDUCE_MEAN = 1, CB_REDUCE_SUM = 2 };
 
-/* out [n][d] = scale * table[ids[i]], zeros where there is no token.  Replaces nn.Embedding
+/* out [n][d] = scale * table[ids[i]], zeros where there is no token; scale is finite.  Replaces nn.Embedding
  * (cirrus/model/model.py:124) for a dense table; cb_embed reads the NVFP4 one. */
 int cb_embedding(const void* table, int32_t dtype, int64_t ld, int32_t V, int32_t d, const void* ids, int32_t ids_64,
                  int64_t n, float scale, void* out, int32_t* status, void* stream);

@@ -1,5 +1,7 @@
 """CPU tests of what the operators at the ends of a model refuse, beside ``test_ends_host``."""
 
+import math
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
@@ -30,3 +32,17 @@ def test_forward_mode_is_refused():
     with pytest.raises(RuntimeError, match="forward mode"):
         torch.func.jvp(lambda a: rms_norm(a, w), (x,), (x,))
     assert _rows.wants_grad(x) is False and _rows.wants_grad(x, w.requires_grad_()) is True
+
+
+def test_embedding_refuses_a_scale_that_is_not_finite(built_lib):  # noqa: F811
+    """Zero rows of ids without a token would not be zero."""
+    L = built_lib
+    before = L.cb_launch_count()
+    for scale in (math.inf, -math.inf, math.nan, 1e39):
+        assert L.cb_embedding(256, 0, 8, 4, 8, 256, 1, 3, scale, 256, None, None) == 1
+        assert L.cb_embedding_grad(256, 0, 8, 256, 1, 3, 4, 8, scale, 256, 256, 1 << 40, None) == 1
+    assert L.cb_launch_count() == before
+    from cirrus_s_1a_b200.embedding import embedding
+
+    with pytest.raises(ValueError, match="scale"):
+        embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8), math.nan)
