@@ -529,8 +529,9 @@ size_t cb_embedding_grad_scratch_bytes(int64_t n, int32_t V, int32_t d);
 int cb_embedding_grad(const void* g, int32_t dtype, int64_t ldg, const void* ids, int32_t ids_64, int64_t n, int32_t V,
                       int32_t d, float scale, void* dtable, void* scratch, size_t scratch_bytes, void* stream);
 
-/* y [rows][d] = x * rsqrt(mean(x^2) + eps) * w; w [d] float32 or x's type.  (Squares are
- * float32: values past 2^63 give 0 or NaN.)  Replaces RMSNorm
+/* y [rows][d] = x * rsqrt(mean(x^2) + eps) * w; w [d] float32 or x's type.  (A row's squares
+ * are added up in float32: a row whose 2-norm reaches 2^64, which values of 2^64 / sqrt(d) make,
+ * gives zeros or NaN, and in the gradient one whose sum of g w x leaves float32's range.)  Replaces RMSNorm
  * (cirrus/model/layers.py:33-44). */
 int cb_rms_norm(const void* x, int32_t dtype, int64_t ld, const void* w, int32_t w_dtype, int32_t rows, int32_t d,
                 float eps, void* y, void* stream);
