@@ -51,13 +51,16 @@ constexpr int kBoxBytes = 32 * 128;  // a box on its way out: a warp's 32 rows, 
 constexpr int kSmem = 7 * kStageBytes + 1024;
 constexpr int kThreads = kEpiWarps * 32 + 64;
 constexpr int kMaxPasses = 6, kMaxPairs = 128;
-// Sums in tensor memory are cut off, not rounded, after every 16 products: over 48 of them a
-// row's lse was 5e-7 off, over 1500 the gradients 4e-5.  So a span of K is added up there,
-// and the spans in registers, rounded: 1024 of K, or 256 where float32 parts are multiplied.
-// 256 also in the logits of up to 64 16-bit rows, which wait for W (5 rows of 768 columns are 8e-8
-// off instead of 2.4e-7, the plain float32 form 4e-8, in 17.5 us instead of 16.5; 16384 rows would
-// take 610 us instead of 545).
-constexpr int kSpan16 = 16, kSpan32 = 4, kSpan32Rows = 64;
+// Sums in tensor memory are cut off, not rounded, after every 16 products, and each product two
+// bits further down: over 1500 additions of float32 parts the gradients were 4e-5 off.  So a
+// span of K is added up there, and the spans in registers, rounded: 1024 of K, or 256 where float32
+// parts are multiplied.
+// Logits, whose errors nothing averages: 768 of K, of float16, whose products have more bits to
+// be cut, 512.  lse of rows of 1024 is then 5.4e-7 (bf16) and 5.7e-7 (f16) off, in spans of 1024
+// 8.6e-7 and 1.2e-6, the plain float32 form 2.5e-7 and 3.8e-7; 16384 x 32000 x 768 takes 615 us in
+// bf16 (640 in spans of 512) and 661 in f16 (647 in spans of 1024, 715 of 256).  256 for up to 64
+// rows, which wait for W (5 rows of 768 columns in bf16 8e-8 off, 17.5 us; one span 2.4e-7, 16.5).
+constexpr int kSpan16 = 16, kSpan32 = 4, kSpanBf16Logits = 12, kSpanF16Logits = 8, kSpan32Rows = 64;
 constexpr uint64_t kWaitNs = 2000000000ull, kDrainNs = 10000000ull;
 // cb_linear_ce_set_wait_limit's
 std::atomic<uint64_t> wait_limit{kWaitNs};
@@ -1316,7 +1319,7 @@ struct Shape {
   // alike.
   void logit_passes(Gemm& g, bool swapped) const {
     passes(g, h_parts, w_parts, dp, dp);
-    if (N <= kSpan32Rows) g.span[0] = kSpan32;
+    if (h_parts == 1) g.span[0] = N <= kSpan32Rows ? kSpan32 : f16 ? kSpanF16Logits : kSpanBf16Logits;
     g.apart = h_parts > w_parts;
     if (g.apart) std::swap(g.a_part[0][0], g.a_part[0][1]);
     if (swapped) std::swap(g.a_part, g.b_part);

@@ -546,8 +546,9 @@ int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const void* g, in
  * the logits x = h w^T: lse [N] = log sum exp x (natural log), and per row lse - x[target],
  * 0 where there is no target.  loss: that for each row [N] (CB_REDUCE_NONE), or its mean
  * over the rows with a target (0 when none has one) or its sum, [1], with their number in
- * count [1].  h and w have one type, or h is CB_F32 and w CB_BF16.  16-bit products are
- * exact and float32 ones carried in about 22 bits, both summed in float32.
+ * count [1].  h and w have one type, or h is CB_F32 and w CB_BF16.  16-bit products
+ * are added up in float32 (by the tensor cores, which cut off instead of rounding, for up to 768 of
+ * them), float32 ones carried in about 22 bits.
  * Scratch, 256-byte aligned: cb_linear_ce_scratch_bytes of the same arguments, for the
  * gradient with 1 for dh + 2 for dw in `gradients`, and dw.  When a bounded wait in a kernel gave up, *status
  * receives CB_ERR_TIMEOUT and the results that it would have gone into are NaN.
