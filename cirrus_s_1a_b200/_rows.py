@@ -4,7 +4,7 @@
 from __future__ import annotations
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 
 from cirrus_s_1a_b200 import _lib
 from cirrus_s_1a_b200.kv8 import DTYPES, current_device, raw_stream
@@ -64,15 +64,17 @@ def status(t: torch.Tensor | None, device) -> int | None:
     return t.data_ptr()
 
 
-def wants_grad(*tensors) -> bool:
+def wants_grad(a: torch.Tensor, b: torch.Tensor | None = None) -> bool:
     """Whether results are to have a gradient; derivatives in forward mode are refused."""
-    no_tangent(*tensors)
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    no_tangent(a, b)
+    return (a.requires_grad or (b is not None and b.requires_grad)) and torch.is_grad_enabled()
 
 
 def no_tangent(*tensors) -> None:
+    if forward_ad._current_level < 0:  # outside of any dual level (0.4 us less a tensor than asking it)
+        return
     for t in tensors:
-        if t is not None and unpack_dual(t).tangent is not None:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError("this operator has no derivative in forward mode")
 
 
