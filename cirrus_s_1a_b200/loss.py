@@ -95,7 +95,7 @@ class _LinearCE(torch.autograd.Function):
     def forward(ctx, hidden, weight, targets, reduction, status):
         loss, lse, count = _forward(hidden, weight, targets, reduction, status)
         ctx.save_for_backward(hidden, weight, targets, lse, count)
-        ctx.reduction, ctx.status, ctx.rows = reduction, status, weight.shape[0]
+        ctx.reduction, ctx.status, ctx.like = reduction, status, (hidden.device, len(lse), weight.shape[0])
         ctx.set_materialize_grads(False)
         return loss, lse
 
@@ -109,12 +109,11 @@ class _LinearCE(torch.autograd.Function):
         # of the tensors as they come back: hooks may have moved them in between
         args, flag = _arguments(hidden, weight, targets, ctx.reduction, ctx.status)
         dev, (N, V, D) = hidden.device, args[6:9]
-        per_row = torch.float32, dev
-        _rows.given(weight, "the saved weight", (ctx.rows, D), weight.dtype, dev)
-        _rows.given(lse, "the saved lse", (N,), *per_row)
+        if (dev, N, V) != ctx.like:  # which the gradients from above go with
+            raise ValueError(f"the saved tensors must be of {ctx.like[1]} rows and {ctx.like[2]} of the vocabulary on "
+                             f"{ctx.like[0]}, not {N} and {V} on {dev}")
+        _rows.given(lse, "the saved lse", (N,), torch.float32, dev)
         _rows.given(count, "the saved number of targets", (1,), torch.int32, dev)
-        _rows.given(g_loss, "the loss's gradient", (N,) if ctx.reduction == "none" else (), *per_row)
-        _rows.given(g_lse, "lse's gradient", (N,), *per_row)
         lse = lse.contiguous()
         dh = torch.empty(N, D, dtype=hidden.dtype, device=dev) if want_h else None
         if N == 0:
