@@ -86,8 +86,8 @@ __device__ __forceinline__ uint32_t at_rank(const void* p, int rank) {
 }
 
 // Tokens [0, n) of the batch by id, those without one (as id V) last: keys and order.
-__global__ void __launch_bounds__(kSortThreads) sort_kernel(Ids ids, int64_t first, int n, int V, int passes, uint32_t* keys,
-                                                            uint32_t* order) {
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(Ids ids, int64_t first, int n, int V, int passes,
+                                                            uint32_t* keys, uint32_t* order) {
   extern __shared__ SortShared sort_shared[];
   SortShared& s = *sort_shared;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(Ids ids, int64_t fir
         order[at] = p.y;
       } else {
         const uint32_t cta = at / per;
-        asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at_rank(in + (at - cta * per), cta)), "r"(p.x), "r"(p.y)
+        asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at_rank(in + (at - cta * per), cta)), "r"(p.x),
+                     "r"(p.y)
                      : "memory");
       }
     }
@@ -217,9 +218,9 @@ __device__ __forceinline__ void write_row(T* dtable, float* total, int64_t at, c
 // part[chunk][which][d]: 0 the sum of the tokens of the row that began before the chunk, 1 of
 // one that begins in it and goes on.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, VEC > 4 ? 2 : 4) sum_kernel(const T* g, int64_t ldg, const uint32_t* keys, const uint32_t* order,
-                                                       int n, int V, int d, int slabs, float scale, T* dtable, float* total,
-                                                       float* part) {
+__global__ void __launch_bounds__(kThreads, VEC > 4 ? 2 : 4)
+    sum_kernel(const T* g, int64_t ldg, const uint32_t* keys, const uint32_t* order, int n, int V, int d, int slabs,
+               float scale, T* dtable, float* total, float* part) {
   const int lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   await_before();
@@ -373,7 +374,9 @@ struct Scratch {
 // elements 82; x 772 54 and 81).
 template <typename T, typename F>
 int with_piece(const void* a, int64_t lda, const void* b, int d, F&& f) {
-  auto fits = [&](int n) { return d % n == 0 && lda % n == 0 && aligned_to(a, n * sizeof(T)) && aligned_to(b, n * sizeof(T)); };
+  auto fits = [&](int n) {
+    return d % n == 0 && lda % n == 0 && aligned_to(a, n * sizeof(T)) && aligned_to(b, n * sizeof(T));
+  };
   if constexpr (sizeof(T) == 2)
     if (fits(8)) return f(std::integral_constant<int, 8>{});
   if (fits(4)) return f(std::integral_constant<int, 4>{});
@@ -413,7 +416,8 @@ int launch_sort(Ids ids, int64_t first, int n, int V, const Scratch& s, cudaStre
 }
 
 template <typename T, int VEC>
-int grad(const T* g, int64_t ldg, Ids ids, int64_t n, int V, int d, float scale, T* dtable, const Scratch& s, cudaStream_t st) {
+int grad(const T* g, int64_t ldg, Ids ids, int64_t n, int V, int d, float scale, T* dtable, const Scratch& s,
+         cudaStream_t st) {
   if (s.total && cudaMemsetAsync(s.total, 0, (size_t)V * d * 4, st) != cudaSuccess) return CB_ERR_CUDA;
   const int slabs = ceil_div(d, 32 * VEC);
   for (int64_t first = 0; first < n; first += kBatch) {
@@ -425,8 +429,8 @@ int grad(const T* g, int64_t ldg, Ids ids, int64_t n, int V, int d, float scale,
                               g + first * ldg, ldg, s.keys, s.order, m, V, d, slabs, scale, dtable, s.total, s.part))
       return rc;
     if (m <= kChunk) continue;
-    if (int rc = launch_after(join_kernel<T, VEC>, dim3((unsigned)((sums + kWarps - 1) / kWarps)), kThreads, 0, st, s.keys, m,
-                              V, d, slabs, scale, dtable, s.total, s.part))
+    if (int rc = launch_after(join_kernel<T, VEC>, dim3((unsigned)((sums + kWarps - 1) / kWarps)), kThreads, 0, st, s.keys,
+                              m, V, d, slabs, scale, dtable, s.total, s.part))
       return rc;
   }
   if (!s.total) return CB_OK;
@@ -440,7 +444,8 @@ using namespace cb;
 
 extern "C" int cb_embedding(const void* table, int32_t dtype, int64_t ld, int32_t V, int32_t d, const void* ids,
                             int32_t ids_64, int64_t n, float scale, void* out, int32_t* status, void* stream) {
-  if (!table || !ids || !out || V <= 0 || d <= 0 || n <= 0 || (V > 1 && ld < d) || !is_dtype(dtype) || !std::isfinite(scale))
+  if (!table || !ids || !out || V <= 0 || d <= 0 || n <= 0 || (V > 1 && ld < d) || !is_dtype(dtype) ||
+      !std::isfinite(scale))
     return CB_ERR_ARG;
   const int size = dtype_size(dtype);
   if (!aligned_to(table, size) || !aligned_to(out, size) || !aligned_to(ids, ids_64 ? 8 : 4)) return CB_ERR_ARG;
@@ -450,8 +455,9 @@ extern "C" int cb_embedding(const void* table, int32_t dtype, int64_t ld, int32_
     auto go = [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
       const int64_t all = n * (d / VEC);
-      return launch_after(embedding_kernel<T, VEC>, dim3((unsigned)((all + kPieces * kThreads - 1) / (kPieces * kThreads))),
-                          kThreads, 0, (cudaStream_t)stream, static_cast<const T*>(table), ld, V, d / VEC, Ids{ids, ids_64},
+      const int64_t ctas = (all + kPieces * kThreads - 1) / (kPieces * kThreads);
+      return launch_after(embedding_kernel<T, VEC>, dim3((unsigned)ctas), kThreads, 0, (cudaStream_t)stream,
+                          static_cast<const T*>(table), ld, V, d / VEC, Ids{ids, ids_64},
                           all, scale, static_cast<T*>(out), status);
     };
     return with_piece<T>(table, V == 1 ? 0 : ld, out, d, go);

@@ -509,7 +509,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         const uint32_t a_step = a_mn ? 2048 / 16 : 2, b_step = MODE == PRODUCTS ? 2048 / 16 : 2;
         const int span = g.span[narrow], passes = g.passes[narrow];
         const int apart = (MODE == STATS || MODE == GRAD) && g.apart && !narrow;
-        for (int from = 0, last = !apart; go && from < it.steps; from += last ? span : 0, last = !apart || !last, ++sums) {
+        for (int from = 0, last = !apart; go && from < it.steps;
+             from += last ? span : 0, last = !apart || !last, ++sums) {
           const int acc = sums & 1, steps = min(span, it.steps - from) * (!apart ? passes : last ? 1 : passes - 1);
           if (sums >= 2) go = __all_sync(0xffffffffu, wait(freed + 8 * acc, (sums / 2 - 1) & 1));
           fence_after();
@@ -677,7 +678,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         if (g.out_f32) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            send(&g.out, v + c * 32, y, it.split ? g.split_mode : g.out_mode, [&](int j) { return __float_as_uint(x[c * 32 + j]); });
+            send(&g.out, v + c * 32, y, it.split ? g.split_mode : g.out_mode,
+                 [&](int j) { return __float_as_uint(x[c * 32 + j]); });
         } else {
 #pragma unroll
           for (int c = 0; c < 2; ++c)
@@ -699,13 +701,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
 #pragma unroll
           for (int j = 0; j < 32; ++j)
             if (b * 32 + (j & 16) < cols)
-              asm volatile("st.shared.f32 [%0], %1;" ::"r"(few_box + (j * 128 + (row ^ j)) * 4), "f"(x[b * 32 + j]) : "memory");
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(few_box + (j * 128 + (row ^ j)) * 4), "f"(x[b * 32 + j])
+                           : "memory");
           half_sync();
           if (few_row[b] < 0) continue;
           float y[32], t = few_m[b];
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y[k]) : "r"(few_box + (lane * 128 + ((quarter * 32 + k) ^ lane)) * 4));
+            asm volatile("ld.shared.f32 %0, [%1];"
+                         : "=f"(y[k])
+                         : "r"(few_box + (lane * 128 + ((quarter * 32 + k) ^ lane)) * 4));
             y[k] = quarter * 32 + k < valid ? y[k] * few_unit[b] : -INFINITY;
           }
 #pragma unroll
@@ -791,9 +796,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
               return u;
             });
           if (f16)
-            send(&p.g[0].out, at_part, y, OUT_STORE, [&](int j) { return pack_f16(x[c * 64 + 2 * j], x[c * 64 + 2 * j + 1]); });
+            send(&p.g[0].out, at_part, y, OUT_STORE,
+                 [&](int j) { return pack_f16(x[c * 64 + 2 * j], x[c * 64 + 2 * j + 1]); });
           else
-            send(&p.g[0].out, at_part, y, OUT_STORE, [&](int j) { return pack_bf16(x[c * 64 + 2 * j], x[c * 64 + 2 * j + 1]); });
+            send(&p.g[0].out, at_part, y, OUT_STORE,
+                 [&](int j) { return pack_bf16(x[c * 64 + 2 * j], x[c * 64 + 2 * j + 1]); });
         }
       }
     }
@@ -802,14 +809,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         half_sync();
-        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(few_box + (quarter * 32 + lane) * 8), "f"(few_m[b]), "f"(few_l[b])
+        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(few_box + (quarter * 32 + lane) * 8), "f"(few_m[b]),
+                     "f"(few_l[b])
                      : "memory");
         half_sync();
         if (quarter == 0 && few_row[b] >= 0) {
           float2 q[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(q[k].x), "=f"(q[k].y) : "r"(few_box + (k * 32 + lane) * 8));
+            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                         : "=f"(q[k].x), "=f"(q[k].y)
+                         : "r"(few_box + (k * 32 + lane) * 8));
           const float t = fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x)), ref = t == -INFINITY ? 0.0f : t;
           float sum = 0.0f;
 #pragma unroll
@@ -820,7 +830,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
-  start_next();  // (at the start it would have small kernels wait beside these CTAs: 33 us instead of 27 for 128 rows of float32)
+  // (at the start it would have small kernels wait beside these CTAs: 33 us instead of 27 for 128 rows of float32)
+  start_next();
   fence_before();
   __syncthreads();
   cluster_sync();  // no CTA leaves while the pair's products or arrivals may reach it
@@ -845,9 +856,9 @@ constexpr int kRowThreads = 256;
 // Joins the runs' parts of a row's sum, LANES threads to a row (32 where few rows are in many
 // parts).  A reduced loss: the CTAs' sums, which the last CTA adds up in order.
 template <int LANES>
-__global__ void __launch_bounds__(kRowThreads) join_kernel(Problem p, int few, int n_tiles, int m_tiles, int pairs, const float2* part,
-                                                           const float* xt, float* rows, float* lse, int reduction,
-                                                           float* loss, int32_t* count, double2* sums, uint32_t* counter,
+__global__ void __launch_bounds__(kRowThreads) join_kernel(Problem p, int few, int n_tiles, int m_tiles, int pairs,
+                                                           const float2* part, const float* xt, float* rows, float* lse,
+                                                           int reduction, float* loss, int32_t* count, double2* sums, uint32_t* counter,
                                                            int32_t* status) {
   __shared__ double s_sum[kRowThreads / 32], s_count[kRowThreads / 32];
   __shared__ int s_last;
@@ -948,8 +959,8 @@ struct Upstream {
 // rows[n] = (a, b, lse, -) as they come from above, and *top = the largest |a| or |b|: one
 // for all rows of a reduced loss; else a maximum (which does not depend on the order it is
 // taken in), *top starting at 0.
-__global__ void __launch_bounds__(kRowThreads) factors_kernel(Problem p, Upstream u, const float* lse, float4* rows, float* top,
-                                                              float* common, uint32_t* wide) {
+__global__ void __launch_bounds__(kRowThreads) factors_kernel(Problem p, Upstream u, const float* lse, float4* rows,
+                                                              float* top, float* common, uint32_t* wide) {
   const int n = blockIdx.x * kRowThreads + threadIdx.x;
   const bool one_top = u.reduction != CB_REDUCE_NONE && !u.lse;
   await_before();
@@ -1004,7 +1015,8 @@ __device__ __forceinline__ Vec<T, 8> load8(const T* row, int j0, int d) {
   if (WIDE) {
     if (j0 < d)
 #pragma unroll
-      for (int k = 0; k < 8; k += 16 / sizeof(T)) *reinterpret_cast<uint4*>(&v.v[k]) = *reinterpret_cast<const uint4*>(row + j0 + k);
+      for (int k = 0; k < 8; k += 16 / sizeof(T))
+        *reinterpret_cast<uint4*>(&v.v[k]) = *reinterpret_cast<const uint4*>(row + j0 + k);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -1185,13 +1197,14 @@ EncodeFn encoder() {
 }
 
 // A matrix of rows `ld` elements apart, in boxes of 128 bytes x box_rows.
-bool map_of(CUtensorMap* map, const void* at, CUtensorMapDataType type, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+bool map_of(CUtensorMap* map, const void* at, CUtensorMapDataType type, int64_t rows, int64_t cols, int64_t ld,
+            int box_rows) {
   const int size = type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(ld * size)};
   const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows}, steps[2] = {1, 1};
-  return encoder() && encoder()(map, type, 2, const_cast<void*>(at), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encoder() && encoder()(map, type, 2, const_cast<void*>(at), dims, strides, box, steps,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 bool bad(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype, int64_t ldw, int32_t N, int32_t V,
@@ -1200,7 +1213,8 @@ bool bad(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_d
   if (h_dtype != w_dtype && !(h_dtype == CB_F32 && w_dtype == CB_BF16)) return true;
   if (ldh < 0 || (V > 1 && ldw < d)) return true;
   if (reduction != CB_REDUCE_NONE && reduction != CB_REDUCE_MEAN && reduction != CB_REDUCE_SUM) return true;
-  return !aligned_to(h, dtype_size(h_dtype)) || !aligned_to(w, dtype_size(w_dtype)) || !aligned_to(targets, targets_64 ? 8 : 4);
+  return !aligned_to(h, dtype_size(h_dtype)) || !aligned_to(w, dtype_size(w_dtype)) ||
+         !aligned_to(targets, targets_64 ? 8 : 4);
 }
 
 bool too_large(int32_t N, int32_t V, int32_t d) {
@@ -1279,7 +1293,8 @@ Deal deal(int pairs, int h_tiles, int h_steps, int h_passes, int w_tiles, int w_
   }
   const int items = w_tiles * o.w, odd = items % pairs, low = items / pairs;
   const double end = end_of(pairs, items, cost(o.w), work).common;
-  const double most = std::max(0.0, end - low * cost(o.w)) / h_passes, less = std::max(0.0, end - (low + 1) * cost(o.w)) / h_passes;
+  const double most = std::max(0.0, end - low * cost(o.w)) / h_passes;
+  const double less = std::max(0.0, end - (low + 1) * cost(o.w)) / h_passes;
   for (int c = 0; c < pairs; ++c) o.from[c] = (int)std::min(steps, c < odd ? c * less : odd * less + (c - odd) * most);
   o.from[pairs] = (int)steps;
   // the most parts that a tile of dh lies in
@@ -1450,7 +1465,8 @@ struct Made {
   Sources p;
   int32_t dtype;
   bool aligned;
-  Made(int32_t dtype_, const Shape& s, const Source& one, const Source& two, const float* top, float* common, uint32_t* wide)
+  Made(int32_t dtype_, const Shape& s, const Source& one, const Source& two, const float* top, float* common,
+       uint32_t* wide)
       : p{{one, two}, s.d, s.dp, top, common, wide}, dtype(dtype_) {
     auto pieces = [&](const Source& x) { return !x.n || (aligned_to(x.x, 16) && x.ld * dtype_size(dtype) % 16 == 0); };
     aligned = s.d % 8 == 0 && pieces(one) && pieces(two);
@@ -1504,8 +1520,8 @@ int make_operands(int32_t h_dtype, int32_t w_dtype, const Shape& s, const Source
   return has_second ? second.whole(st) : (int)CB_OK;
 }
 
-int finish(int32_t dtype, const float* acc, int splits, int64_t split_rows, const Shape& s, int64_t n_rows, const float4* rows,
-           const float* top, const float* common, const uint32_t* wide, void* out, cudaStream_t st) {
+int finish(int32_t dtype, const float* acc, int splits, int64_t split_rows, const Shape& s, int64_t n_rows,
+           const float4* rows, const float* top, const float* common, const uint32_t* wide, void* out, cudaStream_t st) {
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     const bool vecs = s.d % 4 == 0 && aligned_to(out, 4 * sizeof(T));
@@ -1533,7 +1549,8 @@ struct Operand {
 using namespace cb;
 
 extern "C" size_t cb_linear_ce_scratch_bytes(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype,
-                                             int64_t ldw, int32_t N, int32_t V, int32_t d, const void* dw, int32_t gradients) {
+                                             int64_t ldw, int32_t N, int32_t V, int32_t d, const void* dw,
+                                             int32_t gradients) {
   if (N <= 0 || V <= 0 || d <= 0 || too_large(N, V, d) || !is_dtype(h_dtype) || !is_dtype(w_dtype) || gradients < 0 ||
       gradients > 3)
     return 0;
@@ -1601,8 +1618,8 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   if (int rc = f.few ? launch<FEW>(p, st) : launch<STATS>(p, st)) return rc;
   const int lanes = f.lanes();
   return launch_after(lanes == 32 ? join_kernel<32> : join_kernel<4>, dim3(f.join_ctas(N)), kRowThreads, 0, st,
-                      Problem{N, V, d, p.targets}, f.few, f.n_tiles, f.m_tiles, f.pairs, f.part, f.xt, loss, lse, reduction, loss,
-                      count, f.sums, f.counter, status);
+                      Problem{N, V, d, p.targets}, f.few, f.n_tiles, f.m_tiles, f.pairs, f.part, f.xt, loss, lse, reduction,
+                      loss, count, f.sums, f.counter, status);
 }
 
 extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype,
@@ -1622,7 +1639,8 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   if (scratch_bytes < a.used) return CB_ERR_WORKSPACE;
   const Problem pb{N, V, d, Ids{targets, targets_64}};
   const Upstream u{g_loss, g_lse, g_loss_step, g_lse_step, count, reduction};
-  if ((reduction == CB_REDUCE_NONE || g_lse) && cudaMemsetAsync(f.top, 0, sizeof(float), st) != cudaSuccess) return CB_ERR_CUDA;
+  if ((reduction == CB_REDUCE_NONE || g_lse) && cudaMemsetAsync(f.top, 0, sizeof(float), st) != cudaSuccess)
+    return CB_ERR_CUDA;
   if (int rc = launch_after(factors_kernel, dim3(ceil_div(N, kRowThreads)), kRowThreads, 0, st, pb, u, lse, f.rows, f.top,
                             f.common, f.wide))
     return rc;

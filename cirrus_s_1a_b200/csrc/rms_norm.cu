@@ -173,7 +173,8 @@ __global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* part, in
 
 // A CTA to a row that it holds: NV pieces of VEC elements a thread.
 template <typename T, typename W, int VEC, int NV>
-__global__ void __launch_bounds__(kThreads) rms_norm_cta_kernel(const T* x, int64_t ld, const W* w, int d, float eps, T* y) {
+__global__ void __launch_bounds__(kThreads) rms_norm_cta_kernel(const T* x, int64_t ld, const W* w, int d, float eps,
+                                                                T* y) {
   __shared__ float red[33];
   await_before();
   start_next();
@@ -206,8 +207,9 @@ __global__ void __launch_bounds__(kThreads) rms_norm_cta_kernel(const T* x, int6
 // 139 us, 160 with registers for three.  part[cta][d]
 constexpr int row_ctas(int columns) { return columns <= 16 ? 4 : 2; }
 template <typename T, typename W, int VEC, int NV>
-__global__ void __launch_bounds__(kThreads, row_ctas(NV * VEC)) rms_norm_grad_cta_kernel(const T* x, int64_t ld, const T* g, int64_t ldg, const W* w,
-                                                                     int rows, int d, float eps, T* dx, float* part) {
+__global__ void __launch_bounds__(kThreads, row_ctas(NV * VEC))
+    rms_norm_grad_cta_kernel(const T* x, int64_t ld, const T* g, int64_t ldg, const W* w, int rows, int d, float eps, T* dx,
+                             float* part) {
   __shared__ float2 s_sum[2][kWarps];  // one is read while the next row's is written
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float acc[NV][VEC] = {};
@@ -418,12 +420,12 @@ extern "C" int cb_rms_norm(const void* x, int32_t dtype, int64_t ld, const void*
     }
     if (!in_a_warp(rows, d, dtype_size(dtype), pieces, false))
       return cta_pieces<T>(d, pieces, [&](auto vec, auto nv) {
-        return launch_after(rms_norm_cta_kernel<T, W, decltype(vec)::value, decltype(nv)::value>, dim3(rows), kThreads, 0, st,
-                            in, ld, weight, d, eps, static_cast<T*>(y));
+        return launch_after(rms_norm_cta_kernel<T, W, decltype(vec)::value, decltype(nv)::value>, dim3(rows), kThreads, 0,
+                            st, in, ld, weight, d, eps, static_cast<T*>(y));
       });
     return warp_pieces<T>(d, pieces, [&](auto vec, auto nv) {
-      return launch_after(rms_norm_warp_kernel<T, W, decltype(vec)::value, decltype(nv)::value>, dim3(ceil_div(rows, kWarps)), kThreads, 0, st, in,
-                          ld, weight, rows, d, eps, static_cast<T*>(y));
+      return launch_after(rms_norm_warp_kernel<T, W, decltype(vec)::value, decltype(nv)::value>,
+                          dim3(ceil_div(rows, kWarps)), kThreads, 0, st, in, ld, weight, rows, d, eps, static_cast<T*>(y));
     });
   });
 }
@@ -459,16 +461,16 @@ extern "C" int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const 
       part = rstd;
       parts = warp_ctas(rows);
       const int rc = warp_pieces<T>(d, pieces, [&](auto vec, auto nv) {
-        return launch_after(rms_norm_grad_warp_kernel<T, W, decltype(vec)::value, decltype(nv)::value>, dim3(parts), kThreads,
-                            0, st, in, ld, up, ldg, weight, rows, d, eps, static_cast<T*>(dx), part);
+        return launch_after(rms_norm_grad_warp_kernel<T, W, decltype(vec)::value, decltype(nv)::value>, dim3(parts),
+                            kThreads, 0, st, in, ld, up, ldg, weight, rows, d, eps, static_cast<T*>(dx), part);
       });
       if (rc) return rc;
     } else if (in_a_cta(d, pieces)) {
       part = rstd;
       const int rc = cta_pieces<T>(d, pieces, [&](auto vec, auto nv) {
         parts = row_ctas(rows, vec * nv);
-        return launch_after(rms_norm_grad_cta_kernel<T, W, decltype(vec)::value, decltype(nv)::value>, dim3(parts), kThreads, 0,
-                            st, in, ld, up, ldg, weight, rows, d, eps, static_cast<T*>(dx), part);
+        return launch_after(rms_norm_grad_cta_kernel<T, W, decltype(vec)::value, decltype(nv)::value>, dim3(parts),
+                            kThreads, 0, st, in, ld, up, ldg, weight, rows, d, eps, static_cast<T*>(dx), part);
       });
       if (rc) return rc;
     } else {
@@ -476,8 +478,8 @@ extern "C" int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const 
       if (int rc = launch_after(rms_norm_dx_kernel<T, W>, dim3(rows), kThreads, 0, st, in, ld, up, ldg, weight, d, eps,
                                 static_cast<T*>(dx), rstd))
         return rc;
-      if (int rc = launch_after(rms_norm_dw_part_kernel<T>, dim3(parts, ceil_div(d, kThreads)), kThreads, 0, st, in, ld, up,
-                                ldg, rstd, rows, d, part))
+      if (int rc = launch_after(rms_norm_dw_part_kernel<T>, dim3(parts, ceil_div(d, kThreads)), kThreads, 0, st, in, ld,
+                                up, ldg, rstd, rows, d, part))
         return rc;
     }
     return launch_after(rms_norm_dw_kernel<W>, dim3(ceil_div(d, 32)), 1024, 0, st, part, parts, d, static_cast<W*>(dw));
