@@ -33,7 +33,7 @@ CB_KV8_E4M3, CB_KV8_INT8 = 0, 1
 CB_F32, CB_BF16, CB_F16 = 0, 1, 2
 CB_LOGPROB_MAX_TOP, CB_LOGPROB_MAX_VOCAB = 32, 1 << 20
 CB_ENDS_MAX_ROWS, CB_ENDS_MAX_VOCAB, CB_ENDS_MAX_DIM = 1 << 24, 1 << 20, 65536
-CB_REDUCE_NONE, CB_REDUCE_MEAN, CB_REDUCE_SUM = 0, 1, 2
+CB_REDUCE_NONE, CB_REDUCE_MEAN, CB_REDUCE_SUM, CB_REDUCE_REST = 0, 1, 2, 4
 CB_GEMM_PRE_NONE, CB_GEMM_PRE_RMSNORM = 0, 1
 CB_GEMM_EPI_STORE, CB_GEMM_EPI_ADD, CB_GEMM_EPI_SWIGLU = 0, 1, 2
 

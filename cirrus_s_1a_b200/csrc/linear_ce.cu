@@ -858,7 +858,8 @@ constexpr int kRowThreads = 256;
 template <int LANES>
 __global__ void __launch_bounds__(kRowThreads) join_kernel(Problem p, int few, int n_tiles, int m_tiles, int pairs,
                                                            const float2* part, const float* xt, float* rows, float* lse,
-                                                           int reduction, float* loss, int32_t* count, double2* sums, uint32_t* counter,
+                                                           int reduction, float* loss, int32_t* count, float* rest,
+                                                           double2* sums, uint32_t* counter,
                                                            int32_t* status) {
   __shared__ double s_sum[kRowThreads / 32], s_count[kRowThreads / 32];
   __shared__ int s_last;
@@ -891,12 +892,16 @@ __global__ void __launch_bounds__(kRowThreads) join_kernel(Problem p, int few, i
     m = t;
   }
   if (n < p.N && threadIdx.x % LANES == 0) {
-    lse[n] = m + logf(l);
+    // (in 64 bits: log l is off by as much as the sum is rounded, and a loss near 0 is a difference)
+    const double log_l = log((double)l), whole = (double)m + log_l;
+    const float rounded = (float)whole;
+    lse[n] = rounded;
+    if (rest) rest[n] = fabsf(rounded) < INFINITY ? (float)(whole - (double)rounded) : 0.0f;
     const int64_t t = p.targets[n];
     float row = 0.0f;
     if (t >= p.V) set_status(status, CB_ERR_TOKEN);
     if (t >= 0 && t < p.V) {
-      row = (m - xt[n]) + logf(l);
+      row = (float)(((double)m - (double)xt[n]) + log_l);
       sum = row;
       has = 1.0;
     }
@@ -954,6 +959,7 @@ struct Upstream {
   int64_t loss_step, lse_step;
   const int32_t* count;  // mean: rows with a target
   int reduction;
+  const float* rest;     // what rounding took off lse (may be null)
 };
 
 // rows[n] = (a, b, lse, -) as they come from above, and *top = the largest |a| or |b|: one
@@ -976,7 +982,9 @@ __global__ void __launch_bounds__(kRowThreads) factors_kernel(Problem p, Upstrea
     if (u.loss && target_of(p, n) >= 0) b = u.reduction == CB_REDUCE_NONE ? u.loss[n * u.loss_step] : one;
     const float a = b + (u.lse ? u.lse[n * u.lse_step] : 0.0f);
     // (a row without a gradient is read as zeros, and its G is 0 whatever its own lse is)
-    rows[n] = make_float4(a, b, a == 0.0f && b == 0.0f ? 0.0f : lse[n], 0.0f);
+    // p = exp(x - lse - rest)
+    const float of_p = u.rest && a != 0.0f ? a * expf(-u.rest[n]) : a;
+    rows[n] = make_float4(of_p, b, a == 0.0f && b == 0.0f ? 0.0f : lse[n], 0.0f);
     size = fmaxf(fabsf(a), fabsf(b));
     if (!(size < INFINITY)) size = 0.0f;
   }
@@ -1212,7 +1220,8 @@ bool bad(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_d
   if (!h || !w || !targets || N <= 0 || V <= 0 || d <= 0 || !is_dtype(h_dtype) || !is_dtype(w_dtype)) return true;
   if (h_dtype != w_dtype && !(h_dtype == CB_F32 && w_dtype == CB_BF16)) return true;
   if (ldh < 0 || (V > 1 && ldw < d)) return true;
-  if (reduction != CB_REDUCE_NONE && reduction != CB_REDUCE_MEAN && reduction != CB_REDUCE_SUM) return true;
+  const int32_t by = reduction & ~CB_REDUCE_REST;
+  if (by != CB_REDUCE_NONE && by != CB_REDUCE_MEAN && by != CB_REDUCE_SUM) return true;
   return !aligned_to(h, dtype_size(h_dtype)) || !aligned_to(w, dtype_size(w_dtype)) ||
          !aligned_to(targets, targets_64 ? 8 : 4);
 }
@@ -1572,6 +1581,8 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   if (bad(h, h_dtype, ldh, w, w_dtype, ldw, N, V, d, targets, targets_64, reduction) || !loss || !lse || !scratch ||
       !aligned_to(scratch, 256) || (reduction != CB_REDUCE_NONE && !count))
     return CB_ERR_ARG;
+  float* rest = reduction & CB_REDUCE_REST ? reinterpret_cast<float*>(count + 1) : nullptr;
+  reduction &= ~CB_REDUCE_REST;
   if (too_large(N, V, d)) return CB_ERR_SHAPE;
   cudaStream_t st = (cudaStream_t)stream;
   const Shape s(h_dtype, w_dtype, N, V, d);
@@ -1619,7 +1630,7 @@ extern "C" int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const v
   const int lanes = f.lanes();
   return launch_after(lanes == 32 ? join_kernel<32> : join_kernel<4>, dim3(f.join_ctas(N)), kRowThreads, 0, st,
                       Problem{N, V, d, p.targets}, f.few, f.n_tiles, f.m_tiles, f.pairs, f.part, f.xt, loss, lse, reduction,
-                      loss, count, f.sums, f.counter, status);
+                      loss, count, rest, f.sums, f.counter, status);
 }
 
 extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype,
@@ -1628,9 +1639,11 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
                                  int64_t g_loss_step, const float* g_lse, int64_t g_lse_step, void* dh, void* dw,
                                  void* scratch, size_t scratch_bytes, int32_t* status, void* stream) {
   if (bad(h, h_dtype, ldh, w, w_dtype, ldw, N, V, d, targets, targets_64, reduction) || !lse || !scratch ||
-      !aligned_to(scratch, 256) || (reduction == CB_REDUCE_MEAN && !count) || g_loss_step < 0 || g_lse_step < 0 ||
+      !aligned_to(scratch, 256) || (reduction != CB_REDUCE_NONE && reduction != CB_REDUCE_SUM && !count) || g_loss_step < 0 || g_lse_step < 0 ||
       (!dh && !dw) || !aligned_to(dh, dtype_size(h_dtype)) || !aligned_to(dw, dtype_size(w_dtype)))
     return CB_ERR_ARG;
+  const float* rest = reduction & CB_REDUCE_REST ? reinterpret_cast<const float*>(count + 1) : nullptr;
+  reduction &= ~CB_REDUCE_REST;
   if (too_large(N, V, d)) return CB_ERR_SHAPE;
   cudaStream_t st = (cudaStream_t)stream;
   const Shape s(h_dtype, w_dtype, N, V, d);
@@ -1638,7 +1651,7 @@ extern "C" int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, co
   const Backward f(a, s, s.reads_w(w, w_dtype, ldw), dh != nullptr, dw != nullptr, tma_rows(dw, w_dtype, d));
   if (scratch_bytes < a.used) return CB_ERR_WORKSPACE;
   const Problem pb{N, V, d, Ids{targets, targets_64}};
-  const Upstream u{g_loss, g_lse, g_loss_step, g_lse_step, count, reduction};
+  const Upstream u{g_loss, g_lse, g_loss_step, g_lse_step, count, reduction, rest};
   if ((reduction == CB_REDUCE_NONE || g_lse) && cudaMemsetAsync(f.top, 0, sizeof(float), st) != cudaSuccess)
     return CB_ERR_CUDA;
   if (int rc = launch_after(factors_kernel, dim3(ceil_div(N, kRowThreads)), kRowThreads, 0, st, pb, u, lse, f.rows, f.top,

@@ -40,7 +40,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     Runs on the current stream."""
     if _rows.wants_grad(hidden, weight):
         return CrossEntropy(*_LinearCE.apply(hidden, weight, targets, reduction, status))
-    return CrossEntropy(*_forward(hidden, weight, targets, reduction, status)[:2])
+    return CrossEntropy(*_forward(hidden, weight, targets, reduction, status, False)[:2])
 
 
 def check_call(targets, reduction, status, device) -> tuple:
@@ -67,15 +67,18 @@ def _arguments(hidden, weight, targets, reduction, status) -> tuple:
     return (hidden.data_ptr(), h_code, ldh, weight.data_ptr(), w_code, ldw, N, V, D, targets.data_ptr(), wide, code), flag
 
 
-def _forward(hidden, weight, targets, reduction, status) -> tuple:
-    """(loss, lse, count)"""
+def _forward(hidden, weight, targets, reduction, status, rest) -> tuple:
+    """(loss, lse, the number of targets and, with ``rest``, what rounding took off each lse)"""
     args, flag = _arguments(hidden, weight, targets, reduction, status)
     dev, N = hidden.device, args[6]
     lse = torch.empty(N, dtype=torch.float32, device=dev)
     if N == 0:
         return torch.zeros(() if reduction != "none" else 0, device=dev), lse, None
     loss = torch.empty(N if reduction == "none" else (), dtype=torch.float32, device=dev)
-    count = None if reduction == "none" else torch.empty(1, dtype=torch.int32, device=dev)
+    if rest:
+        args = (*args[:-1], args[-1] | _lib.CB_REDUCE_REST)
+    n = 1 + N if rest else int(reduction != "none")
+    count = torch.empty(n, dtype=torch.int32, device=dev) if n else None
     scratch = _scratch(dev, args, None, 0)
     _rows.call(dev, "cb_linear_ce", *args, loss.data_ptr(), lse.data_ptr(), _lib.ptr(count), scratch.data_ptr(),
                scratch.numel(), flag)
@@ -93,7 +96,7 @@ def _scratch(dev, args, dw, gradients) -> torch.Tensor:
 class _LinearCE(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, reduction, status):
-        loss, lse, count = _forward(hidden, weight, targets, reduction, status)
+        loss, lse, count = _forward(hidden, weight, targets, reduction, status, True)
         ctx.save_for_backward(hidden, weight, targets, lse, count)
         ctx.reduction, ctx.status, ctx.like = reduction, status, (hidden.device, len(lse), weight.shape[0])
         ctx.set_materialize_grads(False)
@@ -113,14 +116,15 @@ class _LinearCE(torch.autograd.Function):
             raise ValueError(f"the saved tensors must be of {ctx.like[1]} rows and {ctx.like[2]} of the vocabulary on "
                              f"{ctx.like[0]}, not {N} and {V} on {dev}")
         _rows.given(lse, "the saved lse", (N,), torch.float32, dev)
-        _rows.given(count, "the saved number of targets", (1,), torch.int32, dev)
-        lse = lse.contiguous()
+        _rows.given(count, "the saved number of targets", (1 + N,), torch.int32, dev)
         dh = torch.empty(N, D, dtype=hidden.dtype, device=dev) if want_h else None
         if N == 0:
             return dh, torch.zeros(V, D, dtype=weight.dtype, device=dev) if want_w else None, None, None, None
         dw = torch.empty(V, D, dtype=weight.dtype, device=dev) if want_w else None
         scratch = _scratch(dev, args, dw, want_h + 2 * want_w)
-        _rows.call(dev, "cb_linear_ce_grad", *args, lse.data_ptr(), _lib.ptr(count), _lib.ptr(g_loss), _step(g_loss),
+        lse, count = lse.contiguous(), count.contiguous()
+        args = (*args[:-1], args[-1] | _lib.CB_REDUCE_REST)
+        _rows.call(dev, "cb_linear_ce_grad", *args, lse.data_ptr(), count.data_ptr(), _lib.ptr(g_loss), _step(g_loss),
                    _lib.ptr(g_lse), _step(g_lse), _lib.ptr(dh), _lib.ptr(dw), scratch.data_ptr(), scratch.numel(),
                    flag)
         return dh, dw, None, None, None

@@ -516,7 +516,7 @@ int cb_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int32_t row
 #define CB_ENDS_MAX_ROWS (1 << 24)
 #define CB_ENDS_MAX_VOCAB (1 << 20)
 #define CB_ENDS_MAX_DIM 65536
-enum { CB_REDUCE_NONE = 0, CB_REDUCE_MEAN = 1, CB_REDUCE_SUM = 2 };
+enum { CB_REDUCE_NONE = 0, CB_REDUCE_MEAN = 1, CB_REDUCE_SUM = 2, CB_REDUCE_REST = 4 };
 
 /* out [n][d] = scale * table[ids[i]], zeros where there is no token; scale is finite.  Replaces nn.Embedding
  * (cirrus/model/model.py:124) for a dense table; cb_embed reads the NVFP4 one. */
@@ -546,7 +546,8 @@ int cb_rms_norm_grad(const void* x, int32_t dtype, int64_t ld, const void* g, in
  * the logits x = h w^T: lse [N] = log sum exp x (natural log), and per row lse - x[target],
  * 0 where there is no target.  loss: that for each row [N] (CB_REDUCE_NONE), or its mean
  * over the rows with a target (0 when none has one) or its sum, [1], with their number in
- * count [1].  h and w have one type, or h is CB_F32 and w CB_BF16.  16-bit products
+ * count [1].  CB_REDUCE_REST added to the reduction, in the gradient's call too: count [1 + N] holds
+ * behind it, as float32, what rounding took off each lse.  h and w have one type, or h is CB_F32 and w CB_BF16.  16-bit products
  * are added up in float32 (by the tensor cores, which cut off instead of rounding, for up to 768 of
  * them), float32 ones carried in about 22 bits.
  * Scratch, 256-byte aligned: cb_linear_ce_scratch_bytes of the same arguments, for the
@@ -569,7 +570,8 @@ int cb_linear_ce(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int
  * below 2^-38 of the largest |g_loss + g_lse| or |g_loss| may be taken as 0 (in float16
  * too, of the row's own); in dw also what lies below 2^-39 of the largest value of float32 h.
  * x here has the bits that it had in the forward pass, so that G is 0 where the target has
- * all the probability; lse is rounded to float32, G's relative error is not below that. */
+ * all the probability; p's relative error is not below what rounding took off lse, except with
+ * CB_REDUCE_REST. */
 int cb_linear_ce_grad(const void* h, int32_t h_dtype, int64_t ldh, const void* w, int32_t w_dtype, int64_t ldw,
                       int32_t N, int32_t V, int32_t d, const void* targets, int32_t targets_64, int32_t reduction,
                       const float* lse, const int32_t* count, const float* g_loss, int64_t g_loss_step,

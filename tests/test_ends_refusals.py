@@ -46,3 +46,17 @@ def test_embedding_refuses_a_scale_that_is_not_finite(built_lib):  # noqa: F811
 
     with pytest.raises(ValueError, match="scale"):
         embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8), math.nan)
+
+
+def test_what_rounding_takes_off_lse_has_its_room(built_lib):  # noqa: F811
+    """CB_REDUCE_REST (4) writes behind the count: without one it is refused, in any reduction."""
+    L = built_lib
+    before = L.cb_launch_count()
+    for reduction in (0, 1, 2):
+        assert L.cb_linear_ce(256, 1, 8, 256, 1, 8, 3, 4, 8, 256, 1, reduction | 4, 256, 256, None, 256, 1 << 40, None,
+                              None) == 1
+        assert L.cb_linear_ce_grad(256, 1, 8, 256, 1, 8, 3, 4, 8, 256, 1, reduction | 4, 256, None, 256, 1, None, 0, 256,
+                                   256, 256, 1 << 40, None, None) == 1
+    for reduction in (3, 7, 8, -1):
+        assert L.cb_linear_ce(256, 1, 8, 256, 1, 8, 3, 4, 8, 256, 1, reduction, 256, 256, 256, 256, 1 << 40, None, None) == 1
+    assert L.cb_launch_count() == before

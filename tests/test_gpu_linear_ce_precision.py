@@ -82,3 +82,24 @@ def test_what_tensor_memory_cuts_off_a_logit(pair):
     lse = linear_cross_entropy(h.to(DEV), w.to(DEV), torch.zeros(4096, dtype=torch.int64, device=DEV)).lse
     off = float(((lse.cpu().double() - x) / x).mean())
     assert abs(off) <= (100 if pair == "bf16" else 80) * 2.0 ** -24, off * 2.0 ** 24
+
+
+@pytest.mark.parametrize("weight", ["f32", "bf16"])
+@pytest.mark.parametrize("N", [1, 64, 300])
+def test_probabilities_add_up_to_one(weight, N):
+    """Logits near 1000 that are exact (multiples of 2^-7), and a column of w that holds 250
+    everywhere: dh of lse is 250 times the sum of the probabilities.  lse alone, in float32, is
+    off by up to 2^-15 there.  Beside what rounding took off it: 2^-22 for the parts of G, 2^-20 for
+    the exponentials (2^-22 each, and 2^-24 of exponents below 14), (V / 8 + 8) 2^-23 for the sum."""
+    from cirrus_s_1a_b200.loss import linear_cross_entropy
+
+    V, d = 300, 8
+    g = torch.Generator().manual_seed(N)
+    h, w = torch.randint(-8, 9, (N, d), generator=g) / 8, torch.randint(-32, 33, (V, d), generator=g) / 16
+    h[:, 7], w[:, 7] = 4.0, 250.0
+    hd = h.to(DEV).requires_grad_()
+    r = linear_cross_entropy(hd, w.to(DEV, torch.float32 if weight == "f32" else torch.bfloat16),
+                             torch.full((N,), -1, device=DEV))
+    dh, = torch.autograd.grad(r.lse, hd, torch.ones(N, device=DEV))
+    off = float((dh[:, 7].double() / 250 - 1).abs().max())
+    assert off <= 2.0 ** -22 + 2.0 ** -20 + (V / 8 + 8) * 2.0 ** -23, off
