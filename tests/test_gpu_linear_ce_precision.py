@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import ends
-from test_gpu_linear_ce import call, half_step, inputs, smallest
+from test_gpu_linear_ce import call, compare, half_step, inputs, smallest
 
 pytestmark = pytest.mark.gpu
 
@@ -103,3 +103,33 @@ def test_probabilities_add_up_to_one(weight, N):
     dh, = torch.autograd.grad(r.lse, hd, torch.ones(N, device=DEV))
     off = float((dh[:, 7].double() / 250 - 1).abs().max())
     assert off <= 2.0 ** -22 + 2.0 ** -20 + (V / 8 + 8) * 2.0 ** -23, off
+
+
+@pytest.mark.parametrize("pair", [("bf16", "bf16"), ("f16", "f16"), ("f32", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_entry_points_without_the_remainder(pair, reduction):
+    """A caller in C who keeps lse and the count alone."""
+    from cirrus_s_1a_b200 import _lib, _rows
+    from cirrus_s_1a_b200.kv8 import DTYPES
+    from cirrus_s_1a_b200.loss import REDUCTIONS
+
+    N, V, d = 150, 700, 72
+    h, w, t = inputs(N, V, d, pair, seed=41)
+    hd, wd, td = h.to(DEV), w.to(DEV), t.to(DEV)
+    args = (hd.data_ptr(), DTYPES[h.dtype], d, wd.data_ptr(), DTYPES[w.dtype], d, N, V, d)
+    more = (td.data_ptr(), 1, REDUCTIONS[reduction])
+    up = torch.linspace(0.1, 1, N) if reduction == "none" else torch.full((), 1.0)
+    loss, lse = torch.empty(up.shape, device=DEV), torch.empty(N, device=DEV)
+    count = torch.full((2,), -7, dtype=torch.int32, device=DEV)
+    dh, dw, g = torch.empty_like(hd), torch.empty_like(wd), up.to(DEV)
+    for which, (at, gradients) in enumerate(((None, 0), (dw.data_ptr(), 3))):
+        n = _lib.lib().cb_linear_ce_scratch_bytes(*args, at, gradients)
+        scratch = torch.empty(n, dtype=torch.uint8, device=DEV)
+        if not which:
+            _rows.call(hd.device, "cb_linear_ce", *args, *more, loss.data_ptr(), lse.data_ptr(), count.data_ptr(),
+                       scratch.data_ptr(), n, None)
+        else:
+            _rows.call(hd.device, "cb_linear_ce_grad", *args, *more, lse.data_ptr(), count.data_ptr(), g.data_ptr(),
+                       int(reduction == "none"), None, 0, dh.data_ptr(), dw.data_ptr(), scratch.data_ptr(), n, None)
+    assert int(count[1]) == -7  # nothing behind the number
+    compare({"loss": loss, "lse": lse, "dh": dh, "dw": dw}, ends.cross_entropy(h, w, t, reduction, up), h, w, reduction)
