@@ -20,14 +20,15 @@
 // vocabulary goes to memory in the operands' type, both products of the piece follow in one
 // launch; dh adds the pieces up in float32.
 // float32 operands are two f16 parts each (11 + 11 bits, of the value times a power of two),
-// three products of parts (what is left out is below 2^-24 of a product), where the values
+// three products of parts (what is left out is up to 2^-22 of a product), where the values
 // lie in the range that this is right for, which the kernel that makes the parts finds out;
 // else three bf16 parts (8 + 8 + 8 bits, and float32's range), six products.  Against bf16,
 // which is one part: two products and three.
-// Measured, 16384 x 32000 x 768 in bf16: loss 545 us = 1.48 PFLOP/s (tensor pipe 88 %),
-// with the gradient 2665 us = 1.21 PFLOP/s, at the power limit (G of a quarter of the
-// vocabulary 140 us, both its products 250 us, tensor pipe 77 and 90 %).  5 rows 17 us,
-// 128 rows of float32 against bf16 25 us, of which one read of W is 7.5.
+// Measured, 16384 x 32000 x 768 in bf16, back to back, which the power limit holds down: loss
+// 590 us = 1.36 PFLOP/s (530 to 640 as it sets in), with the gradient 2780 us = 1.16 PFLOP/s.
+// Single launches under ncu, tensor pipe: the logits 87 %, G's pass 74 % (its epilogue; it holds
+// 128 logits a thread and spills 48 bytes of 168 registers), the products 90 %.  5 rows 15.5 us,
+// 128 rows of float32 against bf16 23 us, of which one read of W is 7.5.
 // Every wait is bounded (%globaltimer).  One that gives up sets CB_ERR_TIMEOUT, and what its
 // CTA had still to give is NaN, so that a caller without a status word sees it too.
 #include <cuda.h>

@@ -640,7 +640,8 @@ class CirrusB200:
         """Cross entropy of ``targets`` [B, T], the token that follows each of ``input_ids``
         (negative: none), behind what ``cache`` holds, from the hidden states alone: the
         logits are not kept (``linear_cross_entropy`` over the final norm's output and
-        ``dense_head``).  ``loss`` is [B, T] with reduction "none", ``lse`` always.  Without
+        ``dense_head``).  The forward leaves the LM head out where it takes one launch per op;
+        the persistent launch of up to 8 rows multiplies it all the same.  ``loss`` is [B, T] with reduction "none", ``lse`` always.  Without
         ``status`` a target outside the vocabulary and a wait that gave up are noted where the
         forward's errors are (``read_status`` of the cache and T)."""
         if targets.shape != input_ids.shape:
